@@ -610,6 +610,48 @@ PVB2_API int pvb2_sgd_multi(int n, float* const* params, const float* const* gra
                    const int64_t* numels, double lr, double momentum, double dampening,
                    double weight_decay, int nesterov, int first_step, double grad_scale,
                    pvb2_stream stream);
+/* Adam / AdamW over many tensors: torch's _fused_adam_ / _fused_adamw_ and a
+ * variant with 8-bit moments (the reference has neither: its optimizers ran
+ * one launch per tensor and operation, pointwise_ops.cpp:115-234,414-434).
+ * For every tensor, with t = *step (after adding 1 to it if increment_step):
+ *   g  = maximize ? -grad : grad      (grad / *grad_scale first, written back)
+ *   decoupled: p *= 1 - lr * weight_decay;  else: g += weight_decay * p
+ *   m  = beta1 * m + (1 - beta1) * g;  v = beta2 * v + (1 - beta2) * g^2
+ *   p -= lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * (amsgrad: the running maximum of v in v's place).  Arithmetic in fp32, one
+ * rounding to each stored type.  lr_device, when given, is read in lr's place;
+ * where *found_inf is not 0 nothing is changed.
+ * state_dtype: PVB2_F32, the parameters' type, or PVB2_U8: moments as 8-bit
+ * codes with one fp32 scale for every 256 consecutive elements, m = s c in
+ * exp_avg / exp_avg_scale and sqrt(v) = s c in exp_avg_sq / exp_avg_sq_scale,
+ * c = code bits [sign][exponent 4, bias 15][mantissa 3] for m and
+ * [exponent 4, bias 15][mantissa 4] for sqrt(v); zeroed codes and scales are
+ * zero moments.  8-bit moments take decoupled decay only. */
+typedef struct pvb2_adamw_desc {
+  int32_t param_dtype, state_dtype;
+  int32_t decoupled, maximize, amsgrad, increment_step;
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_device;   /* device memory, or NULL */
+  const float* grad_scale;  /* device memory, or NULL */
+  const float* found_inf;   /* device memory, or NULL */
+} pvb2_adamw_desc;
+typedef struct pvb2_adamw_tensor {
+  void* param;
+  void* grad;              /* of the parameter's type */
+  void* exp_avg;
+  void* exp_avg_sq;
+  void* max_exp_avg_sq;    /* amsgrad only */
+  float* exp_avg_scale;    /* 8-bit moments only: ceil(numel / 256) scales */
+  float* exp_avg_sq_scale;
+  float* step;             /* device memory, one float */
+  int64_t numel;
+} pvb2_adamw_tensor;
+PVB2_API size_t pvb2_adamw_workspace_size(int n);
+PVB2_API int pvb2_adamw_multi(const pvb2_adamw_desc* d, int n, const pvb2_adamw_tensor* tensors, void* workspace,
+                              size_t workspace_bytes, pvb2_stream stream);
+/* the moments that 8-bit codes stand for: m as fp32 into `param`, v into
+ * `grad` (both fp32, numel elements) of every tensor */
+PVB2_API int pvb2_adamw8_values(int n, const pvb2_adamw_tensor* tensors, pvb2_stream stream);
 /* _foreach_* helpers: out[i] = a[i] (op) (b ? b[i] : scalar) with alpha,
  * for op in {ADD, SUB, MUL, DIV}; out may alias a.  fp32 only. */
 PVB2_API int pvb2_foreach_binary(int op, int n, float* const* out, const float* const* a, const float* const* b,
@@ -618,6 +660,30 @@ PVB2_API int pvb2_foreach_binary(int op, int n, float* const* out, const float* 
  * data-parallel gradient buckets.  direction 0: flat <- tensors, 1: tensors <- flat */
 PVB2_API int pvb2_flatten_multi(int n, float* const* tensors, const int64_t* numels, float* flat, int direction,
                        double scale, pvb2_stream stream);
+
+/* ------------------------------------------------------------------ */
+/* learned relative position bias of attention scores (no counterpart   */
+/* in the reference)                                                    */
+/*   out[h][i][j] = table[bucket(j - i - q_offset)][h]                  */
+/* bucket(r): with n = bidirectional ? num_buckets / 2 : num_buckets,   */
+/* d = bidirectional ? |r| : max(-r, 0), e = n / 2:                     */
+/*   d < e: d; else min(n - 1, e + floor(log(d / e) /                   */
+/*                  log(max_distance / e) * (n - e)));                  */
+/*   plus n where bidirectional and r > 0.                              */
+/* table [num_buckets][H] and out [H][Lq][Lk] contiguous, of one type   */
+/* (fp32, fp16, bf16).  The backward pass sums grad [B][H][Lq][Lk] (any */
+/* strides, 0 among them) over b and every (i, j) of a bucket, in a     */
+/* fixed order, into dtable.                                            */
+/* ------------------------------------------------------------------ */
+typedef struct pvb2_relative_bias_desc {
+  int32_t H, num_buckets, bidirectional, dtype;
+  int64_t Lq, Lk, max_distance, q_offset;
+} pvb2_relative_bias_desc;
+PVB2_API int pvb2_relative_bias_fwd(const pvb2_relative_bias_desc* d, const void* table, void* out,
+                                    pvb2_stream stream);
+PVB2_API size_t pvb2_relative_bias_bwd_workspace_size(const pvb2_relative_bias_desc* d, int64_t B);
+PVB2_API int pvb2_relative_bias_bwd(const pvb2_relative_bias_desc* d, const pvb2_tensor* grad, void* dtable,
+                                    void* workspace, size_t workspace_bytes, pvb2_stream stream);
 
 /* ------------------------------------------------------------------ */
 /* random (src/random_ops.cpp): Philox-4x32-10 counter-based generator  */

@@ -180,9 +180,12 @@ class _OCL:
         return _C.impl_launch_count()
 
 
+from . import functional, optim  # noqa: E402
 from .graphs import Graph  # noqa: E402
 
 _OCL.Graph = Graph
+_OCL.functional = functional
+_OCL.optim = optim
 
 
 def synchronize(dev=None):

@@ -959,8 +959,9 @@ static void graph_destroy(uintptr_t handle) {
 
 }  // namespace ocl
 
-// defined in ops_dist.cpp
+// defined in ops_dist.cpp and ops_train.cpp
 void register_dist_bindings(pybind11::module& m);
+void register_train_bindings(pybind11::module& m);
 
 PYBIND11_MODULE(_C, m) {
   using namespace ocl;
@@ -998,4 +999,5 @@ PYBIND11_MODULE(_C, m) {
   m.def("impl_graph_kernels", &graph_kernels, "kernels launched by one replay");
   m.def("impl_graph_destroy", &graph_destroy, "release a graph and its memory pool");
   register_dist_bindings(m);
+  register_train_bindings(m);
 }

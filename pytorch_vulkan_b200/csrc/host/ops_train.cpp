@@ -1,0 +1,347 @@
+// What a transformer's training step needs beside its layers: the AdamW step
+// over many tensors (torch's _fused_adam_ / _fused_adamw_, and the 8-bit
+// state of pytorch_vulkan_b200.optim.AdamW) and the learned relative position
+// bias, as ops of the `ocl` namespace with their gradients.  The reference
+// had neither: its optimizers fell into one mul_/add_ launch per tensor and
+// operation (src/pointwise_ops.cpp:115-234,407-434).
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/extension.h>
+
+#include "ocl.h"
+
+namespace ocl {
+
+// ------------------------------------------------------------------ AdamW
+static bool adam_type(c10::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+
+// memory order of `t` is that of `p`: the flat walk pairs their elements
+static bool same_layout(const at::Tensor& t, const at::Tensor& p) {
+  return t.sizes().equals(p.sizes()) && t.is_non_overlapping_and_dense() && (t.strides().equals(p.strides()) ||
+         (t.is_contiguous() && p.is_contiguous()));
+}
+
+static at::Tensor grad_like(const at::Tensor& g, const at::Tensor& p) {
+  if (same_layout(g, p)) return g;
+  at::Tensor c = empty_strided_dev(p.sizes(), p.strides(), p.scalar_type(), p.device().index());
+  copy_into(c, g, false);
+  return c;
+}
+
+static void check_param(const at::Tensor& p, const at::Tensor& g, int dev, c10::ScalarType type, size_t i) {
+  TORCH_CHECK(is_ocl(p) && p.device().index() == dev && is_ocl(g) && g.device().index() == dev,
+              "ocl AdamW: parameter ", i, " and its gradient have to be on ocl:", dev);
+  TORCH_CHECK(adam_type(p.scalar_type()) && p.scalar_type() == type && g.scalar_type() == type,
+              "ocl AdamW: parameters and gradients of one type (fp32, fp16 or bf16) expected, got ", p.scalar_type(),
+              " and ", g.scalar_type(), " at ", i);
+  TORCH_CHECK(g.sizes().equals(p.sizes()), "ocl AdamW: gradient ", i, " has another shape than its parameter");
+  TORCH_CHECK(p.is_non_overlapping_and_dense(), "ocl AdamW: parameter ", i, " has gaps or overlaps in memory");
+}
+
+static float* step_ptr(const at::Tensor& t, int dev, size_t i) {
+  TORCH_CHECK(is_ocl(t) && t.device().index() == dev && t.scalar_type() == at::kFloat && t.numel() == 1,
+              "ocl AdamW: step ", i, " has to be one fp32 value on ocl:", dev);
+  return t.data_ptr<float>();
+}
+
+static const float* scalar_ptr(const std::optional<at::Tensor>& t, int dev, const char* what) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(is_ocl(*t) && t->device().index() == dev && t->scalar_type() == at::kFloat && t->numel() == 1,
+              "ocl _fused_adam: ", what, " has to be one fp32 value on ocl:", dev);
+  return t->data_ptr<float>();
+}
+
+static void fused_adam(bool decoupled, at::TensorList self, at::TensorList grads, at::TensorList exp_avgs,
+                       at::TensorList exp_avg_sqs, at::TensorList max_exp_avg_sqs, at::TensorList state_steps, double lr,
+                       const float* lr_device, double beta1, double beta2, double weight_decay, double eps,
+                       bool amsgrad, bool maximize, const std::optional<at::Tensor>& grad_scale,
+                       const std::optional<at::Tensor>& found_inf) {
+  if (self.empty()) return;
+  const size_t n = self.size();
+  TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && state_steps.size() == n &&
+                  (!amsgrad || max_exp_avg_sqs.size() == n),
+              "ocl _fused_adam: lists of one length expected");
+  const int dev = self[0].device().index();
+  const c10::ScalarType type = self[0].scalar_type(), state = exp_avgs[0].scalar_type();
+  DeviceScope scope(dev);
+  OCL_OP(decoupled ? "_fused_adamw_" : "_fused_adam_", dev);
+  std::vector<pvb2_adamw_tensor> ts(n);
+  for (size_t i = 0; i < n; ++i) {
+    check_param(self[i], grads[i], dev, type, i);
+    // the gradient is written back where it is unscaled, so no copy will do
+    TORCH_CHECK(same_layout(grads[i], self[i]), "ocl _fused_adam: gradient ", i, " is laid out unlike its parameter");
+    pvb2_adamw_tensor& t = ts[i];
+    memset(&t, 0, sizeof(t));
+    auto held = [&](const at::Tensor& x) {
+      TORCH_CHECK(is_ocl(x) && x.device().index() == dev && x.scalar_type() == state && same_layout(x, self[i]),
+                  "ocl _fused_adam: moments ", i, " have to be of one type and laid out as their parameter");
+      return x.data_ptr();
+    };
+    t.param = self[i].data_ptr();
+    t.grad = grads[i].data_ptr();
+    t.exp_avg = held(exp_avgs[i]);
+    t.exp_avg_sq = held(exp_avg_sqs[i]);
+    if (amsgrad) t.max_exp_avg_sq = held(max_exp_avg_sqs[i]);
+    t.step = step_ptr(state_steps[i], dev, i);
+    t.numel = self[i].numel();
+  }
+  TORCH_CHECK(state == at::kFloat || state == type, "ocl _fused_adam: moments of the parameters' type or fp32 expected");
+  pvb2_adamw_desc d;
+  memset(&d, 0, sizeof(d));
+  d.param_dtype = dtype_code(type);
+  d.state_dtype = dtype_code(state);
+  d.decoupled = decoupled ? 1 : 0;
+  d.maximize = maximize ? 1 : 0;
+  d.amsgrad = amsgrad ? 1 : 0;
+  d.lr = lr;
+  d.beta1 = beta1;
+  d.beta2 = beta2;
+  d.eps = eps;
+  d.weight_decay = weight_decay;
+  d.lr_device = lr_device;
+  d.grad_scale = scalar_ptr(grad_scale, dev, "grad_scale");
+  d.found_inf = scalar_ptr(found_inf, dev, "found_inf");
+  Workspace ws(pvb2_adamw_workspace_size((int)n), dev);
+  OCL_CHECK(pvb2_adamw_multi(&d, (int)n, ts.data(), ws.get(), ws.bytes, stream_for(dev)));
+}
+
+template <bool DECOUPLED>
+static void fused_adam_(at::TensorList self, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
+                        at::TensorList max_exp_avg_sqs, at::TensorList state_steps, double lr, double beta1,
+                        double beta2, double weight_decay, double eps, bool amsgrad, bool maximize,
+                        const std::optional<at::Tensor>& grad_scale, const std::optional<at::Tensor>& found_inf) {
+  fused_adam(DECOUPLED, self, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, state_steps, lr, nullptr, beta1, beta2,
+             weight_decay, eps, amsgrad, maximize, grad_scale, found_inf);
+}
+
+template <bool DECOUPLED>
+static void fused_adam_tensor_lr_(at::TensorList self, at::TensorList grads, at::TensorList exp_avgs,
+                                  at::TensorList exp_avg_sqs, at::TensorList max_exp_avg_sqs,
+                                  at::TensorList state_steps, const at::Tensor& lr, double beta1, double beta2,
+                                  double weight_decay, double eps, bool amsgrad, bool maximize,
+                                  const std::optional<at::Tensor>& grad_scale,
+                                  const std::optional<at::Tensor>& found_inf) {
+  if (self.empty()) return;
+  // a learning rate in host memory is a number; one on the device is read there
+  const bool host = lr.device().is_cpu();
+  fused_adam(DECOUPLED, self, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, state_steps,
+             host ? lr.item().toDouble() : 0.0, host ? nullptr : scalar_ptr(lr, self[0].device().index(), "lr"), beta1,
+             beta2, weight_decay, eps, amsgrad, maximize, grad_scale, found_inf);
+}
+
+// one step of pytorch_vulkan_b200.optim.AdamW for parameters of one type on
+// one device: counts the steps, then updates.  With scales, moments are 8-bit
+// codes (flat, in the parameters' memory order).
+static void adamw_step(const std::vector<at::Tensor>& params, const std::vector<at::Tensor>& grads,
+                       const std::vector<at::Tensor>& exp_avgs, const std::vector<at::Tensor>& exp_avg_sqs,
+                       const std::vector<at::Tensor>& exp_avg_scales, const std::vector<at::Tensor>& exp_avg_sq_scales,
+                       const std::vector<at::Tensor>& steps, double lr, double beta1, double beta2, double eps,
+                       double weight_decay, bool maximize) {
+  const size_t n = params.size();
+  if (n == 0) return;
+  const bool codes = !exp_avg_scales.empty();
+  TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && steps.size() == n &&
+                  exp_avg_scales.size() == (codes ? n : 0) && exp_avg_sq_scales.size() == (codes ? n : 0),
+              "ocl AdamW: lists of one length expected");
+  const int dev = params[0].device().index();
+  const c10::ScalarType type = params[0].scalar_type();
+  DeviceScope scope(dev);
+  OCL_OP("adamw_step", dev);
+  std::vector<pvb2_adamw_tensor> ts(n);
+  std::vector<at::Tensor> copies;  // gradients laid out unlike their parameters
+  for (size_t i = 0; i < n; ++i) {
+    const at::Tensor& p = params[i];
+    check_param(p, grads[i], dev, type, i);
+    const at::Tensor g = grad_like(grads[i], p);
+    if (!g.is_same(grads[i])) copies.push_back(g);
+    pvb2_adamw_tensor& t = ts[i];
+    memset(&t, 0, sizeof(t));
+    auto held = [&](const at::Tensor& x, c10::ScalarType want, int64_t numel, bool flat, const char* what) {
+      TORCH_CHECK(is_ocl(x) && x.device().index() == dev && x.scalar_type() == want && x.numel() == numel &&
+                      (flat ? x.is_contiguous() : same_layout(x, p)),
+                  "ocl AdamW: ", what, " ", i, " of the state does not fit its parameter");
+      return x.data_ptr();
+    };
+    t.numel = p.numel();
+    t.param = p.data_ptr();
+    t.grad = g.data_ptr();
+    const c10::ScalarType kind = codes ? at::kByte : at::kFloat;
+    t.exp_avg = held(exp_avgs[i], kind, t.numel, codes, "first moment");
+    t.exp_avg_sq = held(exp_avg_sqs[i], kind, t.numel, codes, "second moment");
+    if (codes) {
+      const int64_t blocks = (t.numel + 255) / 256;
+      t.exp_avg_scale = (float*)held(exp_avg_scales[i], at::kFloat, blocks, true, "scale of the first moment");
+      t.exp_avg_sq_scale = (float*)held(exp_avg_sq_scales[i], at::kFloat, blocks, true, "scale of the second moment");
+    }
+    t.step = step_ptr(steps[i], dev, i);
+  }
+  pvb2_adamw_desc d;
+  memset(&d, 0, sizeof(d));
+  d.param_dtype = dtype_code(type);
+  d.state_dtype = codes ? PVB2_U8 : PVB2_F32;
+  d.decoupled = 1;
+  d.maximize = maximize ? 1 : 0;
+  d.increment_step = 1;
+  d.lr = lr;
+  d.beta1 = beta1;
+  d.beta2 = beta2;
+  d.eps = eps;
+  d.weight_decay = weight_decay;
+  Workspace ws(pvb2_adamw_workspace_size((int)n), dev);
+  OCL_CHECK(pvb2_adamw_multi(&d, (int)n, ts.data(), ws.get(), ws.bytes, stream_for(dev)));
+  for (const at::Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();
+}
+
+// the moments that 8-bit codes stand for, into fp32 tensors
+static void adamw8_values(const std::vector<at::Tensor>& codes, const std::vector<at::Tensor>& scales,
+                          const std::vector<at::Tensor>& rms_codes, const std::vector<at::Tensor>& rms_scales,
+                          const std::vector<at::Tensor>& exp_avgs, const std::vector<at::Tensor>& exp_avg_sqs) {
+  const size_t n = codes.size();
+  if (n == 0) return;
+  TORCH_CHECK(scales.size() == n && rms_codes.size() == n && rms_scales.size() == n && exp_avgs.size() == n &&
+                  exp_avg_sqs.size() == n,
+              "ocl AdamW: lists of one length expected");
+  const int dev = codes[0].device().index();
+  DeviceScope scope(dev);
+  OCL_OP("adamw8_values", dev);
+  std::vector<pvb2_adamw_tensor> ts(n);
+  for (size_t i = 0; i < n; ++i) {
+    pvb2_adamw_tensor& t = ts[i];
+    memset(&t, 0, sizeof(t));
+    t.numel = codes[i].numel();
+    auto ptr = [&](const at::Tensor& x, c10::ScalarType want, int64_t numel, bool dense) {
+      TORCH_CHECK(is_ocl(x) && x.device().index() == dev && x.scalar_type() == want && x.numel() == numel &&
+                      (dense ? x.is_non_overlapping_and_dense() : x.is_contiguous()),
+                  "ocl AdamW: state or output ", i, " does not fit");
+      return x.data_ptr();
+    };
+    const int64_t blocks = (t.numel + 255) / 256;
+    t.exp_avg = ptr(codes[i], at::kByte, t.numel, false);
+    t.exp_avg_sq = ptr(rms_codes[i], at::kByte, t.numel, false);
+    t.exp_avg_scale = (float*)ptr(scales[i], at::kFloat, blocks, false);
+    t.exp_avg_sq_scale = (float*)ptr(rms_scales[i], at::kFloat, blocks, false);
+    t.param = ptr(exp_avgs[i], at::kFloat, t.numel, true);
+    t.grad = ptr(exp_avg_sqs[i], at::kFloat, t.numel, true);
+  }
+  OCL_CHECK(pvb2_adamw8_values((int)n, ts.data(), stream_for(dev)));
+  for (size_t i = 0; i < n; ++i) {
+    exp_avgs[i].unsafeGetTensorImpl()->bump_version();
+    exp_avg_sqs[i].unsafeGetTensorImpl()->bump_version();
+  }
+}
+
+// -------------------------------------------------- relative position bias
+static pvb2_relative_bias_desc bias_desc(c10::ScalarType type, int64_t buckets, int64_t heads, int64_t q_len,
+                                         int64_t k_len, bool bidirectional, int64_t max_distance, int64_t q_offset) {
+  TORCH_CHECK(type == at::kFloat || type == at::kHalf || type == at::kBFloat16,
+              "ocl relative_position_bias: fp32, fp16 or bf16 expected, got ", type);
+  const int64_t most = std::numeric_limits<int32_t>::max();
+  TORCH_CHECK(buckets <= most && heads <= most, "ocl relative_position_bias: table too large");
+  pvb2_relative_bias_desc d;
+  memset(&d, 0, sizeof(d));
+  d.H = (int32_t)heads;
+  d.num_buckets = (int32_t)buckets;
+  d.bidirectional = bidirectional ? 1 : 0;
+  d.dtype = dtype_code(type);
+  d.Lq = q_len;
+  d.Lk = k_len;
+  d.max_distance = max_distance;
+  d.q_offset = q_offset;
+  return d;
+}
+
+static at::Tensor relative_position_bias(const at::Tensor& table, int64_t q_len, int64_t k_len, bool bidirectional,
+                                         int64_t max_distance, int64_t q_offset) {
+  TORCH_CHECK(is_ocl(table) && table.dim() == 2, "ocl relative_position_bias: table [num_buckets, heads] on ocl expected");
+  TORCH_CHECK(q_len >= 0 && k_len >= 0, "ocl relative_position_bias: lengths below zero");
+  const int dev = table.device().index();
+  DeviceScope scope(dev);
+  OCL_OP("relative_position_bias", dev);
+  const pvb2_relative_bias_desc d = bias_desc(table.scalar_type(), table.size(0), table.size(1), q_len, k_len,
+                                              bidirectional, max_distance, q_offset);
+  const at::Tensor t = contiguous(table);
+  at::Tensor out = empty({1, table.size(1), q_len, k_len}, table.scalar_type(), dev);
+  OCL_CHECK(pvb2_relative_bias_fwd(&d, t.data_ptr(), out.data_ptr(), stream_for(dev)));
+  return out;
+}
+
+static at::Tensor relative_position_bias_backward(const at::Tensor& grad, int64_t num_buckets, bool bidirectional,
+                                                  int64_t max_distance, int64_t q_offset) {
+  TORCH_CHECK(is_ocl(grad) && grad.dim() == 4,
+              "ocl relative_position_bias_backward: grad [batch, heads, q_len, k_len] on ocl expected");
+  const int dev = grad.device().index();
+  DeviceScope scope(dev);
+  OCL_OP("relative_position_bias_backward", dev);
+  const pvb2_relative_bias_desc d = bias_desc(grad.scalar_type(), num_buckets, grad.size(1), grad.size(2), grad.size(3),
+                                              bidirectional, max_distance, q_offset);
+  at::Tensor out = empty({num_buckets, grad.size(1)}, grad.scalar_type(), dev);
+  Workspace ws(pvb2_relative_bias_bwd_workspace_size(&d, grad.size(0)), dev);
+  const pvb2_tensor g = desc(grad);
+  OCL_CHECK(pvb2_relative_bias_bwd(&d, &g, out.data_ptr(), ws.get(), ws.bytes, stream_for(dev)));
+  return out;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// the backward passes below are kernels, not differentiable ops
+static void no_double_backward(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "ocl ", op, ": the backward pass cannot be differentiated again");
+}
+
+struct RelativeBias : public torch::autograd::Function<RelativeBias> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& table, int64_t q_len, int64_t k_len,
+                            bool bidirectional, int64_t max_distance, int64_t q_offset) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->saved_data["buckets"] = table.size(0);
+    ctx->saved_data["bidirectional"] = bidirectional;
+    ctx->saved_data["max_distance"] = max_distance;
+    ctx->saved_data["q_offset"] = q_offset;
+    return relative_position_bias(table, q_len, k_len, bidirectional, max_distance, q_offset);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_double_backward("relative_position_bias");
+    at::Tensor g;
+    if (grads[0].defined())
+      g = relative_position_bias_backward(grads[0], ctx->saved_data["buckets"].toInt(),
+                                          ctx->saved_data["bidirectional"].toBool(),
+                                          ctx->saved_data["max_distance"].toInt(), ctx->saved_data["q_offset"].toInt());
+    const at::Tensor none;
+    return {g, none, none, none, none, none};
+  }
+};
+
+static at::Tensor relative_position_bias_autograd(const at::Tensor& table, int64_t q_len, int64_t k_len,
+                                                  bool bidirectional, int64_t max_distance, int64_t q_offset) {
+  TORCH_CHECK(table.dim() == 2, "ocl relative_position_bias: table [num_buckets, heads] expected");
+  return RelativeBias::apply(table, q_len, k_len, bidirectional, max_distance, q_offset);
+}
+
+}  // namespace ocl
+
+TORCH_LIBRARY(ocl, m) {
+  m.def("relative_position_bias(Tensor table, int q_len, int k_len, bool bidirectional, int max_distance, "
+        "int q_offset) -> Tensor");
+  m.def("relative_position_bias_backward(Tensor grad, int num_buckets, bool bidirectional, int max_distance, "
+        "int q_offset) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(ocl, PrivateUse1, m) {
+  m.impl("relative_position_bias", &ocl::relative_position_bias);
+  m.impl("relative_position_bias_backward", &ocl::relative_position_bias_backward);
+}
+
+TORCH_LIBRARY_IMPL(ocl, AutogradPrivateUse1, m) {
+  m.impl("relative_position_bias", &ocl::relative_position_bias_autograd);
+}
+
+TORCH_LIBRARY_IMPL(aten, PrivateUse1, m) {
+  m.impl("_fused_adam_", &ocl::fused_adam_<false>);
+  m.impl("_fused_adam_.tensor_lr", &ocl::fused_adam_tensor_lr_<false>);
+  m.impl("_fused_adamw_", &ocl::fused_adam_<true>);
+  m.impl("_fused_adamw_.tensor_lr", &ocl::fused_adam_tensor_lr_<true>);
+}
+
+void register_train_bindings(pybind11::module& m) {
+  m.def("impl_adamw_step", &ocl::adamw_step, "one AdamW step over parameters of one type on one device");
+  m.def("impl_adamw8_values", &ocl::adamw8_values, "the moments that 8-bit codes stand for");
+}

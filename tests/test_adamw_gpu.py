@@ -1,0 +1,405 @@
+"""Adam / AdamW steps on `ocl`: torch.optim's fused path and
+pytorch_vulkan_b200.optim.AdamW with 32-bit and 8-bit moments, against the
+formula in float64 on the CPU.
+
+Tolerances count roundings of fp32 (half a step is 2^-24 of the value): a
+moment is two products and a sum on rounded coefficients (at most 5 roundings
+of its larger term); the update is a root, a quotient, two products and a sum
+on rounded factors (at most 12, plus the moments' own); the parameter takes
+one product and one difference (3 of |p|, with the rounded factor) and, in 16
+bits, one rounding to its type.  8-bit moments are compared code by code with
+the formula in fp32, rounded operation by operation.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "ocl:0"
+U = 2.0 ** -24
+LR, B1, B2, EPS, WD = 1e-2, 0.9, 0.99, 1e-8, 0.05
+HYPER = dict(lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD)
+
+
+def reference(p, g, m, v, t, *, decoupled=True, maximize=False, vmax=None):
+    p, g, m, v = (x.double() for x in (p, g, m, v))
+    if maximize:
+        g = -g
+    if decoupled:
+        p = p * (1 - LR * WD)
+    else:
+        g = g + WD * p
+    m = B1 * m + (1 - B1) * g
+    v = B2 * v + (1 - B2) * g * g
+    w = v if vmax is None else torch.maximum(v, vmax.double())
+    up = LR / (1 - B1 ** t) * m / ((w / (1 - B2 ** t)).sqrt() + EPS)
+    return p - up, m, v, up, g, w
+
+
+def close(got, want, bound, what):
+    got = got.detach().cpu().double()
+    fine = torch.isfinite(want)
+    assert torch.equal(fine, torch.isfinite(got)), what
+    got, want, bound = got[fine], want[fine], bound[fine]
+    over = ((got - want).abs() - bound).max().item() if want.numel() else 0.0
+    assert over <= 0, f"{what}: over its bound by {over}"
+
+
+def check_step(p0, g, m0, v0, t, p, m, v, dtype):
+    """p, m, v after the step that began at p0, m0, v0 (CPU tensors)."""
+    rp, rm, rv, up, _, _ = reference(p0, g, m0, v0, t)
+    gd = g.double().abs()
+    close(m, rm, 5 * U * (m0.double().abs() + gd) + 1e-44, "m")
+    close(v, rv, 6 * U * rv + 1e-44, "v")
+    # the update inherits m's error, up to 5 U (|m0| + |g|) / |m| of it
+    spread = LR / (1 - B1 ** t) * (m0.double().abs() + gd) / ((rv / (1 - B2 ** t)).sqrt() + EPS)
+    bound = 3 * U * p0.double().abs() + 12 * U * up.abs() + 5 * U * spread + 1e-44
+    close(p, rp, bound + torch.finfo(dtype).eps / 2 * (rp.abs() + bound) * (dtype != torch.float32) + (6e-8 if dtype == torch.float16 else 0), "p")
+
+
+def rand(shape, g, scale=1.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+SHAPES = [(1,), (255,), (256,), (257,), (33, 65), (8192,), (8193,), (3, 5, 7, 11), (0,), (100, 300)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_adamw_32_bit_moments(ocl, dtype):
+    gen = torch.Generator().manual_seed(1)
+    ps = [rand(s, gen, 0.5, dtype) for s in SHAPES]
+    dev = [p.to(DEV).requires_grad_() for p in ps]
+    opt = ocl.optim.AdamW(dev, **HYPER)
+    ms, vs = [torch.zeros(s) for s in SHAPES], [torch.zeros(s) for s in SHAPES]
+    for t in range(1, 4):
+        gs = [rand(s, gen, 0.1, dtype) for s in SHAPES]
+        for d, g in zip(dev, gs):
+            d.grad = g.to(DEV)
+        opt.step()
+        for p, g, m, v, d in zip(ps, gs, ms, vs, dev):
+            s = opt.state[d]
+            check_step(p, g, m, v, t, d, s["exp_avg"], s["exp_avg_sq"], dtype)
+            assert s["exp_avg"].dtype == torch.float32 and s["step"].item() == t
+        # the next step begins from what the device holds
+        ps = [d.detach().cpu() for d in dev]
+        ms, vs = ([opt.state[d][k].cpu() for d in dev] for k in ("exp_avg", "exp_avg_sq"))
+
+
+def test_adamw_many_unaligned_tensors(ocl):
+    """300 tensors (more than one launch takes) at odd addresses."""
+    gen = torch.Generator().manual_seed(2)
+    sizes = [1 + (37 * i) % 701 for i in range(300)]
+    flat = {k: rand((sum(sizes) + 1,), gen, 0.3) for k in "pgmv"}
+    flat["v"] = flat["v"].abs()
+    held = {k: x.to(DEV) for k, x in flat.items()}
+    at, params, views = 1, [], []
+    opt = None
+    for n in sizes:
+        view = {k: held[k][at:at + n] for k in held}
+        view["p"].grad = view["g"]
+        params.append(view["p"])
+        views.append((at, n, view))
+        at += n
+    opt = ocl.optim.AdamW(params, **HYPER)
+    for (_, _, w), p in zip(views, params):
+        opt.state[p] = {"step": torch.full((), 4.0).to(DEV), "exp_avg": w["m"], "exp_avg_sq": w["v"]}
+    opt.step()
+    check_step(flat["p"][1:], flat["g"][1:], flat["m"][1:], flat["v"][1:], 5, held["p"][1:], held["m"][1:], held["v"][1:],
+               torch.float32)
+    for k in "pmv":  # what is before the first tensor stays
+        assert held[k][0].item() == flat[k][0].item()
+
+
+def test_adamw_channels_last_and_other_gradient_layout(ocl):
+    gen = torch.Generator().manual_seed(3)
+    p0, g0 = rand((6, 5, 4, 3), gen), rand((6, 5, 4, 3), gen)
+    p = p0.to(DEV).contiguous(memory_format=torch.channels_last).requires_grad_()
+    opt = ocl.optim.AdamW([p], **HYPER)
+    p.grad = g0.to(DEV)
+    opt.step()
+    zero = torch.zeros_like(p0)
+    check_step(p0, g0, zero, zero, 1, p, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq"], torch.float32)
+
+
+# ---------------------------------------------------------------- 8-bit moments
+def encode(y, mantissa):
+    n = y.numel()
+    y = torch.nn.functional.pad(y.reshape(-1), (0, -n % 256)).view(-1, 256)
+    s = y.abs().amax(1, keepdim=True) * torch.tensor(1.0 / (2.0 - 2.0 ** -mantissa))
+    r = torch.where(s > 0, y / s, torch.zeros(()))
+    bits = (r.abs() * 2.0 ** -112).view(torch.int32)
+    drop = 23 - mantissa
+    code = ((bits + (2 ** (drop - 1) - 1) + ((bits >> drop) & 1)) >> drop).clamp(max=16 * 2 ** mantissa - 1)
+    code = torch.where(r < 0, code | 128, code) if mantissa == 3 else torch.where((y > 0) & (code == 0), 1, code)
+    return code.to(torch.uint8).view(-1)[:n], s.view(-1)
+
+
+def decode(code, s, mantissa):
+    c = code.to(torch.int32)
+    top = c & 127 if mantissa == 3 else c
+    y = (top << (23 - mantissa)).view(torch.float32) * 2.0 ** 112 * s.repeat_interleave(256)[:c.numel()]
+    return torch.where(c > 127, -y, y) if mantissa == 3 else y
+
+
+def root(x):
+    # the nearest fp32 number to the root: torch's fp32 root on the CPU is a vector library's and may be one off in the
+    # last place; by way of float64 it is not (53 bits >= 2 * 24 + 2, so rounding twice is rounding once)
+    return x.double().sqrt().float()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_adamw_8_bit_moments(ocl, dtype):
+    gen = torch.Generator().manual_seed(4)
+    shapes = SHAPES + [(513, 9)]
+    ps = [rand(s, gen, 0.5, dtype) for s in shapes]
+    dev = [p.to(DEV).requires_grad_() for p in ps]
+    opt = ocl.optim.AdamW(dev, **HYPER, state_bits=8)
+    states = [[torch.zeros(p.numel(), dtype=torch.uint8), torch.zeros(-(-p.numel() // 256))] * 2 for p in ps]
+    f = torch.tensor  # coefficients as fp32
+    for t in range(1, 5):
+        # sizes that differ by element, some of them zero, one block of zeros
+        gs = [(rand(s, gen) * torch.exp(4 * rand(s, gen))).to(dtype) for s in shapes]
+        gs = [torch.where(g.abs() < 0.05, torch.zeros((), dtype=dtype), g) for g in gs]
+        gs[5][256:512] = 0
+        for d, g in zip(dev, gs):
+            d.grad = g.to(DEV)
+        opt.step()
+        for k, (p, g, d) in enumerate(zip(ps, gs, dev)):
+            if not p.numel():
+                continue
+            cm, sm, cu, su = states[k]
+            m0, u0 = decode(cm, sm, 3), decode(cu, su, 4)
+            gf = g.float().reshape(-1)
+            m = m0 * f(B1) + gf * f(1 - B1)
+            u = root(u0 * u0 * f(B2) + gf * gf * f(1 - B2))
+            want = [*encode(m, 3), *encode(u, 4)]
+            s = opt.state[d]
+            got = [s[key].cpu() for key in ("exp_avg_code", "exp_avg_scale", "exp_avg_rms_code", "exp_avg_rms_scale")]
+            for a, b, what in zip(got, want, ("codes of m", "scales of m", "codes of u", "scales of u")):
+                assert ((a == b) | ((a != a) & (b != b))).all(), f"step {t}, tensor {k}: {what}"
+            rp, rm, rv, up, _, _ = reference(p.reshape(-1), gf, m0, u0 * u0, t)
+            spread = LR / (1 - B1 ** t) * (m0.double().abs() + gf.double().abs()) / ((rv / (1 - B2 ** t)).sqrt() + EPS)
+            bound = 3 * U * p.double().abs().reshape(-1) + 14 * U * up.abs() + 5 * U * spread + 1e-44
+            bound = bound + torch.finfo(dtype).eps / 2 * (rp.abs() + bound) * (dtype != torch.float32) + (6e-8 if dtype == torch.float16 else 0)
+            close(d.reshape(-1), rp, bound, f"p of tensor {k} at step {t}")
+            # a stored moment is half a step of its code off at most (below 2^-14 s the step is fixed; a root that is
+            # not zero is one step off at most)
+            hm, hu = decode(got[0], got[1], 3).double(), decode(got[2], got[3], 4).double()
+            # (a gradient that fp16 cannot hold is infinite, and its block's moments are no numbers from then on)
+            at = torch.isfinite(hm) & torch.isfinite(hu) & torch.isfinite(rm) & torch.isfinite(rv)
+            assert at.all() or dtype == torch.float16
+            hm, hu, rm, rv = hm[at], hu[at], rm[at], rv[at]
+            step = got[1].double().repeat_interleave(256)[:at.numel()][at]
+            assert ((hm - rm).abs() <= rm.abs() * 2.0 ** -4 * (1 + 1e-5) + step * 2.0 ** -18 * (1 + 1e-5) + 1e-44).all()
+            step = got[3].double().repeat_interleave(256)[:at.numel()][at]
+            assert ((hu - rv.sqrt()).abs() <= rv.sqrt() * 2.0 ** -5 * (1 + 1e-5) + step * 2.0 ** -18 * (1 + 1e-5) + 1e-44).all()
+            assert ((hu > 0) == (u.double()[at] > 0)).all()
+            states[k] = got
+        ps = [d.detach().cpu() for d in dev]
+    outs = [[torch.empty(p.shape).to(DEV) for p in ps] for _ in range(2)]
+    opt.write_state_values(*outs)
+    for k, (cm, sm, cu, su) in enumerate(states):
+        if ps[k].numel():
+            assert torch.allclose(outs[0][k].cpu().reshape(-1), decode(cm, sm, 3), rtol=0, atol=0, equal_nan=True)
+            assert torch.allclose(outs[1][k].cpu().reshape(-1), decode(cu, su, 4).square(), rtol=0, atol=0, equal_nan=True)
+
+
+def test_adamw_8_bit_extremes(ocl):
+    """A block with one huge and otherwise tiny gradients, the least and the largest magnitudes, and a NaN that stays in
+    its own block."""
+    n = 256 * 4
+    g = torch.full((n,), 1e-6)
+    g[0] = 1e6
+    g[256:512] = 1e-30
+    g[512:768] = 1e18
+    g[800] = float("nan")
+    p = torch.ones(n).to(DEV).requires_grad_()
+    opt = ocl.optim.AdamW([p], **HYPER, state_bits=8)
+    p.grad = g.to(DEV)
+    opt.step()
+    m, v = torch.empty(n).to(DEV), torch.empty(n).to(DEV)
+    opt.write_state_values([m], [v])
+    want = (g * torch.tensor(1 - B1), root(g * g * torch.tensor(1 - B2)))
+    for got, y, bits in ((m, want[0], 3), (v, want[1], 4)):
+        ref = decode(*encode(y, bits), bits)
+        ref = ref if bits == 3 else ref.square()
+        assert torch.equal(got.cpu()[:768], ref[:768])
+        assert torch.isnan(got.cpu()[768:]).all()
+    assert torch.isfinite(p[:768].detach().cpu()).all()
+    assert (v.cpu()[1:256] > 0).all()  # roots far below the block's largest stay above zero
+    assert torch.isnan(p.detach().cpu()[800])
+
+
+# ---------------------------------------------------------------- torch's fused optimizers
+@pytest.mark.parametrize("cls", [torch.optim.AdamW, torch.optim.Adam], ids=["AdamW", "Adam"])
+@pytest.mark.parametrize("amsgrad", [False, True])
+@pytest.mark.parametrize("maximize", [False, True])
+def test_torch_fused_optimizers(ocl, cls, amsgrad, maximize):
+    gen = torch.Generator().manual_seed(5)
+    ps = [rand(s, gen) for s in SHAPES]
+    dev = [p.to(DEV).requires_grad_() for p in ps]
+    kw = dict(HYPER, amsgrad=amsgrad, maximize=maximize)
+    opt = cls(dev, fused=True, **kw)
+    state = [(torch.zeros(s), torch.zeros(s), torch.zeros(s) if amsgrad else None) for s in SHAPES]
+    launches = torch.ocl.kernel_launch_count()
+    for t in range(1, 4):
+        gs = [rand(s, gen, 0.2) for s in SHAPES]
+        for d, g in zip(dev, gs):
+            d.grad = g.to(DEV)
+        opt.step()
+        for p, g, d, (m, v, x) in zip(ps, gs, dev, state):
+            rp, rm, rv, up, ge, w = reference(p, g, m, v, t, decoupled=cls is torch.optim.AdamW, maximize=maximize, vmax=x)
+            s = opt.state[d]
+            # Adam's gradient has a product and a sum of its own (2 roundings of its terms)
+            ge = ge.abs() + WD * p.double().abs() + g.double().abs()
+            close(s["exp_avg"], rm, 7 * U * (m.double().abs() + ge), "m")
+            dv = 6 * U * rv + 4 * U * (1 - B2) * ge * ge
+            close(s["exp_avg_sq"], rv, dv, "v")
+            if amsgrad:
+                close(s["max_exp_avg_sq"], w, dv + 6 * U * w, "max v")
+            root = (w / (1 - B2 ** t)).sqrt() + EPS
+            scale = LR / (1 - B1 ** t)
+            # the update's error from v's: half of it, relative to w
+            bound = 3 * U * p.double().abs() + 12 * U * up.abs() + 7 * U * scale * (m.double().abs() + ge) / root + up.abs() * dv / (2 * w + 1e-300)
+            close(d, rp, 1.01 * bound, "p")
+        ps = [d.detach().cpu() for d in dev]
+        state = [(opt.state[d]["exp_avg"].cpu(), opt.state[d]["exp_avg_sq"].cpu(),
+                  opt.state[d]["max_exp_avg_sq"].cpu() if amsgrad else None) for d in dev]
+    # a step is the step counts, the factors and one launch over all tensors
+    assert torch.ocl.kernel_launch_count() - launches <= 3 * (3 + 2 * len(SHAPES))
+
+
+def _raw(op, p, g, m, v, step, **kw):
+    args = dict(lr=LR, beta1=B1, beta2=B2, weight_decay=WD, eps=EPS, amsgrad=False, maximize=False)
+    args.update(kw)
+    op([p], [g], [m], [v], [], [step], **args)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_fused_adamw_gradient_scale_found_inf_and_tensor_lr(ocl, dtype):
+    gen = torch.Generator().manual_seed(6)
+    p0, g0, m0, v0 = (rand((1000,), gen, 0.3, dtype) for _ in range(4))
+    v0 = v0.abs()
+    op = torch.ops.aten._fused_adamw_
+    p, g, m, v = (x.to(DEV) for x in (p0, (g0.float() * 128).to(dtype), m0, v0))
+    step, scale = torch.full((), 7.0).to(DEV), torch.full((), 128.0).to(DEV)
+    _raw(op, p, g, m, v, step, grad_scale=scale, found_inf=torch.ones(()).to(DEV))
+    for a, b in ((p, p0), (m, m0), (v, v0)):  # a step that is skipped changes nothing
+        assert torch.equal(a.cpu(), b)
+    _raw(op, p, g, m, v, step, grad_scale=scale, found_inf=torch.zeros(()).to(DEV), lr=torch.full((), LR).to(DEV))
+    assert torch.equal(g.cpu(), g0)  # powers of two: unscaled exactly, and written back
+    rp, rm, rv, up, _, _ = reference(p0, g0, m0, v0, 7)
+    h = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    tiny = 6e-8 if dtype == torch.float16 else 0.0
+    big = m0.double().abs() + g0.double().abs()
+    close(m, rm, (5 * U + h) * big + tiny, "m")
+    close(v, rv, (6 * U + h) * rv * 1.01 + tiny, "v")
+    # lr as an fp32 value on the device is off by one rounding
+    spread = LR / (1 - B1 ** 7) * big / ((rv / (1 - B2 ** 7)).sqrt() + EPS)
+    bound = 4 * U * p0.double().abs() + 14 * U * up.abs() + 5 * U * spread
+    close(p, rp, bound + h * (rp.abs() + bound) + tiny, "p")
+
+
+def test_captured_step_advances_like_eager_steps(ocl):
+    for bits in (32, 8):
+        gen = torch.Generator().manual_seed(7)
+        ps = [rand(s, gen) for s in SHAPES]
+        gs = [rand(s, gen, 0.1) for s in SHAPES]
+        results = []
+        for captured in (False, True):
+            dev = [p.to(DEV).requires_grad_() for p in ps]
+            opt = ocl.optim.AdamW(dev, **HYPER, state_bits=bits)
+            for d, g in zip(dev, gs):
+                d.grad = g.to(DEV)
+            opt.step()
+            if captured:
+                graph = torch.ocl.Graph()
+                with graph.capture():
+                    opt.step()
+                for _ in range(3):
+                    graph.replay()
+            else:
+                for _ in range(3):
+                    opt.step()
+            results.append([d.detach().cpu() for d in dev] + [v.cpu() for d in dev for v in opt.state[d].values()])
+            if captured:
+                graph.reset()
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_round_trip(ocl, bits):
+    gen = torch.Generator().manual_seed(8)
+    ps = [rand(s, gen, 1.0, torch.bfloat16) for s in SHAPES[:5]]
+    gs = [rand(s, gen, 0.1, torch.bfloat16) for s in SHAPES[:5]]
+
+    def make(values):
+        dev = [p.to(DEV).requires_grad_() for p in values]
+        for d, g in zip(dev, gs):
+            d.grad = g.to(DEV)
+        return dev, ocl.optim.AdamW(dev, **HYPER, state_bits=bits)
+
+    dev, opt = make(ps)
+    opt.step()
+    saved = opt.state_dict()
+    saved = {"state": {i: {k: v.cpu().clone() for k, v in s.items()} for i, s in saved["state"].items()},
+             "param_groups": saved["param_groups"]}
+    dev2, opt2 = make([d.detach().cpu() for d in dev])
+    opt2.load_state_dict(saved)
+    opt.step()
+    opt2.step()
+    for a, b in zip(dev, dev2):
+        assert torch.equal(a.cpu(), b.cpu())
+        for k, v in opt.state[a].items():
+            assert v.dtype == opt2.state[b][k].dtype and torch.equal(v.cpu(), opt2.state[b][k].cpu())
+    other = ocl.optim.AdamW(dev, **HYPER, state_bits=40 - bits)
+    with pytest.raises(ValueError, match="state of parameter"):
+        other.load_state_dict(saved)
+
+
+def test_refusals(ocl):
+    p = torch.zeros(8).to(DEV).requires_grad_()
+    for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1), dict(state_bits=4)):
+        with pytest.raises(ValueError):
+            ocl.optim.AdamW([p], **bad)
+    with pytest.raises(ValueError, match="twice"):
+        ocl.optim.AdamW([p, p])
+    with pytest.raises(ValueError, match="ocl device expected"):
+        ocl.optim.AdamW([torch.zeros(3, requires_grad=True)])
+    base = torch.zeros(8, 8).to(DEV)
+    gap = base[:, :4]  # rows with gaps between them
+    gap.grad = torch.zeros(8, 4).to(DEV)
+    with pytest.raises(RuntimeError, match="gaps or overlaps"):
+        ocl.optim.AdamW([gap]).step()
+    q = torch.zeros(4).to(DEV)
+    for kw, match in ((dict(g=torch.zeros(5).to(DEV)), "another shape"), (dict(g=torch.zeros(4)), "ocl:0"),
+                      (dict(m=torch.zeros(4, dtype=torch.float16).to(DEV)), "moments"),
+                      (dict(step=torch.zeros(())), "step")):
+        args = dict(p=q, g=torch.zeros(4).to(DEV), m=torch.zeros(4).to(DEV), v=torch.zeros(4).to(DEV),
+                    step=torch.ones(()).to(DEV))
+        args.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            _raw(torch.ops.aten._fused_adamw_, **args)
+    z = [torch.zeros(4).to(DEV) for _ in range(4)]
+    with pytest.raises(RuntimeError, match="listed twice"):
+        torch.ops.aten._fused_adamw_([z[0], z[0]], [z[1]] * 2, [z[2]] * 2, [z[3]] * 2, [], [torch.ones(()).to(DEV)] * 2, lr=LR,
+                                     beta1=B1, beta2=B2, weight_decay=0.0, eps=EPS, amsgrad=False, maximize=False)
+
+
+def test_on_another_stream(ocl):
+    """The step runs on the current stream, behind what was queued there."""
+    gen = torch.Generator().manual_seed(9)
+    p0, g0 = rand((100003,), gen), rand((100003,), gen)
+    p, g = p0.to(DEV).requires_grad_(), g0.to(DEV)
+    opt = ocl.optim.AdamW([p], **HYPER)
+    torch.ocl.synchronize()
+    stream = torch.Stream(device=DEV)
+    with stream:
+        p.grad = g * 2.0
+        opt.step()
+    stream.synchronize()
+    zero = torch.zeros_like(p0)
+    s = opt.state[p]
+    check_step(p0, g0 * 2, zero, zero, 1, p, s["exp_avg"], s["exp_avg_sq"], torch.float32)
