@@ -662,6 +662,44 @@ PVB2_API int pvb2_flatten_multi(int n, float* const* tensors, const int64_t* num
                        double scale, pvb2_stream stream);
 
 /* ------------------------------------------------------------------ */
+/* softmax cross entropy of a linear layer, z = x w^T + bias, without   */
+/* keeping z (the reference ran the linear layer, log_softmax and       */
+/* nll_loss one by one, vision_ops.cpp:243-351, loss_ops.cpp:23-213).   */
+/*   loss_i = lse_i - (1 - s) z_i,t(i) - s / V sum_j z_ij               */
+/* with s the label smoothing; rows whose target is ignore_index or     */
+/* outside [0, V) have no loss and no gradient, and may hold anything.  */
+/* x [N][D], w [V][D] of one type (fp32, fp16, bf16), unit stride along */
+/* D; bias [V] of that type or NULL.  Sums, maxima and losses are fp32. */
+/* 16-bit operands go to the tensor cores as they are.  fp32 ones go as */
+/* sums of bf16 numbers: three each in PVB2_MATH_FP32 (six products,    */
+/* 24 bits), two in PVB2_MATH_TF32 (three products, 16 bits).           */
+/* ------------------------------------------------------------------ */
+enum { PVB2_LOSS_NONE = 0, PVB2_LOSS_MEAN = 1, PVB2_LOSS_SUM = 2 };
+typedef struct pvb2_linear_ce_desc {
+  int64_t N, D, V;
+  int64_t ldx, ldw;          /* row strides, in elements */
+  int64_t ignore_index;
+  double label_smoothing;    /* in [0, 1] */
+  int32_t dtype, reduction, math;
+} pvb2_linear_ce_desc;
+/* out: N losses (PVB2_LOSS_NONE) or one; lse: N; count: one float, the
+ * number of rows that have a loss.  mean over no rows is NaN. */
+PVB2_API size_t pvb2_linear_ce_fwd_workspace_size(const pvb2_linear_ce_desc* d);
+PVB2_API int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias,
+                                const int64_t* target, float* out, float* lse, float* count, void* workspace,
+                                size_t workspace_bytes, pvb2_stream stream);
+/* grad_out: N floats (PVB2_LOSS_NONE) or one; lse and count from the forward
+ * pass.  dx [N][D], dw [V][D] contiguous, dbias [V], of the operands' type;
+ * each may be NULL. */
+PVB2_API size_t pvb2_linear_ce_bwd_workspace_size(const pvb2_linear_ce_desc* d);
+PVB2_API int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias,
+                                const int64_t* target, const float* lse, const float* count, const float* grad_out,
+                                void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes,
+                                pvb2_stream stream);
+/* whether a bounded wait of its kernels ever gave up (as pvb2_tc_status) */
+PVB2_API int pvb2_linear_ce_status(int* timed_out, int reset);
+
+/* ------------------------------------------------------------------ */
 /* learned relative position bias of attention scores (no counterpart   */
 /* in the reference)                                                    */
 /*   out[h][i][j] = table[bucket(j - i - q_offset)][h]                  */

@@ -1,8 +1,9 @@
-// What a transformer's training step needs beside its layers: the AdamW step
+// What a transformer's training step needs beside its layers: the softmax
+// cross entropy of a linear layer over a large vocabulary, the AdamW step
 // over many tensors (torch's _fused_adam_ / _fused_adamw_, and the 8-bit
 // state of pytorch_vulkan_b200.optim.AdamW) and the learned relative position
 // bias, as ops of the `ocl` namespace with their gradients.  The reference
-// had neither: its optimizers fell into one mul_/add_ launch per tensor and
+// had none of them: its optimizers fell into one mul_/add_ launch per tensor and
 // operation (src/pointwise_ops.cpp:115-234,407-434).
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/extension.h>
@@ -316,9 +317,165 @@ static at::Tensor relative_position_bias_autograd(const at::Tensor& table, int64
   return RelativeBias::apply(table, q_len, k_len, bidirectional, max_distance, q_offset);
 }
 
+// ------------------------------------------------- linear cross entropy
+// [rows, length] with unit stride along the length; 16-bit rows that lie 16
+// bytes apart begin on 16-byte boundaries.  Anything else is copied.
+static at::Tensor ce_operand(const at::Tensor& t) {
+  const int64_t R = t.size(0), C = t.size(1);
+  const bool rows = (C == 1 || t.stride(1) == 1) && (R <= 1 || t.stride(0) >= C);
+  const bool aligned = t.scalar_type() == at::kFloat || (R > 1 && t.stride(0) % 8 != 0) ||
+                       (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  if (rows && aligned) return t;
+  at::Tensor c = empty(t.sizes(), t.scalar_type(), t.device().index());
+  copy_into(c, t, false);
+  return c;
+}
+
+static pvb2_linear_ce_desc ce_desc(const at::Tensor& x, const at::Tensor& w, int64_t ignore_index, int64_t reduction,
+                                   double label_smoothing) {
+  pvb2_linear_ce_desc d;
+  memset(&d, 0, sizeof(d));
+  d.N = x.size(0);
+  d.D = x.size(1);
+  d.V = w.size(0);
+  d.ldx = x.stride(0);
+  d.ldw = w.stride(0);
+  d.ignore_index = ignore_index;
+  d.label_smoothing = label_smoothing;
+  d.dtype = dtype_code(x.scalar_type());
+  d.reduction = (int32_t)reduction;
+  d.math = math_mode() == PVB2_MATH_FP32 ? PVB2_MATH_FP32 : PVB2_MATH_TF32;
+  return d;
+}
+
+static void ce_check(const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
+                     const std::optional<at::Tensor>& bias) {
+  const char* op = "ocl linear_cross_entropy: ";
+  TORCH_CHECK(is_ocl(input) && is_ocl(weight) && is_ocl(target), op, "input, weight and target on ocl expected, got ",
+              input.device(), ", ", weight.device(), " and ", target.device());
+  const int dev = input.device().index();
+  TORCH_CHECK(weight.device().index() == dev && target.device().index() == dev, op, "tensors on one device expected");
+  TORCH_CHECK(adam_type(input.scalar_type()) && weight.scalar_type() == input.scalar_type(), op,
+              "input and weight of one type (fp32, fp16 or bf16) expected, got ", input.scalar_type(), " and ",
+              weight.scalar_type());
+  TORCH_CHECK(input.dim() >= 1 && weight.dim() == 2 && input.size(-1) == weight.size(1), op,
+              "input [..., features] and weight [classes, features] expected, got ", input.sizes(), " and ",
+              weight.sizes());
+  TORCH_CHECK(weight.size(0) > 0 && weight.size(1) > 0, op, "no classes or no features");
+  TORCH_CHECK(target.scalar_type() == at::kLong && target.sizes().equals(input.sizes().slice(0, input.dim() - 1)), op,
+              "int64 target shaped like the input without its features expected, got ", target.scalar_type(), " ",
+              target.sizes());
+  if (bias.has_value() && bias->defined())
+    TORCH_CHECK(is_ocl(*bias) && bias->device().index() == dev && bias->scalar_type() == input.scalar_type() &&
+                    bias->dim() == 1 && bias->size(0) == weight.size(0),
+                op, "bias [classes] of the input's type expected");
+}
+
+// (loss, log-sum-exp of each row, rows that have a loss)
+static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_forward(
+    const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target, const std::optional<at::Tensor>& bias,
+    int64_t ignore_index, int64_t reduction, double label_smoothing) {
+  ce_check(input, weight, target, bias);
+  TORCH_CHECK(reduction >= 0 && reduction <= 2, "ocl linear_cross_entropy: unknown reduction");
+  const int dev = input.device().index();
+  DeviceScope scope(dev);
+  OCL_OP("linear_cross_entropy", dev);
+  const at::Tensor x = ce_operand(input.reshape({-1, input.size(-1)})), w = ce_operand(weight);
+  const at::Tensor t = contiguous(target);
+  at::Tensor b;
+  if (bias.has_value() && bias->defined()) b = contiguous(*bias);
+  const pvb2_linear_ce_desc d = ce_desc(x, w, ignore_index, reduction, label_smoothing);
+  at::Tensor loss = reduction == PVB2_LOSS_NONE ? empty(target.sizes(), at::kFloat, dev) : empty({}, at::kFloat, dev);
+  at::Tensor lse = empty({d.N}, at::kFloat, dev), count = empty({}, at::kFloat, dev);
+  Workspace ws(pvb2_linear_ce_fwd_workspace_size(&d), dev);
+  OCL_CHECK(pvb2_linear_ce_fwd(&d, x.data_ptr(), w.data_ptr(), b.defined() ? b.data_ptr() : nullptr,
+                               (const int64_t*)t.data_ptr(), (float*)loss.data_ptr(), (float*)lse.data_ptr(),
+                               (float*)count.data_ptr(), ws.get(), ws.bytes, stream_for(dev)));
+  return {loss, lse, count};
+}
+
+static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backward(
+    const at::Tensor& grad, const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
+    const std::optional<at::Tensor>& bias, const at::Tensor& lse, const at::Tensor& count, int64_t ignore_index,
+    int64_t reduction, double label_smoothing, std::array<bool, 3> mask) {
+  ce_check(input, weight, target, bias);
+  const int dev = input.device().index();
+  const int64_t rows = target.numel();
+  TORCH_CHECK(is_ocl(grad) && grad.scalar_type() == at::kFloat && grad.numel() == (reduction == 0 ? rows : 1) &&
+                  is_ocl(lse) && lse.scalar_type() == at::kFloat && lse.numel() == rows && lse.is_contiguous() &&
+                  is_ocl(count) && count.scalar_type() == at::kFloat && count.numel() == 1,
+              "ocl linear_cross_entropy_backward: gradient or saved tensors do not fit");
+  DeviceScope scope(dev);
+  OCL_OP("linear_cross_entropy_backward", dev);
+  const at::Tensor x = ce_operand(input.reshape({-1, input.size(-1)})), w = ce_operand(weight);
+  const at::Tensor t = contiguous(target), g = contiguous(grad);
+  const bool has_bias = bias.has_value() && bias->defined();
+  at::Tensor b;
+  if (has_bias) b = contiguous(*bias);
+  const pvb2_linear_ce_desc d = ce_desc(x, w, ignore_index, reduction, label_smoothing);
+  at::Tensor dx, dw, db;
+  if (mask[0]) dx = empty(input.sizes(), input.scalar_type(), dev);
+  if (mask[1]) dw = empty(weight.sizes(), weight.scalar_type(), dev);
+  if (mask[2] && has_bias) db = empty({d.V}, input.scalar_type(), dev);
+  Workspace ws(pvb2_linear_ce_bwd_workspace_size(&d), dev);
+  OCL_CHECK(pvb2_linear_ce_bwd(&d, x.data_ptr(), w.data_ptr(), has_bias ? b.data_ptr() : nullptr,
+                               (const int64_t*)t.data_ptr(), (const float*)lse.data_ptr(),
+                               (const float*)count.data_ptr(), (const float*)g.data_ptr(),
+                               dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
+                               db.defined() ? db.data_ptr() : nullptr, ws.get(), ws.bytes, stream_for(dev)));
+  return {dx, dw, db};
+}
+
+static at::Tensor linear_cross_entropy(const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
+                                       const std::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction,
+                                       double label_smoothing) {
+  return std::get<0>(
+      linear_cross_entropy_forward(input, weight, target, bias, ignore_index, reduction, label_smoothing));
+}
+
+struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& input, const at::Tensor& weight,
+                            const at::Tensor& target, const std::optional<at::Tensor>& bias, int64_t ignore_index,
+                            int64_t reduction, double label_smoothing) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    at::Tensor loss, lse, count;
+    std::tie(loss, lse, count) =
+        linear_cross_entropy_forward(input, weight, target, bias, ignore_index, reduction, label_smoothing);
+    ctx->save_for_backward({input, weight, target, bias.value_or(at::Tensor()), lse, count});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["label_smoothing"] = label_smoothing;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_double_backward("linear_cross_entropy");
+    const at::Tensor none;
+    if (!grads[0].defined()) return {none, none, none, none, none, none, none};
+    const variable_list s = ctx->get_saved_variables();
+    const bool has_bias = s[3].defined();
+    // needs_input_grad counts the tensors that were passed: input, weight, target, bias
+    const std::array<bool, 3> mask = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                      has_bias && ctx->needs_input_grad(3)};
+    at::Tensor dx, dw, db;
+    std::tie(dx, dw, db) = linear_cross_entropy_backward(
+        grads[0], s[0], s[1], s[2], has_bias ? std::optional<at::Tensor>(s[3]) : std::nullopt, s[4], s[5],
+        ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt(),
+        ctx->saved_data["label_smoothing"].toDouble(), mask);
+    return {dx, dw, none, db, none, none, none};
+  }
+};
+
+static at::Tensor linear_cross_entropy_autograd(const at::Tensor& input, const at::Tensor& weight,
+                                                const at::Tensor& target, const std::optional<at::Tensor>& bias,
+                                                int64_t ignore_index, int64_t reduction, double label_smoothing) {
+  return LinearCrossEntropy::apply(input, weight, target, bias, ignore_index, reduction, label_smoothing);
+}
+
 }  // namespace ocl
 
 TORCH_LIBRARY(ocl, m) {
+  m.def("linear_cross_entropy(Tensor input, Tensor weight, Tensor target, Tensor? bias, int ignore_index, "
+        "int reduction, float label_smoothing) -> Tensor");
   m.def("relative_position_bias(Tensor table, int q_len, int k_len, bool bidirectional, int max_distance, "
         "int q_offset) -> Tensor");
   m.def("relative_position_bias_backward(Tensor grad, int num_buckets, bool bidirectional, int max_distance, "
@@ -326,11 +483,13 @@ TORCH_LIBRARY(ocl, m) {
 }
 
 TORCH_LIBRARY_IMPL(ocl, PrivateUse1, m) {
+  m.impl("linear_cross_entropy", &ocl::linear_cross_entropy);
   m.impl("relative_position_bias", &ocl::relative_position_bias);
   m.impl("relative_position_bias_backward", &ocl::relative_position_bias_backward);
 }
 
 TORCH_LIBRARY_IMPL(ocl, AutogradPrivateUse1, m) {
+  m.impl("linear_cross_entropy", &ocl::linear_cross_entropy_autograd);
   m.impl("relative_position_bias", &ocl::relative_position_bias_autograd);
 }
 

@@ -121,6 +121,14 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                : "memory");
 }
 
+// fp32 box added to global memory (each element once, at L2)
+__device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, const void* src, int c0, int c1, int c2) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   map),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // wait until at most N committed bulk groups still read their shared-memory source
@@ -189,6 +197,30 @@ __device__ __forceinline__ void mma_tf32(uint32_t d_tmem, uint64_t adesc, uint64
       : "memory");
 }
 
+// 16-bit operands (both fp16, or both bf16): rows of 64 elements (128 B), K
+// steps of 16.  K-major tiles are walked as above (32 bytes a step);
+// MN-major ones hold 64-element runs along M/N, one run per K index, 8-K-row
+// groups 1024 B apart (SBO), 64-element M/N blocks `lbo` bytes apart, a step
+// of 16 K rows 2048 bytes.
+__device__ __forceinline__ uint64_t desc_mnmajor16(uint32_t base, int kk, uint32_t lbo) {
+  return smem_desc(base + kk * 2048, lbo, 1024, 2);
+}
+
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) |
+         ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // arrive on `bar` once every tcgen05.mma issued so far by this thread has completed
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -219,7 +251,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
 // CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B for 32-bit MN-major tiles
 int encode_tiled(CUtensorMap* map, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
                  const uint32_t* box, CUtensorMapSwizzle swizzle,
-                 CUtensorMapL2promotion l2 = CU_TENSOR_MAP_L2_PROMOTION_L2_256B, const uint32_t* elem_strides = nullptr);
+                 CUtensorMapL2promotion l2 = CU_TENSOR_MAP_L2_PROMOTION_L2_256B, const uint32_t* elem_strides = nullptr,
+                 CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
 
 static inline int tc_timeout_flag_local(int* value, int reset) {
   cudaError_t e = cudaMemcpyFromSymbol(value, g_tc_timeout, sizeof(int));

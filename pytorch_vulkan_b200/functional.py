@@ -5,6 +5,32 @@ import torch
 
 from . import _C  # noqa: F401  (registers torch.ops.ocl)
 
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_cross_entropy(input, weight, target, bias=None, *, ignore_index=-100, reduction="mean", label_smoothing=0.0):
+    """``F.cross_entropy(F.linear(input, weight, bias), target, ...)`` without the logits.
+
+    ``input`` is ``[..., features]``, ``weight`` ``[classes, features]`` (a
+    linear layer's), both fp32, bf16 or fp16, ``target`` int64 ``[...]``; any
+    number of classes, from a classifier's to a language model's vocabulary.
+    The loss is fp32 whatever the operands' type: one number, or one per row
+    with ``reduction="none"``.  Gradients of ``input``, ``weight`` and ``bias``
+    have the operands' type, rounded once from fp32 sums.  The logits are
+    formed on the chip, by the forward pass and again, piece by piece of the
+    classes, by the backward pass; memory grows with neither the number of
+    classes nor that of rows alone, but by a bounded piece.
+
+    Rows whose target is ``ignore_index`` or out of range have no loss and no
+    gradient, whatever they hold.  fp32 operands are multiplied to fp32
+    accuracy in math mode 1 and to at least 16 bits in the default mode (see
+    ``torch.ocl.set_math_mode``).
+    """
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{reduction} is not a valid value for reduction")
+    return torch.ops.ocl.linear_cross_entropy(input, weight, target, bias, ignore_index, _REDUCTIONS[reduction],
+                                              float(label_smoothing))
+
 
 def relative_position_bias(table, q_len, k_len, *, bidirectional=True, max_distance=128, q_offset=0):
     """Learned relative position bias of attention scores: ``[1, heads, q_len, k_len]``.
