@@ -29,15 +29,18 @@
 
 namespace pvb2 {
 
-constexpr int kLBM = 128, kLBN = 256, kLBK = 64;
+constexpr int kLBM = 256;  // rows of a tile: 128 for each CTA of a pair
+constexpr int kLBK = 64;
 constexpr int kLProducers = 4, kLMmaWarp = 4, kLEpiWarps = 8;
 constexpr int kLThreads = (kLProducers + 1 + kLEpiWarps) * 32;
 
+// P planes of each operand a stage; this CTA's 128 rows of A and BN / 2 columns of B
+template <int P, int BN>
 struct LceSmem {
-  static constexpr int A_BYTES = kLBM * kLBK * 2;
-  static constexpr int B_BYTES = kLBN * kLBK * 2;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 4;
+  static constexpr int A_BYTES = 128 * kLBK * 2;
+  static constexpr int B_BYTES = BN / 2 * kLBK * 2;
+  static constexpr int STAGE_BYTES = P * (A_BYTES + B_BYTES);
+  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES;
   static constexpr int EPI_OFF = STAGES * STAGE_BYTES;  // one 4 KB store box per epilogue warp
   static constexpr int BAR_OFF = EPI_OFF + kLEpiWarps * 4096;
   static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16;
@@ -48,8 +51,6 @@ enum { kEpiStats = 0, kEpiGrad = 1, kEpiAcc = 2, kEpiOut = 3 };
 struct LceGemm {
   int M, N, K;
   int a_row0, b_row0;     // where the operands' rows (K-major) or K rows (MN-major) begin in their maps
-  int nseg;               // pairs of operand planes
-  int8_t pa[6], pb[6];
   int n_fast;             // tile order: columns fastest
   int splits, kb_per;     // kEpiAcc: split s takes k blocks [s kb_per, (s + 1) kb_per) into slab s
   // epilogues of logits: column n is vocabulary entry v0 + n
@@ -134,25 +135,54 @@ __device__ __forceinline__ void store_box(uint8_t* box, int lane, F fill_and_sto
   }
 }
 
-template <int EPI, typename T, bool PRECISE>
-__global__ void __launch_bounds__(kLThreads, 1)
+// products of operand planes, smallest first; the last is the main one
+template <int P>
+struct LcePairs {
+  static constexpr int N = P == 1 ? 1 : P == 2 ? 3 : 6;
+};
+template <int P>
+__device__ __forceinline__ constexpr int lce_pa(int i) {
+  return P == 3 ? (i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0) : P == 2 ? (i == 0 ? 1 : 0) : 0;
+}
+template <int P>
+__device__ __forceinline__ constexpr int lce_pb(int i) {
+  return P == 3 ? (i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0) : P == 2 ? (i == 1 ? 1 : 0) : 0;
+}
+
+// One tile: C[256 x BN] by a pair of CTAs.  With CHUNK = 0 the accumulator
+// takes the whole of K (BN = 256, two accumulators alternate between tiles).
+// With CHUNK > 0 (BN = 128) it takes CHUNK blocks of K and the epilogue adds
+// the chunks in registers: the tensor core cuts rather than rounds when it
+// adds to an accumulator, so that a sum over thousands of products drifts by
+// 2^-24 of itself for every 16 of them.  The small products of split operands
+// go to an accumulator of their own, which takes the whole of K.
+template <int EPI, typename T, int P, int BN, int CHUNK>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
     lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ LceGemm p, int a_mn, int b_mn) {
-  using L = LceSmem;
+  using L = LceSmem<P, BN>;
+  constexpr bool kPrecise = P > 1;
+  constexpr int kPairs = LcePairs<P>::N;
+  constexpr int kCols = BN / 2;             // columns of an epilogue warp
+  constexpr int kStages = L::STAGES;
+  constexpr int kIssuers = kStages < kLProducers ? kStages : kLProducers;
+  static_assert(CHUNK == 0 || kCols == 64, "chunked sums are held in 64 registers");
+  static_assert(CHUNK > 0 || P == 1, "split operands are summed in chunks");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  constexpr int kStages = L::STAGES;
-  uint64_t* full = (uint64_t*)(smem + L::BAR_OFF);
+  uint64_t* full = (uint64_t*)(smem + L::BAR_OFF);  // waited on in the even CTA
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
-  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* acc_empty = acc_full + 2;               // waited on in the even CTA
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles_m = (p.M + kLBM - 1) / kLBM, tiles_n = (p.N + kLBN - 1) / kLBN;
+  const int rank = (int)cluster_rank();
+  const int tiles_m = (p.M + kLBM - 1) / kLBM, tiles_n = (p.N + BN - 1) / BN;
   const int base_tiles = tiles_m * tiles_n, total_tiles = base_tiles * p.splits;
   const int kblocks = (p.K + kLBK - 1) / kLBK;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -161,105 +191,119 @@ __global__ void __launch_bounds__(kLThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kLEpiWarps);
+      mbar_init(&acc_empty[b], 2 * kLEpiWarps);
     }
     *abort = 0;
     fence_barrier_init();
   }
-  if (warp == kLMmaWarp) tmem_alloc(tmem_slot, 2 * kLBN);
+  if (warp == kLMmaWarp) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before either is signalled
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  // tile -> block row, block column, split
-  auto place = [&](int tile, int& mb, int& nb, int& sp) {
+  // tile -> block row, block column, first and last block of K
+  auto place = [&](int tile, int& mb, int& nb, int& sp, int& kb0, int& kb1) {
     sp = tile / base_tiles;
     const int t = tile % base_tiles;
     mb = p.n_fast ? t / tiles_n : t % tiles_m;
     nb = p.n_fast ? t % tiles_n : t / tiles_m;
+    kb0 = sp * p.kb_per;
+    kb1 = min(kblocks, kb0 + p.kb_per);
   };
 
-  if (warp < kLProducers) {
+  if (warp < kIssuers) {
+    // ------------------------------------------------- loads: stage s by warp s % kIssuers
     if (lane == 0) {
       tma_prefetch(&tmA);
       tma_prefetch(&tmB);
       uint32_t it = 0;
-      for (int tile = blockIdx.x; tile < total_tiles && !*abort; tile += gridDim.x) {
-        int mb, nb, sp;
-        place(tile, mb, nb, sp);
-        const int kb0 = sp * p.kb_per, kb1 = min(kblocks, kb0 + p.kb_per);
-        for (int seg = 0; seg < p.nseg; ++seg) {
-          const int za = p.pa[seg], zb = p.pb[seg];
-          for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const int s = it % kStages;
-            const uint32_t ph = (it / kStages) & 1;
-            if ((int)(it % kLProducers) != warp) continue;
-            if (!mbar_wait(&empty[s], ph ^ 1, abort)) break;
-            uint8_t* sa = smem + s * L::STAGE_BYTES;
-            uint8_t* sb = sa + L::A_BYTES;
-            mbar_arrive_expect_tx(&full[s], L::STAGE_BYTES);
+      for (int tile = pair; tile < total_tiles && !*abort; tile += pairs) {
+        int mb, nb, sp, kb0, kb1;
+        place(tile, mb, nb, sp, kb0, kb1);
+        const int am = mb * kLBM + rank * 128, bn = nb * BN + rank * kCols;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % kStages;
+          if (s % kIssuers != warp) continue;
+          if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, abort)) break;
+          uint8_t* sa = smem + s * L::STAGE_BYTES;
+          uint8_t* sb = sa + P * L::A_BYTES;
+          const uint32_t bar = even_cta_addr(&full[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE_BYTES);
+#pragma unroll
+          for (int z = 0; z < P; ++z) {
             if (!a_mn) {
-              tma_load_3d(sa, &tmA, &full[s], kb * kLBK, p.a_row0 + mb * kLBM, za);
+              tma_load_3d_pair(sa + z * L::A_BYTES, &tmA, bar, kb * kLBK, p.a_row0 + am, z);
             } else {
 #pragma unroll
-              for (int j = 0; j < kLBM / 64; ++j)
-                tma_load_3d(sa + j * 8192, &tmA, &full[s], mb * kLBM + 64 * j, p.a_row0 + kb * kLBK, za);
+              for (int j = 0; j < 2; ++j)
+                tma_load_3d_pair(sa + z * L::A_BYTES + j * 8192, &tmA, bar, am + 64 * j, p.a_row0 + kb * kLBK, z);
             }
             if (!b_mn) {
-              tma_load_3d(sb, &tmB, &full[s], kb * kLBK, p.b_row0 + nb * kLBN, zb);
+              tma_load_3d_pair(sb + z * L::B_BYTES, &tmB, bar, kb * kLBK, p.b_row0 + bn, z);
             } else {
 #pragma unroll
-              for (int j = 0; j < kLBN / 64; ++j)
-                tma_load_3d(sb + j * 8192, &tmB, &full[s], nb * kLBN + 64 * j, p.b_row0 + kb * kLBK, zb);
+              for (int j = 0; j < kCols / 64; ++j)
+                tma_load_3d_pair(sb + z * L::B_BYTES + j * 8192, &tmB, bar, bn + 64 * j, p.b_row0 + kb * kLBK, z);
             }
           }
         }
       }
     }
   } else if (warp == kLMmaWarp) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_f16(kLBM, kLBN, sizeof(T) == 2 && !std::is_same<T, __half>::value, a_mn, b_mn);
-      uint32_t it = 0;
+    // ------------------------------------------------- products, by the even CTA for both
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_f16(kLBM, BN, !std::is_same<T, __half>::value, a_mn, b_mn);
+      uint32_t it = 0, chunk = 0;
       int local = 0;
-      for (int tile = blockIdx.x; tile < total_tiles && !*abort; tile += gridDim.x, ++local) {
-        int mb, nb, sp;
-        place(tile, mb, nb, sp);
-        const int buf = local & 1;
-        if (!mbar_wait(&acc_empty[buf], ((local >> 1) & 1) ^ 1, abort)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + buf * kLBN;
-        const int kb0 = sp * p.kb_per, kb1 = min(kblocks, kb0 + p.kb_per);
-        const int iters = (kb1 - kb0) * p.nseg;
-        for (int k = 0; k < iters; ++k, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&full[s], (it / kStages) & 1, abort)) break;
+      for (int tile = pair; tile < total_tiles && !*abort; tile += pairs, ++local) {
+        int mb, nb, sp, kb0, kb1;
+        place(tile, mb, nb, sp, kb0, kb1);
+        const uint32_t d_small = tmem_base + (2 + (local & 1)) * BN;  // products of the lesser planes
+        for (int c0 = kb0; c0 < kb1; ++chunk) {
+          const int c1 = CHUNK ? min(kb1, c0 + CHUNK) : kb1;
+          const int buf = chunk & 1;
+          if (!mbar_wait(&acc_empty[buf], ((chunk >> 1) & 1) ^ 1, abort)) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * L::STAGE_BYTES);
-          const uint32_t sb = sa + L::A_BYTES;
+          const uint32_t d_main = tmem_base + buf * BN;
+          for (int kb = c0; kb < c1; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait(&full[s], (it / kStages) & 1, abort)) break;
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * L::STAGE_BYTES);
+            const uint32_t sb = sa + P * L::A_BYTES;
 #pragma unroll
-          for (int kk = 0; kk < kLBK / 16; ++kk) {
-            const uint64_t ad = a_mn ? desc_mnmajor16(sa, kk, 8192) : desc_kmajor(sa, kk);
-            const uint64_t bd = b_mn ? desc_mnmajor16(sb, kk, 8192) : desc_kmajor(sb, kk);
-            mma_f16(d_tmem, ad, bd, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+            for (int i = 0; i < kPairs; ++i) {
+              const uint32_t pa = sa + lce_pa<P>(i) * L::A_BYTES, pb = sb + lce_pb<P>(i) * L::B_BYTES;
+#pragma unroll
+              for (int kk = 0; kk < kLBK / 16; ++kk) {
+                const uint64_t ad = a_mn ? desc_mnmajor16(pa, kk, 8192) : desc_kmajor(pa, kk);
+                const uint64_t bd = b_mn ? desc_mnmajor16(pb, kk, 8192) : desc_kmajor(pb, kk);
+                if (i == kPairs - 1) mma_f16_pair(d_main, ad, bd, idesc, (kb > c0 || kk > 0) ? 1u : 0u);
+                else mma_f16_pair(d_small, ad, bd, idesc, (kb > kb0 || i > 0 || kk > 0) ? 1u : 0u);
+              }
+            }
+            mma_commit_pair(&empty[s]);
           }
-          mma_commit(&empty[s]);
+          mma_commit_pair(&acc_full[buf]);
+          c0 = c1;
         }
-        mma_commit(&acc_full[buf]);
       }
     }
-  } else {
-    // epilogue warps: TMEM lane quarter warp % 4, column half (warp - 5) / 4
+  } else if (warp > kLMmaWarp) {
+    // ------------------------------------------------- epilogue: TMEM lane quarter warp % 4, column half (warp - 5) / 4
     const int quarter = warp & 3, half = (warp - kLMmaWarp - 1) >> 2;
     uint8_t* box = smem + L::EPI_OFF + (warp - kLMmaWarp - 1) * 4096;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    uint32_t chunk = 0;
     int local = 0;
-    for (int tile = blockIdx.x; tile < total_tiles && !*abort; tile += gridDim.x, ++local) {
-      int mb, nb, sp;
-      place(tile, mb, nb, sp);
-      const int buf = local & 1;
-      const int m0 = mb * kLBM + quarter * 32, m = m0 + lane;
+    for (int tile = pair; tile < total_tiles && !*abort; tile += pairs, ++local) {
+      int mb, nb, sp, kb0, kb1;
+      place(tile, mb, nb, sp, kb0, kb1);
+      const int m0 = mb * kLBM + rank * 128 + quarter * 32, m = m0 + lane;
       const bool mrow = m < p.M;
-      const int nh = nb * kLBN + half * 128;  // first column of this warp
+      const int nh = nb * BN + half * kCols;  // first column of this warp
       int t = INT32_MIN;  // column of the row's target
       float row_lse = 0.f, row_g = 0.f;
       if (EPI == kEpiStats || EPI == kEpiGrad) {
@@ -273,17 +317,48 @@ __global__ void __launch_bounds__(kLThreads, 1)
         }
       }
       const float oscale = EPI == kEpiOut && p.out_scale ? *p.out_scale : 1.f;
-      if (!mbar_wait(&acc_full[buf], (local >> 1) & 1, abort)) break;
-      tc_fence_after();
       float mx = -INFINITY, sum = 0.f, zs = 0.f;
+      float v[64];
+      bool ok = true;
+      if (CHUNK > 0) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {  // 64 columns at a time
+        for (int c0 = kb0; c0 < kb1 && ok; c0 += CHUNK, ++chunk) {
+          const int buf = chunk & 1;
+          ok = mbar_wait(&acc_full[buf], (chunk >> 1) & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float u[32];
+            tmem_ld32(tmem_base + lanes + buf * BN + half * kCols + 32 * h, u);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[32 * h + j] += u[j];
+            if (kPairs > 1 && c0 + CHUNK >= kb1) {
+              tmem_ld32(tmem_base + lanes + (2 + (local & 1)) * BN + half * kCols + 32 * h, u);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[32 * h + j] += u[j];
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[buf]));
+        }
+      } else {
+        ok = mbar_wait(&acc_full[chunk & 1], (chunk >> 1) & 1, abort);
+        tc_fence_after();
+      }
+      if (!ok) break;
+#pragma unroll 1
+      for (int c = 0; c < kCols / 64; ++c) {  // 64 columns at a time
         const int n0 = nh + c * 64;
         if (n0 >= p.N) break;
-        float v[64];
-        const uint32_t ta = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * kLBN + half * 128 + c * 64;
-        tmem_ld32(ta, v);
-        tmem_ld32(ta + 32, v + 32);
+        if (CHUNK == 0) {
+          const uint32_t ta = tmem_base + lanes + (chunk & 1) * BN + half * kCols + c * 64;
+          tmem_ld32(ta, v);
+          tmem_ld32(ta + 32, v + 32);
+        }
         if (EPI == kEpiStats) {
           float cm = -INFINITY;
 #pragma unroll
@@ -298,16 +373,16 @@ __global__ void __launch_bounds__(kLThreads, 1)
           }
           const float nm = fmaxf(mx, cm);
           const float base = nm == -INFINITY ? 0.f : nm;
-          sum *= lce_exp<PRECISE>(mx - base);
+          sum *= lce_exp<kPrecise>(mx - base);
 #pragma unroll
-          for (int j = 0; j < 64; ++j) sum += lce_exp<PRECISE>(v[j] - base);
+          for (int j = 0; j < 64; ++j) sum += lce_exp<kPrecise>(v[j] - base);
           mx = nm;
         } else if (EPI == kEpiGrad) {
           const float flat = p.smoothing / (float)p.V;
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
             const float z = v[j] + (p.bias && n0 + j < p.N ? lce_bias(p, n0 + j) : 0.f);
-            float e = lce_exp<PRECISE>(z - row_lse) - flat;
+            float e = lce_exp<kPrecise>(z - row_lse) - flat;
             if (t == n0 + j) e -= 1.f - p.smoothing;
             v[j] = row_g == 0.f ? 0.f : e * row_g * p.gscale;
           }
@@ -364,29 +439,33 @@ __global__ void __launch_bounds__(kLThreads, 1)
         }
       }
       if (EPI == kEpiStats && mrow && nh < p.N) {
-        const int64_t at = (int64_t)(p.v0 / 128 + nh / 128) * p.part_ld + m;
+        const int64_t at = (int64_t)(p.v0 / kCols + nh / kCols) * p.part_ld + m;
         p.part[at] = make_float2(mx, sum);
         if (p.zsum) p.zsum[at] = zs;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (CHUNK == 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[chunk & 1]));
+        ++chunk;
+      }
     }
     if (lane == 0) bulk_wait_all();
   }
+  // ------------------------------------------------- teardown
   tc_fence_before();
   __syncthreads();
-  if (warp == kLMmaWarp) {
-    if (*abort) {
-      // let any MMA still in flight finish before the columns are released
-      if (lane == 0) mma_commit(&acc_full[0]);
-      __syncwarp();
-      const uint64_t t0 = globaltimer();
-      while (globaltimer() - t0 < 10000000ull) {
-      }
+  if (warp == kLMmaWarp && *abort) {
+    // let any MMA still in flight finish before the columns are released
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 10000000ull) {
     }
+  }
+  cluster_sync();  // neither CTA's shared memory goes while the other may signal it
+  if (warp == kLMmaWarp) {
+    __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, 2 * kLBN);
+    tmem_dealloc_pair(tmem_base, 512);
   }
 }
 
@@ -450,6 +529,85 @@ __global__ void __launch_bounds__(256)
       if (smoothing != 0.f) v = (1.f - smoothing) * v + smoothing * (l - zs / (float)V);
     }
     loss[i] = v;
+  }
+}
+
+// the same from logits that lie in S partial sums [S][rows][ld]: one block a
+// row
+__device__ __forceinline__ float lce_slab_logit(const float* __restrict__ slab, int S, int64_t size, int64_t at,
+                                                const void* bias, int64_t n, int bias_dtype) {
+  float z = slab[at];
+  for (int s = 1; s < S; ++s) z += slab[s * size + at];
+  return bias ? z + load_as<float>(bias, n, bias_dtype) : z;
+}
+
+__global__ void __launch_bounds__(256)
+    lce_slab_rows_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t ld, const void* __restrict__ bias,
+                         int bias_dtype, const int64_t* __restrict__ target, int64_t V, int64_t ignore, float smoothing,
+                         float* __restrict__ lse, float* __restrict__ loss) {
+  __shared__ float sm[8], ss[8], sz[8], zt;
+  const int64_t i = blockIdx.x, t = target[i];
+  const bool scored = lce_scored(t, V, ignore);
+  float mx = -INFINITY, sum = 0.f, zs = 0.f;
+  for (int64_t n = threadIdx.x; n < V; n += 256) {
+    const float z = lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, n, bias_dtype);
+    if (scored && n == t) zt = z;
+    const float nm = fmaxf(mx, z), base = nm == -INFINITY ? 0.f : nm;
+    sum = sum * expf(mx - base) + expf(z - base);
+    mx = nm;
+    zs += z;
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, mx, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
+    const float nm = fmaxf(mx, om), base = nm == -INFINITY ? 0.f : nm;
+    sum = sum * expf(mx - base) + os * expf(om - base);
+    mx = nm;
+    zs += __shfl_xor_sync(0xffffffffu, zs, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    sm[threadIdx.x >> 5] = mx;
+    ss[threadIdx.x >> 5] = sum;
+    sz[threadIdx.x >> 5] = zs;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int q = 1; q < 8; ++q) {
+      const float nm = fmaxf(mx, sm[q]), base = nm == -INFINITY ? 0.f : nm;
+      sum = sum * expf(mx - base) + ss[q] * expf(sm[q] - base);
+      mx = nm;
+      zs += sz[q];
+    }
+    const float l = (mx == -INFINITY ? 0.f : mx) + logf(sum);
+    lse[i] = l;
+    float v = 0.f;
+    if (scored) {
+      v = l - zt;
+      if (smoothing != 0.f) v = (1.f - smoothing) * v + smoothing * (l - zs / (float)V);
+    }
+    loss[i] = v;
+  }
+}
+
+// G [planes][rows][ldg] of the vocabulary's entries v0 .. v0 + width from such
+// logits
+template <typename T>
+__global__ void __launch_bounds__(256)
+    lce_slab_grad_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t ld, const void* __restrict__ bias,
+                         int bias_dtype, const int64_t* __restrict__ target, int64_t v0, int64_t width, int64_t V,
+                         int64_t ignore, float smoothing, const float* __restrict__ lse, const float* __restrict__ grow,
+                         float gscale, T* __restrict__ G, int64_t ldg, int planes) {
+  const int64_t i = blockIdx.x, tt = target[i];
+  const int64_t t = lce_scored(tt, V, ignore) ? tt - v0 : -1;
+  const float l = lse[i], g = grow[i], flat = smoothing / (float)V;
+  for (int64_t n = threadIdx.x; n < width; n += 256) {
+    float e = expf(lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, v0 + n, bias_dtype) - l) - flat;
+    if (n == t) e -= 1.f - smoothing;
+    e = g == 0.f ? 0.f : e * g * gscale;
+    for (int z = 0; z < planes; ++z) {
+      const T h = from_f32<T>(e);
+      G[(z * rows + i) * ldg + n] = h;
+      e -= to_f32(h);
+    }
   }
 }
 
@@ -570,23 +728,56 @@ __global__ void lce_dbias_kernel(const float* __restrict__ part, int parts, int6
 
 // --------------------------------------------------------------- host side
 static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static int lce_pairs_on_device() { return std::max(1, num_sms() / 2); }
+
+// How a product M x N x K is cut: tiles of 256 x bn, K in `splits` parts of
+// kb_per blocks (each part a slab of partial sums, joined by a launch of its
+// own).
+struct LceTiling {
+  int bn, splits, kb_per;
+  double cycles;
+};
+
+// The cut with the least modelled time.  Cycles of a K block of a tile:
+// 512 for 256 x 256 (both the MMAs' rate and that of the loads from L2), for
+// 256 x 128 the loads' 384, for split operands the MMAs' (256 a product).  A
+// tile costs about 2500 more (its last loads and its epilogue), joining slabs
+// their traffic and a launch.
+static LceTiling lce_tiling(int64_t M, int64_t N, int64_t K, int P, int64_t read_bytes, bool cut = true) {
+  const int64_t kb = cdiv(K, kLBK), pairs = lce_pairs_on_device();
+  const double read = read_bytes / 3200.0;  // cycles at 6.1 TB/s and 1.9 GHz
+  LceTiling best{0, 1, 0, 0};
+  for (int bn = P == 1 ? 256 : 128; bn >= 128; bn /= 2) {
+    const double block = P == 3 ? 1600 : P == 2 ? 800 : bn == 256 ? 520 : 400;
+    const int64_t tiles = cdiv(M, kLBM) * cdiv(N, bn);
+    const int64_t most = cut && tiles < pairs ? std::min<int64_t>(16, std::max<int64_t>(1, kb / 2)) : 1;
+    for (int64_t S = 1; S <= most; ++S) {
+      const int64_t per = cdiv(kb, S);
+      if (cdiv(kb, per) != S) continue;
+      double c = cdiv(tiles * S, pairs) * (per * block + 2500);
+      c = std::max(c, read);
+      if (S > 1) c += 6000 + (double)S * M * N * 8 / 3200.0;
+      if (!best.bn || c < best.cycles) best = LceTiling{bn, (int)S, (int)per, c};
+    }
+  }
+  return best;
+}
 
 struct LcePlan {
   int P;             // planes of an operand
-  int nseg;
   bool half;         // fp16 operands (bf16 otherwise)
   int64_t ldp;       // row length of packed operands
   bool pack_w;       // w is packed piece by piece
-  int64_t piece;     // vocabulary entries of a piece (backward; forward where w is packed)
+  int64_t piece;     // vocabulary entries of a piece
   int pieces;
-  // backward
-  int dx_splits, dx_kb;
-  int dw_splits, dw_kb;
+  LceTiling z, dx, dw;
   int colsum_parts;
   int64_t rows_per;
 };
 
-
+constexpr int64_t kLRowsFwd = 16384;  // rows whose parts are held at a time
 
 // 16-bit operands whose rows begin on 16-byte boundaries are read as they lie
 static bool lce_direct(const pvb2_linear_ce_desc* d, int64_t ld) { return d->dtype != PVB2_F32 && ld % 8 == 0; }
@@ -599,38 +790,48 @@ static pvb2_linear_ce_desc lce_normal(const pvb2_linear_ce_desc* d) {
   return n;
 }
 
-// K of a product with few tiles is cut so that every SM has one: at least 8
-// blocks of K each
-static void lce_split(int64_t M, int64_t N, int64_t K, int* splits, int* kb_per) {
-  const int64_t tiles = up(M, kLBM) / kLBM * (up(N, kLBN) / kLBN), kb = up(K, kLBK) / kLBK;
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>(num_sms() / tiles, kb / 8));
-  *kb_per = (int)((kb + s - 1) / s);
-  *splits = (int)((kb + *kb_per - 1) / *kb_per);
-}
-
 static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   LcePlan p;
   p.half = d->dtype == PVB2_F16;
   p.P = d->dtype != PVB2_F32 ? 1 : d->math == PVB2_MATH_FP32 ? 3 : 2;
-  p.nseg = p.P == 1 ? 1 : p.P == 2 ? 3 : 6;
   p.ldp = up(d->D, 8);
   p.pack_w = !lce_direct(d, d->ldw);
-  // G of a piece in about 128 MB, the packed piece of w in about 256 MB, at
+  const int64_t rows = backward ? d->N : std::min(d->N, kLRowsFwd);
+  const int64_t esize = 2 * p.P;
+  // most entries of a piece: a packed piece of w in 256 MB, G in 128 MB, at
   // least 1024 entries
-  int64_t piece = backward ? ((int64_t)128 << 20) / (std::max<int64_t>(d->N, 1) * 2 * p.P) : d->V;
-  if (p.pack_w) piece = std::min<int64_t>(piece, ((int64_t)256 << 20) / (p.ldp * 2 * p.P));
-  piece = std::max<int64_t>(1024, piece / kLBN * kLBN);
-  p.piece = std::min<int64_t>(piece, up(d->V, kLBN));
-  p.pieces = (int)((d->V + p.piece - 1) / p.piece);
+  int64_t most = up(d->V, 256);
+  if (p.pack_w) most = std::min<int64_t>(most, ((int64_t)256 << 20) / (p.ldp * esize));
+  if (backward) most = std::min<int64_t>(most, ((int64_t)128 << 20) / (rows * esize));
+  most = std::max<int64_t>(std::min<int64_t>(1024, up(d->V, 256)), most / 256 * 256);
+  auto cost = [&](int64_t width) {
+    double c = lce_tiling(rows, width, d->D, p.P, width * d->D * 2).cycles + 4000;
+    if (backward)
+      c += lce_tiling(rows, d->D, width, p.P, 0).cycles + lce_tiling(width, d->D, rows, p.P, 0).cycles + 8000;
+    return c;
+  };
+  p.piece = most;
+  if (backward && most < d->V) {
+    // widths from half of the most on: the one whose tiles fill the SMs best
+    double least = 0;
+    for (int64_t w = most; w >= std::max<int64_t>(1024, most / 2); w -= 256) {
+      const double c = d->V / w * cost(w) + (d->V % w ? cost(d->V % w) : 0);
+      if (least == 0 || c < 0.995 * least) {
+        least = c;
+        p.piece = w;
+      }
+    }
+  }
+  p.pieces = (int)cdiv(d->V, p.piece);
   const int64_t width = std::min(p.piece, d->V);
-  lce_split(d->N, d->D, width, &p.dx_splits, &p.dx_kb);
-  lce_split(width, d->D, d->N, &p.dw_splits, &p.dw_kb);
-  p.colsum_parts = (int)std::min<int64_t>(64, (d->N + 255) / 256);
-  p.rows_per = p.colsum_parts ? up((d->N + p.colsum_parts - 1) / p.colsum_parts, 8) : 0;
+  // the forward pass joins the slabs of a whole row
+  p.z = lce_tiling(rows, width, d->D, p.P, width * d->D * 2, backward || p.pieces == 1);
+  p.dx = lce_tiling(d->N, d->D, width, p.P, 0);
+  p.dw = lce_tiling(width, d->D, d->N, p.P, 0);
+  p.colsum_parts = (int)std::min<int64_t>(64, cdiv(d->N, 256));
+  p.rows_per = p.colsum_parts ? up(cdiv(d->N, p.colsum_parts), 8) : 0;
   return p;
 }
-
-constexpr int64_t kLRowsFwd = 16384;  // rows whose parts are held at a time
 
 // places in the workspace, 1024-byte aligned
 struct Arena {
@@ -646,38 +847,44 @@ struct Arena {
 
 struct LceFwdSpace {
   uint16_t *x, *w;
+  float* slab;
   float2* part;
   float *zsum, *ztarget, *loss;
 };
 
+static bool lce_slabs(const LcePlan& p) { return p.z.splits > 1; }
+
 static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceFwdSpace* s) {
   Arena a{(uint8_t*)base};
-  const int64_t rows = std::min(d->N, kLRowsFwd), parts = up(d->V, kLBN) / 128;
+  const int64_t rows = std::min(d->N, kLRowsFwd), parts = cdiv(up(d->V, 256), p.z.bn / 2);
+  const bool slabs = lce_slabs(p);
   s->x = a.take<uint16_t>(lce_direct(d, d->ldx) ? 0 : rows * p.ldp * p.P);
   s->w = a.take<uint16_t>(p.pack_w ? p.piece * p.ldp * p.P : 0);
-  s->part = a.take<float2>(rows * parts);
-  s->zsum = a.take<float>(d->label_smoothing != 0 ? rows * parts : 0);
-  s->ztarget = a.take<float>(rows);
+  s->slab = a.take<float>(slabs ? p.z.splits * rows * up(d->V, 4) : 0);
+  s->part = a.take<float2>(slabs ? 0 : rows * parts);
+  s->zsum = a.take<float>(!slabs && d->label_smoothing != 0 ? rows * parts : 0);
+  s->ztarget = a.take<float>(slabs ? 0 : rows);
   s->loss = a.take<float>(d->N);
   return a.at;
 }
 
 struct LceBwdSpace {
   uint16_t *x, *w, *G;
-  float *row, *factor, *dx, *dw, *colsum;
+  float *slab, *row, *factor, *dx, *dw, *colsum;
 };
 
 static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceBwdSpace* s) {
   Arena a{(uint8_t*)base};
-  const int64_t ld32 = up(d->D, 4);
+  const int64_t ld32 = up(d->D, 4), width = std::min(p.piece, d->V);
   s->x = a.take<uint16_t>(d->N * p.ldp * p.P);
   s->w = a.take<uint16_t>(p.pack_w ? p.piece * p.ldp * p.P : 0);
-  s->G = a.take<uint16_t>(d->N * p.piece * p.P);
+  s->G = a.take<uint16_t>(d->N * up(width, 8) * p.P);
+  s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
   s->factor = a.take<float>(1);
-  s->dx = a.take<float>(p.pieces > 1 || p.dx_splits > 1 ? p.dx_splits * d->N * ld32 : 0);
-  s->dw = a.take<float>(p.dw_splits > 1 ? p.dw_splits * p.piece * ld32 : 0);
-  s->colsum = a.take<float>(p.colsum_parts * p.piece);
+  s->dx = a.take<float>(p.pieces > 1 || p.dx.splits > 1 ? p.dx.splits * d->N * ld32 : 0);
+  s->dw = a.take<float>(p.dw.splits > 1 ? p.dw.splits * width * ld32 : 0);
+  s->colsum = a.take<float>(p.colsum_parts * width);
   return a.at;
 }
 
@@ -722,39 +929,48 @@ static int lce_map32(CUtensorMap* m, const void* base, int64_t cols, int64_t row
   return encode_tiled(m, 3, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-static void lce_segments(LceGemm* g, const LcePlan& p) {
-  static const int8_t a3[6] = {2, 0, 1, 1, 0, 0}, b3[6] = {0, 2, 1, 0, 1, 0};
-  static const int8_t a2[3] = {1, 0, 0}, b2[3] = {0, 1, 0};
-  g->nseg = p.nseg;
-  for (int i = 0; i < p.nseg; ++i) {
-    g->pa[i] = p.P == 3 ? a3[i] : p.P == 2 ? a2[i] : 0;
-    g->pb[i] = p.P == 3 ? b3[i] : p.P == 2 ? b2[i] : 0;
-  }
+// K-major operands: 128 rows of A, bn / 2 of B
+static int lce_map_a(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, const LcePlan& p) {
+  return lce_map(m, base, cols, rows, ld, p.P, 128, p.half);
+}
+static int lce_map_b(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, const LcePlan& p, int bn) {
+  return lce_map(m, base, cols, rows, ld, p.P, bn / 2, p.half);
+}
+// MN-major operands, and G as it is stored: 64 columns x 64 (32) rows
+static int lce_map_mn(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld, const LcePlan& p) {
+  return lce_map(m, base, cols, rows, ld, p.P, 64, p.half);
 }
 
-template <int EPI, typename T, bool PRECISE>
+template <int EPI, typename T, int P, int BN, int CHUNK>
 static int lce_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const LceGemm& g, bool a_mn,
                       bool b_mn, cudaStream_t s) {
-  constexpr int smem = LceSmem::TOTAL + 1024;
+  constexpr int smem = LceSmem<P, BN>::TOTAL + 1024;
+  auto kernel = lce_gemm_kernel<EPI, T, P, BN, CHUNK>;
   static std::atomic<uint64_t> attr_done{0};
   if (first_on_device(attr_done))
-    PVB2_CUDA_TRY(cudaFuncSetAttribute(lce_gemm_kernel<EPI, T, PRECISE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       smem));
-  const int64_t tiles = up(g.M, kLBM) / kLBM * (up(g.N, kLBN) / kLBN) * g.splits;
+    PVB2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t tiles = cdiv(g.M, kLBM) * cdiv(g.N, BN) * g.splits;
   PVB2_CHECK_ARG(tiles < INT32_MAX / 2, "linear cross entropy: too many tiles");
-  const int grid = (int)std::min<int64_t>(tiles, num_sms());
-  lce_gemm_kernel<EPI, T, PRECISE><<<grid, kLThreads, smem, s>>>(a, b, c, g, a_mn ? 1 : 0, b_mn ? 1 : 0);
+  const int grid = 2 * (int)std::min<int64_t>(tiles, lce_pairs_on_device());
+  kernel<<<grid, kLThreads, smem, s>>>(a, b, c, g, a_mn ? 1 : 0, b_mn ? 1 : 0);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
 
+// Chunks: split operands (results to fp32) every 4 blocks, 16 additions of the
+// main product; 16-bit ones on 256 x 128 tiles every 8, where there is time
+// for it since these tiles wait for their loads.
 template <int EPI>
 static int lce_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const LceGemm& g, bool a_mn,
-                    bool b_mn, const LcePlan& p, cudaStream_t s) {
-  if (p.half) return lce_launch<EPI, __half, false>(a, b, c, g, a_mn, b_mn, s);
-  if ((EPI == kEpiStats || EPI == kEpiGrad) && p.P > 1)
-    return lce_launch<EPI, __nv_bfloat16, true>(a, b, c, g, a_mn, b_mn, s);
-  return lce_launch<EPI, __nv_bfloat16, false>(a, b, c, g, a_mn, b_mn, s);
+                    bool b_mn, const LcePlan& p, int bn, cudaStream_t s) {
+  if (p.P == 3) return lce_launch<EPI, __nv_bfloat16, 3, 128, 4>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 2) return lce_launch<EPI, __nv_bfloat16, 2, 128, 4>(a, b, c, g, a_mn, b_mn, s);
+  if (p.half) {
+    if (bn == 256) return lce_launch<EPI, __half, 1, 256, 0>(a, b, c, g, a_mn, b_mn, s);
+    return lce_launch<EPI, __half, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
+  }
+  if (bn == 256) return lce_launch<EPI, __nv_bfloat16, 1, 256, 0>(a, b, c, g, a_mn, b_mn, s);
+  return lce_launch<EPI, __nv_bfloat16, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
 }
 
 static int lce_pack(const pvb2_linear_ce_desc* d, const LcePlan& p, const void* src, int64_t row0, int64_t rows,
@@ -787,17 +1003,37 @@ static int lce_join(const pvb2_linear_ce_desc* d, const float* slab, int S, int6
   return PVB2_OK;
 }
 
-static void lce_logits(LceGemm* g, const pvb2_linear_ce_desc* d, const LcePlan& p, const void* bias) {
-  memset(g, 0, sizeof(*g));
-  lce_segments(g, p);
-  g->K = (int)d->D;
-  g->splits = 1;
-  g->kb_per = INT32_MAX / 2;
-  g->bias = bias;
-  g->bias_dtype = d->dtype;
-  g->V = d->V;
-  g->ignore = d->ignore_index;
-  g->smoothing = (float)d->label_smoothing;
+static LceGemm lce_logits(const pvb2_linear_ce_desc* d, const void* bias, int64_t rows, int64_t v0, int64_t width,
+                          int w_row0, const int64_t* target) {
+  LceGemm g;
+  memset(&g, 0, sizeof(g));
+  g.M = (int)rows;
+  g.N = (int)width;
+  g.K = (int)d->D;
+  g.v0 = (int)v0;
+  g.b_row0 = w_row0;
+  g.splits = 1;
+  g.kb_per = INT32_MAX / 2;
+  g.bias = bias;
+  g.bias_dtype = d->dtype;
+  g.target = target;
+  g.V = d->V;
+  g.ignore = d->ignore_index;
+  g.smoothing = (float)d->label_smoothing;
+  return g;
+}
+
+static LceGemm lce_product(int64_t M, int64_t N, int64_t K, int b_row0, const LceTiling& t) {
+  LceGemm g;
+  memset(&g, 0, sizeof(g));
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = (int)K;
+  g.b_row0 = b_row0;
+  g.n_fast = 1;
+  g.splits = t.splits;
+  g.kb_per = t.splits > 1 ? t.kb_per : INT32_MAX / 2;
+  return g;
 }
 
 // a map that no kernel reads, where an epilogue has none
@@ -807,9 +1043,9 @@ static CUtensorMap no_map() {
   return m;
 }
 
-// the product A B into `out` (rows x D), through slabs where K is cut
+// the product A B (K not cut) into `out`, rows x D
 static int lce_out(const pvb2_linear_ce_desc* d, const LcePlan& p, const CUtensorMap& a, const CUtensorMap& b, LceGemm g,
-                   bool a_mn, int64_t rows, void* out, const float* factor, cudaStream_t s) {
+                   bool a_mn, int64_t rows, void* out, const float* factor, int bn, cudaStream_t s) {
   const int size = d->dtype == PVB2_F32 ? 4 : 2;
   CUtensorMap c = no_map();
   g.out = out;
@@ -821,7 +1057,32 @@ static int lce_out(const pvb2_linear_ce_desc* d, const LcePlan& p, const CUtenso
     if (size == 4) PVB2_TRY(lce_map32(&c, out, d->D, rows, d->D, 1));
     else PVB2_TRY(lce_map(&c, out, d->D, rows, d->D, 1, 32, p.half));
   }
-  return lce_gemm<kEpiOut>(a, b, c, g, a_mn, true, p, s);
+  return lce_gemm<kEpiOut>(a, b, c, g, a_mn, true, p, bn, s);
+}
+
+// logits of `rows` rows as partial sums
+static int lce_slab_logits(const pvb2_linear_ce_desc* d, const LcePlan& p, const CUtensorMap& x, const CUtensorMap& w,
+                           LceGemm g, float* slab, cudaStream_t s) {
+  CUtensorMap c;
+  g.splits = p.z.splits;
+  g.kb_per = p.z.kb_per;
+  PVB2_TRY(lce_map32(&c, slab, g.N, g.M, up(g.N, 4), p.z.splits));
+  return lce_gemm<kEpiAcc>(x, w, c, g, false, false, p, p.z.bn, s);
+}
+
+template <typename T>
+static int lce_bias_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, int64_t width,
+                         int64_t ldg, void* out, cudaStream_t s) {
+  const dim3 grid((unsigned)cdiv(width, 32), (unsigned)p.colsum_parts);
+  const int blocks = (int)cdiv(width, 256);
+  lce_colsum_kernel<<<grid, 256, 0, s>>>((const T*)sp.G, d->N, width, ldg, p.P, p.rows_per, sp.colsum);
+  PVB2_LAUNCH_CHECK();
+  if (d->dtype == PVB2_F32)
+    lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (float*)out);
+  else
+    lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (T*)out);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
 }
 
 }  // namespace pvb2
@@ -846,51 +1107,52 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   cudaStream_t s = as_stream(stream);
   float* loss = out;
   if (d->N > 0) {
-    PVB2_CHECK_ARG(workspace && workspace_bytes >= pvb2_linear_ce_fwd_workspace_size(d),
-                   "linear cross entropy: workspace of %zu bytes needed", pvb2_linear_ce_fwd_workspace_size(d));
     const LcePlan p = lce_plan(d, false);
     LceFwdSpace sp;
-    lce_fwd_space(d, p, (void*)(((uintptr_t)workspace + 1023) & ~(uintptr_t)1023), &sp);
+    const size_t need = lce_fwd_space(d, p, (void*)(((uintptr_t)workspace + 1023) & ~(uintptr_t)1023), &sp) + 1024;
+    PVB2_CHECK_ARG(workspace && workspace_bytes >= need, "linear cross entropy: workspace of %zu bytes needed", need);
     if (d->reduction != PVB2_LOSS_NONE) loss = sp.loss;
-    const bool direct_x = lce_direct(d, d->ldx), direct_w = !p.pack_w;
+    const bool direct_x = lce_direct(d, d->ldx), slabs = lce_slabs(p);
     PVB2_TRY(lce_aligned(x, direct_x));
-    PVB2_TRY(lce_aligned(w, direct_w));
-    const int64_t piece = direct_w ? up(d->V, kLBN) : p.piece;
-    const int parts = (int)(up(d->V, 128) / 128);
-    const int esize = d->dtype == PVB2_F32 ? 4 : 2;
+    PVB2_TRY(lce_aligned(w, !p.pack_w));
+    const int parts = (int)cdiv(d->V, p.z.bn / 2), esize = d->dtype == PVB2_F32 ? 4 : 2;
+    const float smoothing = (float)d->label_smoothing;
     for (int64_t r0 = 0; r0 < d->N; r0 += kLRowsFwd) {
       const int64_t rows = std::min(kLRowsFwd, d->N - r0);
       CUtensorMap ma, mb;
       if (direct_x) {
-        PVB2_TRY(lce_map(&ma, (const uint8_t*)x + r0 * d->ldx * esize, d->D, rows, d->ldx, 1, kLBM, p.half));
+        PVB2_TRY(lce_map_a(&ma, (const uint8_t*)x + r0 * d->ldx * esize, d->D, rows, d->ldx, p));
       } else {
         PVB2_TRY(lce_pack(d, p, x, r0, rows, d->ldx, sp.x, nullptr, s));
-        PVB2_TRY(lce_map(&ma, sp.x, d->D, rows, p.ldp, p.P, kLBM, p.half));
+        PVB2_TRY(lce_map_a(&ma, sp.x, d->D, rows, p.ldp, p));
       }
-      for (int64_t v0 = 0; v0 < d->V; v0 += piece) {
-        const int64_t width = std::min(piece, d->V - v0);
-        LceGemm g;
-        lce_logits(&g, d, p, bias);
-        if (direct_w) {
-          PVB2_TRY(lce_map(&mb, w, d->D, d->V, d->ldw, 1, kLBN, p.half));
-          g.b_row0 = (int)v0;
+      for (int64_t v0 = 0; v0 < d->V; v0 += p.piece) {
+        const int64_t width = std::min(p.piece, d->V - v0);
+        if (!p.pack_w) {
+          PVB2_TRY(lce_map_b(&mb, w, d->D, d->V, d->ldw, p, p.z.bn));
         } else {
           PVB2_TRY(lce_pack(d, p, w, v0, width, d->ldw, sp.w, nullptr, s));
-          PVB2_TRY(lce_map(&mb, sp.w, d->D, width, p.ldp, p.P, kLBN, p.half));
+          PVB2_TRY(lce_map_b(&mb, sp.w, d->D, width, p.ldp, p, p.z.bn));
         }
-        g.M = (int)rows;
-        g.N = (int)width;
-        g.v0 = (int)v0;
-        g.target = target + r0;
-        g.part = sp.part;
-        g.zsum = d->label_smoothing != 0 ? sp.zsum : nullptr;
-        g.ztarget = sp.ztarget;
-        g.part_ld = rows;
-        PVB2_TRY(lce_gemm<kEpiStats>(ma, mb, no_map(), g, false, false, p, s));
+        LceGemm g = lce_logits(d, bias, rows, v0, width, p.pack_w ? 0 : (int)v0, target + r0);
+        if (slabs) {
+          PVB2_TRY(lce_slab_logits(d, p, ma, mb, g, sp.slab, s));
+        } else {
+          g.part = sp.part;
+          g.zsum = smoothing != 0.f ? sp.zsum : nullptr;
+          g.ztarget = sp.ztarget;
+          g.part_ld = rows;
+          PVB2_TRY(lce_gemm<kEpiStats>(ma, mb, no_map(), g, false, false, p, p.z.bn, s));
+        }
       }
-      lce_rows_kernel<<<(int)((rows + 31) / 32), 256, 0, s>>>(
-          sp.part, d->label_smoothing != 0 ? sp.zsum : nullptr, rows, parts, sp.ztarget, target + r0, rows, d->V,
-          d->ignore_index, (float)d->label_smoothing, lse + r0, loss + r0);
+      if (slabs)
+        lce_slab_rows_kernel<<<(int)rows, 256, 0, s>>>(sp.slab, p.z.splits, rows, up(d->V, 4), bias, d->dtype,
+                                                       target + r0, d->V, d->ignore_index, smoothing, lse + r0,
+                                                       loss + r0);
+      else
+        lce_rows_kernel<<<(int)cdiv(rows, 32), 256, 0, s>>>(sp.part, smoothing != 0.f ? sp.zsum : nullptr, rows, parts,
+                                                            sp.ztarget, target + r0, rows, d->V, d->ignore_index,
+                                                            smoothing, lse + r0, loss + r0);
       PVB2_LAUNCH_CHECK();
     }
   }
@@ -920,12 +1182,12 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   }
   PVB2_CHECK_ARG(x && w && target && lse && count && grad_out, "linear cross entropy backward: null pointer");
   if (!dx && !dw && !dbias) return PVB2_OK;
-  PVB2_CHECK_ARG(workspace && workspace_bytes >= pvb2_linear_ce_bwd_workspace_size(d),
-                 "linear cross entropy backward: workspace of %zu bytes needed", pvb2_linear_ce_bwd_workspace_size(d));
   const LcePlan p = lce_plan(d, true);
   LceBwdSpace sp;
-  lce_bwd_space(d, p, (void*)(((uintptr_t)workspace + 1023) & ~(uintptr_t)1023), &sp);
-  const bool direct_w = !p.pack_w;
+  const size_t need = lce_bwd_space(d, p, (void*)(((uintptr_t)workspace + 1023) & ~(uintptr_t)1023), &sp) + 1024;
+  PVB2_CHECK_ARG(workspace && workspace_bytes >= need, "linear cross entropy backward: workspace of %zu bytes needed",
+                 need);
+  const bool direct_w = !p.pack_w, slabs = lce_slabs(p);
   PVB2_TRY(lce_aligned(w, direct_w));
   const float gscale = p.half ? 32768.f : 1.f;
   lce_grad_rows_kernel<<<1, 1024, 0, s>>>(grad_out, count, target, d->N, d->V, d->ignore_index, d->reduction,
@@ -933,102 +1195,74 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   PVB2_LAUNCH_CHECK();
   PVB2_TRY(lce_pack(d, p, x, 0, d->N, d->ldx, sp.x, target, s));
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;
-  PVB2_TRY(lce_map(&x_k, sp.x, d->D, d->N, p.ldp, p.P, kLBM, p.half));
-  PVB2_TRY(lce_map(&x_mn, sp.x, d->D, d->N, p.ldp, p.P, 64, p.half));
-  const bool dx_slabs = p.pieces > 1 || p.dx_splits > 1;
+  PVB2_TRY(lce_map_a(&x_k, sp.x, d->D, d->N, p.ldp, p));
+  PVB2_TRY(lce_map_mn(&x_mn, sp.x, d->D, d->N, p.ldp, p));
+  const bool dx_slabs = p.pieces > 1 || p.dx.splits > 1;
   const int64_t ld32 = up(d->D, 4);
   for (int q = 0; q < p.pieces; ++q) {
     const int64_t v0 = q * p.piece, width = std::min(p.piece, d->V - v0), ldg = up(width, 8);
     const int row0 = direct_w ? (int)v0 : 0;
     if (direct_w) {
-      PVB2_TRY(lce_map(&w_k, w, d->D, d->V, d->ldw, 1, kLBN, p.half));
-      PVB2_TRY(lce_map(&w_mn, w, d->D, d->V, d->ldw, 1, 64, p.half));
+      PVB2_TRY(lce_map_b(&w_k, w, d->D, d->V, d->ldw, p, p.z.bn));
+      PVB2_TRY(lce_map_mn(&w_mn, w, d->D, d->V, d->ldw, p));
     } else {
       PVB2_TRY(lce_pack(d, p, w, v0, width, d->ldw, sp.w, nullptr, s));
-      PVB2_TRY(lce_map(&w_k, sp.w, d->D, width, p.ldp, p.P, kLBN, p.half));
-      PVB2_TRY(lce_map(&w_mn, sp.w, d->D, width, p.ldp, p.P, 64, p.half));
+      PVB2_TRY(lce_map_b(&w_k, sp.w, d->D, width, p.ldp, p, p.z.bn));
+      PVB2_TRY(lce_map_mn(&w_mn, sp.w, d->D, width, p.ldp, p));
     }
     PVB2_TRY(lce_map(&g_store, sp.G, width, d->N, ldg, p.P, 32, p.half));
-    PVB2_TRY(lce_map(&g_k, sp.G, width, d->N, ldg, p.P, kLBM, p.half));
-    PVB2_TRY(lce_map(&g_mn, sp.G, width, d->N, ldg, p.P, 64, p.half));
+    PVB2_TRY(lce_map_a(&g_k, sp.G, width, d->N, ldg, p));
+    PVB2_TRY(lce_map_mn(&g_mn, sp.G, width, d->N, ldg, p));
     // G of this piece
-    LceGemm g;
-    lce_logits(&g, d, p, bias);
-    g.M = (int)d->N;
-    g.N = (int)width;
-    g.v0 = (int)v0;
-    g.b_row0 = row0;
-    g.target = target;
-    g.lse = lse;
-    g.grow = sp.row;
-    g.planes = p.P;
-    g.gscale = gscale;
-    PVB2_TRY(lce_gemm<kEpiGrad>(x_k, w_k, g_store, g, false, false, p, s));
+    LceGemm g = lce_logits(d, bias, d->N, v0, width, row0, target);
+    if (slabs) {
+      PVB2_TRY(lce_slab_logits(d, p, x_k, w_k, g, sp.slab, s));
+      if (p.half)
+        lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target,
+                                                       v0, width, d->V, d->ignore_index, (float)d->label_smoothing, lse,
+                                                       sp.row, gscale, (__half*)sp.G, ldg, p.P);
+      else
+        lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target,
+                                                       v0, width, d->V, d->ignore_index, (float)d->label_smoothing, lse,
+                                                       sp.row, gscale, (__nv_bfloat16*)sp.G, ldg, p.P);
+      PVB2_LAUNCH_CHECK();
+    } else {
+      g.lse = lse;
+      g.grow = sp.row;
+      g.planes = p.P;
+      g.gscale = gscale;
+      PVB2_TRY(lce_gemm<kEpiGrad>(x_k, w_k, g_store, g, false, false, p, p.z.bn, s));
+    }
     if (dx) {
-      LceGemm h;
-      memset(&h, 0, sizeof(h));
-      lce_segments(&h, p);
-      h.M = (int)d->N;
-      h.N = (int)d->D;
-      h.K = (int)width;
-      h.b_row0 = row0;
-      h.n_fast = 1;
+      LceGemm h = lce_product(d->N, d->D, width, row0, p.dx);
       if (dx_slabs) {
-        h.splits = p.dx_splits;
-        h.kb_per = p.dx_kb;
         // a last piece that is shorter leaves the far slabs alone
-        const int kb = (int)(up(width, kLBK) / kLBK);
-        if (q > 0) h.splits = std::min(h.splits, (kb + h.kb_per - 1) / h.kb_per);
+        if (p.dx.splits > 1) h.splits = (int)std::min<int64_t>(h.splits, cdiv(cdiv(width, kLBK), h.kb_per));
         h.accumulate = q > 0;
-        PVB2_TRY(lce_map32(&acc, sp.dx, d->D, d->N, ld32, p.dx_splits));
-        PVB2_TRY(lce_gemm<kEpiAcc>(g_k, w_mn, acc, h, false, true, p, s));
+        PVB2_TRY(lce_map32(&acc, sp.dx, d->D, d->N, ld32, p.dx.splits));
+        PVB2_TRY(lce_gemm<kEpiAcc>(g_k, w_mn, acc, h, false, true, p, p.dx.bn, s));
       } else {
-        h.splits = 1;
-        h.kb_per = INT32_MAX / 2;
-        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, sp.factor, s));
+        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, sp.factor, p.dx.bn, s));
       }
     }
     if (dw) {
-      LceGemm h;
-      memset(&h, 0, sizeof(h));
-      lce_segments(&h, p);
-      h.M = (int)width;
-      h.N = (int)d->D;
-      h.K = (int)d->N;
-      h.n_fast = 1;
+      LceGemm h = lce_product(width, d->D, d->N, 0, p.dw);
       void* out = (uint8_t*)dw + v0 * d->D * size;
-      if (p.dw_splits > 1) {
-        h.splits = p.dw_splits;
-        h.kb_per = p.dw_kb;
-        PVB2_TRY(lce_map32(&acc, sp.dw, d->D, width, ld32, p.dw_splits));
-        PVB2_TRY(lce_gemm<kEpiAcc>(g_mn, x_mn, acc, h, true, true, p, s));
-        PVB2_TRY(lce_join(d, sp.dw, p.dw_splits, width, sp.factor, out, s));
+      if (p.dw.splits > 1) {
+        PVB2_TRY(lce_map32(&acc, sp.dw, d->D, width, ld32, p.dw.splits));
+        PVB2_TRY(lce_gemm<kEpiAcc>(g_mn, x_mn, acc, h, true, true, p, p.dw.bn, s));
+        PVB2_TRY(lce_join(d, sp.dw, p.dw.splits, width, sp.factor, out, s));
       } else {
-        h.splits = 1;
-        h.kb_per = INT32_MAX / 2;
-        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, sp.factor, s));
+        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, sp.factor, p.dw.bn, s));
       }
     }
     if (dbias) {
-      const dim3 grid((unsigned)((width + 31) / 32), (unsigned)p.colsum_parts);
       void* out = (uint8_t*)dbias + v0 * size;
-      const int blocks = (int)((width + 255) / 256);
-      if (p.half) {
-        lce_colsum_kernel<<<grid, 256, 0, s>>>((const __half*)sp.G, d->N, width, ldg, p.P, p.rows_per, sp.colsum);
-        PVB2_LAUNCH_CHECK();
-        lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (__half*)out);
-      } else {
-        lce_colsum_kernel<<<grid, 256, 0, s>>>((const __nv_bfloat16*)sp.G, d->N, width, ldg, p.P, p.rows_per, sp.colsum);
-        PVB2_LAUNCH_CHECK();
-        if (d->dtype == PVB2_F32)
-          lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (float*)out);
-        else
-          lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (__nv_bfloat16*)out);
-      }
-      PVB2_LAUNCH_CHECK();
+      if (p.half) PVB2_TRY(lce_bias_grad<__half>(d, p, sp, width, ldg, out, s));
+      else PVB2_TRY(lce_bias_grad<__nv_bfloat16>(d, p, sp, width, ldg, out, s));
     }
   }
-  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx_splits, d->N, sp.factor, dx, s));
+  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, sp.factor, dx, s));
   return PVB2_OK;
 }
 
