@@ -680,22 +680,30 @@ typedef struct pvb2_linear_ce_desc {
   int64_t ldx, ldw;          /* row strides, in elements */
   int64_t ignore_index;
   double label_smoothing;    /* in [0, 1] */
+  int64_t kept;              /* 0, or what pvb2_linear_ce_keep made it */
   int32_t dtype, reduction, math;
 } pvb2_linear_ce_desc;
+/* A backward pass forms the logits again, piece by piece, unless the forward
+ * pass kept them: as 16-bit exponentials (fp32 logits for fp32 operands) of
+ * the first d->kept entries, all of them or a multiple of 256.  Sets d->kept
+ * to how many fit into `budget` bytes and returns the bytes that they take
+ * (0: none); that memory goes to the forward pass, and, as it left it, to
+ * the backward pass with the same descriptor. */
+PVB2_API size_t pvb2_linear_ce_keep(pvb2_linear_ce_desc* d, size_t budget);
 /* out: N losses (PVB2_LOSS_NONE) or one; lse: N; count: one float, the
  * number of rows that have a loss.  mean over no rows is NaN. */
 PVB2_API size_t pvb2_linear_ce_fwd_workspace_size(const pvb2_linear_ce_desc* d);
 PVB2_API int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias,
-                                const int64_t* target, float* out, float* lse, float* count, void* workspace,
-                                size_t workspace_bytes, pvb2_stream stream);
+                                const int64_t* target, float* out, float* lse, float* count, void* kept,
+                                void* workspace, size_t workspace_bytes, pvb2_stream stream);
 /* grad_out: N floats (PVB2_LOSS_NONE) or one; lse and count from the forward
  * pass.  dx [N][D], dw [V][D] contiguous, dbias [V], of the operands' type;
  * each may be NULL. */
 PVB2_API size_t pvb2_linear_ce_bwd_workspace_size(const pvb2_linear_ce_desc* d);
 PVB2_API int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias,
-                                const int64_t* target, const float* lse, const float* count, const float* grad_out,
-                                void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes,
-                                pvb2_stream stream);
+                                const int64_t* target, const float* lse, const float* count, const void* kept,
+                                const float* grad_out, void* dx, void* dw, void* dbias, void* workspace,
+                                size_t workspace_bytes, pvb2_stream stream);
 /* whether a bounded wait of its kernels ever gave up (as pvb2_tc_status) */
 PVB2_API int pvb2_linear_ce_status(int* timed_out, int reset);
 

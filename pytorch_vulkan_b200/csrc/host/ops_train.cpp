@@ -371,10 +371,23 @@ static void ce_check(const at::Tensor& input, const at::Tensor& weight, const at
                 op, "bias [classes] of the input's type expected");
 }
 
-// (loss, log-sum-exp of each row, rows that have a loss)
-static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_forward(
-    const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target, const std::optional<at::Tensor>& bias,
-    int64_t ignore_index, int64_t reduction, double label_smoothing) {
+// bytes that a forward pass may keep for its backward pass
+static size_t ce_keep_budget() {
+  const char* e = getenv("B200_CE_KEEP_MB");
+  const double mb = e ? atof(e) : 2048.0;
+  return mb > 0 ? (size_t)(mb * 1048576.0) : 0;
+}
+
+struct CeForward {
+  at::Tensor loss, lse, count;  // lse: of each row; count: rows that have a loss
+  at::Tensor kept;              // what the backward pass takes, of the first `entries` classes (undefined: none)
+  int64_t entries = 0;
+};
+
+static CeForward linear_cross_entropy_forward(const at::Tensor& input, const at::Tensor& weight,
+                                              const at::Tensor& target, const std::optional<at::Tensor>& bias,
+                                              int64_t ignore_index, int64_t reduction, double label_smoothing,
+                                              bool keep) {
   ce_check(input, weight, target, bias);
   TORCH_CHECK(reduction >= 0 && reduction <= 2, "ocl linear_cross_entropy: unknown reduction");
   const int dev = input.device().index();
@@ -384,20 +397,30 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_forwa
   const at::Tensor t = contiguous(target);
   at::Tensor b;
   if (bias.has_value() && bias->defined()) b = contiguous(*bias);
-  const pvb2_linear_ce_desc d = ce_desc(x, w, ignore_index, reduction, label_smoothing);
+  pvb2_linear_ce_desc d = ce_desc(x, w, ignore_index, reduction, label_smoothing);
+  CeForward r;
+  if (keep) {
+    const size_t bytes = pvb2_linear_ce_keep(&d, ce_keep_budget());
+    if (bytes) r.kept = empty({(int64_t)bytes}, at::kByte, dev);
+    r.entries = d.kept;
+  }
   at::Tensor loss = reduction == PVB2_LOSS_NONE ? empty(target.sizes(), at::kFloat, dev) : empty({}, at::kFloat, dev);
   at::Tensor lse = empty({d.N}, at::kFloat, dev), count = empty({}, at::kFloat, dev);
   Workspace ws(pvb2_linear_ce_fwd_workspace_size(&d), dev);
   OCL_CHECK(pvb2_linear_ce_fwd(&d, x.data_ptr(), w.data_ptr(), b.defined() ? b.data_ptr() : nullptr,
                                (const int64_t*)t.data_ptr(), (float*)loss.data_ptr(), (float*)lse.data_ptr(),
-                               (float*)count.data_ptr(), ws.get(), ws.bytes, stream_for(dev)));
-  return {loss, lse, count};
+                               (float*)count.data_ptr(), r.kept.defined() ? r.kept.data_ptr() : nullptr, ws.get(),
+                               ws.bytes, stream_for(dev)));
+  r.loss = loss;
+  r.lse = lse;
+  r.count = count;
+  return r;
 }
 
 static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backward(
     const at::Tensor& grad, const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
-    const std::optional<at::Tensor>& bias, const at::Tensor& lse, const at::Tensor& count, int64_t ignore_index,
-    int64_t reduction, double label_smoothing, std::array<bool, 3> mask) {
+    const std::optional<at::Tensor>& bias, const at::Tensor& lse, const at::Tensor& count, const at::Tensor& kept,
+    int64_t entries, int64_t ignore_index, int64_t reduction, double label_smoothing, std::array<bool, 3> mask) {
   ce_check(input, weight, target, bias);
   const int dev = input.device().index();
   const int64_t rows = target.numel();
@@ -412,7 +435,8 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backw
   const bool has_bias = bias.has_value() && bias->defined();
   at::Tensor b;
   if (has_bias) b = contiguous(*bias);
-  const pvb2_linear_ce_desc d = ce_desc(x, w, ignore_index, reduction, label_smoothing);
+  pvb2_linear_ce_desc d = ce_desc(x, w, ignore_index, reduction, label_smoothing);
+  d.kept = entries;
   at::Tensor dx, dw, db;
   if (mask[0]) dx = empty(input.sizes(), input.scalar_type(), dev);
   if (mask[1]) dw = empty(weight.sizes(), weight.scalar_type(), dev);
@@ -420,7 +444,8 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backw
   Workspace ws(pvb2_linear_ce_bwd_workspace_size(&d), dev);
   OCL_CHECK(pvb2_linear_ce_bwd(&d, x.data_ptr(), w.data_ptr(), has_bias ? b.data_ptr() : nullptr,
                                (const int64_t*)t.data_ptr(), (const float*)lse.data_ptr(),
-                               (const float*)count.data_ptr(), (const float*)g.data_ptr(),
+                               (const float*)count.data_ptr(), kept.defined() ? kept.data_ptr() : nullptr,
+                               (const float*)g.data_ptr(),
                                dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
                                db.defined() ? db.data_ptr() : nullptr, ws.get(), ws.bytes, stream_for(dev)));
   return {dx, dw, db};
@@ -429,8 +454,7 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backw
 static at::Tensor linear_cross_entropy(const at::Tensor& input, const at::Tensor& weight, const at::Tensor& target,
                                        const std::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction,
                                        double label_smoothing) {
-  return std::get<0>(
-      linear_cross_entropy_forward(input, weight, target, bias, ignore_index, reduction, label_smoothing));
+  return linear_cross_entropy_forward(input, weight, target, bias, ignore_index, reduction, label_smoothing, false).loss;
 }
 
 struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
@@ -438,14 +462,14 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
                             const at::Tensor& target, const std::optional<at::Tensor>& bias, int64_t ignore_index,
                             int64_t reduction, double label_smoothing) {
     at::AutoDispatchBelowADInplaceOrView below;
-    at::Tensor loss, lse, count;
-    std::tie(loss, lse, count) =
-        linear_cross_entropy_forward(input, weight, target, bias, ignore_index, reduction, label_smoothing);
-    ctx->save_for_backward({input, weight, target, bias.value_or(at::Tensor()), lse, count});
+    const CeForward r =
+        linear_cross_entropy_forward(input, weight, target, bias, ignore_index, reduction, label_smoothing, true);
+    ctx->save_for_backward({input, weight, target, bias.value_or(at::Tensor()), r.lse, r.count, r.kept});
+    ctx->saved_data["entries"] = r.entries;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["label_smoothing"] = label_smoothing;
-    return loss;
+    return r.loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_double_backward("linear_cross_entropy");
@@ -458,8 +482,8 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
                                       has_bias && ctx->needs_input_grad(3)};
     at::Tensor dx, dw, db;
     std::tie(dx, dw, db) = linear_cross_entropy_backward(
-        grads[0], s[0], s[1], s[2], has_bias ? std::optional<at::Tensor>(s[3]) : std::nullopt, s[4], s[5],
-        ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt(),
+        grads[0], s[0], s[1], s[2], has_bias ? std::optional<at::Tensor>(s[3]) : std::nullopt, s[4], s[5], s[6],
+        ctx->saved_data["entries"].toInt(), ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt(),
         ctx->saved_data["label_smoothing"].toDouble(), mask);
     return {dx, dw, none, db, none, none, none};
   }
@@ -468,6 +492,12 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
 static at::Tensor linear_cross_entropy_autograd(const at::Tensor& input, const at::Tensor& weight,
                                                 const at::Tensor& target, const std::optional<at::Tensor>& bias,
                                                 int64_t ignore_index, int64_t reduction, double label_smoothing) {
+  const bool grads = at::GradMode::is_enabled() && (input.requires_grad() || weight.requires_grad() ||
+                                                    (bias.has_value() && bias->defined() && bias->requires_grad()));
+  if (!grads) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return linear_cross_entropy(input, weight, target, bias, ignore_index, reduction, label_smoothing);
+  }
   return LinearCrossEntropy::apply(input, weight, target, bias, ignore_index, reduction, label_smoothing);
 }
 

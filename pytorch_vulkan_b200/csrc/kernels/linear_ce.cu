@@ -46,6 +46,20 @@ struct LceSmem {
   static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16;
 };
 
+// Kept exponentials, in [0, 1] relative to the largest of 64 columns, as 16-bit
+// numbers of their own: no sign, 4 bits of exponent (bias 15), 12 of mantissa.
+// Half a step is 2^-13 of the value down to 2^-14, and 2^-27 below; fp16 would
+// spend a bit on the sign and one on exponents that are not needed, and its
+// 2^-11 would add to the gradients' own rounding.  The bits are a float's with
+// the exponent shifted by 112.
+__device__ __forceinline__ uint32_t keep_code(float e) {
+  const uint32_t b = __float_as_uint(e * 1.925929944387235853055977942584927e-34f);  // 2^-112
+  return (b + 0x3ffu + ((b >> 11) & 1u)) >> 11;
+}
+__device__ __forceinline__ float keep_value(uint32_t code) {
+  return __uint_as_float(code << 11) * 5192296858534827628530496329220096.f;  // 2^112
+}
+
 enum { kEpiStats = 0, kEpiGrad = 1, kEpiAcc = 2, kEpiOut = 3 };
 
 struct LceGemm {
@@ -64,6 +78,9 @@ struct LceGemm {
   float* zsum;            // kEpiStats with smoothing: sums of z, laid out as part
   float* ztarget;
   int64_t part_ld;
+  int keep;               // kEpiStats: entries (of the whole vocabulary) below this one are kept
+  float* keep_max;        // what their exponentials are relative to: [64-column groups][keep_ld]
+  int64_t keep_ld;
   const float* lse;       // kEpiGrad
   const float* grow;      // kEpiGrad: g_i / max|g| (0 for rows without a loss)
   int planes;             // kEpiGrad: planes of G
@@ -76,9 +93,16 @@ struct LceGemm {
   const float* out_scale; // kEpiOut: factor on the device
 };
 
-__device__ __forceinline__ float lce_bias(const LceGemm& p, int n) {
-  if (!p.bias) return 0.f;
-  return load_as<float>(p.bias, p.v0 + n, p.bias_dtype);
+// the bias of 64 columns added to a row's logits: each lane fetches two, all
+// lanes take them in turn
+__device__ __forceinline__ void lce_add_bias(const LceGemm& p, int n0, int lane, float* v) {
+  const float b0 = n0 + lane < p.N ? load_as<float>(p.bias, p.v0 + n0 + lane, p.bias_dtype) : 0.f;
+  const float b1 = n0 + 32 + lane < p.N ? load_as<float>(p.bias, p.v0 + n0 + 32 + lane, p.bias_dtype) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    v[j] += __shfl_sync(0xffffffffu, b0, j);
+    v[32 + j] += __shfl_sync(0xffffffffu, b1, j);
+  }
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -112,6 +136,16 @@ __device__ __forceinline__ void box16(uint8_t* box, int lane, const float* v) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) w.e[k] = from_f32<T>(v[8 * q + k]);
     *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) * 16)) = w.u;
+  }
+}
+
+__device__ __forceinline__ void box_codes(uint8_t* box, int lane, const float* v) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = keep_code(v[8 * q + 2 * k]) | keep_code(v[8 * q + 2 * k + 1]) << 16;
+    *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -316,6 +350,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
           }
         }
       }
+      const float flat = EPI == kEpiGrad ? p.smoothing / (float)p.V : 0.f;
       const float oscale = EPI == kEpiOut && p.out_scale ? *p.out_scale : 1.f;
       float mx = -INFINITY, sum = 0.f, zs = 0.f;
       float v[64];
@@ -359,32 +394,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
           tmem_ld32(ta, v);
           tmem_ld32(ta + 32, v + 32);
         }
+        // whether any of the warp's targets is among these columns
+        const bool has_target = (EPI == kEpiStats || EPI == kEpiGrad) &&
+                                __any_sync(0xffffffffu, t >= n0 && t < n0 + 64);
+        if ((EPI == kEpiStats || EPI == kEpiGrad) && p.bias) lce_add_bias(p, n0, lane, v);
         if (EPI == kEpiStats) {
-          float cm = -INFINITY;
+          if (n0 + 64 > p.N) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            const bool in = n0 + j < p.N;
-            if (p.bias && in) v[j] += lce_bias(p, n0 + j);
-            if (p.zsum && in) zs += v[j];
-            if (t == n0 + j) p.ztarget[m] = v[j];
-            if (!in) v[j] = -INFINITY;
-            // a NaN logit makes the row's sum NaN by exp below
-            cm = fmaxf(cm, v[j]);
+            for (int j = 0; j < 64; ++j) {
+              if (p.zsum && n0 + j < p.N) zs += v[j];
+              if (n0 + j >= p.N) v[j] = -INFINITY;
+            }
+          } else if (p.zsum) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) zs += v[j];
           }
-          const float nm = fmaxf(mx, cm);
-          const float base = nm == -INFINITY ? 0.f : nm;
-          sum *= lce_exp<kPrecise>(mx - base);
+          if (has_target) {
+            float zt = 0.f;
 #pragma unroll
-          for (int j = 0; j < 64; ++j) sum += lce_exp<kPrecise>(v[j] - base);
-          mx = nm;
-        } else if (EPI == kEpiGrad) {
-          const float flat = p.smoothing / (float)p.V;
+            for (int j = 0; j < 64; ++j) zt = t == n0 + j ? v[j] : zt;
+            if (t >= n0 && t < n0 + 64) p.ztarget[m] = zt;
+          }
+          const bool keep = p.v0 + n0 < p.keep;
+          if (kPrecise && keep && m0 < p.M) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (p.v0 + n0 + 32 * h < p.keep)
+                store_box(box, lane, [&](int phase) {
+                  if (phase == 0) box32(box, lane, v + 32 * h);
+                  else tma_store_3d(&tmC, box, p.v0 + n0 + 32 * h, m0, 0);
+                });
+          }
+          float cm = v[0];
+#pragma unroll
+          for (int j = 1; j < 64; ++j) cm = fmaxf(cm, v[j]);  // a NaN logit makes the sum NaN instead
+          const float base = cm == -INFINITY ? 0.f : cm;
+          float cs = 0.f;
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
-            const float z = v[j] + (p.bias && n0 + j < p.N ? lce_bias(p, n0 + j) : 0.f);
-            float e = lce_exp<kPrecise>(z - row_lse) - flat;
-            if (t == n0 + j) e -= 1.f - p.smoothing;
-            v[j] = row_g == 0.f ? 0.f : e * row_g * p.gscale;
+            v[j] = lce_exp<kPrecise>(v[j] - base);
+            cs += v[j];
+          }
+          const float nm = fmaxf(mx, cm), nb = nm == -INFINITY ? 0.f : nm;
+          sum = sum * lce_exp<kPrecise>(mx - nb) + cs * lce_exp<kPrecise>(cm - nb);
+          mx = nm;
+          if (!kPrecise && keep && m0 < p.M) {
+            if (mrow) p.keep_max[(int64_t)((p.v0 + n0) >> 6) * p.keep_ld + m] = base;
+            store_box(box, lane, [&](int phase) {
+              if (phase == 0) box_codes(box, lane, v);
+              else tma_store_3d(&tmC, box, p.v0 + n0, m0, 0);
+            });
+          }
+        } else if (EPI == kEpiGrad) {
+          const float scale = row_g * p.gscale;
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = lce_exp<kPrecise>(v[j] - row_lse) - flat;
+          if (has_target) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] -= t == n0 + j ? 1.f - p.smoothing : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] *= scale;
+          if (__any_sync(0xffffffffu, row_g == 0.f)) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = row_g == 0.f ? 0.f : v[j];
           }
           if (m0 < p.M) {
             for (int z = 0; z < p.planes; ++z) {
@@ -414,10 +487,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] *= oscale;
           if (!p.out_tma) {
-            if (mrow) {
-              const int64_t row = (int64_t)m * p.out_ld;
-              for (int j = 0; j < 64; ++j)
-                if (n0 + j < p.N) store_as<float>(p.out, row + n0 + j, p.out_dtype, v[j]);
+            // through the box, rotated by the row: lanes then write along rows
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float* f = reinterpret_cast<float*>(box);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[lane * 32 + ((j + lane) & 31)] = v[32 * h + j];
+              __syncwarp();
+              const int n = n0 + 32 * h + lane;
+              if (n < p.N)
+                for (int r = 0; r < 32 && m0 + r < p.M; ++r)
+                  store_as<float>(p.out, (int64_t)(m0 + r) * p.out_ld + n, p.out_dtype, f[r * 32 + ((lane + r) & 31)]);
+              __syncwarp();
             }
           } else if (m0 < p.M) {
             if (p.out_dtype == PVB2_F32) {
@@ -475,34 +556,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
 // given (what they hold, NaN among it, then has no part in a product)
 template <typename S, typename T>
 __global__ void lce_pack_kernel(const S* __restrict__ src, int64_t rows, int64_t cols, int64_t ld, T* __restrict__ dst,
-                                int64_t ldp, int planes, const int64_t* __restrict__ target, int64_t V,
-                                int64_t ignore) {
-  const int64_t total = rows * ldp, plane = rows * ldp;
+                                int64_t ldp, int planes, const int64_t* __restrict__ target, int64_t V, int64_t ignore,
+                                int vec) {
+  const int per_row = (int)(ldp / 8);  // eight columns a thread
+  const int64_t total = rows * per_row, plane = rows * ldp;
   for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = e / ldp, c = e % ldp;
-    float v = c < cols ? to_f32(src[r * ld + c]) : 0.f;
-    if (target && !lce_scored(target[r], V, ignore)) v = 0.f;
+    const int64_t r = total <= INT32_MAX ? (int64_t)((int)e / per_row) : e / per_row;
+    const int64_t c = (e - r * per_row) * 8;
+    float v[8];
+    if (vec && c + 8 <= cols) {
+      load_vec<8>(src + r * ld + c, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(src[r * ld + c + k]) : 0.f;
+    }
+    if (target && !lce_scored(target[r], V, ignore)) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    }
     for (int z = 0; z < planes; ++z) {
-      const T h = from_f32<T>(v);
-      dst[z * plane + e] = h;
-      // infinity is its first part alone
-      v = isinf(to_f32(h)) ? 0.f : v - to_f32(h);
+      store_vec<8>(dst + z * plane + r * ldp + c, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        // infinity is its first part alone
+        const float h = to_f32(from_f32<T>(v[k]));
+        v[k] = isinf(h) ? 0.f : v[k] - h;
+      }
     }
   }
 }
 
 // joins the parts of each row: lse and loss (0 for rows without one).  32
-// rows a block, 8 threads a row.
-__global__ void __launch_bounds__(256)
+// rows a block, 32 threads a row.
+__global__ void __launch_bounds__(1024)
     lce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zsum, int64_t part_ld, int parts,
                     const float* __restrict__ ztarget, const int64_t* __restrict__ target, int64_t N, int64_t V,
                     int64_t ignore, float smoothing, float* __restrict__ lse, float* __restrict__ loss) {
-  __shared__ float sm[8][32], ss[8][32], sz[8][32];
+  __shared__ float sm[32][33], ss[32][33], sz[32][33];
   const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t i = (int64_t)blockIdx.x * 32 + r;
   float mx = -INFINITY, sum = 0.f, zs = 0.f;
   if (i < N) {
-    for (int q = g; q < parts; q += 8) {
+#pragma unroll 4
+    for (int q = g; q < parts; q += 32) {
       const float2 v = part[q * part_ld + i];
       const float nm = fmaxf(mx, v.x), base = nm == -INFINITY ? 0.f : nm;
       sum = sum * expf(mx - base) + v.y * expf(v.x - base);
@@ -514,21 +610,27 @@ __global__ void __launch_bounds__(256)
   ss[g][r] = sum;
   sz[g][r] = zs;
   __syncthreads();
-  if (g == 0 && i < N) {
-    for (int q = 1; q < 8; ++q) {
-      const float nm = fmaxf(mx, sm[q][r]), base = nm == -INFINITY ? 0.f : nm;
-      sum = sum * expf(mx - base) + ss[q][r] * expf(sm[q][r] - base);
-      mx = nm;
-      zs += sz[q][r];
-    }
+  // warp g takes row g, its lanes the 32 threads' shares
+  mx = sm[r][g];
+  sum = ss[r][g];
+  zs = sz[r][g];
+  for (int o = 16; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, mx, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
+    const float nm = fmaxf(mx, om), base = nm == -INFINITY ? 0.f : nm;
+    sum = sum * expf(mx - base) + os * expf(om - base);
+    mx = nm;
+    zs += __shfl_xor_sync(0xffffffffu, zs, o);
+  }
+  const int64_t row = (int64_t)blockIdx.x * 32 + g;
+  if (r == 0 && row < N) {
     const float l = (mx == -INFINITY ? 0.f : mx) + logf(sum);
-    lse[i] = l;
+    lse[row] = l;
     float v = 0.f;
-    if (lce_scored(target[i], V, ignore)) {
-      v = l - ztarget[i];
+    if (lce_scored(target[row], V, ignore)) {
+      v = l - ztarget[row];
       if (smoothing != 0.f) v = (1.f - smoothing) * v + smoothing * (l - zs / (float)V);
     }
-    loss[i] = v;
+    loss[row] = v;
   }
 }
 
@@ -541,16 +643,18 @@ __device__ __forceinline__ float lce_slab_logit(const float* __restrict__ slab, 
   return bias ? z + load_as<float>(bias, n, bias_dtype) : z;
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
     lce_slab_rows_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t ld, const void* __restrict__ bias,
                          int bias_dtype, const int64_t* __restrict__ target, int64_t V, int64_t ignore, float smoothing,
-                         float* __restrict__ lse, float* __restrict__ loss) {
-  __shared__ float sm[8], ss[8], sz[8], zt;
+                         float* __restrict__ lse, float* __restrict__ loss, float* __restrict__ kept, int64_t keep,
+                         int64_t keep_ld, float* __restrict__ ztarget) {
+  __shared__ float sm[16], ss[16], sz[16], zt;
   const int64_t i = blockIdx.x, t = target[i];
   const bool scored = lce_scored(t, V, ignore);
   float mx = -INFINITY, sum = 0.f, zs = 0.f;
-  for (int64_t n = threadIdx.x; n < V; n += 256) {
+  for (int64_t n = threadIdx.x; n < V; n += 512) {
     const float z = lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, n, bias_dtype);
+    if (n < keep) kept[i * keep_ld + n] = z;
     if (scored && n == t) zt = z;
     const float nm = fmaxf(mx, z), base = nm == -INFINITY ? 0.f : nm;
     sum = sum * expf(mx - base) + expf(z - base);
@@ -571,7 +675,7 @@ __global__ void __launch_bounds__(256)
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int q = 1; q < 8; ++q) {
+    for (int q = 1; q < 16; ++q) {
       const float nm = fmaxf(mx, sm[q]), base = nm == -INFINITY ? 0.f : nm;
       sum = sum * expf(mx - base) + ss[q] * expf(sm[q] - base);
       mx = nm;
@@ -583,6 +687,7 @@ __global__ void __launch_bounds__(256)
     if (scored) {
       v = l - zt;
       if (smoothing != 0.f) v = (1.f - smoothing) * v + smoothing * (l - zs / (float)V);
+      if (ztarget) ztarget[i] = zt;
     }
     loss[i] = v;
   }
@@ -607,6 +712,56 @@ __global__ void __launch_bounds__(256)
       const T h = from_f32<T>(e);
       G[(z * rows + i) * ldg + n] = h;
       e -= to_f32(h);
+    }
+  }
+}
+
+// the same from what the forward pass kept of the entries [v0, v0 + width),
+// eight columns a thread: logits in fp32 (FP32), or their exponentials as
+// 16-bit codes relative to a maximum per row and 64 columns.  The target's own comes from
+// its logit in fp32, since 1 - p may be far smaller than p's rounding.
+template <typename T, bool FP32>
+__global__ void __launch_bounds__(256)
+    lce_kept_grad_kernel(const void* __restrict__ kept, int64_t keep_ld, const float* __restrict__ keep_max,
+                         const float* __restrict__ ztarget, int64_t rows, const int64_t* __restrict__ target,
+                         int64_t v0, int64_t width, int64_t V, int64_t ignore, float smoothing,
+                         const float* __restrict__ lse, const float* __restrict__ grow, float gscale,
+                         T* __restrict__ G, int64_t ldg, int planes) {
+  const int per_row = (int)(ldg / 8);
+  const int64_t total = rows * per_row;
+  const float flat = smoothing / (float)V;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t i = total <= INT32_MAX ? (int64_t)((int)e / per_row) : e / per_row;
+    const int64_t n = (e - i * per_row) * 8, col = v0 + n;
+    float v[8];
+    const float l = lse[i], g = grow[i], scale = g * gscale;
+    if (FP32) {
+      load_vec<8>((const float*)kept + i * keep_ld + col, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = expf(v[k] - l);
+    } else {
+      const uint4 c = *reinterpret_cast<const uint4*>((const uint16_t*)kept + i * keep_ld + col);
+      const float f = expf(keep_max[(col >> 6) * rows + i] - l);
+      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[2 * k] = keep_value(w[k] & 0xffffu) * f;
+        v[2 * k + 1] = keep_value(w[k] >> 16) * f;
+      }
+    }
+    const int64_t tt = target[i], t = lce_scored(tt, V, ignore) ? tt - col : -1;
+    if (t >= 0 && t < 8) {
+      const float p = expf(ztarget[i] - l) - (1.f - smoothing);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k == t) v[k] = p;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = g == 0.f ? 0.f : (v[k] - flat) * scale;
+    for (int z = 0; z < planes; ++z) {
+      store_vec<8>(G + (z * rows + i) * ldg + n, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] -= to_f32(from_f32<T>(v[k]));
     }
   }
 }
@@ -678,32 +833,48 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x == 0) *factor = scale * inv_gscale;
 }
 
-// out [rows][cols] = factor * sum of S slabs [rows][ld]
+// out [rows][cols] = factor * sum of S slabs [rows][ld], four columns a thread
 template <typename T>
 __global__ void lce_join_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t cols, int64_t ld,
-                                const float* __restrict__ factor, T* __restrict__ out) {
+                                const float* __restrict__ factor, T* __restrict__ out, int vec) {
   const float f = *factor;
-  const int64_t total = rows * cols, size = rows * ld;
+  const int per_row = (int)(ld / 4);
+  const int64_t total = rows * per_row, size = rows * ld;
   for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t at = e / cols * ld + e % cols;
-    float v = slab[at];
-    for (int s = 1; s < S; ++s) v += slab[s * size + at];
-    out[e] = from_f32<T>(v * f);
+    const int64_t r = total <= INT32_MAX ? (int64_t)((int)e / per_row) : e / per_row;
+    const int64_t c = (e - r * per_row) * 4;
+    float v[4];
+    load_vec<4>(slab + r * ld + c, v);
+    for (int s = 1; s < S; ++s) {
+      float u[4];
+      load_vec<4>(slab + s * size + r * ld + c, u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] += u[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] *= f;
+    if (vec) {
+      store_vec<4>(out + r * cols + c, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < cols) out[r * cols + c + k] = from_f32<T>(v[k]);
+    }
   }
 }
 
-// column sums of G (planes added), 64 rows a thread row: partial sums first,
-// then in order
+// column sums of G (planes added): 32 columns and 32 rows at a time, partial
+// sums per part of the rows first, then in order
 template <typename T>
-__global__ void __launch_bounds__(256) lce_colsum_kernel(const T* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
+__global__ void __launch_bounds__(1024) lce_colsum_kernel(const T* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
                                                          int planes, int64_t rows_per, float* __restrict__ part) {
-  __shared__ float s[8][33];
+  __shared__ float s[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + c;
   const int64_t r0 = blockIdx.y * rows_per, r1 = min(rows, r0 + rows_per);
   float sum = 0.f;
   if (col < cols)
-    for (int64_t r = r0 + g; r < r1; r += 8) {
+    for (int64_t r = r0 + g; r < r1; r += 32) {
       float v = 0.f;
       for (int z = planes - 1; z >= 0; --z) v += to_f32(G[(z * rows + r) * ld + col]);
       sum += v;
@@ -711,7 +882,7 @@ __global__ void __launch_bounds__(256) lce_colsum_kernel(const T* __restrict__ G
   s[g][c] = sum;
   __syncthreads();
   if (g == 0 && col < cols) {
-    for (int q = 1; q < 8; ++q) sum += s[q][c];
+    for (int q = 1; q < 32; ++q) sum += s[q][c];
     part[blockIdx.y * cols + col] = sum;
   }
 }
@@ -826,9 +997,10 @@ static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   const int64_t width = std::min(p.piece, d->V);
   // the forward pass joins the slabs of a whole row
   p.z = lce_tiling(rows, width, d->D, p.P, width * d->D * 2, backward || p.pieces == 1);
-  p.dx = lce_tiling(d->N, d->D, width, p.P, 0);
+  // slabs of dx are laid down by the first piece, which has to be the widest
+  p.dx = lce_tiling(d->N, d->D, width, p.P, 0, d->kept == 0 || d->kept == d->V);
   p.dw = lce_tiling(width, d->D, d->N, p.P, 0);
-  p.colsum_parts = (int)std::min<int64_t>(64, cdiv(d->N, 256));
+  p.colsum_parts = (int)std::min<int64_t>(64, cdiv(d->N, 512));
   p.rows_per = p.colsum_parts ? up(cdiv(d->N, p.colsum_parts), 8) : 0;
   return p;
 }
@@ -845,6 +1017,27 @@ struct Arena {
   }
 };
 
+// What a forward pass keeps for the backward one, of the first d->kept
+// entries: logits in fp32 (fp32 operands, and logits that were formed in
+// slabs), else 16-bit codes of their exponentials with the maxima per 64
+// columns; and every row's target logit.
+struct LceKept {
+  bool fp32;
+  int64_t ld;
+  void* data;
+  float *max, *ztarget;
+};
+
+static size_t lce_kept_space(const pvb2_linear_ce_desc* d, bool fp32, const void* base, LceKept* k) {
+  Arena a{(uint8_t*)base};
+  k->fp32 = fp32;
+  k->ld = up(d->kept, 64);
+  k->data = a.take<uint8_t>(d->N * k->ld * (fp32 ? 4 : 2));
+  k->max = a.take<float>(fp32 ? 0 : k->ld / 64 * d->N);
+  k->ztarget = a.take<float>(d->N);
+  return a.at;
+}
+
 struct LceFwdSpace {
   uint16_t *x, *w;
   float* slab;
@@ -853,6 +1046,8 @@ struct LceFwdSpace {
 };
 
 static bool lce_slabs(const LcePlan& p) { return p.z.splits > 1; }
+
+static bool lce_kept_fp32(const pvb2_linear_ce_desc* d) { return d->dtype == PVB2_F32 || lce_slabs(lce_plan(d, false)); }
 
 static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceFwdSpace* s) {
   Arena a{(uint8_t*)base};
@@ -882,7 +1077,7 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
   s->factor = a.take<float>(1);
-  s->dx = a.take<float>(p.pieces > 1 || p.dx.splits > 1 ? p.dx.splits * d->N * ld32 : 0);
+  s->dx = a.take<float>(p.pieces > 1 || (d->kept > 0 && d->kept < d->V) || p.dx.splits > 1 ? p.dx.splits * d->N * ld32 : 0);
   s->dw = a.take<float>(p.dw.splits > 1 ? p.dw.splits * width * ld32 : 0);
   s->colsum = a.take<float>(p.colsum_parts * width);
   return a.at;
@@ -901,6 +1096,8 @@ static int lce_check(const pvb2_linear_ce_desc* d) {
                  (long long)d->V);
   PVB2_CHECK_ARG((d->N <= 1 || d->ldx >= d->D) && (d->V <= 1 || d->ldw >= d->D),
                  "linear cross entropy: row strides below the row length");
+  PVB2_CHECK_ARG(d->kept >= 0 && d->kept <= d->V && (d->kept == d->V || d->kept % 256 == 0),
+                 "linear cross entropy: all entries or a multiple of 256 are kept (got %lld)", (long long)d->kept);
   PVB2_CHECK_ARG(d->label_smoothing >= 0.0 && d->label_smoothing <= 1.0,
                  "linear cross entropy: label smoothing in [0, 1] expected");
   return PVB2_OK;
@@ -973,32 +1170,34 @@ static int lce_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMa
   return lce_launch<EPI, __nv_bfloat16, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
 }
 
-static int lce_pack(const pvb2_linear_ce_desc* d, const LcePlan& p, const void* src, int64_t row0, int64_t rows,
-                    int64_t ld, uint16_t* dst, const int64_t* target, cudaStream_t s) {
-  const int64_t total = rows * p.ldp;
+template <typename S, typename T>
+static int lce_pack_as(const pvb2_linear_ce_desc* d, const LcePlan& p, const S* src, int64_t rows, int64_t ld,
+                       uint16_t* dst, const int64_t* target, cudaStream_t s) {
+  const int64_t total = rows * (p.ldp / 8);
   if (total == 0) return PVB2_OK;
-  const int grid = grid_for(total, 256);
-  if (d->dtype == PVB2_F32)
-    lce_pack_kernel<<<grid, 256, 0, s>>>((const float*)src + row0 * ld, rows, d->D, ld, (__nv_bfloat16*)dst, p.ldp, p.P,
-                                         target, d->V, d->ignore_index);
-  else if (p.half)
-    lce_pack_kernel<<<grid, 256, 0, s>>>((const __half*)src + row0 * ld, rows, d->D, ld, (__half*)dst, p.ldp, 1, target,
-                                         d->V, d->ignore_index);
-  else
-    lce_pack_kernel<<<grid, 256, 0, s>>>((const __nv_bfloat16*)src + row0 * ld, rows, d->D, ld, (__nv_bfloat16*)dst,
-                                         p.ldp, 1, target, d->V, d->ignore_index);
+  const int vec = ((uintptr_t)src & 15) == 0 && ld * sizeof(S) % 16 == 0;
+  lce_pack_kernel<S, T><<<grid_for(total, 256), 256, 0, s>>>(src, rows, d->D, ld, (T*)dst, p.ldp, p.P, target, d->V,
+                                                             d->ignore_index, vec);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
+}
+
+static int lce_pack(const pvb2_linear_ce_desc* d, const LcePlan& p, const void* src, int64_t row0, int64_t rows,
+                    int64_t ld, uint16_t* dst, const int64_t* target, cudaStream_t s) {
+  if (d->dtype == PVB2_F32)
+    return lce_pack_as<float, __nv_bfloat16>(d, p, (const float*)src + row0 * ld, rows, ld, dst, target, s);
+  if (p.half) return lce_pack_as<__half, __half>(d, p, (const __half*)src + row0 * ld, rows, ld, dst, target, s);
+  return lce_pack_as<__nv_bfloat16, __nv_bfloat16>(d, p, (const __nv_bfloat16*)src + row0 * ld, rows, ld, dst, target, s);
 }
 
 // out = factor * (sum of slabs), as the operands' type
 static int lce_join(const pvb2_linear_ce_desc* d, const float* slab, int S, int64_t rows, const float* factor, void* out,
                     cudaStream_t s) {
-  const int64_t ld = up(d->D, 4), total = rows * d->D;
-  const int grid = grid_for(total, 256);
-  if (d->dtype == PVB2_F32) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (float*)out);
-  else if (d->dtype == PVB2_F16) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (__half*)out);
-  else lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (__nv_bfloat16*)out);
+  const int64_t ld = up(d->D, 4);
+  const int grid = grid_for(rows * (ld / 4), 256), vec = d->D % 4 == 0 && ((uintptr_t)out & 15) == 0;
+  if (d->dtype == PVB2_F32) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (float*)out, vec);
+  else if (d->dtype == PVB2_F16) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (__half*)out, vec);
+  else lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (__nv_bfloat16*)out, vec);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -1071,11 +1270,40 @@ static int lce_slab_logits(const pvb2_linear_ce_desc* d, const LcePlan& p, const
 }
 
 template <typename T>
+static int lce_kept_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, const LceKept& k,
+                         const int64_t* target, const float* lse, int64_t v0, int64_t width, int64_t ldg, float gscale,
+                         cudaStream_t s) {
+  const int grid = grid_for(d->N * (ldg / 8), 256);
+  const float smoothing = (float)d->label_smoothing;
+  if (k.fp32)
+    lce_kept_grad_kernel<T, true><<<grid, 256, 0, s>>>(k.data, k.ld, k.max, k.ztarget, d->N, target, v0, width, d->V,
+                                                       d->ignore_index, smoothing, lse, sp.row, gscale, (T*)sp.G, ldg,
+                                                       p.P);
+  else
+    lce_kept_grad_kernel<T, false><<<grid, 256, 0, s>>>(k.data, k.ld, k.max, k.ztarget, d->N, target, v0, width, d->V,
+                                                        d->ignore_index, smoothing, lse, sp.row, gscale, (T*)sp.G, ldg,
+                                                        p.P);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+template <typename T>
+static int lce_slab_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, const void* bias,
+                         const int64_t* target, const float* lse, int64_t v0, int64_t width, int64_t ldg, float gscale,
+                         cudaStream_t s) {
+  lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target, v0,
+                                                 width, d->V, d->ignore_index, (float)d->label_smoothing, lse, sp.row,
+                                                 gscale, (T*)sp.G, ldg, p.P);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+template <typename T>
 static int lce_bias_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, int64_t width,
                          int64_t ldg, void* out, cudaStream_t s) {
   const dim3 grid((unsigned)cdiv(width, 32), (unsigned)p.colsum_parts);
   const int blocks = (int)cdiv(width, 256);
-  lce_colsum_kernel<<<grid, 256, 0, s>>>((const T*)sp.G, d->N, width, ldg, p.P, p.rows_per, sp.colsum);
+  lce_colsum_kernel<<<grid, 1024, 0, s>>>((const T*)sp.G, d->N, width, ldg, p.P, p.rows_per, sp.colsum);
   PVB2_LAUNCH_CHECK();
   if (d->dtype == PVB2_F32)
     lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (float*)out);
@@ -1099,7 +1327,7 @@ size_t pvb2_linear_ce_fwd_workspace_size(const pvb2_linear_ce_desc* desc) {
 }
 
 int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const void* w, const void* bias,
-                       const int64_t* target, float* out, float* lse, float* count, void* workspace,
+                       const int64_t* target, float* out, float* lse, float* count, void* kept, void* workspace,
                        size_t workspace_bytes, pvb2_stream stream) {
   PVB2_TRY(lce_check(desc));
   const pvb2_linear_ce_desc normal = lce_normal(desc), *d = &normal;
@@ -1117,6 +1345,10 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     PVB2_TRY(lce_aligned(w, !p.pack_w));
     const int parts = (int)cdiv(d->V, p.z.bn / 2), esize = d->dtype == PVB2_F32 ? 4 : 2;
     const float smoothing = (float)d->label_smoothing;
+    PVB2_CHECK_ARG(d->kept == 0 || (kept && ((uintptr_t)kept & 15) == 0),
+                   "linear cross entropy: 16-byte aligned memory for what is kept needed");
+    LceKept k;
+    lce_kept_space(d, d->dtype == PVB2_F32 || slabs, kept, &k);
     for (int64_t r0 = 0; r0 < d->N; r0 += kLRowsFwd) {
       const int64_t rows = std::min(kLRowsFwd, d->N - r0);
       CUtensorMap ma, mb;
@@ -1140,25 +1372,49 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
         } else {
           g.part = sp.part;
           g.zsum = smoothing != 0.f ? sp.zsum : nullptr;
-          g.ztarget = sp.ztarget;
+          g.ztarget = d->kept ? k.ztarget + r0 : sp.ztarget;
           g.part_ld = rows;
-          PVB2_TRY(lce_gemm<kEpiStats>(ma, mb, no_map(), g, false, false, p, p.z.bn, s));
+          CUtensorMap mk = no_map();
+          if (d->kept) {
+            g.keep = (int)d->kept;
+            g.keep_max = k.max + r0;
+            g.keep_ld = d->N;
+            if (k.fp32) PVB2_TRY(lce_map32(&mk, (float*)k.data + r0 * k.ld, d->kept, rows, k.ld, 1));
+            else PVB2_TRY(lce_map(&mk, (uint16_t*)k.data + r0 * k.ld, d->kept, rows, k.ld, 1, 32, true));
+          }
+          PVB2_TRY(lce_gemm<kEpiStats>(ma, mb, mk, g, false, false, p, p.z.bn, s));
         }
       }
       if (slabs)
-        lce_slab_rows_kernel<<<(int)rows, 256, 0, s>>>(sp.slab, p.z.splits, rows, up(d->V, 4), bias, d->dtype,
-                                                       target + r0, d->V, d->ignore_index, smoothing, lse + r0,
-                                                       loss + r0);
+        lce_slab_rows_kernel<<<(int)rows, 512, 0, s>>>(
+            sp.slab, p.z.splits, rows, up(d->V, 4), bias, d->dtype, target + r0, d->V, d->ignore_index, smoothing,
+            lse + r0, loss + r0, (float*)k.data + r0 * k.ld, d->kept, k.ld, d->kept ? k.ztarget + r0 : nullptr);
       else
-        lce_rows_kernel<<<(int)cdiv(rows, 32), 256, 0, s>>>(sp.part, smoothing != 0.f ? sp.zsum : nullptr, rows, parts,
-                                                            sp.ztarget, target + r0, rows, d->V, d->ignore_index,
-                                                            smoothing, lse + r0, loss + r0);
+        lce_rows_kernel<<<(int)cdiv(rows, 32), 1024, 0, s>>>(
+            sp.part, smoothing != 0.f ? sp.zsum : nullptr, rows, parts, d->kept ? k.ztarget + r0 : sp.ztarget,
+            target + r0, rows, d->V, d->ignore_index, smoothing, lse + r0, loss + r0);
       PVB2_LAUNCH_CHECK();
     }
   }
   lce_total_kernel<<<1, 1024, 0, s>>>(loss, target, d->N, d->V, d->ignore_index, d->reduction, out, count);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
+}
+
+size_t pvb2_linear_ce_keep(pvb2_linear_ce_desc* desc, size_t budget) {
+  if (!desc) return 0;
+  desc->kept = 0;
+  if (lce_check(desc) != PVB2_OK || desc->N == 0) return 0;
+  const pvb2_linear_ce_desc normal = lce_normal(desc);
+  const bool fp32 = lce_kept_fp32(&normal);
+  // an entry takes its number for each row, and its share of the maxima
+  const double entry = (double)desc->N * (fp32 ? 4 : 2 + 4.0 / 64);
+  const int64_t fit = (int64_t)std::min<double>((double)desc->V, (double)budget / entry);
+  desc->kept = fit >= desc->V ? desc->V : fit / 256 * 256;
+  if (desc->kept < std::min<int64_t>(desc->V, 1024)) desc->kept = 0;
+  if (desc->kept == 0) return 0;
+  LceKept k;
+  return lce_kept_space(desc, fp32, nullptr, &k);
 }
 
 size_t pvb2_linear_ce_bwd_workspace_size(const pvb2_linear_ce_desc* desc) {
@@ -1169,8 +1425,8 @@ size_t pvb2_linear_ce_bwd_workspace_size(const pvb2_linear_ce_desc* desc) {
 }
 
 int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const void* w, const void* bias,
-                       const int64_t* target, const float* lse, const float* count, const float* grad_out, void* dx,
-                       void* dw, void* dbias, void* workspace, size_t workspace_bytes, pvb2_stream stream) {
+                       const int64_t* target, const float* lse, const float* count, const void* kept,
+                       const float* grad_out, void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes, pvb2_stream stream) {
   PVB2_TRY(lce_check(desc));
   const pvb2_linear_ce_desc normal = lce_normal(desc), *d = &normal;
   cudaStream_t s = as_stream(stream);
@@ -1197,48 +1453,54 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;
   PVB2_TRY(lce_map_a(&x_k, sp.x, d->D, d->N, p.ldp, p));
   PVB2_TRY(lce_map_mn(&x_mn, sp.x, d->D, d->N, p.ldp, p));
-  const bool dx_slabs = p.pieces > 1 || p.dx.splits > 1;
+  PVB2_CHECK_ARG(d->kept == 0 || (kept && ((uintptr_t)kept & 15) == 0),
+                 "linear cross entropy backward: what the forward pass kept is missing");
+  LceKept k;
+  if (d->kept) lce_kept_space(d, lce_kept_fp32(d), kept, &k);
   const int64_t ld32 = up(d->D, 4);
-  for (int q = 0; q < p.pieces; ++q) {
-    const int64_t v0 = q * p.piece, width = std::min(p.piece, d->V - v0), ldg = up(width, 8);
+  // a piece ends where the kept entries do
+  const bool dx_slabs = p.piece < d->V || (d->kept > 0 && d->kept < d->V) || p.dx.splits > 1;
+  for (int64_t v0 = 0, end; v0 < d->V; v0 = end) {
+    end = std::min(d->V, v0 + p.piece);
+    if (v0 < d->kept && end > d->kept) end = d->kept;
+    const int64_t width = end - v0, ldg = up(width, 8);
+    const bool from_kept = v0 < d->kept;
     const int row0 = direct_w ? (int)v0 : 0;
     if (direct_w) {
       PVB2_TRY(lce_map_b(&w_k, w, d->D, d->V, d->ldw, p, p.z.bn));
       PVB2_TRY(lce_map_mn(&w_mn, w, d->D, d->V, d->ldw, p));
-    } else {
+    } else if (dx || !from_kept) {
       PVB2_TRY(lce_pack(d, p, w, v0, width, d->ldw, sp.w, nullptr, s));
       PVB2_TRY(lce_map_b(&w_k, sp.w, d->D, width, p.ldp, p, p.z.bn));
       PVB2_TRY(lce_map_mn(&w_mn, sp.w, d->D, width, p.ldp, p));
     }
-    PVB2_TRY(lce_map(&g_store, sp.G, width, d->N, ldg, p.P, 32, p.half));
     PVB2_TRY(lce_map_a(&g_k, sp.G, width, d->N, ldg, p));
     PVB2_TRY(lce_map_mn(&g_mn, sp.G, width, d->N, ldg, p));
     // G of this piece
-    LceGemm g = lce_logits(d, bias, d->N, v0, width, row0, target);
-    if (slabs) {
-      PVB2_TRY(lce_slab_logits(d, p, x_k, w_k, g, sp.slab, s));
-      if (p.half)
-        lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target,
-                                                       v0, width, d->V, d->ignore_index, (float)d->label_smoothing, lse,
-                                                       sp.row, gscale, (__half*)sp.G, ldg, p.P);
-      else
-        lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target,
-                                                       v0, width, d->V, d->ignore_index, (float)d->label_smoothing, lse,
-                                                       sp.row, gscale, (__nv_bfloat16*)sp.G, ldg, p.P);
-      PVB2_LAUNCH_CHECK();
+    if (from_kept) {
+      if (p.half) PVB2_TRY(lce_kept_grad<__half>(d, p, sp, k, target, lse, v0, width, ldg, gscale, s));
+      else PVB2_TRY(lce_kept_grad<__nv_bfloat16>(d, p, sp, k, target, lse, v0, width, ldg, gscale, s));
     } else {
-      g.lse = lse;
-      g.grow = sp.row;
-      g.planes = p.P;
-      g.gscale = gscale;
-      PVB2_TRY(lce_gemm<kEpiGrad>(x_k, w_k, g_store, g, false, false, p, p.z.bn, s));
+      LceGemm g = lce_logits(d, bias, d->N, v0, width, row0, target);
+      if (slabs) {
+        PVB2_TRY(lce_slab_logits(d, p, x_k, w_k, g, sp.slab, s));
+        if (p.half) PVB2_TRY(lce_slab_grad<__half>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, s));
+        else PVB2_TRY(lce_slab_grad<__nv_bfloat16>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, s));
+      } else {
+        g.lse = lse;
+        g.grow = sp.row;
+        g.planes = p.P;
+        g.gscale = gscale;
+        PVB2_TRY(lce_map(&g_store, sp.G, width, d->N, ldg, p.P, 32, p.half));
+        PVB2_TRY(lce_gemm<kEpiGrad>(x_k, w_k, g_store, g, false, false, p, p.z.bn, s));
+      }
     }
     if (dx) {
       LceGemm h = lce_product(d->N, d->D, width, row0, p.dx);
       if (dx_slabs) {
-        // a last piece that is shorter leaves the far slabs alone
+        // the first piece is the widest; a shorter one leaves the far slabs alone
         if (p.dx.splits > 1) h.splits = (int)std::min<int64_t>(h.splits, cdiv(cdiv(width, kLBK), h.kb_per));
-        h.accumulate = q > 0;
+        h.accumulate = v0 > 0;
         PVB2_TRY(lce_map32(&acc, sp.dx, d->D, d->N, ld32, p.dx.splits));
         PVB2_TRY(lce_gemm<kEpiAcc>(g_k, w_mn, acc, h, false, true, p, p.dx.bn, s));
       } else {

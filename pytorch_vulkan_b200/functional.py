@@ -16,10 +16,12 @@ def linear_cross_entropy(input, weight, target, bias=None, *, ignore_index=-100,
     number of classes, from a classifier's to a language model's vocabulary.
     The loss is fp32 whatever the operands' type: one number, or one per row
     with ``reduction="none"``.  Gradients of ``input``, ``weight`` and ``bias``
-    have the operands' type, rounded once from fp32 sums.  The logits are
-    formed on the chip, by the forward pass and again, piece by piece of the
-    classes, by the backward pass; memory grows with neither the number of
-    classes nor that of rows alone, but by a bounded piece.
+    have the operands' type, rounded once from fp32 sums.  The logits stay on
+    the chip.  A backward pass needs their softmax: of as many classes as fit
+    into ``B200_CE_KEEP_MB`` (2048 MB by default; 0 keeps nothing) the forward
+    pass keeps it, as 16-bit exponentials (fp32 logits for fp32 operands), until
+    the backward pass is done; of the others the backward pass forms the logits
+    again, piece by piece.
 
     Rows whose target is ``ignore_index`` or out of range have no loss and no
     gradient, whatever they hold.  fp32 operands are multiplied to fp32

@@ -7,7 +7,9 @@ round), plus the part of the operands that is left out (2^-23 |x||w| for fp32
 operands in exact mode, 2^-14 in the default one, nothing for 16-bit ones).
 The log of the sum of exponentials errs by at most the largest such error and
 2^-20 of its own; a loss by twice that.  A probability p errs by p (2 e_z +
-2^-19); G is held in 16 bits (2^-9 for bf16, 2^-12 for fp16, 2^-23 as parts of
+2^-19), and, where the forward pass kept it for 16-bit operands (a number with
+12 bits of mantissa and 4 of exponent relative to the largest of 64 columns), by
+half a step more: 2^-13 p, or 2^-27 of that largest (at most 1).  G is held in 16 bits (2^-9 for bf16, 2^-12 for fp16, 2^-23 as parts of
 fp32), and the gradients are sums of products of G, so that each is within
 |G| |w| (or |G|^T |x|) times those errors, the accumulation's, and one rounding
 to its type.
@@ -93,6 +95,8 @@ def check(ocl, x, w, b, t, mode=1, reduction="mean", smooth=0.0, ignore=-100, gr
         G = ((p - goal) * gi[:, None]).abs()
         eg = p * gi.abs()[:, None] * (err[:, None] + 2.0 ** -19) + G * {FP32: left_out, BF16: 2.0 ** -8, FP16: 2.0 ** -11}[dtype]
         eg = eg + 2.0 ** -22 * (p + goal) * gi.abs()[:, None]
+        if dtype != FP32:
+            eg = eg + (2.0 ** -13 * p + 2.0 ** -27) * gi.abs()[:, None]
         if dtype == FP16:  # what is below fp16's steps, scaled by 2^15
             eg = eg + (2.0 ** -25 / 2 ** 15) * gi.abs().max()
         bounds = [eg @ wa + ((V + 8) * 2.0 ** -23 + left_out) * (G @ wa),
@@ -325,9 +329,10 @@ def test_on_another_stream(ocl):
     assert all(torch.equal(a, b.cpu()) for a, b in zip(want, got))
 
 
-def test_memory_stays_bounded(ocl):
-    """No logits: a step takes far less than N x V numbers beyond its operands and gradients."""
+def test_memory_stays_bounded(ocl, monkeypatch):
+    """No logits: a step that keeps nothing takes far less than N x V numbers beyond its operands and gradients."""
     N, D, V = 4096, 64, 131072
+    monkeypatch.setenv("B200_CE_KEEP_MB", "0")
     x, w = torch.zeros(N, D, dtype=BF16).to(DEV).requires_grad_(), torch.zeros(V, D, dtype=BF16).to(DEV).requires_grad_()
     t = torch.zeros(N, dtype=torch.int64).to(DEV)
     torch.ocl.synchronize()
@@ -335,6 +340,40 @@ def test_memory_stays_bounded(ocl):
     before = torch.ocl.memory_allocated()
     torch.autograd.grad(ocl.functional.linear_cross_entropy(x, w, t), [x, w])
     assert torch.ocl.max_memory_allocated() - before < N * V * 2 // 4
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("keep", ["0", "5", "2048"])
+def test_kept_softmax(ocl, monkeypatch, math_fp32, dtype, keep):
+    """Nothing, some, and all of the softmax kept for the backward pass; and a second backward pass of the same graph."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    check(ocl, *make(700, 40, 9001, dtype, bias=True, ignored=0.1), smooth=0.1)
+    check(ocl, *make(30, 520, 900, dtype, bias=True, ignored=0.1), reduction="none")
+    check(ocl, *make(17000, 16, 1100, dtype))
+    x, w, b, t = make(500, 64, 5000, dtype)
+    leaves = [v.to(DEV).requires_grad_() for v in (x, w)]
+    loss = ocl.functional.linear_cross_entropy(*leaves, t.to(DEV))
+    one = torch.autograd.grad(loss, leaves, retain_graph=True)
+    two = torch.autograd.grad(loss, leaves)
+    assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(one, two))
+
+
+def test_what_is_kept_stays_in_its_budget(ocl, monkeypatch):
+    N, D, V = 4096, 64, 65536
+    monkeypatch.setenv("B200_CE_KEEP_MB", "100")
+    x, w = torch.zeros(N, D, dtype=BF16).to(DEV).requires_grad_(), torch.zeros(V, D, dtype=BF16).to(DEV)
+    t = torch.zeros(N, dtype=torch.int64).to(DEV)
+    torch.ocl.synchronize()
+    before = torch.ocl.memory_allocated()
+    loss = ocl.functional.linear_cross_entropy(x, w, t)
+    held = torch.ocl.memory_allocated() - before
+    # the budget, the allocator's size class above it (a quarter), and what belongs to each row
+    assert 50 << 20 < held <= 1.25 * (100 << 20) + (1 << 20)
+    with torch.no_grad():
+        before = torch.ocl.memory_allocated()
+        kept_nothing = ocl.functional.linear_cross_entropy(x, w, t)
+        assert torch.ocl.memory_allocated() - before < 1 << 20
+    assert torch.equal(loss.detach().cpu(), kept_nothing.cpu())
 
 
 def test_no_wait_ran_out(ocl):
