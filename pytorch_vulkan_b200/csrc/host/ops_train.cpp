@@ -129,102 +129,151 @@ static void fused_adam_tensor_lr_(at::TensorList self, at::TensorList grads, at:
              beta2, weight_decay, eps, amsgrad, maximize, grad_scale, found_inf);
 }
 
-// one step of pytorch_vulkan_b200.optim.AdamW for parameters of one type on
-// one device: counts the steps, then updates.  With scales, moments are 8-bit
-// codes (flat, in the parameters' memory order).
-static void adamw_step(const std::vector<at::Tensor>& params, const std::vector<at::Tensor>& grads,
-                       const std::vector<at::Tensor>& exp_avgs, const std::vector<at::Tensor>& exp_avg_sqs,
-                       const std::vector<at::Tensor>& exp_avg_scales, const std::vector<at::Tensor>& exp_avg_sq_scales,
-                       const std::vector<at::Tensor>& steps, double lr, double beta1, double beta2, double eps,
-                       double weight_decay, bool maximize) {
-  const size_t n = params.size();
-  if (n == 0) return;
-  const bool codes = !exp_avg_scales.empty();
-  TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && steps.size() == n &&
-                  exp_avg_scales.size() == (codes ? n : 0) && exp_avg_sq_scales.size() == (codes ? n : 0),
-              "ocl AdamW: lists of one length expected");
-  const int dev = params[0].device().index();
-  const c10::ScalarType type = params[0].scalar_type();
-  DeviceScope scope(dev);
-  OCL_OP("adamw_step", dev);
-  std::vector<pvb2_adamw_tensor> ts(n);
-  std::vector<at::Tensor> copies;  // gradients laid out unlike their parameters
-  for (size_t i = 0; i < n; ++i) {
-    const at::Tensor& p = params[i];
-    check_param(p, grads[i], dev, type, i);
-    const at::Tensor g = grad_like(grads[i], p);
-    if (!g.is_same(grads[i])) copies.push_back(g);
-    pvb2_adamw_tensor& t = ts[i];
-    memset(&t, 0, sizeof(t));
-    auto held = [&](const at::Tensor& x, c10::ScalarType want, int64_t numel, bool flat, const char* what) {
-      TORCH_CHECK(is_ocl(x) && x.device().index() == dev && x.scalar_type() == want && x.numel() == numel &&
-                      (flat ? x.is_contiguous() : same_layout(x, p)),
-                  "ocl AdamW: ", what, " ", i, " of the state does not fit its parameter");
-      return x.data_ptr();
-    };
-    t.numel = p.numel();
-    t.param = p.data_ptr();
-    t.grad = g.data_ptr();
-    const c10::ScalarType kind = codes ? at::kByte : at::kFloat;
-    t.exp_avg = held(exp_avgs[i], kind, t.numel, codes, "first moment");
-    t.exp_avg_sq = held(exp_avg_sqs[i], kind, t.numel, codes, "second moment");
-    if (codes) {
-      const int64_t blocks = (t.numel + 255) / 256;
-      t.exp_avg_scale = (float*)held(exp_avg_scales[i], at::kFloat, blocks, true, "scale of the first moment");
-      t.exp_avg_sq_scale = (float*)held(exp_avg_sq_scales[i], at::kFloat, blocks, true, "scale of the second moment");
-    }
-    t.step = step_ptr(steps[i], dev, i);
-  }
-  pvb2_adamw_desc d;
-  memset(&d, 0, sizeof(d));
-  d.param_dtype = dtype_code(type);
-  d.state_dtype = codes ? PVB2_U8 : PVB2_F32;
-  d.decoupled = 1;
-  d.maximize = maximize ? 1 : 0;
-  d.increment_step = 1;
-  d.lr = lr;
-  d.beta1 = beta1;
-  d.beta2 = beta2;
-  d.eps = eps;
-  d.weight_decay = weight_decay;
-  Workspace ws(pvb2_adamw_workspace_size((int)n), dev);
-  OCL_CHECK(pvb2_adamw_multi(&d, (int)n, ts.data(), ws.get(), ws.bytes, stream_for(dev)));
-  for (const at::Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();
+// The optimizer's Python objects, read here since a loop in Python over the
+// parameters costs more than the launch: tensors, and the dict of a
+// parameter's state.
+static const at::Tensor& py_tensor(PyObject* o, const char* what) {
+  TORCH_CHECK(o && THPVariable_Check(o), "ocl AdamW: ", what, " is not a tensor");
+  return THPVariable_Unpack(o);
 }
 
-// the moments that 8-bit codes stand for, into fp32 tensors
-static void adamw8_values(const std::vector<at::Tensor>& codes, const std::vector<at::Tensor>& scales,
-                          const std::vector<at::Tensor>& rms_codes, const std::vector<at::Tensor>& rms_scales,
-                          const std::vector<at::Tensor>& exp_avgs, const std::vector<at::Tensor>& exp_avg_sqs) {
-  const size_t n = codes.size();
-  if (n == 0) return;
-  TORCH_CHECK(scales.size() == n && rms_codes.size() == n && rms_scales.size() == n && exp_avgs.size() == n &&
-                  exp_avg_sqs.size() == n,
-              "ocl AdamW: lists of one length expected");
-  const int dev = codes[0].device().index();
-  DeviceScope scope(dev);
-  OCL_OP("adamw8_values", dev);
-  std::vector<pvb2_adamw_tensor> ts(n);
-  for (size_t i = 0; i < n; ++i) {
-    pvb2_adamw_tensor& t = ts[i];
-    memset(&t, 0, sizeof(t));
-    t.numel = codes[i].numel();
-    auto ptr = [&](const at::Tensor& x, c10::ScalarType want, int64_t numel, bool dense) {
-      TORCH_CHECK(is_ocl(x) && x.device().index() == dev && x.scalar_type() == want && x.numel() == numel &&
-                      (dense ? x.is_non_overlapping_and_dense() : x.is_contiguous()),
-                  "ocl AdamW: state or output ", i, " does not fit");
-      return x.data_ptr();
-    };
-    const int64_t blocks = (t.numel + 255) / 256;
-    t.exp_avg = ptr(codes[i], at::kByte, t.numel, false);
-    t.exp_avg_sq = ptr(rms_codes[i], at::kByte, t.numel, false);
-    t.exp_avg_scale = (float*)ptr(scales[i], at::kFloat, blocks, false);
-    t.exp_avg_sq_scale = (float*)ptr(rms_scales[i], at::kFloat, blocks, false);
-    t.param = ptr(exp_avgs[i], at::kFloat, t.numel, true);
-    t.grad = ptr(exp_avg_sqs[i], at::kFloat, t.numel, true);
+struct AdamState {  // of one parameter
+  PyObject* dict;
+  const at::Tensor& get(const char* key) const { return py_tensor(PyDict_GetItemString(dict, key), key); }
+};
+
+// undefined state: an empty or a missing dict
+static bool adam_state(const pybind11::dict& state, PyObject* p, AdamState* s) {
+  s->dict = PyDict_GetItemWithError(state.ptr(), p);
+  if (!s->dict && PyErr_Occurred()) throw pybind11::error_already_set();
+  if (s->dict) TORCH_CHECK(PyDict_Check(s->dict), "ocl AdamW: a parameter's state is not a dict");
+  return s->dict && PyDict_Size(s->dict) > 0;
+}
+
+static void* adam_held(const at::Tensor& x, const at::Tensor& p, c10::ScalarType want, int64_t numel, bool flat,
+                       const char* what) {
+  TORCH_CHECK(is_ocl(x) && x.device() == p.device() && x.scalar_type() == want && x.numel() == numel &&
+                  (flat ? x.is_contiguous() : same_layout(x, p)),
+              "ocl AdamW: ", what, " of the state does not fit its parameter");
+  return x.data_ptr();
+}
+
+// the pointers of a parameter's 8-bit moments
+static void adam_codes(const AdamState& s, const at::Tensor& p, pvb2_adamw_tensor& t) {
+  const int64_t n = p.numel(), blocks = (n + 255) / 256;
+  t.exp_avg = adam_held(s.get("exp_avg_code"), p, at::kByte, n, true, "exp_avg_code");
+  t.exp_avg_sq = adam_held(s.get("exp_avg_rms_code"), p, at::kByte, n, true, "exp_avg_rms_code");
+  t.exp_avg_scale = (float*)adam_held(s.get("exp_avg_scale"), p, at::kFloat, blocks, true, "exp_avg_scale");
+  t.exp_avg_sq_scale = (float*)adam_held(s.get("exp_avg_rms_scale"), p, at::kFloat, blocks, true, "exp_avg_rms_scale");
+}
+
+// One step of pytorch_vulkan_b200.optim.AdamW over the parameters of a group
+// that have a gradient: counts the steps, then updates, one call for each
+// device and type among them.  Parameters that have no state yet are returned
+// and nothing is done.
+static pybind11::list adamw_step(const pybind11::list& params, const pybind11::dict& state, int64_t bits, double lr,
+                                 double beta1, double beta2, double eps, double weight_decay, bool maximize) {
+  const bool codes = bits == 8;
+  pybind11::list missing;
+  std::vector<at::Tensor> ps, gs;
+  std::vector<AdamState> states;
+  for (const pybind11::handle h : params) {
+    const at::Tensor& p = py_tensor(h.ptr(), "a parameter");
+    const at::Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    TORCH_CHECK(!g.is_sparse(), "ocl AdamW: sparse gradients are not supported");
+    AdamState s;
+    if (!adam_state(state, h.ptr(), &s)) missing.append(h);
+    ps.push_back(p);
+    gs.push_back(g);
+    states.push_back(s);
   }
-  OCL_CHECK(pvb2_adamw8_values((int)n, ts.data(), stream_for(dev)));
-  for (size_t i = 0; i < n; ++i) {
+  if (missing.size() || ps.empty()) return missing;
+  std::vector<char> done(ps.size(), 0);
+  for (size_t first = 0; first < ps.size(); ++first) {
+    if (done[first]) continue;
+    TORCH_CHECK(is_ocl(ps[first]), "ocl AdamW: parameter ", first, " is on ", ps[first].device());
+    const int dev = ps[first].device().index();
+    const c10::ScalarType type = ps[first].scalar_type();
+    DeviceScope scope(dev);
+    OCL_OP("adamw_step", dev);
+    std::vector<pvb2_adamw_tensor> ts;
+    std::vector<at::Tensor> copies;  // gradients laid out unlike their parameters
+    for (size_t i = first; i < ps.size(); ++i) {
+      const at::Tensor& p = ps[i];
+      if (done[i] || p.device() != ps[first].device() || p.scalar_type() != type) continue;
+      done[i] = 1;
+      check_param(p, gs[i], dev, type, i);
+      const at::Tensor g = grad_like(gs[i], p);
+      if (!g.is_same(gs[i])) copies.push_back(g);
+      pvb2_adamw_tensor t;
+      memset(&t, 0, sizeof(t));
+      t.numel = p.numel();
+      t.param = p.data_ptr();
+      t.grad = g.data_ptr();
+      if (codes) {
+        adam_codes(states[i], p, t);
+      } else {
+        t.exp_avg = adam_held(states[i].get("exp_avg"), p, at::kFloat, t.numel, false, "exp_avg");
+        t.exp_avg_sq = adam_held(states[i].get("exp_avg_sq"), p, at::kFloat, t.numel, false, "exp_avg_sq");
+      }
+      t.step = step_ptr(states[i].get("step"), dev, i);
+      ts.push_back(t);
+    }
+    pvb2_adamw_desc d;
+    memset(&d, 0, sizeof(d));
+    d.param_dtype = dtype_code(type);
+    d.state_dtype = codes ? PVB2_U8 : PVB2_F32;
+    d.decoupled = 1;
+    d.maximize = maximize ? 1 : 0;
+    d.increment_step = 1;
+    d.lr = lr;
+    d.beta1 = beta1;
+    d.beta2 = beta2;
+    d.eps = eps;
+    d.weight_decay = weight_decay;
+    Workspace ws(pvb2_adamw_workspace_size((int)ts.size()), dev);
+    OCL_CHECK(pvb2_adamw_multi(&d, (int)ts.size(), ts.data(), ws.get(), ws.bytes, stream_for(dev)));
+  }
+  for (const at::Tensor& p : ps) p.unsafeGetTensorImpl()->bump_version();
+  return missing;
+}
+
+// the moments that the 8-bit states of `params` (those that have one) stand
+// for, into fp32 tensors laid out like them
+static void adamw8_values(const pybind11::list& params, const pybind11::dict& state,
+                          const std::vector<at::Tensor>& exp_avgs, const std::vector<at::Tensor>& exp_avg_sqs) {
+  std::vector<at::Tensor> ps;
+  std::vector<AdamState> states;
+  for (const pybind11::handle h : params) {
+    AdamState s;
+    if (!adam_state(state, h.ptr(), &s)) continue;
+    ps.push_back(py_tensor(h.ptr(), "a parameter"));
+    states.push_back(s);
+  }
+  TORCH_CHECK_VALUE(exp_avgs.size() == ps.size() && exp_avg_sqs.size() == ps.size(), ps.size(),
+                    " parameters have a state, got ", exp_avgs.size(), " and ", exp_avg_sqs.size(), " tensors");
+  std::vector<char> done(ps.size(), 0);
+  for (size_t first = 0; first < ps.size(); ++first) {
+    if (done[first]) continue;
+    const int dev = ps[first].device().index();
+    DeviceScope scope(dev);
+    OCL_OP("adamw8_values", dev);
+    std::vector<pvb2_adamw_tensor> ts;
+    for (size_t i = first; i < ps.size(); ++i) {
+      if (done[i] || ps[i].device() != ps[first].device()) continue;
+      done[i] = 1;
+      pvb2_adamw_tensor t;
+      memset(&t, 0, sizeof(t));
+      t.numel = ps[i].numel();
+      adam_codes(states[i], ps[i], t);
+      t.param = adam_held(exp_avgs[i], ps[i], at::kFloat, t.numel, false, "the tensor for a first moment");
+      t.grad = adam_held(exp_avg_sqs[i], ps[i], at::kFloat, t.numel, false, "the tensor for a second moment");
+      ts.push_back(t);
+    }
+    OCL_CHECK(pvb2_adamw8_values((int)ts.size(), ts.data(), stream_for(dev)));
+  }
+  for (size_t i = 0; i < ps.size(); ++i) {
     exp_avgs[i].unsafeGetTensorImpl()->bump_version();
     exp_avg_sqs[i].unsafeGetTensorImpl()->bump_version();
   }
@@ -531,6 +580,6 @@ TORCH_LIBRARY_IMPL(aten, PrivateUse1, m) {
 }
 
 void register_train_bindings(pybind11::module& m) {
-  m.def("impl_adamw_step", &ocl::adamw_step, "one AdamW step over parameters of one type on one device");
+  m.def("impl_adamw_step", &ocl::adamw_step, "one AdamW step over a group's parameters");
   m.def("impl_adamw8_values", &ocl::adamw8_values, "the moments that 8-bit codes stand for");
 }

@@ -40,7 +40,7 @@ struct LceSmem {
   static constexpr int A_BYTES = 128 * kLBK * 2;
   static constexpr int B_BYTES = BN / 2 * kLBK * 2;
   static constexpr int STAGE_BYTES = P * (A_BYTES + B_BYTES);
-  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES;
+    static constexpr int STAGES = (192 * 1024) / STAGE_BYTES;
   static constexpr int EPI_OFF = STAGES * STAGE_BYTES;  // one 4 KB store box per epilogue warp
   static constexpr int BAR_OFF = EPI_OFF + kLEpiWarps * 4096;
   static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16;
@@ -56,9 +56,9 @@ __device__ __forceinline__ uint32_t keep_code(float e) {
   const uint32_t b = __float_as_uint(e * 1.925929944387235853055977942584927e-34f);  // 2^-112
   return (b + 0x3ffu + ((b >> 11) & 1u)) >> 11;
 }
-__device__ __forceinline__ float keep_value(uint32_t code) {
-  return __uint_as_float(code << 11) * 5192296858534827628530496329220096.f;  // 2^112
-}
+// the number times 2^-112
+__device__ __forceinline__ float keep_bits(uint32_t code) { return __uint_as_float(code << 11); }
+constexpr float k2p112 = 5192296858534827628530496329220096.f;
 
 enum { kEpiStats = 0, kEpiGrad = 1, kEpiAcc = 2, kEpiOut = 3 };
 
@@ -727,41 +727,63 @@ __global__ void __launch_bounds__(256)
                          int64_t v0, int64_t width, int64_t V, int64_t ignore, float smoothing,
                          const float* __restrict__ lse, const float* __restrict__ grow, float gscale,
                          T* __restrict__ G, int64_t ldg, int planes) {
-  const int per_row = (int)(ldg / 8);
-  const int64_t total = rows * per_row;
-  const float flat = smoothing / (float)V;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t i = total <= INT32_MAX ? (int64_t)((int)e / per_row) : e / per_row;
-    const int64_t n = (e - i * per_row) * 8, col = v0 + n;
-    float v[8];
-    const float l = lse[i], g = grow[i], scale = g * gscale;
-    if (FP32) {
-      load_vec<8>((const float*)kept + i * keep_ld + col, v);
+  constexpr int U = FP32 ? 2 : 4;  // vectors of a thread, 2048 columns apart
+  const int64_t i = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  if (i >= rows) return;
+  const float flat = smoothing / (float)V, l = lse[i], g = grow[i], scale = g * gscale;
+  const int64_t tt = target[i], t = lce_scored(tt, V, ignore) ? tt - v0 : -1;
+  const int64_t n0 = ((int64_t)blockIdx.x * U * 256 + threadIdx.x) * 8;
+  float v[U][8];
+  if (FP32) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = expf(v[k] - l);
-    } else {
-      const uint4 c = *reinterpret_cast<const uint4*>((const uint16_t*)kept + i * keep_ld + col);
-      const float f = expf(keep_max[(col >> 6) * rows + i] - l);
-      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    for (int u = 0; u < U; ++u)
+      if (n0 + u * 2048 < ldg) load_vec<8>((const float*)kept + i * keep_ld + v0 + n0 + u * 2048, v[u]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[2 * k] = keep_value(w[k] & 0xffffu) * f;
-        v[2 * k + 1] = keep_value(w[k] >> 16) * f;
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[u][k] = expf(v[u][k] - l);
+  } else {
+    uint4 c[U];
+    float f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t col = v0 + n0 + u * 2048;
+      c[u] = make_uint4(0u, 0u, 0u, 0u);
+      f[u] = 0.f;
+      if (n0 + u * 2048 < ldg) {
+        c[u] = *reinterpret_cast<const uint4*>((const uint16_t*)kept + i * keep_ld + col);
+        f[u] = keep_max[(col >> 6) * rows + i];
       }
     }
-    const int64_t tt = target[i], t = lce_scored(tt, V, ignore) ? tt - col : -1;
-    if (t >= 0 && t < 8) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float e = expf(f[u] - l) * k2p112;  // the codes' power of two with it: at most 2^112
+      const uint32_t w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[u][2 * k] = keep_bits(w[k] & 0xffffu) * e;
+        v[u][2 * k + 1] = keep_bits(w[k] >> 16) * e;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t n = n0 + u * 2048;
+    if (n >= ldg) break;
+    if (t >= n && t < n + 8) {
       const float p = expf(ztarget[i] - l) - (1.f - smoothing);
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (k == t) v[k] = p;
+        if (n + k == t) v[u][k] = p;
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = g == 0.f ? 0.f : (v[k] - flat) * scale;
+    for (int k = 0; k < 8; ++k) v[u][k] = g == 0.f ? 0.f : (v[u][k] - flat) * scale;
     for (int z = 0; z < planes; ++z) {
-      store_vec<8>(G + (z * rows + i) * ldg + n, v);
+      store_vec<8>(G + (z * rows + i) * ldg + n, v[u]);
+      if (z + 1 < planes) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] -= to_f32(from_f32<T>(v[k]));
+        for (int k = 0; k < 8; ++k) v[u][k] -= to_f32(from_f32<T>(v[u][k]));
+      }
     }
   }
 }
@@ -1273,7 +1295,8 @@ template <typename T>
 static int lce_kept_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, const LceKept& k,
                          const int64_t* target, const float* lse, int64_t v0, int64_t width, int64_t ldg, float gscale,
                          cudaStream_t s) {
-  const int grid = grid_for(d->N * (ldg / 8), 256);
+  const unsigned rows = (unsigned)std::min<int64_t>(d->N, 32768);
+  const dim3 grid((unsigned)cdiv(ldg, k.fp32 ? 4096 : 8192), rows, (unsigned)cdiv(d->N, rows));
   const float smoothing = (float)d->label_smoothing;
   if (k.fp32)
     lce_kept_grad_kernel<T, true><<<grid, 256, 0, s>>>(k.data, k.ld, k.max, k.ztarget, d->N, target, v0, width, d->V,

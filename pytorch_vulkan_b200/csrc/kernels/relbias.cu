@@ -12,12 +12,15 @@
 // whatever the row's shift and the row's alignment in memory, each 16-byte
 // store then takes one aligned 16-byte load from the copy that fits.
 //
-// Backward: a thread owns diagonals.  Lanes read neighbouring diagonals of a
-// row (coalesced) and walk down the rows, so a diagonal's sum stays in a
-// register; a block then adds the diagonals of each bucket in order.  Sums
-// are fp32 over at most 64 rows and fp64 beyond; nothing is added in an order
-// that depends on timing.
+// Backward: a block owns 512 diagonals, two a thread, and walks down the rows
+// of one head, so that the diagonals' sums stay in registers; at the end it
+// adds those of each bucket in order.  32 rows at a time of the slanted strip
+// that the diagonals cut out are staged in shared memory by 16-byte loads (a
+// thread that loaded its own elements, two bytes each and at odd addresses,
+// reached a third of this rate).  Sums are fp32 over at most 64 rows and fp64
+// beyond; nothing is added in an order that depends on timing.
 #include <math.h>
+#include <atomic>
 #include <vector>
 #include "types.cuh"
 
@@ -26,7 +29,8 @@ namespace pvb2 {
 constexpr int kRelMaxBuckets = 512;
 constexpr int kRelCols = 1024;   // columns of a forward block
 constexpr int kRelRows = 64;     // most rows of a block
-constexpr int kRelDiag = 4;      // diagonals of a thread in the backward pass
+constexpr int kRelDiag = 512;    // diagonals of a block in the backward pass
+constexpr int kRelStage = 32;    // rows that are staged at a time
 constexpr int kRelInf = 1 << 30;
 
 struct RelMap {  // bucket b holds r in [lo[b], hi[b]] (empty where lo > hi)
@@ -80,56 +84,87 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// grid: (segments of diagonals) x (row tiles) x (B * H); part: [B*H][row
-// tiles][segments][nb]
-template <typename T>
+// grid: (segments of the rows) x (tiles of 512 diagonals) x (B * H); part:
+// [B*H][tiles][segments][nb].  FLAT: unit stride along the keys.
+template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256)
     rel_bias_bwd_kernel(const __grid_constant__ RelMap map, const T* __restrict__ grad, int64_t sb, int64_t sh,
-                        int64_t si, int64_t sj, double* __restrict__ part, int H, int Lq, int Lk, int q_offset, int R,
-                        int segments, int tiles_per_segment) {
-  __shared__ float diag[256 * kRelDiag];
-  __shared__ double acc[kRelMaxBuckets];
-  const int seg = blockIdx.x, rt = blockIdx.y;
+                        int64_t si, int64_t sj, double* __restrict__ part, int H, int Lq, int Lk, int q_offset) {
+  constexpr int V = 16 / sizeof(T);            // elements of a 16-byte load
+  constexpr int kVecs = kRelDiag / V + 1;      // of a row's strip, wherever it begins
+  constexpr int kPitch = (kVecs + 1) * V;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  T* stage = reinterpret_cast<T*>(smem_raw);   // [32][kPitch]
+  __shared__ double diag[kRelDiag];
+  const int seg = blockIdx.x, tile = blockIdx.y;
+  const int64_t z = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i0 = rt * R, rows = min(R, Lq - i0);
-  const int first = -(i0 + rows - 1), len = rows + Lk - 1;  // diagonals j - i of these rows
-  for (int64_t z = blockIdx.z; z < gridDim.z; z += gridDim.z) {
-    const T* g = grad + (z / H) * sb + (z % H) * sh + (int64_t)i0 * si;
-    for (int b = threadIdx.x; b < map.nb; b += 256) acc[b] = 0.0;
-    for (int tile = seg * tiles_per_segment; tile < (seg + 1) * tiles_per_segment; ++tile) {
-      const int e0 = tile * 256 * kRelDiag;
-      if (e0 >= len) break;
-      float sum[kRelDiag];
-#pragma unroll
-      for (int k = 0; k < kRelDiag; ++k) sum[k] = 0.f;
-      // element of row i0 + r on diagonal e: column first + e + i0 + r
-      const int c0 = first + i0 + e0 + (int)threadIdx.x;
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r) {
-#pragma unroll
-        for (int k = 0; k < kRelDiag; ++k) {
-          const int c = c0 + r + 256 * k;
-          if (c >= 0 && c < Lk) sum[k] += to_f32(g[(int64_t)r * si + (int64_t)c * sj]);
+  const int d0 = tile * kRelDiag - (Lq - 1);  // first diagonal j - i
+  // rows that these diagonals meet, and this segment's share of them
+  const int ra = max(0, -(d0 + kRelDiag - 1)), rb = min(Lq, Lk - d0);
+  const int per = (max(0, rb - ra) + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int i0 = ra + seg * per, i1 = min(rb, i0 + per);
+  const T* g = grad + (z / H) * sb + (z % H) * sh;
+  const int e0 = (int)threadIdx.x;
+  double acc0 = 0.0, acc1 = 0.0;
+  float s0 = 0.f, s1 = 0.f;
+  int held = 0;
+  for (int i = i0; i < i1; i += kRelStage) {
+    const int rows = min(kRelStage, i1 - i);
+    __syncthreads();  // the stage before has been added up
+    // row r: columns c0 + r .. c0 + r + 511, from the 16-byte boundary before
+    if (FLAT) {
+      for (int q = threadIdx.x; q < rows * kVecs; q += 256) {
+        const int r = q / kVecs, k = q - r * kVecs;
+        const T* row = g + (int64_t)(i + r) * si;
+        const int c0 = d0 + i + r;
+        const int lead = (int)(((uintptr_t)(row + c0) & 15) / sizeof(T));
+        const int c = c0 - lead + k * V;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (c >= 0 && c + V <= Lk) {
+          x = *reinterpret_cast<const uint4*>(row + c);
+        } else if (c + V > 0 && c < Lk) {
+          T* e = reinterpret_cast<T*>(&x);
+          for (int j = 0; j < V; ++j)
+            if (c + j >= 0 && c + j < Lk) e[j] = row[c + j];
         }
+        *reinterpret_cast<uint4*>(stage + r * kPitch + k * V) = x;
       }
-      __syncthreads();  // the tile before has been added up
-#pragma unroll
-      for (int k = 0; k < kRelDiag; ++k) diag[threadIdx.x + 256 * k] = sum[k];
-      __syncthreads();
-      const int r0 = first + e0 - q_offset;
-      for (int b = warp; b < map.nb; b += 8) {
-        const int lo = max(map.lo[b], r0), hi = min(map.hi[b], r0 + 256 * kRelDiag - 1);
-        if (lo > hi) continue;
-        double s = 0.0;
-        for (int r = lo + lane; r <= hi; r += 32) s += (double)diag[r - r0];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) acc[b] += s;
+    } else {
+      for (int q = threadIdx.x; q < rows * kRelDiag; q += 256) {
+        const int r = q / kRelDiag, k = q - r * kRelDiag, c = d0 + i + r + k;
+        stage[r * kPitch + k] = c >= 0 && c < Lk ? g[(int64_t)(i + r) * si + (int64_t)c * sj] : from_f32<T>(0.f);
       }
     }
     __syncthreads();
-    double* p = part + (((int64_t)z * gridDim.y + rt) * segments + seg) * map.nb;
-    for (int b = threadIdx.x; b < map.nb; b += 256) p[b] = acc[b];
+    if (held + rows > 64) {
+      acc0 += (double)s0;
+      acc1 += (double)s1;
+      s0 = s1 = 0.f;
+      held = 0;
+    }
+    held += rows;
+    const T* row = g + (int64_t)i * si + d0 + i;  // its address mod 16 moves by si + 1 elements a row
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      const int lead = FLAT ? (int)(((uintptr_t)(row + (int64_t)r * (si + 1)) & 15) / sizeof(T)) : 0;
+      const T* x = stage + r * kPitch + lead + e0;
+      s0 += to_f32(x[0]);
+      s1 += to_f32(x[256]);
+    }
+  }
+  diag[e0] = acc0 + (double)s0;
+  diag[e0 + 256] = acc1 + (double)s1;
+  __syncthreads();
+  double* p = part + ((z * gridDim.y + tile) * gridDim.x + seg) * map.nb;
+  const int r0 = d0 - q_offset;
+  for (int b = warp; b < map.nb; b += 8) {
+    const int lo = max(map.lo[b], r0), hi = min(map.hi[b], r0 + kRelDiag - 1);
+    double s = 0.0;
+    for (int r = lo + lane; r <= hi; r += 32) s += diag[r - r0];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) p[b] = s;
   }
 }
 
@@ -212,19 +247,15 @@ static int rel_rows(int64_t heads, int64_t Lq, int64_t across) {
 }
 
 struct RelBwdPlan {
-  int R, segments, per_segment;
-  int64_t row_tiles;
+  int64_t tiles, segments;
 };
 
+// segments of the rows: eight blocks for every SM, no fewer than 32 rows each
 static RelBwdPlan rel_bwd_plan(const pvb2_relative_bias_desc* d, int64_t B) {
   RelBwdPlan p;
-  p.R = std::max(8, rel_rows(B * d->H, d->Lq, 1));
-  p.row_tiles = cdiv(d->Lq, p.R);
-  const int64_t tiles = cdiv(p.R + d->Lk - 1, 256 * kRelDiag);
-  const int64_t blocks = std::max<int64_t>(1, B * d->H * p.row_tiles);
-  const int64_t want = std::min<int64_t>(tiles, std::max<int64_t>(1, 4 * (int64_t)num_sms() / blocks));
-  p.per_segment = (int)cdiv(tiles, want);
-  p.segments = (int)cdiv(tiles, p.per_segment);
+  p.tiles = cdiv(d->Lq + d->Lk - 1, kRelDiag);
+  const int64_t want = cdiv(8 * (int64_t)num_sms(), std::max<int64_t>(1, B * d->H * p.tiles));
+  p.segments = std::max<int64_t>(1, std::min(want, cdiv(d->Lq, kRelStage)));
   return p;
 }
 
@@ -247,11 +278,18 @@ static int rel_bwd(const pvb2_relative_bias_desc* d, const RelMap& m, const pvb2
   const RelBwdPlan p = rel_bwd_plan(d, B);
   int64_t per_z = 0;
   if (B > 0 && d->Lq > 0 && d->Lk > 0) {
-    PVB2_CHECK_ARG(B * d->H <= 65535 && p.row_tiles <= 65535, "relative bias: batch x heads or rows out of range");
-    per_z = p.row_tiles * p.segments;
-    rel_bias_bwd_kernel<T><<<dim3(p.segments, (unsigned)p.row_tiles, (unsigned)(B * d->H)), 256, 0, s>>>(
-        m, (const T*)g->data, g->strides[0], g->strides[1], g->strides[2], g->strides[3], part, d->H, (int)d->Lq,
-        (int)d->Lk, (int)d->q_offset, p.R, p.segments, p.per_segment);
+    PVB2_CHECK_ARG(B * d->H <= 65535 && p.tiles <= 65535, "relative bias: batch x heads or lengths out of range");
+    per_z = p.tiles * p.segments;
+    constexpr int smem = kRelStage * (kRelDiag + 2 * 16 / (int)sizeof(T)) * (int)sizeof(T);
+    static std::atomic<uint64_t> attr_done{0};
+    if (smem > 40 * 1024 && first_on_device(attr_done)) {
+      PVB2_CUDA_TRY(cudaFuncSetAttribute(rel_bias_bwd_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      PVB2_CUDA_TRY(cudaFuncSetAttribute(rel_bias_bwd_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    }
+    const dim3 grid((unsigned)p.segments, (unsigned)p.tiles, (unsigned)(B * d->H));
+    auto kernel = g->strides[3] == 1 || d->Lk == 1 ? rel_bias_bwd_kernel<T, true> : rel_bias_bwd_kernel<T, false>;
+    kernel<<<grid, 256, smem, s>>>(m, (const T*)g->data, g->strides[0], g->strides[1], g->strides[2], g->strides[3],
+                                   part, d->H, (int)d->Lq, (int)d->Lk, (int)d->q_offset);
     PVB2_LAUNCH_CHECK();
   }
   const int warps = m.nb * d->H;
@@ -282,7 +320,7 @@ int pvb2_relative_bias_fwd(const pvb2_relative_bias_desc* d, const void* table, 
 size_t pvb2_relative_bias_bwd_workspace_size(const pvb2_relative_bias_desc* d, int64_t B) {
   if (rel_check(d) != PVB2_OK || B <= 0 || d->Lq == 0 || d->Lk == 0) return 0;
   const RelBwdPlan p = rel_bwd_plan(d, B);
-  return (size_t)(B * d->H * p.row_tiles * p.segments) * d->num_buckets * sizeof(double);
+  return (size_t)(B * d->H * p.tiles * p.segments) * d->num_buckets * sizeof(double);
 }
 
 int pvb2_relative_bias_bwd(const pvb2_relative_bias_desc* d, const pvb2_tensor* grad, void* dtable, void* workspace,

@@ -80,31 +80,15 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        m, v, *scales = _KEYS[self.state_bits]
         for group in self.param_groups:
-            lists = {}
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                if g.is_sparse:
-                    raise RuntimeError("AdamW does not take sparse gradients")
-                s = self.state[p] or self._init_state(p)
-                of = lists.get((p.device, p.dtype))
-                if of is None:
-                    of = lists[p.device, p.dtype] = ([], [], [], [], [], [], [])
-                of[0].append(p)
-                of[1].append(g)
-                of[2].append(s[m])
-                of[3].append(s[v])
-                if scales:
-                    of[4].append(s[scales[0]])
-                    of[5].append(s[scales[1]])
-                of[6].append(s["step"])
             beta1, beta2 = group["betas"]
-            for of in lists.values():
-                _C.impl_adamw_step(*of, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"],
-                                   group["maximize"])
+            args = (group["params"], self.state, self.state_bits, float(group["lr"]), beta1, beta2, group["eps"],
+                    group["weight_decay"], group["maximize"])
+            missing = _C.impl_adamw_step(*args)
+            if missing:
+                for p in missing:
+                    self._init_state(p)
+                _C.impl_adamw_step(*args)
         return loss
 
     @torch.no_grad()
@@ -115,22 +99,16 @@ class AdamW(torch.optim.Optimizer):
         ``param_groups``, laid out like its parameter (a checkpoint for another
         optimizer, a look at the moments).
         """
-        held = [self.state[p] for group in self.param_groups for p in group["params"] if self.state.get(p)]
+        params = [p for group in self.param_groups for p in group["params"]]
+        if self.state_bits == 8:
+            _C.impl_adamw8_values(params, self.state, exp_avgs, exp_avg_sqs)
+            return
+        held = [self.state[p] for p in params if self.state.get(p)]
         if len(exp_avgs) != len(held) or len(exp_avg_sqs) != len(held):
             raise ValueError(f"{len(held)} parameters have a state, got {len(exp_avgs)} and {len(exp_avg_sqs)} tensors")
-        if self.state_bits == 32:
-            for s, a, b in zip(held, exp_avgs, exp_avg_sqs):
-                a.copy_(s["exp_avg"])
-                b.copy_(s["exp_avg_sq"])
-            return
-        by_device = {}
         for s, a, b in zip(held, exp_avgs, exp_avg_sqs):
-            of = by_device.setdefault(s["step"].device, ([], [], [], [], [], []))
-            for column, t in zip(of, (s["exp_avg_code"], s["exp_avg_scale"], s["exp_avg_rms_code"],
-                                      s["exp_avg_rms_scale"], a, b)):
-                column.append(t)
-        for of in by_device.values():
-            _C.impl_adamw8_values(*of)
+            a.copy_(s["exp_avg"])
+            b.copy_(s["exp_avg_sq"])
 
     def load_state_dict(self, state_dict):
         """As torch's, but the state keeps its own types (torch casts floating state to the parameters')."""
