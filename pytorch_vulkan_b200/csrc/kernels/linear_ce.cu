@@ -289,6 +289,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
     // ------------------------------------------------- products, by the even CTA for both
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_f16(kLBM, BN, !std::is_same<T, __half>::value, a_mn, b_mn);
+      // One thread issues everything in order, so that what it computes between
+      // two MMAs holds up the tensor core: the descriptors are formed once, and
+      // a step along K, a plane or a stage is an addition to their address
+      // (16-byte units, below 2^14).  Formed anew for each MMA they took it
+      // longer than the MMA.
+      const uint32_t smem0 = smem_u32(smem);
+      const uint64_t a0 = a_mn ? desc_mnmajor16(smem0, 0, 8192) : desc_kmajor(smem0, 0);
+      const uint64_t b0 = b_mn ? desc_mnmajor16(smem0 + P * L::A_BYTES, 0, 8192) : desc_kmajor(smem0 + P * L::A_BYTES, 0);
+      const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;
       uint32_t it = 0, chunk = 0;
       int local = 0;
       for (int tile = pair; tile < total_tiles && !*abort; tile += pairs, ++local) {
@@ -305,17 +314,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
             const int s = it % kStages;
             if (!mbar_wait(&full[s], (it / kStages) & 1, abort)) break;
             tc_fence_after();
-            const uint32_t sa = smem_u32(smem + s * L::STAGE_BYTES);
-            const uint32_t sb = sa + P * L::A_BYTES;
+            const uint64_t sa = a0 + (uint32_t)(s * (L::STAGE_BYTES / 16));
+            const uint64_t sb = b0 + (uint32_t)(s * (L::STAGE_BYTES / 16));
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
-              const uint32_t pa = sa + lce_pa<P>(i) * L::A_BYTES, pb = sb + lce_pb<P>(i) * L::B_BYTES;
+              uint64_t ad = sa + lce_pa<P>(i) * (L::A_BYTES / 16), bd = sb + lce_pb<P>(i) * (L::B_BYTES / 16);
 #pragma unroll
               for (int kk = 0; kk < kLBK / 16; ++kk) {
-                const uint64_t ad = a_mn ? desc_mnmajor16(pa, kk, 8192) : desc_kmajor(pa, kk);
-                const uint64_t bd = b_mn ? desc_mnmajor16(pb, kk, 8192) : desc_kmajor(pb, kk);
                 if (i == kPairs - 1) mma_f16_pair(d_main, ad, bd, idesc, (kb > c0 || kk > 0) ? 1u : 0u);
                 else mma_f16_pair(d_small, ad, bd, idesc, (kb > kb0 || i > 0 || kk > 0) ? 1u : 0u);
+                ad += a_step;
+                bd += b_step;
               }
             }
             mma_commit_pair(&empty[s]);
@@ -591,8 +600,9 @@ __global__ void lce_pack_kernel(const S* __restrict__ src, int64_t rows, int64_t
 __global__ void __launch_bounds__(1024)
     lce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zsum, int64_t part_ld, int parts,
                     const float* __restrict__ ztarget, const int64_t* __restrict__ target, int64_t N, int64_t V,
-                    int64_t ignore, float smoothing, float* __restrict__ lse, float* __restrict__ loss) {
-  __shared__ float sm[32][33], ss[32][33], sz[32][33];
+                    int64_t ignore, float smoothing, float* __restrict__ lse, float* __restrict__ loss,
+                    int total_of, float* __restrict__ out, float* __restrict__ count) {
+  __shared__ float sm[32][33], ss[32][33], sz[32][33], sl[32];
   const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t i = (int64_t)blockIdx.x * 32 + r;
   float mx = -INFINITY, sum = 0.f, zs = 0.f;
@@ -631,6 +641,20 @@ __global__ void __launch_bounds__(1024)
       if (smoothing != 0.f) v = (1.f - smoothing) * v + smoothing * (l - zs / (float)V);
     }
     loss[row] = v;
+    sl[g] = v;
+  }
+  if (total_of < 0) return;
+  // all rows are in this block: their total (reduction total_of) as well
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    int n = 0;
+    for (int q = 0; q < (int)N; ++q) {
+      all += (double)sl[q];
+      n += lce_scored(target[q], V, ignore) ? 1 : 0;
+    }
+    *count = (float)n;
+    if (total_of != PVB2_LOSS_NONE) *out = (float)(total_of == PVB2_LOSS_MEAN ? all / (double)n : all);
   }
 }
 
@@ -690,6 +714,137 @@ __global__ void __launch_bounds__(512)
       if (ztarget) ztarget[i] = zt;
     }
     loss[i] = v;
+  }
+}
+
+// Few rows (a token or some while serving): a product with so few rows is a
+// pass over w, bound by HBM, which 256-row tiles read at half the rate (their
+// loads take 128 bytes of each of w's rows at a time, and as many of x's).
+// Here a warp reads R of w's rows at once, each lane 16 bytes of each, and
+// multiplies them by the NT rows of x from shared memory in fp32; its lanes
+// then keep the running maximum and sum of their row of x.  One V = 32768, D =
+// 2048 fp16 row: 25 us against 54.
+template <int L>
+__device__ __forceinline__ float sum_spread(float (&a)[L], int lane) {
+  // sums of L values over the warp, value i in the lanes i * 32 / L ..
+  int o = 16;
+#pragma unroll
+  for (int n = L; n > 1; n /= 2, o /= 2) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float send = upper ? a[i] : a[i + n / 2];
+      a[i] = (upper ? a[i + n / 2] : a[i]) + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  float s = a[0];
+  for (; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+template <typename S, int NT, int R, bool VEC>
+__global__ void __launch_bounds__(256, 2)
+    lce_few_rows_kernel(const S* __restrict__ x, int64_t ldx, const S* __restrict__ w, int64_t ldw,
+                        const S* __restrict__ bias, const int64_t* __restrict__ target, int N, int D, int V,
+                        int64_t ignore, int smooth, float2* __restrict__ part, float* __restrict__ zsum,
+                        float* __restrict__ ztarget, float* __restrict__ kept, int keep, int64_t keep_ld) {
+  constexpr int L = R * NT;          // logits of a pass over R rows of w
+  constexpr int kSpan = 32 / L;      // lanes that hold each
+  extern __shared__ __align__(16) uint8_t few_smem[];
+  S* xs = reinterpret_cast<S*>(few_smem);  // [NT][dp], zeros behind D and N
+  __shared__ float sm[8][L], ss[8][L], sz[8][L];
+  const int dp = (D + 7) / 8 * 8;
+  for (int e = threadIdx.x; e < NT * dp; e += 256) {
+    const int t = e / dp, c = e - t * dp;
+    xs[e] = t < N && c < D ? x[t * ldx + c] : from_f32<S>(0.f);
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int my_r = lane / kSpan / NT, my_t = lane / kSpan % NT;  // the logit that this lane ends up with
+  const int64_t goal = my_t < N ? target[my_t] : -1;
+  const int t_col = my_t < N && lce_scored(goal, V, ignore) ? (int)goal : -1;
+  float mx = -INFINITY, sum = 0.f, zs = 0.f;
+  const int groups = (V + R - 1) / R;
+  for (int q = blockIdx.x * 8 + warp; q < groups; q += gridDim.x * 8) {
+    const int v0 = q * R;
+    const S* rows[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) rows[r] = w + (int64_t)min(v0 + r, V - 1) * ldw;  // behind the last: read, not used
+    float acc[L];
+#pragma unroll
+    for (int k = 0; k < L; ++k) acc[k] = 0.f;
+    auto multiply = [&](const float (&wv)[8], int r, int c) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float xv[8];
+        load_vec<8>(xs + t * dp + c, xv);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[r * NT + t] = fmaf(wv[k], xv[k], acc[r * NT + t]);
+      }
+    };
+    int c = lane * 8;
+    if (VEC) {
+      // the loads of the next 256 columns are on their way while these are multiplied
+      RawVec<8 * sizeof(S)> now[R], next[R];
+      const int whole = D / 8 * 8;
+      if (c < whole) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) now[r] = *reinterpret_cast<const RawVec<8 * sizeof(S)>*>(rows[r] + c);
+      }
+      for (; c < whole; c += 256) {
+        if (c + 256 < whole) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) next[r] = *reinterpret_cast<const RawVec<8 * sizeof(S)>*>(rows[r] + c + 256);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float wv[8];
+          unpack_vec<8, S>(now[r], wv);
+          multiply(wv, r, c);
+          now[r] = next[r];
+        }
+      }
+    }
+    for (; c < D; c += 256) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float wv[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) wv[k] = c + k < D ? to_f32(rows[r][c + k]) : 0.f;
+        multiply(wv, r, c);
+      }
+    }
+    float z = sum_spread<L>(acc, lane);
+    const int v = v0 + my_r;
+    if (v < V && my_t < N && lane % kSpan == 0) {
+      if (bias) z += to_f32(bias[v]);
+      if (v == t_col) ztarget[my_t] = z;
+      if (v < keep) kept[my_t * keep_ld + v] = z;
+      const float nm = fmaxf(mx, z), base = nm == -INFINITY ? 0.f : nm;
+      sum = sum * expf(mx - base) + expf(z - base);
+      mx = nm;
+      zs += z;
+    }
+  }
+  if (lane % kSpan == 0) {
+    sm[warp][lane / kSpan] = mx;
+    ss[warp][lane / kSpan] = sum;
+    sz[warp][lane / kSpan] = zs;
+  }
+  __syncthreads();
+  if (threadIdx.x < N) {
+    mx = -INFINITY;
+    sum = zs = 0.f;
+    for (int g = 0; g < 8; ++g)
+      for (int r = 0; r < R; ++r) {
+        const int at = r * NT + threadIdx.x;
+        const float om = sm[g][at], nm = fmaxf(mx, om), base = nm == -INFINITY ? 0.f : nm;
+        sum = sum * expf(mx - base) + ss[g][at] * expf(om - base);
+        mx = nm;
+        zs += sz[g][at];
+      }
+    part[blockIdx.x * N + threadIdx.x] = make_float2(mx, sum);
+    if (smooth) zsum[blockIdx.x * N + threadIdx.x] = zs;
   }
 }
 
@@ -959,6 +1114,7 @@ static LceTiling lce_tiling(int64_t M, int64_t N, int64_t K, int P, int64_t read
 }
 
 struct LcePlan {
+  bool few;          // forward: few rows, no tiles
   int P;             // planes of an operand
   bool half;         // fp16 operands (bf16 otherwise)
   int64_t ldp;       // row length of packed operands
@@ -969,6 +1125,9 @@ struct LcePlan {
   int colsum_parts;
   int64_t rows_per;
 };
+
+// rows that lce_few_rows_kernel takes, and their bytes in shared memory
+constexpr int kLFewRows = 8, kLFewBytes = 64 * 1024;
 
 constexpr int64_t kLRowsFwd = 16384;  // rows whose parts are held at a time
 
@@ -989,6 +1148,8 @@ static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   p.P = d->dtype != PVB2_F32 ? 1 : d->math == PVB2_MATH_FP32 ? 3 : 2;
   p.ldp = up(d->D, 8);
   p.pack_w = !lce_direct(d, d->ldw);
+  const int size = d->dtype == PVB2_F32 ? 4 : 2;
+  p.few = !backward && d->N <= kLFewRows && (int64_t)kLFewRows * p.ldp * size <= kLFewBytes;
   const int64_t rows = backward ? d->N : std::min(d->N, kLRowsFwd);
   const int64_t esize = 2 * p.P;
   // most entries of a piece: a packed piece of w in 256 MB, G in 128 MB, at
@@ -1067,16 +1228,25 @@ struct LceFwdSpace {
   float *zsum, *ztarget, *loss;
 };
 
-static bool lce_slabs(const LcePlan& p) { return p.z.splits > 1; }
+static bool lce_slabs(const LcePlan& p) { return !p.few && p.z.splits > 1; }
 
-static bool lce_kept_fp32(const pvb2_linear_ce_desc* d) { return d->dtype == PVB2_F32 || lce_slabs(lce_plan(d, false)); }
+// blocks of lce_few_rows_kernel: two for every SM
+static int lce_few_blocks(const pvb2_linear_ce_desc* d) {
+  return (int)std::min<int64_t>(2 * num_sms(), cdiv(d->V, 16));
+}
+
+static bool lce_kept_fp32(const pvb2_linear_ce_desc* d) {
+  const LcePlan p = lce_plan(d, false);
+  return d->dtype == PVB2_F32 || p.few || lce_slabs(p);
+}
 
 static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceFwdSpace* s) {
   Arena a{(uint8_t*)base};
-  const int64_t rows = std::min(d->N, kLRowsFwd), parts = cdiv(up(d->V, 256), p.z.bn / 2);
+  const int64_t rows = std::min(d->N, kLRowsFwd);
+  const int64_t parts = p.few ? lce_few_blocks(d) : cdiv(up(d->V, 256), p.z.bn / 2);
   const bool slabs = lce_slabs(p);
-  s->x = a.take<uint16_t>(lce_direct(d, d->ldx) ? 0 : rows * p.ldp * p.P);
-  s->w = a.take<uint16_t>(p.pack_w ? p.piece * p.ldp * p.P : 0);
+  s->x = a.take<uint16_t>(p.few || lce_direct(d, d->ldx) ? 0 : rows * p.ldp * p.P);
+  s->w = a.take<uint16_t>(!p.few && p.pack_w ? p.piece * p.ldp * p.P : 0);
   s->slab = a.take<float>(slabs ? p.z.splits * rows * up(d->V, 4) : 0);
   s->part = a.take<float2>(slabs ? 0 : rows * parts);
   s->zsum = a.take<float>(!slabs && d->label_smoothing != 0 ? rows * parts : 0);
@@ -1281,6 +1451,34 @@ static int lce_out(const pvb2_linear_ce_desc* d, const LcePlan& p, const CUtenso
   return lce_gemm<kEpiOut>(a, b, c, g, a_mn, true, p, bn, s);
 }
 
+template <typename S, int NT, int R>
+static int lce_few_launch(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias,
+                          const int64_t* target, const LceFwdSpace& sp, const LceKept& k, cudaStream_t s) {
+  const bool vec = ((uintptr_t)w & 15) == 0 && d->ldw * sizeof(S) % 16 == 0;
+  auto kernel = vec ? lce_few_rows_kernel<S, NT, R, true> : lce_few_rows_kernel<S, NT, R, false>;
+  static std::atomic<uint64_t> attr_done{0};
+  if (first_on_device(attr_done)) {
+    PVB2_CUDA_TRY(cudaFuncSetAttribute(lce_few_rows_kernel<S, NT, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLFewBytes));
+    PVB2_CUDA_TRY(cudaFuncSetAttribute(lce_few_rows_kernel<S, NT, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLFewBytes));
+  }
+  const size_t smem = (size_t)NT * up(d->D, 8) * sizeof(S);
+  kernel<<<lce_few_blocks(d), 256, smem, s>>>((const S*)x, d->ldx, (const S*)w, d->ldw, (const S*)bias, target,
+                                              (int)d->N, (int)d->D, (int)d->V, d->ignore_index,
+                                              d->label_smoothing != 0, sp.part, sp.zsum,
+                                              d->kept ? k.ztarget : sp.ztarget, (float*)k.data, (int)d->kept, k.ld);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+template <typename S>
+static int lce_few(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* target,
+                   const LceFwdSpace& sp, const LceKept& k, cudaStream_t s) {
+  if (d->N == 1) return lce_few_launch<S, 1, 8>(d, x, w, bias, target, sp, k, s);
+  if (d->N == 2) return lce_few_launch<S, 2, 4>(d, x, w, bias, target, sp, k, s);
+  if (d->N <= 4) return lce_few_launch<S, 4, 4>(d, x, w, bias, target, sp, k, s);
+  return lce_few_launch<S, 8, 2>(d, x, w, bias, target, sp, k, s);
+}
+
 // logits of `rows` rows as partial sums
 static int lce_slab_logits(const pvb2_linear_ce_desc* d, const LcePlan& p, const CUtensorMap& x, const CUtensorMap& w,
                            LceGemm g, float* slab, cudaStream_t s) {
@@ -1366,22 +1564,26 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     const bool direct_x = lce_direct(d, d->ldx), slabs = lce_slabs(p);
     PVB2_TRY(lce_aligned(x, direct_x));
     PVB2_TRY(lce_aligned(w, !p.pack_w));
-    const int parts = (int)cdiv(d->V, p.z.bn / 2), esize = d->dtype == PVB2_F32 ? 4 : 2;
+    const int parts = p.few ? lce_few_blocks(d) : (int)cdiv(d->V, p.z.bn / 2), esize = d->dtype == PVB2_F32 ? 4 : 2;
     const float smoothing = (float)d->label_smoothing;
     PVB2_CHECK_ARG(d->kept == 0 || (kept && ((uintptr_t)kept & 15) == 0),
                    "linear cross entropy: 16-byte aligned memory for what is kept needed");
     LceKept k;
-    lce_kept_space(d, d->dtype == PVB2_F32 || slabs, kept, &k);
+    lce_kept_space(d, d->dtype == PVB2_F32 || p.few || slabs, kept, &k);
     for (int64_t r0 = 0; r0 < d->N; r0 += kLRowsFwd) {
       const int64_t rows = std::min(kLRowsFwd, d->N - r0);
       CUtensorMap ma, mb;
-      if (direct_x) {
+      if (p.few) {
+        if (d->dtype == PVB2_F32) PVB2_TRY(lce_few<float>(d, x, w, bias, target, sp, k, s));
+        else if (p.half) PVB2_TRY(lce_few<__half>(d, x, w, bias, target, sp, k, s));
+        else PVB2_TRY(lce_few<__nv_bfloat16>(d, x, w, bias, target, sp, k, s));
+      } else if (direct_x) {
         PVB2_TRY(lce_map_a(&ma, (const uint8_t*)x + r0 * d->ldx * esize, d->D, rows, d->ldx, p));
       } else {
         PVB2_TRY(lce_pack(d, p, x, r0, rows, d->ldx, sp.x, nullptr, s));
         PVB2_TRY(lce_map_a(&ma, sp.x, d->D, rows, p.ldp, p));
       }
-      for (int64_t v0 = 0; v0 < d->V; v0 += p.piece) {
+      for (int64_t v0 = 0; v0 < d->V && !p.few; v0 += p.piece) {
         const int64_t width = std::min(p.piece, d->V - v0);
         if (!p.pack_w) {
           PVB2_TRY(lce_map_b(&mb, w, d->D, d->V, d->ldw, p, p.z.bn));
@@ -1415,9 +1617,11 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       else
         lce_rows_kernel<<<(int)cdiv(rows, 32), 1024, 0, s>>>(
             sp.part, smoothing != 0.f ? sp.zsum : nullptr, rows, parts, d->kept ? k.ztarget + r0 : sp.ztarget,
-            target + r0, rows, d->V, d->ignore_index, smoothing, lse + r0, loss + r0);
+            target + r0, rows, d->V, d->ignore_index, smoothing, lse + r0, loss + r0,
+            !slabs && d->N <= 32 ? d->reduction : -1, out, count);
       PVB2_LAUNCH_CHECK();
     }
+    if (!slabs && d->N <= 32) return PVB2_OK;
   }
   lce_total_kernel<<<1, 1024, 0, s>>>(loss, target, d->N, d->V, d->ignore_index, d->reduction, out, count);
   PVB2_LAUNCH_CHECK();

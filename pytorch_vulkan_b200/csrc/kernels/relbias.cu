@@ -106,6 +106,10 @@ __global__ void __launch_bounds__(256)
   const int i0 = ra + seg * per, i1 = min(rb, i0 + per);
   const T* g = grad + (z / H) * sb + (z % H) * sh;
   const int e0 = (int)threadIdx.x;
+  // elements from the 16-byte boundary to the first of row i0's strip; one row
+  // further it is si + 1 elements more
+  const int lead0 = (int)(((uintptr_t)(g + (int64_t)i0 * si + d0 + i0) & 15) / sizeof(T));
+  const int lead_step = (int)((si + 1) & (V - 1));
   double acc0 = 0.0, acc1 = 0.0;
   float s0 = 0.f, s1 = 0.f;
   int held = 0;
@@ -114,21 +118,27 @@ __global__ void __launch_bounds__(256)
     __syncthreads();  // the stage before has been added up
     // row r: columns c0 + r .. c0 + r + 511, from the 16-byte boundary before
     if (FLAT) {
-      for (int q = threadIdx.x; q < rows * kVecs; q += 256) {
-        const int r = q / kVecs, k = q - r * kVecs;
+      // a warp takes every eighth row, a lane every 32nd vector
+#pragma unroll
+      for (int rr = 0; rr < kRelStage; rr += 8) {
+        const int r = rr + warp;
+        if (r >= rows) continue;
         const T* row = g + (int64_t)(i + r) * si;
-        const int c0 = d0 + i + r;
-        const int lead = (int)(((uintptr_t)(row + c0) & 15) / sizeof(T));
-        const int c = c0 - lead + k * V;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (c >= 0 && c + V <= Lk) {
-          x = *reinterpret_cast<const uint4*>(row + c);
-        } else if (c + V > 0 && c < Lk) {
-          T* e = reinterpret_cast<T*>(&x);
-          for (int j = 0; j < V; ++j)
-            if (c + j >= 0 && c + j < Lk) e[j] = row[c + j];
+        const int c0 = d0 + i + r - ((lead0 + (i - i0 + r) * lead_step) & (V - 1));
+#pragma unroll
+        for (int kk = 0; kk < kVecs; kk += 32) {
+          const int k = kk + lane, c = c0 + k * V;
+          if (k >= kVecs) continue;
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (c >= 0 && c + V <= Lk) {
+            x = *reinterpret_cast<const uint4*>(row + c);
+          } else if (c + V > 0 && c < Lk) {
+            T* e = reinterpret_cast<T*>(&x);
+            for (int j = 0; j < V; ++j)
+              if (c + j >= 0 && c + j < Lk) e[j] = row[c + j];
+          }
+          *reinterpret_cast<uint4*>(stage + r * kPitch + k * V) = x;
         }
-        *reinterpret_cast<uint4*>(stage + r * kPitch + k * V) = x;
       }
     } else {
       for (int q = threadIdx.x; q < rows * kRelDiag; q += 256) {
@@ -144,13 +154,20 @@ __global__ void __launch_bounds__(256)
       held = 0;
     }
     held += rows;
-    const T* row = g + (int64_t)i * si + d0 + i;  // its address mod 16 moves by si + 1 elements a row
-#pragma unroll 8
-    for (int r = 0; r < rows; ++r) {
-      const int lead = FLAT ? (int)(((uintptr_t)(row + (int64_t)r * (si + 1)) & 15) / sizeof(T)) : 0;
-      const T* x = stage + r * kPitch + lead + e0;
-      s0 += to_f32(x[0]);
-      s1 += to_f32(x[256]);
+    const int l0 = FLAT ? lead0 + (i - i0) * lead_step : 0;
+    if (rows == kRelStage) {
+#pragma unroll
+      for (int r = 0; r < kRelStage; ++r) {
+        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0) + e0;
+        s0 += to_f32(x[0]);
+        s1 += to_f32(x[256]);
+      }
+    } else {
+      for (int r = 0; r < rows; ++r) {
+        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0) + e0;
+        s0 += to_f32(x[0]);
+        s1 += to_f32(x[256]);
+      }
     }
   }
   diag[e0] = acc0 + (double)s0;

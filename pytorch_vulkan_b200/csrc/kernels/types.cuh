@@ -54,6 +54,18 @@ __device__ __forceinline__ void load_vec(const T* p, float* v) {
 }
 
 template <int N, typename T>
+__device__ __forceinline__ void unpack_vec(const RawVec<N * sizeof(T)>& raw, float* v) {
+  union U {
+    RawVec<N * sizeof(T)> raw;
+    T e[N];
+    __device__ U() {}
+  } u;
+  u.raw = raw;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = to_f32(u.e[i]);
+}
+
+template <int N, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float* v) {
   union U {
     RawVec<N * sizeof(T)> raw;
