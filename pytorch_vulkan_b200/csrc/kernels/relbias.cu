@@ -14,10 +14,11 @@
 //
 // Backward: a block owns 512 diagonals, two a thread, and walks down the rows
 // of one head, so that the diagonals' sums stay in registers; at the end it
-// adds those of each bucket in order.  32 rows at a time of the slanted strip
-// that the diagonals cut out are staged in shared memory by 16-byte loads (a
-// thread that loaded its own elements, two bytes each and at odd addresses,
-// reached a third of this rate).  Sums are fp32 over at most 64 rows and fp64
+// adds those of each bucket in order.  32 rows (16 of fp32) at a time of the
+// slanted strip that the diagonals cut out go to shared memory by 16-byte
+// asynchronous copies, the next ones while these are added (a thread that
+// loaded its own elements, two bytes each and at odd addresses, reached a
+// third of this rate).  Sums are fp32 over at most 64 rows and fp64
 // beyond; nothing is added in an order that depends on timing.
 #include <math.h>
 #include <atomic>
@@ -30,7 +31,8 @@ constexpr int kRelMaxBuckets = 512;
 constexpr int kRelCols = 1024;   // columns of a forward block
 constexpr int kRelRows = 64;     // most rows of a block
 constexpr int kRelDiag = 512;    // diagonals of a block in the backward pass
-constexpr int kRelStage = 32;    // rows that are staged at a time
+template <typename T>
+constexpr int kRelStage = 64 / (int)sizeof(T);  // rows that are staged at a time
 constexpr int kRelInf = 1 << 30;
 
 struct RelMap {  // bucket b holds r in [lo[b], hi[b]] (empty where lo > hi)
@@ -84,17 +86,24 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, int bytes) {  // zeros behind `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+
 // grid: (segments of the rows) x (tiles of 512 diagonals) x (B * H); part:
 // [B*H][tiles][segments][nb].  FLAT: unit stride along the keys.
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256)
     rel_bias_bwd_kernel(const __grid_constant__ RelMap map, const T* __restrict__ grad, int64_t sb, int64_t sh,
                         int64_t si, int64_t sj, double* __restrict__ part, int H, int Lq, int Lk, int q_offset) {
-  constexpr int V = 16 / sizeof(T);            // elements of a 16-byte load
+  constexpr int V = 16 / sizeof(T);            // elements of a 16-byte copy
   constexpr int kVecs = kRelDiag / V + 1;      // of a row's strip, wherever it begins
   constexpr int kPitch = (kVecs + 1) * V;
+  constexpr int kRows = kRelStage<T>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  T* stage = reinterpret_cast<T*>(smem_raw);   // [32][kPitch]
+  T* stages = reinterpret_cast<T*>(smem_raw);  // [2][kRows][kPitch]
   __shared__ double diag[kRelDiag];
   const int seg = blockIdx.x, tile = blockIdx.y;
   const int64_t z = blockIdx.z;
@@ -110,34 +119,26 @@ __global__ void __launch_bounds__(256)
   // further it is si + 1 elements more
   const int lead0 = (int)(((uintptr_t)(g + (int64_t)i0 * si + d0 + i0) & 15) / sizeof(T));
   const int lead_step = (int)((si + 1) & (V - 1));
-  double acc0 = 0.0, acc1 = 0.0;
-  float s0 = 0.f, s1 = 0.f;
-  int held = 0;
-  for (int i = i0; i < i1; i += kRelStage) {
-    const int rows = min(kRelStage, i1 - i);
-    __syncthreads();  // the stage before has been added up
-    // row r: columns c0 + r .. c0 + r + 511, from the 16-byte boundary before
+
+  // row i + r: columns d0 + i + r .., 512 of them, from the 16-byte boundary before
+  auto fetch = [&](int i) {
+    T* stage = stages + ((i - i0) / kRows & 1) * kRows * kPitch;
+    const int rows = min(kRows, i1 - i);
     if (FLAT) {
-      // a warp takes every eighth row, a lane every 32nd vector
-#pragma unroll
-      for (int rr = 0; rr < kRelStage; rr += 8) {
-        const int r = rr + warp;
-        if (r >= rows) continue;
+      for (int r = warp; r < rows; r += 8) {
         const T* row = g + (int64_t)(i + r) * si;
         const int c0 = d0 + i + r - ((lead0 + (i - i0 + r) * lead_step) & (V - 1));
 #pragma unroll
         for (int kk = 0; kk < kVecs; kk += 32) {
           const int k = kk + lane, c = c0 + k * V;
           if (k >= kVecs) continue;
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (c >= 0 && c + V <= Lk) {
-            x = *reinterpret_cast<const uint4*>(row + c);
-          } else if (c + V > 0 && c < Lk) {
-            T* e = reinterpret_cast<T*>(&x);
-            for (int j = 0; j < V; ++j)
-              if (c + j >= 0 && c + j < Lk) e[j] = row[c + j];
+          T* to = stage + r * kPitch + k * V;
+          if (c >= 0 || c + V <= 0) {
+            const int n = c < 0 ? 0 : max(0, min(V, Lk - c));
+            copy_async16(to, n ? row + c : row, n * (int)sizeof(T));
+          } else {  // begins before the row
+            for (int j = 0; j < V; ++j) to[j] = c + j >= 0 && c + j < Lk ? row[c + j] : from_f32<T>(0.f);
           }
-          *reinterpret_cast<uint4*>(stage + r * kPitch + k * V) = x;
         }
       }
     } else {
@@ -145,6 +146,21 @@ __global__ void __launch_bounds__(256)
         const int r = q / kRelDiag, k = q - r * kRelDiag, c = d0 + i + r + k;
         stage[r * kPitch + k] = c >= 0 && c < Lk ? g[(int64_t)(i + r) * si + (int64_t)c * sj] : from_f32<T>(0.f);
       }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  double acc0 = 0.0, acc1 = 0.0;
+  float s0 = 0.f, s1 = 0.f;
+  int held = 0;
+  if (i0 < i1) fetch(i0);
+  for (int i = i0; i < i1; i += kRows) {
+    const int rows = min(kRows, i1 - i);
+    if (i + kRows < i1) {
+      fetch(i + kRows);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     __syncthreads();
     if (held + rows > 64) {
@@ -154,21 +170,23 @@ __global__ void __launch_bounds__(256)
       held = 0;
     }
     held += rows;
+    const T* stage = stages + ((i - i0) / kRows & 1) * kRows * kPitch + e0;
     const int l0 = FLAT ? lead0 + (i - i0) * lead_step : 0;
-    if (rows == kRelStage) {
+    if (rows == kRows) {
 #pragma unroll
-      for (int r = 0; r < kRelStage; ++r) {
-        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0) + e0;
+      for (int r = 0; r < kRows; ++r) {
+        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0);
         s0 += to_f32(x[0]);
         s1 += to_f32(x[256]);
       }
     } else {
       for (int r = 0; r < rows; ++r) {
-        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0) + e0;
+        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0);
         s0 += to_f32(x[0]);
         s1 += to_f32(x[256]);
       }
     }
+    __syncthreads();  // the stage may be filled again
   }
   diag[e0] = acc0 + (double)s0;
   diag[e0 + 256] = acc1 + (double)s1;
@@ -272,7 +290,7 @@ static RelBwdPlan rel_bwd_plan(const pvb2_relative_bias_desc* d, int64_t B) {
   RelBwdPlan p;
   p.tiles = cdiv(d->Lq + d->Lk - 1, kRelDiag);
   const int64_t want = cdiv(8 * (int64_t)num_sms(), std::max<int64_t>(1, B * d->H * p.tiles));
-  p.segments = std::max<int64_t>(1, std::min(want, cdiv(d->Lq, kRelStage)));
+  p.segments = std::max<int64_t>(1, std::min(want, cdiv(d->Lq, 32)));
   return p;
 }
 
@@ -297,9 +315,9 @@ static int rel_bwd(const pvb2_relative_bias_desc* d, const RelMap& m, const pvb2
   if (B > 0 && d->Lq > 0 && d->Lk > 0) {
     PVB2_CHECK_ARG(B * d->H <= 65535 && p.tiles <= 65535, "relative bias: batch x heads or lengths out of range");
     per_z = p.tiles * p.segments;
-    constexpr int smem = kRelStage * (kRelDiag + 2 * 16 / (int)sizeof(T)) * (int)sizeof(T);
+    constexpr int smem = 2 * kRelStage<T> * (kRelDiag + 2 * 16 / (int)sizeof(T)) * (int)sizeof(T);
     static std::atomic<uint64_t> attr_done{0};
-    if (smem > 40 * 1024 && first_on_device(attr_done)) {
+    if (first_on_device(attr_done)) {
       PVB2_CUDA_TRY(cudaFuncSetAttribute(rel_bias_bwd_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
       PVB2_CUDA_TRY(cudaFuncSetAttribute(rel_bias_bwd_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     }
