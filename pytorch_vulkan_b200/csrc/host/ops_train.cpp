@@ -137,10 +137,26 @@ static const at::Tensor& py_tensor(PyObject* o, const char* what) {
   return THPVariable_Unpack(o);
 }
 
+// a key of a state's dict, made once
+struct StateKey {
+  const char* name;
+  PyObject* key;
+  explicit StateKey(const char* n) : name(n), key(PyUnicode_InternFromString(n)) {}
+};
+
 struct AdamState {  // of one parameter
   PyObject* dict;
-  const at::Tensor& get(const char* key) const { return py_tensor(PyDict_GetItemString(dict, key), key); }
+  const at::Tensor& get(const StateKey& k) const { return py_tensor(PyDict_GetItemWithError(dict, k.key), k.name); }
 };
+
+struct StateKeys {
+  StateKey step{"step"}, exp_avg{"exp_avg"}, exp_avg_sq{"exp_avg_sq"}, exp_avg_code{"exp_avg_code"},
+      exp_avg_rms_code{"exp_avg_rms_code"}, exp_avg_scale{"exp_avg_scale"}, exp_avg_rms_scale{"exp_avg_rms_scale"};
+};
+static const StateKeys& state_keys() {
+  static const StateKeys* keys = new StateKeys;  // outlives the interpreter's objects
+  return *keys;
+}
 
 // undefined state: an empty or a missing dict
 static bool adam_state(const pybind11::dict& state, PyObject* p, AdamState* s) {
@@ -160,11 +176,12 @@ static void* adam_held(const at::Tensor& x, const at::Tensor& p, c10::ScalarType
 
 // the pointers of a parameter's 8-bit moments
 static void adam_codes(const AdamState& s, const at::Tensor& p, pvb2_adamw_tensor& t) {
+  const StateKeys& keys = state_keys();
   const int64_t n = p.numel(), blocks = (n + 255) / 256;
-  t.exp_avg = adam_held(s.get("exp_avg_code"), p, at::kByte, n, true, "exp_avg_code");
-  t.exp_avg_sq = adam_held(s.get("exp_avg_rms_code"), p, at::kByte, n, true, "exp_avg_rms_code");
-  t.exp_avg_scale = (float*)adam_held(s.get("exp_avg_scale"), p, at::kFloat, blocks, true, "exp_avg_scale");
-  t.exp_avg_sq_scale = (float*)adam_held(s.get("exp_avg_rms_scale"), p, at::kFloat, blocks, true, "exp_avg_rms_scale");
+  t.exp_avg = adam_held(s.get(keys.exp_avg_code), p, at::kByte, n, true, "exp_avg_code");
+  t.exp_avg_sq = adam_held(s.get(keys.exp_avg_rms_code), p, at::kByte, n, true, "exp_avg_rms_code");
+  t.exp_avg_scale = (float*)adam_held(s.get(keys.exp_avg_scale), p, at::kFloat, blocks, true, "exp_avg_scale");
+  t.exp_avg_sq_scale = (float*)adam_held(s.get(keys.exp_avg_rms_scale), p, at::kFloat, blocks, true, "exp_avg_rms_scale");
 }
 
 // One step of pytorch_vulkan_b200.optim.AdamW over the parameters of a group
@@ -214,10 +231,10 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
       if (codes) {
         adam_codes(states[i], p, t);
       } else {
-        t.exp_avg = adam_held(states[i].get("exp_avg"), p, at::kFloat, t.numel, false, "exp_avg");
-        t.exp_avg_sq = adam_held(states[i].get("exp_avg_sq"), p, at::kFloat, t.numel, false, "exp_avg_sq");
+        t.exp_avg = adam_held(states[i].get(state_keys().exp_avg), p, at::kFloat, t.numel, false, "exp_avg");
+        t.exp_avg_sq = adam_held(states[i].get(state_keys().exp_avg_sq), p, at::kFloat, t.numel, false, "exp_avg_sq");
       }
-      t.step = step_ptr(states[i].get("step"), dev, i);
+      t.step = step_ptr(states[i].get(state_keys().step), dev, i);
       ts.push_back(t);
     }
     pvb2_adamw_desc d;

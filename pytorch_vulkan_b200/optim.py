@@ -74,8 +74,8 @@ class AdamW(torch.optim.Optimizer):
                                      device=p.device)
         return state
 
-    @torch.no_grad()
     def step(self, closure=None):
+        # (no graph is recorded below: the update is no torch operation)
         loss = None
         if closure is not None:
             with torch.enable_grad():
