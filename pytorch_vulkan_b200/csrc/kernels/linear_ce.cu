@@ -5,8 +5,8 @@
 //   G_ij  = g_i (exp(z_ij - lse_i) - (1 - s) [j = t(i)] - s / V)
 //   dx = G w     dw = G^T x     db = sum_i G_i
 //
-// Forward: one matrix product whose epilogue keeps, per row and half tile of
-// 128 columns, the largest logit, the sum of exp(z - largest) and the target's
+// Forward: one matrix product whose epilogue keeps, per row and 64
+// columns, the largest logit, the sum of exp(z - largest) and the target's
 // logit; a second launch joins them.  The logits never leave the chip.
 // Backward: per piece of the vocabulary, the logits are formed again and their
 // epilogue writes G in 16 bits (piece x tokens, sized to stay near the L2
@@ -31,18 +31,26 @@ namespace pvb2 {
 
 constexpr int kLBM = 256;  // rows of a tile: 128 for each CTA of a pair
 constexpr int kLBK = 64;
-constexpr int kLProducers = 4, kLMmaWarp = 4, kLEpiWarps = 8;
-constexpr int kLThreads = (kLProducers + 1 + kLEpiWarps) * 32;
+// Warps: three issue loads, one the products, the others run the epilogue.  12
+// or 20 in all: an SM's four schedulers hold 16384 registers each, and one more
+// warp would cost the others a quarter of theirs.
+constexpr int kLProducers = 3, kLMmaWarp = 3;
 
-// P planes of each operand a stage; this CTA's 128 rows of A and BN / 2 columns of B
+// P planes of each operand a stage; this CTA's 128 rows of A and BN / 2 columns
+// of B.  An epilogue warp takes 32 rows and 64 columns: 16 of them for 256
+// columns (with 8, two for each scheduler, an epilogue of exponentials took
+// twice as long as the products of a K of 1000).
 template <int P, int BN>
 struct LceSmem {
+  static constexpr int EPI_WARPS = BN / 16;
+  static constexpr int THREADS = (kLProducers + 1 + EPI_WARPS) * 32;
+  static constexpr int COLS = 64;
   static constexpr int A_BYTES = 128 * kLBK * 2;
   static constexpr int B_BYTES = BN / 2 * kLBK * 2;
   static constexpr int STAGE_BYTES = P * (A_BYTES + B_BYTES);
-    static constexpr int STAGES = (192 * 1024) / STAGE_BYTES;
+    static constexpr int STAGES = (224 * 1024 - EPI_WARPS * 4096) / STAGE_BYTES;
   static constexpr int EPI_OFF = STAGES * STAGE_BYTES;  // one 4 KB store box per epilogue warp
-  static constexpr int BAR_OFF = EPI_OFF + kLEpiWarps * 4096;
+  static constexpr int BAR_OFF = EPI_OFF + EPI_WARPS * 4096;
   static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16;
 };
 
@@ -74,7 +82,7 @@ struct LceGemm {
   const int64_t* target;
   int64_t V, ignore;
   float smoothing;
-  float2* part;           // kEpiStats: [2 column tiles][part_ld]
+  float2* part;           // kEpiStats: [64-column groups][part_ld]
   float* zsum;            // kEpiStats with smoothing: sums of z, laid out as part
   float* ztarget;
   int64_t part_ld;
@@ -191,16 +199,15 @@ __device__ __forceinline__ constexpr int lce_pb(int i) {
 // 2^-24 of itself for every 16 of them.  The small products of split operands
 // go to an accumulator of their own, which takes the whole of K.
 template <int EPI, typename T, int P, int BN, int CHUNK>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THREADS), 1)
     lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ LceGemm p, int a_mn, int b_mn) {
   using L = LceSmem<P, BN>;
   constexpr bool kPrecise = P > 1;
   constexpr int kPairs = LcePairs<P>::N;
-  constexpr int kCols = BN / 2;             // columns of an epilogue warp
+  constexpr int kCols = L::COLS;            // columns of an epilogue warp
   constexpr int kStages = L::STAGES;
   constexpr int kIssuers = kStages < kLProducers ? kStages : kLProducers;
-  static_assert(CHUNK == 0 || kCols == 64, "chunked sums are held in 64 registers");
   static_assert(CHUNK > 0 || P == 1, "split operands are summed in chunks");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -225,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * kLEpiWarps);
+      mbar_init(&acc_empty[b], 2 * L::EPI_WARPS);
     }
     *abort = 0;
     fence_barrier_init();
@@ -256,7 +263,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
       for (int tile = pair; tile < total_tiles && !*abort; tile += pairs) {
         int mb, nb, sp, kb0, kb1;
         place(tile, mb, nb, sp, kb0, kb1);
-        const int am = mb * kLBM + rank * 128, bn = nb * BN + rank * kCols;
+        const int am = mb * kLBM + rank * 128, bn = nb * BN + rank * (BN / 2);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % kStages;
           if (s % kIssuers != warp) continue;
@@ -278,7 +285,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
               tma_load_3d_pair(sb + z * L::B_BYTES, &tmB, bar, kb * kLBK, p.b_row0 + bn, z);
             } else {
 #pragma unroll
-              for (int j = 0; j < kCols / 64; ++j)
+              for (int j = 0; j < BN / 128; ++j)
                 tma_load_3d_pair(sb + z * L::B_BYTES + j * 8192, &tmB, bar, bn + 64 * j, p.b_row0 + kb * kLBK, z);
             }
           }
@@ -335,8 +342,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
       }
     }
   } else if (warp > kLMmaWarp) {
-    // ------------------------------------------------- epilogue: TMEM lane quarter warp % 4, column half (warp - 5) / 4
-    const int quarter = warp & 3, half = (warp - kLMmaWarp - 1) >> 2;
+    // ------------------------------------------------- epilogue: TMEM lane quarter warp % 4, 64 columns (warp - 4) / 4
+    const int quarter = warp & 3, group = (warp - kLMmaWarp - 1) >> 2;
     uint8_t* box = smem + L::EPI_OFF + (warp - kLMmaWarp - 1) * 4096;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     uint32_t chunk = 0;
@@ -346,7 +353,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
       place(tile, mb, nb, sp, kb0, kb1);
       const int m0 = mb * kLBM + rank * 128 + quarter * 32, m = m0 + lane;
       const bool mrow = m < p.M;
-      const int nh = nb * BN + half * kCols;  // first column of this warp
+      const int nh = nb * BN + group * kCols;  // first column of this warp
       int t = INT32_MIN;  // column of the row's target
       float row_lse = 0.f, row_g = 0.f;
       if (EPI == kEpiStats || EPI == kEpiGrad) {
@@ -376,11 +383,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float u[32];
-            tmem_ld32(tmem_base + lanes + buf * BN + half * kCols + 32 * h, u);
+            tmem_ld32(tmem_base + lanes + buf * BN + group * kCols + 32 * h, u);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[32 * h + j] += u[j];
             if (kPairs > 1 && c0 + CHUNK >= kb1) {
-              tmem_ld32(tmem_base + lanes + (2 + (local & 1)) * BN + half * kCols + 32 * h, u);
+              tmem_ld32(tmem_base + lanes + (2 + (local & 1)) * BN + group * kCols + 32 * h, u);
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[32 * h + j] += u[j];
             }
@@ -394,14 +401,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
         tc_fence_after();
       }
       if (!ok) break;
-#pragma unroll 1
-      for (int c = 0; c < kCols / 64; ++c) {  // 64 columns at a time
-        const int n0 = nh + c * 64;
-        if (n0 >= p.N) break;
+      const int n0 = nh;
+      if (n0 < p.N) {
         if (CHUNK == 0) {
-          const uint32_t ta = tmem_base + lanes + (chunk & 1) * BN + half * kCols + c * 64;
+          const uint32_t ta = tmem_base + lanes + (chunk & 1) * BN + group * kCols;
           tmem_ld32(ta, v);
           tmem_ld32(ta + 32, v + 32);
+          // the accumulator is free: the values are in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[chunk & 1]));
         }
         // whether any of the warp's targets is among these columns
         const bool has_target = (EPI == kEpiStats || EPI == kEpiGrad) &&
@@ -534,9 +543,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
         if (p.zsum) p.zsum[at] = zs;
       }
       if (CHUNK == 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[chunk & 1]));
+        if (n0 >= p.N) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[chunk & 1]));
+        }
         ++chunk;
       }
     }
@@ -563,34 +573,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLThreads, 1)
 // src [rows][cols] (row stride ld) -> planes [P][rows][ldp] of T, columns
 // from cols to ldp zero; rows without a loss become zeros when `target` is
 // given (what they hold, NaN among it, then has no part in a product)
+template <typename S>
+struct LcePackJob {
+  const S* src;
+  int64_t rows, ld;
+  uint16_t* dst;
+  const int64_t* target;  // or NULL
+  int vec;
+};
+
+// what each row's gradient is multiplied by, where that is one number for all
+// rows (mean and sum): row[i] is 1 or 0, and one factor for all results
+struct LceRowsJob {
+  float* row;             // NULL: nothing to do
+  float* factor;
+  const float *grad_out, *count;
+  const int64_t* target;
+  int64_t N;
+  int mean;
+  float inv_gscale;
+};
+
 template <typename S, typename T>
-__global__ void lce_pack_kernel(const S* __restrict__ src, int64_t rows, int64_t cols, int64_t ld, T* __restrict__ dst,
-                                int64_t ldp, int planes, const int64_t* __restrict__ target, int64_t V, int64_t ignore,
-                                int vec) {
-  const int per_row = (int)(ldp / 8);  // eight columns a thread
-  const int64_t total = rows * per_row, plane = rows * ldp;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = total <= INT32_MAX ? (int64_t)((int)e / per_row) : e / per_row;
-    const int64_t c = (e - r * per_row) * 8;
-    float v[8];
-    if (vec && c + 8 <= cols) {
-      load_vec<8>(src + r * ld + c, v);
-    } else {
+__device__ __forceinline__ void lce_pack_one(const LcePackJob<S>& j, int64_t e, int per_row, int64_t cols, int64_t ldp,
+                                             int planes, int64_t V, int64_t ignore) {
+  const int64_t r = e <= INT32_MAX ? (int64_t)((int)e / per_row) : e / per_row;
+  const int64_t c = (e - r * per_row) * 8, plane = j.rows * ldp;
+  float v[8];
+  if (j.vec && c + 8 <= cols) {
+    load_vec<8>(j.src + r * j.ld + c, v);
+  } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(src[r * ld + c + k]) : 0.f;
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(j.src[r * j.ld + c + k]) : 0.f;
+  }
+  if (j.target && !lce_scored(j.target[r], V, ignore)) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.f;
+  }
+  T* dst = reinterpret_cast<T*>(j.dst) + r * ldp + c;
+  for (int z = 0; z < planes; ++z) {
+    store_vec<8>(dst + z * plane, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      // infinity is its first part alone
+      const float h = to_f32(from_f32<T>(v[k]));
+      v[k] = isinf(h) ? 0.f : v[k] - h;
     }
-    if (target && !lce_scored(target[r], V, ignore)) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.f;
-    }
-    for (int z = 0; z < planes; ++z) {
-      store_vec<8>(dst + z * plane + r * ldp + c, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        // infinity is its first part alone
-        const float h = to_f32(from_f32<T>(v[k]));
-        v[k] = isinf(h) ? 0.f : v[k] - h;
-      }
+  }
+}
+
+// one or two operands of the same row length (eight columns a thread), and
+// the rows' factors with them
+template <typename S, typename T>
+__global__ void lce_pack_kernel(LcePackJob<S> a, LcePackJob<S> b, LceRowsJob rj, int64_t cols, int64_t ldp, int planes,
+                                int64_t V, int64_t ignore) {
+  const int per_row = (int)(ldp / 8);
+  const int64_t na = a.rows * per_row, total = na + b.rows * per_row;
+  const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t e = first; e < total; e += step) {
+    if (e < na) lce_pack_one<S, T>(a, e, per_row, cols, ldp, planes, V, ignore);
+    else lce_pack_one<S, T>(b, e - na, per_row, cols, ldp, planes, V, ignore);
+  }
+  if (rj.row) {
+    for (int64_t i = first; i < rj.N; i += step) rj.row[i] = lce_scored(rj.target[i], V, ignore) ? 1.f : 0.f;
+    if (first == 0) {
+      float f = *rj.grad_out;
+      if (rj.mean) f = *rj.count > 0.f ? f / *rj.count : 0.f;
+      *rj.factor = f * rj.inv_gscale;
     }
   }
 }
@@ -600,9 +649,8 @@ __global__ void lce_pack_kernel(const S* __restrict__ src, int64_t rows, int64_t
 __global__ void __launch_bounds__(1024)
     lce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zsum, int64_t part_ld, int parts,
                     const float* __restrict__ ztarget, const int64_t* __restrict__ target, int64_t N, int64_t V,
-                    int64_t ignore, float smoothing, float* __restrict__ lse, float* __restrict__ loss,
-                    int total_of, float* __restrict__ out, float* __restrict__ count) {
-  __shared__ float sm[32][33], ss[32][33], sz[32][33], sl[32];
+                    int64_t ignore, float smoothing, float* __restrict__ lse, float* __restrict__ loss) {
+  __shared__ float sm[32][33], ss[32][33], sz[32][33];
   const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t i = (int64_t)blockIdx.x * 32 + r;
   float mx = -INFINITY, sum = 0.f, zs = 0.f;
@@ -641,20 +689,66 @@ __global__ void __launch_bounds__(1024)
       if (smoothing != 0.f) v = (1.f - smoothing) * v + smoothing * (l - zs / (float)V);
     }
     loss[row] = v;
-    sl[g] = v;
   }
-  if (total_of < 0) return;
-  // all rows are in this block: their total (reduction total_of) as well
+}
+
+// the same for at most 8 rows, a warp each, with their total: the parts of a
+// row are all on their way at once
+__global__ void __launch_bounds__(256)
+    lce_few_join_kernel(const float2* __restrict__ part, const float* __restrict__ zsum, int parts,
+                        const float* __restrict__ ztarget, const int64_t* __restrict__ target, int N, int64_t V,
+                        int64_t ignore, float smoothing, int reduction, float* __restrict__ lse,
+                        float* __restrict__ loss, float* __restrict__ out, float* __restrict__ count) {
+  __shared__ float sl[8];
+  const int i = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (i < N) {
+    float mx = -INFINITY, sum = 0.f, zs = 0.f;
+    for (int q0 = 0; q0 < parts; q0 += 32 * 10) {
+      float2 v[10];
+#pragma unroll
+      for (int k = 0; k < 10; ++k) {
+        const int q = q0 + k * 32 + lane;
+        v[k] = q < parts ? part[q * N + i] : make_float2(-INFINITY, 0.f);
+        if (zsum && q < parts) zs += zsum[q * N + i];
+      }
+      float nm = mx;
+#pragma unroll
+      for (int k = 0; k < 10; ++k) nm = fmaxf(nm, v[k].x);
+      const float base = nm == -INFINITY ? 0.f : nm;
+      sum *= expf(mx - base);
+#pragma unroll
+      for (int k = 0; k < 10; ++k) sum += v[k].y * expf(v[k].x - base);
+      mx = nm;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, mx, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
+      const float nm = fmaxf(mx, om), base = nm == -INFINITY ? 0.f : nm;
+      sum = sum * expf(mx - base) + os * expf(om - base);
+      mx = nm;
+      zs += __shfl_xor_sync(0xffffffffu, zs, o);
+    }
+    if (lane == 0) {
+      const float l = (mx == -INFINITY ? 0.f : mx) + logf(sum);
+      lse[i] = l;
+      float v = 0.f;
+      if (lce_scored(target[i], V, ignore)) {
+        v = l - ztarget[i];
+        if (smoothing != 0.f) v = (1.f - smoothing) * v + smoothing * (l - zs / (float)V);
+      }
+      loss[i] = v;
+      sl[i] = v;
+    }
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     double all = 0.0;
     int n = 0;
-    for (int q = 0; q < (int)N; ++q) {
+    for (int q = 0; q < N; ++q) {
       all += (double)sl[q];
       n += lce_scored(target[q], V, ignore) ? 1 : 0;
     }
     *count = (float)n;
-    if (total_of != PVB2_LOSS_NONE) *out = (float)(total_of == PVB2_LOSS_MEAN ? all / (double)n : all);
+    if (reduction != PVB2_LOSS_NONE) *out = (float)(reduction == PVB2_LOSS_MEAN ? all / (double)n : all);
   }
 }
 
@@ -974,40 +1068,29 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// what each row's gradient is multiplied by: row[i] in [-1, 1] and one factor
-// for all results
+// the rows' factors where each has a gradient of its own: g_i / max |g| and
+// that maximum
 __global__ void __launch_bounds__(1024)
-    lce_grad_rows_kernel(const float* __restrict__ grad_out, const float* __restrict__ count,
-                         const int64_t* __restrict__ target, int64_t N, int64_t V, int64_t ignore, int reduction,
-                         float inv_gscale, float* __restrict__ row, float* __restrict__ factor) {
+    lce_grad_rows_kernel(const float* __restrict__ grad_out, const int64_t* __restrict__ target, int64_t N, int64_t V,
+                         int64_t ignore, float inv_gscale, float* __restrict__ row, float* __restrict__ factor) {
   __shared__ float s_max[32];
-  float scale;
-  if (reduction == PVB2_LOSS_NONE) {
-    float mx = 0.f;
-    for (int64_t i = threadIdx.x; i < N; i += 1024)
-      if (lce_scored(target[i], V, ignore)) {
-        const float a = fabsf(grad_out[i]);
-        mx = (a > mx || a != a) ? a : mx;
-      }
-    for (int o = 16; o > 0; o >>= 1) {
-      const float a = __shfl_xor_sync(0xffffffffu, mx, o);
+  float mx = 0.f;
+  for (int64_t i = threadIdx.x; i < N; i += 1024)
+    if (lce_scored(target[i], V, ignore)) {
+      const float a = fabsf(grad_out[i]);
       mx = (a > mx || a != a) ? a : mx;
     }
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
-    __syncthreads();
-    mx = s_max[0];
-    for (int w = 1; w < 32; ++w) mx = (s_max[w] > mx || s_max[w] != s_max[w]) ? s_max[w] : mx;
-    scale = mx;
-  } else {
-    scale = *grad_out;
-    if (reduction == PVB2_LOSS_MEAN) scale = *count > 0.f ? scale / *count : 0.f;
+  for (int o = 16; o > 0; o >>= 1) {
+    const float a = __shfl_xor_sync(0xffffffffu, mx, o);
+    mx = (a > mx || a != a) ? a : mx;
   }
-  for (int64_t i = threadIdx.x; i < N; i += 1024) {
-    float g = 0.f;
-    if (lce_scored(target[i], V, ignore)) g = reduction == PVB2_LOSS_NONE ? (scale != 0.f ? grad_out[i] / scale : 0.f) : 1.f;
-    row[i] = g;
-  }
-  if (threadIdx.x == 0) *factor = scale * inv_gscale;
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
+  __syncthreads();
+  mx = s_max[0];
+  for (int w = 1; w < 32; ++w) mx = (s_max[w] > mx || s_max[w] != s_max[w]) ? s_max[w] : mx;
+  for (int64_t i = threadIdx.x; i < N; i += 1024)
+    row[i] = lce_scored(target[i], V, ignore) && mx != 0.f ? grad_out[i] / mx : 0.f;
+  if (threadIdx.x == 0) *factor = mx * inv_gscale;
 }
 
 // out [rows][cols] = factor * sum of S slabs [rows][ld], four columns a thread
@@ -1042,9 +1125,10 @@ __global__ void lce_join_kernel(const float* __restrict__ slab, int S, int64_t r
 
 // column sums of G (planes added): 32 columns and 32 rows at a time, partial
 // sums per part of the rows first, then in order
-template <typename T>
+template <typename T, typename O>
 __global__ void __launch_bounds__(1024) lce_colsum_kernel(const T* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
-                                                         int planes, int64_t rows_per, float* __restrict__ part) {
+                                                         int planes, int64_t rows_per, float* __restrict__ part,
+                                                         const float* __restrict__ factor, O* __restrict__ out) {
   __shared__ float s[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + c;
@@ -1060,7 +1144,8 @@ __global__ void __launch_bounds__(1024) lce_colsum_kernel(const T* __restrict__ 
   __syncthreads();
   if (g == 0 && col < cols) {
     for (int q = 1; q < 32; ++q) sum += s[q][c];
-    part[blockIdx.y * cols + col] = sum;
+    if (gridDim.y == 1) out[col] = from_f32<O>(sum * *factor);  // there is one part
+    else part[blockIdx.y * cols + col] = sum;
   }
 }
 
@@ -1142,7 +1227,7 @@ static pvb2_linear_ce_desc lce_normal(const pvb2_linear_ce_desc* d) {
   return n;
 }
 
-static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
+static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
   LcePlan p;
   p.half = d->dtype == PVB2_F16;
   p.P = d->dtype != PVB2_F32 ? 1 : d->math == PVB2_MATH_FP32 ? 3 : 2;
@@ -1186,6 +1271,38 @@ static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   p.colsum_parts = (int)std::min<int64_t>(64, cdiv(d->N, 512));
   p.rows_per = p.colsum_parts ? up(cdiv(d->N, p.colsum_parts), 8) : 0;
   return p;
+}
+
+// The plan of a call is asked for several times over (memory to keep,
+// workspace, launch): the last ones of this thread, by all that they depend
+// on.
+static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
+  struct Made {
+    int64_t N = -1, D, V, ldw, kept;
+    int32_t dtype, math, sms;
+    bool backward;
+    LcePlan plan;
+  };
+  static thread_local Made made[4];
+  static thread_local int next = 0;
+  const int sms = num_sms();
+  for (const Made& m : made)
+    if (m.N == d->N && m.D == d->D && m.V == d->V && m.ldw == d->ldw && m.kept == d->kept && m.dtype == d->dtype &&
+        m.math == d->math && m.sms == sms && m.backward == backward)
+      return m.plan;
+  Made& m = made[next];
+  next = (next + 1) % 4;
+  m.N = d->N;
+  m.D = d->D;
+  m.V = d->V;
+  m.ldw = d->ldw;
+  m.kept = d->kept;
+  m.dtype = d->dtype;
+  m.math = d->math;
+  m.sms = sms;
+  m.backward = backward;
+  m.plan = lce_make_plan(d, backward);
+  return m.plan;
 }
 
 // places in the workspace, 1024-byte aligned
@@ -1243,7 +1360,7 @@ static bool lce_kept_fp32(const pvb2_linear_ce_desc* d) {
 static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceFwdSpace* s) {
   Arena a{(uint8_t*)base};
   const int64_t rows = std::min(d->N, kLRowsFwd);
-  const int64_t parts = p.few ? lce_few_blocks(d) : cdiv(up(d->V, 256), p.z.bn / 2);
+  const int64_t parts = p.few ? lce_few_blocks(d) : up(d->V, 256) / 64;
   const bool slabs = lce_slabs(p);
   s->x = a.take<uint16_t>(p.few || lce_direct(d, d->ldx) ? 0 : rows * p.ldp * p.P);
   s->w = a.take<uint16_t>(!p.few && p.pack_w ? p.piece * p.ldp * p.P : 0);
@@ -1341,7 +1458,7 @@ static int lce_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensor
   const int64_t tiles = cdiv(g.M, kLBM) * cdiv(g.N, BN) * g.splits;
   PVB2_CHECK_ARG(tiles < INT32_MAX / 2, "linear cross entropy: too many tiles");
   const int grid = 2 * (int)std::min<int64_t>(tiles, lce_pairs_on_device());
-  kernel<<<grid, kLThreads, smem, s>>>(a, b, c, g, a_mn ? 1 : 0, b_mn ? 1 : 0);
+  kernel<<<grid, LceSmem<P, BN>::THREADS, smem, s>>>(a, b, c, g, a_mn ? 1 : 0, b_mn ? 1 : 0);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -1362,24 +1479,39 @@ static int lce_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMa
   return lce_launch<EPI, __nv_bfloat16, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
 }
 
+struct LceOperand {  // to be packed
+  const void* src = nullptr;
+  int64_t row0 = 0, rows = 0, ld = 0;
+  uint16_t* dst = nullptr;
+  const int64_t* target = nullptr;
+};
+
 template <typename S, typename T>
-static int lce_pack_as(const pvb2_linear_ce_desc* d, const LcePlan& p, const S* src, int64_t rows, int64_t ld,
-                       uint16_t* dst, const int64_t* target, cudaStream_t s) {
-  const int64_t total = rows * (p.ldp / 8);
+static int lce_pack_as(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceOperand& a, const LceOperand& b,
+                       const LceRowsJob& rows, cudaStream_t s) {
+  auto job = [](const LceOperand& o) {
+    const S* src = (const S*)o.src + o.row0 * o.ld;
+    return LcePackJob<S>{src, o.rows, o.ld, o.dst, o.target, ((uintptr_t)src & 15) == 0 && o.ld * sizeof(S) % 16 == 0};
+  };
+  const int64_t total = std::max((a.rows + b.rows) * (p.ldp / 8), rows.row ? rows.N : 0);
   if (total == 0) return PVB2_OK;
-  const int vec = ((uintptr_t)src & 15) == 0 && ld * sizeof(S) % 16 == 0;
-  lce_pack_kernel<S, T><<<grid_for(total, 256), 256, 0, s>>>(src, rows, d->D, ld, (T*)dst, p.ldp, p.P, target, d->V,
-                                                             d->ignore_index, vec);
+  lce_pack_kernel<S, T><<<grid_for(total, 256), 256, 0, s>>>(job(a), job(b), rows, d->D, p.ldp, p.P, d->V,
+                                                             d->ignore_index);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
 
-static int lce_pack(const pvb2_linear_ce_desc* d, const LcePlan& p, const void* src, int64_t row0, int64_t rows,
-                    int64_t ld, uint16_t* dst, const int64_t* target, cudaStream_t s) {
-  if (d->dtype == PVB2_F32)
-    return lce_pack_as<float, __nv_bfloat16>(d, p, (const float*)src + row0 * ld, rows, ld, dst, target, s);
-  if (p.half) return lce_pack_as<__half, __half>(d, p, (const __half*)src + row0 * ld, rows, ld, dst, target, s);
-  return lce_pack_as<__nv_bfloat16, __nv_bfloat16>(d, p, (const __nv_bfloat16*)src + row0 * ld, rows, ld, dst, target, s);
+static int lce_pack(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceOperand& a, const LceOperand& b,
+                    const LceRowsJob& rows, cudaStream_t s) {
+  if (d->dtype == PVB2_F32) return lce_pack_as<float, __nv_bfloat16>(d, p, a, b, rows, s);
+  if (p.half) return lce_pack_as<__half, __half>(d, p, a, b, rows, s);
+  return lce_pack_as<__nv_bfloat16, __nv_bfloat16>(d, p, a, b, rows, s);
+}
+
+static LceRowsJob lce_no_rows() {
+  LceRowsJob r;
+  memset(&r, 0, sizeof(r));
+  return r;
 }
 
 // out = factor * (sum of slabs), as the operands' type
@@ -1519,19 +1651,23 @@ static int lce_slab_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const L
   return PVB2_OK;
 }
 
-template <typename T>
-static int lce_bias_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, int64_t width,
-                         int64_t ldg, void* out, cudaStream_t s) {
+template <typename T, typename O>
+static int lce_bias_grad_as(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, int64_t width,
+                            int64_t ldg, O* out, cudaStream_t s) {
   const dim3 grid((unsigned)cdiv(width, 32), (unsigned)p.colsum_parts);
-  const int blocks = (int)cdiv(width, 256);
-  lce_colsum_kernel<<<grid, 1024, 0, s>>>((const T*)sp.G, d->N, width, ldg, p.P, p.rows_per, sp.colsum);
+  lce_colsum_kernel<<<grid, 1024, 0, s>>>((const T*)sp.G, d->N, width, ldg, p.P, p.rows_per, sp.colsum, sp.factor, out);
   PVB2_LAUNCH_CHECK();
-  if (d->dtype == PVB2_F32)
-    lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (float*)out);
-  else
-    lce_dbias_kernel<<<blocks, 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, (T*)out);
+  if (p.colsum_parts == 1) return PVB2_OK;
+  lce_dbias_kernel<<<(int)cdiv(width, 256), 256, 0, s>>>(sp.colsum, p.colsum_parts, width, sp.factor, out);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
+}
+
+static int lce_bias_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, int64_t width,
+                         int64_t ldg, void* out, cudaStream_t s) {
+  if (d->dtype == PVB2_F32) return lce_bias_grad_as<__nv_bfloat16, float>(d, p, sp, width, ldg, (float*)out, s);
+  if (p.half) return lce_bias_grad_as<__half, __half>(d, p, sp, width, ldg, (__half*)out, s);
+  return lce_bias_grad_as<__nv_bfloat16, __nv_bfloat16>(d, p, sp, width, ldg, (__nv_bfloat16*)out, s);
 }
 
 }  // namespace pvb2
@@ -1564,7 +1700,7 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     const bool direct_x = lce_direct(d, d->ldx), slabs = lce_slabs(p);
     PVB2_TRY(lce_aligned(x, direct_x));
     PVB2_TRY(lce_aligned(w, !p.pack_w));
-    const int parts = p.few ? lce_few_blocks(d) : (int)cdiv(d->V, p.z.bn / 2), esize = d->dtype == PVB2_F32 ? 4 : 2;
+    const int parts = p.few ? lce_few_blocks(d) : (int)cdiv(d->V, 64), esize = d->dtype == PVB2_F32 ? 4 : 2;
     const float smoothing = (float)d->label_smoothing;
     PVB2_CHECK_ARG(d->kept == 0 || (kept && ((uintptr_t)kept & 15) == 0),
                    "linear cross entropy: 16-byte aligned memory for what is kept needed");
@@ -1577,20 +1713,26 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
         if (d->dtype == PVB2_F32) PVB2_TRY(lce_few<float>(d, x, w, bias, target, sp, k, s));
         else if (p.half) PVB2_TRY(lce_few<__half>(d, x, w, bias, target, sp, k, s));
         else PVB2_TRY(lce_few<__nv_bfloat16>(d, x, w, bias, target, sp, k, s));
-      } else if (direct_x) {
+        lce_few_join_kernel<<<1, 256, 0, s>>>(sp.part, smoothing != 0.f ? sp.zsum : nullptr, parts,
+                                              d->kept ? k.ztarget : sp.ztarget, target, (int)d->N, d->V,
+                                              d->ignore_index, smoothing, d->reduction, lse, loss, out, count);
+        PVB2_LAUNCH_CHECK();
+        return PVB2_OK;
+      }
+      if (direct_x) {
         PVB2_TRY(lce_map_a(&ma, (const uint8_t*)x + r0 * d->ldx * esize, d->D, rows, d->ldx, p));
       } else {
-        PVB2_TRY(lce_pack(d, p, x, r0, rows, d->ldx, sp.x, nullptr, s));
         PVB2_TRY(lce_map_a(&ma, sp.x, d->D, rows, p.ldp, p));
       }
-      for (int64_t v0 = 0; v0 < d->V && !p.few; v0 += p.piece) {
+      for (int64_t v0 = 0; v0 < d->V; v0 += p.piece) {
         const int64_t width = std::min(p.piece, d->V - v0);
-        if (!p.pack_w) {
-          PVB2_TRY(lce_map_b(&mb, w, d->D, d->V, d->ldw, p, p.z.bn));
-        } else {
-          PVB2_TRY(lce_pack(d, p, w, v0, width, d->ldw, sp.w, nullptr, s));
-          PVB2_TRY(lce_map_b(&mb, sp.w, d->D, width, p.ldp, p, p.z.bn));
-        }
+        // x goes with the first piece of w
+        LceOperand px, pw;
+        if (!direct_x && v0 == 0) px = LceOperand{x, r0, rows, d->ldx, sp.x, nullptr};
+        if (p.pack_w) pw = LceOperand{w, v0, width, d->ldw, sp.w, nullptr};
+        PVB2_TRY(lce_pack(d, p, px, pw, lce_no_rows(), s));
+        if (!p.pack_w) PVB2_TRY(lce_map_b(&mb, w, d->D, d->V, d->ldw, p, p.z.bn));
+        else PVB2_TRY(lce_map_b(&mb, sp.w, d->D, width, p.ldp, p, p.z.bn));
         LceGemm g = lce_logits(d, bias, rows, v0, width, p.pack_w ? 0 : (int)v0, target + r0);
         if (slabs) {
           PVB2_TRY(lce_slab_logits(d, p, ma, mb, g, sp.slab, s));
@@ -1617,11 +1759,9 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       else
         lce_rows_kernel<<<(int)cdiv(rows, 32), 1024, 0, s>>>(
             sp.part, smoothing != 0.f ? sp.zsum : nullptr, rows, parts, d->kept ? k.ztarget + r0 : sp.ztarget,
-            target + r0, rows, d->V, d->ignore_index, smoothing, lse + r0, loss + r0,
-            !slabs && d->N <= 32 ? d->reduction : -1, out, count);
+            target + r0, rows, d->V, d->ignore_index, smoothing, lse + r0, loss + r0);
       PVB2_LAUNCH_CHECK();
     }
-    if (!slabs && d->N <= 32) return PVB2_OK;
   }
   lce_total_kernel<<<1, 1024, 0, s>>>(loss, target, d->N, d->V, d->ignore_index, d->reduction, out, count);
   PVB2_LAUNCH_CHECK();
@@ -1673,10 +1813,15 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   const bool direct_w = !p.pack_w, slabs = lce_slabs(p);
   PVB2_TRY(lce_aligned(w, direct_w));
   const float gscale = p.half ? 32768.f : 1.f;
-  lce_grad_rows_kernel<<<1, 1024, 0, s>>>(grad_out, count, target, d->N, d->V, d->ignore_index, d->reduction,
-                                          1.f / gscale, sp.row, sp.factor);
-  PVB2_LAUNCH_CHECK();
-  PVB2_TRY(lce_pack(d, p, x, 0, d->N, d->ldx, sp.x, target, s));
+  LceRowsJob rows = lce_no_rows();
+  if (d->reduction == PVB2_LOSS_NONE) {
+    lce_grad_rows_kernel<<<1, 1024, 0, s>>>(grad_out, target, d->N, d->V, d->ignore_index, 1.f / gscale, sp.row,
+                                            sp.factor);
+    PVB2_LAUNCH_CHECK();
+  } else {
+    rows = LceRowsJob{sp.row, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
+  }
+  LceOperand px{x, 0, d->N, d->ldx, sp.x, target};
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;
   PVB2_TRY(lce_map_a(&x_k, sp.x, d->D, d->N, p.ldp, p));
   PVB2_TRY(lce_map_mn(&x_mn, sp.x, d->D, d->N, p.ldp, p));
@@ -1697,10 +1842,16 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       PVB2_TRY(lce_map_b(&w_k, w, d->D, d->V, d->ldw, p, p.z.bn));
       PVB2_TRY(lce_map_mn(&w_mn, w, d->D, d->V, d->ldw, p));
     } else if (dx || !from_kept) {
-      PVB2_TRY(lce_pack(d, p, w, v0, width, d->ldw, sp.w, nullptr, s));
+      PVB2_TRY(lce_pack(d, p, px, LceOperand{w, v0, width, d->ldw, sp.w, nullptr}, rows, s));
+      px = LceOperand();
+      rows = lce_no_rows();
       PVB2_TRY(lce_map_b(&w_k, sp.w, d->D, width, p.ldp, p, p.z.bn));
       PVB2_TRY(lce_map_mn(&w_mn, sp.w, d->D, width, p.ldp, p));
     }
+    // x and the rows' factors, unless they went with w
+    PVB2_TRY(lce_pack(d, p, px, LceOperand(), rows, s));
+    px = LceOperand();
+    rows = lce_no_rows();
     PVB2_TRY(lce_map_a(&g_k, sp.G, width, d->N, ldg, p));
     PVB2_TRY(lce_map_mn(&g_mn, sp.G, width, d->N, ldg, p));
     // G of this piece
@@ -1747,8 +1898,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     }
     if (dbias) {
       void* out = (uint8_t*)dbias + v0 * size;
-      if (p.half) PVB2_TRY(lce_bias_grad<__half>(d, p, sp, width, ldg, out, s));
-      else PVB2_TRY(lce_bias_grad<__nv_bfloat16>(d, p, sp, width, ldg, out, s));
+      PVB2_TRY(lce_bias_grad(d, p, sp, width, ldg, out, s));
     }
   }
   if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, sp.factor, dx, s));
