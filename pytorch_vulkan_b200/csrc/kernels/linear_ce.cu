@@ -1204,6 +1204,7 @@ struct LcePlan {
   bool half;         // fp16 operands (bf16 otherwise)
   int64_t ldp;       // row length of packed operands
   bool pack_w;       // w is packed piece by piece
+  bool pack_x;       // forward: x is packed (the backward pass always does)
   int64_t piece;     // vocabulary entries of a piece
   int pieces;
   LceTiling z, dx, dw;
@@ -1231,8 +1232,14 @@ static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
   LcePlan p;
   p.half = d->dtype == PVB2_F16;
   p.P = d->dtype != PVB2_F32 ? 1 : d->math == PVB2_MATH_FP32 ? 3 : 2;
-  p.ldp = up(d->D, 8);
-  p.pack_w = !lce_direct(d, d->ldw);
+  // packed rows begin on 128-byte lines, unless that would be mostly padding
+  p.ldp = up(d->D, d->D >= 256 ? 64 : 8);
+  // Rows of w that straddle lines take two reads from L2 for each 128 bytes.  A
+  // copy costs the same for any number of tokens and pays from about 3000 on
+  // (D 1000, V 49999, forward: 397 us as it lies and 376 us with the copy at
+  // 4095 tokens, 196 and 244 us at 2048).
+  p.pack_w = !lce_direct(d, d->ldw) || (d->ldw % 64 != 0 && d->D >= 256 && d->N >= 3500);
+  p.pack_x = !lce_direct(d, d->ldx) || (d->ldx % 64 != 0 && d->D >= 256 && d->V >= 2048);
   const int size = d->dtype == PVB2_F32 ? 4 : 2;
   p.few = !backward && d->N <= kLFewRows && (int64_t)kLFewRows * p.ldp * size <= kLFewBytes;
   const int64_t rows = backward ? d->N : std::min(d->N, kLRowsFwd);
@@ -1278,7 +1285,7 @@ static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
 // on.
 static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   struct Made {
-    int64_t N = -1, D, V, ldw, kept;
+    int64_t N = -1, D, V, ldx, ldw, kept;
     int32_t dtype, math, sms;
     bool backward;
     LcePlan plan;
@@ -1287,7 +1294,7 @@ static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   static thread_local int next = 0;
   const int sms = num_sms();
   for (const Made& m : made)
-    if (m.N == d->N && m.D == d->D && m.V == d->V && m.ldw == d->ldw && m.kept == d->kept && m.dtype == d->dtype &&
+    if (m.N == d->N && m.D == d->D && m.V == d->V && m.ldx == d->ldx && m.ldw == d->ldw && m.kept == d->kept && m.dtype == d->dtype &&
         m.math == d->math && m.sms == sms && m.backward == backward)
       return m.plan;
   Made& m = made[next];
@@ -1295,6 +1302,7 @@ static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   m.N = d->N;
   m.D = d->D;
   m.V = d->V;
+  m.ldx = d->ldx;
   m.ldw = d->ldw;
   m.kept = d->kept;
   m.dtype = d->dtype;
@@ -1362,7 +1370,7 @@ static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   const int64_t rows = std::min(d->N, kLRowsFwd);
   const int64_t parts = p.few ? lce_few_blocks(d) : up(d->V, 256) / 64;
   const bool slabs = lce_slabs(p);
-  s->x = a.take<uint16_t>(p.few || lce_direct(d, d->ldx) ? 0 : rows * p.ldp * p.P);
+  s->x = a.take<uint16_t>(!p.few && p.pack_x ? rows * p.ldp * p.P : 0);
   s->w = a.take<uint16_t>(!p.few && p.pack_w ? p.piece * p.ldp * p.P : 0);
   s->slab = a.take<float>(slabs ? p.z.splits * rows * up(d->V, 4) : 0);
   s->part = a.take<float2>(slabs ? 0 : rows * parts);
@@ -1382,7 +1390,7 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   const int64_t ld32 = up(d->D, 4), width = std::min(p.piece, d->V);
   s->x = a.take<uint16_t>(d->N * p.ldp * p.P);
   s->w = a.take<uint16_t>(p.pack_w ? p.piece * p.ldp * p.P : 0);
-  s->G = a.take<uint16_t>(d->N * up(width, 8) * p.P);
+  s->G = a.take<uint16_t>(d->N * up(width, 64) * p.P);
   s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
   s->factor = a.take<float>(1);
@@ -1697,9 +1705,9 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     const size_t need = lce_fwd_space(d, p, (void*)(((uintptr_t)workspace + 1023) & ~(uintptr_t)1023), &sp) + 1024;
     PVB2_CHECK_ARG(workspace && workspace_bytes >= need, "linear cross entropy: workspace of %zu bytes needed", need);
     if (d->reduction != PVB2_LOSS_NONE) loss = sp.loss;
-    const bool direct_x = lce_direct(d, d->ldx), slabs = lce_slabs(p);
-    PVB2_TRY(lce_aligned(x, direct_x));
-    PVB2_TRY(lce_aligned(w, !p.pack_w));
+    const bool direct_x = !p.pack_x, slabs = lce_slabs(p);
+    PVB2_TRY(lce_aligned(x, direct_x && !p.few));
+    PVB2_TRY(lce_aligned(w, !p.pack_w && !p.few));
     const int parts = p.few ? lce_few_blocks(d) : (int)cdiv(d->V, 64), esize = d->dtype == PVB2_F32 ? 4 : 2;
     const float smoothing = (float)d->label_smoothing;
     PVB2_CHECK_ARG(d->kept == 0 || (kept && ((uintptr_t)kept & 15) == 0),
@@ -1804,6 +1812,8 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     return PVB2_OK;
   }
   PVB2_CHECK_ARG(x && w && target && lse && count && grad_out, "linear cross entropy backward: null pointer");
+  PVB2_CHECK_ARG(d->kept == 0 || (kept && ((uintptr_t)kept & 15) == 0),
+                 "linear cross entropy backward: what the forward pass kept is missing");
   if (!dx && !dw && !dbias) return PVB2_OK;
   const LcePlan p = lce_plan(d, true);
   LceBwdSpace sp;
@@ -1825,8 +1835,6 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;
   PVB2_TRY(lce_map_a(&x_k, sp.x, d->D, d->N, p.ldp, p));
   PVB2_TRY(lce_map_mn(&x_mn, sp.x, d->D, d->N, p.ldp, p));
-  PVB2_CHECK_ARG(d->kept == 0 || (kept && ((uintptr_t)kept & 15) == 0),
-                 "linear cross entropy backward: what the forward pass kept is missing");
   LceKept k;
   if (d->kept) lce_kept_space(d, lce_kept_fp32(d), kept, &k);
   const int64_t ld32 = up(d->D, 4);
@@ -1835,7 +1843,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   for (int64_t v0 = 0, end; v0 < d->V; v0 = end) {
     end = std::min(d->V, v0 + p.piece);
     if (v0 < d->kept && end > d->kept) end = d->kept;
-    const int64_t width = end - v0, ldg = up(width, 8);
+    const int64_t width = end - v0, ldg = up(width, 64);
     const bool from_kept = v0 < d->kept;
     const int row0 = direct_w ? (int)v0 : 0;
     if (direct_w) {
