@@ -191,12 +191,11 @@ __device__ __forceinline__ constexpr int lce_pb(int i) {
   return P == 3 ? (i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0) : P == 2 ? (i == 1 ? 1 : 0) : 0;
 }
 
-// One tile: C[256 x BN] by a pair of CTAs.  With CHUNK = 0 the accumulator
-// takes the whole of K (BN = 256, two accumulators alternate between tiles).
-// With CHUNK > 0 (BN = 128) it takes CHUNK blocks of K and the epilogue adds
-// the chunks in registers: the tensor core cuts rather than rounds when it
-// adds to an accumulator, so that a sum over thousands of products drifts by
-// 2^-24 of itself for every 16 of them.  The small products of split operands
+// One tile: C[256 x BN] by a pair of CTAs, in two accumulators in turn.  With
+// CHUNK = 0 an accumulator takes the whole of K.  With CHUNK > 0 it takes CHUNK
+// blocks of K and the epilogue adds the chunks in registers: the tensor core
+// cuts rather than rounds when it adds to an accumulator, so that a sum over
+// thousands of products drifts by 2^-24 of itself for every 16 of them.  The small products of split operands
 // go to an accumulator of their own, which takes the whole of K.
 template <int EPI, typename T, int P, int BN, int CHUNK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THREADS), 1)
@@ -381,15 +380,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float u[32];
-            tmem_ld32(tmem_base + lanes + buf * BN + group * kCols + 32 * h, u);
+          for (int h = 0; h < 4; ++h) {
+            float u[16];
+            tmem_ld16(tmem_base + lanes + buf * BN + group * kCols + 16 * h, u);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[32 * h + j] += u[j];
+            for (int j = 0; j < 16; ++j) v[16 * h + j] += u[j];
             if (kPairs > 1 && c0 + CHUNK >= kb1) {
-              tmem_ld32(tmem_base + lanes + (2 + (local & 1)) * BN + group * kCols + 32 * h, u);
+              tmem_ld16(tmem_base + lanes + (2 + (local & 1)) * BN + group * kCols + 16 * h, u);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[32 * h + j] += u[j];
+              for (int j = 0; j < 16; ++j) v[16 * h + j] += u[j];
             }
           }
           tc_fence_before();
@@ -1472,18 +1471,19 @@ static int lce_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensor
 }
 
 // Chunks: split operands (results to fp32) every 4 blocks, 16 additions of the
-// main product; 16-bit ones on 256 x 128 tiles every 8, where there is time
-// for it since these tiles wait for their loads.
+// main product; 16-bit ones every 8 on 256 x 128 tiles, which wait for their
+// loads anyway, and every 16 where the result is fp32 (the losses: up to 2e-6
+// off without, 3e-7 with, for 3% of the forward product's time).
 template <int EPI>
 static int lce_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const LceGemm& g, bool a_mn,
                     bool b_mn, const LcePlan& p, int bn, cudaStream_t s) {
   if (p.P == 3) return lce_launch<EPI, __nv_bfloat16, 3, 128, 4>(a, b, c, g, a_mn, b_mn, s);
   if (p.P == 2) return lce_launch<EPI, __nv_bfloat16, 2, 128, 4>(a, b, c, g, a_mn, b_mn, s);
   if (p.half) {
-    if (bn == 256) return lce_launch<EPI, __half, 1, 256, 0>(a, b, c, g, a_mn, b_mn, s);
+    if (bn == 256) return lce_launch<EPI, __half, 1, 256, EPI == kEpiStats ? 16 : 0>(a, b, c, g, a_mn, b_mn, s);
     return lce_launch<EPI, __half, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
   }
-  if (bn == 256) return lce_launch<EPI, __nv_bfloat16, 1, 256, 0>(a, b, c, g, a_mn, b_mn, s);
+  if (bn == 256) return lce_launch<EPI, __nv_bfloat16, 1, 256, EPI == kEpiStats ? 16 : 0>(a, b, c, g, a_mn, b_mn, s);
   return lce_launch<EPI, __nv_bfloat16, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
 }
 
