@@ -66,10 +66,15 @@ static void fused_adam(bool decoupled, at::TensorList self, at::TensorList grads
   DeviceScope scope(dev);
   OCL_OP(decoupled ? "_fused_adamw_" : "_fused_adam_", dev);
   std::vector<pvb2_adamw_tensor> ts(n);
+  std::vector<at::Tensor> copies;  // gradients laid out unlike their parameters
+  const bool scaled = grad_scale.has_value() && grad_scale->defined();
   for (size_t i = 0; i < n; ++i) {
     check_param(self[i], grads[i], dev, type, i);
-    // the gradient is written back where it is unscaled, so no copy will do
-    TORCH_CHECK(same_layout(grads[i], self[i]), "ocl _fused_adam: gradient ", i, " is laid out unlike its parameter");
+    // a gradient that is unscaled is written back, so no copy will do
+    TORCH_CHECK(!scaled || same_layout(grads[i], self[i]),
+                "ocl _fused_adam: gradient ", i, " is laid out unlike its parameter");
+    const at::Tensor g = grad_like(grads[i], self[i]);
+    if (!g.is_same(grads[i])) copies.push_back(g);
     pvb2_adamw_tensor& t = ts[i];
     memset(&t, 0, sizeof(t));
     auto held = [&](const at::Tensor& x) {
@@ -78,7 +83,7 @@ static void fused_adam(bool decoupled, at::TensorList self, at::TensorList grads
       return x.data_ptr();
     };
     t.param = self[i].data_ptr();
-    t.grad = grads[i].data_ptr();
+    t.grad = g.data_ptr();
     t.exp_avg = held(exp_avgs[i]);
     t.exp_avg_sq = held(exp_avg_sqs[i]);
     if (amsgrad) t.max_exp_avg_sq = held(max_exp_avg_sqs[i]);
@@ -441,7 +446,7 @@ static void ce_check(const at::Tensor& input, const at::Tensor& weight, const at
 static size_t ce_keep_budget() {
   const char* e = getenv("B200_CE_KEEP_MB");
   const double mb = e ? atof(e) : 2048.0;
-  return mb > 0 ? (size_t)(mb * 1048576.0) : 0;
+  return mb > 0 ? (size_t)(std::min(mb, 1e9) * 1048576.0) : 0;
 }
 
 struct CeForward {
@@ -467,7 +472,13 @@ static CeForward linear_cross_entropy_forward(const at::Tensor& input, const at:
   CeForward r;
   if (keep) {
     const size_t bytes = pvb2_linear_ce_keep(&d, ce_keep_budget());
-    if (bytes) r.kept = empty({(int64_t)bytes}, at::kByte, dev);
+    if (bytes) {
+      try {
+        r.kept = empty({(int64_t)bytes}, at::kByte, dev);
+      } catch (const c10::Error&) {  // no memory for it: the backward pass does without
+        d.kept = 0;
+      }
+    }
     r.entries = d.kept;
   }
   at::Tensor loss = reduction == PVB2_LOSS_NONE ? empty(target.sizes(), at::kFloat, dev) : empty({}, at::kFloat, dev);

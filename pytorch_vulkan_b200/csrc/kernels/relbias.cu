@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(256)
           T* to = stage + r * kPitch + k * V;
           if (c >= 0 || c + V <= 0) {
             const int n = c < 0 ? 0 : max(0, min(V, Lk - c));
-            copy_async16(to, n ? row + c : row, n * (int)sizeof(T));
+            if (n > 0) copy_async16(to, row + c, n * (int)sizeof(T));
+            else *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
           } else {  // begins before the row
             for (int j = 0; j < V; ++j) to[j] = c + j >= 0 && c + j < Lk ? row[c + j] : from_f32<T>(0.f);
           }

@@ -33,7 +33,8 @@ class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with fp32 or 8-bit moments, one launch for all parameters of a type.
 
     The step count of each parameter lives on the device, so that a step
-    captured in a ``torch.ocl.Graph`` advances it on every replay.
+    captured in a ``torch.ocl.Graph`` advances it on every replay (the learning
+    rate and the other numbers are those of the capture).
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False,
@@ -50,6 +51,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"Invalid weight_decay value: {weight_decay}")
         self.state_bits = state_bits
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits}
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)

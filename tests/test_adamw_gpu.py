@@ -359,6 +359,52 @@ def test_state_dict_round_trip(ocl, bits):
         other.load_state_dict(saved)
 
 
+def test_torch_fused_with_gradients_of_another_layout(ocl):
+    gen = torch.Generator().manual_seed(10)
+    p0, g0 = rand((6, 5, 4, 3), gen), rand((6, 5, 4, 3), gen)
+    p = p0.to(DEV).contiguous(memory_format=torch.channels_last).requires_grad_()
+    opt = torch.optim.AdamW([p], fused=True, **HYPER)
+    p.grad = g0.to(DEV)
+    opt.step()
+    zero = torch.zeros_like(p0)
+    check_step(p0, g0, zero, zero, 1, p, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq"], torch.float32)
+
+
+def test_copies_keep_their_kind_of_state(ocl):
+    import copy
+
+    p = torch.randn(300).to(DEV).requires_grad_()
+    opt = ocl.optim.AdamW([p], state_bits=8)
+    twin = copy.deepcopy(opt)
+    assert twin.state_bits == 8
+    q = twin.param_groups[0]["params"][0]
+    p.grad, q.grad = torch.ones(300).to(DEV), torch.ones(300).to(DEV)
+    opt.step()
+    twin.step()
+    assert torch.equal(p.detach().cpu(), q.detach().cpu()) and "exp_avg_code" in twin.state[q]
+
+
+def test_closure_groups_and_parameters_without_gradient(ocl):
+    a, b, c = (torch.ones(50).to(DEV).requires_grad_() for _ in range(3))
+    h = torch.ones(40, dtype=torch.bfloat16).to(DEV).requires_grad_()
+    opt = ocl.optim.AdamW([{"params": [a, h]}, {"params": [b, c], "lr": 0.5, "weight_decay": 0.0}], lr=0.25, weight_decay=0.0)
+    assert opt.step() is None  # no gradients yet: nothing happens, and no state appears
+    assert not opt.state
+    c.grad = None
+
+    def closure():
+        opt.zero_grad()
+        loss = (a * 2.0).sum() + (b * 3.0).sum() + (h * 1.0).sum()
+        loss.backward()
+        return loss
+
+    assert opt.step(closure).item() == 50 * 2 + 50 * 3 + 40
+    # a first step moves by lr times the gradient's sign
+    for t, want in ((a, 0.75), (b, 0.5), (h, 0.75), (c, 1.0)):
+        assert (t.detach().cpu().float() - want).abs().max() <= 1e-6
+    assert c not in opt.state or not opt.state[c]
+
+
 def test_refusals(ocl):
     p = torch.zeros(8).to(DEV).requires_grad_()
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1), dict(state_bits=4)):

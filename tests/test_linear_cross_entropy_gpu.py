@@ -126,6 +126,31 @@ def test_sizes(ocl, mode, size, dtype):
     check(ocl, *make(*size, dtype), mode=mode)
 
 
+FEW = [(3, 520, 900), (4, 24, 70), (5, 2048, 333), (7, 1, 9), (8, 100, 4100), (8, 4001, 300), (2, 30000, 40), (6, 8, 1)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("size", FEW, ids=["x".join(map(str, s)) for s in FEW])
+def test_few_rows(ocl, math_fp32, size, dtype):
+    """A token or some, as while serving: with and without gradients, smoothing, bias and rows without a loss."""
+    x, w, b, t = make(*size, dtype, bias=True)
+    if size[0] > 2:
+        t[1] = -100
+    check(ocl, x, w, b, t, reduction="none", smooth=0.2, grad=torch.linspace(-1, 1, size[0]))
+    loss, _ = check(ocl, x, w, None, t)
+    with torch.no_grad():
+        again = ocl.functional.linear_cross_entropy(x.to(DEV), w.to(DEV), t.to(DEV))
+    assert torch.equal(again.cpu(), loss.detach().cpu())
+    wide = torch.cat([w, w.new_zeros(w.shape[0], 3)], 1).to(DEV)[:, :w.shape[1]].detach().requires_grad_()
+    check(ocl, x, w, None, t, given=[x.to(DEV).requires_grad_(), wide, None])
+
+
+def test_many_rows_and_few_classes(ocl, math_fp32):
+    """More rows than are joined at once, and K cut because the tiles are few."""
+    for dtype in (BF16, FP32):
+        check(ocl, *make(20001, 600, 12, dtype, bias=True, ignored=0.3))
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("smooth", [0.0, 0.1, 1.0])
@@ -374,6 +399,25 @@ def test_what_is_kept_stays_in_its_budget(ocl, monkeypatch):
         kept_nothing = ocl.functional.linear_cross_entropy(x, w, t)
         assert torch.ocl.memory_allocated() - before < 1 << 20
     assert torch.equal(loss.detach().cpu(), kept_nothing.cpu())
+
+
+def test_two_streams_at_once(ocl):
+    """Calls that overlap on the device share nothing."""
+    x, w, b, t = make(2000, 128, 6000, BF16)
+    x2, _, _, t2 = make(2000, 128, 6000, BF16, seed=3)
+    leaves, other = ([v.to(DEV).requires_grad_() for v in p] for p in ((x, w), (x2, w)))
+    td, td2 = t.to(DEV), t2.to(DEV)
+    f = lambda v, tt: torch.autograd.grad(ocl.functional.linear_cross_entropy(*v, tt), v)
+    want, want2 = [g.cpu() for g in f(leaves, td)], [g.cpu() for g in f(other, td2)]
+    torch.ocl.synchronize()
+    streams = [torch.Stream(device=DEV) for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for k, (v, tt) in enumerate(((leaves, td), (other, td2))):
+            with streams[k]:
+                got[k] = f(v, tt)
+    torch.ocl.synchronize()
+    assert all(torch.equal(a, g.cpu()) for a, g in zip(want + want2, got[0] + got[1]))
 
 
 def test_no_wait_ran_out(ocl):
