@@ -36,10 +36,10 @@ constexpr int kLBK = 64;
 // warp would cost the others a quarter of theirs.
 constexpr int kLProducers = 3, kLMmaWarp = 3;
 
-// P planes of each operand a stage; this CTA's 128 rows of A and BN / 2 columns
-// of B.  An epilogue warp takes 32 rows and 64 columns: 16 of them for 256
-// columns (with 8, two for each scheduler, an epilogue of exponentials took
-// twice as long as the products of a K of 1000).
+// A slot of the ring holds a K block of one plane of each operand: this CTA's
+// 128 rows of A and BN / 2 columns of B.  An epilogue warp takes 32 rows and 64
+// columns: 16 of them for 256 columns (with 8, two for each scheduler, an
+// epilogue of exponentials took twice as long as the products of a K of 1000).
 template <int P, int BN>
 struct LceSmem {
   static constexpr int EPI_WARPS = BN / 16;
@@ -47,11 +47,11 @@ struct LceSmem {
   static constexpr int COLS = 64;
   static constexpr int A_BYTES = 128 * kLBK * 2;
   static constexpr int B_BYTES = BN / 2 * kLBK * 2;
-  static constexpr int STAGE_BYTES = P * (A_BYTES + B_BYTES);
-    static constexpr int STAGES = (224 * 1024 - EPI_WARPS * 4096) / STAGE_BYTES;
-  static constexpr int EPI_OFF = STAGES * STAGE_BYTES;  // one 4 KB store box per epilogue warp
+  static constexpr int SLOT_BYTES = A_BYTES + B_BYTES;
+  static constexpr int SLOTS = (224 * 1024 - EPI_WARPS * 4096) / SLOT_BYTES;
+  static constexpr int EPI_OFF = SLOTS * SLOT_BYTES;  // one 4 KB store box per epilogue warp
   static constexpr int BAR_OFF = EPI_OFF + EPI_WARPS * 4096;
-  static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16;
+  static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 4) * 8 + 16;
 };
 
 // Kept exponentials, in [0, 1] relative to the largest of 64 columns, as 16-bit
@@ -177,42 +177,34 @@ __device__ __forceinline__ void store_box(uint8_t* box, int lane, F fill_and_sto
   }
 }
 
-// products of operand planes, smallest first; the last is the main one
+// the planes of a K block in the order in which they are loaded and released:
+// the main one is needed from the first product to the last
 template <int P>
-struct LcePairs {
-  static constexpr int N = P == 1 ? 1 : P == 2 ? 3 : 6;
-};
-template <int P>
-__device__ __forceinline__ constexpr int lce_pa(int i) {
-  return P == 3 ? (i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0) : P == 2 ? (i == 0 ? 1 : 0) : 0;
-}
-template <int P>
-__device__ __forceinline__ constexpr int lce_pb(int i) {
-  return P == 3 ? (i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0) : P == 2 ? (i == 1 ? 1 : 0) : 0;
+__device__ __forceinline__ constexpr int lce_plane(int j) {
+  return P == 3 && j > 0 ? 3 - j : j;
 }
 
 // One tile: C[256 x BN] by a pair of CTAs, in two accumulators in turn.  With
 // CHUNK = 0 an accumulator takes the whole of K.  With CHUNK > 0 it takes CHUNK
 // blocks of K and the epilogue adds the chunks in registers: the tensor core
 // cuts rather than rounds when it adds to an accumulator, so that a sum over
-// thousands of products drifts by 2^-24 of itself for every 16 of them.  The small products of split operands
-// go to an accumulator of their own, which takes the whole of K.
+// thousands of products drifts by 2^-24 of itself for every 16 of them.  Split
+// operands are chunked by the K block, their small products first, so that only
+// the four additions of the main one are cut at its size.
 template <int EPI, typename T, int P, int BN, int CHUNK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THREADS), 1)
     lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ LceGemm p, int a_mn, int b_mn) {
   using L = LceSmem<P, BN>;
   constexpr bool kPrecise = P > 1;
-  constexpr int kPairs = LcePairs<P>::N;
   constexpr int kCols = L::COLS;            // columns of an epilogue warp
-  constexpr int kStages = L::STAGES;
-  constexpr int kIssuers = kStages < kLProducers ? kStages : kLProducers;
-  static_assert(CHUNK > 0 || P == 1, "split operands are summed in chunks");
+  constexpr int kSlots = L::SLOTS;
+  static_assert(CHUNK == 1 || P == 1, "split operands: a chunk for each K block");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = (uint64_t*)(smem + L::BAR_OFF);  // waited on in the even CTA
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
+  uint64_t* empty = full + kSlots;
+  uint64_t* acc_full = empty + kSlots;
   uint64_t* acc_empty = acc_full + 2;               // waited on in the even CTA
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
@@ -225,7 +217,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kSlots; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -256,8 +248,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
     kb1 = min(kblocks, kb0 + p.kb_per);
   };
 
-  if (warp < kIssuers) {
-    // ------------------------------------------------- loads: stage s by warp s % kIssuers
+  if (warp < kLProducers) {
+    // ------------------------------------------------- loads: slot s by warp s % kLProducers
     if (lane == 0) {
       tma_prefetch(&tmA);
       tma_prefetch(&tmB);
@@ -266,29 +258,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
         int mb, nb, sp, kb0, kb1;
         place(tile, mb, nb, sp, kb0, kb1);
         const int am = mb * kLBM + rank * 128, bn = nb * BN + rank * (BN / 2);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % kStages;
-          if (s % kIssuers != warp) continue;
-          if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, abort)) break;
-          uint8_t* sa = smem + s * L::STAGE_BYTES;
-          uint8_t* sb = sa + P * L::A_BYTES;
-          const uint32_t bar = even_cta_addr(&full[s]);
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE_BYTES);
+        for (int kb = kb0; kb < kb1; ++kb) {
 #pragma unroll
-          for (int z = 0; z < P; ++z) {
+          for (int j = 0; j < P; ++j, ++it) {
+            const int s = it % kSlots, z = lce_plane<P>(j);
+            if (s % kLProducers != warp) continue;
+            if (!mbar_wait(&empty[s], ((it / kSlots) & 1) ^ 1, abort)) break;
+            uint8_t* sa = smem + s * L::SLOT_BYTES;
+            uint8_t* sb = sa + L::A_BYTES;
+            const uint32_t bar = even_cta_addr(&full[s]);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::SLOT_BYTES);
             if (!a_mn) {
-              tma_load_3d_pair(sa + z * L::A_BYTES, &tmA, bar, kb * kLBK, p.a_row0 + am, z);
+              tma_load_3d_pair(sa, &tmA, bar, kb * kLBK, p.a_row0 + am, z);
             } else {
 #pragma unroll
-              for (int j = 0; j < 2; ++j)
-                tma_load_3d_pair(sa + z * L::A_BYTES + j * 8192, &tmA, bar, am + 64 * j, p.a_row0 + kb * kLBK, z);
+              for (int q = 0; q < 2; ++q)
+                tma_load_3d_pair(sa + q * 8192, &tmA, bar, am + 64 * q, p.a_row0 + kb * kLBK, z);
             }
             if (!b_mn) {
-              tma_load_3d_pair(sb + z * L::B_BYTES, &tmB, bar, kb * kLBK, p.b_row0 + bn, z);
+              tma_load_3d_pair(sb, &tmB, bar, kb * kLBK, p.b_row0 + bn, z);
             } else {
 #pragma unroll
-              for (int j = 0; j < BN / 128; ++j)
-                tma_load_3d_pair(sb + z * L::B_BYTES + j * 8192, &tmB, bar, bn + 64 * j, p.b_row0 + kb * kLBK, z);
+              for (int q = 0; q < BN / 128; ++q)
+                tma_load_3d_pair(sb + q * 8192, &tmB, bar, bn + 64 * q, p.b_row0 + kb * kLBK, z);
             }
           }
         }
@@ -300,44 +292,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
       const uint32_t idesc = idesc_f16(kLBM, BN, !std::is_same<T, __half>::value, a_mn, b_mn);
       // One thread issues everything in order, so that what it computes between
       // two MMAs holds up the tensor core: the descriptors are formed once, and
-      // a step along K, a plane or a stage is an addition to their address
+      // a step along K or a slot is an addition to their address
       // (16-byte units, below 2^14).  Formed anew for each MMA they took it
       // longer than the MMA.
       const uint32_t smem0 = smem_u32(smem);
       const uint64_t a0 = a_mn ? desc_mnmajor16(smem0, 0, 8192) : desc_kmajor(smem0, 0);
-      const uint64_t b0 = b_mn ? desc_mnmajor16(smem0 + P * L::A_BYTES, 0, 8192) : desc_kmajor(smem0 + P * L::A_BYTES, 0);
+      const uint64_t b0 = b_mn ? desc_mnmajor16(smem0 + L::A_BYTES, 0, 8192) : desc_kmajor(smem0 + L::A_BYTES, 0);
       const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;
       uint32_t it = 0, chunk = 0;
       int local = 0;
       for (int tile = pair; tile < total_tiles && !*abort; tile += pairs, ++local) {
         int mb, nb, sp, kb0, kb1;
         place(tile, mb, nb, sp, kb0, kb1);
-        const uint32_t d_small = tmem_base + (2 + (local & 1)) * BN;  // products of the lesser planes
         for (int c0 = kb0; c0 < kb1; ++chunk) {
           const int c1 = CHUNK ? min(kb1, c0 + CHUNK) : kb1;
           const int buf = chunk & 1;
           if (!mbar_wait(&acc_empty[buf], ((chunk >> 1) & 1) ^ 1, abort)) break;
           tc_fence_after();
-          const uint32_t d_main = tmem_base + buf * BN;
-          for (int kb = c0; kb < c1; ++kb, ++it) {
-            const int s = it % kStages;
-            if (!mbar_wait(&full[s], (it / kStages) & 1, abort)) break;
-            tc_fence_after();
-            const uint64_t sa = a0 + (uint32_t)(s * (L::STAGE_BYTES / 16));
-            const uint64_t sb = b0 + (uint32_t)(s * (L::STAGE_BYTES / 16));
+          const uint32_t d = tmem_base + buf * BN;
+          // the product of plane slots sa (of A) and sb (of B); `fresh`: into an empty accumulator
+          auto product = [&](int sa, int sb, bool fresh) {
+            uint64_t ad = a0 + (uint32_t)(sa * (L::SLOT_BYTES / 16)), bd = b0 + (uint32_t)(sb * (L::SLOT_BYTES / 16));
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-              uint64_t ad = sa + lce_pa<P>(i) * (L::A_BYTES / 16), bd = sb + lce_pb<P>(i) * (L::B_BYTES / 16);
-#pragma unroll
-              for (int kk = 0; kk < kLBK / 16; ++kk) {
-                if (i == kPairs - 1) mma_f16_pair(d_main, ad, bd, idesc, (kb > c0 || kk > 0) ? 1u : 0u);
-                else mma_f16_pair(d_small, ad, bd, idesc, (kb > kb0 || i > 0 || kk > 0) ? 1u : 0u);
-                ad += a_step;
-                bd += b_step;
-              }
+            for (int kk = 0; kk < kLBK / 16; ++kk) {
+              mma_f16_pair(d, ad, bd, idesc, fresh && kk == 0 ? 0u : 1u);
+              ad += a_step;
+              bd += b_step;
             }
-            mma_commit_pair(&empty[s]);
+          };
+          bool ok = true;
+          auto arrived = [&](uint32_t n) {
+            ok = ok && mbar_wait(&full[n % kSlots], (n / kSlots) & 1, abort);
+            tc_fence_after();
+          };
+          for (int kb = c0; kb < c1 && ok; ++kb, it += P) {
+            // the smallest products first; a slot is released after its last one
+            const int s0 = it % kSlots;
+            arrived(it);
+            if (P == 3) {
+              const int s2 = (it + 1) % kSlots, s1 = (it + 2) % kSlots;
+              arrived(it + 1);
+              product(s2, s0, true);
+              product(s0, s2, false);
+              mma_commit_pair(&empty[s2]);
+              arrived(it + 2);
+              product(s1, s1, false);
+              product(s1, s0, false);
+              product(s0, s1, false);
+              mma_commit_pair(&empty[s1]);
+            } else if (P == 2) {
+              const int s1 = (it + 1) % kSlots;
+              arrived(it + 1);
+              product(s1, s0, true);
+              product(s0, s1, false);
+              mma_commit_pair(&empty[s1]);
+            }
+            product(s0, s0, P == 1 && kb == c0);
+            mma_commit_pair(&empty[s0]);
           }
+          if (!ok) break;
           mma_commit_pair(&acc_full[buf]);
           c0 = c1;
         }
@@ -388,11 +401,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
             tmem_ld16(tmem_base + lanes + buf * BN + group * kCols + 16 * h, u);
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[16 * h + j] += u[j];
-            if (kPairs > 1 && c0 + CHUNK >= kb1) {
-              tmem_ld16(tmem_base + lanes + (2 + (local & 1)) * BN + group * kCols + 16 * h, u);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[16 * h + j] += u[j];
-            }
           }
           tc_fence_before();
           __syncwarp();
@@ -1177,15 +1185,17 @@ struct LceTiling {
 
 // The cut with the least modelled time.  Cycles of a K block of a tile:
 // 512 for 256 x 256 (both the MMAs' rate and that of the loads from L2), for
-// 256 x 128 the loads' 384, for split operands the MMAs' (256 a product).  A
-// tile costs about 2500 more (its last loads and its epilogue), joining slabs
+// 256 x 128 the loads' 384; for split operands 512 a product, and on 256 x 128
+// 400, where the MMAs' reads and the loads' writes share 128 bytes of shared
+// memory a cycle.  A tile costs about 2500 more (its last loads and its epilogue), joining slabs
 // their traffic and a launch.
 static LceTiling lce_tiling(int64_t M, int64_t N, int64_t K, int P, int64_t read_bytes, bool cut = true) {
   const int64_t kb = cdiv(K, kLBK), pairs = lce_pairs_on_device();
   const double read = read_bytes / 3200.0;  // cycles at 6.1 TB/s and 1.9 GHz
   LceTiling best{0, 1, 0, 0};
-  for (int bn = P == 1 ? 256 : 128; bn >= 128; bn /= 2) {
-    const double block = P == 3 ? 1600 : P == 2 ? 800 : bn == 256 ? 520 : 400;
+  for (int bn = 256; bn >= 128; bn /= 2) {
+    const double products = P == 3 ? 6 : P == 2 ? 3 : 1;
+    const double block = products * (bn == 256 ? 520 : 400);
     const int64_t tiles = cdiv(M, kLBM) * cdiv(N, bn);
     const int64_t most = cut && tiles < pairs ? std::min<int64_t>(16, std::max<int64_t>(1, kb / 2)) : 1;
     for (int64_t S = 1; S <= most; ++S) {
@@ -1480,15 +1490,17 @@ static int lce_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensor
   return PVB2_OK;
 }
 
-// Chunks: split operands (results to fp32) every 4 blocks, 16 additions of the
+// Chunks: split operands (results to fp32) every block, four additions of the
 // main product; 16-bit ones every 8 on 256 x 128 tiles, which wait for their
 // loads anyway, and every 16 where the result is fp32 (the losses: up to 2e-6
 // off without, 3e-7 with, for 3% of the forward product's time).
 template <int EPI>
 static int lce_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const LceGemm& g, bool a_mn,
                     bool b_mn, const LcePlan& p, int bn, cudaStream_t s) {
-  if (p.P == 3) return lce_launch<EPI, __nv_bfloat16, 3, 128, 4>(a, b, c, g, a_mn, b_mn, s);
-  if (p.P == 2) return lce_launch<EPI, __nv_bfloat16, 2, 128, 4>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 3 && bn == 256) return lce_launch<EPI, __nv_bfloat16, 3, 256, 1>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 3) return lce_launch<EPI, __nv_bfloat16, 3, 128, 1>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 2 && bn == 256) return lce_launch<EPI, __nv_bfloat16, 2, 256, 1>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 2) return lce_launch<EPI, __nv_bfloat16, 2, 128, 1>(a, b, c, g, a_mn, b_mn, s);
   if (p.half) {
     if (bn == 256) return lce_launch<EPI, __half, 1, 256, EPI == kEpiStats ? 16 : 0>(a, b, c, g, a_mn, b_mn, s);
     return lce_launch<EPI, __half, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
