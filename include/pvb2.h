@@ -670,9 +670,9 @@ PVB2_API int pvb2_flatten_multi(int n, float* const* tensors, const int64_t* num
 /* outside [0, V) have no loss and no gradient, and may hold anything.  */
 /* x [N][D], w [V][D] of one type (fp32, fp16, bf16), unit stride along */
 /* D; bias [V] of that type or NULL.  Sums, maxima and losses are fp32. */
-/* 16-bit operands go to the tensor cores as they are.  fp32 ones go as */
-/* sums of bf16 numbers: three each in PVB2_MATH_FP32 (six products,    */
-/* 24 bits), two in PVB2_MATH_TF32 (three products, 16 bits).           */
+/* 16-bit operands go to the tensor cores as they are, fp32 ones as     */
+/* sums of two fp16 numbers (22 bits), scaled to the largest finite     */
+/* magnitude of x or w, below 2^-39 of which bits are lost.             */
 /* ------------------------------------------------------------------ */
 enum { PVB2_LOSS_NONE = 0, PVB2_LOSS_MEAN = 1, PVB2_LOSS_SUM = 2 };
 typedef struct pvb2_linear_ce_desc {
@@ -681,7 +681,7 @@ typedef struct pvb2_linear_ce_desc {
   int64_t ignore_index;
   double label_smoothing;    /* in [0, 1] */
   int64_t kept;              /* 0, or what pvb2_linear_ce_keep made it */
-  int32_t dtype, reduction, math;
+  int32_t dtype, reduction;
 } pvb2_linear_ce_desc;
 /* A backward pass forms the logits again, piece by piece, unless the forward
  * pass kept them: as 16-bit exponentials (fp32 logits for fp32 operands) of

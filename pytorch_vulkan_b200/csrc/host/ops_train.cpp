@@ -415,7 +415,6 @@ static pvb2_linear_ce_desc ce_desc(const at::Tensor& x, const at::Tensor& w, int
   d.label_smoothing = label_smoothing;
   d.dtype = dtype_code(x.scalar_type());
   d.reduction = (int32_t)reduction;
-  d.math = math_mode() == PVB2_MATH_FP32 ? PVB2_MATH_FP32 : PVB2_MATH_TF32;
   return d;
 }
 

@@ -15,13 +15,16 @@
 // fp32: 8 N V D operations instead of the 6 that a stored z would take.
 //
 // Operands are 16-bit (tcgen05 kind::f16, fp32 accumulators).  fp32 operands
-// are split into P bf16 numbers each, x = x0 + x1 + x2 (8 bits apiece), and
-// the product is the sum of the pairs whose sizes matter: 6 of 9 for P = 3
-// (what is left out is below 2^-24 of |x||w|), 3 of 4 for P = 2.  The loop
-// over K simply runs over the pairs as well, smallest first.
+// are split into two fp16 numbers each, x = x0 + x1 (11 bits apiece), of which
+// three products are formed: x0 w0, x0 w1 and x1 w0.  What is left out is, in
+// the mean, 2^-24 of |x||w| (3 2^-22 at most), as much as rounding the product
+// to fp32 would cost; three bf16 parts, which need no scaling, took six
+// products for the same (1.9 ms a step of N 2048, D 768, V 32768 against
+// 1.2).  fp16's range is met by a power of two for each tensor that brings its
+// largest finite magnitude to 2^14 .. 2^15; parts below 2^-39 of that are lost.
 //
-// fp16 keeps G in range by scaling: G is formed for |g_i| / max|g| and times
-// 2^15, undone on the fp32 results.
+// G is formed for |g_i| / max|g| and, in fp16, times 2^15; all factors are
+// undone on the fp32 results.
 #include <algorithm>
 #include <atomic>
 #include "tc_common.cuh"
@@ -91,7 +94,7 @@ struct LceGemm {
   int64_t keep_ld;
   const float* lse;       // kEpiGrad
   const float* grow;      // kEpiGrad: g_i / max|g| (0 for rows without a loss)
-  int planes;             // kEpiGrad: planes of G
+  const float* zscale;    // two factors of the logits, on the device, for split operands
   float gscale;
   // kEpiAcc / kEpiOut
   int accumulate;         // kEpiAcc: add to the slab
@@ -177,13 +180,6 @@ __device__ __forceinline__ void store_box(uint8_t* box, int lane, F fill_and_sto
   }
 }
 
-// the planes of a K block in the order in which they are loaded and released:
-// the main one is needed from the first product to the last
-template <int P>
-__device__ __forceinline__ constexpr int lce_plane(int j) {
-  return P == 3 && j > 0 ? 3 - j : j;
-}
-
 // One tile: C[256 x BN] by a pair of CTAs, in two accumulators in turn.  With
 // CHUNK = 0 an accumulator takes the whole of K.  With CHUNK > 0 it takes CHUNK
 // blocks of K and the epilogue adds the chunks in registers: the tensor core
@@ -260,8 +256,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
         const int am = mb * kLBM + rank * 128, bn = nb * BN + rank * (BN / 2);
         for (int kb = kb0; kb < kb1; ++kb) {
 #pragma unroll
-          for (int j = 0; j < P; ++j, ++it) {
-            const int s = it % kSlots, z = lce_plane<P>(j);
+          for (int z = 0; z < P; ++z, ++it) {
+            const int s = it % kSlots;
             if (s % kLProducers != warp) continue;
             if (!mbar_wait(&empty[s], ((it / kSlots) & 1) ^ 1, abort)) break;
             uint8_t* sa = smem + s * L::SLOT_BYTES;
@@ -326,21 +322,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
             tc_fence_after();
           };
           for (int kb = c0; kb < c1 && ok; ++kb, it += P) {
-            // the smallest products first; a slot is released after its last one
+            // the lesser products first; a slot is released after its last one
             const int s0 = it % kSlots;
             arrived(it);
-            if (P == 3) {
-              const int s2 = (it + 1) % kSlots, s1 = (it + 2) % kSlots;
-              arrived(it + 1);
-              product(s2, s0, true);
-              product(s0, s2, false);
-              mma_commit_pair(&empty[s2]);
-              arrived(it + 2);
-              product(s1, s1, false);
-              product(s1, s0, false);
-              product(s0, s1, false);
-              mma_commit_pair(&empty[s1]);
-            } else if (P == 2) {
+            if (P == 2) {
               const int s1 = (it + 1) % kSlots;
               arrived(it + 1);
               product(s1, s0, true);
@@ -381,6 +366,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
           }
         }
       }
+      const float zscale0 = P == 2 && p.zscale ? p.zscale[0] : 1.f, zscale1 = P == 2 && p.zscale ? p.zscale[1] : 1.f;
       const float flat = EPI == kEpiGrad ? p.smoothing / (float)p.V : 0.f;
       const float oscale = EPI == kEpiOut && p.out_scale ? *p.out_scale : 1.f;
       float mx = -INFINITY, sum = 0.f, zs = 0.f;
@@ -421,6 +407,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[chunk & 1]));
+        }
+        if ((EPI == kEpiStats || EPI == kEpiGrad) && P == 2) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = v[j] * zscale0 * zscale1;  // their product may be beyond fp32
         }
         // whether any of the warp's targets is among these columns
         const bool has_target = (EPI == kEpiStats || EPI == kEpiGrad) &&
@@ -488,12 +478,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
             for (int j = 0; j < 64; ++j) v[j] = row_g == 0.f ? 0.f : v[j];
           }
           if (m0 < p.M) {
-            for (int z = 0; z < p.planes; ++z) {
+            for (int z = 0; z < P; ++z) {
               store_box(box, lane, [&](int phase) {
                 if (phase == 0) box16<T>(box, lane, v);
                 else tma_store_3d(&tmC, box, n0, m0, z);
               });
-              if (z + 1 < p.planes) {
+              if (z + 1 < P) {
 #pragma unroll
                 for (int j = 0; j < 64; ++j) v[j] -= to_f32(from_f32<T>(v[j]));
               }
@@ -592,11 +582,69 @@ struct LcePackJob {
   int vec;
 };
 
+// Scales of split operands.  One block's largest finite magnitudes of x (rows
+// that have a loss) come first in `part`, then those of w; each block of a
+// later launch reduces them anew.
+constexpr int kLScaleBlocks = 296;
+struct LceScaleJob {
+  const float* part;      // NULL: nothing is scaled
+  int nx, nw;
+  float* scales;          // 1 / s_x and 1 / s_w, written by the first block
+};
+
+// 2^k that brings m to [2^14, 2^15) (k in [-112, 120]), 1 for 0
+__device__ __forceinline__ float lce_pow2(float m) {
+  const int e = (int)(__float_as_uint(m) >> 23) - 127;
+  return m == 0.f ? 1.f : __uint_as_float((uint32_t)(127 + min(120, 14 - e)) << 23);
+}
+
+__global__ void __launch_bounds__(256)
+    lce_absmax_kernel(const float* __restrict__ x, int64_t rows_x, int64_t ldx, const float* __restrict__ w,
+                      int64_t rows_w, int64_t ldw, int64_t cols, const int64_t* __restrict__ target, int64_t V,
+                      int64_t ignore, int nx, float* __restrict__ part) {
+  const bool is_x = (int)blockIdx.x < nx;
+  const float* src = is_x ? x : w;
+  const int64_t rows = is_x ? rows_x : rows_w, ld = is_x ? ldx : ldw;
+  const int64_t block = is_x ? blockIdx.x : blockIdx.x - nx, blocks = is_x ? nx : gridDim.x - nx;
+  const bool vec = ((uintptr_t)src & 15) == 0 && ld % 4 == 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = 0.f;
+  auto take = [&](float v) {
+    v = fabsf(v);
+    m = v <= 3.402823466e38f ? fmaxf(m, v) : m;  // neither infinity nor NaN
+  };
+  for (int64_t r = block * 8 + warp; r < rows; r += blocks * 8) {
+    if (is_x && !lce_scored(target[r], V, ignore)) continue;
+    const float* row = src + r * ld;
+    if (vec) {
+#pragma unroll 4
+      for (int64_t c = lane * 4; c + 4 <= cols; c += 128) {
+        const float4 q = *reinterpret_cast<const float4*>(row + c);
+        take(q.x);
+        take(q.y);
+        take(q.z);
+        take(q.w);
+      }
+      for (int64_t c = cols / 4 * 4 + lane; c < cols; c += 32) take(row[c]);
+    } else {
+      for (int64_t c = lane; c < cols; c += 32) take(row[c]);
+    }
+  }
+  __shared__ float s[8];
+  m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+  if (lane == 0) s[warp] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int q = 1; q < 8; ++q) m = fmaxf(m, s[q]);
+    part[blockIdx.x] = m;
+  }
+}
+
 // what each row's gradient is multiplied by, where that is one number for all
 // rows (mean and sum): row[i] is 1 or 0, and one factor for all results
 struct LceRowsJob {
   float* row;             // NULL: nothing to do
-  float* factor;
+  float* factor;          // of db, dx (which w's scale is in) and dw (x's)
   const float *grad_out, *count;
   const int64_t* target;
   int64_t N;
@@ -606,7 +654,7 @@ struct LceRowsJob {
 
 template <typename S, typename T>
 __device__ __forceinline__ void lce_pack_one(const LcePackJob<S>& j, int64_t e, int per_row, int64_t cols, int64_t ldp,
-                                             int planes, int64_t V, int64_t ignore) {
+                                             int planes, int64_t V, int64_t ignore, float scale) {
   const int64_t r = e <= INT32_MAX ? (int64_t)((int)e / per_row) : e / per_row;
   const int64_t c = (e - r * per_row) * 8, plane = j.rows * ldp;
   float v[8];
@@ -621,6 +669,10 @@ __device__ __forceinline__ void lce_pack_one(const LcePackJob<S>& j, int64_t e, 
     for (int k = 0; k < 8; ++k) v[k] = 0.f;
   }
   T* dst = reinterpret_cast<T*>(j.dst) + r * ldp + c;
+  if (planes > 1) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= scale;
+  }
   for (int z = 0; z < planes; ++z) {
     store_vec<8>(dst + z * plane, v);
 #pragma unroll
@@ -635,21 +687,52 @@ __device__ __forceinline__ void lce_pack_one(const LcePackJob<S>& j, int64_t e, 
 // one or two operands of the same row length (eight columns a thread), and
 // the rows' factors with them
 template <typename S, typename T>
-__global__ void lce_pack_kernel(LcePackJob<S> a, LcePackJob<S> b, LceRowsJob rj, int64_t cols, int64_t ldp, int planes,
-                                int64_t V, int64_t ignore) {
+__global__ void __launch_bounds__(256)
+    lce_pack_kernel(LcePackJob<S> a, LcePackJob<S> b, LceRowsJob rj, LceScaleJob sj, int64_t cols, int64_t ldp,
+                    int planes, int64_t V, int64_t ignore) {
+  float sx = 1.f, sw = 1.f;  // of a and of b
+  if (sj.part) {
+    __shared__ float smax[2][8];
+    float mx = 0.f, mw = 0.f;
+    for (int q = threadIdx.x; q < sj.nx + sj.nw; q += 256) {
+      const float m = sj.part[q];
+      if (q < sj.nx) mx = fmaxf(mx, m);
+      else mw = fmaxf(mw, m);
+    }
+    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+    mw = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mw)));
+    if ((threadIdx.x & 31) == 0) {
+      smax[0][threadIdx.x >> 5] = mx;
+      smax[1][threadIdx.x >> 5] = mw;
+    }
+    __syncthreads();
+    for (int q = 0; q < 8; ++q) {
+      mx = fmaxf(mx, smax[0][q]);
+      mw = fmaxf(mw, smax[1][q]);
+    }
+    sx = lce_pow2(mx);
+    sw = lce_pow2(mw);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      sj.scales[0] = 1.f / sx;
+      sj.scales[1] = 1.f / sw;
+    }
+  }
   const int per_row = (int)(ldp / 8);
   const int64_t na = a.rows * per_row, total = na + b.rows * per_row;
   const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t e = first; e < total; e += step) {
-    if (e < na) lce_pack_one<S, T>(a, e, per_row, cols, ldp, planes, V, ignore);
-    else lce_pack_one<S, T>(b, e - na, per_row, cols, ldp, planes, V, ignore);
+    if (e < na) lce_pack_one<S, T>(a, e, per_row, cols, ldp, planes, V, ignore, sx);
+    else lce_pack_one<S, T>(b, e - na, per_row, cols, ldp, planes, V, ignore, sw);
   }
   if (rj.row) {
     for (int64_t i = first; i < rj.N; i += step) rj.row[i] = lce_scored(rj.target[i], V, ignore) ? 1.f : 0.f;
     if (first == 0) {
       float f = *rj.grad_out;
       if (rj.mean) f = *rj.count > 0.f ? f / *rj.count : 0.f;
-      *rj.factor = f * rj.inv_gscale;
+      f *= rj.inv_gscale;
+      rj.factor[0] = f;
+      rj.factor[1] = f / sw;
+      rj.factor[2] = f / sx;
     }
   }
 }
@@ -765,9 +848,10 @@ __global__ void __launch_bounds__(256)
 // the same from logits that lie in S partial sums [S][rows][ld]: one block a
 // row
 __device__ __forceinline__ float lce_slab_logit(const float* __restrict__ slab, int S, int64_t size, int64_t at,
-                                                const void* bias, int64_t n, int bias_dtype) {
+                                                const void* bias, int64_t n, int bias_dtype, float2 zscale) {
   float z = slab[at];
   for (int s = 1; s < S; ++s) z += slab[s * size + at];
+  z = z * zscale.x * zscale.y;
   return bias ? z + load_as<float>(bias, n, bias_dtype) : z;
 }
 
@@ -775,13 +859,14 @@ __global__ void __launch_bounds__(512)
     lce_slab_rows_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t ld, const void* __restrict__ bias,
                          int bias_dtype, const int64_t* __restrict__ target, int64_t V, int64_t ignore, float smoothing,
                          float* __restrict__ lse, float* __restrict__ loss, float* __restrict__ kept, int64_t keep,
-                         int64_t keep_ld, float* __restrict__ ztarget) {
+                         int64_t keep_ld, float* __restrict__ ztarget, const float* __restrict__ zscale) {
   __shared__ float sm[16], ss[16], sz[16], zt;
+  const float2 unscale = zscale ? make_float2(zscale[0], zscale[1]) : make_float2(1.f, 1.f);
   const int64_t i = blockIdx.x, t = target[i];
   const bool scored = lce_scored(t, V, ignore);
   float mx = -INFINITY, sum = 0.f, zs = 0.f;
   for (int64_t n = threadIdx.x; n < V; n += 512) {
-    const float z = lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, n, bias_dtype);
+    const float z = lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, n, bias_dtype, unscale);
     if (n < keep) kept[i * keep_ld + n] = z;
     if (scored && n == t) zt = z;
     const float nm = fmaxf(mx, z), base = nm == -INFINITY ? 0.f : nm;
@@ -959,12 +1044,13 @@ __global__ void __launch_bounds__(256)
     lce_slab_grad_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t ld, const void* __restrict__ bias,
                          int bias_dtype, const int64_t* __restrict__ target, int64_t v0, int64_t width, int64_t V,
                          int64_t ignore, float smoothing, const float* __restrict__ lse, const float* __restrict__ grow,
-                         float gscale, T* __restrict__ G, int64_t ldg, int planes) {
+                         float gscale, T* __restrict__ G, int64_t ldg, int planes, const float* __restrict__ zscale) {
+  const float2 unscale = zscale ? make_float2(zscale[0], zscale[1]) : make_float2(1.f, 1.f);
   const int64_t i = blockIdx.x, tt = target[i];
   const int64_t t = lce_scored(tt, V, ignore) ? tt - v0 : -1;
   const float l = lse[i], g = grow[i], flat = smoothing / (float)V;
   for (int64_t n = threadIdx.x; n < width; n += 256) {
-    float e = expf(lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, v0 + n, bias_dtype) - l) - flat;
+    float e = expf(lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, v0 + n, bias_dtype, unscale) - l) - flat;
     if (n == t) e -= 1.f - smoothing;
     e = g == 0.f ? 0.f : e * g * gscale;
     for (int z = 0; z < planes; ++z) {
@@ -1082,7 +1168,8 @@ __global__ void __launch_bounds__(1024)
 // that maximum
 __global__ void __launch_bounds__(1024)
     lce_grad_rows_kernel(const float* __restrict__ grad_out, const int64_t* __restrict__ target, int64_t N, int64_t V,
-                         int64_t ignore, float inv_gscale, float* __restrict__ row, float* __restrict__ factor) {
+                         int64_t ignore, float inv_gscale, const float* __restrict__ scales, float* __restrict__ row,
+                         float* __restrict__ factor) {
   __shared__ float s_max[32];
   float mx = 0.f;
   for (int64_t i = threadIdx.x; i < N; i += 1024)
@@ -1100,7 +1187,12 @@ __global__ void __launch_bounds__(1024)
   for (int w = 1; w < 32; ++w) mx = (s_max[w] > mx || s_max[w] != s_max[w]) ? s_max[w] : mx;
   for (int64_t i = threadIdx.x; i < N; i += 1024)
     row[i] = lce_scored(target[i], V, ignore) && mx != 0.f ? grad_out[i] / mx : 0.f;
-  if (threadIdx.x == 0) *factor = mx * inv_gscale;
+  if (threadIdx.x == 0) {
+    const float f = mx * inv_gscale;
+    factor[0] = f;
+    factor[1] = scales ? f * scales[1] : f;
+    factor[2] = scales ? f * scales[0] : f;
+  }
 }
 
 // out [rows][cols] = factor * sum of S slabs [rows][ld], four columns a thread
@@ -1194,7 +1286,7 @@ static LceTiling lce_tiling(int64_t M, int64_t N, int64_t K, int P, int64_t read
   const double read = read_bytes / 3200.0;  // cycles at 6.1 TB/s and 1.9 GHz
   LceTiling best{0, 1, 0, 0};
   for (int bn = 256; bn >= 128; bn /= 2) {
-    const double products = P == 3 ? 6 : P == 2 ? 3 : 1;
+    const double products = P == 2 ? 3 : 1;
     const double block = products * (bn == 256 ? 520 : 400);
     const int64_t tiles = cdiv(M, kLBM) * cdiv(N, bn);
     const int64_t most = cut && tiles < pairs ? std::min<int64_t>(16, std::max<int64_t>(1, kb / 2)) : 1;
@@ -1213,7 +1305,7 @@ static LceTiling lce_tiling(int64_t M, int64_t N, int64_t K, int P, int64_t read
 struct LcePlan {
   bool few;          // forward: few rows, no tiles
   int P;             // planes of an operand
-  bool half;         // fp16 operands (bf16 otherwise)
+  bool half;         // fp16 planes (bf16 otherwise)
   int64_t ldp;       // row length of packed operands
   bool pack_w;       // w is packed piece by piece
   bool pack_x;       // forward: x is packed (the backward pass always does)
@@ -1242,8 +1334,8 @@ static pvb2_linear_ce_desc lce_normal(const pvb2_linear_ce_desc* d) {
 
 static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
   LcePlan p;
-  p.half = d->dtype == PVB2_F16;
-  p.P = d->dtype != PVB2_F32 ? 1 : d->math == PVB2_MATH_FP32 ? 3 : 2;
+  p.half = d->dtype != PVB2_BF16;
+  p.P = d->dtype == PVB2_F32 ? 2 : 1;
   // packed rows begin on 128-byte lines, unless that would be mostly padding
   p.ldp = up(d->D, d->D >= 256 ? 64 : 8);
   // Rows of w that straddle lines take two reads from L2 for each 128 bytes.  A
@@ -1298,7 +1390,7 @@ static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
 static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   struct Made {
     int64_t N = -1, D, V, ldx, ldw, kept;
-    int32_t dtype, math, sms;
+    int32_t dtype, sms;
     bool backward;
     LcePlan plan;
   };
@@ -1307,7 +1399,7 @@ static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   const int sms = num_sms();
   for (const Made& m : made)
     if (m.N == d->N && m.D == d->D && m.V == d->V && m.ldx == d->ldx && m.ldw == d->ldw && m.kept == d->kept && m.dtype == d->dtype &&
-        m.math == d->math && m.sms == sms && m.backward == backward)
+        m.sms == sms && m.backward == backward)
       return m.plan;
   Made& m = made[next];
   next = (next + 1) % 4;
@@ -1318,7 +1410,6 @@ static LcePlan lce_plan(const pvb2_linear_ce_desc* d, bool backward) {
   m.ldw = d->ldw;
   m.kept = d->kept;
   m.dtype = d->dtype;
-  m.math = d->math;
   m.sms = sms;
   m.backward = backward;
   m.plan = lce_make_plan(d, backward);
@@ -1360,6 +1451,7 @@ static size_t lce_kept_space(const pvb2_linear_ce_desc* d, bool fp32, const void
 
 struct LceFwdSpace {
   uint16_t *x, *w;
+  float *absmax, *scales;
   float* slab;
   float2* part;
   float *zsum, *ztarget, *loss;
@@ -1384,6 +1476,8 @@ static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   const bool slabs = lce_slabs(p);
   s->x = a.take<uint16_t>(!p.few && p.pack_x ? rows * p.ldp * p.P : 0);
   s->w = a.take<uint16_t>(!p.few && p.pack_w ? p.piece * p.ldp * p.P : 0);
+  s->absmax = a.take<float>(!p.few && p.P == 2 ? 2 * kLScaleBlocks : 0);
+  s->scales = a.take<float>(2);
   s->slab = a.take<float>(slabs ? p.z.splits * rows * up(d->V, 4) : 0);
   s->part = a.take<float2>(slabs ? 0 : rows * parts);
   s->zsum = a.take<float>(!slabs && d->label_smoothing != 0 ? rows * parts : 0);
@@ -1394,7 +1488,8 @@ static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
 
 struct LceBwdSpace {
   uint16_t *x, *w, *G;
-  float *slab, *row, *factor, *dx, *dw, *colsum;
+  float *absmax, *scales;
+  float *slab, *row, *factor, *dx, *dw, *colsum;  // factor: of db, dx and dw
 };
 
 static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceBwdSpace* s) {
@@ -1405,7 +1500,9 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   s->G = a.take<uint16_t>(d->N * up(width, 64) * p.P);
   s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
-  s->factor = a.take<float>(1);
+  s->absmax = a.take<float>(p.P == 2 ? 2 * kLScaleBlocks : 0);
+  s->scales = a.take<float>(2);
+  s->factor = a.take<float>(3);
   s->dx = a.take<float>(p.pieces > 1 || (d->kept > 0 && d->kept < d->V) || p.dx.splits > 1 ? p.dx.splits * d->N * ld32 : 0);
   s->dw = a.take<float>(p.dw.splits > 1 ? p.dw.splits * width * ld32 : 0);
   s->colsum = a.take<float>(p.colsum_parts * width);
@@ -1418,8 +1515,6 @@ static int lce_check(const pvb2_linear_ce_desc* d) {
                  "linear cross entropy: fp32, fp16 or bf16 expected (got dtype %d)", d->dtype);
   PVB2_CHECK_ARG(d->reduction >= PVB2_LOSS_NONE && d->reduction <= PVB2_LOSS_SUM,
                  "linear cross entropy: unknown reduction %d", d->reduction);
-  PVB2_CHECK_ARG(d->math == PVB2_MATH_FP32 || d->math == PVB2_MATH_TF32, "linear cross entropy: unknown math mode %d",
-                 d->math);
   PVB2_CHECK_ARG(d->N >= 0 && d->V >= 1 && d->D >= 1 && d->N < (1 << 24) && d->V < (1 << 24) && d->D < (1 << 20),
                  "linear cross entropy: sizes N=%lld D=%lld V=%lld out of range", (long long)d->N, (long long)d->D,
                  (long long)d->V);
@@ -1497,10 +1592,8 @@ static int lce_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensor
 template <int EPI>
 static int lce_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const LceGemm& g, bool a_mn,
                     bool b_mn, const LcePlan& p, int bn, cudaStream_t s) {
-  if (p.P == 3 && bn == 256) return lce_launch<EPI, __nv_bfloat16, 3, 256, 1>(a, b, c, g, a_mn, b_mn, s);
-  if (p.P == 3) return lce_launch<EPI, __nv_bfloat16, 3, 128, 1>(a, b, c, g, a_mn, b_mn, s);
-  if (p.P == 2 && bn == 256) return lce_launch<EPI, __nv_bfloat16, 2, 256, 1>(a, b, c, g, a_mn, b_mn, s);
-  if (p.P == 2) return lce_launch<EPI, __nv_bfloat16, 2, 128, 1>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 2 && bn == 256) return lce_launch<EPI, __half, 2, 256, 1>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 2) return lce_launch<EPI, __half, 2, 128, 1>(a, b, c, g, a_mn, b_mn, s);
   if (p.half) {
     if (bn == 256) return lce_launch<EPI, __half, 1, 256, EPI == kEpiStats ? 16 : 0>(a, b, c, g, a_mn, b_mn, s);
     return lce_launch<EPI, __half, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
@@ -1518,24 +1611,39 @@ struct LceOperand {  // to be packed
 
 template <typename S, typename T>
 static int lce_pack_as(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceOperand& a, const LceOperand& b,
-                       const LceRowsJob& rows, cudaStream_t s) {
+                       const LceRowsJob& rows, const LceScaleJob& scale, cudaStream_t s) {
   auto job = [](const LceOperand& o) {
     const S* src = (const S*)o.src + o.row0 * o.ld;
     return LcePackJob<S>{src, o.rows, o.ld, o.dst, o.target, ((uintptr_t)src & 15) == 0 && o.ld * sizeof(S) % 16 == 0};
   };
   const int64_t total = std::max((a.rows + b.rows) * (p.ldp / 8), rows.row ? rows.N : 0);
   if (total == 0) return PVB2_OK;
-  lce_pack_kernel<S, T><<<grid_for(total, 256), 256, 0, s>>>(job(a), job(b), rows, d->D, p.ldp, p.P, d->V,
+  lce_pack_kernel<S, T><<<grid_for(total, 256), 256, 0, s>>>(job(a), job(b), rows, scale, d->D, p.ldp, p.P, d->V,
                                                              d->ignore_index);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
 
 static int lce_pack(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceOperand& a, const LceOperand& b,
-                    const LceRowsJob& rows, cudaStream_t s) {
-  if (d->dtype == PVB2_F32) return lce_pack_as<float, __nv_bfloat16>(d, p, a, b, rows, s);
-  if (p.half) return lce_pack_as<__half, __half>(d, p, a, b, rows, s);
-  return lce_pack_as<__nv_bfloat16, __nv_bfloat16>(d, p, a, b, rows, s);
+                    const LceRowsJob& rows, const LceScaleJob& scale, cudaStream_t s) {
+  if (d->dtype == PVB2_F32) return lce_pack_as<float, __half>(d, p, a, b, rows, scale, s);
+  if (p.half) return lce_pack_as<__half, __half>(d, p, a, b, rows, scale, s);
+  return lce_pack_as<__nv_bfloat16, __nv_bfloat16>(d, p, a, b, rows, scale, s);
+}
+
+// the scales of split operands: their magnitudes, for the launches that pack
+static int lce_scales(const pvb2_linear_ce_desc* d, const LcePlan& p, const void* x, const void* w,
+                      const int64_t* target, float* absmax, float* scales, LceScaleJob* job, cudaStream_t s) {
+  *job = LceScaleJob{nullptr, 0, 0, nullptr};
+  if (p.P == 1) return PVB2_OK;
+  job->part = absmax;
+  job->nx = (int)std::min<int64_t>(kLScaleBlocks, cdiv(d->N * d->D, 8192));
+  job->nw = (int)std::min<int64_t>(kLScaleBlocks, cdiv(d->V * d->D, 8192));
+  job->scales = scales;
+  lce_absmax_kernel<<<job->nx + job->nw, 256, 0, s>>>((const float*)x, d->N, d->ldx, (const float*)w, d->V, d->ldw, d->D,
+                                                      target, d->V, d->ignore_index, job->nx, absmax);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
 }
 
 static LceRowsJob lce_no_rows() {
@@ -1676,7 +1784,7 @@ static int lce_slab_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const L
                          cudaStream_t s) {
   lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target, v0,
                                                  width, d->V, d->ignore_index, (float)d->label_smoothing, lse, sp.row,
-                                                 gscale, (T*)sp.G, ldg, p.P);
+                                                 gscale, (T*)sp.G, ldg, p.P, p.P == 2 ? sp.scales : nullptr);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -1695,7 +1803,7 @@ static int lce_bias_grad_as(const pvb2_linear_ce_desc* d, const LcePlan& p, cons
 
 static int lce_bias_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, int64_t width,
                          int64_t ldg, void* out, cudaStream_t s) {
-  if (d->dtype == PVB2_F32) return lce_bias_grad_as<__nv_bfloat16, float>(d, p, sp, width, ldg, (float*)out, s);
+  if (d->dtype == PVB2_F32) return lce_bias_grad_as<__half, float>(d, p, sp, width, ldg, (float*)out, s);
   if (p.half) return lce_bias_grad_as<__half, __half>(d, p, sp, width, ldg, (__half*)out, s);
   return lce_bias_grad_as<__nv_bfloat16, __nv_bfloat16>(d, p, sp, width, ldg, (__nv_bfloat16*)out, s);
 }
@@ -1736,6 +1844,9 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
                    "linear cross entropy: 16-byte aligned memory for what is kept needed");
     LceKept k;
     lce_kept_space(d, d->dtype == PVB2_F32 || p.few || slabs, kept, &k);
+    LceScaleJob scale;
+    if (!p.few) PVB2_TRY(lce_scales(d, p, x, w, target, sp.absmax, sp.scales, &scale, s));
+    const float* zscale = p.P == 2 ? sp.scales : nullptr;
     for (int64_t r0 = 0; r0 < d->N; r0 += kLRowsFwd) {
       const int64_t rows = std::min(kLRowsFwd, d->N - r0);
       CUtensorMap ma, mb;
@@ -1758,15 +1869,16 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
         const int64_t width = std::min(p.piece, d->V - v0);
         // x goes with the first piece of w
         LceOperand px, pw;
-        if (!direct_x && v0 == 0) px = LceOperand{x, r0, rows, d->ldx, sp.x, nullptr};
+        if (!direct_x && v0 == 0) px = LceOperand{x, r0, rows, d->ldx, sp.x, target + r0};
         if (p.pack_w) pw = LceOperand{w, v0, width, d->ldw, sp.w, nullptr};
-        PVB2_TRY(lce_pack(d, p, px, pw, lce_no_rows(), s));
+        PVB2_TRY(lce_pack(d, p, px, pw, lce_no_rows(), scale, s));
         if (!p.pack_w) PVB2_TRY(lce_map_b(&mb, w, d->D, d->V, d->ldw, p, p.z.bn));
         else PVB2_TRY(lce_map_b(&mb, sp.w, d->D, width, p.ldp, p, p.z.bn));
         LceGemm g = lce_logits(d, bias, rows, v0, width, p.pack_w ? 0 : (int)v0, target + r0);
         if (slabs) {
           PVB2_TRY(lce_slab_logits(d, p, ma, mb, g, sp.slab, s));
         } else {
+          g.zscale = zscale;
           g.part = sp.part;
           g.zsum = smoothing != 0.f ? sp.zsum : nullptr;
           g.ztarget = d->kept ? k.ztarget + r0 : sp.ztarget;
@@ -1785,7 +1897,8 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       if (slabs)
         lce_slab_rows_kernel<<<(int)rows, 512, 0, s>>>(
             sp.slab, p.z.splits, rows, up(d->V, 4), bias, d->dtype, target + r0, d->V, d->ignore_index, smoothing,
-            lse + r0, loss + r0, (float*)k.data + r0 * k.ld, d->kept, k.ld, d->kept ? k.ztarget + r0 : nullptr);
+            lse + r0, loss + r0, (float*)k.data + r0 * k.ld, d->kept, k.ld, d->kept ? k.ztarget + r0 : nullptr,
+            zscale);
       else
         lce_rows_kernel<<<(int)cdiv(rows, 32), 1024, 0, s>>>(
             sp.part, smoothing != 0.f ? sp.zsum : nullptr, rows, parts, d->kept ? k.ztarget + r0 : sp.ztarget,
@@ -1845,14 +1958,13 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   const bool direct_w = !p.pack_w, slabs = lce_slabs(p);
   PVB2_TRY(lce_aligned(w, direct_w));
   const float gscale = p.half ? 32768.f : 1.f;
+  LceScaleJob scale;
+  PVB2_TRY(lce_scales(d, p, x, w, target, sp.absmax, sp.scales, &scale, s));
+  const float* zscale = p.P == 2 ? sp.scales : nullptr;
   LceRowsJob rows = lce_no_rows();
-  if (d->reduction == PVB2_LOSS_NONE) {
-    lce_grad_rows_kernel<<<1, 1024, 0, s>>>(grad_out, target, d->N, d->V, d->ignore_index, 1.f / gscale, sp.row,
-                                            sp.factor);
-    PVB2_LAUNCH_CHECK();
-  } else {
+  if (d->reduction != PVB2_LOSS_NONE)
     rows = LceRowsJob{sp.row, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
-  }
+  bool row_factors = d->reduction != PVB2_LOSS_NONE;  // or still to be formed, after the scales
   LceOperand px{x, 0, d->N, d->ldx, sp.x, target};
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;
   PVB2_TRY(lce_map_a(&x_k, sp.x, d->D, d->N, p.ldp, p));
@@ -1872,16 +1984,22 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       PVB2_TRY(lce_map_b(&w_k, w, d->D, d->V, d->ldw, p, p.z.bn));
       PVB2_TRY(lce_map_mn(&w_mn, w, d->D, d->V, d->ldw, p));
     } else if (dx || !from_kept) {
-      PVB2_TRY(lce_pack(d, p, px, LceOperand{w, v0, width, d->ldw, sp.w, nullptr}, rows, s));
+      PVB2_TRY(lce_pack(d, p, px, LceOperand{w, v0, width, d->ldw, sp.w, nullptr}, rows, scale, s));
       px = LceOperand();
       rows = lce_no_rows();
       PVB2_TRY(lce_map_b(&w_k, sp.w, d->D, width, p.ldp, p, p.z.bn));
       PVB2_TRY(lce_map_mn(&w_mn, sp.w, d->D, width, p.ldp, p));
     }
     // x and the rows' factors, unless they went with w
-    PVB2_TRY(lce_pack(d, p, px, LceOperand(), rows, s));
+    PVB2_TRY(lce_pack(d, p, px, LceOperand(), rows, scale, s));
     px = LceOperand();
     rows = lce_no_rows();
+    if (!row_factors) {
+      lce_grad_rows_kernel<<<1, 1024, 0, s>>>(grad_out, target, d->N, d->V, d->ignore_index, 1.f / gscale,
+                                              p.P == 2 ? sp.scales : nullptr, sp.row, sp.factor);
+      PVB2_LAUNCH_CHECK();
+      row_factors = true;
+    }
     PVB2_TRY(lce_map_a(&g_k, sp.G, width, d->N, ldg, p));
     PVB2_TRY(lce_map_mn(&g_mn, sp.G, width, d->N, ldg, p));
     // G of this piece
@@ -1897,7 +2015,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       } else {
         g.lse = lse;
         g.grow = sp.row;
-        g.planes = p.P;
+        g.zscale = zscale;
         g.gscale = gscale;
         PVB2_TRY(lce_map(&g_store, sp.G, width, d->N, ldg, p.P, 32, p.half));
         PVB2_TRY(lce_gemm<kEpiGrad>(x_k, w_k, g_store, g, false, false, p, p.z.bn, s));
@@ -1912,7 +2030,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
         PVB2_TRY(lce_map32(&acc, sp.dx, d->D, d->N, ld32, p.dx.splits));
         PVB2_TRY(lce_gemm<kEpiAcc>(g_k, w_mn, acc, h, false, true, p, p.dx.bn, s));
       } else {
-        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, sp.factor, p.dx.bn, s));
+        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, sp.factor + 1, p.dx.bn, s));
       }
     }
     if (dw) {
@@ -1921,9 +2039,9 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       if (p.dw.splits > 1) {
         PVB2_TRY(lce_map32(&acc, sp.dw, d->D, width, ld32, p.dw.splits));
         PVB2_TRY(lce_gemm<kEpiAcc>(g_mn, x_mn, acc, h, true, true, p, p.dw.bn, s));
-        PVB2_TRY(lce_join(d, sp.dw, p.dw.splits, width, sp.factor, out, s));
+        PVB2_TRY(lce_join(d, sp.dw, p.dw.splits, width, sp.factor + 2, out, s));
       } else {
-        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, sp.factor, p.dw.bn, s));
+        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, sp.factor + 2, p.dw.bn, s));
       }
     }
     if (dbias) {
@@ -1931,7 +2049,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       PVB2_TRY(lce_bias_grad(d, p, sp, width, ldg, out, s));
     }
   }
-  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, sp.factor, dx, s));
+  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, sp.factor + 1, dx, s));
   return PVB2_OK;
 }
 

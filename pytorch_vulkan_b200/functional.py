@@ -24,9 +24,9 @@ def linear_cross_entropy(input, weight, target, bias=None, *, ignore_index=-100,
     again, piece by piece.
 
     Rows whose target is ``ignore_index`` or out of range have no loss and no
-    gradient, whatever they hold.  fp32 operands are multiplied to fp32
-    accuracy in math mode 1 and to at least 16 bits in the default mode (see
-    ``torch.ocl.set_math_mode``).
+    gradient, whatever they hold.  fp32 operands are multiplied to 22
+    bits, in either math mode (of an element below 2^-17 of its tensor's
+    largest magnitude fewer take part: those above 2^-39 of that).
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"{reduction} is not a valid value for reduction")

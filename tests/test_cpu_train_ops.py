@@ -22,7 +22,7 @@ class Tensor(ctypes.Structure):
 class Ce(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int64) for n in ("N", "D", "V", "ldx", "ldw", "ignore_index")] + [
         ("label_smoothing", ctypes.c_double), ("kept", ctypes.c_int64)] + [
-        (n, ctypes.c_int32) for n in ("dtype", "reduction", "math")]
+        (n, ctypes.c_int32) for n in ("dtype", "reduction")]
 
 
 class Adam(ctypes.Structure):
@@ -53,8 +53,7 @@ def lib():
 
 
 def ce(**kw):
-    d = dict(N=100, D=64, V=1000, ldx=64, ldw=64, ignore_index=-100, label_smoothing=0.0, kept=0, dtype=BF16, reduction=1,
-             math=1)
+    d = dict(N=100, D=64, V=1000, ldx=64, ldw=64, ignore_index=-100, label_smoothing=0.0, kept=0, dtype=BF16, reduction=1)
     d.update(kw)
     return Ce(**d)
 
@@ -76,7 +75,7 @@ def refused(lib, status, text):
 
 def test_linear_cross_entropy_refusals(lib):
     for kw, text in [
-        (dict(dtype=1), "fp32, fp16 or bf16"), (dict(reduction=3), "reduction"), (dict(math=2), "math mode"),
+        (dict(dtype=1), "fp32, fp16 or bf16"), (dict(reduction=3), "reduction"),
         (dict(V=0), "out of range"), (dict(D=0), "out of range"), (dict(N=-1), "out of range"),
         (dict(N=1 << 24), "out of range"), (dict(ldx=63), "row strides"), (dict(ldw=10), "row strides"),
         (dict(label_smoothing=-0.1), "label smoothing"), (dict(label_smoothing=float("nan")), "label smoothing"),

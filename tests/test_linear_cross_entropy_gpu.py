@@ -3,14 +3,17 @@ against F.cross_entropy of the product in float64 on the CPU.
 
 Bounds.  A logit is a sum of D products in fp32 accumulators: its error is at
 most e_z = (D + 8) u' |x||w| with u' = 2^-23 (a tensor core may cut rather than
-round), plus the part of the operands that is left out (2^-23 |x||w| for fp32
-operands in exact mode, 2^-14 in the default one, nothing for 16-bit ones).
+round), plus what two fp16 parts leave of fp32 operands: each part rounds by half
+of 2^-10, so that each operand is within 2^-22 of itself and the product of the
+second parts, which is not formed, below 2^-22 |x||w|, 3 2^-22 in all; and scaled
+so that the largest magnitude is at least 2^14, an operand's second part cannot
+be nearer than half of fp16's least step, 2^-25 / 2^14 = 2^-39 of that largest.
 The log of the sum of exponentials errs by at most the largest such error and
 2^-20 of its own; a loss by twice that.  A probability p errs by p (2 e_z +
 2^-19), and, where the forward pass kept it for 16-bit operands (a number with
 12 bits of mantissa and 4 of exponent relative to the largest of 64 columns), by
-half a step more: 2^-13 p, or 2^-27 of that largest (at most 1).  G is held in 16 bits (2^-9 for bf16, 2^-12 for fp16, 2^-23 as parts of
-fp32), and the gradients are sums of products of G, so that each is within
+half a step more: 2^-13 p, or 2^-27 of that largest (at most 1).  G is held in 16 bits (2^-9 for bf16, 2^-12 for fp16, 3 2^-22 as two of
+them for fp32, both fp16 kinds scaled by 2^15 relative to the largest row's gradient), and the gradients are sums of products of G, so that each is within
 |G| |w| (or |G|^T |x|) times those errors, the accumulation's, and one rounding
 to its type.
 """
@@ -71,8 +74,10 @@ def check(ocl, x, w, b, t, mode=1, reduction="mean", smooth=0.0, ignore=-100, gr
         gi = scored.double() * want_grad.double() / (max(n, 1) if reduction == "mean" else 1)
     with torch.no_grad():
         xa, wa = xr.abs(), ref[1].abs()
-        left_out = 0.0 if dtype != FP32 else 2.0 ** -23 if mode == 1 else 2.0 ** -14
-        ez = ((D + 8) * 2.0 ** -23 + left_out) * (xa @ wa.t()) + (2.0 ** -22 * ref[2].abs() if b is not None else 0.0)
+        left_out = 3 * 2.0 ** -22 if dtype == FP32 else 0.0
+        least = 2.0 ** -39 if dtype == FP32 else 0.0
+        ez = least * (xa.max() * wa.sum(1) + wa.max() * xa.sum(1, keepdim=True))
+        ez = ez + ((D + 8) * 2.0 ** -23 + left_out) * (xa @ wa.t()) + (2.0 ** -22 * ref[2].abs() if b is not None else 0.0)
         ez = ez + 2.0 ** -23 * z.abs()
         err = 2 * ez.max(1).values + 2.0 ** -19 * (1 + z.abs().max(1).values)
         loss_err = err * scored
@@ -97,10 +102,10 @@ def check(ocl, x, w, b, t, mode=1, reduction="mean", smooth=0.0, ignore=-100, gr
         eg = eg + 2.0 ** -22 * (p + goal) * gi.abs()[:, None]
         if dtype != FP32:
             eg = eg + (2.0 ** -13 * p + 2.0 ** -27) * gi.abs()[:, None]
-        if dtype == FP16:  # what is below fp16's steps, scaled by 2^15
+        if dtype != BF16:  # what is below fp16's steps, scaled by 2^15
             eg = eg + (2.0 ** -25 / 2 ** 15) * gi.abs().max()
-        bounds = [eg @ wa + ((V + 8) * 2.0 ** -23 + left_out) * (G @ wa),
-                  eg.t() @ xa + ((N + 8) * 2.0 ** -23 + left_out) * (G.t() @ xa),
+        bounds = [eg @ wa + ((V + 8) * 2.0 ** -23 + left_out) * (G @ wa) + least * wa.max() * G.sum(1, keepdim=True),
+                  eg.t() @ xa + ((N + 8) * 2.0 ** -23 + left_out) * (G.t() @ xa) + least * xa.max() * G.sum(0)[:, None],
                   eg.sum(0) + 2.0 ** -23 * (N + 8) * G.sum(0)]
         bounds[0] = bounds[0].reshape(x.shape)
     for name, a, r, e, leaf in zip("xwb", got, grads, bounds, used):
