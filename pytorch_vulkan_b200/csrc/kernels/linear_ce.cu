@@ -19,8 +19,8 @@
 // three products are formed: x0 w0, x0 w1 and x1 w0.  What is left out is, in
 // the mean, 2^-24 of |x||w| (3 2^-22 at most), as much as rounding the product
 // to fp32 would cost; three bf16 parts, which need no scaling, took six
-// products for the same (1.9 ms a step of N 2048, D 768, V 32768 against
-// 1.2).  fp16's range is met by a power of two for each tensor that brings its
+// products for the same (1.88 ms a step of N 2048, D 768, V 32768 against
+// 1.34).  fp16's range is met by a power of two for each tensor that brings its
 // largest finite magnitude to 2^14 .. 2^15; parts below 2^-39 of that are lost.
 //
 // G is formed for |g_i| / max|g| and, in fp16, times 2^15; all factors are
@@ -184,9 +184,9 @@ __device__ __forceinline__ void store_box(uint8_t* box, int lane, F fill_and_sto
 // CHUNK = 0 an accumulator takes the whole of K.  With CHUNK > 0 it takes CHUNK
 // blocks of K and the epilogue adds the chunks in registers: the tensor core
 // cuts rather than rounds when it adds to an accumulator, so that a sum over
-// thousands of products drifts by 2^-24 of itself for every 16 of them.  Split
-// operands are chunked by the K block, their small products first, so that only
-// the four additions of the main one are cut at its size.
+// thousands of products drifts by 2^-24 of itself for every 16 of them.  Of
+// split operands each K block's lesser products come first, so that in a
+// chunk's first block only the main one's additions are cut at its size.
 template <int EPI, typename T, int P, int BN, int CHUNK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THREADS), 1)
     lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -195,7 +195,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
   constexpr bool kPrecise = P > 1;
   constexpr int kCols = L::COLS;            // columns of an epilogue warp
   constexpr int kSlots = L::SLOTS;
-  static_assert(CHUNK == 1 || P == 1, "split operands: a chunk for each K block");
+  static_assert(CHUNK || P == 1, "split operands are summed in chunks");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = (uint64_t*)(smem + L::BAR_OFF);  // waited on in the even CTA
@@ -328,7 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
             if (P == 2) {
               const int s1 = (it + 1) % kSlots;
               arrived(it + 1);
-              product(s1, s0, true);
+              product(s1, s0, kb == c0);
               product(s0, s1, false);
               mma_commit_pair(&empty[s1]);
             }
@@ -585,20 +585,20 @@ struct LcePackJob {
 // Scales of split operands.  One block's largest finite magnitudes of x (rows
 // that have a loss) come first in `part`, then those of w; each block of a
 // later launch reduces them anew.
-constexpr int kLScaleBlocks = 296;
+constexpr int kLScaleBlocks = 296;  // of x's and w's together: two blocks of 1024 threads for each SM
 struct LceScaleJob {
   const float* part;      // NULL: nothing is scaled
   int nx, nw;
   float* scales;          // 1 / s_x and 1 / s_w, written by the first block
 };
 
-// 2^k that brings m to [2^14, 2^15) (k in [-112, 120]), 1 for 0
+// 2^k that brings m to [2^14, 2^15) (k in [-113, 120]), 1 for 0
 __device__ __forceinline__ float lce_pow2(float m) {
   const int e = (int)(__float_as_uint(m) >> 23) - 127;
   return m == 0.f ? 1.f : __uint_as_float((uint32_t)(127 + min(120, 14 - e)) << 23);
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024, 2)
     lce_absmax_kernel(const float* __restrict__ x, int64_t rows_x, int64_t ldx, const float* __restrict__ w,
                       int64_t rows_w, int64_t ldw, int64_t cols, const int64_t* __restrict__ target, int64_t V,
                       int64_t ignore, int nx, float* __restrict__ part) {
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(256)
     v = fabsf(v);
     m = v <= 3.402823466e38f ? fmaxf(m, v) : m;  // neither infinity nor NaN
   };
-  for (int64_t r = block * 8 + warp; r < rows; r += blocks * 8) {
+  for (int64_t r = block * 32 + warp; r < rows; r += blocks * 32) {
     if (is_x && !lce_scored(target[r], V, ignore)) continue;
     const float* row = src + r * ld;
     if (vec) {
@@ -630,13 +630,13 @@ __global__ void __launch_bounds__(256)
       for (int64_t c = lane; c < cols; c += 32) take(row[c]);
     }
   }
-  __shared__ float s[8];
+  __shared__ float s[32];
   m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
   if (lane == 0) s[warp] = m;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int q = 1; q < 8; ++q) m = fmaxf(m, s[q]);
-    part[blockIdx.x] = m;
+  if (warp == 0) {
+    m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s[lane])));
+    if (lane == 0) part[blockIdx.x] = m;
   }
 }
 
@@ -1476,7 +1476,7 @@ static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   const bool slabs = lce_slabs(p);
   s->x = a.take<uint16_t>(!p.few && p.pack_x ? rows * p.ldp * p.P : 0);
   s->w = a.take<uint16_t>(!p.few && p.pack_w ? p.piece * p.ldp * p.P : 0);
-  s->absmax = a.take<float>(!p.few && p.P == 2 ? 2 * kLScaleBlocks : 0);
+  s->absmax = a.take<float>(!p.few && p.P == 2 ? kLScaleBlocks : 0);
   s->scales = a.take<float>(2);
   s->slab = a.take<float>(slabs ? p.z.splits * rows * up(d->V, 4) : 0);
   s->part = a.take<float2>(slabs ? 0 : rows * parts);
@@ -1500,7 +1500,7 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   s->G = a.take<uint16_t>(d->N * up(width, 64) * p.P);
   s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
-  s->absmax = a.take<float>(p.P == 2 ? 2 * kLScaleBlocks : 0);
+  s->absmax = a.take<float>(p.P == 2 ? kLScaleBlocks : 0);
   s->scales = a.take<float>(2);
   s->factor = a.take<float>(3);
   s->dx = a.take<float>(p.pieces > 1 || (d->kept > 0 && d->kept < d->V) || p.dx.splits > 1 ? p.dx.splits * d->N * ld32 : 0);
@@ -1585,15 +1585,17 @@ static int lce_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensor
   return PVB2_OK;
 }
 
-// Chunks: split operands (results to fp32) every block, four additions of the
-// main product; 16-bit ones every 8 on 256 x 128 tiles, which wait for their
+// Chunks: split operands (results to fp32) every two blocks (N 2048, D 768, V
+// 16384, mean error of losses and gradients: 6e-8 and 3.4e-7, where a product in
+// fp32 has 6e-8 and 6 to 8e-7; every block 5e-8 and 2e-7, but a step of V 32768
+// takes 1.21 ms instead of 1.00; every three 5e-7 and 0.98 ms); 16-bit ones every 8 on 256 x 128 tiles, which wait for their
 // loads anyway, and every 16 where the result is fp32 (the losses: up to 2e-6
 // off without, 3e-7 with, for 3% of the forward product's time).
 template <int EPI>
 static int lce_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const LceGemm& g, bool a_mn,
                     bool b_mn, const LcePlan& p, int bn, cudaStream_t s) {
-  if (p.P == 2 && bn == 256) return lce_launch<EPI, __half, 2, 256, 1>(a, b, c, g, a_mn, b_mn, s);
-  if (p.P == 2) return lce_launch<EPI, __half, 2, 128, 1>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 2 && bn == 256) return lce_launch<EPI, __half, 2, 256, 2>(a, b, c, g, a_mn, b_mn, s);
+  if (p.P == 2) return lce_launch<EPI, __half, 2, 128, 2>(a, b, c, g, a_mn, b_mn, s);
   if (p.half) {
     if (bn == 256) return lce_launch<EPI, __half, 1, 256, EPI == kEpiStats ? 16 : 0>(a, b, c, g, a_mn, b_mn, s);
     return lce_launch<EPI, __half, 1, 128, 8>(a, b, c, g, a_mn, b_mn, s);
@@ -1637,10 +1639,11 @@ static int lce_scales(const pvb2_linear_ce_desc* d, const LcePlan& p, const void
   *job = LceScaleJob{nullptr, 0, 0, nullptr};
   if (p.P == 1) return PVB2_OK;
   job->part = absmax;
-  job->nx = (int)std::min<int64_t>(kLScaleBlocks, cdiv(d->N * d->D, 8192));
-  job->nw = (int)std::min<int64_t>(kLScaleBlocks, cdiv(d->V * d->D, 8192));
+  const int64_t blocks = std::min<int64_t>(kLScaleBlocks, std::max<int64_t>(2, cdiv((d->N + d->V) * d->D, 16384)));
+  job->nx = (int)std::min(blocks - 1, std::max<int64_t>(1, blocks * d->N / (d->N + d->V)));
+  job->nw = (int)blocks - job->nx;
   job->scales = scales;
-  lce_absmax_kernel<<<job->nx + job->nw, 256, 0, s>>>((const float*)x, d->N, d->ldx, (const float*)w, d->V, d->ldw, d->D,
+  lce_absmax_kernel<<<job->nx + job->nw, 1024, 0, s>>>((const float*)x, d->N, d->ldx, (const float*)w, d->V, d->ldw, d->D,
                                                       target, d->V, d->ignore_index, job->nx, absmax);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
