@@ -690,8 +690,9 @@ typedef struct pvb2_linear_ce_desc {
  * (0: none); that memory goes to the forward pass, and, as it left it, to
  * the backward pass with the same descriptor. */
 PVB2_API size_t pvb2_linear_ce_keep(pvb2_linear_ce_desc* d, size_t budget);
-/* out: N losses (PVB2_LOSS_NONE) or one; lse: N; count: one float, the
- * number of rows that have a loss.  mean over no rows is NaN. */
+/* out: N losses (PVB2_LOSS_NONE) or one; lse: N; count: three floats, the
+ * number of rows that have a loss and two that the backward pass reads.
+ * mean over no rows is NaN. */
 PVB2_API size_t pvb2_linear_ce_fwd_workspace_size(const pvb2_linear_ce_desc* d);
 PVB2_API int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias,
                                 const int64_t* target, float* out, float* lse, float* count, void* kept,

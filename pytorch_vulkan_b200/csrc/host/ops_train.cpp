@@ -449,7 +449,7 @@ static size_t ce_keep_budget() {
 }
 
 struct CeForward {
-  at::Tensor loss, lse, count;  // lse: of each row; count: rows that have a loss
+  at::Tensor loss, lse, count;  // lse: of each row; count: rows that have a loss, and the operands' scales
   at::Tensor kept;              // what the backward pass takes, of the first `entries` classes (undefined: none)
   int64_t entries = 0;
 };
@@ -481,7 +481,7 @@ static CeForward linear_cross_entropy_forward(const at::Tensor& input, const at:
     r.entries = d.kept;
   }
   at::Tensor loss = reduction == PVB2_LOSS_NONE ? empty(target.sizes(), at::kFloat, dev) : empty({}, at::kFloat, dev);
-  at::Tensor lse = empty({d.N}, at::kFloat, dev), count = empty({}, at::kFloat, dev);
+  at::Tensor lse = empty({d.N}, at::kFloat, dev), count = empty({3}, at::kFloat, dev);
   Workspace ws(pvb2_linear_ce_fwd_workspace_size(&d), dev);
   OCL_CHECK(pvb2_linear_ce_fwd(&d, x.data_ptr(), w.data_ptr(), b.defined() ? b.data_ptr() : nullptr,
                                (const int64_t*)t.data_ptr(), (float*)loss.data_ptr(), (float*)lse.data_ptr(),
@@ -502,7 +502,7 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backw
   const int64_t rows = target.numel();
   TORCH_CHECK(is_ocl(grad) && grad.scalar_type() == at::kFloat && grad.numel() == (reduction == 0 ? rows : 1) &&
                   is_ocl(lse) && lse.scalar_type() == at::kFloat && lse.numel() == rows && lse.is_contiguous() &&
-                  is_ocl(count) && count.scalar_type() == at::kFloat && count.numel() == 1,
+                  is_ocl(count) && count.scalar_type() == at::kFloat && count.numel() == 3 && count.is_contiguous(),
               "ocl linear_cross_entropy_backward: gradient or saved tensors do not fit");
   DeviceScope scope(dev);
   OCL_OP("linear_cross_entropy_backward", dev);

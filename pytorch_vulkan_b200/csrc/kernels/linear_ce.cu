@@ -587,9 +587,10 @@ struct LcePackJob {
 // later launch reduces them anew.
 constexpr int kLScaleBlocks = 296;  // of x's and w's together: two blocks of 1024 threads for each SM
 struct LceScaleJob {
-  const float* part;      // NULL: nothing is scaled
+  const float* part;      // or NULL
   int nx, nw;
   float* scales;          // 1 / s_x and 1 / s_w, written by the first block
+  const float* given;     // these two from the forward pass, or NULL
 };
 
 // 2^k that brings m to [2^14, 2^15) (k in [-113, 120]), 1 for 0
@@ -613,21 +614,24 @@ __global__ void __launch_bounds__(1024, 2)
     v = fabsf(v);
     m = v <= 3.402823466e38f ? fmaxf(m, v) : m;  // neither infinity nor NaN
   };
-  for (int64_t r = block * 32 + warp; r < rows; r += blocks * 32) {
+  // a warp takes 512 columns of a row at a time
+  const int64_t segs = (cols + 511) / 512;
+  for (int64_t i = block * 32 + warp; i < rows * segs; i += blocks * 32) {
+    const int64_t r = i <= INT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)segs) : i / segs, c0 = (i - r * segs) * 512;
     if (is_x && !lce_scored(target[r], V, ignore)) continue;
     const float* row = src + r * ld;
-    if (vec) {
-#pragma unroll 4
-      for (int64_t c = lane * 4; c + 4 <= cols; c += 128) {
-        const float4 q = *reinterpret_cast<const float4*>(row + c);
-        take(q.x);
-        take(q.y);
-        take(q.z);
-        take(q.w);
+    if (vec && c0 + 512 <= cols) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 v = *reinterpret_cast<const float4*>(row + c0 + q * 128 + lane * 4);
+        take(v.x);
+        take(v.y);
+        take(v.z);
+        take(v.w);
       }
-      for (int64_t c = cols / 4 * 4 + lane; c < cols; c += 32) take(row[c]);
     } else {
-      for (int64_t c = lane; c < cols; c += 32) take(row[c]);
+#pragma unroll 4
+      for (int64_t c = c0 + lane; c < min(cols, c0 + 512); c += 32) take(row[c]);
     }
   }
   __shared__ float s[32];
@@ -691,7 +695,10 @@ __global__ void __launch_bounds__(256)
     lce_pack_kernel(LcePackJob<S> a, LcePackJob<S> b, LceRowsJob rj, LceScaleJob sj, int64_t cols, int64_t ldp,
                     int planes, int64_t V, int64_t ignore) {
   float sx = 1.f, sw = 1.f;  // of a and of b
-  if (sj.part) {
+  if (sj.given) {
+    sx = 1.f / sj.given[0];  // powers of two
+    sw = 1.f / sj.given[1];
+  } else if (sj.part) {
     __shared__ float smax[2][8];
     float mx = 0.f, mw = 0.f;
     for (int q = threadIdx.x; q < sj.nx + sj.nw; q += 256) {
@@ -1332,6 +1339,10 @@ static pvb2_linear_ce_desc lce_normal(const pvb2_linear_ce_desc* d) {
   return n;
 }
 
+static bool lce_few_rows(const pvb2_linear_ce_desc* d, int64_t ldp) {
+  return d->N <= kLFewRows && kLFewRows * ldp * (d->dtype == PVB2_F32 ? 4 : 2) <= kLFewBytes;
+}
+
 static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
   LcePlan p;
   p.half = d->dtype != PVB2_BF16;
@@ -1344,8 +1355,7 @@ static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
   // 4095 tokens, 196 and 244 us at 2048).
   p.pack_w = !lce_direct(d, d->ldw) || (d->ldw % 64 != 0 && d->D >= 256 && d->N >= 3500);
   p.pack_x = !lce_direct(d, d->ldx) || (d->ldx % 64 != 0 && d->D >= 256 && d->V >= 2048);
-  const int size = d->dtype == PVB2_F32 ? 4 : 2;
-  p.few = !backward && d->N <= kLFewRows && (int64_t)kLFewRows * p.ldp * size <= kLFewBytes;
+  p.few = !backward && lce_few_rows(d, p.ldp);
   const int64_t rows = backward ? d->N : std::min(d->N, kLRowsFwd);
   const int64_t esize = 2 * p.P;
   // most entries of a piece: a packed piece of w in 256 MB, G in 128 MB, at
@@ -1451,7 +1461,7 @@ static size_t lce_kept_space(const pvb2_linear_ce_desc* d, bool fp32, const void
 
 struct LceFwdSpace {
   uint16_t *x, *w;
-  float *absmax, *scales;
+  float* absmax;
   float* slab;
   float2* part;
   float *zsum, *ztarget, *loss;
@@ -1477,7 +1487,6 @@ static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   s->x = a.take<uint16_t>(!p.few && p.pack_x ? rows * p.ldp * p.P : 0);
   s->w = a.take<uint16_t>(!p.few && p.pack_w ? p.piece * p.ldp * p.P : 0);
   s->absmax = a.take<float>(!p.few && p.P == 2 ? kLScaleBlocks : 0);
-  s->scales = a.take<float>(2);
   s->slab = a.take<float>(slabs ? p.z.splits * rows * up(d->V, 4) : 0);
   s->part = a.take<float2>(slabs ? 0 : rows * parts);
   s->zsum = a.take<float>(!slabs && d->label_smoothing != 0 ? rows * parts : 0);
@@ -1500,8 +1509,9 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   s->G = a.take<uint16_t>(d->N * up(width, 64) * p.P);
   s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
-  s->absmax = a.take<float>(p.P == 2 ? kLScaleBlocks : 0);
-  s->scales = a.take<float>(2);
+  const bool scales = p.P == 2 && lce_few_rows(d, p.ldp);
+  s->absmax = a.take<float>(scales ? kLScaleBlocks : 0);
+  s->scales = a.take<float>(scales ? 2 : 0);
   s->factor = a.take<float>(3);
   s->dx = a.take<float>(p.pieces > 1 || (d->kept > 0 && d->kept < d->V) || p.dx.splits > 1 ? p.dx.splits * d->N * ld32 : 0);
   s->dw = a.take<float>(p.dw.splits > 1 ? p.dw.splits * width * ld32 : 0);
@@ -1636,7 +1646,6 @@ static int lce_pack(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceOpe
 // the scales of split operands: their magnitudes, for the launches that pack
 static int lce_scales(const pvb2_linear_ce_desc* d, const LcePlan& p, const void* x, const void* w,
                       const int64_t* target, float* absmax, float* scales, LceScaleJob* job, cudaStream_t s) {
-  *job = LceScaleJob{nullptr, 0, 0, nullptr};
   if (p.P == 1) return PVB2_OK;
   job->part = absmax;
   const int64_t blocks = std::min<int64_t>(kLScaleBlocks, std::max<int64_t>(2, cdiv((d->N + d->V) * d->D, 16384)));
@@ -1784,10 +1793,10 @@ static int lce_kept_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const L
 template <typename T>
 static int lce_slab_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, const void* bias,
                          const int64_t* target, const float* lse, int64_t v0, int64_t width, int64_t ldg, float gscale,
-                         cudaStream_t s) {
+                         const float* zscale, cudaStream_t s) {
   lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target, v0,
                                                  width, d->V, d->ignore_index, (float)d->label_smoothing, lse, sp.row,
-                                                 gscale, (T*)sp.G, ldg, p.P, p.P == 2 ? sp.scales : nullptr);
+                                                 gscale, (T*)sp.G, ldg, p.P, zscale);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -1847,9 +1856,9 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
                    "linear cross entropy: 16-byte aligned memory for what is kept needed");
     LceKept k;
     lce_kept_space(d, d->dtype == PVB2_F32 || p.few || slabs, kept, &k);
-    LceScaleJob scale;
-    if (!p.few) PVB2_TRY(lce_scales(d, p, x, w, target, sp.absmax, sp.scales, &scale, s));
-    const float* zscale = p.P == 2 ? sp.scales : nullptr;
+    LceScaleJob scale{};
+    if (!p.few) PVB2_TRY(lce_scales(d, p, x, w, target, sp.absmax, count + 1, &scale, s));
+    const float* zscale = p.P == 2 ? count + 1 : nullptr;
     for (int64_t r0 = 0; r0 < d->N; r0 += kLRowsFwd) {
       const int64_t rows = std::min(kLRowsFwd, d->N - r0);
       CUtensorMap ma, mb;
@@ -1961,9 +1970,12 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   const bool direct_w = !p.pack_w, slabs = lce_slabs(p);
   PVB2_TRY(lce_aligned(w, direct_w));
   const float gscale = p.half ? 32768.f : 1.f;
-  LceScaleJob scale;
-  PVB2_TRY(lce_scales(d, p, x, w, target, sp.absmax, sp.scales, &scale, s));
-  const float* zscale = p.P == 2 ? sp.scales : nullptr;
+  // the forward pass found the scales, unless its rows were few
+  LceScaleJob scale{};
+  const bool given = p.P == 2 && !lce_few_rows(d, p.ldp);
+  if (given) scale.given = count + 1;
+  else PVB2_TRY(lce_scales(d, p, x, w, target, sp.absmax, sp.scales, &scale, s));
+  const float* zscale = given ? count + 1 : p.P == 2 ? sp.scales : nullptr;
   LceRowsJob rows = lce_no_rows();
   if (d->reduction != PVB2_LOSS_NONE)
     rows = LceRowsJob{sp.row, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
@@ -1999,7 +2011,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     rows = lce_no_rows();
     if (!row_factors) {
       lce_grad_rows_kernel<<<1, 1024, 0, s>>>(grad_out, target, d->N, d->V, d->ignore_index, 1.f / gscale,
-                                              p.P == 2 ? sp.scales : nullptr, sp.row, sp.factor);
+                                              zscale, sp.row, sp.factor);
       PVB2_LAUNCH_CHECK();
       row_factors = true;
     }
@@ -2013,8 +2025,8 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       LceGemm g = lce_logits(d, bias, d->N, v0, width, row0, target);
       if (slabs) {
         PVB2_TRY(lce_slab_logits(d, p, x_k, w_k, g, sp.slab, s));
-        if (p.half) PVB2_TRY(lce_slab_grad<__half>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, s));
-        else PVB2_TRY(lce_slab_grad<__nv_bfloat16>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, s));
+        if (p.half) PVB2_TRY(lce_slab_grad<__half>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, zscale, s));
+        else PVB2_TRY(lce_slab_grad<__nv_bfloat16>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, zscale, s));
       } else {
         g.lse = lse;
         g.grow = sp.row;
