@@ -12,16 +12,21 @@
 // whatever the row's shift and the row's alignment in memory, each 16-byte
 // store then takes one aligned 16-byte load from the copy that fits.
 //
-// Backward: a block owns 512 diagonals, two a thread, and walks down the rows
-// of one head, so that the diagonals' sums stay in registers; at the end it
-// adds those of each bucket in order.  32 rows (16 of fp32) at a time of the
-// slanted strip that the diagonals cut out go to shared memory by 16-byte
-// asynchronous copies, the next ones while these are added (a thread that
-// loaded its own elements, two bytes each and at odd addresses, reached a
-// third of this rate).  Sums are fp32 over at most 64 rows and fp64
-// beyond; nothing is added in an order that depends on timing.
+// Backward: a block owns 248 diagonals and walks down the rows of one head; at
+// the end it adds those of each bucket in order.  16 bytes of a row begin on a
+// boundary, and the row below it is shifted by an element against the
+// diagonals; but 8 rows further the boundary is at the same diagonals again,
+// whatever the row stride.  So a warp takes every eighth row, 256 elements from
+// the boundary before its first diagonal, and its lanes' 16-byte loads meet the
+// same 8 diagonals in each: their sums stay in registers, and nothing is staged
+// or shifted.  Loads at a row's ends reach into what lies beside it, as far as
+// the gradient itself reaches, and the foreign elements are set to 0 (16 x 4096
+// x 4096 bf16: 109 us; 158 with slanted strips staged in shared memory, from
+// which threads read their diagonals' two bytes; 142 where loads at the ends
+// were guarded one by one; 118 with 504 diagonals a block, which meet more ends).
+// Sums are fp32 over at most 64 rows and fp64 beyond; nothing is added in an
+// order that depends on timing.
 #include <math.h>
-#include <atomic>
 #include <vector>
 #include "types.cuh"
 
@@ -30,9 +35,7 @@ namespace pvb2 {
 constexpr int kRelMaxBuckets = 512;
 constexpr int kRelCols = 1024;   // columns of a forward block
 constexpr int kRelRows = 64;     // most rows of a block
-constexpr int kRelDiag = 512;    // diagonals of a block in the backward pass
-template <typename T>
-constexpr int kRelStage = 64 / (int)sizeof(T);  // rows that are staged at a time
+constexpr int kRelDiag = 248;    // diagonals of a block in the backward pass
 constexpr int kRelInf = 1 << 30;
 
 struct RelMap {  // bucket b holds r in [lo[b], hi[b]] (empty where lo > hi)
@@ -86,135 +89,171 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-__device__ __forceinline__ void copy_async16(void* dst, const void* src, int bytes) {  // zeros behind `bytes`
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
-               "r"(bytes)
-               : "memory");
-}
-
-// grid: (segments of the rows) x (tiles of 512 diagonals) x (B * H); part:
-// [B*H][tiles][segments][nb].  FLAT: unit stride along the keys.
+// grid: (segments of the rows) x (tiles of diagonals) x (B * H); part:
+// [B*H][nb][tiles][segments].  FLAT: unit stride along the keys; the gradient's
+// first element is at `low`, its last one 16 bytes before `high`.
 template <typename T, bool FLAT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
     rel_bias_bwd_kernel(const __grid_constant__ RelMap map, const T* __restrict__ grad, int64_t sb, int64_t sh,
-                        int64_t si, int64_t sj, double* __restrict__ part, int H, int Lq, int Lk, int q_offset) {
-  constexpr int V = 16 / sizeof(T);            // elements of a 16-byte copy
-  constexpr int kVecs = kRelDiag / V + 1;      // of a row's strip, wherever it begins
-  constexpr int kPitch = (kVecs + 1) * V;
-  constexpr int kRows = kRelStage<T>;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  T* stages = reinterpret_cast<T*>(smem_raw);  // [2][kRows][kPitch]
-  __shared__ double diag[kRelDiag];
+                        int64_t si, int64_t sj, double* __restrict__ part, int H, int Lq, int Lk, int q_offset,
+                        int per, const T* low, const T* high) {
+  constexpr int V = 16 / sizeof(T);  // elements of a 16-byte load
+  constexpr int M = 8 / V;           // loads of a row, 256 elements for a warp
+  constexpr int U = 8 / M;           // rows in flight
+  __shared__ double sums[FLAT ? 8 : 1][FLAT ? kRelDiag : 1], diag[kRelDiag];
   const int seg = blockIdx.x, tile = blockIdx.y;
   const int64_t z = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int d0 = tile * kRelDiag - (Lq - 1);  // first diagonal j - i
-  // rows that these diagonals meet, and this segment's share of them
+  const int parts = gridDim.y * gridDim.x;
+  double* p = part + z * map.nb * parts + tile * gridDim.x + seg;  // of bucket 0
+  // of the rows that these diagonals meet `per`
   const int ra = max(0, -(d0 + kRelDiag - 1)), rb = min(Lq, Lk - d0);
-  const int per = (max(0, rb - ra) + (int)gridDim.x - 1) / (int)gridDim.x;
   const int i0 = ra + seg * per, i1 = min(rb, i0 + per);
-  const T* g = grad + (z / H) * sb + (z % H) * sh;
-  const int e0 = (int)threadIdx.x;
-  // elements from the 16-byte boundary to the first of row i0's strip; one row
-  // further it is si + 1 elements more
-  const int lead0 = (int)(((uintptr_t)(g + (int64_t)i0 * si + d0 + i0) & 15) / sizeof(T));
-  const int lead_step = (int)((si + 1) & (V - 1));
-
-  // row i + r: columns d0 + i + r .., 512 of them, from the 16-byte boundary before
-  auto fetch = [&](int i) {
-    T* stage = stages + ((i - i0) / kRows & 1) * kRows * kPitch;
-    const int rows = min(kRows, i1 - i);
-    if (FLAT) {
-      for (int r = warp; r < rows; r += 8) {
-        const T* row = g + (int64_t)(i + r) * si;
-        const int c0 = d0 + i + r - ((lead0 + (i - i0 + r) * lead_step) & (V - 1));
-#pragma unroll
-        for (int kk = 0; kk < kVecs; kk += 32) {
-          const int k = kk + lane, c = c0 + k * V;
-          if (k >= kVecs) continue;
-          T* to = stage + r * kPitch + k * V;
-          if (c >= 0 || c + V <= 0) {
-            const int n = c < 0 ? 0 : max(0, min(V, Lk - c));
-            if (n > 0) copy_async16(to, row + c, n * (int)sizeof(T));
-            else *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
-          } else {  // begins before the row
-            for (int j = 0; j < V; ++j) to[j] = c + j >= 0 && c + j < Lk ? row[c + j] : from_f32<T>(0.f);
-          }
-        }
-      }
-    } else {
-      for (int q = threadIdx.x; q < rows * kRelDiag; q += 256) {
-        const int r = q / kRelDiag, k = q - r * kRelDiag, c = d0 + i + r + k;
-        stage[r * kPitch + k] = c >= 0 && c < Lk ? g[(int64_t)(i + r) * si + (int64_t)c * sj] : from_f32<T>(0.f);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-
-  double acc0 = 0.0, acc1 = 0.0;
-  float s0 = 0.f, s1 = 0.f;
-  int held = 0;
-  if (i0 < i1) fetch(i0);
-  for (int i = i0; i < i1; i += kRows) {
-    const int rows = min(kRows, i1 - i);
-    if (i + kRows < i1) {
-      fetch(i + kRows);
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-    } else {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-    }
-    __syncthreads();
-    if (held + rows > 64) {
-      acc0 += (double)s0;
-      acc1 += (double)s1;
-      s0 = s1 = 0.f;
-      held = 0;
-    }
-    held += rows;
-    const T* stage = stages + ((i - i0) / kRows & 1) * kRows * kPitch + e0;
-    const int l0 = FLAT ? lead0 + (i - i0) * lead_step : 0;
-    if (rows == kRows) {
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0);
-        s0 += to_f32(x[0]);
-        s1 += to_f32(x[256]);
-      }
-    } else {
-      for (int r = 0; r < rows; ++r) {
-        const T* x = stage + r * kPitch + (FLAT ? (l0 + r * lead_step) & (V - 1) : 0);
-        s0 += to_f32(x[0]);
-        s1 += to_f32(x[256]);
-      }
-    }
-    __syncthreads();  // the stage may be filled again
+  if (i0 >= i1) {
+    for (int b = threadIdx.x; b < map.nb; b += 256) p[(int64_t)b * parts] = 0.0;
+    return;
   }
-  diag[e0] = acc0 + (double)s0;
-  diag[e0 + 256] = acc1 + (double)s1;
+  const T* g = grad + ((int)blockIdx.z / H) * sb + ((int)blockIdx.z % H) * sh;
+
+  if (FLAT) {
+    const int first = i0 + warp;
+    // elements from the 16-byte boundary to the first diagonal: the same in every eighth row
+    const int lead = (int)(((uintptr_t)(g + (int64_t)first * si + d0 + first) & 15) / sizeof(T));
+    for (int e = lane; e < kRelDiag; e += 32) sums[warp][e] = 0.0;
+    __syncwarp();
+    float s[M][V];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[m][j] = 0.f;
+    int held = 0;
+    const int64_t step = 8 * (si + 1);
+    // only the first and the last rows of all can meet an end
+    const bool ends = g + (int64_t)i0 * si < low + V || g + (int64_t)(i1 - 1) * si + Lk > high;
+    auto flush = [&]() {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int e = (m * 32 + lane) * V + j - lead;
+          if (e >= 0 && e < kRelDiag) sums[warp][e] += (double)s[m][j];
+          s[m][j] = 0.f;
+        }
+      held = 0;
+    };
+    for (int i = first; i < i1; i += 8 * U) {
+      uint4 v[U][M];
+      const int c0 = d0 + i - lead + lane * V;  // column of load m of row u: c0 + 8 u + 32 V m
+      const T* at0 = g + (int64_t)i * si + c0;
+      held += U;
+      if (d0 + i >= lead && d0 + i + 8 * (U - 1) - lead + 32 * V * M <= Lk && i + 8 * (U - 1) < i1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int m = 0; m < M; ++m) v[u][m] = *reinterpret_cast<const uint4*>(at0 + u * step + 32 * V * m);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            float x[V];
+            unpack_vec<V, T>(RawVec<16>{v[u][m]}, x);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[m][j] += x[j];
+          }
+        if (held == 64) flush();
+        continue;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int c = c0 + 8 * u + 32 * V * m;
+          const T* at = at0 + u * step + 32 * V * m;
+          v[u][m] = make_uint4(0u, 0u, 0u, 0u);
+          if (i + 8 * u < i1 && c > -V && c < Lk && at >= low && at <= high) v[u][m] = *reinterpret_cast<const uint4*>(at);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int c = c0 + 8 * u + 32 * V * m;
+          float x[V];
+          unpack_vec<V, T>(RawVec<16>{v[u][m]}, x);
+          if (c < 0 || c + V > Lk) {  // what lies beside the row
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = c + j >= 0 && c + j < Lk ? x[j] : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < V; ++j) s[m][j] += x[j];
+        }
+      if (ends) {  // loads that would reach beyond the whole gradient
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            const int c = c0 + 8 * u + 32 * V * m;
+            const T* at = at0 + u * step + 32 * V * m;
+            if (i + 8 * u < i1 && c > -V && c < Lk && !(at >= low && at <= high)) {
+#pragma unroll
+              for (int j = 0; j < V; ++j)
+                if (c + j >= 0 && c + j < Lk) s[m][j] += to_f32(at[j]);
+            }
+          }
+      }
+      if (held == 64) flush();
+    }
+    flush();
+    __syncthreads();
+    for (int e = threadIdx.x; e < kRelDiag; e += 256) {
+      double t = 0.0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t += sums[w][e];
+      diag[e] = t;
+    }
+  } else {
+    for (int e = threadIdx.x; e < kRelDiag; e += 256) {
+      double t = 0.0;
+      for (int i = i0; i < i1; i += 64) {
+        float s = 0.f;
+#pragma unroll 4
+        for (int q = i; q < min(i1, i + 64); ++q) {
+          const int c = d0 + q + e;
+          if (c >= 0 && c < Lk) s += to_f32(g[(int64_t)q * si + (int64_t)c * sj]);
+        }
+        t += (double)s;
+      }
+      diag[e] = t;
+    }
+  }
   __syncthreads();
-  double* p = part + ((z * gridDim.y + tile) * gridDim.x + seg) * map.nb;
   const int r0 = d0 - q_offset;
   for (int b = warp; b < map.nb; b += 8) {
     const int lo = max(map.lo[b], r0), hi = min(map.hi[b], r0 + kRelDiag - 1);
+    if (lo > hi) {
+      if (lane == 0) p[(int64_t)b * parts] = 0.0;
+      continue;
+    }
     double s = 0.0;
     for (int r = lo + lane; r <= hi; r += 32) s += diag[r - r0];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) p[b] = s;
+    if (lane == 0) p[(int64_t)b * parts] = s;
   }
 }
 
 // one warp per (bucket, head)
 template <typename T>
-__global__ void rel_bias_sum_kernel(const double* __restrict__ part, T* __restrict__ dtable, int nb, int H, int64_t B,
-                                    int64_t per_z) {
+__global__ void rel_bias_sum_kernel(const double* __restrict__ part, T* __restrict__ dtable, int nb, int H, int B,
+                                    int per_z) {
   const int w = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (w >= nb * H) return;
   const int b = w / H, h = w % H;
   double s = 0.0;
-  for (int64_t q = lane; q < B * per_z; q += 32) {
-    const int64_t z = (q / per_z) * H + h;
-    s += part[(z * per_z + q % per_z) * nb + b];
+#pragma unroll 8
+  for (uint32_t q = lane; q < (uint32_t)(B * per_z); q += 32) {
+    const uint32_t at = q / (uint32_t)per_z;  // of the batch
+    s += part[((int64_t)(at * H + h) * nb + b) * per_z + (q - at * per_z)];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -273,6 +312,7 @@ static int rel_check(const pvb2_relative_bias_desc* d) {
 }
 
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
 // rows of a block: as many as keep four blocks for every SM (fewer rows, more
 // blocks: a block's fixed work, the diagonals, is shared by its rows)
@@ -284,14 +324,19 @@ static int rel_rows(int64_t heads, int64_t Lq, int64_t across) {
 
 struct RelBwdPlan {
   int64_t tiles, segments;
+  int per;  // rows of a segment
 };
 
-// segments of the rows: eight blocks for every SM, no fewer than 32 rows each
+// Rows of a segment: as many as leave five blocks for every SM (16 x 4096 x 4096
+// bf16: 118 us with three, 109 with five, 115 with twelve), at least 128 (12 x
+// 197 x 4096: 19 us, 22 with 64).  Every row meets as many tiles as its columns
+// take, and a tile at most Lk + 247 rows.
 static RelBwdPlan rel_bwd_plan(const pvb2_relative_bias_desc* d, int64_t B) {
   RelBwdPlan p;
   p.tiles = cdiv(d->Lq + d->Lk - 1, kRelDiag);
-  const int64_t want = cdiv(8 * (int64_t)num_sms(), std::max<int64_t>(1, B * d->H * p.tiles));
-  p.segments = std::max<int64_t>(1, std::min(want, cdiv(d->Lq, 32)));
+  const double visits = (double)B * d->H * d->Lq * (1.0 + (double)d->Lk / kRelDiag);
+  p.per = (int)std::max<int64_t>(128, up((int64_t)std::min<double>(1 << 28, visits / (5.0 * num_sms())), 32));
+  p.segments = cdiv(std::min(d->Lq, d->Lk + kRelDiag - 1), p.per);
   return p;
 }
 
@@ -314,23 +359,21 @@ static int rel_bwd(const pvb2_relative_bias_desc* d, const RelMap& m, const pvb2
   const RelBwdPlan p = rel_bwd_plan(d, B);
   int64_t per_z = 0;
   if (B > 0 && d->Lq > 0 && d->Lk > 0) {
-    PVB2_CHECK_ARG(B * d->H <= 65535 && p.tiles <= 65535, "relative bias: batch x heads or lengths out of range");
+    PVB2_CHECK_ARG(B * d->H <= 65535 && p.tiles <= 65535 && B * p.tiles * p.segments <= INT32_MAX,
+                   "relative bias: batch x heads or lengths out of range");
     per_z = p.tiles * p.segments;
-    constexpr int smem = 2 * kRelStage<T> * (kRelDiag + 2 * 16 / (int)sizeof(T)) * (int)sizeof(T);
-    static std::atomic<uint64_t> attr_done{0};
-    if (first_on_device(attr_done)) {
-      PVB2_CUDA_TRY(cudaFuncSetAttribute(rel_bias_bwd_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      PVB2_CUDA_TRY(cudaFuncSetAttribute(rel_bias_bwd_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    }
+    int64_t extent = 1;
+    for (int k = 0; k < 4; ++k) extent += (g->sizes[k] - 1) * g->strides[k];
     const dim3 grid((unsigned)p.segments, (unsigned)p.tiles, (unsigned)(B * d->H));
     auto kernel = g->strides[3] == 1 || d->Lk == 1 ? rel_bias_bwd_kernel<T, true> : rel_bias_bwd_kernel<T, false>;
-    kernel<<<grid, 256, smem, s>>>(m, (const T*)g->data, g->strides[0], g->strides[1], g->strides[2], g->strides[3],
-                                   part, d->H, (int)d->Lq, (int)d->Lk, (int)d->q_offset);
+    kernel<<<grid, 256, 0, s>>>(m, (const T*)g->data, g->strides[0], g->strides[1], g->strides[2], g->strides[3],
+                                   part, d->H, (int)d->Lq, (int)d->Lk, (int)d->q_offset, p.per, (const T*)g->data,
+                                 (const T*)g->data + extent - 16 / (int)sizeof(T));
     PVB2_LAUNCH_CHECK();
   }
   const int warps = m.nb * d->H;
-  rel_bias_sum_kernel<T><<<(int)cdiv(warps, 8), 256, 0, s>>>(part, (T*)dtable, m.nb, d->H, per_z ? B : 0,
-                                                             std::max<int64_t>(per_z, 1));
+  rel_bias_sum_kernel<T><<<(int)cdiv(warps, 8), 256, 0, s>>>(part, (T*)dtable, m.nb, d->H, (int)(per_z ? B : 0),
+                                                             (int)std::max<int64_t>(per_z, 1));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }

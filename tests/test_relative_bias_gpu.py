@@ -1,8 +1,8 @@
 """Learned relative position bias on `ocl` against its definition: buckets by
 whole-number arithmetic, values exact, gradients summed in float64.
 
-A table's gradient is summed in fp32 over at most 64 rows of a diagonal and in
-float64 beyond, then rounded once to the table's type: its error is at most
+A table's gradient is summed in fp32 over at most 64 rows of a diagonal, or 64
+elements of a row where one bucket holds all, and in float64 beyond, then rounded once to the table's type: its error is at most
 64 * 2^-24 of the sum of magnitudes and half a step of the result.
 """
 import math
@@ -50,6 +50,8 @@ CASES = [
     (3, 16, 16, 8, True, 100, 1000),      # every key far behind
     (3, 16, 16, 8, False, 100, -1000),    # every key far ahead
     (1, 300, 2100, 512, False, 1 << 20, 7),
+    (2, 37, 5003, 32, True, 40, 2600),    # long runs of one bucket before and behind the others
+    (2, 90, 5003, 32, False, 40, 2600),
     (2, 0, 5, 8, True, 9, 0),
     (2, 5, 0, 8, True, 9, 0),
 ]
@@ -97,6 +99,7 @@ def test_gradient_strides_and_batches(ocl):
     check(h.to(DEV).permute(0, 3, 2, 1), h.permute(0, 3, 2, 1))
     w = torch.randn(2, H, q, 2 * k + 1, generator=gen)
     check(w.to(DEV)[..., 1::2], w[..., 1::2])
+    check(w.to(DEV)[..., 1:k + 1], w[..., 1:k + 1])
     check(g.to(DEV)[:0], g[:0])
 
 
