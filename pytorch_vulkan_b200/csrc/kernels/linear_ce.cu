@@ -919,7 +919,9 @@ __global__ void __launch_bounds__(512)
 // Here a warp reads R of w's rows at once, each lane 16 bytes of each, and
 // multiplies them by the NT rows of x from shared memory in fp32; its lanes
 // then keep the running maximum and sum of their row of x.  One V = 32768, D =
-// 2048 fp16 row: 25 us against 54.
+// 2048 fp16 row: 25 us against 54.  R fills the registers: four rows of w for
+// one row of x in fp32 (V 32768, D 2048: 55 us, 75 with eight), four for eight
+// (87 us, 101 with two, where x's reads from shared memory bound it).
 template <int L>
 __device__ __forceinline__ float sum_spread(float (&a)[L], int lane) {
   // sums of L values over the warp, value i in the lanes i * 32 / L ..
@@ -1339,8 +1341,13 @@ static pvb2_linear_ce_desc lce_normal(const pvb2_linear_ce_desc* d) {
   return n;
 }
 
+// Five to eight 16-bit rows go there while w is below 64 MB (768 x 8000: 17 us
+// against 21 on tiles); beyond, the products in fp32 cost more than w's slower
+// reads (2048 x 32768: 64 and 55 us, 4096 x 50000: 150 and 117).  fp32 tiles need
+// three products and w's parts (768 x 32768: 45 us for eight rows, 115 for nine).
 static bool lce_few_rows(const pvb2_linear_ce_desc* d, int64_t ldp) {
-  return d->N <= kLFewRows && kLFewRows * ldp * (d->dtype == PVB2_F32 ? 4 : 2) <= kLFewBytes;
+  const int64_t most = d->dtype == PVB2_F32 || d->V * d->D < (1 << 25) ? kLFewRows : 4;
+  return d->N <= most && kLFewRows * ldp * (d->dtype == PVB2_F32 ? 4 : 2) <= kLFewBytes;
 }
 
 static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
@@ -1755,10 +1762,10 @@ static int lce_few_launch(const pvb2_linear_ce_desc* d, const void* x, const voi
 template <typename S>
 static int lce_few(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* target,
                    const LceFwdSpace& sp, const LceKept& k, cudaStream_t s) {
-  if (d->N == 1) return lce_few_launch<S, 1, 8>(d, x, w, bias, target, sp, k, s);
+  if (d->N == 1) return lce_few_launch<S, 1, sizeof(S) == 4 ? 4 : 8>(d, x, w, bias, target, sp, k, s);
   if (d->N == 2) return lce_few_launch<S, 2, 4>(d, x, w, bias, target, sp, k, s);
   if (d->N <= 4) return lce_few_launch<S, 4, 4>(d, x, w, bias, target, sp, k, s);
-  return lce_few_launch<S, 8, 2>(d, x, w, bias, target, sp, k, s);
+  return lce_few_launch<S, 8, 4>(d, x, w, bias, target, sp, k, s);
 }
 
 // logits of `rows` rows as partial sums
