@@ -180,6 +180,14 @@ __device__ __forceinline__ void store_box(uint8_t* box, int lane, F fill_and_sto
   }
 }
 
+// the two factors that undo the scales of x and w on a logit: their product and
+// 1, unless that is beyond fp32
+__device__ __forceinline__ float2 lce_unscale(const float* scales) {
+  if (!scales) return make_float2(1.f, 1.f);
+  const float a = scales[0], b = scales[1], both = a * b;
+  return both >= 1e-37f && both <= 1e37f ? make_float2(both, 1.f) : make_float2(a, b);
+}
+
 // One tile: C[256 x BN] by a pair of CTAs, in two accumulators in turn.  With
 // CHUNK = 0 an accumulator takes the whole of K.  With CHUNK > 0 it takes CHUNK
 // blocks of K and the epilogue adds the chunks in registers: the tensor core
@@ -366,7 +374,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
           }
         }
       }
-      const float zscale0 = P == 2 && p.zscale ? p.zscale[0] : 1.f, zscale1 = P == 2 && p.zscale ? p.zscale[1] : 1.f;
+      const float2 unscale = lce_unscale(P == 2 ? p.zscale : nullptr);
       const float flat = EPI == kEpiGrad ? p.smoothing / (float)p.V : 0.f;
       const float oscale = EPI == kEpiOut && p.out_scale ? *p.out_scale : 1.f;
       float mx = -INFINITY, sum = 0.f, zs = 0.f;
@@ -410,7 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
         }
         if ((EPI == kEpiStats || EPI == kEpiGrad) && P == 2) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = v[j] * zscale0 * zscale1;  // their product may be beyond fp32
+          for (int j = 0; j < 64; ++j) v[j] = v[j] * unscale.x * unscale.y;
         }
         // whether any of the warp's targets is among these columns
         const bool has_target = (EPI == kEpiStats || EPI == kEpiGrad) &&
@@ -868,7 +876,7 @@ __global__ void __launch_bounds__(512)
                          float* __restrict__ lse, float* __restrict__ loss, float* __restrict__ kept, int64_t keep,
                          int64_t keep_ld, float* __restrict__ ztarget, const float* __restrict__ zscale) {
   __shared__ float sm[16], ss[16], sz[16], zt;
-  const float2 unscale = zscale ? make_float2(zscale[0], zscale[1]) : make_float2(1.f, 1.f);
+  const float2 unscale = lce_unscale(zscale);
   const int64_t i = blockIdx.x, t = target[i];
   const bool scored = lce_scored(t, V, ignore);
   float mx = -INFINITY, sum = 0.f, zs = 0.f;
@@ -1054,7 +1062,7 @@ __global__ void __launch_bounds__(256)
                          int bias_dtype, const int64_t* __restrict__ target, int64_t v0, int64_t width, int64_t V,
                          int64_t ignore, float smoothing, const float* __restrict__ lse, const float* __restrict__ grow,
                          float gscale, T* __restrict__ G, int64_t ldg, int planes, const float* __restrict__ zscale) {
-  const float2 unscale = zscale ? make_float2(zscale[0], zscale[1]) : make_float2(1.f, 1.f);
+  const float2 unscale = lce_unscale(zscale);
   const int64_t i = blockIdx.x, tt = target[i];
   const int64_t t = lce_scored(tt, V, ignore) ? tt - v0 : -1;
   const float l = lse[i], g = grow[i], flat = smoothing / (float)V;

@@ -242,6 +242,20 @@ def test_extreme_logits(ocl, math_fp32):
         assert all(torch.isfinite(g.cpu()).all() for g in torch.autograd.grad(loss, leaves))
 
 
+@pytest.mark.parametrize("size", [(150, 72, 520), (20, 1000, 90), (4, 40, 60)], ids=["tiles", "slabs", "few"])
+def test_operands_of_extreme_magnitude(ocl, math_fp32, size):
+    """fp32 operands whose scales are far from 1, in both directions, and a row far above the others."""
+    x, w, b, t = make(*size, FP32, bias=True)
+    for s in (1e30, 1e-30):
+        check(ocl, x * s, w / s, b, t)
+    check(ocl, x * 1e-25, w * 1e-20, b, t, reduction="sum")
+    x[1] *= 1e4
+    check(ocl, x, w, None, t, reduction="none")
+    x[1] = 1e38
+    t[1] = -100
+    check(ocl, x, w, b, t)
+
+
 def test_strides_offsets_and_shapes(ocl):
     for dtype in (BF16, FP32):
         x, w, b, t = make(6 * 20, 56, 300, dtype, bias=True)
