@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(512)
   const int64_t i = blockIdx.x, t = target[i];
   const bool scored = lce_scored(t, V, ignore);
   float mx = -INFINITY, sum = 0.f, zs = 0.f;
-  for (int64_t n = threadIdx.x; n < V; n += 512) {
+  for (int64_t n = threadIdx.x; n < V; n += blockDim.x) {
     const float z = lce_slab_logit(slab, S, rows * ld, i * ld + n, bias, n, bias_dtype, unscale);
     if (n < keep) kept[i * keep_ld + n] = z;
     if (scored && n == t) zt = z;
@@ -903,7 +903,7 @@ __global__ void __launch_bounds__(512)
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int q = 1; q < 16; ++q) {
+    for (int q = 1; q < (int)blockDim.x / 32; ++q) {
       const float nm = fmaxf(mx, sm[q]), base = nm == -INFINITY ? 0.f : nm;
       sum = sum * expf(mx - base) + ss[q] * expf(sm[q] - base);
       mx = nm;
@@ -1921,15 +1921,19 @@ int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
           PVB2_TRY(lce_gemm<kEpiStats>(ma, mb, mk, g, false, false, p, p.z.bn, s));
         }
       }
-      if (slabs)
-        lce_slab_rows_kernel<<<(int)rows, 512, 0, s>>>(
+      if (slabs) {
+        // two logits a thread (7663 rows of 24: 117 us with 512 threads, 10 with 32)
+        int threads = 32;
+        while (threads < 512 && 2 * threads < d->V) threads *= 2;
+        lce_slab_rows_kernel<<<(int)rows, threads, 0, s>>>(
             sp.slab, p.z.splits, rows, up(d->V, 4), bias, d->dtype, target + r0, d->V, d->ignore_index, smoothing,
             lse + r0, loss + r0, (float*)k.data + r0 * k.ld, d->kept, k.ld, d->kept ? k.ztarget + r0 : nullptr,
             zscale);
-      else
+      } else {
         lce_rows_kernel<<<(int)cdiv(rows, 32), 1024, 0, s>>>(
             sp.part, smoothing != 0.f ? sp.zsum : nullptr, rows, parts, d->kept ? k.ztarget + r0 : sp.ztarget,
             target + r0, rows, d->V, d->ignore_index, smoothing, lse + r0, loss + r0);
+      }
       PVB2_LAUNCH_CHECK();
     }
   }

@@ -120,7 +120,7 @@ def check(ocl, x, w, b, t, mode=1, reduction="mean", smooth=0.0, ignore=-100, gr
 SIZES = [
     (1, 1, 1), (1, 8, 2), (2, 3, 5), (127, 64, 255), (128, 64, 256), (129, 72, 257), (64, 100, 1000), (33, 513, 129),
     (300, 40, 2500), (1, 2048, 4099), (257, 65, 1025), (700, 200, 300),
-    (6, 4104, 8200),
+    (6, 4104, 8200), (3000, 520, 24), (700, 1713, 70),
 ]
 
 
