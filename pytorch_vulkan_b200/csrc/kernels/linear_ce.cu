@@ -465,7 +465,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
           sum = sum * lce_exp<kPrecise>(mx - nb) + cs * lce_exp<kPrecise>(cm - nb);
           mx = nm;
           if (!kPrecise && keep && m0 < p.M) {
-            if (mrow) p.keep_max[(int64_t)((p.v0 + n0) >> 6) * p.keep_ld + m] = base;
+            // -inf where all 64 are masked, whose codes are 0: any finite number there could make the factor that the
+            // backward pass forms of it, exp(maximum - lse), infinite
+            if (mrow) p.keep_max[(int64_t)((p.v0 + n0) >> 6) * p.keep_ld + m] = cm;
             store_box(box, lane, [&](int phase) {
               if (phase == 0) box_codes(box, lane, v);
               else tma_store_3d(&tmC, box, p.v0 + n0, m0, 0);

@@ -1,0 +1,105 @@
+"""Gradients of functional.linear_cross_entropy where rows, vocabulary entries
+or operands differ by many powers of ten, and at sizes whose tiles outnumber
+the SM pairs, against the formula in float64 (on the GPU's CUDA device, for the
+larger sizes' sake).
+
+Bounds.  As in the other tests of this operator: a logit errs by e_z = (D + 8)
+2^-23 |x||w|, for fp32 operands 3 2^-22 |x||w| more and 2^-39 of each operand's
+largest magnitude, and 2^-23 of itself; a loss by twice the row's largest e_z and
+2^-19 (1 + |z|).  A probability errs by p times that, and by 2^-13 p + 2^-27
+where it was kept in 16 bits.  What the products read, G_ij = p_ij - goal_ij,
+rounds to 16 bits: 2^-9 of itself in bf16, 2^-12 in fp16 (each taken as twice
+that here), 3 2^-22 as two fp16 parts, and 2^-40 as least step of either fp16
+kind.  For dx that is of a G without the row's own gradient g_i, which multiplies
+the row afterwards: the errors of dx_i are g_i times the row's.  For dw, G_ij is
+relative to the largest |g| of all rows.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "ocl:0"
+FP32, BF16, FP16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=["fp32", "bf16", "fp16"])
+KEEP = pytest.mark.parametrize("keep", ["0", "2048"], ids=["formed", "kept"])
+HALF = {FP32: 2.0 ** -24, BF16: 2.0 ** -8, FP16: 2.0 ** -11}
+
+
+def make(N, D, V, dtype, bias=False, ignored=0.0, seed=0):
+    g = torch.Generator().manual_seed(seed + 7 * N + 3 * D + V)
+    w = (torch.randn(V, D, generator=g) / D ** 0.5).to(dtype)
+    t = torch.randint(0, V, (N,), generator=g)
+    x = (torch.randn(N, D, generator=g) + 3 * torch.rand(N, 1, generator=g) * w[t].float()).to(dtype)
+    b = (torch.randn(V, generator=g) * 0.5).to(dtype) if bias else None
+    t[torch.rand(N, generator=g) < ignored] = -100
+    return x, w, b, t
+
+
+def run(ocl, x, w, b, t, grad=None, **kw):
+    leaves = [v.to(DEV).requires_grad_() for v in (x, w, b) if v is not None]
+    loss = ocl.functional.linear_cross_entropy(leaves[0], leaves[1], t.to(DEV), leaves[2] if b is not None else None, **kw)
+    got = torch.autograd.grad(loss, leaves, grad.to(DEV) if grad is not None else None)
+    return [loss.detach().cpu(), *(g.cpu() for g in got)]
+
+
+def formula(x, w, b, t, gi, smooth=0.0, on="cpu"):
+    """The losses of the rows, and dx, dw, db for row gradients gi (0 for rows without a loss), each with its bound."""
+    dtype, (N, D), V = x.dtype, x.shape, w.shape[0]
+    x, w, t, gi = x.double().to(on), w.double().to(on), t.to(on), gi.double().to(on)
+    at = t.clamp(min=0)[:, None]
+    z = x @ w.t()
+    if b is not None:
+        z += b.double().to(on)
+    logp = torch.log_softmax(z, 1)
+    losses = -(1 - smooth) * logp.gather(1, at)[:, 0] - smooth * logp.mean(1)
+    left_out = 3 * 2.0 ** -22 if dtype == FP32 else 0.0
+    least = 2.0 ** -39 if dtype == FP32 else 0.0
+    xa, wa, ga = x.abs(), w.abs(), gi.abs()
+    ez = least * (xa.max() * wa.sum(1) + wa.max() * xa.sum(1, keepdim=True)) + ((D + 8) * 2.0 ** -23 + left_out) * (xa @ wa.t())
+    err = (2 * (ez + 2.0 ** -22 * z.abs()).max(1).values + 2.0 ** -19 * (1 + z.abs().max(1).values))[:, None]
+    p = logp.exp_()
+    G = p - smooth / V
+    G.scatter_add_(1, at, torch.full_like(G[:, :1], smooth - 1))
+    dx, dw, db = (G @ w) * gi[:, None], (G * gi[:, None]).t() @ x, gi @ G
+    one = G.abs_()
+    eg = p * (err + 2.0 ** -19 + 2.0 ** -22) + one * {FP32: left_out, BF16: 2.0 ** -8, FP16: 2.0 ** -11}[dtype] + 2.0 ** -22 * smooth / V
+    eg.scatter_add_(1, at, torch.full_like(eg[:, :1], 2.0 ** -22))
+    if dtype != FP32:
+        eg += 2.0 ** -13 * p + 2.0 ** -27
+    step = 0.0 if dtype == BF16 else 2.0 ** -40
+    row = (eg + step) @ wa + ((V + 10) * 2.0 ** -23 + left_out) * (one @ wa) + least * wa.max() * one.sum(1, keepdim=True)
+    eg, one = eg * ga[:, None] + step * ga.max(), one * ga[:, None]
+    col = eg.t() @ xa + ((N + 10) * 2.0 ** -23 + left_out) * (one.t() @ xa) + least * xa.max() * one.sum(0)[:, None]
+    bounds = [row * ga[:, None], col, eg.sum(0) + (N + 10) * 2.0 ** -23 * one.sum(0)]
+    grads = [dx, dw, db]
+    bounds = [e + HALF[dtype] * (r.abs() + e) + (2.0 ** -25 if dtype == FP16 else 1e-44) for r, e in zip(grads, bounds)]
+    return losses, err[:, 0], grads, bounds
+
+
+def within(got, want, bound, what):
+    got = got.double().to(want.device)
+    assert torch.isfinite(got).all(), what
+    over = ((got - want).abs() - bound).max().item()
+    assert over <= 0, f"{what}: over its bound by {over}"
+
+
+@TYPES
+@KEEP
+@pytest.mark.parametrize("shift", [0.0, 30.0, 200.0])
+def test_whole_groups_masked_by_the_bias(ocl, monkeypatch, math_fp32, dtype, keep, shift):
+    """Entries whose bias is -inf, 64 neighbours and more of them, take no part, however small the others' logits are."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    x, w, b, t = make(70, 32, 1200, dtype, bias=True)
+    out = torch.zeros(1200, dtype=torch.bool)
+    out[100:600] = out[700:1100] = True
+    b[~out] -= shift
+    b[out] = float("-inf")
+    left = torch.nonzero(~out)[:, 0]
+    t = left[t % len(left)]
+    loss, dx, dw, db = run(ocl, x, w, b, t, reduction="sum")
+    place = torch.cumsum(~out, 0) - 1
+    losses, err, grads, bounds = formula(x, w[left], b[left], place[t], torch.ones(70))
+    assert (loss.double() - losses.sum()).abs() <= err.sum() + 2.0 ** -23 * losses.sum()
+    for a, r, e, what in zip((dx, dw[left], db[left]), grads, bounds, "xwb"):
+        within(a, r, e, what)
+    assert (dw[out] == 0).all() and (db[out] == 0).all()
