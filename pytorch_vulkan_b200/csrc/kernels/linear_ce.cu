@@ -23,8 +23,11 @@
 // 1.34).  fp16's range is met by a power of two for each tensor that brings its
 // largest finite magnitude to 2^14 .. 2^15; parts below 2^-39 of that are lost.
 //
-// G is formed for |g_i| / max|g| and, in fp16, times 2^15; all factors are
-// undone on the fp32 results.
+// G is formed without the factor that all rows share and, in fp16, times 2^15;
+// both are undone on the fp32 results.  Where each row has a gradient g_i of its
+// own, dx multiplies its rows by g_i at the end, so that a row's errors are
+// relative to itself, and what is not finite in one reaches no other; dw and db,
+// sums over rows, take a second G, of g_i / max|g|.
 #include <algorithm>
 #include <atomic>
 #include "tc_common.cuh"
@@ -93,7 +96,7 @@ struct LceGemm {
   float* keep_max;        // what their exponentials are relative to: [64-column groups][keep_ld]
   int64_t keep_ld;
   const float* lse;       // kEpiGrad
-  const float* grow;      // kEpiGrad: g_i / max|g| (0 for rows without a loss)
+  const float* grow;      // kEpiGrad: the rows' factors (0 for rows without a loss)
   const float* zscale;    // two factors of the logits, on the device, for split operands
   float gscale;
   // kEpiAcc / kEpiOut
@@ -102,6 +105,7 @@ struct LceGemm {
   int64_t out_ld;
   int out_dtype, out_tma;
   const float* out_scale; // kEpiOut: factor on the device
+  const float* out_row;   // kEpiOut: a factor for each row, or NULL
 };
 
 // the bias of 64 columns added to a row's logits: each lane fetches two, all
@@ -377,6 +381,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
       const float2 unscale = lce_unscale(P == 2 ? p.zscale : nullptr);
       const float flat = EPI == kEpiGrad ? p.smoothing / (float)p.V : 0.f;
       const float oscale = EPI == kEpiOut && p.out_scale ? *p.out_scale : 1.f;
+      const float orow = EPI == kEpiOut && p.out_row && mrow ? p.out_row[m] : 1.f;
       float mx = -INFINITY, sum = 0.f, zs = 0.f;
       float v[64];
       bool ok = true;
@@ -513,7 +518,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] *= oscale;
+          for (int j = 0; j < 64; ++j) v[j] = v[j] * oscale * orow;
           if (!p.out_tma) {
             // through the box, rotated by the row: lanes then write along rows
 #pragma unroll
@@ -1183,12 +1188,13 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// the rows' factors where each has a gradient of its own: g_i / max |g| and
-// that maximum
+// the rows' factors where each has a gradient of its own: whether it has a loss
+// (one) and g_i (own; 0 without a loss) for dx, and for the sums over rows
+// g_i / max |g| (row) with that maximum in their common factors
 __global__ void __launch_bounds__(1024)
     lce_grad_rows_kernel(const float* __restrict__ grad_out, const int64_t* __restrict__ target, int64_t N, int64_t V,
                          int64_t ignore, float inv_gscale, const float* __restrict__ scales, float* __restrict__ row,
-                         float* __restrict__ factor) {
+                         float* __restrict__ one, float* __restrict__ own, float* __restrict__ factor) {
   __shared__ float s_max[32];
   float mx = 0.f;
   for (int64_t i = threadIdx.x; i < N; i += 1024)
@@ -1204,20 +1210,27 @@ __global__ void __launch_bounds__(1024)
   __syncthreads();
   mx = s_max[0];
   for (int w = 1; w < 32; ++w) mx = (s_max[w] > mx || s_max[w] != s_max[w]) ? s_max[w] : mx;
-  for (int64_t i = threadIdx.x; i < N; i += 1024)
-    row[i] = lce_scored(target[i], V, ignore) && mx != 0.f ? grad_out[i] / mx : 0.f;
+  for (int64_t i = threadIdx.x; i < N; i += 1024) {
+    const bool scored = lce_scored(target[i], V, ignore);
+    const float g = grad_out[i];
+    row[i] = scored && mx != 0.f ? g / mx : 0.f;
+    one[i] = scored ? 1.f : 0.f;
+    own[i] = scored ? g : 0.f;
+  }
   if (threadIdx.x == 0) {
     const float f = mx * inv_gscale;
     factor[0] = f;
-    factor[1] = scales ? f * scales[1] : f;
+    factor[1] = scales ? inv_gscale * scales[1] : inv_gscale;
     factor[2] = scales ? f * scales[0] : f;
   }
 }
 
-// out [rows][cols] = factor * sum of S slabs [rows][ld], four columns a thread
+// out [rows][cols] = factor * sum of S slabs [rows][ld], times each row's own
+// factor where there are some; four columns a thread
 template <typename T>
 __global__ void lce_join_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t cols, int64_t ld,
-                                const float* __restrict__ factor, T* __restrict__ out, int vec) {
+                                const float* __restrict__ factor, const float* __restrict__ own, T* __restrict__ out,
+                                int vec) {
   const float f = *factor;
   const int per_row = (int)(ld / 4);
   const int64_t total = rows * per_row, size = rows * ld;
@@ -1232,8 +1245,9 @@ __global__ void lce_join_kernel(const float* __restrict__ slab, int S, int64_t r
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] += u[k];
     }
+    const float g = own ? own[r] : 1.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] *= f;
+    for (int k = 0; k < 4; ++k) v[k] = v[k] * f * g;
     if (vec) {
       store_vec<4>(out + r * cols + c, v);
     } else {
@@ -1516,6 +1530,7 @@ struct LceBwdSpace {
   uint16_t *x, *w, *G;
   float *absmax, *scales;
   float *slab, *row, *factor, *dx, *dw, *colsum;  // factor: of db, dx and dw
+  float *one, *own;                               // where each row has its own gradient: see lce_grad_rows_kernel
 };
 
 static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceBwdSpace* s) {
@@ -1526,6 +1541,8 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   s->G = a.take<uint16_t>(d->N * up(width, 64) * p.P);
   s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
+  s->one = a.take<float>(d->reduction == PVB2_LOSS_NONE ? d->N : 0);
+  s->own = a.take<float>(d->reduction == PVB2_LOSS_NONE ? d->N : 0);
   const bool scales = p.P == 2 && lce_few_rows(d, p.ldp);
   s->absmax = a.take<float>(scales ? kLScaleBlocks : 0);
   s->scales = a.take<float>(scales ? 2 : 0);
@@ -1682,13 +1699,13 @@ static LceRowsJob lce_no_rows() {
 }
 
 // out = factor * (sum of slabs), as the operands' type
-static int lce_join(const pvb2_linear_ce_desc* d, const float* slab, int S, int64_t rows, const float* factor, void* out,
-                    cudaStream_t s) {
+static int lce_join(const pvb2_linear_ce_desc* d, const float* slab, int S, int64_t rows, const float* factor,
+                    const float* own, void* out, cudaStream_t s) {
   const int64_t ld = up(d->D, 4);
   const int grid = grid_for(rows * (ld / 4), 256), vec = d->D % 4 == 0 && ((uintptr_t)out & 15) == 0;
-  if (d->dtype == PVB2_F32) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (float*)out, vec);
-  else if (d->dtype == PVB2_F16) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (__half*)out, vec);
-  else lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, (__nv_bfloat16*)out, vec);
+  if (d->dtype == PVB2_F32) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, own, (float*)out, vec);
+  else if (d->dtype == PVB2_F16) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, own, (__half*)out, vec);
+  else lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, own, (__nv_bfloat16*)out, vec);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -1735,13 +1752,14 @@ static CUtensorMap no_map() {
 
 // the product A B (K not cut) into `out`, rows x D
 static int lce_out(const pvb2_linear_ce_desc* d, const LcePlan& p, const CUtensorMap& a, const CUtensorMap& b, LceGemm g,
-                   bool a_mn, int64_t rows, void* out, const float* factor, int bn, cudaStream_t s) {
+                   bool a_mn, int64_t rows, void* out, const float* factor, const float* own, int bn, cudaStream_t s) {
   const int size = d->dtype == PVB2_F32 ? 4 : 2;
   CUtensorMap c = no_map();
   g.out = out;
   g.out_ld = d->D;
   g.out_dtype = d->dtype;
   g.out_scale = factor;
+  g.out_row = own;
   g.out_tma = ((uintptr_t)out & 15) == 0 && d->D * size % 16 == 0;
   if (g.out_tma) {
     if (size == 4) PVB2_TRY(lce_map32(&c, out, d->D, rows, d->D, 1));
@@ -1790,18 +1808,18 @@ static int lce_slab_logits(const pvb2_linear_ce_desc* d, const LcePlan& p, const
 
 template <typename T>
 static int lce_kept_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, const LceKept& k,
-                         const int64_t* target, const float* lse, int64_t v0, int64_t width, int64_t ldg, float gscale,
-                         cudaStream_t s) {
+                         const int64_t* target, const float* lse, const float* grow, int64_t v0, int64_t width, int64_t ldg,
+                         float gscale, cudaStream_t s) {
   const unsigned rows = (unsigned)std::min<int64_t>(d->N, 32768);
   const dim3 grid((unsigned)cdiv(ldg, k.fp32 ? 4096 : 8192), rows, (unsigned)cdiv(d->N, rows));
   const float smoothing = (float)d->label_smoothing;
   if (k.fp32)
     lce_kept_grad_kernel<T, true><<<grid, 256, 0, s>>>(k.data, k.ld, k.max, k.ztarget, d->N, target, v0, width, d->V,
-                                                       d->ignore_index, smoothing, lse, sp.row, gscale, (T*)sp.G, ldg,
+                                                       d->ignore_index, smoothing, lse, grow, gscale, (T*)sp.G, ldg,
                                                        p.P);
   else
     lce_kept_grad_kernel<T, false><<<grid, 256, 0, s>>>(k.data, k.ld, k.max, k.ztarget, d->N, target, v0, width, d->V,
-                                                        d->ignore_index, smoothing, lse, sp.row, gscale, (T*)sp.G, ldg,
+                                                        d->ignore_index, smoothing, lse, grow, gscale, (T*)sp.G, ldg,
                                                         p.P);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
@@ -1809,10 +1827,10 @@ static int lce_kept_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const L
 
 template <typename T>
 static int lce_slab_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, const void* bias,
-                         const int64_t* target, const float* lse, int64_t v0, int64_t width, int64_t ldg, float gscale,
-                         const float* zscale, cudaStream_t s) {
+                         const int64_t* target, const float* lse, const float* grow, int64_t v0, int64_t width,
+                         int64_t ldg, float gscale, const float* zscale, cudaStream_t s) {
   lce_slab_grad_kernel<<<(int)d->N, 256, 0, s>>>(sp.slab, p.z.splits, d->N, up(width, 4), bias, d->dtype, target, v0,
-                                                 width, d->V, d->ignore_index, (float)d->label_smoothing, lse, sp.row,
+                                                 width, d->V, d->ignore_index, (float)d->label_smoothing, lse, grow,
                                                  gscale, (T*)sp.G, ldg, p.P, zscale);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
@@ -2000,7 +2018,8 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   LceRowsJob rows = lce_no_rows();
   if (d->reduction != PVB2_LOSS_NONE)
     rows = LceRowsJob{sp.row, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
-  bool row_factors = d->reduction != PVB2_LOSS_NONE;  // or still to be formed, after the scales
+  const bool own = d->reduction == PVB2_LOSS_NONE;  // each row has its own gradient
+  bool row_factors = !own;                          // or still to be formed, after the scales
   LceOperand px{x, 0, d->N, d->ldx, sp.x, target};
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;
   PVB2_TRY(lce_map_a(&x_k, sp.x, d->D, d->N, p.ldp, p));
@@ -2032,31 +2051,35 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     rows = lce_no_rows();
     if (!row_factors) {
       lce_grad_rows_kernel<<<1, 1024, 0, s>>>(grad_out, target, d->N, d->V, d->ignore_index, 1.f / gscale,
-                                              zscale, sp.row, sp.factor);
+                                              zscale, sp.row, sp.one, sp.own, sp.factor);
       PVB2_LAUNCH_CHECK();
       row_factors = true;
     }
     PVB2_TRY(lce_map_a(&g_k, sp.G, width, d->N, ldg, p));
     PVB2_TRY(lce_map_mn(&g_mn, sp.G, width, d->N, ldg, p));
-    // G of this piece
-    if (from_kept) {
-      if (p.half) PVB2_TRY(lce_kept_grad<__half>(d, p, sp, k, target, lse, v0, width, ldg, gscale, s));
-      else PVB2_TRY(lce_kept_grad<__nv_bfloat16>(d, p, sp, k, target, lse, v0, width, ldg, gscale, s));
-    } else {
+    // G of this piece, for one kind of row factors
+    bool logits = false;  // those of the slabs are there
+    auto form = [&](const float* grow) {
+      if (from_kept) {
+        if (p.half) return lce_kept_grad<__half>(d, p, sp, k, target, lse, grow, v0, width, ldg, gscale, s);
+        return lce_kept_grad<__nv_bfloat16>(d, p, sp, k, target, lse, grow, v0, width, ldg, gscale, s);
+      }
       LceGemm g = lce_logits(d, bias, d->N, v0, width, row0, target);
       if (slabs) {
-        PVB2_TRY(lce_slab_logits(d, p, x_k, w_k, g, sp.slab, s));
-        if (p.half) PVB2_TRY(lce_slab_grad<__half>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, zscale, s));
-        else PVB2_TRY(lce_slab_grad<__nv_bfloat16>(d, p, sp, bias, target, lse, v0, width, ldg, gscale, zscale, s));
-      } else {
-        g.lse = lse;
-        g.grow = sp.row;
-        g.zscale = zscale;
-        g.gscale = gscale;
-        PVB2_TRY(lce_map(&g_store, sp.G, width, d->N, ldg, p.P, 32, p.half));
-        PVB2_TRY(lce_gemm<kEpiGrad>(x_k, w_k, g_store, g, false, false, p, p.z.bn, s));
+        if (!logits) PVB2_TRY(lce_slab_logits(d, p, x_k, w_k, g, sp.slab, s));
+        logits = true;
+        if (p.half)
+          return lce_slab_grad<__half>(d, p, sp, bias, target, lse, grow, v0, width, ldg, gscale, zscale, s);
+        return lce_slab_grad<__nv_bfloat16>(d, p, sp, bias, target, lse, grow, v0, width, ldg, gscale, zscale, s);
       }
-    }
+      g.lse = lse;
+      g.grow = grow;
+      g.zscale = zscale;
+      g.gscale = gscale;
+      PVB2_TRY(lce_map(&g_store, sp.G, width, d->N, ldg, p.P, 32, p.half));
+      return lce_gemm<kEpiGrad>(x_k, w_k, g_store, g, false, false, p, p.z.bn, s);
+    };
+    PVB2_TRY(form(dx && own ? sp.one : sp.row));
     if (dx) {
       LceGemm h = lce_product(d->N, d->D, width, row0, p.dx);
       if (dx_slabs) {
@@ -2066,8 +2089,9 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
         PVB2_TRY(lce_map32(&acc, sp.dx, d->D, d->N, ld32, p.dx.splits));
         PVB2_TRY(lce_gemm<kEpiAcc>(g_k, w_mn, acc, h, false, true, p, p.dx.bn, s));
       } else {
-        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, sp.factor + 1, p.dx.bn, s));
+        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, sp.factor + 1, own ? sp.own : nullptr, p.dx.bn, s));
       }
+      if (own && (dw || dbias)) PVB2_TRY(form(sp.row));
     }
     if (dw) {
       LceGemm h = lce_product(width, d->D, d->N, 0, p.dw);
@@ -2075,9 +2099,9 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       if (p.dw.splits > 1) {
         PVB2_TRY(lce_map32(&acc, sp.dw, d->D, width, ld32, p.dw.splits));
         PVB2_TRY(lce_gemm<kEpiAcc>(g_mn, x_mn, acc, h, true, true, p, p.dw.bn, s));
-        PVB2_TRY(lce_join(d, sp.dw, p.dw.splits, width, sp.factor + 2, out, s));
+        PVB2_TRY(lce_join(d, sp.dw, p.dw.splits, width, sp.factor + 2, nullptr, out, s));
       } else {
-        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, sp.factor + 2, p.dw.bn, s));
+        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, sp.factor + 2, nullptr, p.dw.bn, s));
       }
     }
     if (dbias) {
@@ -2085,7 +2109,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       PVB2_TRY(lce_bias_grad(d, p, sp, width, ldg, out, s));
     }
   }
-  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, sp.factor + 1, dx, s));
+  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, sp.factor + 1, own ? sp.own : nullptr, dx, s));
   return PVB2_OK;
 }
 

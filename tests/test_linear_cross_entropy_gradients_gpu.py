@@ -103,3 +103,49 @@ def test_whole_groups_masked_by_the_bias(ocl, monkeypatch, math_fp32, dtype, kee
     for a, r, e, what in zip((dx, dw[left], db[left]), grads, bounds, "xwb"):
         within(a, r, e, what)
     assert (dw[out] == 0).all() and (db[out] == 0).all()
+
+
+ROWS = pytest.mark.parametrize("size", [(150, 72, 520), (20, 1000, 90), (5, 40, 600), (1500, 24, 47003)],
+                               ids=["tiles", "slabs", "few", "pieces"])
+
+
+@TYPES
+@KEEP
+@ROWS
+def test_row_gradients_of_all_sizes(ocl, monkeypatch, math_fp32, size, dtype, keep):
+    """reduction="none": the gradients of the rows over twelve powers of ten; each row of dx errs relative to its own."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    N = size[0]
+    x, w, b, t = make(*size, dtype, bias=True)
+    grad = 10.0 ** torch.linspace(0, -12, N) * torch.where(torch.arange(N) % 3 == 0, -1.0, 1.0)
+    if dtype == FP16:
+        grad = grad * 1e4  # so that most rows are above fp16's least number
+    grad = grad[torch.randperm(N, generator=torch.Generator().manual_seed(1))].contiguous()
+    losses, err, grads, bounds = formula(x, w, b, t, grad, smooth=0.1)
+    got = run(ocl, x, w, b, t, grad=grad, reduction="none", label_smoothing=0.1)
+    within(got[0], losses, err, "losses")
+    for a, r, e, what in zip(got[1:], grads, bounds, "xwb"):
+        within(a, r, e, what)
+
+
+@TYPES
+@KEEP
+@ROWS
+def test_row_gradients_that_are_no_numbers(ocl, monkeypatch, math_fp32, size, dtype, keep):
+    """reduction="none": an infinite gradient, or NaN, reaches its own row of dx only; in a row without a loss nothing."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    N = size[0]
+    x, w, b, t = make(*size, dtype, bias=True)
+    t[4] = -100
+    grad = torch.linspace(0.5, -0.25, N)
+    fine = run(ocl, x, w, b, t, grad=grad, reduction="none")
+    grad[4] = float("nan")
+    same = run(ocl, x, w, b, t, grad=grad, reduction="none")
+    assert all(torch.equal(a, b) for a, b in zip(fine, same))
+    grad[1], grad[3] = float("inf"), float("nan")
+    got = run(ocl, x, w, b, t, grad=grad, reduction="none")
+    others = torch.ones(N, dtype=torch.bool)
+    others[1] = others[3] = False
+    assert torch.equal(got[1][others], fine[1][others])
+    assert not torch.isfinite(got[1][1]).any() and torch.isnan(got[1][3]).all()
+    assert not torch.isfinite(got[2]).any()
