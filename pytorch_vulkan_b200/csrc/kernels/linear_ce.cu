@@ -76,6 +76,12 @@ constexpr float k2p112 = 5192296858534827628530496329220096.f;
 
 enum { kEpiStats = 0, kEpiGrad = 1, kEpiAcc = 2, kEpiOut = 3 };
 
+// what a gradient's fp32 sums are multiplied by, on the device: a power of two
+// (fp16's scales), and a number for all rows or, unless NULL, one for each
+struct LceScale {
+  const float *unit, *common, *own;
+};
+
 struct LceGemm {
   int M, N, K;
   int a_row0, b_row0;     // where the operands' rows (K-major) or K rows (MN-major) begin in their maps
@@ -104,8 +110,7 @@ struct LceGemm {
   void* out;              // kEpiOut without a tensor map
   int64_t out_ld;
   int out_dtype, out_tma;
-  const float* out_scale; // kEpiOut: factor on the device
-  const float* out_row;   // kEpiOut: a factor for each row, or NULL
+  LceScale out_scale;     // kEpiOut
 };
 
 // the bias of 64 columns added to a row's logits: each lane fetches two, all
@@ -190,6 +195,16 @@ __device__ __forceinline__ float2 lce_unscale(const float* scales) {
   if (!scales) return make_float2(1.f, 1.f);
   const float a = scales[0], b = scales[1], both = a * b;
   return both >= 1e-37f && both <= 1e37f ? make_float2(both, 1.f) : make_float2(a, b);
+}
+
+// the same for a row of a gradient.  Where the product of the two is beyond
+// fp32's normal numbers, the one that keeps the sum in the middle comes first:
+// the larger where the product is too small, the smaller where it is too large.
+__device__ __forceinline__ float2 lce_row_scale(const LceScale& p, int64_t row) {
+  const float a = *p.unit, b = p.own ? p.own[row] : *p.common, both = a * b, size = fabsf(both);
+  if (size >= 1e-37f && size <= 1e37f) return make_float2(both, 1.f);
+  const bool a_first = size < 1e-37f ? a >= fabsf(b) : a <= fabsf(b);
+  return a_first ? make_float2(a, b) : make_float2(b, a);
 }
 
 // One tile: C[256 x BN] by a pair of CTAs, in two accumulators in turn.  With
@@ -380,8 +395,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
       }
       const float2 unscale = lce_unscale(P == 2 ? p.zscale : nullptr);
       const float flat = EPI == kEpiGrad ? p.smoothing / (float)p.V : 0.f;
-      const float oscale = EPI == kEpiOut && p.out_scale ? *p.out_scale : 1.f;
-      const float orow = EPI == kEpiOut && p.out_row && mrow ? p.out_row[m] : 1.f;
+      const float2 oscale = EPI == kEpiOut && mrow ? lce_row_scale(p.out_scale, m) : make_float2(0.f, 0.f);
       float mx = -INFINITY, sum = 0.f, zs = 0.f;
       float v[64];
       bool ok = true;
@@ -518,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = v[j] * oscale * orow;
+          for (int j = 0; j < 64; ++j) v[j] = v[j] * oscale.x * oscale.y;
           if (!p.out_tma) {
             // through the box, rotated by the row: lanes then write along rows
 #pragma unroll
@@ -663,7 +677,7 @@ __global__ void __launch_bounds__(1024, 2)
 // rows (mean and sum): row[i] is 1 or 0, and one factor for all results
 struct LceRowsJob {
   float* row;             // NULL: nothing to do
-  float* factor;          // of db, dx (which w's scale is in) and dw (x's)
+  float* factor;          // powers of two of db, dx (w's scale is in it) and dw (x's), and the number for all rows
   const float *grad_out, *count;
   const int64_t* target;
   int64_t N;
@@ -751,10 +765,10 @@ __global__ void __launch_bounds__(256)
     if (first == 0) {
       float f = *rj.grad_out;
       if (rj.mean) f = *rj.count > 0.f ? f / *rj.count : 0.f;
-      f *= rj.inv_gscale;
-      rj.factor[0] = f;
-      rj.factor[1] = f / sw;
-      rj.factor[2] = f / sx;
+      rj.factor[0] = rj.inv_gscale;
+      rj.factor[1] = rj.inv_gscale / sw;
+      rj.factor[2] = rj.inv_gscale / sx;
+      rj.factor[3] = f;
     }
   }
 }
@@ -1190,7 +1204,7 @@ __global__ void __launch_bounds__(1024)
 
 // the rows' factors where each has a gradient of its own: whether it has a loss
 // (one) and g_i (own; 0 without a loss) for dx, and for the sums over rows
-// g_i / max |g| (row) with that maximum in their common factors
+// g_i / max |g| (row) with that maximum as the number for all
 __global__ void __launch_bounds__(1024)
     lce_grad_rows_kernel(const float* __restrict__ grad_out, const int64_t* __restrict__ target, int64_t N, int64_t V,
                          int64_t ignore, float inv_gscale, const float* __restrict__ scales, float* __restrict__ row,
@@ -1218,20 +1232,17 @@ __global__ void __launch_bounds__(1024)
     own[i] = scored ? g : 0.f;
   }
   if (threadIdx.x == 0) {
-    const float f = mx * inv_gscale;
-    factor[0] = f;
+    factor[0] = inv_gscale;
     factor[1] = scales ? inv_gscale * scales[1] : inv_gscale;
-    factor[2] = scales ? f * scales[0] : f;
+    factor[2] = scales ? inv_gscale * scales[0] : inv_gscale;
+    factor[3] = mx;
   }
 }
 
-// out [rows][cols] = factor * sum of S slabs [rows][ld], times each row's own
-// factor where there are some; four columns a thread
+// out [rows][cols] = scale * sum of S slabs [rows][ld], four columns a thread
 template <typename T>
 __global__ void lce_join_kernel(const float* __restrict__ slab, int S, int64_t rows, int64_t cols, int64_t ld,
-                                const float* __restrict__ factor, const float* __restrict__ own, T* __restrict__ out,
-                                int vec) {
-  const float f = *factor;
+                                LceScale scale, T* __restrict__ out, int vec) {
   const int per_row = (int)(ld / 4);
   const int64_t total = rows * per_row, size = rows * ld;
   for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
@@ -1245,9 +1256,9 @@ __global__ void lce_join_kernel(const float* __restrict__ slab, int S, int64_t r
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] += u[k];
     }
-    const float g = own ? own[r] : 1.f;
+    const float2 f = lce_row_scale(scale, r);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = v[k] * f * g;
+    for (int k = 0; k < 4; ++k) v[k] = v[k] * f.x * f.y;
     if (vec) {
       store_vec<4>(out + r * cols + c, v);
     } else {
@@ -1279,7 +1290,7 @@ __global__ void __launch_bounds__(1024) lce_colsum_kernel(const T* __restrict__ 
   __syncthreads();
   if (g == 0 && col < cols) {
     for (int q = 1; q < 32; ++q) sum += s[q][c];
-    if (gridDim.y == 1) out[col] = from_f32<O>(sum * *factor);  // there is one part
+    if (gridDim.y == 1) out[col] = from_f32<O>(sum * factor[0] * factor[3]);  // there is one part
     else part[blockIdx.y * cols + col] = sum;
   }
 }
@@ -1291,7 +1302,7 @@ __global__ void lce_dbias_kernel(const float* __restrict__ part, int parts, int6
   if (c >= cols) return;
   double s = 0.0;
   for (int q = 0; q < parts; ++q) s += (double)part[q * cols + c];
-  out[c] = from_f32<T>((float)(s * (double)*factor));
+  out[c] = from_f32<T>((float)(s * (double)factor[0] * (double)factor[3]));
 }
 
 // --------------------------------------------------------------- host side
@@ -1529,7 +1540,7 @@ static size_t lce_fwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
 struct LceBwdSpace {
   uint16_t *x, *w, *G;
   float *absmax, *scales;
-  float *slab, *row, *factor, *dx, *dw, *colsum;  // factor: of db, dx and dw
+  float *slab, *row, *factor, *dx, *dw, *colsum;  // factor: see LceRowsJob
   float *one, *own;                               // where each row has its own gradient: see lce_grad_rows_kernel
 };
 
@@ -1546,7 +1557,7 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   const bool scales = p.P == 2 && lce_few_rows(d, p.ldp);
   s->absmax = a.take<float>(scales ? kLScaleBlocks : 0);
   s->scales = a.take<float>(scales ? 2 : 0);
-  s->factor = a.take<float>(3);
+  s->factor = a.take<float>(4);
   s->dx = a.take<float>(p.pieces > 1 || (d->kept > 0 && d->kept < d->V) || p.dx.splits > 1 ? p.dx.splits * d->N * ld32 : 0);
   s->dw = a.take<float>(p.dw.splits > 1 ? p.dw.splits * width * ld32 : 0);
   s->colsum = a.take<float>(p.colsum_parts * width);
@@ -1698,14 +1709,14 @@ static LceRowsJob lce_no_rows() {
   return r;
 }
 
-// out = factor * (sum of slabs), as the operands' type
-static int lce_join(const pvb2_linear_ce_desc* d, const float* slab, int S, int64_t rows, const float* factor,
-                    const float* own, void* out, cudaStream_t s) {
+// out = scale * (sum of slabs), as the operands' type
+static int lce_join(const pvb2_linear_ce_desc* d, const float* slab, int S, int64_t rows, const LceScale& scale,
+                    void* out, cudaStream_t s) {
   const int64_t ld = up(d->D, 4);
   const int grid = grid_for(rows * (ld / 4), 256), vec = d->D % 4 == 0 && ((uintptr_t)out & 15) == 0;
-  if (d->dtype == PVB2_F32) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, own, (float*)out, vec);
-  else if (d->dtype == PVB2_F16) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, own, (__half*)out, vec);
-  else lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, factor, own, (__nv_bfloat16*)out, vec);
+  if (d->dtype == PVB2_F32) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, scale, (float*)out, vec);
+  else if (d->dtype == PVB2_F16) lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, scale, (__half*)out, vec);
+  else lce_join_kernel<<<grid, 256, 0, s>>>(slab, S, rows, d->D, ld, scale, (__nv_bfloat16*)out, vec);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -1752,14 +1763,13 @@ static CUtensorMap no_map() {
 
 // the product A B (K not cut) into `out`, rows x D
 static int lce_out(const pvb2_linear_ce_desc* d, const LcePlan& p, const CUtensorMap& a, const CUtensorMap& b, LceGemm g,
-                   bool a_mn, int64_t rows, void* out, const float* factor, const float* own, int bn, cudaStream_t s) {
+                   bool a_mn, int64_t rows, void* out, const LceScale& scale, int bn, cudaStream_t s) {
   const int size = d->dtype == PVB2_F32 ? 4 : 2;
   CUtensorMap c = no_map();
   g.out = out;
   g.out_ld = d->D;
   g.out_dtype = d->dtype;
-  g.out_scale = factor;
-  g.out_row = own;
+  g.out_scale = scale;
   g.out_tma = ((uintptr_t)out & 15) == 0 && d->D * size % 16 == 0;
   if (g.out_tma) {
     if (size == 4) PVB2_TRY(lce_map32(&c, out, d->D, rows, d->D, 1));
@@ -2020,6 +2030,8 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
     rows = LceRowsJob{sp.row, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
   const bool own = d->reduction == PVB2_LOSS_NONE;  // each row has its own gradient
   bool row_factors = !own;                          // or still to be formed, after the scales
+  const LceScale dx_scale{sp.factor + 1, sp.factor + 3, own ? sp.own : nullptr};
+  const LceScale dw_scale{sp.factor + 2, sp.factor + 3, nullptr};
   LceOperand px{x, 0, d->N, d->ldx, sp.x, target};
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;
   PVB2_TRY(lce_map_a(&x_k, sp.x, d->D, d->N, p.ldp, p));
@@ -2089,7 +2101,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
         PVB2_TRY(lce_map32(&acc, sp.dx, d->D, d->N, ld32, p.dx.splits));
         PVB2_TRY(lce_gemm<kEpiAcc>(g_k, w_mn, acc, h, false, true, p, p.dx.bn, s));
       } else {
-        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, sp.factor + 1, own ? sp.own : nullptr, p.dx.bn, s));
+        PVB2_TRY(lce_out(d, p, g_k, w_mn, h, false, d->N, dx, dx_scale, p.dx.bn, s));
       }
       if (own && (dw || dbias)) PVB2_TRY(form(sp.row));
     }
@@ -2099,9 +2111,9 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       if (p.dw.splits > 1) {
         PVB2_TRY(lce_map32(&acc, sp.dw, d->D, width, ld32, p.dw.splits));
         PVB2_TRY(lce_gemm<kEpiAcc>(g_mn, x_mn, acc, h, true, true, p, p.dw.bn, s));
-        PVB2_TRY(lce_join(d, sp.dw, p.dw.splits, width, sp.factor + 2, nullptr, out, s));
+        PVB2_TRY(lce_join(d, sp.dw, p.dw.splits, width, dw_scale, out, s));
       } else {
-        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, sp.factor + 2, nullptr, p.dw.bn, s));
+        PVB2_TRY(lce_out(d, p, g_mn, x_mn, h, true, width, out, dw_scale, p.dw.bn, s));
       }
     }
     if (dbias) {
@@ -2109,7 +2121,7 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
       PVB2_TRY(lce_bias_grad(d, p, sp, width, ldg, out, s));
     }
   }
-  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, sp.factor + 1, own ? sp.own : nullptr, dx, s));
+  if (dx && dx_slabs) PVB2_TRY(lce_join(d, sp.dx, p.dx.splits, d->N, dx_scale, dx, s));
   return PVB2_OK;
 }
 

@@ -149,3 +149,25 @@ def test_row_gradients_that_are_no_numbers(ocl, monkeypatch, math_fp32, size, dt
     assert torch.equal(got[1][others], fine[1][others])
     assert not torch.isfinite(got[1][1]).any() and torch.isnan(got[1][3]).all()
     assert not torch.isfinite(got[2]).any()
+
+
+@KEEP
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("size", [(150, 72, 520), (20, 1000, 90), (5, 40, 600), (2100, 24, 12000)],
+                         ids=["tiles", "slabs", "few", "pieces"])
+def test_operands_scaled_by_powers_of_two(ocl, monkeypatch, math_fp32, size, reduction, keep):
+    """x 2^k and w 2^-k have the logits of x and w, and gradients that are theirs times 2^-k and 2^k, bit for bit where
+    they are no denormal numbers (an error of one rounding to such a number, 2^-150, where they are)."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    x, w, b, t = make(*size, FP32, bias=True)
+    grad = torch.linspace(0.01, 0.02, size[0]) if reduction == "none" else torch.tensor(0.01)
+    loss, dx, dw, db = run(ocl, x, w, b, t, grad=grad, reduction=reduction)
+    for k in (96, -96):
+        loss2, dx2, dw2, db2 = run(ocl, x * 2.0 ** k, w * 2.0 ** -k, b, t, grad=grad, reduction=reduction)
+        assert torch.equal(loss, loss2) and torch.equal(db, db2)
+        for a, a2, by in ((dx, dx2, -k), (dw, dw2, k)):
+            want = a.double() * 2.0 ** by
+            normal = want.abs() >= 2.0 ** -126
+            assert normal.double().mean() > 0.99
+            assert torch.equal(a2.double()[normal], want[normal])
+            assert ((a2.double() - want).abs()[~normal] <= 2.0 ** -149).all()
