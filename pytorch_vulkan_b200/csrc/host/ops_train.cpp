@@ -579,8 +579,10 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
 static at::Tensor linear_cross_entropy_autograd(const at::Tensor& input, const at::Tensor& weight,
                                                 const at::Tensor& target, const std::optional<at::Tensor>& bias,
                                                 int64_t ignore_index, int64_t reduction, double label_smoothing) {
-  const bool grads = at::GradMode::is_enabled() && (input.requires_grad() || weight.requires_grad() ||
-                                                    (bias.has_value() && bias->defined() && bias->requires_grad()));
+  auto any = [&](auto f) { return f(input) || f(weight) || (bias.has_value() && bias->defined() && f(*bias)); };
+  // a tangent (forward mode, for which requires_grad says nothing) goes to the function too, which refuses it
+  const bool grads = (at::GradMode::is_enabled() && any([](const at::Tensor& t) { return t.requires_grad(); })) ||
+                     any([](const at::Tensor& t) { return t._fw_grad(0).defined(); });
   if (!grads) {
     at::AutoDispatchBelowADInplaceOrView below;
     return linear_cross_entropy(input, weight, target, bias, ignore_index, reduction, label_smoothing);

@@ -171,3 +171,25 @@ def test_operands_scaled_by_powers_of_two(ocl, monkeypatch, math_fp32, size, red
             assert normal.double().mean() > 0.99
             assert torch.equal(a2.double()[normal], want[normal])
             assert ((a2.double() - want).abs()[~normal] <= 2.0 ** -149).all()
+
+
+def test_forward_mode_is_refused(ocl):
+    """A tangent is not lost without a word."""
+    import torch.autograd.forward_ad as fw
+
+    x, w, b, t = make(12, 16, 40, FP32, bias=True)
+    given = [v.to(DEV) for v in (x, w, b)]
+    with fw.dual_level():
+        for k in range(3):
+            for requires in (False, True):
+                args = [v.detach().requires_grad_(requires) for v in given]
+                args[k] = fw.make_dual(args[k], torch.ones_like(given[k]))
+                with pytest.raises(RuntimeError, match="jvp"):
+                    ocl.functional.linear_cross_entropy(args[0], args[1], t.to(DEV), args[2])
+                with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                    ocl.functional.linear_cross_entropy(args[0], args[1], t.to(DEV), args[2])
+        table = fw.make_dual(torch.zeros(8, 2).to(DEV), torch.ones(8, 2).to(DEV))
+        with pytest.raises(RuntimeError, match="jvp"):
+            ocl.functional.relative_position_bias(table, 5, 5)
+    want = ocl.functional.linear_cross_entropy(given[0], given[1], t.to(DEV), given[2])  # outside, as ever
+    assert torch.isfinite(want.cpu())
