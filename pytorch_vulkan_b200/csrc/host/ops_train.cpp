@@ -171,11 +171,17 @@ static bool adam_state(const pybind11::dict& state, PyObject* p, AdamState* s) {
   return s->dict && PyDict_Size(s->dict) > 0;
 }
 
-static void* adam_held(const at::Tensor& x, const at::Tensor& p, c10::ScalarType want, int64_t numel, bool flat,
+// How a tensor of the state lies in memory: as its parameter; as its parameter,
+// or in a row if the parameter does (codes; their order is the parameter's
+// memory order, which a row says only of a contiguous one); in a row.
+enum class Held { kAsParam, kCodes, kRow };
+
+static void* adam_held(const at::Tensor& x, const at::Tensor& p, c10::ScalarType want, int64_t numel, Held how,
                        const char* what) {
-  TORCH_CHECK(is_ocl(x) && x.device() == p.device() && x.scalar_type() == want && x.numel() == numel &&
-                  (flat ? x.is_contiguous() : same_layout(x, p)),
-              "ocl AdamW: ", what, " of the state does not fit its parameter");
+  const bool row = x.dim() == 1 && x.is_contiguous();
+  const bool fits = how == Held::kRow ? row : same_layout(x, p) || (how == Held::kCodes && row && p.is_contiguous());
+  TORCH_CHECK(is_ocl(x) && x.device() == p.device() && x.scalar_type() == want && x.numel() == numel && fits,
+              "ocl AdamW: ", what, " of the state does not fit its parameter (shape, type, device or memory order)");
   return x.data_ptr();
 }
 
@@ -183,10 +189,11 @@ static void* adam_held(const at::Tensor& x, const at::Tensor& p, c10::ScalarType
 static void adam_codes(const AdamState& s, const at::Tensor& p, pvb2_adamw_tensor& t) {
   const StateKeys& keys = state_keys();
   const int64_t n = p.numel(), blocks = (n + 255) / 256;
-  t.exp_avg = adam_held(s.get(keys.exp_avg_code), p, at::kByte, n, true, "exp_avg_code");
-  t.exp_avg_sq = adam_held(s.get(keys.exp_avg_rms_code), p, at::kByte, n, true, "exp_avg_rms_code");
-  t.exp_avg_scale = (float*)adam_held(s.get(keys.exp_avg_scale), p, at::kFloat, blocks, true, "exp_avg_scale");
-  t.exp_avg_sq_scale = (float*)adam_held(s.get(keys.exp_avg_rms_scale), p, at::kFloat, blocks, true, "exp_avg_rms_scale");
+  t.exp_avg = adam_held(s.get(keys.exp_avg_code), p, at::kByte, n, Held::kCodes, "exp_avg_code");
+  t.exp_avg_sq = adam_held(s.get(keys.exp_avg_rms_code), p, at::kByte, n, Held::kCodes, "exp_avg_rms_code");
+  t.exp_avg_scale = (float*)adam_held(s.get(keys.exp_avg_scale), p, at::kFloat, blocks, Held::kRow, "exp_avg_scale");
+  t.exp_avg_sq_scale =
+      (float*)adam_held(s.get(keys.exp_avg_rms_scale), p, at::kFloat, blocks, Held::kRow, "exp_avg_rms_scale");
 }
 
 // One step of pytorch_vulkan_b200.optim.AdamW over the parameters of a group
@@ -247,8 +254,8 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
       if (codes) {
         adam_codes(it.state, p, t);
       } else {
-        t.exp_avg = adam_held(it.state.get(state_keys().exp_avg), p, at::kFloat, t.numel, false, "exp_avg");
-        t.exp_avg_sq = adam_held(it.state.get(state_keys().exp_avg_sq), p, at::kFloat, t.numel, false, "exp_avg_sq");
+        t.exp_avg = adam_held(it.state.get(state_keys().exp_avg), p, at::kFloat, t.numel, Held::kAsParam, "exp_avg");
+        t.exp_avg_sq = adam_held(it.state.get(state_keys().exp_avg_sq), p, at::kFloat, t.numel, Held::kAsParam, "exp_avg_sq");
       }
       t.step = step_ptr(it.state.get(state_keys().step), dev, i);
       ts.push_back(t);
@@ -300,8 +307,8 @@ static void adamw8_values(const pybind11::list& params, const pybind11::dict& st
       memset(&t, 0, sizeof(t));
       t.numel = ps[i].numel();
       adam_codes(states[i], ps[i], t);
-      t.param = adam_held(exp_avgs[i], ps[i], at::kFloat, t.numel, false, "the tensor for a first moment");
-      t.grad = adam_held(exp_avg_sqs[i], ps[i], at::kFloat, t.numel, false, "the tensor for a second moment");
+      t.param = adam_held(exp_avgs[i], ps[i], at::kFloat, t.numel, Held::kAsParam, "the tensor for a first moment");
+      t.grad = adam_held(exp_avg_sqs[i], ps[i], at::kFloat, t.numel, Held::kAsParam, "the tensor for a second moment");
       ts.push_back(t);
     }
     OCL_CHECK(pvb2_adamw8_values((int)ts.size(), ts.data(), stream_for(dev)));

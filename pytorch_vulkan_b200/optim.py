@@ -73,9 +73,12 @@ class AdamW(torch.optim.Optimizer):
             return state
         n = p.numel()
         for key in _KEYS[8]:
-            code = key.endswith("code")
-            state[key] = torch.zeros(n if code else -(-n // _BLOCK), dtype=torch.uint8 if code else torch.float32,
-                                     device=p.device)
+            if not key.endswith("code"):
+                state[key] = torch.zeros(-(-n // _BLOCK), dtype=torch.float32, device=p.device)
+            elif p.is_contiguous():
+                state[key] = torch.zeros(n, dtype=torch.uint8, device=p.device)
+            else:  # codes follow the parameter's memory order, which their strides keep
+                state[key] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
         return state
 
     def step(self, closure=None):

@@ -449,3 +449,64 @@ def test_on_another_stream(ocl):
     zero = torch.zeros_like(p0)
     s = opt.state[p]
     check_step(p0, g0 * 2, zero, zero, 1, p, s["exp_avg"], s["exp_avg_sq"], torch.float32)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_in_another_memory_order_is_refused(ocl, bits):
+    """Moments lie in memory as their parameter did: after a change of its memory order they belong to other elements."""
+    gen = torch.Generator().manual_seed(11)
+    p0, g0 = rand((6, 5, 4, 3), gen), rand((6, 5, 4, 3), gen)
+    formats = (torch.contiguous_format, torch.channels_last)
+    for first, then in (formats, formats[::-1]):
+        p = p0.to(DEV).contiguous(memory_format=first).requires_grad_()
+        opt = ocl.optim.AdamW([p], **HYPER, state_bits=bits)
+        p.grad = g0.to(DEV).contiguous(memory_format=first)
+        opt.step()
+        held = p.detach().cpu().clone()
+        saved = opt.state_dict()
+        # a program that goes on in the old order, from a checkpoint too
+        q = held.to(DEV).contiguous(memory_format=first).requires_grad_()
+        twin = ocl.optim.AdamW([q], **HYPER, state_bits=bits)
+        twin.load_state_dict(saved)
+        q.grad = g0.to(DEV)
+        twin.step()
+        # and one that changes it, as module.to(memory_format=...) does
+        p.data = p.data.contiguous(memory_format=then)
+        with pytest.raises(RuntimeError, match="does not fit"):
+            opt.step()
+        out = [torch.empty_like(p, memory_format=torch.preserve_format) for _ in range(2)]
+        if bits == 8:
+            with pytest.raises(RuntimeError, match="does not fit"):
+                opt.write_state_values([out[0].detach()], [out[1].detach()])
+        assert torch.equal(p.detach().cpu(), held)
+        r = held.to(DEV).contiguous(memory_format=then).requires_grad_()
+        other = ocl.optim.AdamW([r], **HYPER, state_bits=bits)
+        r.grad = g0.to(DEV)
+        with pytest.raises((RuntimeError, ValueError), match="fit"):
+            other.load_state_dict(saved)
+            other.step()
+        # back in its order the state goes on as if nothing had been
+        p.data = p.data.contiguous(memory_format=first)
+        opt.step()
+        assert torch.equal(p.detach().cpu(), q.detach().cpu())
+
+
+def test_8_bit_moments_in_any_dense_order(ocl):
+    """A channels-last parameter takes the steps that the same numbers take in a row."""
+    gen = torch.Generator().manual_seed(12)
+    p0 = rand((9, 8, 7, 5), gen)
+    p = p0.to(DEV).contiguous(memory_format=torch.channels_last).requires_grad_()
+    flat = p0.permute(0, 2, 3, 1).contiguous().view(-1).to(DEV).requires_grad_()
+    one, two = (ocl.optim.AdamW([v], **HYPER, state_bits=8) for v in (p, flat))
+    for _ in range(3):
+        g = rand((9, 8, 7, 5), gen, 0.1)
+        p.grad, flat.grad = g.to(DEV), g.permute(0, 2, 3, 1).contiguous().view(-1).to(DEV)
+        one.step()
+        two.step()
+    assert torch.equal(p.detach().cpu().permute(0, 2, 3, 1).reshape(-1), flat.detach().cpu())
+    m, v = (torch.empty_like(p, memory_format=torch.preserve_format).detach() for _ in range(2))
+    mf, vf = (torch.empty_like(flat).detach() for _ in range(2))
+    one.write_state_values([m], [v])
+    two.write_state_values([mf], [vf])
+    for a, b in ((m, mf), (v, vf)):
+        assert torch.equal(a.cpu().permute(0, 2, 3, 1).reshape(-1), b.cpu())
