@@ -58,11 +58,16 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
         params = self.param_groups[-1]["params"]
-        if len({id(p) for p in params}) != len(params):
-            raise ValueError("a parameter is listed twice")
-        for p in params:
-            if p.device.type != "ocl" or p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-                raise ValueError(f"fp32, bf16 or fp16 parameters on the ocl device expected, got {p.dtype} on {p.device}")
+        try:
+            if len({id(p) for p in params}) != len(params):
+                raise ValueError("a parameter is listed twice")
+            for p in params:
+                if p.device.type != "ocl" or p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                    raise ValueError(
+                        f"fp32, bf16 or fp16 parameters on the ocl device expected, got {p.dtype} on {p.device}")
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     def _init_state(self, p):
         state = self.state[p]

@@ -510,3 +510,19 @@ def test_8_bit_moments_in_any_dense_order(ocl):
     two.write_state_values([mf], [vf])
     for a, b in ((m, mf), (v, vf)):
         assert torch.equal(a.cpu().permute(0, 2, 3, 1).reshape(-1), b.cpu())
+
+
+def test_a_refused_group_is_not_added(ocl):
+    p, q = torch.ones(8).to(DEV).requires_grad_(), torch.ones(8).to(DEV).requires_grad_()
+    opt = ocl.optim.AdamW([p], **HYPER)
+    for bad, match in ((dict(params=[q, q]), "twice"), (dict(params=[q, torch.ones(3, requires_grad=True)]), "ocl device expected"),
+                       (dict(params=[torch.ones(3, dtype=torch.float64, device="cpu", requires_grad=True)]), "expected")):
+        with pytest.raises(ValueError, match=match):
+            opt.add_param_group(bad)
+        assert len(opt.param_groups) == 1 and opt.param_groups[0]["params"] == [p]
+    q.grad = p.grad = torch.ones(8).to(DEV)
+    opt.step()
+    assert (q.detach().cpu() == 1).all() and (p.detach().cpu() != 1).all()
+    opt.add_param_group({"params": [q]})
+    opt.step()
+    assert (q.detach().cpu() != 1).all()
