@@ -122,15 +122,38 @@ class AdamW(torch.optim.Optimizer):
             a.copy_(s["exp_avg"])
             b.copy_(s["exp_avg_sq"])
 
+    def _fits(self, p, state):
+        n, blocks = p.numel(), -(-p.numel() // _BLOCK)
+        numels = {"step": 1, "exp_avg": n, "exp_avg_sq": n, "exp_avg_code": n, "exp_avg_rms_code": n,
+                  "exp_avg_scale": blocks, "exp_avg_rms_scale": blocks}
+        return set(state) == {"step", *_KEYS[self.state_bits]} and all(
+            isinstance(v, torch.Tensor) and v.numel() == numels[k] for k, v in state.items())
+
     def load_state_dict(self, state_dict):
-        """As torch's, but the state keeps its own types (torch casts floating state to the parameters')."""
-        super().load_state_dict(state_dict)
-        old = [i for group in state_dict["param_groups"] for i in group["params"]]
-        new = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(old, new):
-            saved = state_dict["state"].get(i)
-            if not saved:
-                continue
-            if set(saved) != {"step", *_KEYS[self.state_bits]}:
-                raise ValueError(f"the state of parameter {i} is not one of {self.state_bits} bits")
-            self.state[p] = {k: v.detach().to(device=p.device, copy=True) for k, v in saved.items()}
+        """As torch's, but the state keeps its own types (torch casts floating state to the parameters'), and one that
+        does not fit is refused before anything is replaced."""
+        loaded = {}
+
+        def take(_, state_dict):  # after the program's own hooks; torch sees the groups and what belongs to no parameter
+            old = [i for group in state_dict["param_groups"] for i in group["params"]]
+            new = [p for group in self.param_groups for p in group["params"]]
+            for i, p in zip(old, new):
+                saved = state_dict["state"].get(i)
+                if not saved:
+                    continue
+                if not self._fits(p, saved):
+                    raise ValueError(f"the state of parameter {i} is not one of {self.state_bits} bits that fits it")
+                loaded[p] = {k: v.detach().to(device=p.device, copy=True) for k, v in saved.items()}
+            ids = set(old)
+            return {**state_dict, "state": {k: v for k, v in state_dict["state"].items() if k not in ids}}
+
+        def put(_):  # before the program's own
+            self.state.update(loaded)
+
+        hooks = (self.register_load_state_dict_pre_hook(take),
+                 self.register_load_state_dict_post_hook(put, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()

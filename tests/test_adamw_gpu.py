@@ -526,3 +526,52 @@ def test_a_refused_group_is_not_added(ocl):
     opt.add_param_group({"params": [q]})
     opt.step()
     assert (q.detach().cpu() != 1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_is_refused_changes_nothing(ocl, bits):
+    gen = torch.Generator().manual_seed(13)
+    ps = [rand(s, gen, 1.0, torch.bfloat16) for s in ((300,), (20, 30))]
+
+    def make(lr, state_bits):
+        dev = [p.to(DEV).requires_grad_() for p in ps]
+        opt = ocl.optim.AdamW(dev, lr=lr, state_bits=state_bits)
+        for d in dev:
+            d.grad = torch.ones_like(d)
+        opt.step()
+        return opt
+
+    opt, good = make(0.125, bits), make(0.25, bits).state_dict()
+    cut = {"state": {k: dict(v) for k, v in good["state"].items()}, "param_groups": good["param_groups"]}
+    key = "exp_avg_sq" if bits == 32 else "exp_avg_rms_scale"
+    cut["state"][1][key] = cut["state"][1][key].reshape(-1)[:1]
+    number = {"state": {k: dict(v) for k, v in good["state"].items()}, "param_groups": good["param_groups"]}
+    number["state"][0]["step"] = 3
+    before = {p: {k: v.cpu().clone() for k, v in s.items()} for p, s in opt.state.items()}
+    for bad in (make(0.25, 40 - bits).state_dict(), cut, number):
+        with pytest.raises(ValueError, match="state of parameter"):
+            opt.load_state_dict(bad)
+        assert opt.param_groups[0]["lr"] == 0.125 and set(opt.state) == set(before)
+        for p, s in before.items():
+            assert set(opt.state[p]) == set(s)
+            for k, v in s.items():
+                assert torch.equal(opt.state[p][k].cpu(), v) and opt.state[p][k].dtype == v.dtype
+    seen = []
+    opt.register_load_state_dict_post_hook(lambda o: seen.append({k: v.dtype for k, v in o.state[o.param_groups[0]["params"][0]].items()}))
+    opt.load_state_dict(good)
+    assert opt.param_groups[0]["lr"] == 0.25
+    assert seen == [{k: v.dtype for k, v in good["state"][0].items()}]  # whole when a hook sees it
+
+
+def test_loading_takes_no_more_memory_than_the_state(ocl):
+    p = torch.zeros(1 << 22, dtype=torch.float32).to(DEV).requires_grad_()
+    opt = ocl.optim.AdamW([p], state_bits=8)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    saved = opt.state_dict()
+    torch.ocl.synchronize()
+    torch.ocl.reset_peak_memory_stats()
+    before = torch.ocl.memory_allocated()
+    opt.load_state_dict(saved)
+    # two tensors of 4 MB and two of 64 KB; their fp32 form would take 16 MB each
+    assert torch.ocl.max_memory_allocated() - before <= 10 << 20
