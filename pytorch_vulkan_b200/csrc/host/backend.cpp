@@ -893,6 +893,13 @@ static uintptr_t graph_capture_begin(int d) {
   return reinterpret_cast<uintptr_t>(h.release());
 }
 
+static bool graph_capturing(int d) {
+  check_index(d);
+  Pool& pool = pools()[d];
+  std::lock_guard<std::mutex> g(pool.m);
+  return pool.capturing != nullptr;
+}
+
 static void graph_capture_end(uintptr_t handle) {
   HostGraph* h = reinterpret_cast<HostGraph*>(handle);
   TORCH_CHECK(h && !h->graph, "ocl graphs: no capture in progress for this handle");
@@ -994,6 +1001,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("impl_event_elapsed_ms", &event_elapsed);
   m.def("impl_event_destroy", &event_destroy);
   m.def("impl_graph_capture_begin", &graph_capture_begin, "begin capturing device d's current stream");
+  m.def("impl_graph_capturing", &graph_capturing, "whether work of device d is being captured");
   m.def("impl_graph_capture_end", &graph_capture_end, "end the capture and instantiate the graph");
   m.def("impl_graph_replay", &graph_replay, "replay a captured graph on its device's current stream");
   m.def("impl_graph_kernels", &graph_kernels, "kernels launched by one replay");

@@ -34,7 +34,8 @@ class AdamW(torch.optim.Optimizer):
 
     The step count of each parameter lives on the device, so that a step
     captured in a ``torch.ocl.Graph`` advances it on every replay (the learning
-    rate and the other numbers are those of the capture).
+    rate and the other numbers are those of the capture).  A parameter's first
+    step makes its state and cannot be captured.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False,
@@ -98,6 +99,9 @@ class AdamW(torch.optim.Optimizer):
                     group["weight_decay"], group["maximize"])
             missing = _C.impl_adamw_step(*args)
             if missing:
+                if any(_C.impl_graph_capturing(p.device.index) for p in missing):
+                    # every replay would begin by zeroing the moments and the step count
+                    raise RuntimeError("ocl AdamW: a parameter has no state yet; it needs one step before it is captured")
                 for p in missing:
                     self._init_state(p)
                 _C.impl_adamw_step(*args)

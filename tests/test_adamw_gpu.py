@@ -575,3 +575,32 @@ def test_loading_takes_no_more_memory_than_the_state(ocl):
     opt.load_state_dict(saved)
     # two tensors of 4 MB and two of 64 KB; their fp32 form would take 16 MB each
     assert torch.ocl.max_memory_allocated() - before <= 10 << 20
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_first_step_is_not_captured(ocl, bits):
+    """What a graph would replay of it is the zeroed state, again and again."""
+    p, q = (torch.ones(300).to(DEV).requires_grad_() for _ in range(2))
+    opt = ocl.optim.AdamW([p, q], **HYPER, state_bits=bits)
+    p.grad = torch.ones(300).to(DEV)
+    q.grad = None
+
+    def captured():
+        graph = torch.ocl.Graph()
+        with graph.capture():
+            opt.step()
+        return graph
+
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        captured()
+    assert not any(opt.state.values())
+    opt.step()
+    q.grad = torch.ones(300).to(DEV)  # a parameter that takes part for the first time
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        captured()
+    opt.step()
+    graph = captured()
+    graph.replay()
+    graph.replay()
+    assert opt.state[p]["step"].item() == 4 and opt.state[q]["step"].item() == 3
+    graph.reset()
