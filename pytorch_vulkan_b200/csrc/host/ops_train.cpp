@@ -150,8 +150,11 @@ struct StateKey {
 };
 
 struct AdamState {  // of one parameter
-  PyObject* dict;
-  const at::Tensor& get(const StateKey& k) const { return py_tensor(PyDict_GetItemWithError(dict, k.key), k.name); }
+  pybind11::object dict;  // held: another parameter's lookup may drop it
+  // (a key's hash and comparison are a string's: no Python code runs here)
+  const at::Tensor& get(const StateKey& k) const {
+    return py_tensor(PyDict_GetItemWithError(dict.ptr(), k.key), k.name);
+  }
 };
 
 struct StateKeys {
@@ -163,12 +166,15 @@ static const StateKeys& state_keys() {
   return *keys;
 }
 
-// undefined state: an empty or a missing dict
+// undefined state: an empty or a missing dict.  A tensor's hash is Python code,
+// in which anything may happen to the program's lists, gradients and states,
+// from another thread too: whatever was read before is held.
 static bool adam_state(const pybind11::dict& state, PyObject* p, AdamState* s) {
-  s->dict = PyDict_GetItemWithError(state.ptr(), p);
-  if (!s->dict && PyErr_Occurred()) throw pybind11::error_already_set();
-  if (s->dict) TORCH_CHECK(PyDict_Check(s->dict), "ocl AdamW: a parameter's state is not a dict");
-  return s->dict && PyDict_Size(s->dict) > 0;
+  PyObject* found = PyDict_GetItemWithError(state.ptr(), p);
+  if (!found && PyErr_Occurred()) throw pybind11::error_already_set();
+  s->dict = pybind11::reinterpret_borrow<pybind11::object>(found);
+  if (found) TORCH_CHECK(PyDict_Check(found), "ocl AdamW: a parameter's state is not a dict");
+  return found && PyDict_Size(found) > 0;
 }
 
 // How a tensor of the state lies in memory: as its parameter; as its parameter,
@@ -199,28 +205,27 @@ static void adam_codes(const AdamState& s, const at::Tensor& p, pvb2_adamw_tenso
 // One step of pytorch_vulkan_b200.optim.AdamW over the parameters of a group
 // that have a gradient: counts the steps, then updates, one call for each
 // device and type among them.  Parameters that have no state yet are returned
-// and nothing is done.
+// and nothing is done.  Python code runs while the states are looked up, and
+// not from there to the launches.
 static pybind11::list adamw_step(const pybind11::list& params, const pybind11::dict& state, int64_t bits, double lr,
                                  double beta1, double beta2, double eps, double weight_decay, bool maximize) {
   const bool codes = bits == 8;
   pybind11::list missing;
-  // the list and the parameters hold what these point to (211 of them: 55 us a
-  // call, 65 where each reference was counted up and down)
   struct Item {
-    const at::Tensor *p, *g;
+    const at::Tensor* p;  // of an object in `held`
+    at::Tensor g;
     AdamState state;
     bool done;
   };
+  const pybind11::tuple held(params);
   std::vector<Item> items;
-  items.reserve(params.size());
-  for (const pybind11::handle h : params) {
+  items.reserve(held.size());
+  for (const pybind11::handle h : held) {
     const at::Tensor& p = py_tensor(h.ptr(), "a parameter");
-    const at::Tensor& g = p.grad();
-    if (!g.defined()) continue;
-    TORCH_CHECK(!g.is_sparse(), "ocl AdamW: sparse gradients are not supported");
-    AdamState s;
-    if (!adam_state(state, h.ptr(), &s)) missing.append(h);
-    items.push_back({&p, &g, s, false});
+    if (!p.grad().defined()) continue;
+    TORCH_CHECK(!p.grad().is_sparse(), "ocl AdamW: sparse gradients are not supported");
+    items.push_back({&p, p.grad(), {}, false});
+    if (!adam_state(state, h.ptr(), &items.back().state)) missing.append(h);
   }
   if (missing.size() || items.empty()) return missing;
   std::vector<pvb2_adamw_tensor> ts;
@@ -240,8 +245,8 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
       const at::Tensor& p = *it.p;
       if (it.done || p.device() != lead.device() || p.scalar_type() != type) continue;
       it.done = true;
-      check_param(p, *it.g, dev, type, i);
-      const at::Tensor* g = it.g;
+      check_param(p, it.g, dev, type, i);
+      const at::Tensor* g = &it.g;
       if (!same_layout(*g, p)) {
         copies.push_back(grad_like(*g, p));
         g = &copies.back();
@@ -285,11 +290,12 @@ static void adamw8_values(const pybind11::list& params, const pybind11::dict& st
                           const std::vector<at::Tensor>& exp_avgs, const std::vector<at::Tensor>& exp_avg_sqs) {
   std::vector<at::Tensor> ps;
   std::vector<AdamState> states;
-  for (const pybind11::handle h : params) {
+  const pybind11::tuple held(params);
+  for (const pybind11::handle h : held) {
     AdamState s;
     if (!adam_state(state, h.ptr(), &s)) continue;
     ps.push_back(py_tensor(h.ptr(), "a parameter"));
-    states.push_back(s);
+    states.push_back(std::move(s));
   }
   TORCH_CHECK_VALUE(exp_avgs.size() == ps.size() && exp_avg_sqs.size() == ps.size(), ps.size(),
                     " parameters have a state, got ", exp_avgs.size(), " and ", exp_avg_sqs.size(), " tensors");

@@ -104,7 +104,8 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("ocl AdamW: a parameter has no state yet; it needs one step before it is captured")
                 for p in missing:
                     self._init_state(p)
-                _C.impl_adamw_step(*args)
+                if _C.impl_adamw_step(*args):
+                    raise RuntimeError("ocl AdamW: the state of a parameter went away during the step")
         return loss
 
     @torch.no_grad()

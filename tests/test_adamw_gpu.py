@@ -604,3 +604,58 @@ def test_a_first_step_is_not_captured(ocl, bits):
     graph.replay()
     assert opt.state[p]["step"].item() == 4 and opt.state[q]["step"].item() == 3
     graph.reset()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_lookups_that_run_python(ocl, bits):
+    """A parameter's hash is Python code, in which gradients and states of others may go away: what the step found before
+    stays alive until it is done."""
+    import gc
+
+    at_last = []
+
+    class Leaf(torch.nn.Parameter):
+        def __hash__(self):
+            if at_last and self is params[3]:
+                at_last.pop()()
+            return super().__hash__()
+
+    params = []
+    params.extend(Leaf(torch.ones(70000 + i).to(DEV)) for i in range(4))
+    opt = ocl.optim.AdamW(params, **HYPER, state_bits=bits)
+    for p in params:
+        p.grad = torch.full_like(p, 2.0)
+    opt.step()
+    outs = [[torch.zeros(p.shape).to(DEV) for p in params] for _ in range(2)]
+
+    def drop():
+        for p in params[:3]:
+            p.grad = None
+            del opt.state[p]
+        gc.collect()
+        # whatever was freed is written over
+        junk = [torch.full((70000 + i,), float("nan")).to(DEV) for i in range(4) for _ in range(6)]
+        del junk
+
+    if bits == 8:
+        kept = dict(opt.state)
+        at_last.append(drop)
+        opt.write_state_values(*outs)
+        for m, v in zip(*outs):  # (1 - B1) 2 and (1 - B2) 4 to half a step of their codes, twice that for a square
+            assert ((m.cpu() / (2 * (1 - B1)) - 1).abs() <= 2.0 ** -4).all()
+            assert ((v.cpu() / (4 * (1 - B2)) - 1).abs() <= 2.0 ** -3).all()
+        opt.state.update(kept)
+        del kept
+        for p in params:
+            p.grad = torch.full_like(p, 2.0)
+    before = [p.detach().cpu().clone() for p in params]
+    at_last.append(drop)
+    opt.step()
+    for p, b in zip(params, before):
+        after = p.detach().cpu()
+        assert torch.isfinite(after).all() and (after < b).all()
+    assert list(opt.state) == params[3:]
+    p = params[0]
+    p.grad = torch.full_like(p, 2.0)  # its next step is a first one
+    opt.step()
+    assert opt.state[p]["step"].item() == 1
