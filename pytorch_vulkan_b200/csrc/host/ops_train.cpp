@@ -228,8 +228,14 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
     if (!adam_state(state, h.ptr(), &items.back().state)) missing.append(h);
   }
   if (missing.size() || items.empty()) return missing;
-  std::vector<pvb2_adamw_tensor> ts;
-  ts.reserve(items.size());
+  // everything is checked before anything is launched
+  struct Call {
+    int dev;
+    c10::ScalarType type;
+    std::vector<pvb2_adamw_tensor> ts;
+  };
+  std::vector<Call> calls;
+  std::vector<at::Tensor> copies;  // gradients laid out unlike their parameters
   for (size_t first = 0; first < items.size(); ++first) {
     if (items[first].done) continue;
     const at::Tensor& lead = *items[first].p;
@@ -237,9 +243,9 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
     const int dev = lead.device().index();
     const c10::ScalarType type = lead.scalar_type();
     DeviceScope scope(dev);
-    OCL_OP("adamw_step", dev);
-    ts.clear();
-    std::vector<at::Tensor> copies;  // gradients laid out unlike their parameters
+    calls.push_back({dev, type, {}});
+    std::vector<pvb2_adamw_tensor>& ts = calls.back().ts;
+    ts.reserve(items.size() - first);
     for (size_t i = first; i < items.size(); ++i) {
       Item& it = items[i];
       const at::Tensor& p = *it.p;
@@ -265,9 +271,14 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
       t.step = step_ptr(it.state.get(state_keys().step), dev, i);
       ts.push_back(t);
     }
+  }
+  for (const Call& call : calls) {
+    DeviceScope scope(call.dev);
+    OCL_OP("adamw_step", call.dev);
+    const int n = (int)call.ts.size();
     pvb2_adamw_desc d;
     memset(&d, 0, sizeof(d));
-    d.param_dtype = dtype_code(type);
+    d.param_dtype = dtype_code(call.type);
     d.state_dtype = codes ? PVB2_U8 : PVB2_F32;
     d.decoupled = 1;
     d.maximize = maximize ? 1 : 0;
@@ -277,8 +288,8 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
     d.beta2 = beta2;
     d.eps = eps;
     d.weight_decay = weight_decay;
-    Workspace ws(pvb2_adamw_workspace_size((int)ts.size()), dev);
-    OCL_CHECK(pvb2_adamw_multi(&d, (int)ts.size(), ts.data(), ws.get(), ws.bytes, stream_for(dev)));
+    Workspace ws(pvb2_adamw_workspace_size(n), call.dev);
+    OCL_CHECK(pvb2_adamw_multi(&d, n, call.ts.data(), ws.get(), ws.bytes, stream_for(call.dev)));
   }
   for (const Item& it : items) it.p->unsafeGetTensorImpl()->bump_version();
   return missing;

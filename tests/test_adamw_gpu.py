@@ -659,3 +659,18 @@ def test_lookups_that_run_python(ocl, bits):
     p.grad = torch.full_like(p, 2.0)  # its next step is a first one
     opt.step()
     assert opt.state[p]["step"].item() == 1
+
+
+def test_a_refused_step_changes_nothing(ocl):
+    """Of parameters of several types, one whose state does not fit: the others are not updated before the refusal."""
+    a = torch.ones(300).to(DEV).requires_grad_()
+    b = torch.ones(300, dtype=torch.bfloat16).to(DEV).requires_grad_()
+    for bits, key in ((32, "exp_avg"), (8, "exp_avg_scale")):
+        opt = ocl.optim.AdamW([a, b], **HYPER, state_bits=bits)
+        a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+        opt.step()
+        held = a.detach().cpu().clone()
+        opt.state[b][key] = torch.zeros(7).to(DEV)
+        with pytest.raises(RuntimeError, match="does not fit"):
+            opt.step()
+        assert torch.equal(a.detach().cpu(), held) and opt.state[a]["step"].item() == 1
