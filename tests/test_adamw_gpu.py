@@ -608,8 +608,8 @@ def test_a_first_step_is_not_captured(ocl, bits):
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_lookups_that_run_python(ocl, bits):
-    """A parameter's hash is Python code, in which gradients and states of others may go away: what the step found before
-    stays alive until it is done."""
+    """A parameter's hash is Python code, in which gradients and states of others may go away: a state that was found
+    before stays alive until the step is done, and a parameter whose gradient went is left as it is."""
     import gc
 
     at_last = []
@@ -630,8 +630,9 @@ def test_lookups_that_run_python(ocl, bits):
 
     def drop():
         for p in params[:3]:
-            p.grad = None
             del opt.state[p]
+        params[0].grad = None
+        params[1].grad = params[1].grad * 1.0
         gc.collect()
         # whatever was freed is written over
         junk = [torch.full((70000 + i,), float("nan")).to(DEV) for i in range(4) for _ in range(6)]
@@ -651,7 +652,8 @@ def test_lookups_that_run_python(ocl, bits):
     before = [p.detach().cpu().clone() for p in params]
     at_last.append(drop)
     opt.step()
-    for p, b in zip(params, before):
+    assert torch.equal(params[0].detach().cpu(), before[0])
+    for p, b in zip(params[1:], before[1:]):
         after = p.detach().cpu()
         assert torch.isfinite(after).all() and (after < b).all()
     assert list(opt.state) == params[3:]
