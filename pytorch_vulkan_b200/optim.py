@@ -71,12 +71,13 @@ class AdamW(torch.optim.Optimizer):
             raise
 
     def _init_state(self, p):
-        state = self.state[p]
-        state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+        # whole or not at all: memory may run out on the way
+        state = {"step": torch.zeros((), dtype=torch.float32, device=p.device)}
         if self.state_bits == 32:
             for key in _KEYS[32]:
                 state[key] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-            return state
+            self.state[p] = state
+            return
         n = p.numel()
         for key in _KEYS[8]:
             if not key.endswith("code"):
@@ -85,7 +86,7 @@ class AdamW(torch.optim.Optimizer):
                 state[key] = torch.zeros(n, dtype=torch.uint8, device=p.device)
             else:  # codes follow the parameter's memory order, which their strides keep
                 state[key] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
-        return state
+        self.state[p] = state
 
     def step(self, closure=None):
         # (no graph is recorded below: the update is no torch operation)

@@ -676,3 +676,29 @@ def test_a_refused_step_changes_nothing(ocl):
         with pytest.raises(RuntimeError, match="does not fit"):
             opt.step()
         assert torch.equal(a.detach().cpu(), held) and opt.state[a]["step"].item() == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_could_not_be_made_is_made_again(ocl, monkeypatch, bits):
+    """Memory that runs out while a state is made leaves none behind, and the next step makes it."""
+    p = torch.ones(300).to(DEV).requires_grad_()
+    opt = ocl.optim.AdamW([p], **HYPER, state_bits=bits)
+    p.grad = torch.ones(300).to(DEV)
+    made, zeros, zeros_like = [], torch.zeros, torch.zeros_like
+
+    def limited(f):
+        def call(*args, **kw):
+            made.append(1)
+            if len(made) == 2:
+                raise RuntimeError("out of memory")
+            return f(*args, **kw)
+        return call
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "zeros", limited(zeros))
+        m.setattr(torch, "zeros_like", limited(zeros_like))
+        with pytest.raises(RuntimeError, match="out of memory"):
+            opt.step()
+    assert (p.detach().cpu() == 1).all()
+    opt.step()
+    assert opt.state[p]["step"].item() == 1 and (p.detach().cpu() < 1).all()
