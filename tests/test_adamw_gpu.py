@@ -702,3 +702,23 @@ def test_a_state_that_could_not_be_made_is_made_again(ocl, monkeypatch, bits):
     assert (p.detach().cpu() == 1).all()
     opt.step()
     assert opt.state[p]["step"].item() == 1 and (p.detach().cpu() < 1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_maximize_is_the_step_along_the_negated_gradient(ocl, bits):
+    gen = torch.Generator().manual_seed(14)
+    ps = [rand(s, gen) for s in SHAPES]
+    up, down = ([p.to(DEV).requires_grad_() for p in ps] for _ in range(2))
+    one = ocl.optim.AdamW(up, **HYPER, state_bits=bits, maximize=True)
+    two = ocl.optim.AdamW(down, **HYPER, state_bits=bits)
+    for _ in range(3):
+        for a, b in zip(up, down):
+            g = rand(a.shape, gen, 0.1)
+            a.grad, b.grad = g.to(DEV), (-g).to(DEV)
+        one.step()
+        two.step()
+    for a, b, p in zip(up, down, ps):
+        assert torch.equal(a.detach().cpu(), b.detach().cpu())
+        assert not p.numel() or not torch.equal(a.detach().cpu(), p)
+        for k, v in one.state[a].items():
+            assert torch.equal(v.cpu(), two.state[b][k].cpu())

@@ -193,3 +193,24 @@ def test_forward_mode_is_refused(ocl):
             ocl.functional.relative_position_bias(table, 5, 5)
     want = ocl.functional.linear_cross_entropy(given[0], given[1], t.to(DEV), given[2])  # outside, as ever
     assert torch.isfinite(want.cpu())
+
+
+@TYPES
+@KEEP
+@pytest.mark.parametrize("size", [(2304, 1160, 4608), (2310, 8192, 2310), (9000, 520, 9001), (2304, 2304, 4608)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_more_tiles_than_pairs(ocl, monkeypatch, math_fp32, size, dtype, keep):
+    """Tiles of 256 columns that outnumber the pairs of SMs, with sums over K in several chunks, so that accumulators are
+    used again with either phase; tiles in groups the last of which is narrower; and dx laid down by one piece of the
+    vocabulary and added to by the next on tiles whose K is not cut."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    x, w, b, t = make(*size, dtype, bias=True, ignored=0.1)
+    scored = t >= 0
+    gi = scored.double() / scored.sum()
+    losses, err, grads, bounds = formula(x, w, b, t, gi, smooth=0.05, on="cuda")
+    got = run(ocl, x, w, b, t, label_smoothing=0.05)
+    want, bound = (gi.to("cuda") * losses).sum(), (gi.to("cuda") * err).sum()
+    within(got[0], want, bound + 2.0 ** -22 * want, "loss")
+    for a, r, e, what in zip(got[1:], grads, bounds, "xwb"):
+        within(a, r, e, what)
+    torch.cuda.empty_cache()
