@@ -84,7 +84,7 @@ struct LceScale {
 
 struct LceGemm {
   int M, N, K;
-  int a_row0, b_row0;     // where the operands' rows (K-major) or K rows (MN-major) begin in their maps
+  int b_row0;             // where B's rows (K-major) or K rows (MN-major) begin in its map
   int n_fast, group;      // tile order: columns (else rows) fastest, `group` of them at a time
   int splits, kb_per;     // kEpiAcc: split s takes k blocks [s kb_per, (s + 1) kb_per) into slab s
   // epilogues of logits: column n is vocabulary entry v0 + n
@@ -292,11 +292,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
             const uint32_t bar = even_cta_addr(&full[s]);
             if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::SLOT_BYTES);
             if (!a_mn) {
-              tma_load_3d_pair(sa, &tmA, bar, kb * kLBK, p.a_row0 + am, z);
+              tma_load_3d_pair(sa, &tmA, bar, kb * kLBK, am, z);
             } else {
 #pragma unroll
               for (int q = 0; q < 2; ++q)
-                tma_load_3d_pair(sa + q * 8192, &tmA, bar, am + 64 * q, p.a_row0 + kb * kLBK, z);
+                tma_load_3d_pair(sa + q * 8192, &tmA, bar, am + 64 * q, kb * kLBK, z);
             }
             if (!b_mn) {
               tma_load_3d_pair(sb, &tmB, bar, kb * kLBK, p.b_row0 + bn, z);
@@ -323,8 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
       const uint64_t b0 = b_mn ? desc_mnmajor16(smem0 + L::A_BYTES, 0, 8192) : desc_kmajor(smem0 + L::A_BYTES, 0);
       const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;
       uint32_t it = 0, chunk = 0;
-      int local = 0;
-      for (int tile = pair; tile < total_tiles && !*abort; tile += pairs, ++local) {
+      for (int tile = pair; tile < total_tiles && !*abort; tile += pairs) {
         int mb, nb, sp, kb0, kb1;
         place(tile, mb, nb, sp, kb0, kb1);
         for (int c0 = kb0; c0 < kb1; ++chunk) {
@@ -374,8 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
     uint8_t* box = smem + L::EPI_OFF + (warp - kLMmaWarp - 1) * 4096;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     uint32_t chunk = 0;
-    int local = 0;
-    for (int tile = pair; tile < total_tiles && !*abort; tile += pairs, ++local) {
+    for (int tile = pair; tile < total_tiles && !*abort; tile += pairs) {
       int mb, nb, sp, kb0, kb1;
       place(tile, mb, nb, sp, kb0, kb1);
       const int m0 = mb * kLBM + rank * 128 + quarter * 32, m = m0 + lane;
@@ -470,23 +468,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((LceSmem<P, BN>::THR
                   else tma_store_3d(&tmC, box, p.v0 + n0 + 32 * h, m0, 0);
                 });
           }
-          float cm = v[0];
+          mx = v[0];
 #pragma unroll
-          for (int j = 1; j < 64; ++j) cm = fmaxf(cm, v[j]);  // a NaN logit makes the sum NaN instead
-          const float base = cm == -INFINITY ? 0.f : cm;
-          float cs = 0.f;
+          for (int j = 1; j < 64; ++j) mx = fmaxf(mx, v[j]);  // a NaN logit makes the sum NaN instead
+          const float base = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
             v[j] = lce_exp<kPrecise>(v[j] - base);
-            cs += v[j];
+            sum += v[j];
           }
-          const float nm = fmaxf(mx, cm), nb = nm == -INFINITY ? 0.f : nm;
-          sum = sum * lce_exp<kPrecise>(mx - nb) + cs * lce_exp<kPrecise>(cm - nb);
-          mx = nm;
           if (!kPrecise && keep && m0 < p.M) {
             // -inf where all 64 are masked, whose codes are 0: any finite number there could make the factor that the
             // backward pass forms of it, exp(maximum - lse), infinite
-            if (mrow) p.keep_max[(int64_t)((p.v0 + n0) >> 6) * p.keep_ld + m] = cm;
+            if (mrow) p.keep_max[(int64_t)((p.v0 + n0) >> 6) * p.keep_ld + m] = mx;
             store_box(box, lane, [&](int phase) {
               if (phase == 0) box_codes(box, lane, v);
               else tma_store_3d(&tmC, box, p.v0 + n0, m0, 0);

@@ -90,8 +90,9 @@ __global__ void __launch_bounds__(256)
 }
 
 // grid: (segments of the rows) x (tiles of diagonals) x (B * H); part:
-// [B*H][nb][tiles][segments].  FLAT: unit stride along the keys; the gradient's
-// first element is at `low`, its last one 16 bytes before `high`.
+// [B*H][nb][tiles][segments].  FLAT: unit stride along the keys; `low` is the
+// gradient's first element and `high` the last address from which 16 bytes lie
+// within it.
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256, 3)
     rel_bias_bwd_kernel(const __grid_constant__ RelMap map, const T* __restrict__ grad, int64_t sb, int64_t sh,
