@@ -77,7 +77,7 @@ constexpr float k2p112 = 5192296858534827628530496329220096.f;
 enum { kEpiStats = 0, kEpiGrad = 1, kEpiAcc = 2, kEpiOut = 3 };
 
 // what a gradient's fp32 sums are multiplied by, on the device: a power of two
-// (fp16's scales), and a number for all rows or, unless NULL, one for each
+// (fp16's scales), and one number for each row (own) or for all (common)
 struct LceScale {
   const float *unit, *common, *own;
 };
@@ -668,9 +668,10 @@ __global__ void __launch_bounds__(1024, 2)
 }
 
 // what each row's gradient is multiplied by, where that is one number for all
-// rows (mean and sum): row[i] is 1 or 0, and one factor for all results
+// rows (mean and sum): row[i] is 1, and own[i] that number, or both 0 where row i
+// has no loss, whose dx is 0 under a gradient that is not finite too
 struct LceRowsJob {
-  float* row;             // NULL: nothing to do
+  float *row, *own;       // NULL: nothing to do
   float* factor;          // powers of two of db, dx (w's scale is in it) and dw (x's), and the number for all rows
   const float *grad_out, *count;
   const int64_t* target;
@@ -755,10 +756,13 @@ __global__ void __launch_bounds__(256)
     else lce_pack_one<S, T>(b, e - na, per_row, cols, ldp, planes, V, ignore, sw);
   }
   if (rj.row) {
-    for (int64_t i = first; i < rj.N; i += step) rj.row[i] = lce_scored(rj.target[i], V, ignore) ? 1.f : 0.f;
+    const float n = *rj.count, f = n > 0.f ? (rj.mean ? *rj.grad_out / n : *rj.grad_out) : 0.f;
+    for (int64_t i = first; i < rj.N; i += step) {
+      const bool scored = lce_scored(rj.target[i], V, ignore);
+      rj.row[i] = scored ? 1.f : 0.f;
+      rj.own[i] = scored ? f : 0.f;
+    }
     if (first == 0) {
-      float f = *rj.grad_out;
-      if (rj.mean) f = *rj.count > 0.f ? f / *rj.count : 0.f;
       rj.factor[0] = rj.inv_gscale;
       rj.factor[1] = rj.inv_gscale / sw;
       rj.factor[2] = rj.inv_gscale / sx;
@@ -1535,7 +1539,7 @@ struct LceBwdSpace {
   uint16_t *x, *w, *G;
   float *absmax, *scales;
   float *slab, *row, *factor, *dx, *dw, *colsum;  // factor: see LceRowsJob
-  float *one, *own;                               // where each row has its own gradient: see lce_grad_rows_kernel
+  float *own, *one;                               // see LceRowsJob; one: see lce_grad_rows_kernel
 };
 
 static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void* base, LceBwdSpace* s) {
@@ -1546,8 +1550,8 @@ static size_t lce_bwd_space(const pvb2_linear_ce_desc* d, const LcePlan& p, void
   s->G = a.take<uint16_t>(d->N * up(width, 64) * p.P);
   s->slab = a.take<float>(lce_slabs(p) ? p.z.splits * d->N * up(width, 4) : 0);
   s->row = a.take<float>(d->N);
+  s->own = a.take<float>(d->N);
   s->one = a.take<float>(d->reduction == PVB2_LOSS_NONE ? d->N : 0);
-  s->own = a.take<float>(d->reduction == PVB2_LOSS_NONE ? d->N : 0);
   const bool scales = p.P == 2 && lce_few_rows(d, p.ldp);
   s->absmax = a.take<float>(scales ? kLScaleBlocks : 0);
   s->scales = a.take<float>(scales ? 2 : 0);
@@ -2021,10 +2025,10 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   const float* zscale = given ? count + 1 : p.P == 2 ? sp.scales : nullptr;
   LceRowsJob rows = lce_no_rows();
   if (d->reduction != PVB2_LOSS_NONE)
-    rows = LceRowsJob{sp.row, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
+    rows = LceRowsJob{sp.row, sp.own, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
   const bool own = d->reduction == PVB2_LOSS_NONE;  // each row has its own gradient
   bool row_factors = !own;                          // or still to be formed, after the scales
-  const LceScale dx_scale{sp.factor + 1, sp.factor + 3, own ? sp.own : nullptr};
+  const LceScale dx_scale{sp.factor + 1, nullptr, sp.own};
   const LceScale dw_scale{sp.factor + 2, sp.factor + 3, nullptr};
   LceOperand px{x, 0, d->N, d->ldx, sp.x, target};
   CUtensorMap x_k, x_mn, w_k, w_mn, g_store, g_k, g_mn, acc;

@@ -214,3 +214,22 @@ def test_more_tiles_than_pairs(ocl, monkeypatch, math_fp32, size, dtype, keep):
     for a, r, e, what in zip(got[1:], grads, bounds, "xwb"):
         within(a, r, e, what)
     torch.cuda.empty_cache()
+
+
+@TYPES
+@KEEP
+@ROWS
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_upstream_gradients_that_are_no_numbers(ocl, monkeypatch, math_fp32, size, dtype, keep, reduction):
+    """An infinite gradient of the loss, or NaN: rows without a loss have the gradient 0 all the same, and without any row
+    that has one everything is 0."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    x, w, b, t = make(*size, dtype, bias=True)
+    t[4], t[1] = -100, size[2]
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        _, dx, dw, db = run(ocl, x, w, b, t, grad=torch.tensor(bad), reduction=reduction)
+        assert (dx[4] == 0).all() and (dx[1] == 0).all()
+        assert not torch.isfinite(dx[0]).any() and not torch.isfinite(dx[2:4]).any()
+        assert not torch.isfinite(db).any()
+        for g in run(ocl, x, w, b, torch.full_like(t, -100), grad=torch.tensor(bad), reduction=reduction)[1:]:
+            assert (g == 0).all()
