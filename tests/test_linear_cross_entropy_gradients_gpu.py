@@ -233,3 +233,29 @@ def test_upstream_gradients_that_are_no_numbers(ocl, monkeypatch, math_fp32, siz
         assert not torch.isfinite(db).any()
         for g in run(ocl, x, w, b, torch.full_like(t, -100), grad=torch.tensor(bad), reduction=reduction)[1:]:
             assert (g == 0).all()
+
+
+@TYPES
+@KEEP
+def test_losses_that_are_summed_afterwards(ocl, monkeypatch, math_fp32, dtype, keep):
+    """reduction="none" and a sum or mean of the losses: one number comes back for all rows, whatever the shape."""
+    monkeypatch.setenv("B200_CE_KEEP_MB", keep)
+    x, w, b, t = make(150, 72, 520, dtype, bias=True, ignored=0.2)
+    for shape in ((150,), (10, 15), (1, 150), (150, 1)):
+        leaves = [v.to(DEV).requires_grad_() for v in (x, w, b)]
+        xs, ts = leaves[0].view(*shape, 72), t.view(shape).to(DEV)
+        f = lambda red: ocl.functional.linear_cross_entropy(xs, leaves[1], ts, leaves[2], reduction=red)
+        want = torch.autograd.grad(f("sum"), leaves)
+        got = torch.autograd.grad(f("none").sum(), leaves)
+        assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(want, got))
+        each = torch.autograd.grad(f("none"), leaves, torch.ones(shape).to(DEV))
+        assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(want, each))
+        part = torch.full(shape[:-1] + (1,), 0.5)  # rows of the batch with a gradient each: no single number
+        part.view(-1)[0] = 2.0
+        expanded = torch.autograd.grad(f("none"), leaves, part.to(DEV).expand(shape))
+        each = torch.autograd.grad(f("none"), leaves, part.expand(shape).contiguous().to(DEV))
+        assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(expanded, each))
+    one = [v.to(DEV).requires_grad_() for v in (x[:1], w)]
+    f = lambda red: ocl.functional.linear_cross_entropy(*one, t.clamp(min=0)[:1].to(DEV), reduction=red)
+    for a, b in zip(torch.autograd.grad(f("none").sum() * 0.25, one), torch.autograd.grad(f("sum") * 0.25, one)):
+        assert torch.equal(a.cpu(), b.cpu())
