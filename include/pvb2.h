@@ -643,7 +643,7 @@ typedef struct pvb2_adamw_tensor {
   void* max_exp_avg_sq;    /* amsgrad only */
   float* exp_avg_scale;    /* 8-bit moments only: ceil(numel / 256) scales */
   float* exp_avg_sq_scale;
-  float* step;             /* device memory, one float */
+  float* step;             /* device memory, one float; with increment_step no other tensor's */
   int64_t numel;
 } pvb2_adamw_tensor;
 PVB2_API size_t pvb2_adamw_workspace_size(int n);
@@ -662,9 +662,9 @@ PVB2_API int pvb2_flatten_multi(int n, float* const* tensors, const int64_t* num
                        double scale, pvb2_stream stream);
 
 /* ------------------------------------------------------------------ */
-/* softmax cross entropy of a linear layer, z = x w^T + bias, without   */
-/* keeping z (the reference ran the linear layer, log_softmax and       */
-/* nll_loss one by one, vision_ops.cpp:243-351, loss_ops.cpp:23-213).   */
+/* softmax cross entropy of a linear layer, z = x w^T + bias (the       */
+/* reference ran the linear layer, log_softmax and nll_loss one by one, */
+/* vision_ops.cpp:243-351, loss_ops.cpp:23-213).                        */
 /*   loss_i = lse_i - (1 - s) z_i,t(i) - s / V sum_j z_ij               */
 /* with s the label smoothing; rows whose target is ignore_index or     */
 /* outside [0, V) have no loss and no gradient, and may hold anything.  */
@@ -699,7 +699,11 @@ PVB2_API int pvb2_linear_ce_fwd(const pvb2_linear_ce_desc* d, const void* x, con
                                 void* workspace, size_t workspace_bytes, pvb2_stream stream);
 /* grad_out: N floats (PVB2_LOSS_NONE) or one; lse and count from the forward
  * pass.  dx [N][D], dw [V][D] contiguous, dbias [V], of the operands' type;
- * each may be NULL. */
+ * each may be NULL.  They are fp32 sums of products with the logits' gradient,
+ * which is rounded to bf16 or fp16 before (two fp16 numbers for fp32 operands),
+ * either fp16 kind in steps of 2^-39 of the row's own; for dw and dbias, where
+ * each row has a gradient, of the largest of those.  After a forward pass with
+ * PVB2_LOSS_NONE the descriptor may say PVB2_LOSS_SUM, for one number. */
 PVB2_API size_t pvb2_linear_ce_bwd_workspace_size(const pvb2_linear_ce_desc* d);
 PVB2_API int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* d, const void* x, const void* w, const void* bias,
                                 const int64_t* target, const float* lse, const float* count, const void* kept,

@@ -1,5 +1,5 @@
 // Softmax cross entropy of a linear layer over a large vocabulary, z = x w^T + b,
-// and its gradients, without keeping z.
+// and its gradients.
 //
 //   lse_i = log sum_j exp z_ij      loss_i = lse_i - (1 - s) z_i,t(i) - s / V sum_j z_ij
 //   G_ij  = g_i (exp(z_ij - lse_i) - (1 - s) [j = t(i)] - s / V)
@@ -7,27 +7,38 @@
 //
 // Forward: one matrix product whose epilogue keeps, per row and 64
 // columns, the largest logit, the sum of exp(z - largest) and the target's
-// logit; a second launch joins them.  The logits never leave the chip.
-// Backward: per piece of the vocabulary, the logits are formed again and their
-// epilogue writes G in 16 bits (piece x tokens, sized to stay near the L2
-// cache); two products make dx += G w and the piece's rows of dw = G^T x.
-// Going by pieces of the vocabulary finishes dw in one go and adds dx up in
-// fp32: 8 N V D operations instead of the 6 that a stored z would take.
+// logit; a second launch joins them.  For a backward pass it also writes what
+// that needs of the first `kept` entries: the exponentials as 16-bit codes, for
+// fp32 operands the logits themselves (as the caller has memory for them).
+// Backward: per piece of the vocabulary, G in 16 bits (piece x tokens, sized to
+// stay near the L2 cache), from what was kept or from logits that are formed
+// again; two products make dx += G w and the piece's rows of dw = G^T x.  Going
+// by pieces of the vocabulary finishes dw in one go and adds dx up in fp32: 6 N
+// V D operations in all from what was kept, 8 without it, when nothing of the
+// size N x V exists.
 //
 // Operands are 16-bit (tcgen05 kind::f16, fp32 accumulators).  fp32 operands
 // are split into two fp16 numbers each, x = x0 + x1 (11 bits apiece), of which
 // three products are formed: x0 w0, x0 w1 and x1 w0.  What is left out is, in
 // the mean, 2^-24 of |x||w| (3 2^-22 at most), as much as rounding the product
 // to fp32 would cost; three bf16 parts, which need no scaling, took six
-// products for the same (1.88 ms a step of N 2048, D 768, V 32768 against
-// 1.34).  fp16's range is met by a power of two for each tensor that brings its
-// largest finite magnitude to 2^14 .. 2^15; parts below 2^-39 of that are lost.
+// products for the same (1.88 ms a step of N 2048, D 768, V 32768, where these
+// took 1.34 then and 1.08 now).  fp16's range is met by a power of two for each
+// tensor that brings its largest finite magnitude to 2^14 .. 2^15; parts below
+// 2^-39 of that are lost.
 //
-// G is formed without the factor that all rows share and, in fp16, times 2^15;
-// both are undone on the fp32 results.  Where each row has a gradient g_i of its
-// own, dx multiplies its rows by g_i at the end, so that a row's errors are
-// relative to itself, and what is not finite in one reaches no other; dw and db,
-// sums over rows, take a second G, of g_i / max|g|.
+// G is rounded to what the products take: bf16 or fp16 for such operands, which
+// puts a gradient 2.3e-3 (bf16, N 4095, D 1000, V 49999) from its value where
+// rounding it alone makes 1.7e-3, and saves half of both products against two
+// parts; two fp16 parts for fp32 operands.  db is summed from the same numbers.
+// G is formed without the factor that all rows share and, in fp16, times 2^15
+// (steps of 2^-39 are the least); both are undone on the fp32 results.  Where
+// each row has a gradient g_i of its own, dx multiplies its rows by g_i at the
+// end, so that a row's errors are relative to itself, and what is not finite in
+// one reaches no other; dw and db, sums over rows, take a second G, of g_i /
+// max|g| (8192 x 4096 -> 32768 bf16: 5.4 ms as with one G from what was kept,
+// 8.5 and 7.0 ms with nothing kept; 4095 x 1000 -> 49999: 1.46 and 1.27, 1.90 and
+// 1.59).
 #include <algorithm>
 #include <atomic>
 #include "tc_common.cuh"
@@ -946,7 +957,7 @@ __global__ void __launch_bounds__(512)
 // Here a warp reads R of w's rows at once, each lane 16 bytes of each, and
 // multiplies them by the NT rows of x from shared memory in fp32; its lanes
 // then keep the running maximum and sum of their row of x.  One V = 32768, D =
-// 2048 fp16 row: 25 us against 54.  R fills the registers: four rows of w for
+// 2048 fp16 row: 30 us and 4 for the join, against 54 on tiles.  R fills the registers: four rows of w for
 // one row of x in fp32 (V 32768, D 2048: 55 us, 75 with eight), four for eight
 // (87 us, 101 with two, where x's reads from shared memory bound it).
 template <int L>
@@ -1317,11 +1328,11 @@ struct LceTiling {
   double cycles;
 };
 
-// The cut with the least modelled time.  Cycles of a K block of a tile:
-// 512 for 256 x 256 (both the MMAs' rate and that of the loads from L2), for
-// 256 x 128 the loads' 384; for split operands 512 a product, and on 256 x 128
-// 400, where the MMAs' reads and the loads' writes share 128 bytes of shared
-// memory a cycle.  A tile costs about 2500 more (its last loads and its epilogue), joining slabs
+// The cut with the least modelled time.  Cycles of a K block of a tile, for each
+// product: 520 for 256 x 256 (512 is both the MMAs' rate and that of 16-bit
+// operands' loads from L2), 400 for 256 x 128, where 16-bit operands wait for
+// their loads (384) and split ones' MMA reads share 128 bytes of shared memory a
+// cycle with the loads' writes.  A tile costs about 2500 more (its last loads and its epilogue), joining slabs
 // their traffic and a launch.
 static LceTiling lce_tiling(int64_t M, int64_t N, int64_t K, int P, int64_t read_bytes, bool cut = true) {
   const int64_t kb = cdiv(K, kLBK), pairs = lce_pairs_on_device();
@@ -1390,9 +1401,10 @@ static LcePlan lce_make_plan(const pvb2_linear_ce_desc* d, bool backward) {
   // packed rows begin on 128-byte lines, unless that would be mostly padding
   p.ldp = up(d->D, d->D >= 256 ? 64 : 8);
   // Rows of w that straddle lines take two reads from L2 for each 128 bytes.  A
-  // copy costs the same for any number of tokens and pays from about 3000 on
+  // copy costs the same for any number of tokens and pays from about 3500 on
   // (D 1000, V 49999, forward: 397 us as it lies and 376 us with the copy at
-  // 4095 tokens, 196 and 244 us at 2048).
+  // 4095 tokens, 196 and 244 us at 2048; between the two, where a line through
+  // the differences is 0).
   p.pack_w = !lce_direct(d, d->ldw) || (d->ldw % 64 != 0 && d->D >= 256 && d->N >= 3500);
   p.pack_x = !lce_direct(d, d->ldx) || (d->ldx % 64 != 0 && d->D >= 256 && d->V >= 2048);
   p.few = !backward && lce_few_rows(d, p.ldp);
