@@ -768,14 +768,6 @@ static int at_check(const pvb2_sdpa_desc* d) {
   return PVB2_OK;
 }
 
-// `done`: the calling kernel's own per-device flag
-template <typename K>
-static int at_smem_attr(K kernel, int bytes, std::atomic<uint64_t>& done) {
-  if (first_on_device(done))
-    PVB2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  return PVB2_OK;
-}
-
 template <int D>
 static int at_fwd(const AtView& q, const AtView& k, const AtView& v, const AtView& o, float* lse, const AtArgs& a,
                   bool tc, cudaStream_t s) {
@@ -783,16 +775,16 @@ static int at_fwd(const AtView& q, const AtView& k, const AtView& v, const AtVie
   if constexpr (D <= 64) {
     if (tc) {
       const int smem = (2 * kAtB * (D + 4) + kAtB * (D + 8) + 4 * 16 * kTcPS) * 4;
-      static std::atomic<uint64_t> attr_tc{0};
-      PVB2_TRY(at_smem_attr(sdpa_fwd_tc_kernel<D>, smem, attr_tc));
+      static DeviceOnce attr_tc;
+      PVB2_TRY(allow_smem(sdpa_fwd_tc_kernel<D>, smem, attr_tc));
       sdpa_fwd_tc_kernel<D><<<grid, kTcThreads, smem, s>>>(q, k, v, o, lse, a);
       PVB2_LAUNCH_CHECK();
       return PVB2_OK;
     }
   }
   const int smem = (3 * AtCfg<D>::TILE + AtCfg<D>::PTILE) * 4;
-  static std::atomic<uint64_t> attr{0};
-  PVB2_TRY(at_smem_attr(sdpa_fwd_kernel<D>, smem, attr));
+  static DeviceOnce attr;
+  PVB2_TRY(allow_smem(sdpa_fwd_kernel<D>, smem, attr));
   sdpa_fwd_kernel<D><<<grid, kAtThreads, smem, s>>>(q, k, v, o, lse, a);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
@@ -817,14 +809,14 @@ static int at_bwd(const AtView& q, const AtView& k, const AtView& v, const AtVie
   sdpa_bwd_di_kernel<D><<<(unsigned)((rows * 32 + 255) / 256), 256, 0, s>>>(g, o, di, a);
   PVB2_LAUNCH_CHECK();
   using C = AtCfg<D>;
-  static std::atomic<uint64_t> attr_kv{0}, attr_q{0}, attr_tc{0};
+  static DeviceOnce attr_kv, attr_q, attr_tc;
   const int nkb = (a.Lk + kAtB - 1) / kAtB;
   const dim3 gk((unsigned)nkb, (unsigned)(a.B * a.H));
   bool done = false;
   if constexpr (D <= 64) {
     if (tc) {
       const int stc = (4 * kAtB * (D + 4) + 2 * kAtB * kTcPS + 2 * kAtB) * 4;
-      PVB2_TRY(at_smem_attr(sdpa_bwd_kv_tc_kernel<D>, stc, attr_tc));
+      PVB2_TRY(allow_smem(sdpa_bwd_kv_tc_kernel<D>, stc, attr_tc));
       sdpa_bwd_kv_tc_kernel<D><<<gk, kTcThreads, stc, s>>>(q, k, v, g, lse, di, dk, dv, dq_part, a);
       PVB2_LAUNCH_CHECK();
       done = true;
@@ -832,7 +824,7 @@ static int at_bwd(const AtView& q, const AtView& k, const AtView& v, const AtVie
   }
   if (!done) {
     const int skv = (4 * C::TILE + 2 * C::PTILE + 2 * kAtB) * 4;
-    PVB2_TRY(at_smem_attr(sdpa_bwd_kv_kernel<D>, skv, attr_kv));
+    PVB2_TRY(allow_smem(sdpa_bwd_kv_kernel<D>, skv, attr_kv));
     sdpa_bwd_kv_kernel<D><<<gk, kAtThreads, skv, s>>>(q, k, v, g, lse, di, dk, dv, dq_part, a);
     PVB2_LAUNCH_CHECK();
   }
@@ -842,7 +834,7 @@ static int at_bwd(const AtView& q, const AtView& k, const AtView& v, const AtVie
     return PVB2_OK;
   }
   const int sq = (4 * C::TILE + C::PTILE + 2 * kAtB) * 4;
-  PVB2_TRY(at_smem_attr(sdpa_bwd_dq_kernel<D>, sq, attr_q));
+  PVB2_TRY(allow_smem(sdpa_bwd_dq_kernel<D>, sq, attr_q));
   const dim3 gq((unsigned)((a.Lq + kAtB - 1) / kAtB), (unsigned)(a.B * a.H));
   sdpa_bwd_dq_kernel<D><<<gq, kAtThreads, sq, s>>>(q, k, v, g, lse, di, dq, a);
   PVB2_LAUNCH_CHECK();

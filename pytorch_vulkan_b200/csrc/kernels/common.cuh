@@ -7,6 +7,7 @@
 #include <stdio.h>
 #include <string.h>
 #include <atomic>
+#include <mutex>
 #include <string>
 #include "../../../include/pvb2.h"
 
@@ -172,13 +173,24 @@ __device__ __forceinline__ void iter_offsets(const IterShape& it, int nargs, int
   }
 }
 
-// true the first time it is called with `mask` on the current device (for
-// per-device one-time setup such as cudaFuncSetAttribute)
-inline bool first_on_device(std::atomic<uint64_t>& mask) {
+// The shared memory that a kernel may take, set once on each device.  A thread
+// that finds it not done waits for the one that sets it: a launch before that
+// would be refused.  `once`: the kernel's own.
+struct DeviceOnce {
+  std::atomic<uint64_t> done{0};
+  std::mutex m;
+};
+template <typename K>
+int allow_smem(K kernel, int bytes, DeviceOnce& once) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return true;
+  PVB2_CUDA_TRY(cudaGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
-  return (mask.fetch_or(bit) & bit) == 0;
+  if (once.done.load(std::memory_order_acquire) & bit) return PVB2_OK;
+  std::lock_guard<std::mutex> lock(once.m);
+  if (once.done.load(std::memory_order_relaxed) & bit) return PVB2_OK;
+  PVB2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  once.done.fetch_or(bit, std::memory_order_release);
+  return PVB2_OK;
 }
 
 // Division by a runtime divisor d as a multiply-high and shift (Granlund and

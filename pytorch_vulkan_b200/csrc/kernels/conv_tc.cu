@@ -1000,10 +1000,8 @@ template <int BN, int MODE, int KB = 1>
 static int launch_conv(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, const ConvTcArgs& a,
                        cudaStream_t s) {
   constexpr int smem = ConvSmem<BN, KB>::TOTAL + 1024;
-  static std::atomic<uint64_t> attr_done{0};
-  if (first_on_device(attr_done))
-    PVB2_CUDA_TRY(
-        cudaFuncSetAttribute(conv_tf32_kernel<BN, MODE, KB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static DeviceOnce once;
+  PVB2_TRY(allow_smem(conv_tf32_kernel<BN, MODE, KB>, smem, once));
   if (a.tiles <= 0) return PVB2_OK;
   const int grid = std::min(a.tiles, num_sms());
   conv_tf32_kernel<BN, MODE, KB><<<grid, cThreads, smem, s>>>(ma, mb, mc, a);

@@ -389,10 +389,8 @@ template <int BN, bool A_MN, bool B_MN>
 static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, const GemmEpi& ep,
                        cudaStream_t s) {
   constexpr int smem = GemmSmem<BN>::TOTAL + 1024;
-  static std::atomic<uint64_t> attr_done{0};
-  if (first_on_device(attr_done))
-    PVB2_CUDA_TRY(cudaFuncSetAttribute(gemm_tf32_kernel<BN, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       smem));
+  static DeviceOnce once;
+  PVB2_TRY(allow_smem(gemm_tf32_kernel<BN, A_MN, B_MN>, smem, once));
   const int tiles = ((ep.M + kBM - 1) / kBM) * ((ep.N + BN - 1) / BN) * ep.batch * ep.splits;
   const int grid = std::min(tiles, num_sms());
   gemm_tf32_kernel<BN, A_MN, B_MN><<<grid, kThreads, smem, s>>>(ma, mb, mc, ep);

@@ -40,7 +40,6 @@
 // 8.5 and 7.0 ms with nothing kept; 4095 x 1000 -> 49999: 1.46 and 1.27, 1.90 and
 // 1.59).
 #include <algorithm>
-#include <atomic>
 #include "tc_common.cuh"
 #include "types.cuh"
 
@@ -1632,9 +1631,8 @@ static int lce_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensor
                       bool b_mn, cudaStream_t s) {
   constexpr int smem = LceSmem<P, BN>::TOTAL + 1024;
   auto kernel = lce_gemm_kernel<EPI, T, P, BN, CHUNK>;
-  static std::atomic<uint64_t> attr_done{0};
-  if (first_on_device(attr_done))
-    PVB2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static DeviceOnce once;
+  PVB2_TRY(allow_smem(kernel, smem, once));
   const int64_t tiles = cdiv(g.M, kLBM) * cdiv(g.N, BN) * g.splits;
   PVB2_CHECK_ARG(tiles < INT32_MAX / 2, "linear cross entropy: too many tiles");
   const int grid = 2 * (int)std::min<int64_t>(tiles, lce_pairs_on_device());
@@ -1793,11 +1791,8 @@ static int lce_few_launch(const pvb2_linear_ce_desc* d, const void* x, const voi
                           const int64_t* target, const LceFwdSpace& sp, const LceKept& k, cudaStream_t s) {
   const bool vec = ((uintptr_t)w & 15) == 0 && d->ldw * sizeof(S) % 16 == 0;
   auto kernel = vec ? lce_few_rows_kernel<S, NT, R, true> : lce_few_rows_kernel<S, NT, R, false>;
-  static std::atomic<uint64_t> attr_done{0};
-  if (first_on_device(attr_done)) {
-    PVB2_CUDA_TRY(cudaFuncSetAttribute(lce_few_rows_kernel<S, NT, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLFewBytes));
-    PVB2_CUDA_TRY(cudaFuncSetAttribute(lce_few_rows_kernel<S, NT, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLFewBytes));
-  }
+  static DeviceOnce once[2];
+  PVB2_TRY(allow_smem(kernel, kLFewBytes, once[vec]));
   const size_t smem = (size_t)NT * up(d->D, 8) * sizeof(S);
   kernel<<<lce_few_blocks(d), 256, smem, s>>>((const S*)x, d->ldx, (const S*)w, d->ldw, (const S*)bias, target,
                                               (int)d->N, (int)d->D, (int)d->V, d->ignore_index,
