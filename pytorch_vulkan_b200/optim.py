@@ -133,7 +133,8 @@ class AdamW(torch.optim.Optimizer):
         numels = {"step": 1, "exp_avg": n, "exp_avg_sq": n, "exp_avg_code": n, "exp_avg_rms_code": n,
                   "exp_avg_scale": blocks, "exp_avg_rms_scale": blocks}
         return set(state) == {"step", *_KEYS[self.state_bits]} and all(
-            isinstance(v, torch.Tensor) and v.numel() == numels[k] for k, v in state.items())
+            isinstance(v, torch.Tensor) and v.numel() == numels[k]
+            and v.dtype == (torch.uint8 if k.endswith("code") else torch.float32) for k, v in state.items())
 
     def load_state_dict(self, state_dict):
         """As torch's, but the state keeps its own types (torch casts floating state to the parameters'), and one that

@@ -722,3 +722,28 @@ def test_maximize_is_the_step_along_the_negated_gradient(ocl, bits):
         assert not p.numel() or not torch.equal(a.detach().cpu(), p)
         for k, v in one.state[a].items():
             assert torch.equal(v.cpu(), two.state[b][k].cpu())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_of_other_types_is_refused_when_it_is_loaded(ocl, bits):
+    """torch's optimizers keep moments in the parameters' type: refused at once, not by the next step."""
+    p = torch.ones(300, dtype=torch.bfloat16).to(DEV).requires_grad_()
+    opt = ocl.optim.AdamW([p], **HYPER, state_bits=bits)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    held = {k: v.cpu().clone() for k, v in opt.state[p].items()}
+    saved = opt.state_dict()
+    for key in held:
+        other = {"state": {0: dict(saved["state"][0])}, "param_groups": saved["param_groups"]}
+        other["state"][0][key] = other["state"][0][key].cpu().to(torch.bfloat16)
+        with pytest.raises(ValueError, match="state of parameter 0"):
+            opt.load_state_dict(other)
+        assert all(torch.equal(opt.state[p][k].cpu(), v) for k, v in held.items())
+    opt.step()
+    if bits == 32:
+        q = torch.ones(300, dtype=torch.bfloat16).to(DEV).requires_grad_()
+        theirs = torch.optim.AdamW([q], fused=True, **HYPER)
+        q.grad = torch.ones_like(q)
+        theirs.step()
+        with pytest.raises(ValueError, match="state of parameter 0"):
+            opt.load_state_dict(theirs.state_dict())
