@@ -288,7 +288,8 @@ static pybind11::list adamw_step(const pybind11::list& params, const pybind11::d
         adam_codes(it.state, p, t);
       } else {
         t.exp_avg = adam_held(it.state.get(state_keys().exp_avg), p, at::kFloat, t.numel, Held::kAsParam, "exp_avg");
-        t.exp_avg_sq = adam_held(it.state.get(state_keys().exp_avg_sq), p, at::kFloat, t.numel, Held::kAsParam, "exp_avg_sq");
+        t.exp_avg_sq =
+            adam_held(it.state.get(state_keys().exp_avg_sq), p, at::kFloat, t.numel, Held::kAsParam, "exp_avg_sq");
       }
       t.step = step_ptr(it.state.get(state_keys().step), dev, i);
       ts.push_back(t);

@@ -956,9 +956,10 @@ __global__ void __launch_bounds__(512)
 // Here a warp reads R of w's rows at once, each lane 16 bytes of each, and
 // multiplies them by the NT rows of x from shared memory in fp32; its lanes
 // then keep the running maximum and sum of their row of x.  One V = 32768, D =
-// 2048 fp16 row: 30 us and 4 for the join, against 54 on tiles.  R fills the registers: four rows of w for
-// one row of x in fp32 (V 32768, D 2048: 55 us, 75 with eight), four for eight
-// (87 us, 101 with two, where x's reads from shared memory bound it).
+// 2048 fp16 row: 30 us and 4 for the join, against 54 on tiles.  R fills the
+// registers: four rows of w for one row of x in fp32 (V 32768, D 2048: 55 us, 75
+// with eight), four for eight (87 us, 101 with two, where x's reads from shared
+// memory bound it).
 template <int L>
 __device__ __forceinline__ float sum_spread(float (&a)[L], int lane) {
   // sums of L values over the warp, value i in the lanes i * 32 / L ..
@@ -1331,8 +1332,8 @@ struct LceTiling {
 // product: 520 for 256 x 256 (512 is both the MMAs' rate and that of 16-bit
 // operands' loads from L2), 400 for 256 x 128, where 16-bit operands wait for
 // their loads (384) and split ones' MMA reads share 128 bytes of shared memory a
-// cycle with the loads' writes.  A tile costs about 2500 more (its last loads and its epilogue), joining slabs
-// their traffic and a launch.
+// cycle with the loads' writes.  A tile costs about 2500 more (its last loads and
+// its epilogue), joining slabs their traffic and a launch.
 static LceTiling lce_tiling(int64_t M, int64_t N, int64_t K, int P, int64_t read_bytes, bool cut = true) {
   const int64_t kb = cdiv(K, kLBK), pairs = lce_pairs_on_device();
   const double read = read_bytes / 3200.0;  // cycles at 6.1 TB/s and 1.9 GHz
@@ -1823,8 +1824,8 @@ static int lce_slab_logits(const pvb2_linear_ce_desc* d, const LcePlan& p, const
 
 template <typename T>
 static int lce_kept_grad(const pvb2_linear_ce_desc* d, const LcePlan& p, const LceBwdSpace& sp, const LceKept& k,
-                         const int64_t* target, const float* lse, const float* grow, int64_t v0, int64_t width, int64_t ldg,
-                         float gscale, cudaStream_t s) {
+                         const int64_t* target, const float* lse, const float* grow, int64_t v0, int64_t width,
+                         int64_t ldg, float gscale, cudaStream_t s) {
   const unsigned rows = (unsigned)std::min<int64_t>(d->N, 32768);
   const dim3 grid((unsigned)cdiv(ldg, k.fp32 ? 4096 : 8192), rows, (unsigned)cdiv(d->N, rows));
   const float smoothing = (float)d->label_smoothing;
@@ -2032,7 +2033,8 @@ int pvb2_linear_ce_bwd(const pvb2_linear_ce_desc* desc, const void* x, const voi
   const float* zscale = given ? count + 1 : p.P == 2 ? sp.scales : nullptr;
   LceRowsJob rows = lce_no_rows();
   if (d->reduction != PVB2_LOSS_NONE)
-    rows = LceRowsJob{sp.row, sp.own, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN, 1.f / gscale};
+    rows = LceRowsJob{sp.row, sp.own, sp.factor, grad_out, count, target, d->N, d->reduction == PVB2_LOSS_MEAN,
+                      1.f / gscale};
   const bool own = d->reduction == PVB2_LOSS_NONE;  // each row has its own gradient
   bool row_factors = !own;                          // or still to be formed, after the scales
   const LceScale dx_scale{sp.factor + 1, nullptr, sp.own};
