@@ -291,8 +291,10 @@ def _plain_norm(case, s):
         short = -D % _GROUP
         y = torch.nn.functional.pad(y, (0, short)).view(rows, -1, _GROUP)
         most = y.abs().amax(2, keepdim=True)
-        codes = (y * torch.where(most > 2.0 ** -100, 448.0 / most, 0.0)).to(torch.float8_e4m3fn)
-        scales = torch.where(most > 2.0 ** -100, most / 448.0, 0.0)
+        # (448 as a tensor: a quotient with a number is a product with a reciprocal, rounded twice)
+        top = torch.full_like(most, 448.0)
+        codes = (y * torch.where(most > 2.0 ** -100, top / most, 0.0)).to(torch.float8_e4m3fn)
+        scales = torch.where(most > 2.0 ** -100, most / top, 0.0)
         return [(codes.float() * scales).view(rows, -1)[:, :D], *kept]
     if case["mode"] == "serve":
         return [y.to(dt), *kept]
