@@ -737,6 +737,99 @@ PVB2_API int pvb2_relative_bias_bwd(const pvb2_relative_bias_desc* d, const pvb2
                                     void* workspace, size_t workspace_bytes, pvb2_stream stream);
 
 /* ------------------------------------------------------------------ */
+/* root-mean-square norm of rows (no counterpart in the reference, whose */
+/* layer norm is norm_ops.cpp:167-351)                                  */
+/*   h = x + residual (x without one), rounded to the type              */
+/*   y = h / sqrt(mean(h^2) + eps) * weight                             */
+/* fp32, fp16 or bf16, all of one type, unit stride along a row; weight */
+/* may be NULL (ones).  The mean of squares is summed in 64 bits, all   */
+/* else is fp32, one rounding to the type.                              */
+/* ------------------------------------------------------------------ */
+typedef struct pvb2_rms_norm_desc {
+  int64_t rows, D;
+  int64_t ldx, ldr, ldg, ldc;  /* row strides of x (backward: h), residual (backward: gsum), gy, codes */
+  double eps;
+  int32_t dtype;
+} pvb2_rms_norm_desc;
+/* y and sum (h; with a residual only) [rows][D] contiguous; rstd: one float
+ * per row for the backward pass, or NULL */
+PVB2_API int pvb2_rms_norm_fwd(const pvb2_rms_norm_desc* d, const void* x, const void* residual, const void* weight,
+                               void* y, void* sum, float* rstd, pvb2_stream stream);
+/* gsum: the gradient of `sum`, or NULL; dx (x's and the residual's) [rows][D]
+ * and dw [D] contiguous, each may be NULL.  dw is summed in a fixed order. */
+PVB2_API size_t pvb2_rms_norm_bwd_workspace_size(const pvb2_rms_norm_desc* d);
+PVB2_API int pvb2_rms_norm_bwd(const pvb2_rms_norm_desc* d, const void* h, const void* weight, const float* rstd,
+                               const void* gy, const void* gsum, void* dx, void* dw, void* workspace,
+                               size_t workspace_bytes, pvb2_stream stream);
+/* 8-bit floating point with scales: e4m3 codes, one fp32 scale for every 128
+ * consecutive elements of a row ("tall": for 128 x 128 of a matrix), the last
+ * ones short.  scale = m / 448 with m the block's largest magnitude, codes are
+ * y (448 / m) rounded to nearest even; a block of 2^-100 or less is 0 with the
+ * scale 0, one with an infinity or a NaN is NaN.  rms_norm_8bit: the codes of y
+ * before it is rounded to the type.  scales [rows or ceil(rows / 128)][ceil(D / 128)]. */
+PVB2_API int pvb2_rms_norm_8bit(const pvb2_rms_norm_desc* d, const void* x, const void* residual, const void* weight,
+                                uint8_t* codes, float* scales, void* sum, pvb2_stream stream);
+PVB2_API int pvb2_quantize_8bit(int dtype, int64_t rows, int64_t D, const void* x, int64_t ldx, int tall,
+                                uint8_t* codes, int64_t ldc, float* scales, pvb2_stream stream);
+/* out [rows][D] = code * scale */
+PVB2_API int pvb2_dequantize_8bit(int64_t rows, int64_t D, const uint8_t* codes, int64_t ldc, const float* scales,
+                                  int tall, int dtype, void* out, pvb2_stream stream);
+/* y [M][N] = x w^T + bias of such codes: x [M][K] with a scale for every 128
+ * of a row, w [N][K] with one for every 128 x 128; rows begin on 16-byte
+ * boundaries.  y and bias (or NULL) are of d->dtype.  Blocks of 128 inputs are
+ * multiplied on the tensor cores and summed in fp32. */
+typedef struct pvb2_linear8_desc {
+  int64_t M, N, K;
+  int64_t ldx, ldw;
+  int32_t dtype;
+} pvb2_linear8_desc;
+PVB2_API int pvb2_linear8(const pvb2_linear8_desc* d, const uint8_t* x, const float* x_scales, const uint8_t* w,
+                          const float* w_scales, const void* bias, void* y, pvb2_stream stream);
+/* whether a bounded wait of its kernels ever gave up (as pvb2_tc_status) */
+PVB2_API int pvb2_linear8_status(int* timed_out, int reset);
+
+/* ------------------------------------------------------------------ */
+/* log probabilities of given tokens, entropy and best alternatives of  */
+/* logits [N][V] (the reference had log_softmax and nll_loss,           */
+/* loss_ops.cpp:23-213): logp = z_t - lse, entropy = -sum p log p.      */
+/* A token outside [0, V) has the log probability 0 and no gradient; a  */
+/* row whose logits are all -inf has -inf, the entropy 0 and no         */
+/* gradient.  The top best (at most 32) by falling logit, of equal ones */
+/* the lower index first, with their log probabilities.                 */
+/* ------------------------------------------------------------------ */
+typedef struct pvb2_token_logp_desc {
+  int64_t N, V, ldz;
+  int32_t dtype, top;
+} pvb2_token_logp_desc;
+/* logp, entropy [N]; stats: 3 N floats for the backward pass, or NULL;
+ * top_logp, top_index [N][top] */
+PVB2_API int pvb2_token_logp_fwd(const pvb2_token_logp_desc* d, const void* logits, const int64_t* tokens, float* logp,
+                                 float* entropy, float* stats, float* top_logp, int64_t* top_index,
+                                 pvb2_stream stream);
+/* g_logp, g_entropy: [N], one number for all rows where one_* is not 0, or
+ * NULL; dlogits [N][V] contiguous, of the logits' type */
+PVB2_API int pvb2_token_logp_bwd(const pvb2_token_logp_desc* d, const void* logits, const int64_t* tokens,
+                                 const float* stats, const float* g_logp, int one_logp, const float* g_entropy,
+                                 int one_entropy, void* dlogits, pvb2_stream stream);
+
+/* ------------------------------------------------------------------ */
+/* the norm of many gradients as one vector, and their scaling          */
+/*   norm = (sum |g|^p)^(1/p), p = norm_type 1 or 2, 0: the maximum     */
+/*   scale: g *= min(1, max_norm / (norm + 1e-6)), rounded to g's type  */
+/* *norm (device memory) is written in either case.  Gradients are      */
+/* dense; fp32, fp16 and bf16 ones may be mixed.  Sums are in 64 bits   */
+/* and in a fixed order.                                                */
+/* ------------------------------------------------------------------ */
+typedef struct pvb2_grad {
+  void* data;
+  int64_t numel;
+  int32_t dtype;
+} pvb2_grad;
+PVB2_API size_t pvb2_clip_grad_norm_workspace_size(int n);
+PVB2_API int pvb2_clip_grad_norm(int n, const pvb2_grad* tensors, int norm_type, int scale, double max_norm, float* norm,
+                                 void* workspace, size_t workspace_bytes, pvb2_stream stream);
+
+/* ------------------------------------------------------------------ */
 /* random (src/random_ops.cpp): Philox-4x32-10 counter-based generator  */
 /* (Salmon et al., SC'11).  Element i of the output uses counter        */
 /* (offset + i/4) and key `seed`, lane i%4.                             */

@@ -361,6 +361,42 @@ static void adamw8_values(const pybind11::list& params, const pybind11::dict& st
   }
 }
 
+// ------------------------------------------------------- clipping by the norm
+// The norm of the gradients of `params` (those that have one) as one vector:
+// norm_type 1, 2, or 0 for the maximum; with `scale` they are scaled to it.
+static at::Tensor clip_grad_norm(const pybind11::list& params, double max_norm, int64_t norm_type, bool scale) {
+  const pybind11::tuple list(params);
+  std::vector<at::Tensor> grads;
+  std::vector<pvb2_grad> gs;
+  grads.reserve(list.size());
+  gs.reserve(list.size());
+  for (const pybind11::handle h : list) {
+    const at::Tensor& g = py_tensor(h.ptr(), "a parameter").grad();
+    if (!g.defined()) continue;
+    const size_t i = grads.size();
+    TORCH_CHECK(!g.is_sparse() && is_ocl(g) && adam_type(g.scalar_type()),
+                "ocl clip_grad_norm_: fp32, fp16 or bf16 gradients on ocl expected, got ", g.scalar_type(), " on ", g.device(),
+                " at ", i);
+    TORCH_CHECK(grads.empty() || g.device() == grads[0].device(), "ocl clip_grad_norm_: gradients on ", grads[0].device(),
+                " and ", g.device());
+    TORCH_CHECK(g.is_non_overlapping_and_dense(), "ocl clip_grad_norm_: gradient ", i, " has gaps or overlaps in memory");
+    grads.push_back(g);
+    gs.push_back({g.numel() ? g.data_ptr() : nullptr, g.numel(), dtype_code(g.scalar_type())});
+  }
+  if (grads.empty()) return at::zeros({}, at::kFloat);
+  const int dev = grads[0].device().index();
+  DeviceScope scope(dev);
+  OCL_OP("clip_grad_norm_", dev);
+  at::Tensor norm = empty({}, at::kFloat, dev);
+  const int n = (int)gs.size();
+  Workspace ws(pvb2_clip_grad_norm_workspace_size(n), dev);
+  OCL_CHECK(pvb2_clip_grad_norm(n, gs.data(), (int)norm_type, scale ? 1 : 0, max_norm, (float*)norm.data_ptr(), ws.get(),
+                                ws.bytes, stream_for(dev)));
+  if (scale)
+    for (const at::Tensor& g : grads) g.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 // -------------------------------------------------- relative position bias
 static pvb2_relative_bias_desc bias_desc(c10::ScalarType type, int64_t buckets, int64_t heads, int64_t q_len,
                                          int64_t k_len, bool bidirectional, int64_t max_distance, int64_t q_offset) {
@@ -676,5 +712,6 @@ TORCH_LIBRARY_IMPL(aten, PrivateUse1, m) {
 
 void register_train_bindings(pybind11::module& m) {
   m.def("impl_adamw_step", &ocl::adamw_step, "one AdamW step over a group's parameters");
+  m.def("impl_clip_grad_norm", &ocl::clip_grad_norm, "the gradients' norm, and their scaling to it");
   m.def("impl_adamw8_values", &ocl::adamw8_values, "the moments that 8-bit codes stand for");
 }

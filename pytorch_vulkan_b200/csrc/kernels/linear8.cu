@@ -1,0 +1,573 @@
+// A linear layer in 8-bit floating point: e4m3 codes with one fp32 scale for
+// every 128 inputs of a row of x and for every 128 x 128 of the weight,
+//
+//   y[m][n] = sum over b of xs[m][b] ws[n / 128][b] sum_{k in block b} xc[m][k] wc[n][k]  + bias[n]
+//
+// The inner sums are the tensor cores' (tcgen05.mma kind::f8f6f4, four steps of
+// 32 along K, fp32 in TMEM); the outer one is formed in registers, since the
+// scales change with the block.  A block's products go to one of two
+// accumulators; while the epilogue's warps read one, multiply it by its scales
+// and add it to their sums, the tensor core fills the other.  Products of codes
+// are exact, a block's 128 of them lose bits below 2^-24 of their largest, and
+// what the epilogue adds rounds as fp32 does.
+//
+// Two kernels:
+//   * many rows: CTA pairs (cta_group::2) on tiles of 256 rows x 256 outputs,
+//     persistent, loads by TMA into a ring of six K blocks, stores by TMA.  A
+//     block's products take the tensor core 512 clocks, the epilogue about as
+//     many instructions: it is bound by both, and by the board's power.
+//   * few rows: tiles of 128 outputs x 16 to 128 rows, the weight in the
+//     place of the left operand, so that one row costs little; K is split over
+//     the CTAs of a cluster where the tiles are few, whose sums join through
+//     shared memory in a fixed order.  Bound by the weight's bytes.
+#include <algorithm>
+#include <type_traits>
+#include "quant8.cuh"
+#include "tc_common.cuh"
+
+namespace pvb2 {
+
+constexpr int kL8BK = kGroup8;  // a K block: one scale, and a 128-byte row of a swizzled tile
+
+struct L8Args {
+  const float* xs;   // [M][blocks]
+  const float* ws;   // [ceil(N / 128)][blocks]
+  const void* bias;  // of the output's type, or null
+  void* y;           // [M][N]
+  int M, N, blocks;
+  int tma_store;
+  int group;         // blocks of rows whose tiles lie together
+};
+
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- many rows
+constexpr int kL8M = 256, kL8N = 256;
+// Warps: three issue loads, one the products, 16 run the epilogue, 32 rows and
+// 64 columns each: five for each of the SM's four schedulers.
+constexpr int kL8Producers = 3, kL8MmaWarp = 3, kL8EpiWarps = 16;
+struct L8Smem {
+  static constexpr int THREADS = (kL8Producers + 1 + kL8EpiWarps) * 32;
+  static constexpr int A_BYTES = 128 * kL8BK;          // this CTA's rows of x
+  static constexpr int B_BYTES = kL8N / 2 * kL8BK;     // and its half of the outputs
+  static constexpr int SLOT_BYTES = A_BYTES + B_BYTES;
+  static constexpr int SLOTS = (224 * 1024 - kL8EpiWarps * 4096) / SLOT_BYTES;
+  static constexpr int EPI_OFF = SLOTS * SLOT_BYTES;   // one 4 KB store box per epilogue warp
+  static constexpr int BAR_OFF = EPI_OFF + kL8EpiWarps * 4096;
+  static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 4) * 8 + 16;
+};
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
+    linear8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ CUtensorMap tmY, const __grid_constant__ L8Args p) {
+  using L = L8Smem;
+  constexpr int kSlots = L::SLOTS;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(smem + L::BAR_OFF);  // waited on in the even CTA
+  uint64_t* empty = full + kSlots;
+  uint64_t* acc_full = empty + kSlots;
+  uint64_t* acc_empty = acc_full + 2;               // waited on in the even CTA
+  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+  volatile int* abort = (volatile int*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank();
+  const int tiles_m = (p.M + kL8M - 1) / kL8M, tiles_n = (p.N + kL8N - 1) / kL8N;
+  const int tiles = tiles_m * tiles_n;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kL8EpiWarps);
+    }
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kL8MmaWarp) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before either is signalled
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // `group` blocks of rows go past all outputs before the next ones do
+  auto place = [&](int tile, int& mb, int& nb) {
+    const int first = tile / (p.group * tiles_n) * p.group, wide = min(p.group, tiles_m - first);
+    const int r = tile - first * tiles_n;
+    mb = first + r % wide;
+    nb = r / wide;
+  };
+
+  if (warp < kL8Producers) {
+    // ------------------------------------------------- loads: slot s by warp s % kL8Producers
+    if (lane == 0) {
+      tma_prefetch(&tmX);
+      tma_prefetch(&tmW);
+      uint32_t it = 0;
+      for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
+        int mb, nb;
+        place(tile, mb, nb);
+        const int am = mb * kL8M + rank * 128, bn = nb * kL8N + rank * (kL8N / 2);
+        for (int kb = 0; kb < p.blocks; ++kb, ++it) {
+          const int s = it % kSlots;
+          if (s % kL8Producers != warp) continue;
+          if (!mbar_wait(&empty[s], ((it / kSlots) & 1) ^ 1, abort)) break;
+          uint8_t* sa = smem + s * L::SLOT_BYTES;
+          const uint32_t bar = even_cta_addr(&full[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::SLOT_BYTES);
+          tma_load_3d_pair(sa, &tmX, bar, kb * kL8BK, am, 0);
+          tma_load_3d_pair(sa + L::A_BYTES, &tmW, bar, kb * kL8BK, bn, 0);
+        }
+      }
+    }
+  } else if (warp == kL8MmaWarp) {
+    // ------------------------------------------------- products, by the even CTA for both
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(kL8M, kL8N);
+      const uint64_t a0 = desc_kmajor(smem_u32(smem), 0), b0 = desc_kmajor(smem_u32(smem) + L::A_BYTES, 0);
+      uint32_t it = 0;
+      for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
+        bool ok = true;
+        for (int kb = 0; kb < p.blocks; ++kb, ++it) {
+          const int buf = it & 1, s = it % kSlots;
+          ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort) && mbar_wait(&full[s], (it / kSlots) & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+          uint64_t ad = a0 + (uint32_t)(s * (L::SLOT_BYTES / 16)), bd = b0 + (uint32_t)(s * (L::SLOT_BYTES / 16));
+#pragma unroll
+          for (int kk = 0; kk < kL8BK / 32; ++kk) {
+            mma_e4m3_pair(tmem_base + buf * kL8N, ad, bd, idesc, kk ? 1u : 0u);
+            ad += 2;
+            bd += 2;
+          }
+          mma_commit_pair(&empty[s]);
+          mma_commit_pair(&acc_full[buf]);
+        }
+        if (!ok) break;
+      }
+    }
+  } else {
+    // ------------------------------------------------- epilogue: TMEM lane quarter warp % 4, 64 columns (warp - 4) / 4
+    const int quarter = warp & 3, part = (warp - kL8MmaWarp - 1) >> 2;
+    uint8_t* box = smem + L::EPI_OFF + (warp - kL8MmaWarp - 1) * 4096;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    uint32_t it = 0;
+    for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
+      int mb, nb;
+      place(tile, mb, nb);
+      const int m0 = mb * kL8M + rank * 128 + quarter * 32, m = m0 + lane;
+      const int n0 = nb * kL8N + part * 64;
+      // rows and outputs past the end: zero codes times some scale in range
+      const float* xs = p.xs + (int64_t)min(m, p.M - 1) * p.blocks;
+      const float* ws = p.ws + (int64_t)(min(n0, p.N - 1) / kGroup8) * p.blocks;
+      float v[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) v[j] = 0.f;
+      bool ok = true;
+      float scale = __ldg(xs) * __ldg(ws);
+#pragma unroll 1
+      for (int kb = 0; kb < p.blocks; ++kb, ++it) {
+        const int buf = it & 1, next = min(kb + 1, p.blocks - 1);
+        const float xs_next = __ldg(xs + next), ws_next = __ldg(ws + next);
+        ok = mbar_wait(&acc_full[buf], (it >> 1) & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          float u[16];
+          tmem_ld16(tmem_base + lanes + buf * kL8N + part * 64 + 16 * h, u);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[16 * h + j] = fmaf(u[j], scale, v[16 * h + j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[buf]));
+        scale = xs_next * ws_next;
+      }
+      if (!ok) break;
+      if (n0 >= p.N || m0 >= p.M) continue;
+      if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] += to_f32(((const T*)p.bias)[min(n0 + j, p.N - 1)]);
+      }
+      // through the box: 32 rows of 128 bytes
+      constexpr int kWide = 128 / (int)sizeof(T), E = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int h = 0; h < 64 / kWide; ++h) {
+        if (p.tma_store) {
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          store_vec<E>((T*)(box + lane * 128 + ((q ^ (lane & 7)) * 16)), v + h * kWide + q * E);
+        const int nn = n0 + h * kWide;
+        if (p.tma_store) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && nn < p.N) {
+            tma_store_3d(&tmY, box, nn, m0, 0);
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
+          for (int r = 0; r < 32 && m0 + r < p.M; ++r) {
+            T* row = (T*)p.y + (int64_t)(m0 + r) * p.N;
+#pragma unroll
+            for (int c = 0; c < kWide; c += 32) {
+              const int j = c + lane;
+              if (nn + j < p.N) row[nn + j] = *(const T*)(box + r * 128 + (((j / E) ^ (r & 7)) * 16) + (j % E) * sizeof(T));
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+  __syncthreads();
+  if (warp == kL8MmaWarp && *abort) {
+    // let any MMA still in flight finish before the columns are released
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 10000000ull) {
+    }
+  }
+  cluster_sync();  // neither CTA's shared memory goes while the other may signal it
+  if (warp == kL8MmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ----------------------------------------------------------------- few rows
+// Warps: one issues loads, one the products, four run the epilogue.
+template <int NT>
+struct L8Few {
+  static constexpr int THREADS = 192;
+  static constexpr int W_BYTES = 128 * kL8BK;
+  static constexpr int SLOT_BYTES = W_BYTES + NT * kL8BK;
+  static constexpr int SLOTS = std::min(12, 200 * 1024 / SLOT_BYTES);
+  static constexpr int SCALE_OFF = SLOTS * SLOT_BYTES;  // each epilogue warp's row scales of two K blocks
+  static constexpr int BAR_OFF = SCALE_OFF + 4 * 2 * NT * 4;
+  static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 4) * 8 + 16;
+  static constexpr int COLUMNS = 2 * NT < 32 ? 32 : 2 * NT;  // of TMEM
+  static_assert(SLOTS * SLOT_BYTES >= 128 * NT * 4, "the sums go where the ring was");
+};
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
+    linear8_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                       const __grid_constant__ L8Args p, int splits) {
+  using L = L8Few<NT>;
+  constexpr int kSlots = L::SLOTS;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(smem + L::BAR_OFF);
+  uint64_t* empty = full + kSlots;
+  uint64_t* acc_full = empty + kSlots;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+  volatile int* abort = (volatile int*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
+  // tiles of the same outputs lie together: their weight is read once
+  const int tiles_m = (p.M + NT - 1) / NT;
+  const int m0 = tile % tiles_m * NT, nb = tile / tiles_m, n0 = nb * 128;
+  const int kb0 = (int)((int64_t)p.blocks * rank / splits), kb1 = (int)((int64_t)p.blocks * (rank + 1) / splits);
+
+  if (threadIdx.x == 0) {
+    tma_prefetch(&tmX);
+    tma_prefetch(&tmW);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, L::COLUMNS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  float v[NT];
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+        const int s = it % kSlots;
+        if (!mbar_wait(&empty[s], ((it / kSlots) & 1) ^ 1, abort)) break;
+        uint8_t* sw = smem + s * L::SLOT_BYTES;
+        mbar_arrive_expect_tx(&full[s], L::SLOT_BYTES);
+        tma_load_3d(sw, &tmW, &full[s], kb * kL8BK, n0, 0);
+        tma_load_3d(sw + L::W_BYTES, &tmX, &full[s], kb * kL8BK, m0, 0);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(128, NT);
+      const uint64_t a0 = desc_kmajor(smem_u32(smem), 0), b0 = desc_kmajor(smem_u32(smem) + L::W_BYTES, 0);
+      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+        const int buf = it & 1, s = it % kSlots;
+        if (!mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort) || !mbar_wait(&full[s], (it / kSlots) & 1, abort)) break;
+        tc_fence_after();
+        uint64_t ad = a0 + (uint32_t)(s * (L::SLOT_BYTES / 16)), bd = b0 + (uint32_t)(s * (L::SLOT_BYTES / 16));
+#pragma unroll
+        for (int kk = 0; kk < kL8BK / 32; ++kk) {
+          mma_e4m3(tmem_base + buf * NT, ad, bd, idesc, kk ? 1u : 0u);
+          ad += 2;
+          bd += 2;
+        }
+        mma_commit(&empty[s]);
+        mma_commit(&acc_full[buf]);
+      }
+    }
+  } else {
+    // ------------------------------------------------- epilogue: lane = output, register = row of x
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    float* scales = (float*)(smem + L::SCALE_OFF) + (warp & 3) * 2 * NT;
+    const float* ws = p.ws + (int64_t)nb * p.blocks;
+    constexpr int kPer = (NT + 31) / 32;  // row scales that a lane loads
+    float w_next = 0.f, x_next[kPer];
+    auto fetch = [&](int kb) {
+      w_next = __ldg(ws + kb);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int j = i * 32 + lane;
+        x_next[i] = j < NT && m0 + j < p.M ? __ldg(p.xs + (int64_t)(m0 + j) * p.blocks + kb) : 0.f;
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < NT; ++j) v[j] = 0.f;
+    if (kb0 < kb1) fetch(kb0);
+#pragma unroll 1
+    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+      const int buf = it & 1;
+      float* mine = scales + buf * NT;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i * 32 + lane < NT) mine[i * 32 + lane] = x_next[i] * w_next;
+      if (kb + 1 < kb1) fetch(kb + 1);
+      __syncwarp();
+      if (!mbar_wait(&acc_full[buf], (it >> 1) & 1, abort)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < NT / 16; ++h) {
+        float u[16];
+        tmem_ld16(tmem_base + lanes + buf * NT + 16 * h, u);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(mine + 16 * h + j);
+          v[16 * h + j] = fmaf(u[j], s.x, v[16 * h + j]);
+          v[16 * h + j + 1] = fmaf(u[j + 1], s.y, v[16 * h + j + 1]);
+          v[16 * h + j + 2] = fmaf(u[j + 2], s.z, v[16 * h + j + 2]);
+          v[16 * h + j + 3] = fmaf(u[j + 3], s.w, v[16 * h + j + 3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+    }
+  }
+
+  // ---------------------------------------------------- the splits' sums, and y
+  const int out = (warp & 3) * 32 + lane, n = n0 + out;
+  float* sums = (float*)smem;  // [NT][128]: every load has landed and every product been formed
+  const bool epi = warp >= 2;
+  const float b = epi && p.bias && n < p.N ? to_f32(((const T*)p.bias)[n]) : 0.f;
+  if (splits == 1) {
+    if (epi && n < p.N && !*abort) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        if (m0 + j < p.M) ((T*)p.y)[(int64_t)(m0 + j) * p.N + n] = from_f32<T>(v[j] + b);
+    }
+  } else {
+    const bool gave_up = *abort;
+    if (epi && !gave_up) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        if (m0 + j < p.M) sums[j * 128 + out] = v[j];
+    }
+    cluster_sync();
+    if (epi && !gave_up) {
+      for (int j = rank; j < NT && m0 + j < p.M; j += splits) {
+        float s = 0.f;
+        for (int r = 0; r < splits; ++r) {
+          uint32_t at;
+          float other;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sums + j * 128 + out)), "r"(r));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(at) : "memory");
+          s += other;
+        }
+        if (n < p.N) ((T*)p.y)[(int64_t)(m0 + j) * p.N + n] = from_f32<T>(s + b);
+      }
+    }
+    cluster_sync();  // no block leaves while its sums are read
+  }
+  __syncthreads();
+  if (warp == 1) {
+    if (*abort) {
+      const uint64_t t0 = globaltimer();
+      while (globaltimer() - t0 < 10000000ull) {
+      }
+    }
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::COLUMNS);
+  }
+}
+
+// --------------------------------------------------------------- host side
+static int64_t l8_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static int l8_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld_bytes, int box_cols, int box_rows,
+                  CUtensorMapDataType type) {
+  uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, 1};
+  uint64_t str[2] = {(uint64_t)ld_bytes, (uint64_t)ld_bytes * rows};
+  uint32_t box[3] = {(uint32_t)box_cols, (uint32_t)box_rows, 1};
+  return encode_tiled(m, 3, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, nullptr, type);
+}
+static int l8_codes(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
+  // (one row: its stride counts for nothing, but has to be one)
+  return l8_map(m, base, K, rows, rows == 1 ? l8_div(K, 16) * 16 : ld, kL8BK, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8);
+}
+
+template <typename T>
+static int l8_many(const pvb2_linear8_desc* d, const void* x, const void* w, L8Args p, cudaStream_t s) {
+  constexpr int smem = L8Smem::TOTAL + 1024;
+  static DeviceOnce once;
+  PVB2_TRY(allow_smem(linear8_kernel<T>, smem, once));
+  CUtensorMap mx, mw, my;
+  PVB2_TRY(l8_codes(&mx, x, d->K, d->M, d->ldx, 128));
+  PVB2_TRY(l8_codes(&mw, w, d->K, d->N, d->ldw, kL8N / 2));
+  p.tma_store = ((uintptr_t)p.y & 15) == 0 && d->N * (int64_t)sizeof(T) % 16 == 0;
+  memset(&my, 0, sizeof(my));
+  if (p.tma_store)
+    PVB2_TRY(l8_map(&my, p.y, d->N, d->M, d->N * sizeof(T), 128 / (int)sizeof(T), 32,
+                    sizeof(T) == 4                              ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                    : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16));
+  const int64_t tiles = l8_div(d->M, kL8M) * l8_div(d->N, kL8N);
+  // blocks of rows that stay in L2 (32 MB of its 126) while the outputs go by
+  p.group = (int)std::max<int64_t>(8, std::min<int64_t>(l8_div(d->M, kL8M), ((int64_t)32 << 20) / (kL8M * d->K)));
+  const int grid = 2 * (int)std::min<int64_t>(tiles, std::max(1, num_sms() / 2));
+  linear8_kernel<T><<<grid, L8Smem::THREADS, smem, s>>>(mx, mw, my, p);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+template <typename T, int NT>
+static int l8_few(const pvb2_linear8_desc* d, const void* x, const void* w, const L8Args& p, int splits, cudaStream_t s) {
+  constexpr int smem = L8Few<NT>::TOTAL + 1024;
+  static DeviceOnce once;
+  PVB2_TRY(allow_smem(linear8_few_kernel<T, NT>, smem, once));
+  CUtensorMap mx, mw;
+  PVB2_TRY(l8_codes(&mx, x, d->K, d->M, d->ldx, NT));
+  PVB2_TRY(l8_codes(&mw, w, d->K, d->N, d->ldw, 128));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(l8_div(d->N, 128) * l8_div(d->M, NT) * splits));
+  cfg.blockDim = dim3(L8Few<NT>::THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PVB2_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear8_few_kernel<T, NT>, mx, mw, p, splits));
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+// CTAs of a cluster that share K: as many as have an SM, two K blocks each at least
+static int l8_splits(int64_t tiles, int64_t blocks) {
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= num_sms() && blocks >= 4 * splits) splits *= 2;
+  return splits;
+}
+
+template <typename T>
+static int l8_run(const pvb2_linear8_desc* d, const void* x, const void* w, const L8Args& p, cudaStream_t s) {
+  const int nt = d->M <= 16 ? 16 : d->M <= 32 ? 32 : d->M <= 64 ? 64 : 128;
+  const int64_t few = l8_div(d->N, 128) * l8_div(d->M, nt);
+  // pairs once they have half the device's SMs at least
+  if (d->M > 128 && l8_div(d->M, kL8M) * l8_div(d->N, kL8N) * 4 >= num_sms()) return l8_many<T>(d, x, w, p, s);
+  const int splits = l8_splits(few, p.blocks);
+  if (nt == 16) return l8_few<T, 16>(d, x, w, p, splits, s);
+  if (nt == 32) return l8_few<T, 32>(d, x, w, p, splits, s);
+  if (nt == 64) return l8_few<T, 64>(d, x, w, p, splits, s);
+  return l8_few<T, 128>(d, x, w, p, splits, s);
+}
+
+}  // namespace pvb2
+
+using namespace pvb2;
+
+extern "C" {
+
+int pvb2_linear8(const pvb2_linear8_desc* d, const uint8_t* x, const float* x_scales, const uint8_t* w,
+                 const float* w_scales, const void* bias, void* y, pvb2_stream stream) {
+  PVB2_CHECK_ARG(d, "linear_8bit: no descriptor");
+  PVB2_CHECK_ARG(d->dtype == PVB2_F32 || d->dtype == PVB2_F16 || d->dtype == PVB2_BF16,
+                 "linear_8bit: an output in fp32, fp16 or bf16 expected (got dtype %d)", d->dtype);
+  const int64_t most = (int64_t)1 << 30;
+  PVB2_CHECK_ARG(d->M >= 0 && d->M < most && d->N >= 0 && d->N < most && d->K >= 1 && d->K < most,
+                 "linear_8bit: %lld rows, %lld outputs of %lld inputs out of range", (long long)d->M, (long long)d->N,
+                 (long long)d->K);
+  PVB2_CHECK_ARG(l8_div(d->M, 16) * l8_div(d->N, 128) < ((int64_t)1 << 27), "linear_8bit: more outputs than one launch has tiles for");
+  if (d->M == 0 || d->N == 0) return PVB2_OK;
+  PVB2_CHECK_ARG(x && x_scales && w && w_scales && y, "linear_8bit: null pointer");
+  PVB2_CHECK_ARG((d->M == 1 || d->ldx >= d->K) && (d->N == 1 || d->ldw >= d->K), "linear_8bit: row strides below the inputs");
+  PVB2_CHECK_ARG(((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && (d->M == 1 || d->ldx % 16 == 0) &&
+                     (d->N == 1 || d->ldw % 16 == 0),
+                 "linear_8bit: rows of codes have to begin on 16-byte boundaries");
+  L8Args p = {};
+  p.xs = x_scales;
+  p.ws = w_scales;
+  p.bias = bias;
+  p.y = y;
+  p.M = (int)d->M;
+  p.N = (int)d->N;
+  p.blocks = (int)l8_div(d->K, kL8BK);
+  cudaStream_t s = as_stream(stream);
+  if (d->dtype == PVB2_F32) return l8_run<float>(d, x, w, p, s);
+  if (d->dtype == PVB2_BF16) return l8_run<__nv_bfloat16>(d, x, w, p, s);
+  return l8_run<__half>(d, x, w, p, s);
+}
+
+int pvb2_linear8_status(int* timed_out, int reset) { return tc_timeout_flag_local(timed_out, reset); }
+
+}  // extern "C"

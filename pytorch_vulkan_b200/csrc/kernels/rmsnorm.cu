@@ -1,0 +1,723 @@
+// Root-mean-square norm of rows, with the residual's addition before it and
+// 8-bit codes with scales after it, its gradients, and the codes of plain rows
+// and weights.
+//
+//   h = x + r, rounded to the type (the residual stream as it goes on)
+//   rstd = 1 / sqrt(mean(h^2) + eps);   n = h rstd;   y = n w
+//   backward, with a = gy w:  dh = rstd (a - n mean(a n)) + gh;   dw = sum over rows of gy n
+//
+// One pass over the data: a row's elements stay in the registers of the
+// threads that share it (a warp up to 1024 16-bit elements, a block of up to
+// 1024 threads beyond) between the sum and the output, so every kernel here is
+// bound by HBM.  Longer rows are read twice, the second time out of L2.
+//
+// The mean of squares is summed in 64 bits and rounded once, root and quotient
+// are the IEEE ones, and n and y are rounded products: a code of the 8-bit
+// output changes where y moves across the border of two codes, so that y must
+// not depend on the order of a sum.  (The conversions to 64 bits cost nothing
+// beside the loads: a square is converted for 4 to 8 bytes of traffic.)
+//
+// Elements go to threads in chunks of 16 bytes; where rows do not begin on
+// 16-byte boundaries, in chunks of four that lie 32 elements apart, so that a
+// warp still reads consecutive ones and 128 of them, a group of one scale, are
+// a warp's.
+#include <algorithm>
+#include "quant8.cuh"
+
+namespace pvb2 {
+
+enum { kNorm = 0, kNorm8 = 1, kQuant8 = 2 };
+
+struct NormArgs {
+  const void* x;
+  const void* r;   // residual, or null
+  const void* w;   // or null: ones
+  void* y;         // kNorm
+  void* sum;       // with a residual
+  float* rstd;     // or null
+  uint8_t* codes;  // kNorm8, kQuant8
+  float* scales;
+  int64_t rows, ldx, ldr, ldc;
+  int D, groups;
+  float eps;
+};
+
+struct NormBwdArgs {
+  const void* h;
+  const void* w;
+  const float* rstd;
+  const void* gy;
+  const void* gh;   // or null
+  void* dx;         // or null
+  float* partial;   // [blocks][D], or null
+  int64_t rows, ldh, ldg, ldgh;
+  int D;
+};
+
+// E elements of a chunk: consecutive (VEC), or 32 apart
+template <typename T, bool VEC>
+struct Chunk {
+  static constexpr int E = VEC ? 16 / (int)sizeof(T) : 4;
+  // first element of chunk c, and the step to the next
+  static __device__ __forceinline__ int64_t at(int c) { return VEC ? (int64_t)c * E : (int64_t)(c >> 5) * 128 + (c & 31); }
+  static constexpr int kStep = VEC ? 1 : 32;
+
+  T e[E];
+  __device__ __forceinline__ void load(const T* row, int c, int D) {
+    const int64_t i = at(c);
+    if (VEC) {
+      if (i < D) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(row + i);
+      else *reinterpret_cast<uint4*>(e) = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < E; ++k) e[k] = i + k * kStep < D ? row[i + k * kStep] : from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int c, int D) const {
+    const int64_t i = at(c);
+    if (VEC) {
+      if (i < D) *reinterpret_cast<uint4*>(row + i) = *reinterpret_cast<const uint4*>(e);
+    } else {
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (i + k * kStep < D) row[i + k * kStep] = e[k];
+    }
+  }
+};
+// (16-byte accesses to its elements)
+template <typename T, bool VEC>
+struct alignas(16) AChunk : Chunk<T, VEC> {};
+
+// Sum over the G threads of a row, in a fixed order; all of them get it.
+// `line`: one number per warp of the block.
+template <int G, typename A>
+__device__ __forceinline__ A row_sum(A v, A* line) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  if (G > 32) {
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();  // the last sum has been read
+    if ((threadIdx.x & 31) == 0) line[warp] = v;
+    __syncthreads();
+    v = line[0];
+#pragma unroll
+    for (int i = 1; i < G / 32; ++i) v += line[i];
+  }
+  return v;
+}
+
+__device__ __forceinline__ float rstd_of(double squares, int D, float eps) {
+  return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn((float)(squares / (double)D), eps)));
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void scale_row(const AChunk<T, VEC>& h, const T* w, int c, int D, float rstd, float* y) {
+  constexpr int E = Chunk<T, VEC>::E;
+  AChunk<T, VEC> cw;
+  if (w) cw.load(w, c, D);
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    y[k] = __fmul_rn(to_f32(h.e[k]), rstd);
+    if (w) y[k] = __fmul_rn(y[k], to_f32(cw.e[k]));
+  }
+}
+
+// the group's scale and this chunk's codes
+template <typename T, bool VEC>
+__device__ __forceinline__ void put_codes(const float* y, uint8_t* row, float* scales, int c, int D) {
+  constexpr int E = Chunk<T, VEC>::E;
+  constexpr int kLanes = VEC ? kGroup8 / E : 32;  // that share a group
+  const int64_t i = Chunk<T, VEC>::at(c);
+  uint32_t most = 0;
+#pragma unroll
+  for (int k = 0; k < E; ++k) most = max(most, abs_bits(y[k]));
+#pragma unroll
+  for (int o = kLanes / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(~0u, most, o));
+  const Scale8 s = scale8(most);
+  const int64_t group = i / kGroup8;
+  if ((c & (kLanes - 1)) == 0 && i < D) scales[group] = s.scale;
+  float q[E];
+#pragma unroll
+  for (int k = 0; k < E; ++k) q[k] = __fmul_rn(y[k], s.inv);
+  if (VEC) {
+    if (i < D) {
+      if (E == 8) {
+        *reinterpret_cast<uint2*>(row + i) =
+            make_uint2(codes4(q[0], q[1], q[2], q[3]), codes4(q[E - 4], q[E - 3], q[E - 2], q[E - 1]));
+      } else {
+        *reinterpret_cast<uint32_t*>(row + i) = codes4(q[0], q[1], q[2], q[3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+      if (i + 32 * k < D) row[i + 32 * k] = (uint8_t)codes2(q[k], 0.f);
+  }
+}
+
+// h of a chunk, stored where there is a residual
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_sum(const NormArgs& a, int64_t row, int c, AChunk<T, VEC>& h) {
+  h.load((const T*)a.x + row * a.ldx, c, a.D);
+  if (a.r) {
+    AChunk<T, VEC> r;
+    r.load((const T*)a.r + row * a.ldr, c, a.D);
+#pragma unroll
+    for (int k = 0; k < Chunk<T, VEC>::E; ++k) h.e[k] = from_f32<T>(to_f32(h.e[k]) + to_f32(r.e[k]));
+    h.store((T*)a.sum + row * a.D, c, a.D);
+  }
+}
+
+// G threads share a row and keep NV chunks each; blocks of max(G, 128)
+template <typename T, bool VEC, int G, int NV, int MODE>
+__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_kernel(NormArgs a) {
+  using C = Chunk<T, VEC>;
+  __shared__ double line[G / 32];
+  const int t = threadIdx.x % G;
+  const int64_t row = (int64_t)blockIdx.x * (G < 128 ? 128 / G : 1) + threadIdx.x / G;
+  if (row >= a.rows) return;  // whole warps: only where a warp has a row of its own
+  AChunk<T, VEC> h[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) load_sum(a, row, i * G + t, h[i]);
+  float rstd = 1.f;
+  if (MODE != kQuant8) {
+    double q = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) {
+        const double v = to_f32(h[i].e[k]);
+        q = fma(v, v, q);
+      }
+    rstd = rstd_of(row_sum<G>(q, line), a.D, a.eps);
+    if (a.rstd && t == 0) a.rstd[row] = rstd;
+  }
+  const T* w = MODE == kQuant8 ? nullptr : (const T*)a.w;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = i * G + t;
+    float y[C::E];
+    if (MODE == kQuant8) {
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) y[k] = to_f32(h[i].e[k]);
+    } else {
+      scale_row<T, VEC>(h[i], w, c, a.D, rstd, y);
+    }
+    if (MODE == kNorm) {
+      AChunk<T, VEC> out;
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) out.e[k] = from_f32<T>(y[k]);
+      out.store((T*)a.y + row * a.D, c, a.D);
+    } else {
+      put_codes<T, VEC>(y, a.codes + row * a.ldc, a.scales + row * a.groups, c, a.D);
+    }
+  }
+}
+
+// rows that outgrow the registers: read again for the output
+template <typename T, bool VEC, int MODE>
+__global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
+  using C = Chunk<T, VEC>;
+  __shared__ double line[32];
+  const int64_t row = blockIdx.x;
+  // whole warps stay together: a group's lanes meet
+  const int chunks = (a.D + C::E * 32 - 1) / (C::E * 32) * 32;
+  float rstd = 1.f;
+  if (MODE != kQuant8) {
+    double q = 0;
+    for (int c = threadIdx.x; c < chunks; c += 1024) {
+      AChunk<T, VEC> h;
+      load_sum(a, row, c, h);
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) {
+        const double v = to_f32(h.e[k]);
+        q = fma(v, v, q);
+      }
+    }
+    rstd = rstd_of(row_sum<1024>(q, line), a.D, a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+  }
+  // the sum that this thread wrote, or x
+  const T* src = a.r ? (const T*)a.sum + row * a.D : (const T*)a.x + row * a.ldx;
+  for (int c = threadIdx.x; c < chunks; c += 1024) {
+    AChunk<T, VEC> h;
+    h.load(src, c, a.D);
+    float y[C::E];
+    if (MODE == kQuant8) {
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) y[k] = to_f32(h.e[k]);
+    } else {
+      scale_row<T, VEC>(h, (const T*)a.w, c, a.D, rstd, y);
+    }
+    if (MODE == kNorm) {
+      AChunk<T, VEC> out;
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) out.e[k] = from_f32<T>(y[k]);
+      out.store((T*)a.y + row * a.D, c, a.D);
+    } else {
+      put_codes<T, VEC>(y, a.codes + row * a.ldc, a.scales + row * a.groups, c, a.D);
+    }
+  }
+}
+
+// ------------------------------------------------------------- backward
+// A block walks rows and keeps its share of dw in registers: gy and h are read
+// once for both gradients.  The blocks' shares are summed by a second launch,
+// in a fixed order.
+template <typename T, bool VEC, int G, int NV>
+__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(NormBwdArgs a) {
+  using C = Chunk<T, VEC>;
+  constexpr int kRows = G < 128 ? 128 / G : 1;  // of a block
+  __shared__ float line[G / 32];
+  extern __shared__ float share[];  // kRows > 1: dw of the rows' warps
+  const int t = threadIdx.x % G, mine = threadIdx.x / G;
+  AChunk<T, VEC> w[NV];
+  float dw[NV][C::E];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (a.w) w[i].load((const T*)a.w, i * G + t, a.D);
+#pragma unroll
+    for (int k = 0; k < C::E; ++k) {
+      dw[i][k] = 0.f;
+      if (!a.w) w[i].e[k] = from_f32<T>(1.f);
+    }
+  }
+  for (int64_t row = (int64_t)blockIdx.x * kRows + mine; row < a.rows; row += (int64_t)gridDim.x * kRows) {
+    AChunk<T, VEC> h[NV], g[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      h[i].load((const T*)a.h + row * a.ldh, i * G + t, a.D);
+      g[i].load((const T*)a.gy + row * a.ldg, i * G + t, a.D);
+    }
+    const float rstd = a.rstd[row];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) {
+        const float n = to_f32(h[i].e[k]) * rstd, gv = to_f32(g[i].e[k]);
+        dot = fmaf(gv * to_f32(w[i].e[k]), n, dot);
+        dw[i][k] = fmaf(gv, n, dw[i][k]);
+      }
+    if (!a.dx) continue;
+    const float mean = row_sum<G>(dot, line) / (float)a.D;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * G + t;
+      AChunk<T, VEC> gh, out;
+      if (a.gh) gh.load((const T*)a.gh + row * a.ldgh, c, a.D);
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) {
+        const float n = to_f32(h[i].e[k]) * rstd;
+        float d = fmaf(-n, mean, to_f32(g[i].e[k]) * to_f32(w[i].e[k])) * rstd;
+        if (a.gh) d += to_f32(gh.e[k]);
+        out.e[k] = from_f32<T>(d);
+      }
+      out.store((T*)a.dx + row * a.D, c, a.D);
+    }
+  }
+  if (!a.partial) return;
+  if (kRows > 1) {
+    // (NV * G * E numbers for each row's warp)
+    constexpr int kWide = NV * G * C::E;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) share[mine * kWide + (int)C::at(i * G + t) + k * C::kStep] = dw[i][k];
+    __syncthreads();
+    for (int j = threadIdx.x; j < a.D; j += 128) {
+      float s = share[j];
+#pragma unroll
+      for (int m = 1; m < kRows; ++m) s += share[m * kWide + j];
+      a.partial[(int64_t)blockIdx.x * a.D + j] = s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) {
+        const int64_t j = C::at(i * G + t) + k * C::kStep;
+        if (j < a.D) a.partial[(int64_t)blockIdx.x * a.D + j] = dw[i][k];
+      }
+  }
+}
+
+// long rows: dh alone, and the shares of dw by columns
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
+  using C = Chunk<T, VEC>;
+  __shared__ float line[32];
+  const int64_t row = blockIdx.x;
+  const int chunks = (a.D + C::E * 32 - 1) / (C::E * 32) * 32;
+  const float rstd = a.rstd[row];
+  float dot = 0.f, mean = 0.f;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int c = threadIdx.x; c < chunks; c += 1024) {
+      AChunk<T, VEC> h, g, w, gh, out;
+      h.load((const T*)a.h + row * a.ldh, c, a.D);
+      g.load((const T*)a.gy + row * a.ldg, c, a.D);
+      if (a.w) w.load((const T*)a.w, c, a.D);
+      if (pass && a.gh) gh.load((const T*)a.gh + row * a.ldgh, c, a.D);
+#pragma unroll
+      for (int k = 0; k < C::E; ++k) {
+        const float n = to_f32(h.e[k]) * rstd, v = to_f32(g.e[k]) * (a.w ? to_f32(w.e[k]) : 1.f);
+        if (!pass) {
+          dot = fmaf(v, n, dot);
+        } else {
+          float d = fmaf(-n, mean, v) * rstd;
+          if (a.gh) d += to_f32(gh.e[k]);
+          out.e[k] = from_f32<T>(d);
+        }
+      }
+      if (pass) out.store((T*)a.dx + row * a.D, c, a.D);
+    }
+    if (!pass) mean = row_sum<1024>(dot, line) / (float)a.D;
+  }
+}
+
+// rows blockIdx.y, blockIdx.y + gridDim.y, ... of 256 columns
+template <typename T>
+__global__ void __launch_bounds__(256) norm_dw_columns_kernel(NormBwdArgs a) {
+  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (j >= a.D) return;
+  float s = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y)
+    s = fmaf(to_f32(((const T*)a.gy)[row * a.ldg + j]), to_f32(((const T*)a.h)[row * a.ldh + j]) * a.rstd[row], s);
+  a.partial[(int64_t)blockIdx.y * a.D + j] = s;
+}
+
+// dw[j] = sum of the shares, 32 columns a block, in a fixed order
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_dw_sum_kernel(const float* partial, int count, int D, T* dw) {
+  __shared__ float part[32][33];
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (j < D)
+    for (int p = y; p < count; p += 32) s += partial[(int64_t)p * D + j];
+  part[y][lane] = s;
+  __syncthreads();
+  s = part[lane][y];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  const int64_t jj = (int64_t)blockIdx.x * 32 + y;
+  if (lane == 0 && jj < D) dw[jj] = from_f32<T>(s);
+}
+
+// ------------------------------------------- codes of weights, and values
+// 128 x 128 elements with one scale; a warp reads 4 x 32 of a row at a time
+template <typename T>
+__global__ void __launch_bounds__(256) quant_tile_kernel(const T* x, int64_t rows, int64_t D, int64_t ldx, uint8_t* codes,
+                                                         int64_t ldc, float* scales, int64_t groups) {
+  __shared__ uint32_t most_of[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
+  float v[16][4];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t r = r0 + i * 8 + warp, c = c0 + k * 32 + lane;
+      v[i][k] = r < rows && c < D ? to_f32(x[r * ldx + c]) : 0.f;
+      most = max(most, abs_bits(v[i][k]));
+    }
+  most = __reduce_max_sync(~0u, most);
+  if (lane == 0) most_of[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, most_of[i]);
+  const Scale8 s = scale8(most);
+  if (threadIdx.x == 0) scales[blockIdx.y * groups + blockIdx.x] = s.scale;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t r = r0 + i * 8 + warp, c = c0 + k * 32 + lane;
+      if (r < rows && c < D) codes[r * ldc + c] = (uint8_t)codes2(__fmul_rn(v[i][k], s.inv), 0.f);
+    }
+}
+
+// values of codes: 8 consecutive ones a thread (VEC), or one
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* codes, const float* scales, T* out, int64_t rows, int D,
+                                                      int64_t ldc, int groups, int tall) {
+  constexpr int E = VEC ? 8 : 1;
+  const int wide = (D + E - 1) / E;
+  const int64_t total = rows * wide;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / wide;
+    const int c = (int)(i - row * wide) * E;
+    const float s = scales[(tall ? row / 128 : row) * groups + c / kGroup8];
+    if (VEC) {
+      const uint2 q = *reinterpret_cast<const uint2*>(codes + row * ldc + c);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 p = values2((k < 2 ? q.x : q.y) >> (16 * (k & 1)));
+        v[2 * k] = p.x * s;
+        v[2 * k + 1] = p.y * s;
+      }
+      store_vec<8>(out + row * D + c, v);
+    } else {
+      out[row * D + c] = from_f32<T>(values2(codes[row * ldc + c]).x * s);
+    }
+  }
+}
+
+// --------------------------------------------------------------- host side
+static bool on16(const void* p, int64_t ld, int size, int64_t rows) {
+  return ((uintptr_t)p & 15) == 0 && (rows <= 1 || ld * size % 16 == 0);
+}
+
+constexpr int64_t kNormMostRows = (int64_t)1 << 31;
+
+static int norm_check(const char* op, const pvb2_rms_norm_desc* d) {
+  PVB2_CHECK_ARG(d, "%s: no descriptor", op);
+  PVB2_CHECK_ARG(d->dtype == PVB2_F32 || d->dtype == PVB2_F16 || d->dtype == PVB2_BF16,
+                 "%s: fp32, fp16 or bf16 expected (got dtype %d)", op, d->dtype);
+  PVB2_CHECK_ARG(d->rows >= 0 && d->rows < kNormMostRows && d->D >= 0 && d->D <= (1 << 24), "%s: %lld rows of %lld out of range",
+                 op, (long long)d->rows, (long long)d->D);
+  PVB2_CHECK_ARG(d->eps >= 0 && d->eps <= 3e38, "%s: eps has to be finite and not below 0", op);
+  return PVB2_OK;
+}
+
+static int norm_strides(const char* op, const pvb2_rms_norm_desc* d, std::initializer_list<int64_t> lds) {
+  for (int64_t ld : lds)
+    PVB2_CHECK_ARG(d->rows <= 1 || ld >= d->D, "%s: row strides below the rows' length", op);
+  return PVB2_OK;
+}
+
+template <typename T, bool VEC, int MODE>
+static int launch_norm(const NormArgs& a, cudaStream_t s) {
+  const int chunks = (a.D + Chunk<T, VEC>::E - 1) / Chunk<T, VEC>::E;
+  const unsigned rows = (unsigned)a.rows;
+  // as few threads a row as keep it in four chunks each: a warp needs no barrier
+  if (chunks <= 32) norm_kernel<T, VEC, 32, 1, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
+  else if (chunks <= 64) norm_kernel<T, VEC, 32, 2, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
+  else if (chunks <= 128) norm_kernel<T, VEC, 32, 4, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
+  else if (chunks <= 256) norm_kernel<T, VEC, 128, 2, MODE><<<rows, 128, 0, s>>>(a);
+  else if (chunks <= 512) norm_kernel<T, VEC, 128, 4, MODE><<<rows, 128, 0, s>>>(a);
+  else if (chunks <= 1024) norm_kernel<T, VEC, 256, 4, MODE><<<rows, 256, 0, s>>>(a);
+  else if (chunks <= 2048) norm_kernel<T, VEC, 512, 4, MODE><<<rows, 512, 0, s>>>(a);
+  else if (chunks <= 4096) norm_kernel<T, VEC, 1024, 4, MODE><<<rows, 1024, 0, s>>>(a);
+  else norm_long_kernel<T, VEC, MODE><<<rows, 1024, 0, s>>>(a);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+template <int MODE>
+static int run_norm(const NormArgs& a, int dtype, bool vec, cudaStream_t s) {
+  if (dtype == PVB2_F32) return vec ? launch_norm<float, true, MODE>(a, s) : launch_norm<float, false, MODE>(a, s);
+  if (dtype == PVB2_BF16)
+    return vec ? launch_norm<__nv_bfloat16, true, MODE>(a, s) : launch_norm<__nv_bfloat16, false, MODE>(a, s);
+  return vec ? launch_norm<__half, true, MODE>(a, s) : launch_norm<__half, false, MODE>(a, s);
+}
+
+static NormArgs norm_args(const pvb2_rms_norm_desc* d, const void* x, const void* r, const void* w, void* sum) {
+  NormArgs a = {};
+  a.x = x;
+  a.r = r;
+  a.w = w;
+  a.sum = sum;
+  a.rows = d->rows;
+  a.ldx = d->ldx;
+  a.ldr = d->ldr;
+  a.ldc = d->ldc;
+  a.D = (int)d->D;
+  a.groups = (int)((d->D + kGroup8 - 1) / kGroup8);
+  a.eps = (float)d->eps;
+  return a;
+}
+
+static bool norm_vec(const NormArgs& a, int dtype) {
+  const int size = dtype_size(dtype);
+  return (int64_t)a.D * size % 16 == 0 && on16(a.x, a.ldx, size, a.rows) && (!a.r || on16(a.r, a.ldr, size, a.rows)) &&
+         (!a.w || on16(a.w, 0, size, 1)) && (!a.y || on16(a.y, a.D, size, a.rows)) &&
+         (!a.sum || on16(a.sum, a.D, size, a.rows)) &&
+         (!a.codes || (((uintptr_t)a.codes & 7) == 0 && (a.rows <= 1 || a.ldc % 8 == 0)));
+}
+
+// blocks of the backward pass that keep a share of dw: two full SMs' worth of
+// threads each, and 16 rows a block at least, so that the shares are few
+// beside the rows
+struct NormBwdPlan {
+  int threads, rows_per_block;  // threads of a row (0: long rows)
+  int64_t blocks;
+};
+static NormBwdPlan bwd_plan(const pvb2_rms_norm_desc* d, bool vec) {
+  const int size = dtype_size(d->dtype);
+  const int E = vec ? 16 / size : 4;
+  const int64_t chunks = (d->D + E - 1) / E;
+  NormBwdPlan p = {};
+  p.threads = chunks <= 64 ? 32 : chunks <= 256 ? 128 : chunks <= 512 ? 256 : chunks <= 1024 ? 512 : chunks <= 2048 ? 1024 : 0;
+  p.rows_per_block = p.threads == 32 ? 4 : 1;
+  const int64_t most = (int64_t)num_sms() * (p.threads == 0 ? 1 : p.threads <= 128 ? 8 : 1024 / p.threads);
+  const int64_t want = (d->rows + p.rows_per_block - 1) / p.rows_per_block;
+  p.blocks = std::max<int64_t>(1, std::min(want, most));
+  return p;
+}
+
+template <typename T, bool VEC>
+static int launch_bwd(const NormBwdArgs& a, const NormBwdPlan& p, cudaStream_t s) {
+  constexpr int E = Chunk<T, VEC>::E;
+  const int chunks = (a.D + E - 1) / E;
+  const unsigned grid = (unsigned)p.blocks;
+  if (chunks <= 32) norm_bwd_kernel<T, VEC, 32, 1><<<grid, 128, 4 * 32 * E * 4, s>>>(a);
+  else if (chunks <= 64) norm_bwd_kernel<T, VEC, 32, 2><<<grid, 128, 4 * 64 * E * 4, s>>>(a);
+  else if (chunks <= 128) norm_bwd_kernel<T, VEC, 128, 1><<<grid, 128, 0, s>>>(a);
+  else if (chunks <= 256) norm_bwd_kernel<T, VEC, 128, 2><<<grid, 128, 0, s>>>(a);
+  else if (chunks <= 512) norm_bwd_kernel<T, VEC, 256, 2><<<grid, 256, 0, s>>>(a);
+  else if (chunks <= 1024) norm_bwd_kernel<T, VEC, 512, 2><<<grid, 512, 0, s>>>(a);
+  else if (chunks <= 2048) norm_bwd_kernel<T, VEC, 1024, 2><<<grid, 1024, 0, s>>>(a);
+  else {
+    if (a.dx) {
+      norm_bwd_long_kernel<T, VEC><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+      PVB2_LAUNCH_CHECK();
+    }
+    if (!a.partial) return PVB2_OK;
+    norm_dw_columns_kernel<T><<<dim3((unsigned)((a.D + 255) / 256), grid), 256, 0, s>>>(a);
+  }
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+template <typename T>
+static int run_bwd(const NormBwdArgs& a, const NormBwdPlan& p, bool vec, void* dw, cudaStream_t s) {
+  if (a.rows) PVB2_TRY((vec ? launch_bwd<T, true>(a, p, s) : launch_bwd<T, false>(a, p, s)));
+  if (!dw) return PVB2_OK;
+  norm_dw_sum_kernel<T><<<(unsigned)((a.D + 31) / 32), 1024, 0, s>>>(a.partial, a.rows ? (int)p.blocks : 0, a.D, (T*)dw);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+}  // namespace pvb2
+
+using namespace pvb2;
+
+extern "C" {
+
+int pvb2_rms_norm_fwd(const pvb2_rms_norm_desc* d, const void* x, const void* residual, const void* weight, void* y,
+                      void* sum, float* rstd, pvb2_stream stream) {
+  PVB2_TRY(norm_check("rms_norm", d));
+  if (d->rows == 0 || d->D == 0) return PVB2_OK;
+  PVB2_CHECK_ARG(x && y && (!residual || sum), "rms_norm: null pointer");
+  PVB2_TRY(norm_strides("rms_norm", d, {d->ldx, residual ? d->ldr : d->D}));
+  NormArgs a = norm_args(d, x, residual, weight, residual ? sum : nullptr);
+  a.y = y;
+  a.rstd = rstd;
+  return run_norm<kNorm>(a, d->dtype, norm_vec(a, d->dtype), as_stream(stream));
+}
+
+int pvb2_rms_norm_8bit(const pvb2_rms_norm_desc* d, const void* x, const void* residual, const void* weight,
+                       uint8_t* codes, float* scales, void* sum, pvb2_stream stream) {
+  PVB2_TRY(norm_check("rms_norm_8bit", d));
+  if (d->rows == 0 || d->D == 0) return PVB2_OK;
+  PVB2_CHECK_ARG(x && codes && scales && (!residual || sum), "rms_norm_8bit: null pointer");
+  PVB2_TRY(norm_strides("rms_norm_8bit", d, {d->ldx, residual ? d->ldr : d->D, d->ldc}));
+  NormArgs a = norm_args(d, x, residual, weight, residual ? sum : nullptr);
+  a.codes = codes;
+  a.scales = scales;
+  return run_norm<kNorm8>(a, d->dtype, norm_vec(a, d->dtype), as_stream(stream));
+}
+
+size_t pvb2_rms_norm_bwd_workspace_size(const pvb2_rms_norm_desc* d) {
+  if (norm_check("rms_norm", d) != PVB2_OK) return 0;
+  // (rows without 16-byte boundaries may have more blocks)
+  return (size_t)std::max(bwd_plan(d, true).blocks, bwd_plan(d, false).blocks) * d->D * 4;
+}
+
+int pvb2_rms_norm_bwd(const pvb2_rms_norm_desc* d, const void* h, const void* weight, const float* rstd, const void* gy,
+                      const void* gsum, void* dx, void* dw, void* workspace, size_t workspace_bytes, pvb2_stream stream) {
+  PVB2_TRY(norm_check("rms_norm_bwd", d));
+  if (d->D == 0 || (!dx && !dw) || (d->rows == 0 && !dw)) return PVB2_OK;
+  if (d->rows) {
+    PVB2_CHECK_ARG(h && rstd && gy, "rms_norm_bwd: null pointer");
+    PVB2_TRY(norm_strides("rms_norm_bwd", d, {d->ldx, d->ldg, gsum ? d->ldr : d->D}));
+  }
+  PVB2_CHECK_ARG(!dw || (workspace && ((uintptr_t)workspace & 3) == 0 &&
+                         workspace_bytes >= pvb2_rms_norm_bwd_workspace_size(d)),
+                 "rms_norm_bwd: workspace of %zu bytes needed", pvb2_rms_norm_bwd_workspace_size(d));
+  NormBwdArgs a = {};
+  a.h = h;
+  a.w = weight;
+  a.rstd = rstd;
+  a.gy = gy;
+  a.gh = gsum;
+  a.dx = dx;
+  a.partial = dw ? (float*)workspace : nullptr;
+  a.rows = d->rows;
+  a.ldh = d->ldx;
+  a.ldg = d->ldg;
+  a.ldgh = d->ldr;
+  a.D = (int)d->D;
+  const int size = dtype_size(d->dtype);
+  const bool vec = (int64_t)a.D * size % 16 == 0 && on16(h, a.ldh, size, a.rows) && on16(gy, a.ldg, size, a.rows) &&
+                   (!gsum || on16(gsum, a.ldgh, size, a.rows)) && (!weight || on16(weight, 0, size, 1)) &&
+                   (!dx || on16(dx, a.D, size, a.rows));
+  const NormBwdPlan p = bwd_plan(d, vec);
+  cudaStream_t s = as_stream(stream);
+  if (d->dtype == PVB2_F32) return run_bwd<float>(a, p, vec, dw, s);
+  if (d->dtype == PVB2_BF16) return run_bwd<__nv_bfloat16>(a, p, vec, dw, s);
+  return run_bwd<__half>(a, p, vec, dw, s);
+}
+
+int pvb2_quantize_8bit(int dtype, int64_t rows, int64_t D, const void* x, int64_t ldx, int tall, uint8_t* codes,
+                       int64_t ldc, float* scales, pvb2_stream stream) {
+  pvb2_rms_norm_desc d = {};
+  d.rows = rows;
+  d.D = D;
+  d.ldx = ldx;
+  d.ldc = ldc;
+  d.dtype = dtype;
+  PVB2_TRY(norm_check("quantize_8bit", &d));
+  if (rows == 0 || D == 0) return PVB2_OK;
+  PVB2_CHECK_ARG(x && codes && scales, "quantize_8bit: null pointer");
+  PVB2_TRY(norm_strides("quantize_8bit", &d, {ldx, ldc}));
+  cudaStream_t s = as_stream(stream);
+  if (!tall) {
+    NormArgs a = norm_args(&d, x, nullptr, nullptr, nullptr);
+    a.codes = codes;
+    a.scales = scales;
+    return run_norm<kQuant8>(a, dtype, norm_vec(a, dtype), s);
+  }
+  const int64_t groups = (D + 127) / 128, blocks = (rows + 127) / 128;
+  PVB2_CHECK_ARG(blocks <= 65535, "quantize_8bit: more than %d rows in blocks of 128", 65535 * 128);
+  const dim3 grid((unsigned)groups, (unsigned)blocks);
+  if (dtype == PVB2_F32)
+    quant_tile_kernel<float><<<grid, 256, 0, s>>>((const float*)x, rows, D, ldx, codes, ldc, scales, groups);
+  else if (dtype == PVB2_BF16)
+    quant_tile_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>((const __nv_bfloat16*)x, rows, D, ldx, codes, ldc, scales, groups);
+  else quant_tile_kernel<__half><<<grid, 256, 0, s>>>((const __half*)x, rows, D, ldx, codes, ldc, scales, groups);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+int pvb2_dequantize_8bit(int64_t rows, int64_t D, const uint8_t* codes, int64_t ldc, const float* scales, int tall,
+                         int dtype, void* out, pvb2_stream stream) {
+  pvb2_rms_norm_desc d = {};
+  d.rows = rows;
+  d.D = D;
+  d.dtype = dtype;
+  PVB2_TRY(norm_check("dequantize_8bit", &d));
+  if (rows == 0 || D == 0) return PVB2_OK;
+  PVB2_CHECK_ARG(codes && scales && out, "dequantize_8bit: null pointer");
+  PVB2_TRY(norm_strides("dequantize_8bit", &d, {ldc}));
+  const int groups = (int)((D + 127) / 128), size = dtype_size(dtype);
+  const bool vec = D % 8 == 0 && ((uintptr_t)codes & 7) == 0 && (rows <= 1 || ldc % 8 == 0) && ((uintptr_t)out & 15) == 0 &&
+                   D * size % 16 == 0;
+  cudaStream_t s = as_stream(stream);
+  const int grid = grid_for(rows * (vec ? D / 8 : D), 256, 8);
+  auto go = [&](auto* p) {
+    using T = std::remove_pointer_t<decltype(p)>;
+    if (vec) dequant_kernel<T, true><<<grid, 256, 0, s>>>(codes, scales, p, rows, (int)D, ldc, groups, tall);
+    else dequant_kernel<T, false><<<grid, 256, 0, s>>>(codes, scales, p, rows, (int)D, ldc, groups, tall);
+  };
+  if (dtype == PVB2_F32) go((float*)out);
+  else if (dtype == PVB2_BF16) go((__nv_bfloat16*)out);
+  else go((__half*)out);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
+}  // extern "C"

@@ -60,3 +60,85 @@ def relative_position_bias(table, q_len, k_len, *, bidirectional=True, max_dista
     a mask it takes its unfused path); in 16 bits, to scores of a program's own.
     """
     return torch.ops.ocl.relative_position_bias(table, q_len, k_len, bidirectional, max_distance, q_offset)
+
+
+def rms_norm(input, weight=None, residual=None, *, eps=1e-6):
+    """Root-mean-square norm over the last dimension, with the residual's addition before it.
+
+    ``y = h / sqrt(mean(h**2) + eps) * weight`` with ``h = input``, or with
+    ``h = input + residual`` rounded to their type; then the result is ``(y, h)``,
+    ``h`` being the residual stream as it goes on.  fp32, bf16 or fp16, all of
+    one type; ``weight`` ``[features]`` or None.  The mean of squares is summed in
+    64 bits, the rest is fp32, rounded once.  Gradients of ``input``,
+    ``residual`` and ``weight`` (the last in a fixed order); forward mode and
+    second derivatives are refused.
+    """
+    if residual is None:
+        return torch.ops.ocl.rms_norm(input, weight, eps)
+    return torch.ops.ocl.rms_norm_add(input, residual, weight, eps)
+
+
+def rms_norm_8bit(input, weight=None, residual=None, *, eps=1e-6):
+    """``rms_norm`` whose output is ``quantize_8bit``'s: ``(codes, scales)``, or ``(codes, scales, h)`` with a residual.
+
+    The codes are those of ``y`` before it is rounded to the input's type.  They
+    have no gradient: tensors that require one are refused outside
+    ``torch.no_grad()``.
+    """
+    return tuple(torch.ops.ocl.rms_norm_8bit(input, weight, residual, eps))
+
+
+def quantize_8bit(input, *, block_rows=1):
+    """``(codes, scales)`` of fp32, bf16 or fp16 numbers in 8-bit floating point.
+
+    ``codes`` are uint8 and hold e4m3 numbers (``codes.cpu().view(torch.float8_e4m3fn)``
+    shows them), rows beginning on 16-byte boundaries.  One fp32 scale belongs to
+    128 consecutive elements of a row (``block_rows=1``: activations, scales
+    ``[..., ceil(features / 128)]``) or to 128 x 128 elements of a matrix
+    (``block_rows=128``: weights, scales ``[ceil(rows / 128), ceil(features / 128)]``).
+    The scale is the largest magnitude over 448, the largest code; a block whose
+    magnitudes are 2**-100 or less becomes 0, one that holds an infinity or a NaN
+    is NaN throughout.
+    """
+    if block_rows not in (1, 128):
+        raise ValueError(f"block_rows is 1 or 128, got {block_rows!r}")
+    return torch.ops.ocl.quantize_8bit(input, block_rows == 128)
+
+
+def dequantize_8bit(codes, scales, *, dtype=torch.float32):
+    """The numbers that ``quantize_8bit``'s or ``rms_norm_8bit``'s codes stand for."""
+    return torch.ops.ocl.dequantize_8bit(codes, scales, dtype)
+
+
+def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None, *, dtype=torch.bfloat16):
+    """``F.linear`` of operands in 8 bits: ``x w^T + bias`` as fp32, bf16 or fp16.
+
+    ``codes`` ``[..., features]`` with a scale for every 128 of a row
+    (``rms_norm_8bit``, ``quantize_8bit(x)``), ``weight_codes`` ``[outputs, features]``
+    with one for every 128 x 128 (``quantize_8bit(w, block_rows=128)``, once);
+    ``bias`` ``[outputs]`` of the output's type.  Any sizes, one row as well as
+    many.  Codes whose rows do not begin on 16-byte boundaries are copied first.
+    Products are exact and summed in fp32: by the tensor cores over 128 features,
+    then block by block with the scales.  No gradients (they are refused).
+    """
+    return torch.ops.ocl.linear_8bit(codes, scales, weight_codes, weight_scales, bias, dtype)
+
+
+def token_log_probs(logits, tokens, *, top=0):
+    """Log probabilities of given tokens and the entropy of their distributions, ``(log_probs, entropy)``, in fp32.
+
+    ``logits`` ``[..., vocabulary]`` in fp32, bf16 or fp16, ``tokens`` int64
+    ``[...]``: ``log_probs = log_softmax(logits)[tokens]``, ``entropy = -sum(p log p)``
+    in nats.  With ``top`` (at most 32 and the vocabulary) also the best
+    alternatives, ``(log_probs, entropy, top_log_probs, top_tokens)`` with
+    ``[..., top]``, by falling logit and of equal ones the lower token first.
+
+    ``log_probs`` and ``entropy`` have gradients (the alternatives have none);
+    forward mode and second derivatives are refused.  Logits of -inf have no
+    probability and no gradient.  Tokens outside the vocabulary (-100 for a
+    prompt's, say) have the log probability 0 and no gradient through it, whatever
+    their entropy's.  A row whose logits are all -inf has -inf, the entropy 0 and no
+    gradient; one that holds a NaN or +inf is NaN.
+    """
+    out = torch.ops.ocl.token_log_probs(logits, tokens, top)
+    return out if top else out[:2]

@@ -13,9 +13,14 @@ is the same step with moments that do not follow the parameters' type:
 
     opt = pytorch_vulkan_b200.optim.AdamW(model.parameters(), lr=1e-3, state_bits=8)
     loss.backward()
+    pytorch_vulkan_b200.optim.clip_grad_norm_(model.parameters(), 1.0)
     opt.step()
+
+``clip_grad_norm_`` is torch.nn.utils' in two launches over all gradients.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -164,3 +169,31 @@ class AdamW(torch.optim.Optimizer):
         finally:
             for hook in hooks:
                 hook.remove()
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scale the gradients of ``parameters`` so that their norm as one vector is at most ``max_norm``; returns the norm.
+
+    As ``torch.nn.utils.clip_grad_norm_``: each gradient is multiplied by
+    ``min(1, max_norm / (norm + 1e-6))``, and is not touched where that is 1.
+    ``norm_type`` is 1, 2 or ``inf``.  The norm is an fp32 number on the device
+    whatever the gradients' types (fp32, bf16 and fp16 may be mixed), summed in a
+    fixed order, and nothing is read back to the host, so that the call can be
+    captured in a graph; ``error_if_nonfinite=True`` does read it, and raises
+    before anything is scaled.  Parameters without a gradient are passed over;
+    gradients that are listed twice, that overlap or have gaps in memory, or
+    that lie on several devices are refused.
+    """
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    kinds = {1.0: 1, 2.0: 2, math.inf: 0}
+    if float(norm_type) not in kinds:
+        raise ValueError(f"norm_type is 1, 2 or inf, got {norm_type!r}")
+    max_norm, kind = float(max_norm), kinds[float(norm_type)]
+    if not max_norm >= 0.0:
+        raise ValueError(f"Invalid max_norm value: {max_norm}")
+    if error_if_nonfinite:
+        norm = _C.impl_clip_grad_norm(parameters, max_norm, kind, False)
+        if not math.isfinite(norm.item()):
+            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it "
+                               "cannot be clipped")
+    return _C.impl_clip_grad_norm(parameters, max_norm, kind, True)
