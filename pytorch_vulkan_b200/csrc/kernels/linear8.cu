@@ -13,7 +13,7 @@
 //
 // Two kernels:
 //   * many rows: CTA pairs (cta_group::2) on tiles of 256 rows x 256 outputs,
-//     persistent, loads by TMA into a ring of six K blocks, stores by TMA.  A
+//     persistent, loads by TMA into a ring of five K blocks, stores by TMA.  A
 //     block's products take the tensor core 512 clocks, the epilogue about as
 //     many instructions: it is bound by both, and by the board's power.
 //   * few rows: tiles of 128 outputs x 16 to 128 rows, the weight in the
@@ -60,20 +60,49 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, u
       : "memory");
 }
 
+// tells the even CTA that an accumulator has been read.  What it guards is in
+// TMEM, and has arrived in registers: nothing in memory has to be ordered, and
+// releasing it for the cluster cost more than the epilogue's arithmetic
+__device__ __forceinline__ void arrive_even_cta(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// (a0, a1) = (b0, b1) s + (a0, a1), each rounded once
+__device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, uint64_t ss) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "fma.rn.f32x2 a, b, %4, a;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1), "l"(ss));
+}
+__device__ __forceinline__ uint64_t pair_of(float s) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "f"(s));
+  return p;
+}
+
 // ---------------------------------------------------------------- many rows
 constexpr int kL8M = 256, kL8N = 256;
-// Warps: three issue loads, one the products, 16 run the epilogue, 32 rows and
-// 64 columns each: five for each of the SM's four schedulers.
-constexpr int kL8Producers = 3, kL8MmaWarp = 3, kL8EpiWarps = 16;
+// Warps: two issue loads, one prepares the scales, one issues the products, 16
+// run the epilogue, 32 rows and 64 columns each: five for each of the SM's four
+// schedulers.  The epilogue's 96 registers hold 64 sums and 16 columns on their
+// way from TMEM; scales loaded by its own threads did not fit beside them, and
+// what spilled had left L1 (the ring takes it) by the time it was needed.
+constexpr int kL8Producers = 2, kL8ScaleWarp = 2, kL8MmaWarp = 3, kL8EpiWarps = 16;
 struct L8Smem {
-  static constexpr int THREADS = (kL8Producers + 1 + kL8EpiWarps) * 32;
+  static constexpr int THREADS = (kL8MmaWarp + 1 + kL8EpiWarps) * 32;
   static constexpr int A_BYTES = 128 * kL8BK;          // this CTA's rows of x
   static constexpr int B_BYTES = kL8N / 2 * kL8BK;     // and its half of the outputs
   static constexpr int SLOT_BYTES = A_BYTES + B_BYTES;
-  static constexpr int SLOTS = (224 * 1024 - kL8EpiWarps * 4096) / SLOT_BYTES;
-  static constexpr int EPI_OFF = SLOTS * SLOT_BYTES;   // one 4 KB store box per epilogue warp
-  static constexpr int BAR_OFF = EPI_OFF + kL8EpiWarps * 4096;
-  static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 4) * 8 + 16;
+  static constexpr int SLOTS = 5;
+  static constexpr int BOX = 2048;                     // of an epilogue warp: 32 rows of 64 bytes
+  static constexpr int EPI_OFF = SLOTS * SLOT_BYTES;
+  static constexpr int SCALE_BYTES = 4 * 2 * 128 * 4;  // [block of four][half of the outputs][row]
+  static constexpr int SCALE_OFF = EPI_OFF + kL8EpiWarps * BOX;
+  static constexpr int BAR_OFF = SCALE_OFF + 2 * SCALE_BYTES;
+  static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 8) * 8 + 16;
 };
 
 template <typename T>
@@ -88,7 +117,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   uint64_t* empty = full + kSlots;
   uint64_t* acc_full = empty + kSlots;
   uint64_t* acc_empty = acc_full + 2;               // waited on in the even CTA
-  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+  uint64_t* scales_full = acc_empty + 2;
+  uint64_t* scales_empty = scales_full + 2;
+  uint32_t* tmem_slot = (uint32_t*)(scales_empty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -105,6 +136,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 2 * kL8EpiWarps);
+      mbar_init(&scales_full[b], 1);
+      mbar_init(&scales_empty[b], kL8EpiWarps);
     }
     *abort = 0;
     fence_barrier_init();
@@ -146,6 +179,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
         }
       }
     }
+  } else if (warp == kL8ScaleWarp) {
+    // ------------------------------------------------- the scales of four blocks at a time: x's times the weight's
+    uint32_t group = 0;
+    for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
+      int mb, nb;
+      place(tile, mb, nb);
+      const int m0 = mb * kL8M + rank * 128 + lane;
+      // (rows and outputs past the end: some scale, of codes that are 0)
+      const float* ws0 = p.ws + (int64_t)(nb * (kL8N / kGroup8)) * p.blocks;
+      const float* ws1 = p.ws + (int64_t)min(nb * (kL8N / kGroup8) + 1, (p.N - 1) / kGroup8) * p.blocks;
+      float x[4][4], w[2][4];
+      auto fetch = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = min(kb + i, p.blocks - 1);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r][i] = __ldg(p.xs + (int64_t)min(m0 + 32 * r, p.M - 1) * p.blocks + k);
+          w[0][i] = __ldg(ws0 + k);
+          w[1][i] = __ldg(ws1 + k);
+        }
+      };
+      fetch(0);
+      for (int kb = 0; kb < p.blocks; kb += 4, ++group) {
+        const int slot = group & 1;
+        if (!mbar_wait(&scales_empty[slot], ((group >> 1) & 1) ^ 1, abort)) break;
+        float* to = (float*)(smem + L::SCALE_OFF + slot * L::SCALE_BYTES) + lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[(i * 2 + h) * 128 + 32 * r] = x[r][i] * w[h][i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scales_full[slot]);
+        if (kb + 4 < p.blocks) fetch(kb + 4);
+      }
+    }
   } else if (warp == kL8MmaWarp) {
     // ------------------------------------------------- products, by the even CTA for both
     if (lane == 0 && rank == 0) {
@@ -175,49 +245,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   } else {
     // ------------------------------------------------- epilogue: TMEM lane quarter warp % 4, 64 columns (warp - 4) / 4
     const int quarter = warp & 3, part = (warp - kL8MmaWarp - 1) >> 2;
-    uint8_t* box = smem + L::EPI_OFF + (warp - kL8MmaWarp - 1) * 4096;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    uint32_t it = 0;
+    uint8_t* box = smem + L::EPI_OFF + (warp - kL8MmaWarp - 1) * L::BOX;
+    const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + part * 64;
+    const float* scales = (const float*)(smem + L::SCALE_OFF) + (part >> 1) * 128 + quarter * 32 + lane;
+    const uint32_t even_empty = even_cta_addr(acc_empty);
+    uint32_t it = 0, group = 0;
     for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
-      int mb, nb;
-      place(tile, mb, nb);
-      const int m0 = mb * kL8M + rank * 128 + quarter * 32, m = m0 + lane;
-      const int n0 = nb * kL8N + part * 64;
-      // rows and outputs past the end: zero codes times some scale in range
-      const float* xs = p.xs + (int64_t)min(m, p.M - 1) * p.blocks;
-      const float* ws = p.ws + (int64_t)(min(n0, p.N - 1) / kGroup8) * p.blocks;
       float v[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) v[j] = 0.f;
       bool ok = true;
-      float scale = __ldg(xs) * __ldg(ws);
 #pragma unroll 1
       for (int kb = 0; kb < p.blocks; ++kb, ++it) {
-        const int buf = it & 1, next = min(kb + 1, p.blocks - 1);
-        const float xs_next = __ldg(xs + next), ws_next = __ldg(ws + next);
-        ok = mbar_wait(&acc_full[buf], (it >> 1) & 1, abort);
+        const int buf = it & 1, slot = group & 1;
+        if ((kb & 3) == 0) ok = mbar_wait(&scales_full[slot], (group >> 1) & 1, abort);
+        const uint64_t ss = pair_of(scales[slot * (L::SCALE_BYTES / 4) + (kb & 3) * 256]);
+        ok = ok && mbar_wait(&acc_full[buf], (it >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
+        const bool last = (kb & 3) == 3 || kb + 1 == p.blocks;  // of the scales' slot
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           float u[16];
-          tmem_ld16(tmem_base + lanes + buf * kL8N + part * 64 + 16 * h, u);
+          tmem_ld16(acc + buf * kL8N + 16 * h, u);
+          if (h == 3) {  // all of it is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              arrive_even_cta(even_empty + buf * 8);
+              if (last) mbar_arrive(&scales_empty[slot]);
+            }
+          }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[16 * h + j] = fmaf(u[j], scale, v[16 * h + j]);
+          for (int j = 0; j < 16; j += 2) fma2(v[16 * h + j], v[16 * h + j + 1], u[j], u[j + 1], ss);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(even_cta_addr(&acc_empty[buf]));
-        scale = xs_next * ws_next;
+        group += last;
       }
       if (!ok) break;
+      int mb, nb;
+      place(tile, mb, nb);
+      const int m0 = mb * kL8M + rank * 128 + quarter * 32, n0 = nb * kL8N + part * 64;
       if (n0 >= p.N || m0 >= p.M) continue;
       if (p.bias) {
 #pragma unroll
         for (int j = 0; j < 64; ++j) v[j] += to_f32(((const T*)p.bias)[min(n0 + j, p.N - 1)]);
       }
-      // through the box: 32 rows of 128 bytes
-      constexpr int kWide = 128 / (int)sizeof(T), E = 16 / (int)sizeof(T);
+      // through the box: 32 rows of 64 bytes, 16-byte pieces swizzled by bits 1 and 2 of the row
+      constexpr int kWide = 64 / (int)sizeof(T), E = 16 / (int)sizeof(T);
 #pragma unroll
       for (int h = 0; h < 64 / kWide; ++h) {
         if (p.tma_store) {
@@ -225,8 +299,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
           __syncwarp();
         }
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          store_vec<E>((T*)(box + lane * 128 + ((q ^ (lane & 7)) * 16)), v + h * kWide + q * E);
+        for (int q = 0; q < 4; ++q)
+          store_vec<E>((T*)(box + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)), v + h * kWide + q * E);
         const int nn = n0 + h * kWide;
         if (p.tma_store) {
           fence_proxy_async_smem();
@@ -237,13 +311,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
           }
         } else {
           __syncwarp();
-          for (int r = 0; r < 32 && m0 + r < p.M; ++r) {
-            T* row = (T*)p.y + (int64_t)(m0 + r) * p.N;
-#pragma unroll
-            for (int c = 0; c < kWide; c += 32) {
-              const int j = c + lane;
-              if (nn + j < p.N) row[nn + j] = *(const T*)(box + r * 128 + (((j / E) ^ (r & 7)) * 16) + (j % E) * sizeof(T));
-            }
+          // 32 / kWide rows at a time
+#pragma unroll 4
+          for (int r = lane / kWide; r < 32; r += 32 / std::min(32, kWide)) {
+            const int j = lane % kWide;
+            if (m0 + r < p.M && nn + j < p.N)
+              ((T*)p.y)[(int64_t)(m0 + r) * p.N + nn + j] =
+                  *(const T*)(box + r * 64 + (((j / E) ^ ((r >> 1) & 3)) * 16) + (j % E) * sizeof(T));
           }
           __syncwarp();
         }
@@ -453,15 +527,16 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
 static int64_t l8_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 static int l8_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t ld_bytes, int box_cols, int box_rows,
-                  CUtensorMapDataType type) {
+                  CUtensorMapDataType type, CUtensorMapSwizzle swizzle) {
   uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, 1};
   uint64_t str[2] = {(uint64_t)ld_bytes, (uint64_t)ld_bytes * rows};
   uint32_t box[3] = {(uint32_t)box_cols, (uint32_t)box_rows, 1};
-  return encode_tiled(m, 3, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, nullptr, type);
+  return encode_tiled(m, 3, base, dims, str, box, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, nullptr, type);
 }
 static int l8_codes(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
   // (one row: its stride counts for nothing, but has to be one)
-  return l8_map(m, base, K, rows, rows == 1 ? l8_div(K, 16) * 16 : ld, kL8BK, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8);
+  return l8_map(m, base, K, rows, rows == 1 ? l8_div(K, 16) * 16 : ld, kL8BK, box_rows,
+                CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <typename T>
@@ -475,10 +550,11 @@ static int l8_many(const pvb2_linear8_desc* d, const void* x, const void* w, L8A
   p.tma_store = ((uintptr_t)p.y & 15) == 0 && d->N * (int64_t)sizeof(T) % 16 == 0;
   memset(&my, 0, sizeof(my));
   if (p.tma_store)
-    PVB2_TRY(l8_map(&my, p.y, d->N, d->M, d->N * sizeof(T), 128 / (int)sizeof(T), 32,
+    PVB2_TRY(l8_map(&my, p.y, d->N, d->M, d->N * sizeof(T), 64 / (int)sizeof(T), 32,
                     sizeof(T) == 4                              ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                     : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16));
+                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                    CU_TENSOR_MAP_SWIZZLE_64B));
   const int64_t tiles = l8_div(d->M, kL8M) * l8_div(d->N, kL8N);
   // blocks of rows that stay in L2 (32 MB of its 126) while the outputs go by
   p.group = (int)std::max<int64_t>(8, std::min<int64_t>(l8_div(d->M, kL8M), ((int64_t)32 << 20) / (kL8M * d->K)));
