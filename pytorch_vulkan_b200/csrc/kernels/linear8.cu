@@ -35,7 +35,8 @@ struct L8Args {
   const void* bias;  // of the output's type, or null
   void* y;           // [M][N]
   int M, N, blocks;
-  int tma_store;
+  int tma_store;     // many rows: y's rows lie on 16-byte boundaries
+  int vector_store;  // few rows: and four outputs on theirs
   int group;         // blocks of rows whose tiles lie together
 };
 
@@ -67,21 +68,55 @@ __device__ __forceinline__ void arrive_even_cta(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// (a0, a1) = (b0, b1) s + (a0, a1), each rounded once
-__device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, uint64_t ss) {
-  asm("{\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%0, %1};\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "fma.rn.f32x2 a, b, %4, a;\n\t"
-      "mov.b64 {%0, %1}, a;\n\t}"
-      : "+f"(a0), "+f"(a1)
-      : "f"(b0), "f"(b1), "l"(ss));
-}
-__device__ __forceinline__ uint64_t pair_of(float s) {
+// two fp32 numbers in a register pair; a = b s + a, each rounded once
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
   uint64_t p;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "f"(s));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
   return p;
 }
+__device__ __forceinline__ void fma2(uint64_t& a, uint64_t b, uint64_t s) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(b), "l"(s));
+}
+__device__ __forceinline__ float2 numbers(uint64_t p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+
+// 16 columns of this warp's 32 lanes, as pairs.  The wait is part of the
+// statement: apart from it, each value was copied before its use
+__device__ __forceinline__ void tmem_ld16_pairs(uint32_t taddr, uint64_t* u) {
+  asm volatile(
+      "{\n\t.reg .b32 r<16>;\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{r0,r1,r2,r3,r4,r5,r6,r7,r8,r9,r10,r11,r12,r13,r14,r15}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "mov.b64 %0, {r0, r1};\n\t"
+      "mov.b64 %1, {r2, r3};\n\t"
+      "mov.b64 %2, {r4, r5};\n\t"
+      "mov.b64 %3, {r6, r7};\n\t"
+      "mov.b64 %4, {r8, r9};\n\t"
+      "mov.b64 %5, {r10, r11};\n\t"
+      "mov.b64 %6, {r12, r13};\n\t"
+      "mov.b64 %7, {r14, r15};\n\t"
+      "}"
+      : "=l"(u[0]), "=l"(u[1]), "=l"(u[2]), "=l"(u[3]), "=l"(u[4]), "=l"(u[5]), "=l"(u[6]), "=l"(u[7])
+      : "r"(taddr)
+      : "memory");
+}
+
+// The issuing warp stays whole: its loop runs in all lanes, on values that the
+// compiler knows to be the same in each (a warp's number by a shuffle, a wait's
+// result by a vote, TMEM's base by a reduction), and one lane is elected for the
+// instructions alone.  Descriptors are then in uniform registers; from within
+// a branch of lane 0 each MMA took 75 clocks to issue, a block of four, with
+// its waits and commits, 700, where the tensor core needs 512.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ int warp_number() { return __shfl_sync(~0u, (int)(threadIdx.x >> 5), 0); }
 
 // ---------------------------------------------------------------- many rows
 constexpr int kL8M = 256, kL8N = 256;
@@ -122,7 +157,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   uint32_t* tmem_slot = (uint32_t*)(scales_empty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_number(), lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int tiles_m = (p.M + kL8M - 1) / kL8M, tiles_n = (p.N + kL8N - 1) / kL8N;
   const int tiles = tiles_m * tiles_n;
@@ -218,28 +253,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
     }
   } else if (warp == kL8MmaWarp) {
     // ------------------------------------------------- products, by the even CTA for both
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = idesc_e4m3(kL8M, kL8N);
+      const uint32_t base = __reduce_or_sync(~0u, tmem_base);
       const uint64_t a0 = desc_kmajor(smem_u32(smem), 0), b0 = desc_kmajor(smem_u32(smem) + L::A_BYTES, 0);
       uint32_t it = 0;
-      for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
-        bool ok = true;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
         for (int kb = 0; kb < p.blocks; ++kb, ++it) {
           const int buf = it & 1, s = it % kSlots;
-          ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort) && mbar_wait(&full[s], (it / kSlots) & 1, abort);
+          ok = __all_sync(~0u, mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort) &&
+                                   mbar_wait(&full[s], (it / kSlots) & 1, abort));
           if (!ok) break;
           tc_fence_after();
-          uint64_t ad = a0 + (uint32_t)(s * (L::SLOT_BYTES / 16)), bd = b0 + (uint32_t)(s * (L::SLOT_BYTES / 16));
+          if (elect_one()) {
+            const uint64_t ad = a0 + (uint32_t)(s * (L::SLOT_BYTES / 16)), bd = b0 + (uint32_t)(s * (L::SLOT_BYTES / 16));
 #pragma unroll
-          for (int kk = 0; kk < kL8BK / 32; ++kk) {
-            mma_e4m3_pair(tmem_base + buf * kL8N, ad, bd, idesc, kk ? 1u : 0u);
-            ad += 2;
-            bd += 2;
+            for (int kk = 0; kk < kL8BK / 32; ++kk)
+              mma_e4m3_pair(base + buf * kL8N, ad + 2 * kk, bd + 2 * kk, idesc, kk ? 1u : 0u);
+            mma_commit_pair(&empty[s]);
+            mma_commit_pair(&acc_full[buf]);
           }
-          mma_commit_pair(&empty[s]);
-          mma_commit_pair(&acc_full[buf]);
+          __syncwarp();
         }
-        if (!ok) break;
       }
     }
   } else {
@@ -251,23 +287,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
     const uint32_t even_empty = even_cta_addr(acc_empty);
     uint32_t it = 0, group = 0;
     for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
-      float v[64];
+      uint64_t sums[32];  // of two columns each
 #pragma unroll
-      for (int j = 0; j < 64; ++j) v[j] = 0.f;
+      for (int j = 0; j < 32; ++j) sums[j] = 0;
       bool ok = true;
 #pragma unroll 1
       for (int kb = 0; kb < p.blocks; ++kb, ++it) {
         const int buf = it & 1, slot = group & 1;
         if ((kb & 3) == 0) ok = mbar_wait(&scales_full[slot], (group >> 1) & 1, abort);
-        const uint64_t ss = pair_of(scales[slot * (L::SCALE_BYTES / 4) + (kb & 3) * 256]);
+        const float scale = scales[slot * (L::SCALE_BYTES / 4) + (kb & 3) * 256];
+        const uint64_t ss = pair_of(scale, scale);
         ok = ok && mbar_wait(&acc_full[buf], (it >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
         const bool last = (kb & 3) == 3 || kb + 1 == p.blocks;  // of the scales' slot
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-          float u[16];
-          tmem_ld16(acc + buf * kL8N + 16 * h, u);
+          if (h) __syncwarp();  // (the next columns stay behind these sums: 626 -> 615 us for 8192^3)
+          uint64_t u[8];
+          tmem_ld16_pairs(acc + buf * kL8N + 16 * h, u);
           if (h == 3) {  // all of it is in registers
             tc_fence_before();
             __syncwarp();
@@ -277,7 +315,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
             }
           }
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) fma2(v[16 * h + j], v[16 * h + j + 1], u[j], u[j + 1], ss);
+          for (int j = 0; j < 8; ++j) fma2(sums[8 * h + j], u[j], ss);
         }
         group += last;
       }
@@ -286,6 +324,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
       place(tile, mb, nb);
       const int m0 = mb * kL8M + rank * 128 + quarter * 32, n0 = nb * kL8N + part * 64;
       if (n0 >= p.N || m0 >= p.M) continue;
+      float v[64];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float2 f = numbers(sums[j]);
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      }
       if (p.bias) {
 #pragma unroll
         for (int j = 0; j < 64; ++j) v[j] += to_f32(((const T*)p.bias)[min(n0 + j, p.N - 1)]);
@@ -341,66 +386,148 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
 }
 
 // ----------------------------------------------------------------- few rows
-// Warps: one issues loads, one the products, four run the epilogue.
+// Warps: one issues loads, one the products, eight run the epilogue, 32
+// outputs and half the rows each (four of them took half as long again for
+// short K: alone on its scheduler, a warp waits for each of its instructions).
+// As many accumulators as TMEM holds, eight at most: a block of 16 rows is
+// multiplied faster than its accumulator goes to the epilogue and back.
+constexpr int kL8FewEpi = 8;
 template <int NT>
 struct L8Few {
-  static constexpr int THREADS = 192;
+  static constexpr int THREADS = (2 + kL8FewEpi) * 32;
   static constexpr int W_BYTES = 128 * kL8BK;
   static constexpr int SLOT_BYTES = W_BYTES + NT * kL8BK;
-  static constexpr int SLOTS = std::min(12, 200 * 1024 / SLOT_BYTES);
-  static constexpr int SCALE_OFF = SLOTS * SLOT_BYTES;  // each epilogue warp's row scales of two K blocks
-  static constexpr int BAR_OFF = SCALE_OFF + 4 * 2 * NT * 4;
-  static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 4) * 8 + 16;
-  static constexpr int COLUMNS = 2 * NT < 32 ? 32 : 2 * NT;  // of TMEM
+  static constexpr int BUFS = std::min(8, 512 / NT);
+  static constexpr int COLUMNS = BUFS * NT;             // of TMEM
+  static constexpr int RUN = 32;                        // blocks whose scales are at hand
+  static constexpr int PITCH = NT + 4;                  // of a block's scales
+  static constexpr int SLOTS = std::min(11, (224 * 1024 - RUN * PITCH * 4) / SLOT_BYTES);
+  static constexpr int SCALE_OFF = SLOTS * SLOT_BYTES;  // [block][row]: x's times the weight's
+  static constexpr int BAR_OFF = SCALE_OFF + RUN * PITCH * 4;
+  static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 2 * BUFS) * 8 + 16;
   static_assert(SLOTS * SLOT_BYTES >= 128 * NT * 4, "the sums go where the ring was");
 };
+
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kL8FewEpi * 32) : "memory"); }
+// four floats of another CTA of the cluster
+__device__ __forceinline__ float4 load_cluster(const float* p, int rank) {
+  uint32_t at;
+  float4 f;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(at) : "memory");
+  return f;
+}
+// COLS columns of this warp's 32 lanes
+template <int COLS>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float* v) {
+  if constexpr (COLS == 32) {
+    tmem_ld32(taddr, v);
+  } else if constexpr (COLS == 16) {
+    tmem_ld16(taddr, v);
+  } else {
+    static_assert(COLS == 8, "8, 16 or 32 columns");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+        : "r"(taddr)
+        : "memory");
+  }
+}
+
+// The scales of the blocks [kb, kb + count) for the tile's rows, x's times the
+// weight's, by the epilogue's threads.
+template <int NT>
+__device__ __forceinline__ void load_scales(const L8Args& p, const float* ws, int m0, int kb, int count, float* run, int warp,
+                                            int lane) {
+  constexpr int kPitch = L8Few<NT>::PITCH;
+  if (NT >= 64) {
+    // some threads to a row, eight blocks at a time each
+    constexpr int kPer = NT >= 64 ? kL8FewEpi * 32 / NT : 1;
+    const int t = (warp - 2) * 32 + lane, j = t % NT;
+    const float* row = p.xs + (int64_t)min(m0 + j, p.M - 1) * p.blocks + kb;
+#pragma unroll 1
+    for (int k0 = t / NT * 8; k0 < count; k0 += 8 * kPer) {
+      float x[8], w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __ldg(row + min(k0 + i, count - 1));
+        w[i] = __ldg(ws + kb + min(k0 + i, count - 1));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k0 + i < count) run[(k0 + i) * kPitch + j] = x[i] * w[i];
+    }
+  } else {
+    // a warp to a row, a lane to a block
+    constexpr int kRows = NT / kL8FewEpi;
+    const int k = min(lane, count - 1);
+    const float w = __ldg(ws + kb + k);
+    float x[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      x[i] = __ldg(p.xs + (int64_t)min(m0 + warp - 2 + kL8FewEpi * i, p.M - 1) * p.blocks + kb + k);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (lane < count) run[lane * kPitch + warp - 2 + kL8FewEpi * i] = x[i] * w;
+  }
+}
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
     linear8_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                        const __grid_constant__ L8Args p, int splits) {
   using L = L8Few<NT>;
-  constexpr int kSlots = L::SLOTS;
+  constexpr int kSlots = L::SLOTS, kBufs = L::BUFS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = (uint64_t*)(smem + L::BAR_OFF);
   uint64_t* empty = full + kSlots;
   uint64_t* acc_full = empty + kSlots;
-  uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+  uint64_t* acc_empty = acc_full + kBufs;
+  uint32_t* tmem_slot = (uint32_t*)(acc_empty + kBufs);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_number(), lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
   // tiles of the same outputs lie together: their weight is read once
   const int tiles_m = (p.M + NT - 1) / NT;
   const int m0 = tile % tiles_m * NT, nb = tile / tiles_m, n0 = nb * 128;
   const int kb0 = (int)((int64_t)p.blocks * rank / splits), kb1 = (int)((int64_t)p.blocks * (rank + 1) / splits);
 
-  if (threadIdx.x == 0) {
-    tma_prefetch(&tmX);
-    tma_prefetch(&tmW);
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
-    }
-    *abort = 0;
+  const float* ws = p.ws + (int64_t)nb * p.blocks;
+  float* run = (float*)(smem + L::SCALE_OFF);
+  if (warp == 0) {
+#pragma unroll
+    for (int i = lane; i < 2 * kSlots + 2 * kBufs; i += 32) mbar_init(&full[i], i < 2 * kSlots + kBufs ? 1 : kL8FewEpi);
     fence_barrier_init();
+    __syncwarp();
+    if (lane == 0) {
+      *abort = 0;
+      // the first loads need nothing of the others
+      for (int it = 0; it < min(kSlots, kb1 - kb0); ++it) {
+        uint8_t* sw = smem + it * L::SLOT_BYTES;
+        mbar_arrive_expect_tx(&full[it], L::SLOT_BYTES);
+        tma_load_3d(sw, &tmW, &full[it], (kb0 + it) * kL8BK, n0, 0);
+        tma_load_3d(sw + L::W_BYTES, &tmX, &full[it], (kb0 + it) * kL8BK, m0, 0);
+      }
+    }
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, L::COLUMNS);
+  } else {
+    load_scales<NT>(p, ws, m0, kb0, min(L::RUN, kb1 - kb0), run, warp, lane);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, L::COLUMNS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  float v[NT];
+  constexpr int kHalf = NT / 2, kWide = kHalf < 32 ? kHalf : 32;
+  const int first = warp < 6 ? 0 : kHalf;  // an epilogue warp's first row of the tile
+  float v[kHalf];
   if (warp == 0) {
     if (lane == 0) {
-      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+      for (int kb = kb0 + kSlots, it = kSlots; kb < kb1; ++kb, ++it) {
         const int s = it % kSlots;
         if (!mbar_wait(&empty[s], ((it / kSlots) & 1) ^ 1, abort)) break;
         uint8_t* sw = smem + s * L::SLOT_BYTES;
@@ -410,64 +537,53 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(128, NT);
-      const uint64_t a0 = desc_kmajor(smem_u32(smem), 0), b0 = desc_kmajor(smem_u32(smem) + L::W_BYTES, 0);
-      for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-        const int buf = it & 1, s = it % kSlots;
-        if (!mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort) || !mbar_wait(&full[s], (it / kSlots) & 1, abort)) break;
-        tc_fence_after();
-        uint64_t ad = a0 + (uint32_t)(s * (L::SLOT_BYTES / 16)), bd = b0 + (uint32_t)(s * (L::SLOT_BYTES / 16));
+    constexpr uint32_t idesc = idesc_e4m3(128, NT);
+    const uint32_t base = __reduce_or_sync(~0u, tmem_base);
+    const uint64_t a0 = desc_kmajor(smem_u32(smem), 0), b0 = desc_kmajor(smem_u32(smem) + L::W_BYTES, 0);
+    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+      const int buf = it % kBufs, s = it % kSlots;
+      if (!__all_sync(~0u, mbar_wait(&acc_empty[buf], ((it / kBufs) & 1) ^ 1, abort) &&
+                               mbar_wait(&full[s], (it / kSlots) & 1, abort)))
+        break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t ad = a0 + (uint32_t)(s * (L::SLOT_BYTES / 16)), bd = b0 + (uint32_t)(s * (L::SLOT_BYTES / 16));
 #pragma unroll
-        for (int kk = 0; kk < kL8BK / 32; ++kk) {
-          mma_e4m3(tmem_base + buf * NT, ad, bd, idesc, kk ? 1u : 0u);
-          ad += 2;
-          bd += 2;
-        }
+        for (int kk = 0; kk < kL8BK / 32; ++kk) mma_e4m3(base + buf * NT, ad + 2 * kk, bd + 2 * kk, idesc, kk ? 1u : 0u);
         mma_commit(&empty[s]);
         mma_commit(&acc_full[buf]);
       }
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------- epilogue: lane = output, register = row of x
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    float* scales = (float*)(smem + L::SCALE_OFF) + (warp & 3) * 2 * NT;
-    const float* ws = p.ws + (int64_t)nb * p.blocks;
-    constexpr int kPer = (NT + 31) / 32;  // row scales that a lane loads
-    float w_next = 0.f, x_next[kPer];
-    auto fetch = [&](int kb) {
-      w_next = __ldg(ws + kb);
+    const uint32_t acc = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + first;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int j = i * 32 + lane;
-        x_next[i] = j < NT && m0 + j < p.M ? __ldg(p.xs + (int64_t)(m0 + j) * p.blocks + kb) : 0.f;
-      }
-    };
-#pragma unroll
-    for (int j = 0; j < NT; ++j) v[j] = 0.f;
-    if (kb0 < kb1) fetch(kb0);
+    for (int j = 0; j < kHalf; ++j) v[j] = 0.f;
+    bool ok = true;  // where a wait gave up, the others still meet at the barriers
 #pragma unroll 1
     for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-      const int buf = it & 1;
-      float* mine = scales + buf * NT;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i * 32 + lane < NT) mine[i * 32 + lane] = x_next[i] * w_next;
-      if (kb + 1 < kb1) fetch(kb + 1);
-      __syncwarp();
-      if (!mbar_wait(&acc_full[buf], (it >> 1) & 1, abort)) break;
+      const int in_run = it % L::RUN, buf = it % kBufs;
+      if (in_run == 0 && it > 0) {
+        epilogue_sync();  // the last run's have been read
+        load_scales<NT>(p, ws, m0, kb, min(L::RUN, kb1 - kb), run, warp, lane);
+        epilogue_sync();
+      }
+      ok = ok && mbar_wait(&acc_full[buf], (it / kBufs) & 1, abort);
+      if (!ok) continue;
       tc_fence_after();
 #pragma unroll
-      for (int h = 0; h < NT / 16; ++h) {
-        float u[16];
-        tmem_ld16(tmem_base + lanes + buf * NT + 16 * h, u);
+      for (int h = 0; h < kHalf / kWide; ++h) {
+        float u[kWide];
+        tmem_ld<kWide>(acc + buf * NT + kWide * h, u);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(mine + 16 * h + j);
-          v[16 * h + j] = fmaf(u[j], s.x, v[16 * h + j]);
-          v[16 * h + j + 1] = fmaf(u[j + 1], s.y, v[16 * h + j + 1]);
-          v[16 * h + j + 2] = fmaf(u[j + 2], s.z, v[16 * h + j + 2]);
-          v[16 * h + j + 3] = fmaf(u[j + 3], s.w, v[16 * h + j + 3]);
+        for (int j = 0; j < kWide; j += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(run + in_run * L::PITCH + first + kWide * h + j);
+          float* a = v + kWide * h + j;
+          a[0] = fmaf(u[j], s.x, a[0]);
+          a[1] = fmaf(u[j + 1], s.y, a[1]);
+          a[2] = fmaf(u[j + 2], s.z, a[2]);
+          a[3] = fmaf(u[j + 3], s.w, a[3]);
         }
       }
       tc_fence_before();
@@ -477,35 +593,93 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
   }
 
   // ---------------------------------------------------- the splits' sums, and y
-  const int out = (warp & 3) * 32 + lane, n = n0 + out;
+  // By way of shared memory and in loops that stay loops: a straight line with a
+  // store per register took longer than all the rest of a short K.  Several
+  // rows are read before the first is stored, since the compiler cannot know
+  // that y is not in shared memory.
   float* sums = (float*)smem;  // [NT][128]: every load has landed and every product been formed
-  const bool epi = warp >= 2;
-  const float b = epi && p.bias && n < p.N ? to_f32(((const T*)p.bias)[n]) : 0.f;
-  if (splits == 1) {
-    if (epi && n < p.N && !*abort) {
+  const bool epi = warp >= 2, gave_up = *abort;
+  if (epi && !gave_up) {
+    const int out = (warp & 3) * 32 + lane;
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (m0 + j < p.M) ((T*)p.y)[(int64_t)(m0 + j) * p.N + n] = from_f32<T>(v[j] + b);
+    for (int j = 0; j < kHalf; ++j) sums[(first + j) * 128 + out] = v[j];
+  }
+  const int rows = min(NT, p.M - m0);
+  T* y = (T*)p.y + (int64_t)m0 * p.N + n0;
+  // four outputs of a row for each lane, next to each other or 32 apart
+  const int step = p.vector_store || splits > 1 ? 1 : 32, o = step == 1 ? lane * 4 : lane;
+  float b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = epi && p.bias && n0 + o + i * step < p.N ? to_f32(((const T*)p.bias)[n0 + o + i * step]) : 0.f;
+  if (splits == 1) {
+    if (epi) {
+      epilogue_sync();
+      if (!gave_up && p.vector_store) {
+        constexpr int R = 8;
+#pragma unroll 1
+        for (int j0 = warp - 2; j0 < rows; j0 += kL8FewEpi * R) {
+          float4 x[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[r] = *reinterpret_cast<const float4*>(sums + min(j0 + kL8FewEpi * r, NT - 1) * 128 + o);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float all[4] = {x[r].x + b[0], x[r].y + b[1], x[r].z + b[2], x[r].w + b[3]};
+            if (j0 + kL8FewEpi * r < rows && n0 + o < p.N) store_vec<4>(y + (int64_t)(j0 + kL8FewEpi * r) * p.N + o, all);
+          }
+        }
+      } else if (!gave_up) {
+        constexpr int R = 4;
+#pragma unroll 1
+        for (int j0 = warp - 2; j0 < rows; j0 += kL8FewEpi * R) {
+          float x[R][4];
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[r][i] = sums[min(j0 + kL8FewEpi * r, NT - 1) * 128 + i * 32 + lane] + b[i];
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            T* row = y + (int64_t)(j0 + kL8FewEpi * r) * p.N + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (j0 + kL8FewEpi * r < rows && n0 + i * 32 + lane < p.N) row[i * 32] = from_f32<T>(x[r][i]);
+          }
+        }
+      }
     }
   } else {
-    const bool gave_up = *abort;
-    if (epi && !gave_up) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (m0 + j < p.M) sums[j * 128 + out] = v[j];
-    }
     cluster_sync();
     if (epi && !gave_up) {
-      for (int j = rank; j < NT && m0 + j < p.M; j += splits) {
-        float s = 0.f;
-        for (int r = 0; r < splits; ++r) {
-          uint32_t at;
-          float other;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sums + j * 128 + out)), "r"(r));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(at) : "memory");
-          s += other;
+      constexpr int R = 2;
+#pragma unroll 1
+      for (int j0 = rank + (warp - 2) * splits; j0 < rows; j0 += kL8FewEpi * R * splits) {
+        float4 part[R][8];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < splits) part[r][k] = load_cluster(sums + min(j0 + kL8FewEpi * r * splits, NT - 1) * 128 + o, k);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float all[4] = {b[0], b[1], b[2], b[3]};
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < splits) {
+              all[0] += part[r][k].x;
+              all[1] += part[r][k].y;
+              all[2] += part[r][k].z;
+              all[3] += part[r][k].w;
+            }
+          const int j = j0 + kL8FewEpi * r * splits;
+          if (j >= rows) break;
+          T* row = y + (int64_t)j * p.N + o;
+          if (p.vector_store) {
+            if (n0 + o < p.N) store_vec<4>(row, all);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (n0 + o + i < p.N) row[i] = from_f32<T>(all[i]);
+          }
         }
-        if (n < p.N) ((T*)p.y)[(int64_t)(m0 + j) * p.N + n] = from_f32<T>(s + b);
       }
     }
     cluster_sync();  // no block leaves while its sums are read
@@ -638,6 +812,7 @@ int pvb2_linear8(const pvb2_linear8_desc* d, const uint8_t* x, const float* x_sc
   p.M = (int)d->M;
   p.N = (int)d->N;
   p.blocks = (int)l8_div(d->K, kL8BK);
+  p.vector_store = d->N % 4 == 0 && ((uintptr_t)y & 15) == 0;
   cudaStream_t s = as_stream(stream);
   if (d->dtype == PVB2_F32) return l8_run<float>(d, x, w, p, s);
   if (d->dtype == PVB2_BF16) return l8_run<__nv_bfloat16>(d, x, w, p, s);
