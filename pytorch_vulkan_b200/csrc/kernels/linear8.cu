@@ -762,10 +762,13 @@ static int l8_few(const pvb2_linear8_desc* d, const void* x, const void* w, cons
   return PVB2_OK;
 }
 
-// CTAs of a cluster that share K: as many as have an SM, two K blocks each at least
+// CTAs of a cluster that share K: as many as have an SM, and eight K blocks
+// before each halving (joining the sums takes as long as four blocks do: 512
+// outputs of 512 inputs, 128 rows: 7.3 us whole, 8.3 in two; 4096 of 4096: 20.7
+// whole, 15.0 in two, 11.4 in four)
 static int l8_splits(int64_t tiles, int64_t blocks) {
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= num_sms() && blocks >= 4 * splits) splits *= 2;
+  while (splits < 8 && tiles * splits * 2 <= num_sms() && blocks >= 8 * splits) splits *= 2;
   return splits;
 }
 
@@ -773,8 +776,12 @@ template <typename T>
 static int l8_run(const pvb2_linear8_desc* d, const void* x, const void* w, const L8Args& p, cudaStream_t s) {
   const int nt = d->M <= 16 ? 16 : d->M <= 32 ? 32 : d->M <= 64 ? 64 : 128;
   const int64_t few = l8_div(d->N, 128) * l8_div(d->M, nt);
-  // pairs once they have half the device's SMs at least
-  if (d->M > 128 && l8_div(d->M, kL8M) * l8_div(d->N, kL8N) * 4 >= num_sms()) return l8_many<T>(d, x, w, p, s);
+  // Tiles of 128 x 128 as long as each has an SM of its own, then pairs' of 256 x
+  // 256 (us, the former and the latter: 512 rows, 4096 outputs of 4096 inputs
+  // 21.5 and 21.9, 1024 rows 41 and 23; 300 rows, 5001 of 1008 9.9 and 13.0, 512
+  // rows 17.6 and 13.4; 1024 rows, 1024 of 8192 23.5 and 37); few rows are bound
+  // by the weight, whatever its tiles.
+  if (d->M > 64 && few > num_sms()) return l8_many<T>(d, x, w, p, s);
   const int splits = l8_splits(few, p.blocks);
   if (nt == 16) return l8_few<T, 16>(d, x, w, p, splits, s);
   if (nt == 32) return l8_few<T, 32>(d, x, w, p, splits, s);
