@@ -44,7 +44,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kLpTop = 32;
 constexpr int kLpCluster = 8;
-constexpr int kLpRing = 8;  // chunks of a thread on their way
+constexpr int kLpRing = 8;  // chunks of a thread on their way, two to a step
 
 struct LpArgs {
   const void* z;
@@ -113,11 +113,38 @@ __device__ __forceinline__ void take_slowly(Running& r, const float* z) {
   }
 }
 
+// two fp32 numbers in a register pair, which one instruction works on
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 numbers(uint64_t p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // the same in powers of two, relative to `ref`
 struct Running2 {
   float m, ref, s, u;
 };
-template <int E>
+template <int N>
 __device__ __forceinline__ void take(Running2& r, const float* z, float most) {
   if (most > r.m) {
     // (logits of 2e38 make it infinite and those of -2e38 clamp it: nothing is summed)
@@ -130,22 +157,27 @@ __device__ __forceinline__ void take(Running2& r, const float* z, float most) {
     r.m = most;
     r.ref = ref;
   }
-  float s = 0.f, u = 0.f;
+  const uint64_t l = pair_of(kLog2e, kLog2e), ref = pair_of(-r.ref, -r.ref);
+  uint64_t s2 = 0, u2 = 0;
 #pragma unroll
-  for (int k = 0; k < E; ++k) {
-    const float d = fmaf(z[k], kLog2e, -r.ref), e = exp2_of(d);
-    s += e;
-    u = fmaf(e, d, u);
+  for (int k = 0; k < N; k += 2) {
+    const uint64_t d2 = fma2(pair_of(z[k], z[k + 1]), l, ref);
+    const float2 d = numbers(d2);
+    const uint64_t e2 = pair_of(exp2_of(d.x), exp2_of(d.y));
+    s2 = k ? add2(s2, e2) : e2;
+    u2 = k ? fma2(e2, d2, u2) : mul2(e2, d2);
   }
+  const float2 s = numbers(s2), us = numbers(u2);
+  float u = us.x + us.y;
   if (u != u) {  // e is 0 and d -inf somewhere (or something is NaN, which s is too)
     u = 0.f;
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
+    for (int k = 0; k < N; ++k) {
       const float d = fmaf(z[k], kLog2e, -r.ref);
       u = fmaf(exp2_of(d), fmaxf(d, -200.f), u);
     }
   }
-  r.s += s;
+  r.s += s.x + s.y;
   r.u += u;
 }
 
@@ -294,32 +326,99 @@ __device__ __forceinline__ RawVec<16> load_chunk(const T* z, int64_t at, int64_t
   return u.raw;
 }
 
-template <typename T>
-__device__ __forceinline__ float most_of(const RawVec<16>& raw, const float* v) {
+// (a NaN loses, to the other and to r.m)
+template <typename T, int CHUNKS>
+__device__ __forceinline__ float most_of(const RawVec<16>* raw) {
   if constexpr (sizeof(T) == 2) {
     using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
     union U {
-      RawVec<16> raw;
-      T2 e[4];
+      RawVec<16> raw[CHUNKS];
+      T2 e[4 * CHUNKS];
       __device__ U() {}
     } u;
-    u.raw = raw;
-    const T2 m = __hmax2(__hmax2(u.e[0], u.e[1]), __hmax2(u.e[2], u.e[3]));
-    return fmaxf(to_f32(m.x), to_f32(m.y));  // (a NaN loses, as it does below)
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) u.raw[i] = raw[i];
+    T2 m = u.e[0];
+#pragma unroll
+    for (int i = 1; i < 4 * CHUNKS; ++i) m = __hmax2(m, u.e[i]);
+    return fmaxf(to_f32(m.x), to_f32(m.y));
   } else {
-    return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      float v[4];
+      unpack_vec<4, float>(raw[i], v);
+      m = fmaxf(m, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+    }
+    return m;
   }
 }
 
-__device__ __forceinline__ void copy16_async(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
+// A thread's chunks of 16 bytes, STEP bytes apart, by way of its slots in shared memory.
+template <int THREADS>
+struct Ring {
+  uint32_t slots;
+  const char* next;
+  int left;  // chunks that have not been asked for
+  static constexpr int kSlot = THREADS * 16;
+
+  __device__ __forceinline__ void ask(int slot, bool there, int64_t ahead) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %2, 0;\n\t"
+        "@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(slots + slot * kSlot),
+        "l"(next + ahead), "r"((int)there)
+        : "memory");
+  }
+  __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  template <int STEP>
+  __device__ __forceinline__ void begin(void* smem, const void* first, int n) {
+    slots = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+    next = (const char*)first;
+    left = n;
+#pragma unroll
+    for (int i = 0; i < kLpRing; i += 2) {
+      ask(i, i < left, (int64_t)i * STEP);
+      ask(i + 1, i + 1 < left, (int64_t)(i + 1) * STEP);
+      commit();
+    }
+    left -= kLpRing;
+    next += (int64_t)kLpRing * STEP;
+  }
+  __device__ __forceinline__ RawVec<16> get(int slot) const {
+    RawVec<16> raw;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(raw.a.x), "=r"(raw.a.y), "=r"(raw.a.z), "=r"(raw.a.w)
+                 : "r"(slots + slot * kSlot)
+                 : "memory");
+    return raw;
+  }
+  // the n chunks go to `f` in twos: their number, they, whether there is a second
+  template <int STEP, typename F>
+  __device__ __forceinline__ void walk(int n, F f) {
+    for (int i0 = 0; i0 < n; i0 += kLpRing) {
+#pragma unroll
+      for (int i = 0; i < kLpRing; i += 2) {
+        if (i0 + i >= n) break;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kLpRing / 2 - 1) : "memory");
+        const RawVec<16> raw[2] = {get(i), get(i + 1)};
+        f(i0 + i, raw, i0 + i + 1 < n);
+        // (the slots have been read: their numbers have been used)
+        ask(i, i < left, (int64_t)i * STEP);
+        ask(i + 1, i + 1 < left, (int64_t)(i + 1) * STEP);
+        commit();
+      }
+      left -= kLpRing;
+      next += (int64_t)kLpRing * STEP;
+    }
+  }
+};
 
 template <typename T, bool TOP, int G>
 __global__ void __launch_bounds__(LpRow<G>::THREADS, G == 512 ? 2 : 8) logp_kernel(LpArgs a, int cluster) {
-  constexpr int E = LpChunk<T>::E, R = kLpRing;
+  constexpr int E = LpChunk<T>::E;
   using Row = LpRow<G>;
-  extern __shared__ __align__(16) uint8_t ring[];  // [R][threads][16]
+  extern __shared__ __align__(16) uint8_t ring[];  // [kLpRing][threads][16]
   __shared__ Row rows[Row::ROWS];
   const int t = threadIdx.x % G, lane = threadIdx.x & 31, warp = t >> 5;
   Row& mine = rows[threadIdx.x / G];
@@ -343,18 +442,8 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, G == 512 ? 2 : 8) logp_kern
 
   // this thread's chunks: from + t, and every G-th from there
   const int n = (int)max((int64_t)0, (to - from - t + G - 1) / G);
-  const T* next = z + ((from + t) * E - off);
-  uint32_t slot0;
-  slot0 = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
-  constexpr int kSlot = Row::THREADS * 16;
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (i < n) {
-      copy16_async(slot0 + i * kSlot, next);
-      next += G * E;
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  Ring<Row::THREADS> chunks;
+  chunks.template begin<G * 16>(ring, z + ((from + t) * E - off), n);
   Running2 r = {-INFINITY, 0.f, 0.f, 0.f};
   {
     const int64_t at = end_of(t);
@@ -362,30 +451,19 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, G == 512 ? 2 : 8) logp_kern
       const RawVec<16> raw = load_chunk<T>(z, at, a.V);
       float v[E];
       unpack_vec<E, T>(raw, v);
-      take<E>(r, v, most_of<T>(raw, v));
+      take<E>(r, v, most_of<T, 1>(&raw));
     }
   }
-  for (int i0 = 0; i0 < n; i0 += R) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (i0 + i >= n) break;
-      asm volatile("cp.async.wait_group %0;" ::"n"(R - 1) : "memory");
-      RawVec<16> raw;
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(raw.a.x), "=r"(raw.a.y), "=r"(raw.a.z), "=r"(raw.a.w)
-                   : "r"(slot0 + i * kSlot)
-                   : "memory");
-      float v[E];
-      unpack_vec<E, T>(raw, v);
-      take<E>(r, v, most_of<T>(raw, v));
-      // (the slot has been read: its numbers have been used)
-      if (i0 + i + R < n) {
-        copy16_async(slot0 + i * kSlot, next);
-        next += G * E;
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+  chunks.template walk<G * 16>(n, [&](int, const RawVec<16>* raw, bool two) {
+    float v[2 * E];
+    unpack_vec<E, T>(raw[0], v);
+    if (two) {
+      unpack_vec<E, T>(raw[1], v + E);
+      take<2 * E>(r, v, most_of<T, 2>(raw));
+    } else {
+      take<E>(r, v, most_of<T, 1>(raw));
     }
-  }
+  });
   const float most = r.m;
   Running sum = moved(r);
   if (r.s == 0.f && most > -INFINITY) {  // beyond fp32 times log2(e)
@@ -513,57 +591,112 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, G == 512 ? 2 : 8) logp_kern
 }
 
 // ---------------------------------------------------------------- backward
-// blockIdx.x: row, blockIdx.y: part of it
+// two numbers, rounded
 template <typename T>
-__global__ void __launch_bounds__(256) logp_bwd_kernel(LpBwdArgs a, int64_t share, int same) {
-  constexpr int E = LpChunk<T>::E, U = 4;
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+struct LpRowGrad {
+  float m, logs2, slope, rest, g;
+  int64_t t;  // place of the token, -1: none
+  bool empty;
+  __device__ __forceinline__ LpRowGrad(const LpBwdArgs& a, int64_t row) {
+    m = a.stats[3 * row];
+    const float logs = a.stats[3 * row + 1], h = a.stats[3 * row + 2];
+    const int64_t token = a.token[row];
+    t = token >= 0 && token < a.V ? token : -1;
+    g = t >= 0 && a.g_logp ? a.g_logp[a.one_logp ? 0 : row] : 0.f;
+    const float k = a.g_entropy ? a.g_entropy[a.one_entropy ? 0 : row] : 0.f;
+    logs2 = -logs * kLog2e;
+    slope = -k * kLn2;
+    rest = -fmaf(k, h, g);
+    // (a row without any probability has m = inf and no other number)
+    empty = m == INFINITY && logs == 0.f && h == 0.f;
+  }
+  // -p (g + k (log p + H)); p is 0 below 2^-126, where log p may be -inf
+  __device__ __forceinline__ float one(float z) const {
+    const float lp = fmaf(z - m, kLog2e, logs2);
+    return exp2_of(lp) * fmaf(fmaxf(lp, -300.f), slope, rest);
+  }
+  __device__ __forceinline__ float with_token(float d, int64_t at) const { return empty ? 0.f : at == t ? d + g : d; }
+};
+
+constexpr int kLpBwdThreads = 256;
+
+// blockIdx.x: row, blockIdx.y: part of it, of `share` whole chunks.  SAME: the
+// chunks of z and of dz lie on the same boundaries.
+template <typename T, bool SAME>
+__global__ void __launch_bounds__(kLpBwdThreads, 5) logp_bwd_kernel(LpBwdArgs a, int64_t share) {
+  constexpr int E = LpChunk<T>::E, G = kLpBwdThreads;
+  extern __shared__ __align__(16) uint8_t ring[];  // [kLpRing][threads][16]
   const int64_t row = blockIdx.x;
   const T* z = (const T*)a.z + row * a.ldz;
   T* dz = (T*)a.dz + row * a.V;
-  const int64_t t = a.token[row];
-  const float m = a.stats[3 * row], logs = a.stats[3 * row + 1], h = a.stats[3 * row + 2];
-  const bool given = t >= 0 && t < a.V;
-  const float g = given && a.g_logp ? a.g_logp[a.one_logp ? 0 : row] : 0.f;
-  const float k = a.g_entropy ? a.g_entropy[a.one_entropy ? 0 : row] : 0.f;
-  // (a row without any probability has m = inf and no other number)
-  const bool empty = m == INFINITY && logs == 0.f && h == 0.f;
-  const float logs2 = -logs * kLog2e, slope = -k * kLn2, rest = -fmaf(k, h, g);
-  // -p (g + k (log p + H)); p is 0 below 2^-126, where log p may be -inf
-  auto one = [&](float zz) {
-    const float lp = fmaf(zz - m, kLog2e, logs2), p = exp2_of(lp);
-    return p * fmaf(fmaxf(lp, -300.f), slope, rest);
-  };
-  auto with_token = [&](float d, int64_t at) { return empty ? 0.f : at == t && given ? d + g : d; };
+  if (!SAME) {  // element by element
+    const LpRowGrad r(a, row);
+    const int64_t end = min(a.V, (blockIdx.y + 1) * share * E);
+    for (int64_t i = blockIdx.y * share * E + threadIdx.x; i < end; i += G)
+      dz[i] = from_f32<T>(r.with_token(r.one(to_f32(z[i])), i));
+    return;
+  }
   const int off = (int)(((uintptr_t)dz & 15) / sizeof(T));
-  const int64_t chunks = (a.V + off + E - 1) / E;
-  const int64_t to = min(chunks, (blockIdx.y + 1) * share);
-  for (int64_t c0 = blockIdx.y * share + threadIdx.x; c0 < to; c0 += U * 256) {
-    RawVec<16> raw[U];
+  const int64_t lo = off ? 1 : 0, hi = max(lo, (a.V + off) / E);
+  const int64_t from = min(hi, lo + blockIdx.y * share), to = min(hi, from + share);
+  const int n = (int)max((int64_t)0, (to - from - threadIdx.x + G - 1) / G);
+  const int64_t first = (from + threadIdx.x) * E - off;
+  Ring<G> chunks;
+  chunks.template begin<G * 16>(ring, z + first, n);
+  const LpRowGrad r(a, row);
+  // the chunk with the token, if it is this thread's
+  int token_at = -1;
+  const int64_t rel = r.t >= 0 ? (r.t + off) / E - from - threadIdx.x : -1;
+  if (rel >= 0 && rel % G == 0 && rel / G < n) token_at = (int)(rel / G);
+  const uint64_t l = pair_of(kLog2e, kLog2e), m2 = pair_of(-r.m, -r.m), logs2 = pair_of(r.logs2, r.logs2),
+                 slope = pair_of(r.slope, r.slope), rest = pair_of(r.rest, r.rest);
+  T* out = dz + first;
+  chunks.template walk<G * 16>(n, [&](int i, const RawVec<16>* raw, bool two) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int64_t at = (c0 + i * 256) * E - off;
-      if (same && c0 + i * 256 < to && at >= 0 && at + E <= a.V) raw[i] = *reinterpret_cast<const RawVec<16>*>(z + at);
-    }
+    for (int c = 0; c < 2; ++c) {
+      if (c && !two) break;
+      float v[E];
+      unpack_vec<E, T>(raw[c], v);
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (c0 + i * 256 >= to) break;
-      const int64_t at = (c0 + i * 256) * E - off;
-      if (same && at >= 0 && at + E <= a.V) {
-        float v[E];
-        unpack_vec<E, T>(raw[i], v);
+      for (int j = 0; j < E; j += 2) {
+        const float2 lp = numbers(fma2(add2(pair_of(v[j], v[j + 1]), m2), l, logs2));
+        const uint64_t w = fma2(pair_of(fmaxf(lp.x, -300.f), fmaxf(lp.y, -300.f)), slope, rest);
+        const float2 d = numbers(mul2(pair_of(exp2_of(lp.x), exp2_of(lp.y)), w));
+        v[j] = d.x;
+        v[j + 1] = d.y;
+      }
+      T* to = out + (int64_t)(i + c) * (G * E);
+      if (r.empty || i + c == token_at) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = one(v[j]);
-        if (empty || (uint64_t)(t - at) < E) {
-#pragma unroll
-          for (int j = 0; j < E; ++j) v[j] = with_token(v[j], at + j);
-        }
-        store_vec<E>(dz + at, v);
+        for (int j = 0; j < E; ++j) v[j] = r.with_token(v[j], (to - dz) + j);
+      }
+      if constexpr (sizeof(T) == 4) {
+        store_vec<4>(to, v);
       } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (at + j >= 0 && at + j < a.V) dz[at + j] = from_f32<T>(with_token(one(to_f32(z[at + j])), at + j));
+        uint4 q;
+        q.x = pack2<T>(v[0], v[1]);
+        q.y = pack2<T>(v[2], v[3]);
+        q.z = pack2<T>(v[4], v[5]);
+        q.w = pack2<T>(v[6], v[7]);
+        *reinterpret_cast<uint4*>(to) = q;
       }
     }
+  });
+  // the ends
+  if (threadIdx.x < E) {
+    const int64_t head = (int64_t)threadIdx.x - off, tail = hi * E - off + threadIdx.x;
+    if (blockIdx.y == 0 && off && head >= 0 && head < a.V) dz[head] = from_f32<T>(r.with_token(r.one(to_f32(z[head])), head));
+    if (blockIdx.y == gridDim.y - 1 && tail < a.V) dz[tail] = from_f32<T>(r.with_token(r.one(to_f32(z[tail])), tail));
   }
 }
 
@@ -616,18 +749,28 @@ static int launch_lp(const LpArgs& a, cudaStream_t s) {
   return launch_lp_as<T, TOP, 512>(a, cluster, s);
 }
 
+template <typename T, bool SAME>
+static int launch_lp_bwd_as(const LpBwdArgs& a, int64_t share, int64_t parts, cudaStream_t s) {
+  constexpr int smem = kLpRing * kLpBwdThreads * 16;
+  static DeviceOnce once;
+  PVB2_TRY(allow_smem(logp_bwd_kernel<T, SAME>, smem, once));
+  logp_bwd_kernel<T, SAME><<<dim3((unsigned)a.N, (unsigned)parts), kLpBwdThreads, SAME ? smem : 0, s>>>(a, share);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
 template <typename T>
 static int launch_lp_bwd(const LpBwdArgs& a, cudaStream_t s) {
   constexpr int E = LpChunk<T>::E;
-  // parts of 8 rounds of a block, fewer where the rows alone do not fill the SMs
-  const int64_t chunks = (a.V + 2 * E - 2) / E;
-  int64_t share = 8 * 4 * 256;
-  while (share > 256 && a.N * ((chunks + share - 1) / share) < 4 * (int64_t)num_sms()) share /= 2;
-  share = std::max(share, (chunks + 65534) / 65535);
-  const int same = ((uintptr_t)a.z & 15) == ((uintptr_t)a.dz & 15) && (a.N <= 1 || (a.ldz - a.V) * (int64_t)sizeof(T) % 16 == 0);
-  logp_bwd_kernel<T><<<dim3((unsigned)a.N, (unsigned)((chunks + share - 1) / share)), 256, 0, s>>>(a, share, same);
-  PVB2_LAUNCH_CHECK();
-  return PVB2_OK;
+  // parts of 32 chunks for each thread, fewer where the rows alone do not fill the SMs
+  const int64_t chunks = (a.V + E - 1) / E;
+  int64_t share = 32 * kLpBwdThreads;
+  while (share > kLpBwdThreads && a.N * ((chunks + share - 1) / share) < 5 * (int64_t)num_sms()) share /= 2;
+  const int64_t parts = std::min<int64_t>(65535, (chunks + share - 1) / share);
+  share = (chunks + parts - 1) / parts;
+  if (((uintptr_t)a.z & 15) == ((uintptr_t)a.dz & 15) && (a.N <= 1 || (a.ldz - a.V) * (int64_t)sizeof(T) % 16 == 0))
+    return launch_lp_bwd_as<T, true>(a, share, parts, s);
+  return launch_lp_bwd_as<T, false>(a, share, parts, s);
 }
 
 }  // namespace pvb2
