@@ -17,7 +17,7 @@
 //
 // Each thread copies its chunks of 16 bytes into a ring of its own in shared
 // memory, eight ahead, without barriers: registers for as many loads in flight
-// would halve the threads.  A row is a warp's, a block's of 128 or 512, or, where
+// would halve the threads.  A row is a warp's, a block's of 128 or 256, or, where
 // rows are few, a cluster's, whose blocks join through shared memory: one
 // launch, no workspace.
 //
@@ -415,7 +415,7 @@ struct Ring {
 };
 
 template <typename T, bool TOP, int G>
-__global__ void __launch_bounds__(LpRow<G>::THREADS, G == 512 ? 2 : 8) logp_kernel(LpArgs a, int cluster) {
+__global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) logp_kernel(LpArgs a, int cluster) {
   constexpr int E = LpChunk<T>::E;
   using Row = LpRow<G>;
   extern __shared__ __align__(16) uint8_t ring[];  // [kLpRing][threads][16]
@@ -739,14 +739,24 @@ static int launch_lp_as(const LpArgs& a, int cluster, cudaStream_t s) {
 template <typename T, bool TOP>
 static int launch_lp(const LpArgs& a, cudaStream_t s) {
   const int64_t bytes = a.V * (int64_t)sizeof(T);
-  // Rows of up to eight chunks for each of their threads are a warp's, or 128
-  // threads'; where they leave SMs without a row, more threads' and, while each
-  // block keeps 16 KB, several blocks'.
-  if (bytes <= 4096 && (a.N >= num_sms() || bytes <= 1024)) return launch_lp_as<T, TOP, 32>(a, 1, s);
-  if (bytes <= 32768 && (a.N >= num_sms() || bytes <= 8192)) return launch_lp_as<T, TOP, 128>(a, 1, s);
-  int cluster = 1;
-  while (cluster < kLpCluster && a.N * cluster < num_sms() && bytes / (2 * cluster) >= 16384) cluster *= 2;
-  return launch_lp_as<T, TOP, 512>(a, cluster, s);
+  if (a.N < num_sms()) {
+    // fewer rows than SMs: more threads to a row, and several blocks, while there
+    // are SMs for them and each keeps 16 KB
+    if (bytes <= 1024) return launch_lp_as<T, TOP, 32>(a, 1, s);
+    if (bytes <= 10240) return launch_lp_as<T, TOP, 128>(a, 1, s);
+    int cluster = 1;
+    while (cluster < kLpCluster && a.N * cluster * 2 <= num_sms() && bytes / (2 * cluster) >= 16384) cluster *= 2;
+    return launch_lp_as<T, TOP, 256>(a, cluster, s);
+  }
+  // Short rows a warp's, since a block's joins take longer than the row; long ones
+  // few threads' all the same, so that many rows begin and end at different
+  // times (us for a warp, 128, 256 and 512 threads: 16384 x 1000 bf16 17, 44,
+  // 81, 168; 8192 x 10000 34, 45, 68, 122, with 20 alternatives 97, 83, 111, 206;
+  // 4096 x 49999 79, 72, 81, 112; 2048 x 131072 with 5 alternatives 235, 115,
+  // 105, 123).
+  if (bytes <= (TOP ? 10240 : 20480)) return launch_lp_as<T, TOP, 32>(a, 1, s);
+  if (bytes <= 160 * 1024) return launch_lp_as<T, TOP, 128>(a, 1, s);
+  return launch_lp_as<T, TOP, 256>(a, 1, s);
 }
 
 template <typename T, bool SAME>

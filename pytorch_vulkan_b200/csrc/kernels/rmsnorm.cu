@@ -22,6 +22,8 @@
 // warp still reads consecutive ones and 128 of them, a group of one scale, are
 // a warp's.
 #include <algorithm>
+#include <atomic>
+#include <initializer_list>
 #include "quant8.cuh"
 
 namespace pvb2 {
@@ -88,20 +90,17 @@ struct Chunk {
 template <typename T, bool VEC>
 struct alignas(16) AChunk : Chunk<T, VEC> {};
 
-// Sum over the G threads of a row, in a fixed order; all of them get it.
-// `line`: one number per warp of the block.
-template <int G, typename A>
+// Sum over the threads of a row, a warp or a block, in a fixed order; all of
+// them get it.  `line`: one number per warp, that nobody reads any more.
+template <bool WARP, typename A>
 __device__ __forceinline__ A row_sum(A v, A* line) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  if (G > 32) {
-    const int warp = threadIdx.x >> 5;
-    __syncthreads();  // the last sum has been read
-    if ((threadIdx.x & 31) == 0) line[warp] = v;
+  if (!WARP) {
+    if ((threadIdx.x & 31) == 0) line[threadIdx.x >> 5] = v;
     __syncthreads();
     v = line[0];
-#pragma unroll
-    for (int i = 1; i < G / 32; ++i) v += line[i];
+    for (int i = 1; i < (int)blockDim.x / 32; ++i) v += line[i];
   }
   return v;
 }
@@ -168,13 +167,13 @@ __device__ __forceinline__ void load_sum(const NormArgs& a, int64_t row, int c, 
   }
 }
 
-// G threads share a row and keep NV chunks each; blocks of max(G, 128)
-template <typename T, bool VEC, int G, int NV, int MODE>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_kernel(NormArgs a) {
+// A warp (WARP; blocks of four) or a block shares a row, each thread keeps NV chunks.
+template <typename T, bool VEC, bool WARP, int NV, int MODE>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
   using C = Chunk<T, VEC>;
-  __shared__ double line[G / 32];
-  const int t = threadIdx.x % G;
-  const int64_t row = (int64_t)blockIdx.x * (G < 128 ? 128 / G : 1) + threadIdx.x / G;
+  __shared__ double line[32];
+  const int G = WARP ? 32 : (int)blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
   if (row >= a.rows) return;  // whole warps: only where a warp has a row of its own
   AChunk<T, VEC> h[NV];
 #pragma unroll
@@ -189,7 +188,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_kernel(NormArgs a) {
         const double v = to_f32(h[i].e[k]);
         q = fma(v, v, q);
       }
-    rstd = rstd_of(row_sum<G>(q, line), a.D, a.eps);
+    rstd = rstd_of(row_sum<WARP>(q, line), a.D, a.eps);
     if (a.rstd && t == 0) a.rstd[row] = rstd;
   }
   const T* w = MODE == kQuant8 ? nullptr : (const T*)a.w;
@@ -234,7 +233,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
         q = fma(v, v, q);
       }
     }
-    rstd = rstd_of(row_sum<1024>(q, line), a.D, a.eps);
+    rstd = rstd_of(row_sum<false>(q, line), a.D, a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
   }
   // the sum that this thread wrote, or x
@@ -268,7 +267,7 @@ template <typename T, bool VEC, int G, int NV>
 __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(NormBwdArgs a) {
   using C = Chunk<T, VEC>;
   constexpr int kRows = G < 128 ? 128 / G : 1;  // of a block
-  __shared__ float line[G / 32];
+  __shared__ float line[2][32];
   extern __shared__ float share[];  // kRows > 1: dw of the rows' warps
   const int t = threadIdx.x % G, mine = threadIdx.x / G;
   AChunk<T, VEC> w[NV];
@@ -282,12 +281,14 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(NormBwdArgs
       if (!a.w) w[i].e[k] = from_f32<T>(1.f);
     }
   }
-  for (int64_t row = (int64_t)blockIdx.x * kRows + mine; row < a.rows; row += (int64_t)gridDim.x * kRows) {
-    AChunk<T, VEC> h[NV], g[NV];
+  int parity = 0;
+  for (int64_t row = (int64_t)blockIdx.x * kRows + mine; row < a.rows; row += (int64_t)gridDim.x * kRows, parity ^= 1) {
+    AChunk<T, VEC> h[NV], g[NV], gh[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       h[i].load((const T*)a.h + row * a.ldh, i * G + t, a.D);
       g[i].load((const T*)a.gy + row * a.ldg, i * G + t, a.D);
+      if (a.gh) gh[i].load((const T*)a.gh + row * a.ldgh, i * G + t, a.D);
     }
     const float rstd = a.rstd[row];
     float dot = 0.f;
@@ -300,20 +301,18 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(NormBwdArgs
         dw[i][k] = fmaf(gv, n, dw[i][k]);
       }
     if (!a.dx) continue;
-    const float mean = row_sum<G>(dot, line) / (float)a.D;
+    const float mean = row_sum<G == 32>(dot, line[parity]) / (float)a.D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = i * G + t;
-      AChunk<T, VEC> gh, out;
-      if (a.gh) gh.load((const T*)a.gh + row * a.ldgh, c, a.D);
+      AChunk<T, VEC> out;
 #pragma unroll
       for (int k = 0; k < C::E; ++k) {
         const float n = to_f32(h[i].e[k]) * rstd;
         float d = fmaf(-n, mean, to_f32(g[i].e[k]) * to_f32(w[i].e[k])) * rstd;
-        if (a.gh) d += to_f32(gh.e[k]);
+        if (a.gh) d += to_f32(gh[i].e[k]);
         out.e[k] = from_f32<T>(d);
       }
-      out.store((T*)a.dx + row * a.D, c, a.D);
+      out.store((T*)a.dx + row * a.D, i * G + t, a.D);
     }
   }
   if (!a.partial) return;
@@ -371,7 +370,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
       }
       if (pass) out.store((T*)a.dx + row * a.D, c, a.D);
     }
-    if (!pass) mean = row_sum<1024>(dot, line) / (float)a.D;
+    if (!pass) mean = row_sum<false>(dot, line) / (float)a.D;
   }
 }
 
@@ -393,8 +392,17 @@ __global__ void __launch_bounds__(1024) norm_dw_sum_kernel(const float* partial,
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t j = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (j < D)
-    for (int p = y; p < count; p += 32) s += partial[(int64_t)p * D + j];
+  if (j < D) {
+    int p = y;
+    for (; p + 7 * 32 < count; p += 8 * 32) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = partial[(int64_t)(p + 32 * i) * D + j];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    for (; p < count; p += 32) s += partial[(int64_t)p * D + j];
+  }
   part[y][lane] = s;
   __syncthreads();
   s = part[lane][y];
@@ -438,16 +446,16 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const T* x, int64_t row
     }
 }
 
-// values of codes: 8 consecutive ones a thread (VEC), or one
+// values of codes: 8 consecutive ones a thread (VEC), or one; blockIdx.x: part of
+// a row, blockIdx.y: which rows
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* codes, const float* scales, T* out, int64_t rows, int D,
                                                       int64_t ldc, int groups, int tall) {
   constexpr int E = VEC ? 8 : 1;
-  const int wide = (D + E - 1) / E;
-  const int64_t total = rows * wide;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / wide;
-    const int c = (int)(i - row * wide) * E;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * E;
+  if (c >= D) return;
+#pragma unroll 4
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     const float s = scales[(tall ? row / 128 : row) * groups + c / kGroup8];
     if (VEC) {
       const uint2 q = *reinterpret_cast<const uint2*>(codes + row * ldc + c);
@@ -492,15 +500,14 @@ template <typename T, bool VEC, int MODE>
 static int launch_norm(const NormArgs& a, cudaStream_t s) {
   const int chunks = (a.D + Chunk<T, VEC>::E - 1) / Chunk<T, VEC>::E;
   const unsigned rows = (unsigned)a.rows;
-  // as few threads a row as keep it in four chunks each: a warp needs no barrier
-  if (chunks <= 32) norm_kernel<T, VEC, 32, 1, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
-  else if (chunks <= 64) norm_kernel<T, VEC, 32, 2, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
-  else if (chunks <= 128) norm_kernel<T, VEC, 32, 4, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
-  else if (chunks <= 256) norm_kernel<T, VEC, 128, 2, MODE><<<rows, 128, 0, s>>>(a);
-  else if (chunks <= 512) norm_kernel<T, VEC, 128, 4, MODE><<<rows, 128, 0, s>>>(a);
-  else if (chunks <= 1024) norm_kernel<T, VEC, 256, 4, MODE><<<rows, 256, 0, s>>>(a);
-  else if (chunks <= 2048) norm_kernel<T, VEC, 512, 4, MODE><<<rows, 512, 0, s>>>(a);
-  else if (chunks <= 4096) norm_kernel<T, VEC, 1024, 4, MODE><<<rows, 1024, 0, s>>>(a);
+  // a warp where it keeps a row in four chunks a thread, since it needs no
+  // barrier; else as many threads as the row needs
+  auto threads = [&](int nv) { return (unsigned)(((chunks + nv - 1) / nv + 31) / 32 * 32); };
+  if (chunks <= 32) norm_kernel<T, VEC, true, 1, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
+  else if (chunks <= 64) norm_kernel<T, VEC, true, 2, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
+  else if (chunks <= 128) norm_kernel<T, VEC, true, 4, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
+  else if (chunks <= 512) norm_kernel<T, VEC, false, 2, MODE><<<rows, threads(2), 0, s>>>(a);
+  else if (chunks <= 4096) norm_kernel<T, VEC, false, 4, MODE><<<rows, threads(4), 0, s>>>(a);
   else norm_long_kernel<T, VEC, MODE><<<rows, 1024, 0, s>>>(a);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
@@ -538,9 +545,9 @@ static bool norm_vec(const NormArgs& a, int dtype) {
          (!a.codes || (((uintptr_t)a.codes & 7) == 0 && (a.rows <= 1 || a.ldc % 8 == 0)));
 }
 
-// blocks of the backward pass that keep a share of dw: two full SMs' worth of
-// threads each, and 16 rows a block at least, so that the shares are few
-// beside the rows
+// Blocks of the backward pass, each of which keeps a share of dw: as many as the
+// workspace is for, and no more than are resident (a second wave of a few blocks
+// would take as long as the first).
 struct NormBwdPlan {
   int threads, rows_per_block;  // threads of a row (0: long rows)
   int64_t blocks;
@@ -558,32 +565,54 @@ static NormBwdPlan bwd_plan(const pvb2_rms_norm_desc* d, bool vec) {
   return p;
 }
 
+// resident blocks of a kernel on an SM, asked for once
+template <typename K>
+static int resident(K kernel, int threads, int smem, std::atomic<int>& known) {
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+template <typename T, bool VEC, int G, int NV>
+static int launch_bwd_as(const NormBwdArgs& a, NormBwdPlan& p, cudaStream_t s) {
+  constexpr int threads = G < 128 ? 128 : G, smem = G < 128 ? 4 * NV * G * Chunk<T, VEC>::E * 4 : 0;
+  static std::atomic<int> known{0};
+  auto kernel = norm_bwd_kernel<T, VEC, G, NV>;
+  p.blocks = std::min<int64_t>(p.blocks, (int64_t)num_sms() * resident(kernel, threads, smem, known));
+  kernel<<<(unsigned)p.blocks, threads, smem, s>>>(a);
+  PVB2_LAUNCH_CHECK();
+  return PVB2_OK;
+}
+
 template <typename T, bool VEC>
-static int launch_bwd(const NormBwdArgs& a, const NormBwdPlan& p, cudaStream_t s) {
+static int launch_bwd(const NormBwdArgs& a, NormBwdPlan& p, cudaStream_t s) {
   constexpr int E = Chunk<T, VEC>::E;
   const int chunks = (a.D + E - 1) / E;
-  const unsigned grid = (unsigned)p.blocks;
-  if (chunks <= 32) norm_bwd_kernel<T, VEC, 32, 1><<<grid, 128, 4 * 32 * E * 4, s>>>(a);
-  else if (chunks <= 64) norm_bwd_kernel<T, VEC, 32, 2><<<grid, 128, 4 * 64 * E * 4, s>>>(a);
-  else if (chunks <= 128) norm_bwd_kernel<T, VEC, 128, 1><<<grid, 128, 0, s>>>(a);
-  else if (chunks <= 256) norm_bwd_kernel<T, VEC, 128, 2><<<grid, 128, 0, s>>>(a);
-  else if (chunks <= 512) norm_bwd_kernel<T, VEC, 256, 2><<<grid, 256, 0, s>>>(a);
-  else if (chunks <= 1024) norm_bwd_kernel<T, VEC, 512, 2><<<grid, 512, 0, s>>>(a);
-  else if (chunks <= 2048) norm_bwd_kernel<T, VEC, 1024, 2><<<grid, 1024, 0, s>>>(a);
-  else {
-    if (a.dx) {
-      norm_bwd_long_kernel<T, VEC><<<(unsigned)a.rows, 1024, 0, s>>>(a);
-      PVB2_LAUNCH_CHECK();
-    }
-    if (!a.partial) return PVB2_OK;
-    norm_dw_columns_kernel<T><<<dim3((unsigned)((a.D + 255) / 256), grid), 256, 0, s>>>(a);
+  if (chunks <= 32) return launch_bwd_as<T, VEC, 32, 1>(a, p, s);
+  if (chunks <= 64) return launch_bwd_as<T, VEC, 32, 2>(a, p, s);
+  if (chunks <= 128) return launch_bwd_as<T, VEC, 128, 1>(a, p, s);
+  if (chunks <= 256) return launch_bwd_as<T, VEC, 128, 2>(a, p, s);
+  if (chunks <= 512) return launch_bwd_as<T, VEC, 256, 2>(a, p, s);
+  if (chunks <= 1024) return launch_bwd_as<T, VEC, 512, 2>(a, p, s);
+  if (chunks <= 2048) return launch_bwd_as<T, VEC, 1024, 2>(a, p, s);
+  if (a.dx) {
+    norm_bwd_long_kernel<T, VEC><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    PVB2_LAUNCH_CHECK();
   }
+  if (!a.partial) return PVB2_OK;
+  norm_dw_columns_kernel<T><<<dim3((unsigned)((a.D + 255) / 256), (unsigned)p.blocks), 256, 0, s>>>(a);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
 
 template <typename T>
-static int run_bwd(const NormBwdArgs& a, const NormBwdPlan& p, bool vec, void* dw, cudaStream_t s) {
+static int run_bwd(const NormBwdArgs& a, NormBwdPlan p, bool vec, void* dw, cudaStream_t s) {
   if (a.rows) PVB2_TRY((vec ? launch_bwd<T, true>(a, p, s) : launch_bwd<T, false>(a, p, s)));
   if (!dw) return PVB2_OK;
   norm_dw_sum_kernel<T><<<(unsigned)((a.D + 31) / 32), 1024, 0, s>>>(a.partial, a.rows ? (int)p.blocks : 0, a.D, (T*)dw);
@@ -707,7 +736,9 @@ int pvb2_dequantize_8bit(int64_t rows, int64_t D, const uint8_t* codes, int64_t 
   const bool vec = D % 8 == 0 && ((uintptr_t)codes & 7) == 0 && (rows <= 1 || ldc % 8 == 0) && ((uintptr_t)out & 15) == 0 &&
                    D * size % 16 == 0;
   cudaStream_t s = as_stream(stream);
-  const int grid = grid_for(rows * (vec ? D / 8 : D), 256, 8);
+  const unsigned wide = (unsigned)((D / (vec ? 8 : 1) + 255) / 256);
+  // four rows a block, while that leaves each SM eight blocks
+  const dim3 grid(wide, (unsigned)std::min<int64_t>(65535, std::max<int64_t>((rows + 3) / 4, std::min<int64_t>(rows, num_sms() * 8 / wide))));
   auto go = [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
     if (vec) dequant_kernel<T, true><<<grid, 256, 0, s>>>(codes, scales, p, rows, (int)D, ldc, groups, tall);
