@@ -7,9 +7,9 @@
 //   backward, with a = gy w:  dh = rstd (a - n mean(a n)) + gh;   dw = sum over rows of gy n
 //
 // One pass over the data: a row's elements stay in the registers of the
-// threads that share it (a warp up to 1024 16-bit elements, a block of up to
-// 1024 threads beyond) between the sum and the output, so every kernel here is
-// bound by HBM.  Longer rows are read twice, the second time out of L2.
+// threads that share it (a warp up to 1024 16-bit elements, a block beyond)
+// between the sum and the output, so every kernel here is bound by HBM.  Rows of
+// more than 32768 16-bit elements are read twice, the second time out of L2.
 //
 // The mean of squares is summed in 64 bits and rounded once, root and quotient
 // are the IEEE ones, and n and y are rounded products: a code of the 8-bit
@@ -42,6 +42,7 @@ struct NormArgs {
   int64_t rows, ldx, ldr, ldc;
   int D, groups;
   float eps;
+  double per_element;  // 1 / D
 };
 
 struct NormBwdArgs {
@@ -97,28 +98,40 @@ __device__ __forceinline__ A row_sum(A v, A* line) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   if (!WARP) {
+    const int warps = blockDim.x / 32;
     if ((threadIdx.x & 31) == 0) line[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = line[0];
-    for (int i = 1; i < (int)blockDim.x / 32; ++i) v += line[i];
+    // (eight loads at once, where a loop would wait for each)
+    A part[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[i] = i < warps ? line[i] : A(0);
+    v = part[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += part[i];
+    for (int i = 8; i < warps; ++i) v += line[i];
   }
   return v;
 }
 
-__device__ __forceinline__ float rstd_of(double squares, int D, float eps) {
-  return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn((float)(squares / (double)D), eps)));
+__device__ __forceinline__ float rstd_of(double squares, double per_element, float eps) {
+  return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn((float)(squares * per_element), eps)));
+}
+
+// the weight's numbers, or ones
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_weight(AChunk<T, VEC>& w, const void* p, int c, int D) {
+  if (p) {
+    w.load((const T*)p, c, D);
+  } else {
+#pragma unroll
+    for (int k = 0; k < Chunk<T, VEC>::E; ++k) w.e[k] = from_f32<T>(1.f);
+  }
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void scale_row(const AChunk<T, VEC>& h, const T* w, int c, int D, float rstd, float* y) {
-  constexpr int E = Chunk<T, VEC>::E;
-  AChunk<T, VEC> cw;
-  if (w) cw.load(w, c, D);
+__device__ __forceinline__ void scale_row(const AChunk<T, VEC>& h, const AChunk<T, VEC>& w, float rstd, float* y) {
 #pragma unroll
-  for (int k = 0; k < E; ++k) {
-    y[k] = __fmul_rn(to_f32(h.e[k]), rstd);
-    if (w) y[k] = __fmul_rn(y[k], to_f32(cw.e[k]));
-  }
+  for (int k = 0; k < Chunk<T, VEC>::E; ++k) y[k] = __fmul_rn(__fmul_rn(to_f32(h.e[k]), rstd), to_f32(w.e[k]));
 }
 
 // the group's scale and this chunk's codes
@@ -154,20 +167,17 @@ __device__ __forceinline__ void put_codes(const float* y, uint8_t* row, float* s
   }
 }
 
-// h of a chunk, stored where there is a residual
+// h of a chunk: x, or x + r, which is stored
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_sum(const NormArgs& a, int64_t row, int c, AChunk<T, VEC>& h) {
-  h.load((const T*)a.x + row * a.ldx, c, a.D);
-  if (a.r) {
-    AChunk<T, VEC> r;
-    r.load((const T*)a.r + row * a.ldr, c, a.D);
+__device__ __forceinline__ void form_sum(const NormArgs& a, int64_t row, int c, AChunk<T, VEC>& x, const AChunk<T, VEC>& r) {
+  if (!a.r) return;
 #pragma unroll
-    for (int k = 0; k < Chunk<T, VEC>::E; ++k) h.e[k] = from_f32<T>(to_f32(h.e[k]) + to_f32(r.e[k]));
-    h.store((T*)a.sum + row * a.D, c, a.D);
-  }
+  for (int k = 0; k < Chunk<T, VEC>::E; ++k) x.e[k] = from_f32<T>(to_f32(x.e[k]) + to_f32(r.e[k]));
+  x.store((T*)a.sum + row * a.D, c, a.D);
 }
 
-// A warp (WARP; blocks of four) or a block shares a row, each thread keeps NV chunks.
+// A warp (WARP; blocks of four) or a block shares a row, each thread keeps NV
+// chunks of it.
 template <typename T, bool VEC, bool WARP, int NV, int MODE>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
   using C = Chunk<T, VEC>;
@@ -176,8 +186,17 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
   const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
   if (row >= a.rows) return;  // whole warps: only where a warp has a row of its own
   AChunk<T, VEC> h[NV];
+  {
+    AChunk<T, VEC> r[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) load_sum(a, row, i * G + t, h[i]);
+    for (int i = 0; i < NV; ++i) h[i].load((const T*)a.x + row * a.ldx, i * G + t, a.D);
+    if (a.r) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) r[i].load((const T*)a.r + row * a.ldr, i * G + t, a.D);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) form_sum(a, row, i * G + t, h[i], r[i]);
+  }
   float rstd = 1.f;
   if (MODE != kQuant8) {
     double q = 0;
@@ -188,10 +207,9 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
         const double v = to_f32(h[i].e[k]);
         q = fma(v, v, q);
       }
-    rstd = rstd_of(row_sum<WARP>(q, line), a.D, a.eps);
+    rstd = rstd_of(row_sum<WARP>(q, line), a.per_element, a.eps);
     if (a.rstd && t == 0) a.rstd[row] = rstd;
   }
-  const T* w = MODE == kQuant8 ? nullptr : (const T*)a.w;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = i * G + t;
@@ -200,7 +218,9 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
 #pragma unroll
       for (int k = 0; k < C::E; ++k) y[k] = to_f32(h[i].e[k]);
     } else {
-      scale_row<T, VEC>(h[i], w, c, a.D, rstd, y);
+      AChunk<T, VEC> w;
+      load_weight(w, a.w, c, a.D);
+      scale_row(h[i], w, rstd, y);
     }
     if (MODE == kNorm) {
       AChunk<T, VEC> out;
@@ -225,15 +245,17 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
   if (MODE != kQuant8) {
     double q = 0;
     for (int c = threadIdx.x; c < chunks; c += 1024) {
-      AChunk<T, VEC> h;
-      load_sum(a, row, c, h);
+      AChunk<T, VEC> h, r;
+      h.load((const T*)a.x + row * a.ldx, c, a.D);
+      if (a.r) r.load((const T*)a.r + row * a.ldr, c, a.D);
+      form_sum(a, row, c, h, r);
 #pragma unroll
       for (int k = 0; k < C::E; ++k) {
         const double v = to_f32(h.e[k]);
         q = fma(v, v, q);
       }
     }
-    rstd = rstd_of(row_sum<false>(q, line), a.D, a.eps);
+    rstd = rstd_of(row_sum<false>(q, line), a.per_element, a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
   }
   // the sum that this thread wrote, or x
@@ -246,7 +268,9 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
 #pragma unroll
       for (int k = 0; k < C::E; ++k) y[k] = to_f32(h.e[k]);
     } else {
-      scale_row<T, VEC>(h, (const T*)a.w, c, a.D, rstd, y);
+      AChunk<T, VEC> w;
+      load_weight(w, a.w, c, a.D);
+      scale_row(h, w, rstd, y);
     }
     if (MODE == kNorm) {
       AChunk<T, VEC> out;
@@ -264,7 +288,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
 // once for both gradients.  The blocks' shares are summed by a second launch,
 // in a fixed order.
 template <typename T, bool VEC, int G, int NV>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(NormBwdArgs a) {
+__global__ void __launch_bounds__(G < 128 ? 128 : G, (sizeof(T) == 4 ? 1024 : G == 1024 ? 1024 : 768) / (G < 128 ? 128 : G)) norm_bwd_kernel(NormBwdArgs a) {
   using C = Chunk<T, VEC>;
   constexpr int kRows = G < 128 ? 128 / G : 1;  // of a block
   __shared__ float line[2][32];
@@ -274,12 +298,9 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(NormBwdArgs
   float dw[NV][C::E];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (a.w) w[i].load((const T*)a.w, i * G + t, a.D);
+    load_weight(w[i], a.w, i * G + t, a.D);
 #pragma unroll
-    for (int k = 0; k < C::E; ++k) {
-      dw[i][k] = 0.f;
-      if (!a.w) w[i].e[k] = from_f32<T>(1.f);
-    }
+    for (int k = 0; k < C::E; ++k) dw[i][k] = 0.f;
   }
   int parity = 0;
   for (int64_t row = (int64_t)blockIdx.x * kRows + mine; row < a.rows; row += (int64_t)gridDim.x * kRows, parity ^= 1) {
@@ -385,30 +406,33 @@ __global__ void __launch_bounds__(256) norm_dw_columns_kernel(NormBwdArgs a) {
   a.partial[(int64_t)blockIdx.y * a.D + j] = s;
 }
 
-// dw[j] = sum of the shares, 32 columns a block, in a fixed order
+// dw[j] = sum of the shares, eight columns a block (a sector of each share), in
+// a fixed order: a thread every 128th, then the threads of a column
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_dw_sum_kernel(const float* partial, int count, int D, T* dw) {
-  __shared__ float part[32][33];
-  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+  __shared__ float part[8][129];
+  const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
+  const int64_t j = (int64_t)blockIdx.x * 8 + x;
   float s = 0.f;
   if (j < D) {
     int p = y;
-    for (; p + 7 * 32 < count; p += 8 * 32) {
-      float v[8];
+    for (; p + 3 * 128 < count; p += 4 * 128) {
+      float v[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = partial[(int64_t)(p + 32 * i) * D + j];
+      for (int i = 0; i < 4; ++i) v[i] = partial[(int64_t)(p + 128 * i) * D + j];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[i];
+      for (int i = 0; i < 4; ++i) s += v[i];
     }
-    for (; p < count; p += 32) s += partial[(int64_t)p * D + j];
+    for (; p < count; p += 128) s += partial[(int64_t)p * D + j];
   }
-  part[y][lane] = s;
+  part[x][y] = s;
   __syncthreads();
-  s = part[lane][y];
+  if (threadIdx.x >= 256) return;
+  const int c = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  s = (part[c][lane] + part[c][lane + 32]) + (part[c][lane + 64] + part[c][lane + 96]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  const int64_t jj = (int64_t)blockIdx.x * 32 + y;
+  const int64_t jj = (int64_t)blockIdx.x * 8 + c;
   if (lane == 0 && jj < D) dw[jj] = from_f32<T>(s);
 }
 
@@ -446,29 +470,43 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const T* x, int64_t row
     }
 }
 
-// values of codes: 8 consecutive ones a thread (VEC), or one; blockIdx.x: part of
+// values of codes: 16 bytes of values a thread (VEC), or one; blockIdx.x: part of
 // a row, blockIdx.y: which rows
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* codes, const float* scales, T* out, int64_t rows, int D,
                                                       int64_t ldc, int groups, int tall) {
-  constexpr int E = VEC ? 8 : 1;
+  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
   const int c = (blockIdx.x * 256 + threadIdx.x) * E;
   if (c >= D) return;
-#pragma unroll 4
-  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    const float s = scales[(tall ? row / 128 : row) * groups + c / kGroup8];
-    if (VEC) {
-      const uint2 q = *reinterpret_cast<const uint2*>(codes + row * ldc + c);
-      float v[8];
+  constexpr int R = 4;  // rows at a time
+  for (int64_t row0 = (int64_t)blockIdx.y * R; row0 < rows; row0 += (int64_t)gridDim.y * R) {
+    uint2 q[R];
+    float s[R];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 p = values2((k < 2 ? q.x : q.y) >> (16 * (k & 1)));
-        v[2 * k] = p.x * s;
-        v[2 * k + 1] = p.y * s;
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = min(row0 + r, rows - 1);
+      s[r] = scales[(tall ? row / 128 : row) * groups + c / kGroup8];
+      const uint8_t* from = codes + row * ldc + c;
+      if (E == 8) q[r] = *reinterpret_cast<const uint2*>(from);
+      else if (E == 4) q[r].x = *reinterpret_cast<const uint32_t*>(from);
+      else q[r].x = *from;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r >= rows) break;
+      T* to = out + (row0 + r) * D + c;
+      if constexpr (VEC) {
+        float v[E];
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          const float2 p = values2((k < 2 ? q[r].x : q[r].y) >> (16 * (k & 1)));
+          v[2 * k] = p.x * s[r];
+          v[2 * k + 1] = p.y * s[r];
+        }
+        store_vec<E>(to, v);
+      } else {
+        *to = from_f32<T>(values2(q[r].x).x * s[r]);
       }
-      store_vec<8>(out + row * D + c, v);
-    } else {
-      out[row * D + c] = from_f32<T>(values2(codes[row * ldc + c]).x * s);
     }
   }
 }
@@ -496,18 +534,35 @@ static int norm_strides(const char* op, const pvb2_rms_norm_desc* d, std::initia
   return PVB2_OK;
 }
 
+// resident blocks of a kernel on an SM, asked for once
+template <typename K>
+static int resident(K kernel, int threads, int smem, std::atomic<int>& known) {
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 template <typename T, bool VEC, int MODE>
 static int launch_norm(const NormArgs& a, cudaStream_t s) {
   const int chunks = (a.D + Chunk<T, VEC>::E - 1) / Chunk<T, VEC>::E;
-  const unsigned rows = (unsigned)a.rows;
-  // a warp where it keeps a row in four chunks a thread, since it needs no
-  // barrier; else as many threads as the row needs
-  auto threads = [&](int nv) { return (unsigned)(((chunks + nv - 1) / nv + 31) / 32 * 32); };
-  if (chunks <= 32) norm_kernel<T, VEC, true, 1, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
-  else if (chunks <= 64) norm_kernel<T, VEC, true, 2, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
-  else if (chunks <= 128) norm_kernel<T, VEC, true, 4, MODE><<<(rows + 3) / 4, 128, 0, s>>>(a);
-  else if (chunks <= 512) norm_kernel<T, VEC, false, 2, MODE><<<rows, threads(2), 0, s>>>(a);
-  else if (chunks <= 4096) norm_kernel<T, VEC, false, 4, MODE><<<rows, threads(4), 0, s>>>(a);
+  const unsigned rows = (unsigned)a.rows, fours = (unsigned)((a.rows + 3) / 4);
+  // A warp to a row that its lanes hold in four chunks each, since it needs no
+  // barrier; else a block, with four chunks a thread as well: each thread takes a
+  // root and a quotient for its row (8192 x 4096 bf16 with a residual: 41 us; in
+  // two chunks 47, a warp to the row with 16 chunks a lane 73).  Few rows have
+  // more threads, for the first chunk to be the only one.
+  const bool few = a.rows < num_sms();
+  if (chunks <= 32) norm_kernel<T, VEC, true, 1, MODE><<<fours, 128, 0, s>>>(a);
+  else if (chunks <= 64 && !few) norm_kernel<T, VEC, true, 2, MODE><<<fours, 128, 0, s>>>(a);
+  else if (chunks <= 128 && !few) norm_kernel<T, VEC, true, 4, MODE><<<fours, 128, 0, s>>>(a);
+  else if (chunks <= 1024 && few) norm_kernel<T, VEC, false, 1, MODE><<<rows, (unsigned)((chunks + 31) / 32 * 32), 0, s>>>(a);
+  else if (chunks <= 4096) norm_kernel<T, VEC, false, 4, MODE><<<rows, (unsigned)((chunks + 127) / 128 * 32), 0, s>>>(a);
   else norm_long_kernel<T, VEC, MODE><<<rows, 1024, 0, s>>>(a);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
@@ -534,6 +589,7 @@ static NormArgs norm_args(const pvb2_rms_norm_desc* d, const void* x, const void
   a.D = (int)d->D;
   a.groups = (int)((d->D + kGroup8 - 1) / kGroup8);
   a.eps = (float)d->eps;
+  a.per_element = 1.0 / (double)d->D;
   return a;
 }
 
@@ -563,20 +619,6 @@ static NormBwdPlan bwd_plan(const pvb2_rms_norm_desc* d, bool vec) {
   const int64_t want = (d->rows + p.rows_per_block - 1) / p.rows_per_block;
   p.blocks = std::max<int64_t>(1, std::min(want, most));
   return p;
-}
-
-// resident blocks of a kernel on an SM, asked for once
-template <typename K>
-static int resident(K kernel, int threads, int smem, std::atomic<int>& known) {
-  int n = known.load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) {
-      cudaGetLastError();
-      n = 1;
-    }
-    known.store(n, std::memory_order_relaxed);
-  }
-  return n;
 }
 
 template <typename T, bool VEC, int G, int NV>
@@ -615,7 +657,7 @@ template <typename T>
 static int run_bwd(const NormBwdArgs& a, NormBwdPlan p, bool vec, void* dw, cudaStream_t s) {
   if (a.rows) PVB2_TRY((vec ? launch_bwd<T, true>(a, p, s) : launch_bwd<T, false>(a, p, s)));
   if (!dw) return PVB2_OK;
-  norm_dw_sum_kernel<T><<<(unsigned)((a.D + 31) / 32), 1024, 0, s>>>(a.partial, a.rows ? (int)p.blocks : 0, a.D, (T*)dw);
+  norm_dw_sum_kernel<T><<<(unsigned)((a.D + 7) / 8), 1024, 0, s>>>(a.partial, a.rows ? (int)p.blocks : 0, a.D, (T*)dw);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -736,9 +778,8 @@ int pvb2_dequantize_8bit(int64_t rows, int64_t D, const uint8_t* codes, int64_t 
   const bool vec = D % 8 == 0 && ((uintptr_t)codes & 7) == 0 && (rows <= 1 || ldc % 8 == 0) && ((uintptr_t)out & 15) == 0 &&
                    D * size % 16 == 0;
   cudaStream_t s = as_stream(stream);
-  const unsigned wide = (unsigned)((D / (vec ? 8 : 1) + 255) / 256);
-  // four rows a block, while that leaves each SM eight blocks
-  const dim3 grid(wide, (unsigned)std::min<int64_t>(65535, std::max<int64_t>((rows + 3) / 4, std::min<int64_t>(rows, num_sms() * 8 / wide))));
+  const unsigned wide = (unsigned)((D / (vec ? 16 / size : 1) + 255) / 256);
+  const dim3 grid(wide, (unsigned)std::min<int64_t>(65535, (rows + 3) / 4));
   auto go = [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
     if (vec) dequant_kernel<T, true><<<grid, 256, 0, s>>>(codes, scales, p, rows, (int)D, ldc, groups, tall);
