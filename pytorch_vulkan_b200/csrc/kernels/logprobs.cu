@@ -274,7 +274,7 @@ __device__ __forceinline__ void take_best(uint64_t& list, const float* z, int64_
 template <int G>
 struct LpRow {
   static constexpr int THREADS = G < 128 ? 128 : G, ROWS = THREADS / G, WARPS = G / 32;
-  static constexpr int LIST = G < 128 ? 64 : 256;  // candidates that fit
+  static constexpr int LIST = G < 128 ? 96 : 256;  // candidates that fit: three times the best at least
   // of a row
   Running parts[WARPS];
   float maxima[WARPS][32];
@@ -488,6 +488,8 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) l
     const float least = mine.maxima[0][a.top - 1];
     if (some && most >= least) mine.shares[atomicAdd(&mine.n_shares, 1)] = t;
     row_sync<G>();
+    // (a mask that leaves fewer shares than that: what it left, and the first of what it hid)
+    const bool masked = least == -INFINITY;
     // the chunks of these shares, and the ends
     const int shares = mine.n_shares, per = (int)((to - from + G - 1) / G) + 1;
     const int pairs = shares * per;
@@ -503,17 +505,28 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) l
       return at;
     };
     for (int pair = t; pair < pairs; pair += G) {
+      if (*(volatile int*)&mine.n_found > Row::LIST) break;  // (they are counted one at a time)
       float v[E];
       const int64_t at = chunk_of(pair, v);
 #pragma unroll
       for (int k = 0; k < E; ++k)
-        if (at + k >= 0 && at + k < a.V && !(v[k] < least)) {
+        if (at + k >= 0 && at + k < a.V && !(masked ? v[k] == -INFINITY : v[k] < least)) {
           const int i = atomicAdd(&mine.n_found, 1);
           if (i < Row::LIST) mine.found[i] = entry(v[k], (uint32_t)(at + k));
         }
     }
     row_sync<G>();
-    const int found = mine.n_found;
+    int found = mine.n_found;
+    if (masked && found < a.top) {
+      // among as many places as there are to find and have been found, enough are hidden
+      const int64_t begin = rank == 0 ? 0 : from * E - off, end = rank == cluster - 1 ? a.V : to * E - off;
+      row_sync<G>();
+      for (int i = t; i < a.top + found; i += G)
+        if (begin + i < end && to_f32(z[begin + i]) == -INFINITY)
+          mine.found[atomicAdd(&mine.n_found, 1)] = entry(-INFINITY, (uint32_t)(begin + i));
+      row_sync<G>();
+      found = mine.n_found;
+    }
     if (found <= Row::LIST) {
       if (warp == 0)
         for (int i = 0; i < found; i += 32) {

@@ -158,7 +158,7 @@ def test_clip_refusals(lib):
     refused(lib, clip(lib, [one()], ws_bytes=7), "workspace")
     refused(lib, clip(lib, [one()], ws=None), "workspace")
     assert lib.pvb2_clip_grad_norm_workspace_size(0) == 0
-    assert 8 * 148 <= lib.pvb2_clip_grad_norm_workspace_size(1) <= lib.pvb2_clip_grad_norm_workspace_size(5000) < 1 << 20
+    assert 8 * 132 <= lib.pvb2_clip_grad_norm_workspace_size(1) <= lib.pvb2_clip_grad_norm_workspace_size(5000) < 1 << 20
 
 
 def test_python_surface():

@@ -245,3 +245,22 @@ def test_captured(ocl):
             v.zero_()
         graph.replay()
         assert all(torch.equal(a.cpu(), b) for a, b in zip(out, eager))
+
+
+@pytest.mark.parametrize("V", [40, 3000, 50003, 131072])
+@pytest.mark.parametrize("rows", [1, 200])
+def test_few_tokens_are_left(ocl, V, rows):
+    """A mask that leaves fewer tokens than alternatives are asked for: these, and then hidden ones by their places."""
+    g = torch.Generator().manual_seed(V)
+    for left in (0, 1, 3, 19, 20, 33):
+        z = torch.full((rows, V), float("-inf"))
+        for r in range(rows):
+            z[r, torch.randperm(V, generator=g)[:left]] = torch.randn(left, generator=g)
+        z = z.to(torch.bfloat16)
+        t = torch.zeros(rows, dtype=torch.int64)
+        _, _, tlp, tat = ocl.functional.token_log_probs(z.to(DEV), t.to(DEV), top=20)
+        at = best(z, 20)
+        assert torch.equal(tat.cpu(), at)
+        ref = Reference(z, t)
+        want = torch.where(ref.empty[:, None], float("-inf"), ref.logp.gather(1, at))
+        near(tlp, want, ref.bound_lp(want.clamp(min=-1e9)))
