@@ -17,10 +17,14 @@
 // not depend on the order of a sum.  (The conversions to 64 bits cost nothing
 // beside the loads: a square is converted for 4 to 8 bytes of traffic.)
 //
-// Elements go to threads in chunks of 16 bytes; where rows do not begin on
-// 16-byte boundaries, in chunks of four that lie 32 elements apart, so that a
-// warp still reads consecutive ones and 128 of them, a group of one scale, are
-// a warp's.
+// Elements go to threads in chunks of 16 bytes where rows begin on 16-byte
+// boundaries, else in chunks of four that lie 32 elements apart, so that a warp
+// still reads consecutive ones and 128 of them, a group of one scale, are a
+// warp's.  16-bit rows of 2048 or more elements whose operands all begin alike
+// between the boundaries (an odd length) take the chunks of memory, with a
+// row's first and last element by element: steps of 4000 x 5001 bf16 100 us
+// against 127 with chunks of four, 9760 x 2049 116 against 159, 3001 x 10001 fp16
+// 132 against 228; but 13012 x 1537 114 against 114, 19512 x 1025 146 against 126.
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>
@@ -57,38 +61,68 @@ struct NormBwdArgs {
   int D;
 };
 
-// E elements of a chunk: consecutive (VEC), or 32 apart
-template <typename T, bool VEC>
+enum { kApart = 0, kWhole = 1, kShifted = 2 };  // chunks: see above
+
+// E elements of a chunk
+template <typename T, int VEC>
 struct Chunk {
   static constexpr int E = VEC ? 16 / (int)sizeof(T) : 4;
-  // first element of chunk c, and the step to the next
-  static __device__ __forceinline__ int64_t at(int c) { return VEC ? (int64_t)c * E : (int64_t)(c >> 5) * 128 + (c & 31); }
+  // first element of chunk c, and the step to the next; `off`: where in its
+  // 16 bytes a shifted row begins
+  static __device__ __forceinline__ int64_t at(int c, int off) {
+    return VEC ? (int64_t)c * E - off : (int64_t)(c >> 5) * 128 + (c & 31);
+  }
   static constexpr int kStep = VEC ? 1 : 32;
 
   T e[E];
-  __device__ __forceinline__ void load(const T* row, int c, int D) {
-    const int64_t i = at(c);
-    if (VEC) {
-      if (i < D) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(row + i);
-      else *reinterpret_cast<uint4*>(e) = make_uint4(0, 0, 0, 0);
-    } else {
+  __device__ __forceinline__ void load_each(const T* row, int c, int D, int off) {
+    const int64_t i = at(c, off);
 #pragma unroll
-      for (int k = 0; k < E; ++k) e[k] = i + k * kStep < D ? row[i + k * kStep] : from_f32<T>(0.f);
+    for (int k = 0; k < E; ++k) {
+      const int64_t j = i + k * kStep;
+      e[k] = j < D && (VEC != kShifted || j >= 0) ? row[j] : from_f32<T>(0.f);
     }
   }
-  __device__ __forceinline__ void store(T* row, int c, int D) const {
-    const int64_t i = at(c);
-    if (VEC) {
+  __device__ __forceinline__ void load(const T* row, int c, int D, int off) {
+    const int64_t i = at(c, off);
+    if (VEC == kWhole) {
+      if (i < D) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(row + i);
+      else *reinterpret_cast<uint4*>(e) = make_uint4(0, 0, 0, 0);
+    } else if (VEC == kShifted) {
+      // (the ends by load_ends, once all other loads are on their way)
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (i >= 0 && i + E <= D) v = *reinterpret_cast<const uint4*>(row + i);
+      *reinterpret_cast<uint4*>(e) = v;
+    } else {
+      load_each(row, c, D, off);
+    }
+  }
+  __device__ __forceinline__ void load_ends(const T* row, int c, int D, int off) {
+    if (VEC != kShifted) return;
+    const int64_t i = at(c, off);
+    if (i < D && (i < 0 || i + E > D)) load_each(row, c, D, off);
+  }
+  __device__ __forceinline__ void store(T* row, int c, int D, int off) const {
+    const int64_t i = at(c, off);
+    if (VEC == kWhole) {
       if (i < D) *reinterpret_cast<uint4*>(row + i) = *reinterpret_cast<const uint4*>(e);
+    } else if (VEC == kShifted && i >= 0 && i + E <= D) {
+      *reinterpret_cast<uint4*>(row + i) = *reinterpret_cast<const uint4*>(e);
     } else {
 #pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (i + k * kStep < D) row[i + k * kStep] = e[k];
+      for (int k = 0; k < E; ++k) {
+        const int64_t j = i + k * kStep;
+        if (j < D && (VEC != kShifted || j >= 0)) row[j] = e[k];
+      }
     }
   }
 };
+template <typename T, int VEC>
+__device__ __forceinline__ int shift_of(const T* row) {
+  return VEC == kShifted ? (int)(((uintptr_t)row & 15) / sizeof(T)) : 0;
+}
 // (16-byte accesses to its elements)
-template <typename T, bool VEC>
+template <typename T, int VEC>
 struct alignas(16) AChunk : Chunk<T, VEC> {};
 
 // Sum over the threads of a row, a warp or a block, in a fixed order; all of
@@ -118,28 +152,51 @@ __device__ __forceinline__ float rstd_of(double squares, double per_element, flo
 }
 
 // the weight's numbers, or ones
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_weight(AChunk<T, VEC>& w, const void* p, int c, int D) {
+// elements [cE - off, cE - off + E) of what itself begins on a 16-byte boundary:
+// the two chunks that hold them, moved together
+template <typename T, int VEC>
+__device__ __forceinline__ void load_beside(AChunk<T, VEC>& w, const T* p, int c, int D, int off) {
+  constexpr int E = Chunk<T, VEC>::E;
+  if ((int64_t)(c + 1) * E > D) {
+    w.load_each(p, c, D, off);
+    return;
+  }
+  alignas(16) uint32_t v[9] = {};
+  if (c > 0) *reinterpret_cast<uint4*>(v) = *(reinterpret_cast<const uint4*>(p) + c - 1);
+  *reinterpret_cast<uint4*>(v + 4) = *(reinterpret_cast<const uint4*>(p) + c);
+  const int skip = 16 - off * (int)sizeof(T);  // bytes
+#pragma unroll
+  for (int step = 4; step; step >>= 1)
+#pragma unroll
+    for (int k = 0; k + step < 9; ++k) v[k] = skip >> 2 & step ? v[k + step] : v[k];
+  uint32_t* to = reinterpret_cast<uint32_t*>(w.e);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) to[k] = __funnelshift_r(v[k], v[k + 1], (skip & 3) * 8);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void load_weight(AChunk<T, VEC>& w, const void* p, int c, int D, int off) {
   if (p) {
-    w.load((const T*)p, c, D);
+    if (VEC == kShifted) load_beside(w, (const T*)p, c, D, off);
+    else w.load((const T*)p, c, D, off);
   } else {
 #pragma unroll
     for (int k = 0; k < Chunk<T, VEC>::E; ++k) w.e[k] = from_f32<T>(1.f);
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __device__ __forceinline__ void scale_row(const AChunk<T, VEC>& h, const AChunk<T, VEC>& w, float rstd, float* y) {
 #pragma unroll
   for (int k = 0; k < Chunk<T, VEC>::E; ++k) y[k] = __fmul_rn(__fmul_rn(to_f32(h.e[k]), rstd), to_f32(w.e[k]));
 }
 
 // the group's scale and this chunk's codes
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __device__ __forceinline__ void put_codes(const float* y, uint8_t* row, float* scales, int c, int D) {
+  static_assert(VEC != kShifted, "groups of a scale count from the row's beginning");
   constexpr int E = Chunk<T, VEC>::E;
   constexpr int kLanes = VEC ? kGroup8 / E : 32;  // that share a group
-  const int64_t i = Chunk<T, VEC>::at(c);
+  const int64_t i = Chunk<T, VEC>::at(c, 0);
   uint32_t most = 0;
 #pragma unroll
   for (int k = 0; k < E; ++k) most = max(most, abs_bits(y[k]));
@@ -168,37 +225,46 @@ __device__ __forceinline__ void put_codes(const float* y, uint8_t* row, float* s
 }
 
 // h of a chunk: x, or x + r, which is stored
-template <typename T, bool VEC>
-__device__ __forceinline__ void form_sum(const NormArgs& a, int64_t row, int c, AChunk<T, VEC>& x, const AChunk<T, VEC>& r) {
+template <typename T, int VEC>
+__device__ __forceinline__ void form_sum(const NormArgs& a, int64_t row, int c, int off, AChunk<T, VEC>& x,
+                                         const AChunk<T, VEC>& r) {
   if (!a.r) return;
 #pragma unroll
   for (int k = 0; k < Chunk<T, VEC>::E; ++k) x.e[k] = from_f32<T>(to_f32(x.e[k]) + to_f32(r.e[k]));
-  x.store((T*)a.sum + row * a.D, c, a.D);
+  x.store((T*)a.sum + row * a.D, c, a.D, off);
 }
 
 // A warp (WARP; blocks of four) or a block shares a row, each thread keeps NV
 // chunks of it.
-template <typename T, bool VEC, bool WARP, int NV, int MODE>
+template <typename T, int VEC, bool WARP, int NV, int MODE>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
   using C = Chunk<T, VEC>;
   __shared__ double line[32];
   const int G = WARP ? 32 : (int)blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
   if (row >= a.rows) return;  // whole warps: only where a warp has a row of its own
+  const int off = shift_of<T, VEC>((const T*)a.x + row * a.ldx);
   AChunk<T, VEC> h[NV];
   {
     AChunk<T, VEC> r[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) h[i].load((const T*)a.x + row * a.ldx, i * G + t, a.D);
+    for (int i = 0; i < NV; ++i) h[i].load((const T*)a.x + row * a.ldx, i * G + t, a.D, off);
     if (a.r) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) r[i].load((const T*)a.r + row * a.ldr, i * G + t, a.D);
+      for (int i = 0; i < NV; ++i) r[i].load((const T*)a.r + row * a.ldr, i * G + t, a.D, off);
+    }
+    if (VEC == kShifted) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        h[i].load_ends((const T*)a.x + row * a.ldx, i * G + t, a.D, off);
+        if (a.r) r[i].load_ends((const T*)a.r + row * a.ldr, i * G + t, a.D, off);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) form_sum(a, row, i * G + t, h[i], r[i]);
+    for (int i = 0; i < NV; ++i) form_sum(a, row, i * G + t, off, h[i], r[i]);
   }
   float rstd = 1.f;
-  if (MODE != kQuant8) {
+  if constexpr (MODE != kQuant8) {
     double q = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -214,19 +280,19 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
   for (int i = 0; i < NV; ++i) {
     const int c = i * G + t;
     float y[C::E];
-    if (MODE == kQuant8) {
+    if constexpr (MODE == kQuant8) {
 #pragma unroll
       for (int k = 0; k < C::E; ++k) y[k] = to_f32(h[i].e[k]);
     } else {
       AChunk<T, VEC> w;
-      load_weight(w, a.w, c, a.D);
+      load_weight(w, a.w, c, a.D, off);
       scale_row(h[i], w, rstd, y);
     }
-    if (MODE == kNorm) {
+    if constexpr (MODE == kNorm) {
       AChunk<T, VEC> out;
 #pragma unroll
       for (int k = 0; k < C::E; ++k) out.e[k] = from_f32<T>(y[k]);
-      out.store((T*)a.y + row * a.D, c, a.D);
+      out.store((T*)a.y + row * a.D, c, a.D, off);
     } else {
       put_codes<T, VEC>(y, a.codes + row * a.ldc, a.scales + row * a.groups, c, a.D);
     }
@@ -234,7 +300,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
 }
 
 // rows that outgrow the registers: read again for the output
-template <typename T, bool VEC, int MODE>
+template <typename T, int VEC, int MODE>
 __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
   using C = Chunk<T, VEC>;
   __shared__ double line[32];
@@ -242,13 +308,13 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
   // whole warps stay together: a group's lanes meet
   const int chunks = (a.D + C::E * 32 - 1) / (C::E * 32) * 32;
   float rstd = 1.f;
-  if (MODE != kQuant8) {
+  if constexpr (MODE != kQuant8) {
     double q = 0;
     for (int c = threadIdx.x; c < chunks; c += 1024) {
       AChunk<T, VEC> h, r;
-      h.load((const T*)a.x + row * a.ldx, c, a.D);
-      if (a.r) r.load((const T*)a.r + row * a.ldr, c, a.D);
-      form_sum(a, row, c, h, r);
+      h.load((const T*)a.x + row * a.ldx, c, a.D, 0);
+      if (a.r) r.load((const T*)a.r + row * a.ldr, c, a.D, 0);
+      form_sum(a, row, c, 0, h, r);
 #pragma unroll
       for (int k = 0; k < C::E; ++k) {
         const double v = to_f32(h.e[k]);
@@ -262,21 +328,21 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
   const T* src = a.r ? (const T*)a.sum + row * a.D : (const T*)a.x + row * a.ldx;
   for (int c = threadIdx.x; c < chunks; c += 1024) {
     AChunk<T, VEC> h;
-    h.load(src, c, a.D);
+    h.load(src, c, a.D, 0);
     float y[C::E];
-    if (MODE == kQuant8) {
+    if constexpr (MODE == kQuant8) {
 #pragma unroll
       for (int k = 0; k < C::E; ++k) y[k] = to_f32(h.e[k]);
     } else {
       AChunk<T, VEC> w;
-      load_weight(w, a.w, c, a.D);
+      load_weight(w, a.w, c, a.D, 0);
       scale_row(h, w, rstd, y);
     }
-    if (MODE == kNorm) {
+    if constexpr (MODE == kNorm) {
       AChunk<T, VEC> out;
 #pragma unroll
       for (int k = 0; k < C::E; ++k) out.e[k] = from_f32<T>(y[k]);
-      out.store((T*)a.y + row * a.D, c, a.D);
+      out.store((T*)a.y + row * a.D, c, a.D, 0);
     } else {
       put_codes<T, VEC>(y, a.codes + row * a.ldc, a.scales + row * a.groups, c, a.D);
     }
@@ -287,18 +353,23 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
 // A block walks rows and keeps its share of dw in registers: gy and h are read
 // once for both gradients.  The blocks' shares are summed by a second launch,
 // in a fixed order.
-template <typename T, bool VEC, int G, int NV>
-__global__ void __launch_bounds__(G < 128 ? 128 : G, (sizeof(T) == 4 ? 1024 : G == 1024 ? 1024 : 768) / (G < 128 ? 128 : G)) norm_bwd_kernel(NormBwdArgs a) {
+// MOST: 32 for a warp to a row, else the most threads of a row.
+template <typename T, int VEC, int MOST, int NV>
+__global__ void __launch_bounds__(MOST < 128 ? 128 : MOST, (sizeof(T) == 4 ? 1024 : MOST == 1024 ? 1024 : 768) / (MOST < 128 ? 128 : MOST)) norm_bwd_kernel(NormBwdArgs a) {
   using C = Chunk<T, VEC>;
-  constexpr int kRows = G < 128 ? 128 / G : 1;  // of a block
+  constexpr int kRows = MOST == 32 ? 4 : 1;  // of a block
+  const int G = MOST == 32 ? 32 : blockDim.x;
   __shared__ float line[2][32];
   extern __shared__ float share[];  // kRows > 1: dw of the rows' warps
-  const int t = threadIdx.x % G, mine = threadIdx.x / G;
+  const int t = MOST == 32 ? threadIdx.x % 32 : threadIdx.x, mine = MOST == 32 ? threadIdx.x / 32 : 0;
+  static_assert(VEC != kShifted || kRows == 1, "a warp's row is too short to be shifted");
+  // (all rows of a block begin alike: the host sees to it)
+  const int off = shift_of<T, VEC>((const T*)a.h + (int64_t)blockIdx.x * a.ldh);
   AChunk<T, VEC> w[NV];
   float dw[NV][C::E];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_weight(w[i], a.w, i * G + t, a.D);
+    load_weight(w[i], a.w, i * G + t, a.D, off);
 #pragma unroll
     for (int k = 0; k < C::E; ++k) dw[i][k] = 0.f;
   }
@@ -307,9 +378,17 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, (sizeof(T) == 4 ? 1024 : G 
     AChunk<T, VEC> h[NV], g[NV], gh[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      h[i].load((const T*)a.h + row * a.ldh, i * G + t, a.D);
-      g[i].load((const T*)a.gy + row * a.ldg, i * G + t, a.D);
-      if (a.gh) gh[i].load((const T*)a.gh + row * a.ldgh, i * G + t, a.D);
+      h[i].load((const T*)a.h + row * a.ldh, i * G + t, a.D, off);
+      g[i].load((const T*)a.gy + row * a.ldg, i * G + t, a.D, off);
+      if (a.gh) gh[i].load((const T*)a.gh + row * a.ldgh, i * G + t, a.D, off);
+    }
+    if (VEC == kShifted) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        h[i].load_ends((const T*)a.h + row * a.ldh, i * G + t, a.D, off);
+        g[i].load_ends((const T*)a.gy + row * a.ldg, i * G + t, a.D, off);
+        if (a.gh) gh[i].load_ends((const T*)a.gh + row * a.ldgh, i * G + t, a.D, off);
+      }
     }
     const float rstd = a.rstd[row];
     float dot = 0.f;
@@ -322,7 +401,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, (sizeof(T) == 4 ? 1024 : G 
         dw[i][k] = fmaf(gv, n, dw[i][k]);
       }
     if (!a.dx) continue;
-    const float mean = row_sum<G == 32>(dot, line[parity]) / (float)a.D;
+    const float mean = row_sum<MOST == 32>(dot, line[parity]) / (float)a.D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       AChunk<T, VEC> out;
@@ -333,17 +412,17 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, (sizeof(T) == 4 ? 1024 : G 
         if (a.gh) d += to_f32(gh[i].e[k]);
         out.e[k] = from_f32<T>(d);
       }
-      out.store((T*)a.dx + row * a.D, i * G + t, a.D);
+      out.store((T*)a.dx + row * a.D, i * G + t, a.D, off);
     }
   }
   if (!a.partial) return;
   if (kRows > 1) {
-    // (NV * G * E numbers for each row's warp)
-    constexpr int kWide = NV * G * C::E;
+    // (NV * 32 * E numbers for each row's warp)
+    constexpr int kWide = NV * 32 * C::E;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < C::E; ++k) share[mine * kWide + (int)C::at(i * G + t) + k * C::kStep] = dw[i][k];
+      for (int k = 0; k < C::E; ++k) share[mine * kWide + (int)C::at(i * G + t, off) + k * C::kStep] = dw[i][k];
     __syncthreads();
     for (int j = threadIdx.x; j < a.D; j += 128) {
       float s = share[j];
@@ -356,14 +435,14 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, (sizeof(T) == 4 ? 1024 : G 
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int k = 0; k < C::E; ++k) {
-        const int64_t j = C::at(i * G + t) + k * C::kStep;
-        if (j < a.D) a.partial[(int64_t)blockIdx.x * a.D + j] = dw[i][k];
+        const int64_t j = C::at(i * G + t, off) + k * C::kStep;
+        if (j >= 0 && j < a.D) a.partial[(int64_t)blockIdx.x * a.D + j] = dw[i][k];
       }
   }
 }
 
 // long rows: dh alone, and the shares of dw by columns
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
   using C = Chunk<T, VEC>;
   __shared__ float line[32];
@@ -374,10 +453,10 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
   for (int pass = 0; pass < 2; ++pass) {
     for (int c = threadIdx.x; c < chunks; c += 1024) {
       AChunk<T, VEC> h, g, w, gh, out;
-      h.load((const T*)a.h + row * a.ldh, c, a.D);
-      g.load((const T*)a.gy + row * a.ldg, c, a.D);
-      if (a.w) w.load((const T*)a.w, c, a.D);
-      if (pass && a.gh) gh.load((const T*)a.gh + row * a.ldgh, c, a.D);
+      h.load((const T*)a.h + row * a.ldh, c, a.D, 0);
+      g.load((const T*)a.gy + row * a.ldg, c, a.D, 0);
+      if (a.w) w.load((const T*)a.w, c, a.D, 0);
+      if (pass && a.gh) gh.load((const T*)a.gh + row * a.ldgh, c, a.D, 0);
 #pragma unroll
       for (int k = 0; k < C::E; ++k) {
         const float n = to_f32(h.e[k]) * rstd, v = to_f32(g.e[k]) * (a.w ? to_f32(w.e[k]) : 1.f);
@@ -389,7 +468,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
           out.e[k] = from_f32<T>(d);
         }
       }
-      if (pass) out.store((T*)a.dx + row * a.D, c, a.D);
+      if (pass) out.store((T*)a.dx + row * a.D, c, a.D, 0);
     }
     if (!pass) mean = row_sum<false>(dot, line) / (float)a.D;
   }
@@ -472,7 +551,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const T* x, int64_t row
 
 // values of codes: 16 bytes of values a thread (VEC), or one; blockIdx.x: part of
 // a row, blockIdx.y: which rows
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* codes, const float* scales, T* out, int64_t rows, int D,
                                                       int64_t ldc, int groups, int tall) {
   constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
@@ -548,9 +627,12 @@ static int resident(K kernel, int threads, int smem, std::atomic<int>& known) {
   return n;
 }
 
-template <typename T, bool VEC, int MODE>
+// chunks of a row, however it is shifted
+static int chunks_of(int64_t D, int E, int vec) { return (int)((D + (vec == kShifted ? E - 1 : 0) + E - 1) / E); }
+
+template <typename T, int VEC, int MODE>
 static int launch_norm(const NormArgs& a, cudaStream_t s) {
-  const int chunks = (a.D + Chunk<T, VEC>::E - 1) / Chunk<T, VEC>::E;
+  const int chunks = chunks_of(a.D, Chunk<T, VEC>::E, VEC);
   const unsigned rows = (unsigned)a.rows, fours = (unsigned)((a.rows + 3) / 4);
   // A warp to a row that its lanes hold in four chunks each, since it needs no
   // barrier; else a block, with four chunks a thread as well: each thread takes a
@@ -558,22 +640,35 @@ static int launch_norm(const NormArgs& a, cudaStream_t s) {
   // two chunks 47, a warp to the row with 16 chunks a lane 73).  Few rows have
   // more threads, for the first chunk to be the only one.
   const bool few = a.rows < num_sms();
-  if (chunks <= 32) norm_kernel<T, VEC, true, 1, MODE><<<fours, 128, 0, s>>>(a);
-  else if (chunks <= 64 && !few) norm_kernel<T, VEC, true, 2, MODE><<<fours, 128, 0, s>>>(a);
-  else if (chunks <= 128 && !few) norm_kernel<T, VEC, true, 4, MODE><<<fours, 128, 0, s>>>(a);
-  else if (chunks <= 1024 && few) norm_kernel<T, VEC, false, 1, MODE><<<rows, (unsigned)((chunks + 31) / 32 * 32), 0, s>>>(a);
+  if constexpr (VEC != kShifted) {  // (which has 257 or more)
+    if (chunks <= 128 && (chunks <= 32 || !few)) {
+      if (chunks <= 32) norm_kernel<T, VEC, true, 1, MODE><<<fours, 128, 0, s>>>(a);
+      else if (chunks <= 64) norm_kernel<T, VEC, true, 2, MODE><<<fours, 128, 0, s>>>(a);
+      else norm_kernel<T, VEC, true, 4, MODE><<<fours, 128, 0, s>>>(a);
+      PVB2_LAUNCH_CHECK();
+      return PVB2_OK;
+    }
+  }
+  if (chunks <= 1024 && few) norm_kernel<T, VEC, false, 1, MODE><<<rows, (unsigned)((chunks + 31) / 32 * 32), 0, s>>>(a);
   else if (chunks <= 4096) norm_kernel<T, VEC, false, 4, MODE><<<rows, (unsigned)((chunks + 127) / 128 * 32), 0, s>>>(a);
-  else norm_long_kernel<T, VEC, MODE><<<rows, 1024, 0, s>>>(a);
+  else norm_long_kernel<T, VEC == kWhole ? kWhole : kApart, MODE><<<rows, 1024, 0, s>>>(a);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
 
+template <typename T, int MODE>
+static int run_norm_as(const NormArgs& a, int vec, cudaStream_t s) {
+  if (vec == kWhole) return launch_norm<T, kWhole, MODE>(a, s);
+  if constexpr (MODE == kNorm)
+    if constexpr (sizeof(T) == 2)
+      if (vec == kShifted) return launch_norm<T, kShifted, MODE>(a, s);
+  return launch_norm<T, kApart, MODE>(a, s);
+}
 template <int MODE>
-static int run_norm(const NormArgs& a, int dtype, bool vec, cudaStream_t s) {
-  if (dtype == PVB2_F32) return vec ? launch_norm<float, true, MODE>(a, s) : launch_norm<float, false, MODE>(a, s);
-  if (dtype == PVB2_BF16)
-    return vec ? launch_norm<__nv_bfloat16, true, MODE>(a, s) : launch_norm<__nv_bfloat16, false, MODE>(a, s);
-  return vec ? launch_norm<__half, true, MODE>(a, s) : launch_norm<__half, false, MODE>(a, s);
+static int run_norm(const NormArgs& a, int dtype, int vec, cudaStream_t s) {
+  if (dtype == PVB2_F32) return run_norm_as<float, MODE>(a, vec, s);
+  if (dtype == PVB2_BF16) return run_norm_as<__nv_bfloat16, MODE>(a, vec, s);
+  return run_norm_as<__half, MODE>(a, vec, s);
 }
 
 static NormArgs norm_args(const pvb2_rms_norm_desc* d, const void* x, const void* r, const void* w, void* sum) {
@@ -593,58 +688,82 @@ static NormArgs norm_args(const pvb2_rms_norm_desc* d, const void* x, const void
   return a;
 }
 
-static bool norm_vec(const NormArgs& a, int dtype) {
+// an operand of the rows: its address and row stride
+struct RowsAt {
+  const void* p;
+  int64_t ld;
+};
+// how its rows lie: on 16-byte boundaries, or all operands' alike off them, or neither
+static int rows_lie(int64_t rows, int64_t D, int size, std::initializer_list<RowsAt> all, const void* weight) {
+  const int E = 16 / size;
+  bool whole = D % E == 0 && ((uintptr_t)weight & 15) == 0, alike = true;
+  const RowsAt* first = nullptr;
+  for (const RowsAt& r : all) {
+    if (!r.p) continue;
+    if (!first) first = &r;
+    whole = whole && on16(r.p, r.ld, size, rows);
+    alike = alike && ((uintptr_t)r.p & 15) == ((uintptr_t)first->p & 15) && (rows <= 1 || (r.ld - first->ld) % E == 0);
+  }
+  if (whole) return kWhole;
+  return size == 2 && D >= 2048 && alike && ((uintptr_t)weight & 15) == 0 ? kShifted : kApart;
+}
+static int norm_vec(const NormArgs& a, int dtype) {
   const int size = dtype_size(dtype);
-  return (int64_t)a.D * size % 16 == 0 && on16(a.x, a.ldx, size, a.rows) && (!a.r || on16(a.r, a.ldr, size, a.rows)) &&
-         (!a.w || on16(a.w, 0, size, 1)) && (!a.y || on16(a.y, a.D, size, a.rows)) &&
-         (!a.sum || on16(a.sum, a.D, size, a.rows)) &&
-         (!a.codes || (((uintptr_t)a.codes & 7) == 0 && (a.rows <= 1 || a.ldc % 8 == 0)));
+  const int lie = rows_lie(a.rows, a.D, size, {{a.x, a.ldx}, {a.r, a.ldr}, {a.y, a.D}, {a.sum, a.D}}, a.w);
+  if (!a.codes) return lie;
+  return lie == kWhole && ((uintptr_t)a.codes & 7) == 0 && (a.rows <= 1 || a.ldc % 8 == 0) ? kWhole : kApart;
 }
 
 // Blocks of the backward pass, each of which keeps a share of dw: as many as the
 // workspace is for, and no more than are resident (a second wave of a few blocks
 // would take as long as the first).
+// A row has the warps that hold it in two chunks a thread (a step of 4000 x 5000
+// bf16 82 us; rounded up to a power of two 92).
 struct NormBwdPlan {
   int threads, rows_per_block;  // threads of a row (0: long rows)
   int64_t blocks;
 };
-static NormBwdPlan bwd_plan(const pvb2_rms_norm_desc* d, bool vec) {
+static NormBwdPlan bwd_plan(const pvb2_rms_norm_desc* d, int vec) {
   const int size = dtype_size(d->dtype);
-  const int E = vec ? 16 / size : 4;
-  const int64_t chunks = (d->D + E - 1) / E;
+  const int chunks = chunks_of(d->D, vec ? 16 / size : 4, vec);
   NormBwdPlan p = {};
-  p.threads = chunks <= 64 ? 32 : chunks <= 256 ? 128 : chunks <= 512 ? 256 : chunks <= 1024 ? 512 : chunks <= 2048 ? 1024 : 0;
+  p.threads = chunks <= 64 ? 32 : chunks <= 128 ? (chunks + 31) / 32 * 32 : chunks <= 2048 ? (chunks + 63) / 64 * 32 : 0;
   p.rows_per_block = p.threads == 32 ? 4 : 1;
-  const int64_t most = (int64_t)num_sms() * (p.threads == 0 ? 1 : p.threads <= 128 ? 8 : 1024 / p.threads);
+  const int64_t most = (int64_t)num_sms() * (p.threads == 0 ? 1 : std::min(8, 1024 / p.threads));
   const int64_t want = (d->rows + p.rows_per_block - 1) / p.rows_per_block;
   p.blocks = std::max<int64_t>(1, std::min(want, most));
   return p;
 }
 
-template <typename T, bool VEC, int G, int NV>
+template <typename T, int VEC, int MOST, int NV>
 static int launch_bwd_as(const NormBwdArgs& a, NormBwdPlan& p, cudaStream_t s) {
-  constexpr int threads = G < 128 ? 128 : G, smem = G < 128 ? 4 * NV * G * Chunk<T, VEC>::E * 4 : 0;
-  static std::atomic<int> known{0};
-  auto kernel = norm_bwd_kernel<T, VEC, G, NV>;
-  p.blocks = std::min<int64_t>(p.blocks, (int64_t)num_sms() * resident(kernel, threads, smem, known));
+  const int threads = MOST == 32 ? 128 : p.threads, smem = MOST == 32 ? 4 * NV * 32 * Chunk<T, VEC>::E * 4 : 0;
+  static std::atomic<int> known[33];  // by warps
+  auto kernel = norm_bwd_kernel<T, VEC, MOST, NV>;
+  p.blocks = std::min<int64_t>(p.blocks, (int64_t)num_sms() * resident(kernel, threads, smem, known[threads / 32]));
+  // (the rows of a block begin alike where they lie a multiple of E rows apart)
+  constexpr int E = Chunk<T, VEC>::E;
+  if (VEC == kShifted && p.blocks < a.rows) p.blocks = p.blocks / E * E;
   kernel<<<(unsigned)p.blocks, threads, smem, s>>>(a);
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
 
-template <typename T, bool VEC>
+template <typename T, int VEC>
 static int launch_bwd(const NormBwdArgs& a, NormBwdPlan& p, cudaStream_t s) {
-  constexpr int E = Chunk<T, VEC>::E;
-  const int chunks = (a.D + E - 1) / E;
-  if (chunks <= 32) return launch_bwd_as<T, VEC, 32, 1>(a, p, s);
-  if (chunks <= 64) return launch_bwd_as<T, VEC, 32, 2>(a, p, s);
-  if (chunks <= 128) return launch_bwd_as<T, VEC, 128, 1>(a, p, s);
-  if (chunks <= 256) return launch_bwd_as<T, VEC, 128, 2>(a, p, s);
+  const int chunks = chunks_of(a.D, Chunk<T, VEC>::E, VEC);
+  if constexpr (VEC != kShifted) {  // (which has 257 or more)
+    if (chunks <= 32) return launch_bwd_as<T, VEC, 32, 1>(a, p, s);
+    if (chunks <= 64) return launch_bwd_as<T, VEC, 32, 2>(a, p, s);
+    if (chunks <= 128) return launch_bwd_as<T, VEC, 128, 1>(a, p, s);
+    if (chunks <= 256) return launch_bwd_as<T, VEC, 128, 2>(a, p, s);
+  }
   if (chunks <= 512) return launch_bwd_as<T, VEC, 256, 2>(a, p, s);
+  if (chunks <= 768) return launch_bwd_as<T, VEC, 384, 2>(a, p, s);
   if (chunks <= 1024) return launch_bwd_as<T, VEC, 512, 2>(a, p, s);
   if (chunks <= 2048) return launch_bwd_as<T, VEC, 1024, 2>(a, p, s);
   if (a.dx) {
-    norm_bwd_long_kernel<T, VEC><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    norm_bwd_long_kernel<T, VEC == kWhole ? kWhole : kApart><<<(unsigned)a.rows, 1024, 0, s>>>(a);
     PVB2_LAUNCH_CHECK();
   }
   if (!a.partial) return PVB2_OK;
@@ -654,8 +773,14 @@ static int launch_bwd(const NormBwdArgs& a, NormBwdPlan& p, cudaStream_t s) {
 }
 
 template <typename T>
-static int run_bwd(const NormBwdArgs& a, NormBwdPlan p, bool vec, void* dw, cudaStream_t s) {
-  if (a.rows) PVB2_TRY((vec ? launch_bwd<T, true>(a, p, s) : launch_bwd<T, false>(a, p, s)));
+static int run_bwd(const NormBwdArgs& a, NormBwdPlan p, int vec, void* dw, cudaStream_t s) {
+  if (a.rows) {
+    if (vec == kWhole) PVB2_TRY((launch_bwd<T, kWhole>(a, p, s)));
+    else if constexpr (sizeof(T) == 2) {
+      if (vec == kShifted) PVB2_TRY((launch_bwd<T, kShifted>(a, p, s)));
+      else PVB2_TRY((launch_bwd<T, kApart>(a, p, s)));
+    } else PVB2_TRY((launch_bwd<T, kApart>(a, p, s)));
+  }
   if (!dw) return PVB2_OK;
   norm_dw_sum_kernel<T><<<(unsigned)((a.D + 7) / 8), 1024, 0, s>>>(a.partial, a.rows ? (int)p.blocks : 0, a.D, (T*)dw);
   PVB2_LAUNCH_CHECK();
@@ -694,8 +819,10 @@ int pvb2_rms_norm_8bit(const pvb2_rms_norm_desc* d, const void* x, const void* r
 
 size_t pvb2_rms_norm_bwd_workspace_size(const pvb2_rms_norm_desc* d) {
   if (norm_check("rms_norm", d) != PVB2_OK) return 0;
-  // (rows without 16-byte boundaries may have more blocks)
-  return (size_t)std::max(bwd_plan(d, true).blocks, bwd_plan(d, false).blocks) * d->D * 4;
+  // (how the rows lie is not known here)
+  int64_t blocks = 0;
+  for (int vec : {(int)kApart, (int)kWhole, (int)kShifted}) blocks = std::max(blocks, bwd_plan(d, vec).blocks);
+  return (size_t)blocks * d->D * 4;
 }
 
 int pvb2_rms_norm_bwd(const pvb2_rms_norm_desc* d, const void* h, const void* weight, const float* rstd, const void* gy,
@@ -722,10 +849,7 @@ int pvb2_rms_norm_bwd(const pvb2_rms_norm_desc* d, const void* h, const void* we
   a.ldg = d->ldg;
   a.ldgh = d->ldr;
   a.D = (int)d->D;
-  const int size = dtype_size(d->dtype);
-  const bool vec = (int64_t)a.D * size % 16 == 0 && on16(h, a.ldh, size, a.rows) && on16(gy, a.ldg, size, a.rows) &&
-                   (!gsum || on16(gsum, a.ldgh, size, a.rows)) && (!weight || on16(weight, 0, size, 1)) &&
-                   (!dx || on16(dx, a.D, size, a.rows));
+  const int vec = rows_lie(a.rows, a.D, dtype_size(d->dtype), {{h, a.ldh}, {gy, a.ldg}, {gsum, a.ldgh}, {dx, a.D}}, weight);
   const NormBwdPlan p = bwd_plan(d, vec);
   cudaStream_t s = as_stream(stream);
   if (d->dtype == PVB2_F32) return run_bwd<float>(a, p, vec, dw, s);

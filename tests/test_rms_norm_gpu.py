@@ -124,6 +124,33 @@ def test_strides_orders_and_no_weight(ocl, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 2051), (300, 1025), (2500, 2057), (9, 5001), (1210, 4099), (5, 12289), (3, 16375), (2, 16377)],
+                         ids=lambda s: "-".join(map(str, s)))
+def test_rows_between_boundaries(ocl, shape, dtype):
+    """Odd lengths: rows that begin anywhere, operands that begin alike and not, more rows than blocks; what lies between
+    the rows is not written."""
+    rows, D = shape
+    x, r, w, gy, gs = make(rows, D, dtype)
+    f = ocl.functional.rms_norm
+    h = summed(x, r)
+    dx, bx, dw, bw = reference_gradients(h, w, gy, gs, 1e-6)
+    for wide, at in ((D, 0), (D + 8, 8), (D + 16, 3), (D + 3, 0)):
+        back = torch.full((rows, wide), float("nan"), dtype=dtype)
+        back[:, at:at + D] = x
+        xd = back.to(DEV)[:, at:at + D].detach().requires_grad_()
+        rd, wd = r.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        y, s = f(xd, wd, rd, eps=1e-6)
+        assert torch.equal(s.detach().cpu(), h)
+        check_forward(y.detach(), h, w, 1e-6)
+        torch.autograd.backward([y, s], [gy.to(DEV), gs.to(DEV)])
+        for got, want, bound in ((xd.grad, dx, bx), (rd.grad, dx, bx), (wd.grad, dw, bw)):
+            close(got, want, bound + rounding(want, dtype) + torch.finfo(dtype).eps * bound)
+    # a weight that begins between boundaries
+    wide = torch.cat([torch.ones(1, dtype=dtype), w]).to(DEV)
+    check_forward(f(x.to(DEV), wide[1:], eps=1e-6), x, w, 1e-6)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_what_is_asked_for(ocl, dtype):
     """Only some gradients; only the sum used; a leaf that is both terms; backward twice over a kept graph."""
     x, r, w, gy, gs = make(40, 257, dtype)
