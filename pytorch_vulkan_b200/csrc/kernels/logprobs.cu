@@ -11,9 +11,10 @@
 // with x = z log2(e) - M, one multiply-add, M being the thread's running maximum
 // times log2(e), rounded.  A thread's s and u hold relative to M exactly as it
 // is, and are moved to m itself at the end, so that M's rounding does not count
-// however large the logits are.  Where M is beyond fp32 (logits of 2e38, or
-// nothing but the type's lowest number) a thread that has summed nothing reads
-// its share again and subtracts before it multiplies.
+// however large the logits are.  M is rounded up; where its steps are so wide that
+// a thread has summed nothing (logits of 1e10 or more, or nothing but -1e10 or
+// less, as a finite mask leaves it), it reads its share again and subtracts
+// before it multiplies.
 //
 // Each thread copies its chunks of 16 bytes into a ring of its own in shared
 // memory, eight ahead, without barriers: registers for as many loads in flight
@@ -147,8 +148,9 @@ struct Running2 {
 template <int N>
 __device__ __forceinline__ void take(Running2& r, const float* z, float most) {
   if (most > r.m) {
-    // (logits of 2e38 make it infinite and those of -2e38 clamp it: nothing is summed)
-    const float ref = fmaxf(most * kLog2e, -FLT_MAX);
+    // rounded up, so that no power is above 1: where ref's steps are wide (logits
+    // of 1e10 either way; 2e38 makes it infinite) nothing is summed
+    const float ref = fmaxf(__fmul_ru(most, kLog2e), -FLT_MAX);
     if (r.s != 0.f) {
       const float d = r.ref - ref, c = exp2_of(d);
       r.u = c > 0.f || r.s != r.s ? c * fmaf(r.s, d, r.u) : 0.f;
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) l
   });
   const float most = r.m;
   Running sum = moved(r);
-  if (r.s == 0.f && most > -INFINITY) {  // beyond fp32 times log2(e)
+  if (r.s == 0.f && most > -INFINITY) {  // M is further from log2(e) times the maximum than 126
     sum = {-INFINITY, 0.f, 0.f};
     float v[E];
     for (int i = 0; i < n; ++i) {

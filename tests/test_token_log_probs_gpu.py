@@ -128,6 +128,33 @@ def test_equal_falling_and_rising_logits(ocl, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [5, 1000, 70001])
+def test_far_from_zero(ocl, dtype, V):
+    """Rows of logits of one magnitude, alike or a step or more apart, of either sign, and what a finite mask leaves."""
+    g = torch.Generator().manual_seed(V)
+    most = float(torch.finfo(dtype).max)
+    rows = []
+    for size in (1e3, 6e4, 1e6, 1e8, 1e9, 3e9, 1e10, 2e10, 1e15, 1e20, 1e30, 1e38, 2e38):
+        for sign in (-1, 1):
+            v = sign * min(size, most)
+            near_it = v * (1 + torch.randint(0, 3, (V,), generator=g) * 2.0 ** -20).clamp(max=most / abs(v))
+            rows += [torch.full((V,), v), near_it, torch.where(torch.arange(V) % 5 == 3, torch.randn(V, generator=g), -abs(v))]
+    z = torch.stack(rows).to(dtype)
+    t = torch.randint(0, V, (len(rows),), generator=g)
+    gl, gh = torch.randn(len(rows), generator=g), torch.randn(len(rows), generator=g)
+    zd = z.to(DEV).requires_grad_()
+    lp, H = ocl.functional.token_log_probs(zd, t.to(DEV))
+    ref = Reference(z, t)
+    near(lp.detach(), ref.lp, ref.bound_lp(ref.lp))
+    near(H.detach(), ref.H, ref.bound_H)
+    (dz,) = torch.autograd.grad([lp, H], zd, [gl.to(DEV), gh.to(DEV)])
+    want, bound = ref.gradient(gl, gh)
+    eps = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0
+    bound = torch.where(ref.p > 0, bound, 2.0 ** -126 * 300)  # (log p of -1e38 times p of 0)
+    near(dz, want, bound + eps * (want.abs() + bound) + (2.0 ** -25 if dtype == torch.float16 else 0))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_masks(ocl, dtype):
     """-inf has no probability and no gradient, a row of nothing else none at all; NaN and +inf spoil their own row."""
     V = 777
