@@ -6,21 +6,25 @@
 //   dz_j = p_j (-g - k (log p_j + H)) + g [j = t]      (g of log p_t, k of H)
 //
 // The forward pass reads the logits once, the backward pass reads them once
-// more and writes as much: both are bound by HBM.  16-bit logits come at a rate
-// at which the forward pass has ten instructions for each: exponentials are 2^x
-// with x = z log2(e) - M, one multiply-add, M being the thread's running maximum
-// times log2(e), rounded.  A thread's s and u hold relative to M exactly as it
-// is, and are moved to m itself at the end, so that M's rounding does not count
-// however large the logits are.  M is rounded up; where its steps are so wide that
-// a thread has summed nothing (logits of 1e10 or more, or nothing but -1e10 or
-// less, as a finite mask leaves it), it reads its share again and subtracts
-// before it multiplies.
+// more and writes as much: both are bound by HBM (8192 x 131072 bf16: 355 us
+// forward, 6.0 TB/s, and 650 us backward, 6.6 TB/s; called without a pause the
+// forward pass draws all of the board's power and takes 420 at 1.5 GHz).  16-bit
+// logits come at a rate at which the forward pass has ten instructions for each;
+// it takes 6.6.  Exponentials are 2^x with x = z log2(e) - M, one multiply-add, M
+// being the thread's running maximum times log2(e), rounded, or that of an
+// earlier maximum at most 2 below.  A thread's s and u hold relative to M exactly
+// as it is, and are moved to m itself at the end, so that M's rounding does not
+// count however large the logits are.  M is rounded up; where its steps are so
+// wide that a thread has summed nothing (logits of 1e10 or more, or nothing but
+// -1e10 or less, as a finite mask leaves it), it reads its share again and
+// subtracts before it multiplies.
 //
 // Each thread copies its chunks of 16 bytes into a ring of its own in shared
 // memory, eight ahead, without barriers: registers for as many loads in flight
-// would halve the threads.  A row is a warp's, a block's of 128 or 256, or, where
-// rows are few, a cluster's, whose blocks join through shared memory: one
-// launch, no workspace.
+// would halve the threads.  The forward pass takes four at a time (4095 x 49999
+// with 5 alternatives: 97 us; in twos 104).  A row is a warp's, a block's of 128
+// or 256, or, where rows are few, a cluster's, whose blocks join through shared
+// memory: one launch, no workspace.
 //
 // The best ones.  A thread's maximum is the best of its share of the row.  Of
 // the k best, none is in a share whose maximum is below the k-th best maximum
@@ -45,7 +49,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kLpTop = 32;
 constexpr int kLpCluster = 8;
-constexpr int kLpRing = 8;  // chunks of a thread on their way, two to a step
+constexpr int kLpRing = 8;  // chunks of a thread on their way
+constexpr int kLpGroup = 4;  // that the forward pass takes at a time
 
 struct LpArgs {
   const void* z;
@@ -141,22 +146,27 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// the same in powers of two, relative to `ref`
+// the same in powers of two, relative to `ref`, which serves logits up to `next`
 struct Running2 {
-  float m, ref, s, u;
+  float m, next, ref, s, u;
 };
+constexpr float kAhead = 2.f;
 template <int N>
 __device__ __forceinline__ void take(Running2& r, const float* z, float most) {
-  if (most > r.m) {
-    // rounded up, so that no power is above 1: where ref's steps are wide (logits
-    // of 1e10 either way; 2e38 makes it infinite) nothing is summed
+  r.m = fmaxf(r.m, most);
+  // (a maximum that grows by less than kAhead leaves ref where it is: powers up
+  // to 8 cost the sums nothing, and some lane of a warp has a new one nearly
+  // every time)
+  if (most > r.next) {
+    // rounded up, so that the maximum's power is no more than 1: where ref's steps
+    // are wide (logits of 1e10 either way; 2e38 makes it infinite) nothing is summed
     const float ref = fmaxf(__fmul_ru(most, kLog2e), -FLT_MAX);
     if (r.s != 0.f) {
       const float d = r.ref - ref, c = exp2_of(d);
       r.u = c > 0.f || r.s != r.s ? c * fmaf(r.s, d, r.u) : 0.f;
       r.s *= c;
     }
-    r.m = most;
+    r.next = most + kAhead;
     r.ref = ref;
   }
   const uint64_t l = pair_of(kLog2e, kLog2e), ref = pair_of(-r.ref, -r.ref);
@@ -356,34 +366,38 @@ __device__ __forceinline__ float most_of(const RawVec<16>* raw) {
   }
 }
 
-// A thread's chunks of 16 bytes, STEP bytes apart, by way of its slots in shared memory.
-template <int THREADS>
+// A thread's chunks of 16 bytes, STEP bytes apart, by way of its slots in shared
+// memory, GROUP of them at a time.
+template <int THREADS, int GROUP>
 struct Ring {
   uint32_t slots;
   const char* next;
   int left;  // chunks that have not been asked for
   static constexpr int kSlot = THREADS * 16;
 
-  __device__ __forceinline__ void ask(int slot, bool there, int64_t ahead) {
+  // chunk `i` from here, if there is one
+  template <int STEP>
+  __device__ __forceinline__ void ask(int i) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %2, 0;\n\t"
-        "@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(slots + slot * kSlot),
-        "l"(next + ahead), "r"((int)there)
+        "setp.gt.s32 p, %2, %3;\n\t"
+        "@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(slots + i * kSlot),
+        "l"(next + (int64_t)i * STEP), "r"(left), "r"(i)
         : "memory");
   }
-  __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  template <int STEP>
+  __device__ __forceinline__ void ask_group(int slot) {
+#pragma unroll
+    for (int i = slot; i < slot + GROUP; ++i) ask<STEP>(i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
   template <int STEP>
   __device__ __forceinline__ void begin(void* smem, const void* first, int n) {
     slots = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
     next = (const char*)first;
     left = n;
 #pragma unroll
-    for (int i = 0; i < kLpRing; i += 2) {
-      ask(i, i < left, (int64_t)i * STEP);
-      ask(i + 1, i + 1 < left, (int64_t)(i + 1) * STEP);
-      commit();
-    }
+    for (int i = 0; i < kLpRing; i += GROUP) ask_group<STEP>(i);
     left -= kLpRing;
     next += (int64_t)kLpRing * STEP;
   }
@@ -395,23 +409,35 @@ struct Ring {
                  : "memory");
     return raw;
   }
-  // the n chunks go to `f` in twos: their number, they, whether there is a second
+  // the n chunks go to `f`, in groups and the last ones singly: the first's number, they, how many
   template <int STEP, typename F>
   __device__ __forceinline__ void walk(int n, F f) {
-    for (int i0 = 0; i0 < n; i0 += kLpRing) {
+    int i0 = 0;
+    for (; i0 + kLpRing <= n; i0 += kLpRing) {
 #pragma unroll
-      for (int i = 0; i < kLpRing; i += 2) {
-        if (i0 + i >= n) break;
-        asm volatile("cp.async.wait_group %0;" ::"n"(kLpRing / 2 - 1) : "memory");
-        const RawVec<16> raw[2] = {get(i), get(i + 1)};
-        f(i0 + i, raw, i0 + i + 1 < n);
+      for (int i = 0; i < kLpRing; i += GROUP) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kLpRing / GROUP - 1) : "memory");
+        RawVec<16> raw[GROUP];
+#pragma unroll
+        for (int k = 0; k < GROUP; ++k) raw[k] = get(i + k);
+        f(i0 + i, raw, std::integral_constant<int, GROUP>());
         // (the slots have been read: their numbers have been used)
-        ask(i, i < left, (int64_t)i * STEP);
-        ask(i + 1, i + 1 < left, (int64_t)(i + 1) * STEP);
-        commit();
+        ask_group<STEP>(i);
       }
       left -= kLpRing;
       next += (int64_t)kLpRing * STEP;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    int i = 0;
+    for (; i0 + i + GROUP <= n; i += GROUP) {
+      RawVec<16> raw[GROUP];
+#pragma unroll
+      for (int k = 0; k < GROUP; ++k) raw[k] = get(i + k);
+      f(i0 + i, raw, std::integral_constant<int, GROUP>());
+    }
+    for (; i0 + i < n; ++i) {
+      const RawVec<16> raw[1] = {get(i)};
+      f(i0 + i, raw, std::integral_constant<int, 1>());
     }
   }
 };
@@ -444,9 +470,9 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) l
 
   // this thread's chunks: from + t, and every G-th from there
   const int n = (int)max((int64_t)0, (to - from - t + G - 1) / G);
-  Ring<Row::THREADS> chunks;
+  Ring<Row::THREADS, kLpGroup> chunks;
   chunks.template begin<G * 16>(ring, z + ((from + t) * E - off), n);
-  Running2 r = {-INFINITY, 0.f, 0.f, 0.f};
+  Running2 r = {-INFINITY, -INFINITY, 0.f, 0.f, 0.f};
   {
     const int64_t at = end_of(t);
     if (at < a.V) {
@@ -456,15 +482,12 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) l
       take<E>(r, v, most_of<T, 1>(&raw));
     }
   }
-  chunks.template walk<G * 16>(n, [&](int, const RawVec<16>* raw, bool two) {
-    float v[2 * E];
-    unpack_vec<E, T>(raw[0], v);
-    if (two) {
-      unpack_vec<E, T>(raw[1], v + E);
-      take<2 * E>(r, v, most_of<T, 2>(raw));
-    } else {
-      take<E>(r, v, most_of<T, 1>(raw));
-    }
+  chunks.template walk<G * 16>(n, [&](int, const RawVec<16>* raw, auto count) {
+    constexpr int N = decltype(count)::value;
+    float v[N * E];
+#pragma unroll
+    for (int k = 0; k < N; ++k) unpack_vec<E, T>(raw[k], v + k * E);
+    take<N * E>(r, v, most_of<T, N>(raw));
   });
   const float most = r.m;
   Running sum = moved(r);
@@ -666,7 +689,7 @@ __global__ void __launch_bounds__(kLpBwdThreads, 5) logp_bwd_kernel(LpBwdArgs a,
   const int64_t from = min(hi, lo + blockIdx.y * share), to = min(hi, from + share);
   const int n = (int)max((int64_t)0, (to - from - threadIdx.x + G - 1) / G);
   const int64_t first = (from + threadIdx.x) * E - off;
-  Ring<G> chunks;
+  Ring<G, 2> chunks;
   chunks.template begin<G * 16>(ring, z + first, n);
   const LpRowGrad r(a, row);
   // the chunk with the token, if it is this thread's
@@ -676,10 +699,9 @@ __global__ void __launch_bounds__(kLpBwdThreads, 5) logp_bwd_kernel(LpBwdArgs a,
   const uint64_t l = pair_of(kLog2e, kLog2e), m2 = pair_of(-r.m, -r.m), logs2 = pair_of(r.logs2, r.logs2),
                  slope = pair_of(r.slope, r.slope), rest = pair_of(r.rest, r.rest);
   T* out = dz + first;
-  chunks.template walk<G * 16>(n, [&](int i, const RawVec<16>* raw, bool two) {
+  chunks.template walk<G * 16>(n, [&](int i, const RawVec<16>* raw, auto count) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      if (c && !two) break;
+    for (int c = 0; c < decltype(count)::value; ++c) {
       float v[E];
       unpack_vec<E, T>(raw[c], v);
 #pragma unroll
