@@ -22,6 +22,7 @@
 //     shared memory in a fixed order.  Bound by the weight's bytes.
 #include <algorithm>
 #include <type_traits>
+#include "overlap.cuh"
 #include "quant8.cuh"
 #include "tc_common.cuh"
 
@@ -157,6 +158,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   uint32_t* tmem_slot = (uint32_t*)(scales_empty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
 
+  let_next_come();
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int tiles_m = (p.M + kL8M - 1) / kL8M, tiles_n = (p.N + kL8N - 1) / kL8N;
@@ -178,6 +180,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
     fence_barrier_init();
   }
   if (warp == kL8MmaWarp) tmem_alloc_pair(tmem_slot, 512);
+  wait_for_last();
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist before either is signalled
@@ -230,9 +233,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
         for (int i = 0; i < 4; ++i) {
           const int k = min(kb + i, p.blocks - 1);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r][i] = __ldg(p.xs + (int64_t)min(m0 + 32 * r, p.M - 1) * p.blocks + k);
-          w[0][i] = __ldg(ws0 + k);
-          w[1][i] = __ldg(ws1 + k);
+          for (int r = 0; r < 4; ++r) x[r][i] = p.xs[(int64_t)min(m0 + 32 * r, p.M - 1) * p.blocks + k];
+          w[0][i] = ws0[k];
+          w[1][i] = ws1[k];
         }
       };
       fetch(0);
@@ -451,8 +454,8 @@ __device__ __forceinline__ void load_scales(const L8Args& p, const float* ws, in
       float x[8], w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = __ldg(row + min(k0 + i, count - 1));
-        w[i] = __ldg(ws + kb + min(k0 + i, count - 1));
+        x[i] = row[min(k0 + i, count - 1)];
+        w[i] = ws[kb + min(k0 + i, count - 1)];
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -462,11 +465,11 @@ __device__ __forceinline__ void load_scales(const L8Args& p, const float* ws, in
     // a warp to a row, a lane to a block
     constexpr int kRows = NT / kL8FewEpi;
     const int k = min(lane, count - 1);
-    const float w = __ldg(ws + kb + k);
+    const float w = ws[kb + k];
     float x[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
-      x[i] = __ldg(p.xs + (int64_t)min(m0 + warp - 2 + kL8FewEpi * i, p.M - 1) * p.blocks + kb + k);
+      x[i] = p.xs[(int64_t)min(m0 + warp - 2 + kL8FewEpi * i, p.M - 1) * p.blocks + kb + k];
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
       if (lane < count) run[lane * kPitch + warp - 2 + kL8FewEpi * i] = x[i] * w;
@@ -488,6 +491,7 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + kBufs);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
 
+  let_next_come();
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
   // tiles of the same outputs lie together: their weight is read once
@@ -502,6 +506,7 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
     for (int i = lane; i < 2 * kSlots + 2 * kBufs; i += 32) mbar_init(&full[i], i < 2 * kSlots + kBufs ? 1 : kL8FewEpi);
     fence_barrier_init();
     __syncwarp();
+    wait_for_last();
     if (lane == 0) {
       *abort = 0;
       // the first loads need nothing of the others
@@ -515,6 +520,7 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
   } else if (warp == 1) {
     tmem_alloc(tmem_slot, L::COLUMNS);
   } else {
+    wait_for_last();
     load_scales<NT>(p, ws, m0, kb0, min(L::RUN, kb1 - kb0), run, warp, lane);
   }
   tc_fence_before();
@@ -733,7 +739,7 @@ static int l8_many(const pvb2_linear8_desc* d, const void* x, const void* w, L8A
   // blocks of rows that stay in L2 (32 MB of its 126) while the outputs go by
   p.group = (int)std::max<int64_t>(8, std::min<int64_t>(l8_div(d->M, kL8M), ((int64_t)32 << 20) / (kL8M * d->K)));
   const int grid = 2 * (int)std::min<int64_t>(tiles, std::max(1, num_sms() / 2));
-  linear8_kernel<T><<<grid, L8Smem::THREADS, smem, s>>>(mx, mw, my, p);
+  PVB2_CUDA_TRY(launch_over(linear8_kernel<T>, grid, L8Smem::THREADS, smem, s, 0, mx, mw, my, p));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -746,18 +752,8 @@ static int l8_few(const pvb2_linear8_desc* d, const void* x, const void* w, cons
   CUtensorMap mx, mw;
   PVB2_TRY(l8_codes(&mx, x, d->K, d->M, d->ldx, NT));
   PVB2_TRY(l8_codes(&mw, w, d->K, d->N, d->ldw, 128));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(l8_div(d->N, 128) * l8_div(d->M, NT) * splits));
-  cfg.blockDim = dim3(L8Few<NT>::THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  PVB2_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear8_few_kernel<T, NT>, mx, mw, p, splits));
+  PVB2_CUDA_TRY(launch_over(linear8_few_kernel<T, NT>, (unsigned)(l8_div(d->N, 128) * l8_div(d->M, NT) * splits),
+                            L8Few<NT>::THREADS, smem, s, (unsigned)splits, mx, mw, p, splits));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }

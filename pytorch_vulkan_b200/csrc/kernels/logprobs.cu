@@ -42,6 +42,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
+#include "overlap.cuh"
 #include "types.cuh"
 
 namespace pvb2 {
@@ -444,6 +445,8 @@ struct Ring {
 
 template <typename T, bool TOP, int G>
 __global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) logp_kernel(LpArgs a, int cluster) {
+  let_next_come();
+  wait_for_last();
   constexpr int E = LpChunk<T>::E;
   using Row = LpRow<G>;
   extern __shared__ __align__(16) uint8_t ring[];  // [kLpRing][threads][16]
@@ -672,6 +675,8 @@ constexpr int kLpBwdThreads = 256;
 // chunks of z and of dz lie on the same boundaries.
 template <typename T, bool SAME>
 __global__ void __launch_bounds__(kLpBwdThreads, 5) logp_bwd_kernel(LpBwdArgs a, int64_t share) {
+  let_next_come();
+  wait_for_last();
   constexpr int E = LpChunk<T>::E, G = kLpBwdThreads;
   extern __shared__ __align__(16) uint8_t ring[];  // [kLpRing][threads][16]
   const int64_t row = blockIdx.x;
@@ -757,18 +762,8 @@ static int launch_lp_as(const LpArgs& a, int cluster, cudaStream_t s) {
   auto kernel = logp_kernel<T, TOP, G>;
   static DeviceOnce once;
   PVB2_TRY(allow_smem(kernel, smem, once));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.N + Row::ROWS - 1) / Row::ROWS * cluster));
-  cfg.blockDim = dim3(Row::THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  PVB2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, cluster));
+  PVB2_CUDA_TRY(launch_over(kernel, dim3((unsigned)((a.N + Row::ROWS - 1) / Row::ROWS * cluster)), Row::THREADS, smem, s,
+                            (unsigned)cluster, a, cluster));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -801,7 +796,8 @@ static int launch_lp_bwd_as(const LpBwdArgs& a, int64_t share, int64_t parts, cu
   constexpr int smem = kLpRing * kLpBwdThreads * 16;
   static DeviceOnce once;
   PVB2_TRY(allow_smem(logp_bwd_kernel<T, SAME>, smem, once));
-  logp_bwd_kernel<T, SAME><<<dim3((unsigned)a.N, (unsigned)parts), kLpBwdThreads, SAME ? smem : 0, s>>>(a, share);
+  PVB2_CUDA_TRY(launch_over(logp_bwd_kernel<T, SAME>, dim3((unsigned)a.N, (unsigned)parts), kLpBwdThreads, SAME ? smem : 0,
+                            s, 0, a, share));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }

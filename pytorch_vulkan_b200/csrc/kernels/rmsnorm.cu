@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>
+#include "overlap.cuh"
 #include "quant8.cuh"
 
 namespace pvb2 {
@@ -238,6 +239,8 @@ __device__ __forceinline__ void form_sum(const NormArgs& a, int64_t row, int c, 
 // chunks of it.
 template <typename T, int VEC, bool WARP, int NV, int MODE>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
+  let_next_come();
+  wait_for_last();
   using C = Chunk<T, VEC>;
   __shared__ double line[32];
   const int G = WARP ? 32 : (int)blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
@@ -302,6 +305,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
 // rows that outgrow the registers: read again for the output
 template <typename T, int VEC, int MODE>
 __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
+  let_next_come();
+  wait_for_last();
   using C = Chunk<T, VEC>;
   __shared__ double line[32];
   const int64_t row = blockIdx.x;
@@ -355,7 +360,10 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
 // in a fixed order.
 // MOST: 32 for a warp to a row, else the most threads of a row.
 template <typename T, int VEC, int MOST, int NV>
-__global__ void __launch_bounds__(MOST < 128 ? 128 : MOST, (sizeof(T) == 4 ? 1024 : MOST == 1024 ? 1024 : 768) / (MOST < 128 ? 128 : MOST)) norm_bwd_kernel(NormBwdArgs a) {
+__global__ void __launch_bounds__(MOST < 128 ? 128 : MOST, (sizeof(T) == 4 || MOST == 1024 ? 1024 : 768) /
+                                                               (MOST < 128 ? 128 : MOST)) norm_bwd_kernel(NormBwdArgs a) {
+  let_next_come();
+  wait_for_last();
   using C = Chunk<T, VEC>;
   constexpr int kRows = MOST == 32 ? 4 : 1;  // of a block
   const int G = MOST == 32 ? 32 : blockDim.x;
@@ -444,6 +452,8 @@ __global__ void __launch_bounds__(MOST < 128 ? 128 : MOST, (sizeof(T) == 4 ? 102
 // long rows: dh alone, and the shares of dw by columns
 template <typename T, int VEC>
 __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
+  let_next_come();
+  wait_for_last();
   using C = Chunk<T, VEC>;
   __shared__ float line[32];
   const int64_t row = blockIdx.x;
@@ -477,6 +487,8 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
 // rows blockIdx.y, blockIdx.y + gridDim.y, ... of 256 columns
 template <typename T>
 __global__ void __launch_bounds__(256) norm_dw_columns_kernel(NormBwdArgs a) {
+  let_next_come();
+  wait_for_last();
   const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (j >= a.D) return;
   float s = 0.f;
@@ -489,6 +501,8 @@ __global__ void __launch_bounds__(256) norm_dw_columns_kernel(NormBwdArgs a) {
 // a fixed order: a thread every 128th, then the threads of a column
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_dw_sum_kernel(const float* partial, int count, int D, T* dw) {
+  let_next_come();
+  wait_for_last();
   __shared__ float part[8][129];
   const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
   const int64_t j = (int64_t)blockIdx.x * 8 + x;
@@ -520,6 +534,8 @@ __global__ void __launch_bounds__(1024) norm_dw_sum_kernel(const float* partial,
 template <typename T>
 __global__ void __launch_bounds__(256) quant_tile_kernel(const T* x, int64_t rows, int64_t D, int64_t ldx, uint8_t* codes,
                                                          int64_t ldc, float* scales, int64_t groups) {
+  let_next_come();
+  wait_for_last();
   __shared__ uint32_t most_of[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
@@ -554,6 +570,8 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const T* x, int64_t row
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* codes, const float* scales, T* out, int64_t rows, int D,
                                                       int64_t ldc, int groups, int tall) {
+  let_next_come();
+  wait_for_last();
   constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
   const int c = (blockIdx.x * 256 + threadIdx.x) * E;
   if (c >= D) return;
@@ -642,16 +660,17 @@ static int launch_norm(const NormArgs& a, cudaStream_t s) {
   const bool few = a.rows < num_sms();
   if constexpr (VEC != kShifted) {  // (which has 257 or more)
     if (chunks <= 128 && (chunks <= 32 || !few)) {
-      if (chunks <= 32) norm_kernel<T, VEC, true, 1, MODE><<<fours, 128, 0, s>>>(a);
-      else if (chunks <= 64) norm_kernel<T, VEC, true, 2, MODE><<<fours, 128, 0, s>>>(a);
-      else norm_kernel<T, VEC, true, 4, MODE><<<fours, 128, 0, s>>>(a);
+      if (chunks <= 32) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, true, 1, MODE>, fours, 128, 0, s, 0, a));
+      else if (chunks <= 64) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, true, 2, MODE>, fours, 128, 0, s, 0, a));
+      else PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, true, 4, MODE>, fours, 128, 0, s, 0, a));
       PVB2_LAUNCH_CHECK();
       return PVB2_OK;
     }
   }
-  if (chunks <= 1024 && few) norm_kernel<T, VEC, false, 1, MODE><<<rows, (unsigned)((chunks + 31) / 32 * 32), 0, s>>>(a);
-  else if (chunks <= 4096) norm_kernel<T, VEC, false, 4, MODE><<<rows, (unsigned)((chunks + 127) / 128 * 32), 0, s>>>(a);
-  else norm_long_kernel<T, VEC == kWhole ? kWhole : kApart, MODE><<<rows, 1024, 0, s>>>(a);
+  const unsigned one = (unsigned)((chunks + 31) / 32 * 32), four = (unsigned)((chunks + 127) / 128 * 32);
+  if (chunks <= 1024 && few) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, false, 1, MODE>, rows, one, 0, s, 0, a));
+  else if (chunks <= 4096) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, false, 4, MODE>, rows, four, 0, s, 0, a));
+  else PVB2_CUDA_TRY(launch_over(norm_long_kernel<T, VEC == kWhole ? kWhole : kApart, MODE>, rows, 1024, 0, s, 0, a));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -744,7 +763,7 @@ static int launch_bwd_as(const NormBwdArgs& a, NormBwdPlan& p, cudaStream_t s) {
   // (the rows of a block begin alike where they lie a multiple of E rows apart)
   constexpr int E = Chunk<T, VEC>::E;
   if (VEC == kShifted && p.blocks < a.rows) p.blocks = p.blocks / E * E;
-  kernel<<<(unsigned)p.blocks, threads, smem, s>>>(a);
+  PVB2_CUDA_TRY(launch_over(kernel, (unsigned)p.blocks, threads, smem, s, 0, a));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -763,11 +782,13 @@ static int launch_bwd(const NormBwdArgs& a, NormBwdPlan& p, cudaStream_t s) {
   if (chunks <= 1024) return launch_bwd_as<T, VEC, 512, 2>(a, p, s);
   if (chunks <= 2048) return launch_bwd_as<T, VEC, 1024, 2>(a, p, s);
   if (a.dx) {
-    norm_bwd_long_kernel<T, VEC == kWhole ? kWhole : kApart><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    constexpr int kVec = VEC == kWhole ? kWhole : kApart;
+    PVB2_CUDA_TRY(launch_over(norm_bwd_long_kernel<T, kVec>, (unsigned)a.rows, 1024, 0, s, 0, a));
     PVB2_LAUNCH_CHECK();
   }
   if (!a.partial) return PVB2_OK;
-  norm_dw_columns_kernel<T><<<dim3((unsigned)((a.D + 255) / 256), (unsigned)p.blocks), 256, 0, s>>>(a);
+  const dim3 columns((unsigned)((a.D + 255) / 256), (unsigned)p.blocks);
+  PVB2_CUDA_TRY(launch_over(norm_dw_columns_kernel<T>, columns, 256, 0, s, 0, a));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -782,7 +803,8 @@ static int run_bwd(const NormBwdArgs& a, NormBwdPlan p, int vec, void* dw, cudaS
     } else PVB2_TRY((launch_bwd<T, kApart>(a, p, s)));
   }
   if (!dw) return PVB2_OK;
-  norm_dw_sum_kernel<T><<<(unsigned)((a.D + 7) / 8), 1024, 0, s>>>(a.partial, a.rows ? (int)p.blocks : 0, a.D, (T*)dw);
+  PVB2_CUDA_TRY(launch_over(norm_dw_sum_kernel<T>, (unsigned)((a.D + 7) / 8), 1024, 0, s, 0,
+                            a.partial, a.rows ? (int)p.blocks : 0, a.D, (T*)dw));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -880,10 +902,13 @@ int pvb2_quantize_8bit(int dtype, int64_t rows, int64_t D, const void* x, int64_
   PVB2_CHECK_ARG(blocks <= 65535, "quantize_8bit: more than %d rows in blocks of 128", 65535 * 128);
   const dim3 grid((unsigned)groups, (unsigned)blocks);
   if (dtype == PVB2_F32)
-    quant_tile_kernel<float><<<grid, 256, 0, s>>>((const float*)x, rows, D, ldx, codes, ldc, scales, groups);
+    PVB2_CUDA_TRY(launch_over(quant_tile_kernel<float>, grid, 256, 0, s, 0,
+                              (const float*)x, rows, D, ldx, codes, ldc, scales, groups));
   else if (dtype == PVB2_BF16)
-    quant_tile_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>((const __nv_bfloat16*)x, rows, D, ldx, codes, ldc, scales, groups);
-  else quant_tile_kernel<__half><<<grid, 256, 0, s>>>((const __half*)x, rows, D, ldx, codes, ldc, scales, groups);
+    PVB2_CUDA_TRY(launch_over(quant_tile_kernel<__nv_bfloat16>, grid, 256, 0, s, 0,
+                              (const __nv_bfloat16*)x, rows, D, ldx, codes, ldc, scales, groups));
+  else PVB2_CUDA_TRY(launch_over(quant_tile_kernel<__half>, grid, 256, 0, s, 0,
+                                 (const __half*)x, rows, D, ldx, codes, ldc, scales, groups));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }
@@ -906,8 +931,10 @@ int pvb2_dequantize_8bit(int64_t rows, int64_t D, const uint8_t* codes, int64_t 
   const dim3 grid(wide, (unsigned)std::min<int64_t>(65535, (rows + 3) / 4));
   auto go = [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    if (vec) dequant_kernel<T, true><<<grid, 256, 0, s>>>(codes, scales, p, rows, (int)D, ldc, groups, tall);
-    else dequant_kernel<T, false><<<grid, 256, 0, s>>>(codes, scales, p, rows, (int)D, ldc, groups, tall);
+    if (vec) PVB2_CUDA_TRY(launch_over(dequant_kernel<T, true>, grid, 256, 0, s, 0,
+                                       codes, scales, p, rows, (int)D, ldc, groups, tall));
+    else PVB2_CUDA_TRY(launch_over(dequant_kernel<T, false>, grid, 256, 0, s, 0,
+                                   codes, scales, p, rows, (int)D, ldc, groups, tall));
   };
   if (dtype == PVB2_F32) go((float*)out);
   else if (dtype == PVB2_BF16) go((__nv_bfloat16*)out);

@@ -220,3 +220,43 @@ def test_on_another_stream_and_thread(ocl):
             th.join()
         for i in range(2):
             assert all(torch.equal(a, b) for a, b in zip(results[i], want))
+
+
+@pytest.mark.parametrize("rows", [1, 130, 700])
+def test_one_call_after_the_other(ocl, rows):
+    """A launch may begin before the one in front of it ends: a long chain of small calls, each of which reads what the
+    last one wrote and writes where an earlier one read, gives the bits of the same chain with a pause after each."""
+    f = ocl.functional
+    g = torch.Generator().manual_seed(rows)
+    D, V = 640, 1000
+    w1, ws1 = f.quantize_8bit((0.05 * torch.randn(D, D, generator=g)).to(torch.bfloat16).to("ocl"), block_rows=128)
+    w2, ws2 = f.quantize_8bit((0.05 * torch.randn(V, D, generator=g)).to(torch.bfloat16).to("ocl"), block_rows=128)
+    x0 = torch.randn(rows, D, generator=g).to(torch.bfloat16)
+    gain = (1 + 0.1 * torch.randn(D, generator=g)).to(torch.bfloat16).to("ocl")
+    tokens = torch.randint(0, V, (rows,), generator=g).to("ocl")
+
+    def chain(pause):
+        out = []
+        wait = torch.ocl.synchronize if pause else (lambda: None)
+        x, stream = x0.to("ocl"), x0.to("ocl")
+        with torch.no_grad():
+            for i in range(30):
+                codes, scales, stream = f.rms_norm_8bit(x, gain, stream)
+                wait()
+                x = f.linear_8bit(codes, scales, w1, ws1)
+                wait()
+                codes, scales = f.quantize_8bit(f.rms_norm(x, gain))
+                wait()
+                logits = f.linear_8bit(codes, scales, w2, ws2)
+                wait()
+                lp, entropy, _, best = f.token_log_probs(logits, tokens, top=3)
+                wait()
+                x = f.dequantize_8bit(codes, scales, dtype=torch.bfloat16)
+                wait()
+                out.append((lp + entropy, best))
+        return [(a.cpu(), b.cpu()) for a, b in out] + [(x.cpu(), stream.cpu())]
+
+    want = chain(True)
+    for _ in range(3):
+        for (a, b), (c, d) in zip(chain(False), want):
+            assert torch.equal(a, c) and torch.equal(b, d)
