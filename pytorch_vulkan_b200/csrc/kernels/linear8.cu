@@ -759,7 +759,8 @@ static int l8_few(const pvb2_linear8_desc* d, const void* x, const void* w, cons
 }
 
 // CTAs of a cluster that share K: as many as have an SM, and eight K blocks
-// before each halving (joining the sums takes as long as four blocks do: 512
+// before each halving (joining the sums takes as long as four blocks do; one
+// launch after the other, without overlap: 512
 // outputs of 512 inputs, 128 rows: 7.3 us whole, 8.3 in two; 4096 of 4096: 20.7
 // whole, 15.0 in two, 11.4 in four)
 static int l8_splits(int64_t tiles, int64_t blocks) {
@@ -773,7 +774,7 @@ static int l8_run(const pvb2_linear8_desc* d, const void* x, const void* w, cons
   const int nt = d->M <= 16 ? 16 : d->M <= 32 ? 32 : d->M <= 64 ? 64 : 128;
   const int64_t few = l8_div(d->N, 128) * l8_div(d->M, nt);
   // Tiles of 128 x 128 as long as each has an SM of its own, then pairs' of 256 x
-  // 256 (us, the former and the latter: 512 rows, 4096 outputs of 4096 inputs
+  // 256 (us without overlap, the former and the latter: 512 rows, 4096 outputs of 4096 inputs
   // 21.5 and 21.9, 1024 rows 41 and 23; 300 rows, 5001 of 1008 9.9 and 13.0, 512
   // rows 17.6 and 13.4; 1024 rows, 1024 of 8192 23.5 and 37); few rows are bound
   // by the weight, whatever its tiles.
