@@ -777,7 +777,8 @@ PVB2_API int pvb2_dequantize_8bit(int64_t rows, int64_t D, const uint8_t* codes,
 /* y [M][N] = x w^T + bias of such codes: x [M][K] with a scale for every 128
  * of a row, w [N][K] with one for every 128 x 128; rows begin on 16-byte
  * boundaries.  y and bias (or NULL) are of d->dtype.  Blocks of 128 inputs are
- * multiplied on the tensor cores and summed in fp32. */
+ * multiplied on the tensor cores and summed in fp32; a product of two scales may
+ * lie outside fp32's normal numbers where the result does not. */
 typedef struct pvb2_linear8_desc {
   int64_t M, N, K;
   int64_t ldx, ldw;

@@ -21,6 +21,7 @@
 //     the CTAs of a cluster where the tiles are few, whose sums join through
 //     shared memory in a fixed order.  Bound by the weight's bytes.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 #include "overlap.cuh"
 #include "quant8.cuh"
@@ -35,7 +36,10 @@ struct L8Args {
   const float* ws;   // [ceil(N / 128)][blocks]
   const void* bias;  // of the output's type, or null
   void* y;           // [M][N]
-  int M, N, blocks;
+  const uint8_t* x;  // the codes, for blocks whose scales' product is odd
+  const uint8_t* w;
+  int64_t ldx, ldw;
+  int M, N, K, blocks;
   int tma_store;     // many rows: y's rows lie on 16-byte boundaries
   int vector_store;  // few rows: and four outputs on theirs
   int group;         // blocks of rows whose tiles lie together
@@ -82,6 +86,33 @@ __device__ __forceinline__ float2 numbers(uint64_t p) {
   float2 f;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
   return f;
+}
+
+// The scales' product x w where it leaves fp32's normal numbers ("odd"): a block's
+// sum is 0 or has 2^-18 to 2^25, so that its multiple may be a number all the same.
+// The sum is then multiplied by 2^100 or 2^-100 first, which is exact, and by what
+// is left of the product afterwards.  (Beyond 2^228 that is cut to fp32's largest:
+// the multiple of any sum but 0 is infinite, and that of 0 is 0.  Scales that are
+// 0, infinite or NaN are multiplied as they are.)
+__device__ __forceinline__ bool normal(float f) { return abs_bits(f) - 0x00800000u < 0x7f000000u; }
+__device__ __forceinline__ bool odd_product(float x, float w, float product) {
+  return !normal(product) && x != 0.f && w != 0.f && fabsf(x) <= FLT_MAX && fabsf(w) <= FLT_MAX;
+}
+// No product is odd of an x of 2^-62 to 2^66 and a w of 2^-62 to 2^61.  Of any
+// number of them, `or`ed: the top bit says whether one lies beyond.  (It does where
+// the exponent is not among the 128 from 65 on, for w also not among those from 60.)
+__device__ __forceinline__ uint32_t beyond_x(float x) { return 2 * __float_as_uint(x) - (65u << 24); }
+__device__ __forceinline__ uint32_t beyond_w(float w) { return beyond_x(w) | (2 * __float_as_uint(w) - (60u << 24)); }
+__device__ __forceinline__ bool unusual(uint32_t beyond) { return (int32_t)beyond < 0; }
+// the two parts
+__device__ __forceinline__ float odd_first(float x, float w) {
+  const float product = x * w;
+  return odd_product(x, w, product) ? (fabsf(product) > 1.f ? 0x1p100f : 0x1p-100f) : 1.f;
+}
+__device__ __forceinline__ float odd_rest(float x, float w, float first) {
+  if (first == 1.f) return x * w;
+  const float rest = (first > 1.f ? x * 0x1p-100f : x * 0x1p100f) * w;
+  return fminf(fmaxf(rest, -FLT_MAX), FLT_MAX);
 }
 
 // 16 columns of this warp's 32 lanes, as pairs.  The wait is part of the
@@ -141,6 +172,67 @@ struct L8Smem {
   static constexpr int TOTAL = BAR_OFF + (2 * SLOTS + 8) * 8 + 16;
 };
 
+// `group` blocks of rows go past all outputs before the next ones do
+__device__ __forceinline__ void l8_place(int group, int tiles_m, int tiles_n, int tile, int& mb, int& nb) {
+  const int first = tile / (group * tiles_n) * group, wide = min(group, tiles_m - first);
+  const int r = tile - first * tiles_n;
+  mb = first + r % wide;
+  nb = r / wide;
+}
+
+// The rows of this CTA's tiles in which a product of scales is odd, formed again
+// from the codes in memory, with such products in two parts.  That is slow (4096^3,
+// all rows: 30 ms against 76 us), for operands that next to nothing has: the
+// epilogue has no register for a second way through its loop (with one, or with
+// the loop once more in the same kernel, all calls took a tenth longer).
+template <typename T>
+__device__ __forceinline__ void form_odd_rows(const L8Args& p) {
+  const int tiles_m = (p.M + kL8M - 1) / kL8M, tiles_n = (p.N + kL8N - 1) / kL8N;
+#pragma unroll 1
+  for (int tile = blockIdx.x >> 1; tile < tiles_m * tiles_n; tile += gridDim.x >> 1) {
+    int mb, nb;
+    l8_place(p.group, tiles_m, tiles_n, tile, mb, nb);
+    const int m0 = mb * kL8M + (blockIdx.x & 1) * 128, m1 = min(m0 + 128, p.M);
+    // a warp to a row and the 128 outputs of one scale, 32 at a time
+#pragma unroll 1
+    for (int job = threadIdx.x >> 5; job < 256; job += L8Smem::THREADS / 32) {
+      const int m = m0 + (job >> 1), n0 = nb * kL8N + (job & 1) * kGroup8;
+      if (m >= m1 || n0 >= p.N) continue;
+      const float* xs = p.xs + (int64_t)m * p.blocks;
+      const float* ws = p.ws + (int64_t)(n0 / kGroup8) * p.blocks;
+      bool odd = false;
+      for (int kb = threadIdx.x & 31; kb < p.blocks; kb += 32) odd |= odd_product(xs[kb], ws[kb], xs[kb] * ws[kb]);
+      if (!__any_sync(~0u, odd)) continue;
+      const uint8_t* xc = p.x + (int64_t)m * p.ldx;
+#pragma unroll 1
+      for (int n = n0 + (threadIdx.x & 31); n < min(n0 + kGroup8, p.N); n += 32) {
+        const uint8_t* wc = p.w + (int64_t)n * p.ldw;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int kb = 0; kb < p.blocks; ++kb) {
+          const int k1 = min((kb + 1) * kL8BK, p.K);
+          float u = 0.f;
+          int k = kb * kL8BK;
+          for (; k + 16 <= k1; k += 16) {  // (rows begin on 16-byte boundaries)
+            const uint4 a = *(const uint4*)(xc + k), b = *(const uint4*)(wc + k);
+            const uint32_t as[4] = {a.x, a.y, a.z, a.w}, bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 av = values2(as[i / 2] >> (16 * (i & 1))), bv = values2(bs[i / 2] >> (16 * (i & 1)));
+              u = fmaf(av.y, bv.y, fmaf(av.x, bv.x, u));
+            }
+          }
+          for (; k < k1; ++k) u = fmaf(values2(xc[k]).x, values2(wc[k]).x, u);
+          const float first = odd_first(xs[kb], ws[kb]);
+          sum = fmaf(u * first, odd_rest(xs[kb], ws[kb], first), sum);
+        }
+        if (p.bias) sum += to_f32(((const T*)p.bias)[n]);
+        ((T*)p.y)[(int64_t)m * p.N + n] = from_f32<T>(sum);
+      }
+    }
+  }
+}
+
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
     linear8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
@@ -157,6 +249,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   uint64_t* scales_empty = scales_full + 2;
   uint32_t* tmem_slot = (uint32_t*)(scales_empty + 2);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
+  int* odd_met = (int*)(tmem_slot + 2);             // whether a product of scales was odd
 
   let_next_come();
   const int warp = warp_number(), lane = threadIdx.x & 31;
@@ -176,7 +269,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
       mbar_init(&scales_full[b], 1);
       mbar_init(&scales_empty[b], kL8EpiWarps);
     }
-    *abort = 0;
+    *abort = *odd_met = 0;
     fence_barrier_init();
   }
   if (warp == kL8MmaWarp) tmem_alloc_pair(tmem_slot, 512);
@@ -187,13 +280,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  // `group` blocks of rows go past all outputs before the next ones do
-  auto place = [&](int tile, int& mb, int& nb) {
-    const int first = tile / (p.group * tiles_n) * p.group, wide = min(p.group, tiles_m - first);
-    const int r = tile - first * tiles_n;
-    mb = first + r % wide;
-    nb = r / wide;
-  };
+  auto place = [&](int tile, int& mb, int& nb) { l8_place(p.group, tiles_m, tiles_n, tile, mb, nb); };
 
   if (warp < kL8Producers) {
     // ------------------------------------------------- loads: slot s by warp s % kL8Producers
@@ -249,6 +336,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 4; ++r) to[(i * 2 + h) * 128 + 32 * r] = x[r][i] * w[h][i];
+        // Whether a product is odd.  (As little as can be, and no detail in registers:
+        // it is issued beside the epilogue, and took a tenth of its time when the
+        // products were looked at one by one in a straight line.)
+        uint32_t out = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) out |= beyond_w(w[h][i]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out |= beyond_x(x[r][i]);
+        }
+        if (unusual(out)) {
+          out = 0;  // zeros are as usual as others
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) out |= w[h][i] != 0.f ? beyond_w(w[h][i]) : 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) out |= x[r][i] != 0.f ? beyond_x(x[r][i]) : 0;
+          }
+          if (unusual(out)) {  // (blocks of 1e-16 and less are: 29 us in place of 22.5 for 1024 rows, 4096 of 4096)
+#pragma unroll 8
+            for (int j = 0; j < 32; ++j) {
+              const float product = to[(j >> 2) * 128 + 32 * (j & 3)];
+              if (normal(product)) continue;
+              const int k = min(kb + (j >> 3), p.blocks - 1);
+              if (odd_product(p.xs[(int64_t)min(m0 + 32 * (j & 3), p.M - 1) * p.blocks + k], (j & 4 ? ws1 : ws0)[k], product)) *odd_met = 1;
+            }
+          }
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&scales_full[slot]);
         if (kb + 4 < p.blocks) fetch(kb + 4);
@@ -386,6 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
   }
+  if (*odd_met) form_odd_rows<T>(p);
 }
 
 // ----------------------------------------------------------------- few rows
@@ -412,6 +530,19 @@ struct L8Few {
 };
 
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kL8FewEpi * 32) : "memory"); }
+// and whether any of its threads says so
+__device__ __forceinline__ bool epilogue_any(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)mine), "n"(kL8FewEpi * 32)
+      : "memory");
+  return any != 0;
+}
 // four floats of another CTA of the cluster
 __device__ __forceinline__ float4 load_cluster(const float* p, int rank) {
   uint32_t at;
@@ -439,11 +570,12 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float* v) {
 }
 
 // The scales of the blocks [kb, kb + count) for the tile's rows, x's times the
-// weight's, by the epilogue's threads.
+// weight's, by the epilogue's threads; whether one of this thread's is odd.
 template <int NT>
-__device__ __forceinline__ void load_scales(const L8Args& p, const float* ws, int m0, int kb, int count, float* run, int warp,
+__device__ __forceinline__ bool load_scales(const L8Args& p, const float* ws, int m0, int kb, int count, float* run, int warp,
                                             int lane) {
   constexpr int kPitch = L8Few<NT>::PITCH;
+  bool odd = false;
   if (NT >= 64) {
     // some threads to a row, eight blocks at a time each
     constexpr int kPer = NT >= 64 ? kL8FewEpi * 32 / NT : 1;
@@ -457,9 +589,20 @@ __device__ __forceinline__ void load_scales(const L8Args& p, const float* ws, in
         x[i] = row[min(k0 + i, count - 1)];
         w[i] = ws[kb + min(k0 + i, count - 1)];
       }
+      uint32_t out = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        out |= beyond_x(x[i]) | beyond_w(w[i]);
         if (k0 + i < count) run[(k0 + i) * kPitch + j] = x[i] * w[i];
+      }
+      if (unusual(out)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k0 + i < count && odd_product(x[i], w[i], x[i] * w[i])) {
+            odd = true;
+            run[(k0 + i) * kPitch + j] = odd_rest(x[i], w[i], odd_first(x[i], w[i]));
+          }
+      }
     }
   } else {
     // a warp to a row, a lane to a block
@@ -470,10 +613,22 @@ __device__ __forceinline__ void load_scales(const L8Args& p, const float* ws, in
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
       x[i] = p.xs[(int64_t)min(m0 + warp - 2 + kL8FewEpi * i, p.M - 1) * p.blocks + kb + k];
+    uint32_t out = beyond_w(w);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
+    for (int i = 0; i < kRows; ++i) {
+      out |= beyond_x(x[i]);
       if (lane < count) run[lane * kPitch + warp - 2 + kL8FewEpi * i] = x[i] * w;
+    }
+    if (unusual(out)) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        if (lane < count && odd_product(x[i], w, x[i] * w)) {
+          odd = true;
+          run[lane * kPitch + warp - 2 + kL8FewEpi * i] = odd_rest(x[i], w, odd_first(x[i], w));
+        }
+    }
   }
+  return odd;
 }
 
 template <typename T, int NT>
@@ -501,6 +656,7 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
 
   const float* ws = p.ws + (int64_t)nb * p.blocks;
   float* run = (float*)(smem + L::SCALE_OFF);
+  bool odd = false;  // whether one of the run's scales is
   if (warp == 0) {
 #pragma unroll
     for (int i = lane; i < 2 * kSlots + 2 * kBufs; i += 32) mbar_init(&full[i], i < 2 * kSlots + kBufs ? 1 : kL8FewEpi);
@@ -521,10 +677,10 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
     tmem_alloc(tmem_slot, L::COLUMNS);
   } else {
     wait_for_last();
-    load_scales<NT>(p, ws, m0, kb0, min(L::RUN, kb1 - kb0), run, warp, lane);
+    odd = load_scales<NT>(p, ws, m0, kb0, min(L::RUN, kb1 - kb0), run, warp, lane);
   }
   tc_fence_before();
-  __syncthreads();
+  odd = __syncthreads_or(odd);
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -567,34 +723,52 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
 #pragma unroll
     for (int j = 0; j < kHalf; ++j) v[j] = 0.f;
     bool ok = true;  // where a wait gave up, the others still meet at the barriers
+    // the blocks of a run, whose scales are at hand; with odd ones in narrow loads, for the registers
+    auto add = [&](int first_block, int count, auto any_scales) {
+      constexpr bool kAny = decltype(any_scales)::value;
+      constexpr int kCols = kAny ? 8 : kWide;
 #pragma unroll 1
-    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-      const int in_run = it % L::RUN, buf = it % kBufs;
-      if (in_run == 0 && it > 0) {
-        epilogue_sync();  // the last run's have been read
-        load_scales<NT>(p, ws, m0, kb, min(L::RUN, kb1 - kb), run, warp, lane);
-        epilogue_sync();
-      }
-      ok = ok && mbar_wait(&acc_full[buf], (it / kBufs) & 1, abort);
-      if (!ok) continue;
-      tc_fence_after();
+      for (int i = 0; i < count; ++i) {
+        const int it = first_block + i, buf = it % kBufs;
+        int row = m0 + first;
+        if constexpr (kAny) asm volatile("" : "+r"(row));  // (places of 64 scales are not worth registers)
+        ok = ok && mbar_wait(&acc_full[buf], (it / kBufs) & 1, abort);
+        if (!ok) return;
+        tc_fence_after();
 #pragma unroll
-      for (int h = 0; h < kHalf / kWide; ++h) {
-        float u[kWide];
-        tmem_ld<kWide>(acc + buf * NT + kWide * h, u);
+        for (int h = 0; h < kHalf / kCols; ++h) {
+          float u[kCols];
+          tmem_ld<kCols>(acc + buf * NT + kCols * h, u);
+          if constexpr (kAny) {
+            const int kb = kb0 + it;
 #pragma unroll
-        for (int j = 0; j < kWide; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(run + in_run * L::PITCH + first + kWide * h + j);
-          float* a = v + kWide * h + j;
-          a[0] = fmaf(u[j], s.x, a[0]);
-          a[1] = fmaf(u[j + 1], s.y, a[1]);
-          a[2] = fmaf(u[j + 2], s.z, a[2]);
-          a[3] = fmaf(u[j + 3], s.w, a[3]);
+            for (int j = 0; j < kCols; ++j)
+              u[j] *= odd_first(p.xs[(int64_t)min(row + kCols * h + j, p.M - 1) * p.blocks + kb], ws[kb]);
+          }
+#pragma unroll
+          for (int j = 0; j < kCols; j += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(run + i * L::PITCH + first + kCols * h + j);
+            float* a = v + kCols * h + j;
+            a[0] = fmaf(u[j], s.x, a[0]);
+            a[1] = fmaf(u[j + 1], s.y, a[1]);
+            a[2] = fmaf(u[j + 2], s.z, a[2]);
+            a[3] = fmaf(u[j + 3], s.w, a[3]);
+          }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+    };
+#pragma unroll 1
+    for (int kb = kb0; kb < kb1; kb += L::RUN) {
+      const int count = min(L::RUN, kb1 - kb);
+      if (kb > kb0) {
+        epilogue_sync();  // the last run's have been read
+        odd = epilogue_any(load_scales<NT>(p, ws, m0, kb, count, run, warp, lane));
+      }
+      if (!odd) add(kb - kb0, count, std::false_type());
+      else add(kb - kb0, count, std::true_type());
     }
   }
 
@@ -813,6 +987,11 @@ int pvb2_linear8(const pvb2_linear8_desc* d, const uint8_t* x, const float* x_sc
   p.ws = w_scales;
   p.bias = bias;
   p.y = y;
+  p.x = x;
+  p.w = w;
+  p.ldx = d->ldx;
+  p.ldw = d->ldw;
+  p.K = (int)d->K;
   p.M = (int)d->M;
   p.N = (int)d->N;
   p.blocks = (int)l8_div(d->K, kL8BK);

@@ -119,7 +119,9 @@ def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None, *, dtype=
     ``bias`` ``[outputs]`` of the output's type.  Any sizes, one row as well as
     many.  Codes whose rows do not begin on 16-byte boundaries are copied first.
     Products are exact and summed in fp32: by the tensor cores over 128 features,
-    then block by block with the scales.  No gradients (they are refused).
+    then block by block with the scales, whose product may lie outside fp32 where
+    the result does not (of many rows, those with such products take much longer).
+    No gradients (they are refused).
     """
     return torch.ops.ocl.linear_8bit(codes, scales, weight_codes, weight_scales, bias, dtype)
 
