@@ -251,7 +251,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   volatile int* abort = (volatile int*)(tmem_slot + 1);
   int* odd_met = (int*)(tmem_slot + 2);             // whether a product of scales was odd
 
-  let_next_come();
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int tiles_m = (p.M + kL8M - 1) / kL8M, tiles_n = (p.N + kL8N - 1) / kL8N;
@@ -278,6 +277,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L8Smem::THREADS, 1)
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist before either is signalled
   tc_fence_after();
+  let_next_come();
   const uint32_t tmem_base = *tmem_slot;
 
   auto place = [&](int tile, int& mb, int& nb) { l8_place(p.group, tiles_m, tiles_n, tile, mb, nb); };
@@ -646,7 +646,6 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + kBufs);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
 
-  let_next_come();
   const int warp = warp_number(), lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
   // tiles of the same outputs lie together: their weight is read once
@@ -682,6 +681,7 @@ __global__ void __launch_bounds__(L8Few<NT>::THREADS, 1)
   tc_fence_before();
   odd = __syncthreads_or(odd);
   tc_fence_after();
+  let_next_come();
   const uint32_t tmem_base = *tmem_slot;
 
   constexpr int kHalf = NT / 2, kWide = kHalf < 32 ? kHalf : 32;

@@ -4,8 +4,11 @@
 // come at once may be scheduled while the last one's blocks finish: the two to
 // three microseconds between dependent launches are spent in the shadow of the
 // last one.  wait_for_last() returns when all of the last launch's work is done
-// and visible, so nothing may be read or written before it, by any thread;
-// kernels without it are not affected, whichever side of these they are on.
+// and visible, so no thread may read or write global memory that has not met it, or
+// a barrier behind one that has; kernels without it are not affected, whichever
+// side of these they are on.  A kernel that allocates tensor memory does so before
+// it lets the next one come: that one's blocks could take the memory first, and
+// hold it until this launch has ended, which waits for them.
 // A stream of calls, us with and without: 8-bit layer 300 x 1000 -> 5001 9.3 and
 // 11.3, 128 x 4096 -> 4096 10.2 and 12.4; log probabilities of 8192 x 1000 9.8 and
 // 12.4, of 1 x 32768 with 20 alternatives 7.8 and 10.2; norm of 2047 x 5000 to 8 bits
