@@ -67,10 +67,11 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, u
 }
 
 // tells the even CTA that an accumulator has been read.  What it guards is in
-// TMEM, and has arrived in registers: nothing in memory has to be ordered, and
+// TMEM, and has arrived in registers (tcgen05.wait::ld) ahead of the fence for
+// tcgen05 that every caller has made: nothing in memory has to be ordered, and
 // releasing it for the cluster cost more than the epilogue's arithmetic
 __device__ __forceinline__ void arrive_even_cta(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // two fp32 numbers in a register pair; a = b s + a, each rounded once

@@ -3,8 +3,6 @@ import glob
 import os
 import re
 
-import pytest
-
 KERNELS = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorch_vulkan_b200", "csrc", "kernels")
 SOURCES = sorted(glob.glob(os.path.join(KERNELS, "*.cu")) + glob.glob(os.path.join(KERNELS, "*.cuh")))
 
@@ -45,3 +43,11 @@ def test_the_next_launch_comes_after_tensor_memory_is_had():
         had = body.rindex("tmem_alloc")
         come = body.index("let_next_come()")
         assert had < come and "__syncthreads" in body[had:come], (path, name)
+
+
+def test_arrivals_at_another_blocks_barrier_have_the_clusters_scope():
+    """Without one an arrival has its own block's, in which the other block does not take part."""
+    arrivals = [(os.path.basename(p), m[0]) for p in SOURCES for m in re.finditer(r"mbarrier\.arrive[\w.:]*shared::cluster\S*", code(p))]
+    assert len(arrivals) >= 2
+    for path, text in arrivals:
+        assert re.match(r"mbarrier\.arrive(\.expect_tx)?\.(release|relaxed)\.cluster\.", text), (path, text)
