@@ -611,6 +611,10 @@ __global__ void __launch_bounds__(LpRow<G>::THREADS, 1024 / LpRow<G>::THREADS) l
   sum = {__shfl_sync(~0u, sum.m, 0), __shfl_sync(~0u, sum.s, 0), __shfl_sync(~0u, sum.u, 0)};
   // a row without any probability: log p is -inf, H is 0
   const bool empty = sum.s == 0.f;
+  // (s holds the maximum's 1, u nothing above 0: roundings must not make a log
+  // probability of more than 0 or an entropy of less; a NaN stays one)
+  if (sum.s < 1.f && !empty) sum.s = 1.f;
+  if (sum.u > 0.f) sum.u = 0.f;
   const float logs = empty ? 0.f : logf(sum.s);
   const float m = empty ? INFINITY : sum.m;
   if (lane == 0) {
