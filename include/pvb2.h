@@ -794,6 +794,7 @@ PVB2_API int pvb2_linear8_status(int* timed_out, int reset);
 /* logits [N][V] (the reference had log_softmax and nll_loss,           */
 /* loss_ops.cpp:23-213): logp = z_t - lse, entropy = -sum p log p.      */
 /* A token outside [0, V) has the log probability 0 and no gradient; a  */
+/* token whose logit is -inf has -inf, and its gradient is g_logp; a    */
 /* row whose logits are all -inf has -inf, the entropy 0 and no         */
 /* gradient.  The top best (at most 32) by falling logit, of equal ones */
 /* the lower index first, with their log probabilities.                 */

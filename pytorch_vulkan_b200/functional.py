@@ -137,7 +137,8 @@ def token_log_probs(logits, tokens, *, top=0):
 
     ``log_probs`` and ``entropy`` have gradients (the alternatives have none);
     forward mode and second derivatives are refused.  Logits of -inf have no
-    probability and no gradient.  Tokens outside the vocabulary (-100 for a
+    probability and no gradient, but for a given token's own: its log probability is
+    -inf, and it gets that one's gradient.  Tokens outside the vocabulary (-100 for a
     prompt's, say) have the log probability 0 and no gradient through it, whatever
     their entropy's.  A row whose logits are all -inf has -inf, the entropy 0 and no
     gradient; one that holds a NaN or +inf is NaN.
