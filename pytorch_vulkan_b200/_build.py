@@ -57,6 +57,7 @@ def _compile_cu(src, force, extra_flags):
         return obj, ""
     os.makedirs(os.path.dirname(obj), exist_ok=True)
     cmd = [NVCC, "-ccbin", CXX, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
+           "-Xcompiler", "-Werror=return-type",
            "--expt-relaxed-constexpr", "-I", INCLUDE, "-c", src, "-o", obj, *extra_flags]
     out = _run(cmd)
     return obj, out
@@ -71,7 +72,7 @@ def _torch_flags():
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     py_inc = sysconfig.get_paths()["include"]
     cflags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
-              "-DTORCH_API_INCLUDE_EXTENSION_H", "-Wno-unused-parameter", "-Wno-sign-compare"]
+              "-DTORCH_API_INCLUDE_EXTENSION_H", "-Wno-unused-parameter", "-Wno-sign-compare", "-Werror=return-type"]
     # the CUDA include tree only for the header-only NVTX v3 ranges of the op guard
     for i in incs + [py_inc, CUDA_INC, INCLUDE]:
         cflags += ["-isystem" if i != INCLUDE else "-I", i]

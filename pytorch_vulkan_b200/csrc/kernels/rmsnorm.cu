@@ -929,18 +929,18 @@ int pvb2_dequantize_8bit(int64_t rows, int64_t D, const uint8_t* codes, int64_t 
   cudaStream_t s = as_stream(stream);
   const unsigned wide = (unsigned)((D / (vec ? 16 / size : 1) + 255) / 256);
   const dim3 grid(wide, (unsigned)std::min<int64_t>(65535, (rows + 3) / 4));
-  auto go = [&](auto* p) {
+  auto go = [&](auto* p) -> int {
     using T = std::remove_pointer_t<decltype(p)>;
     if (vec) PVB2_CUDA_TRY(launch_over(dequant_kernel<T, true>, grid, 256, 0, s, 0,
                                        codes, scales, p, rows, (int)D, ldc, groups, tall));
     else PVB2_CUDA_TRY(launch_over(dequant_kernel<T, false>, grid, 256, 0, s, 0,
                                    codes, scales, p, rows, (int)D, ldc, groups, tall));
+    PVB2_LAUNCH_CHECK();
+    return PVB2_OK;
   };
-  if (dtype == PVB2_F32) go((float*)out);
-  else if (dtype == PVB2_BF16) go((__nv_bfloat16*)out);
-  else go((__half*)out);
-  PVB2_LAUNCH_CHECK();
-  return PVB2_OK;
+  if (dtype == PVB2_F32) return go((float*)out);
+  if (dtype == PVB2_BF16) return go((__nv_bfloat16*)out);
+  return go((__half*)out);
 }
 
 }  // extern "C"

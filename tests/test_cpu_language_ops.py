@@ -184,3 +184,24 @@ def test_python_surface():
     for args in ((-1.0,), (1.0, 3.0), (math.nan,)):
         with pytest.raises(ValueError):
             pkg.optim.clip_grad_norm_([p], *args)
+
+
+def test_launches_that_fail_say_so(lib):
+    """Where there is no device every launch fails: its own error comes back, from every entry point."""
+    count = ctypes.c_int(-1)
+    lib.pvb2_device_count(ctypes.byref(count))
+    if count.value != 0:
+        pytest.skip("a launch of these addresses is for machines without a device alone")
+    n, z = norm(), Logp(N=4, V=100, ldz=100, dtype=BF16, top=0)
+    need = ctypes.c_size_t(1 << 30)
+    calls = [
+        ("launch_over", lambda: norm_fwd(lib, n)),
+        ("launch_over", lambda: lib.pvb2_rms_norm_bwd(ctypes.byref(n), SOME, SOME, SOME, SOME, None, SOME, SOME, SOME, need, None)),
+        ("quant_tile_kernel", lambda: lib.pvb2_quantize_8bit(F32, I64(8), I64(64), SOME, I64(64), 1, SOME, I64(64), SOME, None)),
+        ("dequant_kernel", lambda: lib.pvb2_dequantize_8bit(I64(8), I64(64), SOME, I64(64), SOME, 0, F32, SOME, None)),
+        ("failed", lambda: lib.pvb2_token_logp_fwd(ctypes.byref(z), SOME, SOME, SOME, SOME, None, None, None, None)),
+    ]
+    for what, call in calls:
+        assert call() == 3, what
+        text = lib.pvb2_last_error().decode()
+        assert what in text and "failed" in text, (what, text)
