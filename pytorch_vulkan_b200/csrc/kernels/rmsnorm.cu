@@ -7,9 +7,12 @@
 //   backward, with a = gy w:  dh = rstd (a - n mean(a n)) + gh;   dw = sum over rows of gy n
 //
 // One pass over the data: a row's elements stay in the registers of the
-// threads that share it (a warp up to 1024 16-bit elements, a block beyond)
-// between the sum and the output, so every kernel here is bound by HBM.  Rows of
-// more than 32768 16-bit elements are read twice, the second time out of L2.
+// threads that share it (a warp up to 128 chunks, a block beyond) between the sum
+// and the output.  Rows of more than 4096 chunks (32768 16-bit elements, 16384 in
+// fp32 or in the chunks of four below; backward half as many) are read twice, the
+// second time out of L2.  Large forward passes are bound by HBM (8192 x 4096 bf16
+// with a residual 6.4 TB/s); the others are by what a block does in turn: load, meet,
+// store (codes of 2047 x 5000 19 us for 11 us of bytes, backward 55 for 41).
 //
 // The mean of squares is summed in 64 bits and rounded once, root and quotient
 // are the IEEE ones, and n and y are rounded products: a code of the 8-bit
@@ -148,11 +151,17 @@ __device__ __forceinline__ A row_sum(A v, A* line) {
   return v;
 }
 
+// SMALL: with an eps that is next to nothing the mean may lie beneath fp32's normal
+// numbers; then by way of powers of two.  (Kernels of their own: in the others this
+// took registers, 4000 x 5001 fp32 with a residual 55 us in place of 52.)
+constexpr float kSmallEps = 0x1p-101f;
+template <bool SMALL>
 __device__ __forceinline__ float rstd_of(double squares, double per_element, float eps) {
-  return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn((float)(squares * per_element), eps)));
+  const double mean = squares * per_element;
+  if (SMALL && mean < kSmallEps) return __fdiv_rn(0x1p99f, __fsqrt_rn((float)((mean + eps) * 0x1p198)));
+  return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn((float)mean, eps)));
 }
 
-// the weight's numbers, or ones
 // elements [cE - off, cE - off + E) of what itself begins on a 16-byte boundary:
 // the two chunks that hold them, moved together
 template <typename T, int VEC>
@@ -174,6 +183,7 @@ __device__ __forceinline__ void load_beside(AChunk<T, VEC>& w, const T* p, int c
 #pragma unroll
   for (int k = 0; k < 4; ++k) to[k] = __funnelshift_r(v[k], v[k + 1], (skip & 3) * 8);
 }
+// the weight's numbers, or ones
 template <typename T, int VEC>
 __device__ __forceinline__ void load_weight(AChunk<T, VEC>& w, const void* p, int c, int D, int off) {
   if (p) {
@@ -237,7 +247,7 @@ __device__ __forceinline__ void form_sum(const NormArgs& a, int64_t row, int c, 
 
 // A warp (WARP; blocks of four) or a block shares a row, each thread keeps NV
 // chunks of it.
-template <typename T, int VEC, bool WARP, int NV, int MODE>
+template <typename T, int VEC, bool WARP, int NV, int MODE, bool SMALL = false>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
   let_next_come();
   wait_for_last();
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
         const double v = to_f32(h[i].e[k]);
         q = fma(v, v, q);
       }
-    rstd = rstd_of(row_sum<WARP>(q, line), a.per_element, a.eps);
+    rstd = rstd_of<SMALL>(row_sum<WARP>(q, line), a.per_element, a.eps);
     if (a.rstd && t == 0) a.rstd[row] = rstd;
   }
 #pragma unroll
@@ -303,7 +313,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(NormArgs a) {
 }
 
 // rows that outgrow the registers: read again for the output
-template <typename T, int VEC, int MODE>
+template <typename T, int VEC, int MODE, bool SMALL = false>
 __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
   let_next_come();
   wait_for_last();
@@ -326,7 +336,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
         q = fma(v, v, q);
       }
     }
-    rstd = rstd_of(row_sum<false>(q, line), a.per_element, a.eps);
+    rstd = rstd_of<SMALL>(row_sum<false>(q, line), a.per_element, a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
   }
   // the sum that this thread wrote, or x
@@ -530,7 +540,8 @@ __global__ void __launch_bounds__(1024) norm_dw_sum_kernel(const float* partial,
 }
 
 // ------------------------------------------- codes of weights, and values
-// 128 x 128 elements with one scale; a warp reads 4 x 32 of a row at a time
+// 128 x 128 elements with one scale; a warp reads 4 x 32 of a row at a time, an
+// element a thread (4096 x 4096 bf16 26 us, 1.9 TB/s: weights, once)
 template <typename T>
 __global__ void __launch_bounds__(256) quant_tile_kernel(const T* x, int64_t rows, int64_t D, int64_t ldx, uint8_t* codes,
                                                          int64_t ldc, float* scales, int64_t groups) {
@@ -658,6 +669,16 @@ static int launch_norm(const NormArgs& a, cudaStream_t s) {
   // two chunks 47, a warp to the row with 16 chunks a lane 73).  Few rows have
   // more threads, for the first chunk to be the only one.
   const bool few = a.rows < num_sms();
+  const unsigned one = (unsigned)((chunks + 31) / 32 * 32), four = (unsigned)((chunks + 127) / 128 * 32);
+  constexpr int kLong = VEC == kWhole ? kWhole : kApart;
+  if constexpr (MODE != kQuant8) {
+    if (a.eps < kSmallEps) {  // (fewer kinds: next to nobody asks for it)
+      if (chunks <= 4096) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, false, 4, MODE, true>, rows, four, 0, s, 0, a));
+      else PVB2_CUDA_TRY(launch_over(norm_long_kernel<T, kLong, MODE, true>, rows, 1024, 0, s, 0, a));
+      PVB2_LAUNCH_CHECK();
+      return PVB2_OK;
+    }
+  }
   if constexpr (VEC != kShifted) {  // (which has 257 or more)
     if (chunks <= 128 && (chunks <= 32 || !few)) {
       if (chunks <= 32) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, true, 1, MODE>, fours, 128, 0, s, 0, a));
@@ -667,10 +688,9 @@ static int launch_norm(const NormArgs& a, cudaStream_t s) {
       return PVB2_OK;
     }
   }
-  const unsigned one = (unsigned)((chunks + 31) / 32 * 32), four = (unsigned)((chunks + 127) / 128 * 32);
   if (chunks <= 1024 && few) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, false, 1, MODE>, rows, one, 0, s, 0, a));
   else if (chunks <= 4096) PVB2_CUDA_TRY(launch_over(norm_kernel<T, VEC, false, 4, MODE>, rows, four, 0, s, 0, a));
-  else PVB2_CUDA_TRY(launch_over(norm_long_kernel<T, VEC == kWhole ? kWhole : kApart, MODE>, rows, 1024, 0, s, 0, a));
+  else PVB2_CUDA_TRY(launch_over(norm_long_kernel<T, kLong, MODE>, rows, 1024, 0, s, 0, a));
   PVB2_LAUNCH_CHECK();
   return PVB2_OK;
 }

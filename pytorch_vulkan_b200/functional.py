@@ -69,9 +69,11 @@ def rms_norm(input, weight=None, residual=None, *, eps=1e-6):
     ``h = input + residual`` rounded to their type; then the result is ``(y, h)``,
     ``h`` being the residual stream as it goes on.  fp32, bf16 or fp16, all of
     one type; ``weight`` ``[features]`` or None.  The mean of squares is summed in
-    64 bits, the rest is fp32, rounded once.  Gradients of ``input``,
-    ``residual`` and ``weight`` (the last in a fixed order); forward mode and
-    second derivatives are refused.
+    64 bits, the rest is fp32, rounded once; with an ``eps`` of next to nothing rows
+    may be as small as fp32's normal numbers, but rows whose mean of squares is
+    beyond fp32 (1.8e19 and more) are 0.  Gradients of ``input``, ``residual`` and
+    ``weight`` (the last in a fixed order); forward mode and second derivatives are
+    refused.
     """
     if residual is None:
         return torch.ops.ocl.rms_norm(input, weight, eps)
