@@ -5,17 +5,19 @@
 //
 // The inner sums are the tensor cores' (tcgen05.mma kind::f8f6f4, four steps of
 // 32 along K, fp32 in TMEM); the outer one is formed in registers, since the
-// scales change with the block.  A block's products go to one of two
-// accumulators; while the epilogue's warps read one, multiply it by its scales
-// and add it to their sums, the tensor core fills the other.  Products of codes
+// scales change with the block.  A block's products go to one of two accumulators
+// (of up to eight, few rows); while the epilogue's warps read one, multiply it by its
+// scales and add it to their sums, the tensor core fills another.  Products of codes
 // are exact, a block's 128 of them lose bits below 2^-24 of their largest, and
 // what the epilogue adds rounds as fp32 does.
 //
 // Two kernels:
 //   * many rows: CTA pairs (cta_group::2) on tiles of 256 rows x 256 outputs,
 //     persistent, loads by TMA into a ring of five K blocks, stores by TMA.  A
-//     block's products take the tensor core 512 clocks, the epilogue about as
-//     many instructions: it is bound by both, and by the board's power.
+//     block's products take the tensor core 512 clocks and a block as a whole 1040
+//     (8192^3: 896 one after the other in 596 us, at the 1.57 GHz that the board's
+//     power leaves; 514 in a burst): bound by the epilogue, whose four rounds of
+//     load, wait and multiply-add stand in line, with no load behind the arithmetic.
 //   * few rows: tiles of 128 outputs x 16 to 128 rows, the weight in the
 //     place of the left operand, so that one row costs little; K is split over
 //     the CTAs of a cluster where the tiles are few, whose sums join through

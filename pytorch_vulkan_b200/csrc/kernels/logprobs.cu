@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kLpBwdThreads, 5) logp_bwd_kernel(LpBwdArgs a,
   const int64_t row = blockIdx.x;
   const T* z = (const T*)a.z + row * a.ldz;
   T* dz = (T*)a.dz + row * a.V;
-  if (!SAME) {  // element by element
+  if (!SAME) {  // element by element (8192 rows of 50257 bf16, 50304 apart: 762 us; next to each other 253)
     const LpRowGrad r(a, row);
     const int64_t end = min(a.V, (blockIdx.y + 1) * share * E);
     for (int64_t i = blockIdx.y * share * E + threadIdx.x; i < end; i += G)
@@ -786,10 +786,9 @@ static int launch_lp(const LpArgs& a, cudaStream_t s) {
   }
   // Short rows a warp's, since a block's joins take longer than the row; long ones
   // few threads' all the same, so that many rows begin and end at different
-  // times (us for a warp, 128, 256 and 512 threads: 16384 x 1000 bf16 17, 44,
-  // 81, 168; 8192 x 10000 34, 45, 68, 122, with 20 alternatives 97, 83, 111, 206;
-  // 4096 x 49999 79, 72, 81, 112; 2048 x 131072 with 5 alternatives 235, 115,
-  // 105, 123).
+  // times (us for a warp, 128 and 256 threads, bf16: 16384 x 1000 18, 45, 84; 8192 x
+  // 10000 35, 45, 68, with 20 alternatives 120, 80, 111; 4096 x 49999 79, 73, 82, with
+  // 5 alternatives 165, 91, 104; 2048 x 131072 109, 92, 102, with 5 274, 115, 106).
   if (bytes <= (TOP ? 10240 : 20480)) return launch_lp_as<T, TOP, 32>(a, 1, s);
   if (bytes <= 160 * 1024) return launch_lp_as<T, TOP, 128>(a, 1, s);
   return launch_lp_as<T, TOP, 256>(a, 1, s);

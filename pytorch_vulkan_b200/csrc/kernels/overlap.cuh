@@ -9,11 +9,12 @@
 // side of these they are on.  A kernel that allocates tensor memory does so before
 // it lets the next one come: that one's blocks could take the memory first, and
 // hold it until this launch has ended, which waits for them.
-// A stream of calls, us with and without: 8-bit layer 300 x 1000 -> 5001 9.3 and
-// 11.3, 128 x 4096 -> 4096 10.2 and 12.4; log probabilities of 8192 x 1000 9.8 and
-// 12.4, of 1 x 32768 with 20 alternatives 7.8 and 10.2; norm of 2047 x 5000 to 8 bits
-// and back 26.8 and 30.9, with gradients 8192 x 4096 104 and 109.  (Launches with
-// a long list of tensors as their argument gain nothing: the host is the bound.)
+// A stream of calls of the C functions, us with and without: 8-bit layer 1 x 4096 ->
+// 4096 5.7 and 8.2, 300 x 1000 -> 5001 8.1 and 10.3, 128 x 4096 -> 4096 10.0 and 12.3;
+// log probabilities of 8192 x 1000 9.7 and 12.3, of 1 x 32768 with 20 alternatives
+// 7.8 and 10.3; norm of 2047 x 5000 to 8 bits and back 25.5 and 30.7, with gradients
+// 8192 x 4096 101 and 107.  (Launches with a long list of tensors as their argument
+// gain nothing: the host is the bound.)
 #pragma once
 #include "common.cuh"
 
